@@ -47,8 +47,11 @@ typedef enum s2_dtype {
 typedef enum s2_activation {
     S2_ACT_NONE = 0,
     S2_ACT_GELU = 1,   /* erf-GELU, 0.5 x (1 + erf(x / sqrt 2)) */
-    S2_ACT_SWIGLU = 2  /* silu(gate) * up over a gate/up weight pair, see
+    S2_ACT_SWIGLU = 2, /* silu(gate) * up over a gate/up weight pair, see
                           s2_shared_linear_forward */
+    /* of s2_linear, s2_grouped_linear and s2_group_norm only: */
+    S2_ACT_SILU = 3,      /* x / (1 + e^-x) */
+    S2_ACT_GELU_TANH = 4  /* 0.5 x (1 + tanh(sqrt(2 / pi) (x + 0.044715 x^3))) */
 } s2_activation;
 
 /* One attention window.  Same fields and meaning as the reference
@@ -488,6 +491,75 @@ S2_API int s2_shared_linear_residual(const void* x_video, int m_video, const voi
                                      const float* gate, const float* video_gate,
                                      const float* text_gate, void* out_video, void* out_text,
                                      s2_stream_t stream);
+
+/* ---- group norm, linear, grouped linear ---------------------------------- */
+/* What stands between the attention and convolution layers of the VAE's and
+ * the DiT's graphs as ncnn built-ins (GroupNorm, InnerProduct / Gemm with their
+ * activations and sums: the graphs the reference loads at
+ * src/seedvr2/seedvr2_vae.cpp:508-549 and seedvr2_dit.cpp:603-633, whose .param
+ * files it does not hold), on rows with channels last.  Activations:
+ * S2_ACT_NONE, _GELU, _SILU, _GELU_TANH.  All arithmetic is fp32 or wider; each
+ * output is rounded once. */
+
+/* y[f][p][c] = act((x[f][p][c] - mean) / sqrt(var + epsilon) * gamma[c] +
+ * beta[c]), mean and (biased) variance over the pixels of frame f and the
+ * channels of c's group, channels / groups neighbours.
+ *
+ * x: device [frames][pixels][channels] in x_dtype, frame and pixel strides in
+ *   elements, channels contiguous; y likewise.  y is x itself (same type and
+ *   strides) or does not overlap it.
+ * gamma, beta: device fp32 [channels] or NULL (1 and 0).
+ * channels: a multiple of groups, at most 4096; frames at most 65535.
+ *   frames == 0 or pixels == 0 does nothing.
+ * workspace: s2_group_norm_workspace_bytes, 8-byte aligned (partial
+ *   statistics; calls that may overlap in time need one each).
+ * An infinity or NaN makes its frame's group NaN, no other. */
+S2_API int s2_group_norm_workspace_bytes(int frames, int pixels, int channels, int groups,
+                                         size_t* bytes);
+S2_API int s2_group_norm(const void* x, s2_dtype x_dtype, long x_frame_stride,
+                         long x_pixel_stride, int frames, int pixels, int channels, int groups,
+                         const float* gamma, const float* beta, float epsilon, int activation,
+                         void* y, s2_dtype y_dtype, long y_frame_stride, long y_pixel_stride,
+                         void* workspace, size_t workspace_bytes, s2_stream_t stream);
+
+/* y = residual + act(x W^T + bias).
+ *
+ * x: device [m][k] in x_dtype, row stride x_stride >= k; weight: device [n][k]
+ *   in w_dtype, contiguous; BF16 with F32 or BF16 x, or F16 with F16 x.  The
+ *   products are those of the operands as given: an fp32 x is taken as two
+ *   (y 16 bits wide: to 2^-15) or three (exactly) bf16 terms on the matrix
+ *   cores.
+ * bias: device fp32 [n] or NULL.  residual: device [m][n] in y_dtype, row
+ *   stride residual_stride >= n, or NULL; y: device [m][n], row stride y_stride
+ *   >= n.  y is the residual itself (same stride) or does not overlap it; y
+ *   overlaps nothing else.
+ * Any m >= 0 (0 does nothing), n and k; pointers aligned to their elements.
+ *   Rows whose starts are 16-byte aligned are fastest.
+ * workspace: s2_linear_workspace_bytes, 16-byte aligned (calls that may overlap
+ *   in time need one each), or NULL: then nothing is split along k, which is
+ *   slower where there are few output tiles. */
+S2_API int s2_linear_workspace_bytes(int m, int n, int k, s2_dtype x_dtype, size_t* bytes);
+S2_API int s2_linear(const void* x, s2_dtype x_dtype, long x_stride, int m, const void* weight,
+                     s2_dtype w_dtype, const float* bias, int n, int k, int activation,
+                     const void* residual, long residual_stride, void* y, s2_dtype y_dtype,
+                     long y_stride, void* workspace, size_t workspace_bytes, s2_stream_t stream);
+
+/* s2_linear over row groups: rows offsets[g] .. offsets[g + 1] - 1 of x, the
+ * residual and y with weight[g] and bias[g].  The two token streams of a DiT
+ * block that do not share weights, a weight per sample or per expert.
+ *
+ * offsets: device int32 [groups + 1], ascending, 0 <= offsets[g] <= m, read by
+ *   the kernels.  Groups may be empty.  Rows before offsets[0] and from
+ *   offsets[groups] on are neither read nor written.  Offsets outside [0, m] are
+ *   taken as the nearest of the two; rows that descending offsets put into two
+ *   groups, or into none, have unspecified values.
+ * weight: device [groups][n][k]; bias: device fp32 [groups][n] or NULL; the
+ *   rest as for s2_linear. */
+S2_API int s2_grouped_linear(const void* x, s2_dtype x_dtype, long x_stride, int m,
+                             const int* offsets, int groups, const void* weight, s2_dtype w_dtype,
+                             const float* bias, int n, int k, int activation,
+                             const void* residual, long residual_stride, void* y,
+                             s2_dtype y_dtype, long y_stride, s2_stream_t stream);
 
 /* ---- DecomposedConv3D (VAE) ---------------------------------------------- */
 /* The causal 3-D convolution of the VAE (src/seedvr2/decomposed_conv3d.h:33-88,

@@ -25,6 +25,8 @@ DTYPE_F16 = 2
 ACT_NONE = 0
 ACT_GELU = 1
 ACT_SWIGLU = 2
+ACT_SILU = 3        # of group_norm, linear and grouped_linear only, as the next
+ACT_GELU_TANH = 4
 
 # Every symbol include/seedvr2_hip.h declares.
 EXPORTS = (
@@ -43,7 +45,8 @@ EXPORTS = (
     "s2_awa_qkv_forward", "s2_gelu", "s2_swiglu_pack_weight", "s2_awa_plan_cache_rope",
     "s2_stream_wait", "s2_stream_scratch_acquire", "s2_stream_scratch_release",
     "s2_binary_op", "s2_unary_op", "s2_reduce", "s2_rms_norm", "s2_copy_2d",
-    "s2_shared_linear_residual",
+    "s2_shared_linear_residual", "s2_group_norm_workspace_bytes", "s2_group_norm",
+    "s2_linear_workspace_bytes", "s2_linear", "s2_grouped_linear",
 )
 
 
@@ -175,6 +178,14 @@ def lib() -> ctypes.CDLL:
                                         ci, cl, vp]
         L.s2_shared_linear_residual.argtypes = [vp, ci, vp, ci, vp, vp, ci, ci, ci, P(ci), P(ci),
                                                 vp, vp, ci, vp, vp, vp, vp, vp, vp]
+        L.s2_group_norm_workspace_bytes.argtypes = [ci, ci, ci, ci, P(sz)]
+        L.s2_group_norm.argtypes = [vp, ci, cl, cl, ci, ci, ci, ci, vp, vp, cf, ci, vp, ci, cl, cl,
+                                    vp, sz, vp]
+        L.s2_linear_workspace_bytes.argtypes = [ci, ci, ci, ci, P(sz)]
+        L.s2_linear.argtypes = [vp, ci, cl, ci, vp, ci, vp, ci, ci, ci, vp, cl, vp, ci, cl, vp, sz,
+                                vp]
+        L.s2_grouped_linear.argtypes = [vp, ci, cl, ci, vp, ci, vp, ci, vp, ci, ci, ci, vp, cl, vp,
+                                        ci, cl, vp]
         _LIB = L
     return _LIB
 
@@ -671,6 +682,138 @@ def denoise_update(positive_patches, negative_patches, frames, height, width, cf
                                   _ptr(latent), channel_stride, _stream(stream)),
           "s2_denoise_update")
     return latent
+
+
+# ---- group norm, linear, grouped linear --------------------------------------
+
+def _vector(t, size, name):
+    """Checks an optional contiguous fp32 device vector (gamma, beta, bias)."""
+    import torch
+    if t is not None and (t.dtype != torch.float32 or t.numel() != size or not t.is_contiguous()):
+        raise ValueError(f"{name} must be {size} contiguous fp32 values")
+
+
+def _on_current_device(*tensors):
+    """Refuses tensors that the current device's kernels cannot reach."""
+    import torch
+    device = torch.cuda.current_device() if torch.cuda.is_available() else 0
+    for t in tensors:
+        if t is not None and t.get_device() != device:
+            raise ValueError(f"operands must be on the current device, cuda:{device}")
+
+
+def group_norm(x, groups, gamma=None, beta=None, epsilon=1e-6, activation=ACT_NONE, out=None,
+               out_dtype=None, workspace=None, stream=None):
+    """s2_group_norm: act(normalised x * gamma + beta) of frames [frames, pixels,
+    channels] (any frame and pixel strides, contiguous channels), statistics per
+    frame and group of channels.  out may be x.  workspace: at least
+    group_norm_workspace(...) bytes, allocated on the current stream if None.
+    Returns out."""
+    import torch
+    if x.dim() != 3:
+        raise ValueError("x must be [frames, pixels, channels]")
+    f, p, c = x.shape
+    xd = _dtype_code(x)
+    if out is None:
+        out = torch.empty((f, p, c), dtype=out_dtype or x.dtype, device=x.device)
+    if out.shape != x.shape or (c > 1 and (x.stride(2) != 1 or out.stride(2) != 1)):
+        raise ValueError("x and out must be of one shape with contiguous channels")
+    _vector(gamma, c, "gamma")
+    _vector(beta, c, "beta")
+    _on_current_device(x, out, gamma, beta, workspace)
+    if workspace is None:
+        workspace = torch.empty(group_norm_workspace(f, p, c, groups), dtype=torch.uint8,
+                                device=x.device)
+    check(lib().s2_group_norm(_ptr(x), xd, x.stride(0), x.stride(1), f, p, c, groups,
+                              _ptr(gamma), _ptr(beta), float(epsilon), activation, _ptr(out),
+                              _dtype_code(out), out.stride(0), out.stride(1), _ptr(workspace),
+                              workspace.numel() * workspace.element_size(), _stream(stream)),
+          "s2_group_norm")
+    return out
+
+
+def group_norm_workspace(frames, pixels, channels, groups) -> int:
+    """s2_group_norm_workspace_bytes."""
+    n = ctypes.c_size_t()
+    check(lib().s2_group_norm_workspace_bytes(frames, pixels, channels, groups, ctypes.byref(n)),
+          "s2_group_norm_workspace_bytes")
+    return n.value
+
+
+def _matmul_views(x, n, k, weight, residual, out, out_dtype):
+    """The checked output of linear and grouped_linear."""
+    import torch
+    if x.dim() != 2 or x.shape[1] != k:
+        raise ValueError(f"x must be [m, {k}]")
+    if not weight.is_contiguous():
+        raise ValueError("weight must be contiguous")
+    m = x.shape[0]
+    if out is None:
+        out = torch.empty((m, n), dtype=out_dtype or x.dtype, device=x.device)
+    for t in (x, residual, out):
+        if t is not None and t.shape[1] > 1 and t.stride(1) != 1:
+            raise ValueError("rows must be contiguous")
+    if out.shape != (m, n) or (residual is not None and
+                               (residual.shape != out.shape or residual.dtype != out.dtype)):
+        raise ValueError(f"out and residual must be [{m}, {n}] of one type")
+    return out
+
+
+def linear_workspace(m, n, k, x_dtype=DTYPE_BF16) -> int:
+    """s2_linear_workspace_bytes."""
+    b = ctypes.c_size_t()
+    check(lib().s2_linear_workspace_bytes(m, n, k, x_dtype, ctypes.byref(b)),
+          "s2_linear_workspace_bytes")
+    return b.value
+
+
+def linear(x, weight, bias=None, activation=ACT_NONE, residual=None, out=None, out_dtype=None,
+           workspace=None, stream=None):
+    """s2_linear: residual + act(x W^T + bias) of rows x [m, k] with weight
+    [n, k] (bf16 for fp32 and bf16 rows, fp16 for fp16 rows).  Rows may be
+    strided.  out may be the residual.  workspace: linear_workspace(...) bytes,
+    allocated on the current stream if None.  Returns out [m, n]."""
+    import torch
+    n, k = weight.shape
+    out = _matmul_views(x, n, k, weight, residual, out, out_dtype)
+    _vector(bias, n, "bias")
+    m, xd = x.shape[0], _dtype_code(x)
+    _on_current_device(x, weight, bias, residual, out, workspace)
+    size = 0
+    if workspace is None:
+        size = linear_workspace(m, n, k, xd)
+        if size:
+            workspace = torch.empty(size, dtype=torch.uint8, device=x.device)
+    else:
+        size = workspace.numel() * workspace.element_size()
+    check(lib().s2_linear(_ptr(x), xd, x.stride(0), m, _ptr(weight), _dtype_code(weight),
+                          _ptr(bias), n, k, activation, _ptr(residual),
+                          residual.stride(0) if residual is not None else 0, _ptr(out),
+                          _dtype_code(out), out.stride(0), _ptr(workspace), size,
+                          _stream(stream)), "s2_linear")
+    return out
+
+
+def grouped_linear(x, offsets, weight, bias=None, activation=ACT_NONE, residual=None, out=None,
+                   out_dtype=None, stream=None):
+    """s2_grouped_linear: linear over the row groups offsets[g] ..
+    offsets[g + 1] - 1 (int32 on the device) with weight [groups, n, k] and
+    bias [groups, n].  Rows in no group are left as they are in out (undefined
+    in one that this call makes).  Returns out [m, n]."""
+    import torch
+    groups, n, k = weight.shape
+    out = _matmul_views(x, n, k, weight, residual, out, out_dtype)
+    if offsets.dtype != torch.int32 or offsets.numel() != groups + 1 or not offsets.is_contiguous():
+        raise ValueError(f"offsets must be {groups + 1} contiguous int32 values")
+    _vector(bias, groups * n, "bias")
+    _on_current_device(x, offsets, weight, bias, residual, out)
+    check(lib().s2_grouped_linear(_ptr(x), _dtype_code(x), x.stride(0), x.shape[0], _ptr(offsets),
+                                  groups, _ptr(weight), _dtype_code(weight), _ptr(bias), n, k,
+                                  activation, _ptr(residual),
+                                  residual.stride(0) if residual is not None else 0, _ptr(out),
+                                  _dtype_code(out), out.stride(0), _stream(stream)),
+          "s2_grouped_linear")
+    return out
 
 
 # ---- DecomposedConv3D ------------------------------------------------------------

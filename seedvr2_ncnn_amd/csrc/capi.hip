@@ -12,6 +12,8 @@
 #include "block_kernels.h"
 #include "conv3d_kernels.h"
 #include "graph_ops_kernels.h"
+#include "group_norm_kernels.h"
+#include "matmul_kernels.h"
 #include "mha_kernels.h"
 #include "pipeline_kernels.h"
 #include "seedvr2_hip.h"
@@ -1237,6 +1239,138 @@ int s2_dit_ada_out_in(int hidden, int batch, const int* video_rows, const int* t
     a.scale_b[0] = video_scale;
     a.scale_b[1] = text_scale;
     S2_HIP(s2::launch_ada_out(a, (hipStream_t)stream));
+    return S2_OK;
+}
+
+/* ---- group norm, linear, grouped linear ----------------------------------- */
+
+static bool row_activation(int a) {
+    return a == S2_ACT_NONE || a == S2_ACT_GELU || a == S2_ACT_SILU || a == S2_ACT_GELU_TANH;
+}
+
+static int group_norm_shape_ok(int frames, int pixels, int channels, int groups) {
+    if (frames < 0 || frames > 65535 || pixels < 0)
+        return fail(S2_ERR_INVALID, "group norm needs 0..65535 frames and pixels >= 0");
+    if (groups <= 0 || channels <= 0 || channels > 4096 || channels % groups != 0)
+        return fail(S2_ERR_INVALID, "group norm needs channels a multiple of groups, at most 4096");
+    return S2_OK;
+}
+
+int s2_group_norm_workspace_bytes(int frames, int pixels, int channels, int groups, size_t* bytes) {
+    if (!bytes) return fail(S2_ERR_INVALID, "null bytes");
+    const int ret = group_norm_shape_ok(frames, pixels, channels, groups);
+    if (ret != S2_OK) return ret;
+    *bytes = s2::group_norm_workspace(frames, pixels, channels, groups);
+    return S2_OK;
+}
+
+int s2_group_norm(const void* x, s2_dtype x_dtype, long x_frame_stride, long x_pixel_stride,
+                  int frames, int pixels, int channels, int groups, const float* gamma,
+                  const float* beta, float epsilon, int activation, void* y, s2_dtype y_dtype,
+                  long y_frame_stride, long y_pixel_stride, void* workspace,
+                  size_t workspace_bytes, s2_stream_t stream) {
+    const int ret = group_norm_shape_ok(frames, pixels, channels, groups);
+    if (ret != S2_OK) return ret;
+    if (!dtype_ok(x_dtype) || !dtype_ok(y_dtype)) return fail(S2_ERR_INVALID, "unsupported dtype");
+    if (!row_activation(activation)) return fail(S2_ERR_INVALID, "unknown activation");
+    if (!(epsilon >= 0.f)) return fail(S2_ERR_INVALID, "epsilon must be >= 0");
+    if (frames == 0 || pixels == 0) return S2_OK;
+    if (!x || !y) return fail(S2_ERR_INVALID, "null operand");
+    // x may be broadcast (stride 0); rows of y are apart, frames outside pixels or
+    // the other way round
+    typedef __int128 wide;   // strides have 64 bits, extents 31
+    const wide yf = frames > 1 ? y_frame_stride : 0, yp = pixels > 1 ? y_pixel_stride : 0;
+    if ((frames > 1 && x_frame_stride < 0) || (pixels > 1 && x_pixel_stride < 0) ||
+        (frames > 1 && yf < channels) || (pixels > 1 && yp < channels) ||
+        (frames > 1 && pixels > 1 && yf < (pixels - 1) * yp + channels &&
+         yp < (frames - 1) * yf + channels))
+        return fail(S2_ERR_INVALID, "negative strides, or rows of y that overlap");
+    if (!aligned(x, dtype_bytes(x_dtype)) || !aligned(y, dtype_bytes(y_dtype)) ||
+        !aligned(gamma, 4) || !aligned(beta, 4))
+        return fail(S2_ERR_INVALID, "operands must be aligned to their elements");
+    if (x == y && (x_dtype != y_dtype || x_frame_stride != y_frame_stride ||
+                   x_pixel_stride != y_pixel_stride))
+        return fail(S2_ERR_INVALID, "in place needs one type and one pair of strides");
+    const size_t need = s2::group_norm_workspace(frames, pixels, channels, groups);
+    if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 8)))
+        return fail(S2_ERR_INVALID, "workspace too small or not 8-byte aligned");
+    s2::GroupNormArgs p;
+    p.x = x;
+    p.x_kind = (int)x_dtype;
+    p.x_frame = x_frame_stride;
+    p.x_pixel = x_pixel_stride;
+    p.frames = frames;
+    p.pixels = pixels;
+    p.channels = channels;
+    p.groups = groups;
+    p.gamma = gamma;
+    p.beta = beta;
+    p.eps = epsilon;
+    p.act = activation;
+    p.y = y;
+    p.y_kind = (int)y_dtype;
+    p.y_frame = y_frame_stride;
+    p.y_pixel = y_pixel_stride;
+    S2_HIP(s2::launch_group_norm(p, workspace, (hipStream_t)stream));
+    return S2_OK;
+}
+
+// Argument checks of s2_linear and s2_grouped_linear.
+static int matmul_args_ok(const s2::MatmulArgs& a, bool any_rows) {
+    if (a.m < 0 || a.n <= 0 || a.k <= 0) return fail(S2_ERR_INVALID, "invalid linear shape");
+    if (!dtype_ok((s2_dtype)a.x_kind) || !dtype_ok((s2_dtype)a.w_kind) || !dtype_ok((s2_dtype)a.y_kind))
+        return fail(S2_ERR_INVALID, "unsupported dtype");
+    if (!((a.w_kind == S2_DTYPE_BF16 && a.x_kind != S2_DTYPE_F16) ||
+          (a.w_kind == S2_DTYPE_F16 && a.x_kind == S2_DTYPE_F16)))
+        return fail(S2_ERR_INVALID, "the weight is bf16 for fp32 and bf16 rows, fp16 for fp16 rows");
+    if (!row_activation(a.act)) return fail(S2_ERR_INVALID, "unknown activation");
+    if (!any_rows) return S2_OK;
+    if (!a.x || !a.w || !a.y) return fail(S2_ERR_INVALID, "null operand");
+    if (a.m > 1 && (a.x_stride < a.k || a.y_stride < a.n || (a.res && a.res_stride < a.n)))
+        return fail(S2_ERR_INVALID, "row strides shorter than rows");
+    const size_t ye = dtype_bytes((s2_dtype)a.y_kind);
+    if (!aligned(a.x, dtype_bytes((s2_dtype)a.x_kind)) || !aligned(a.w, 2) || !aligned(a.y, ye) ||
+        !aligned(a.res, ye) || !aligned(a.bias, 4) || !aligned(a.offsets, 4))
+        return fail(S2_ERR_INVALID, "operands must be aligned to their elements");
+    if (a.res == a.y && a.m > 1 && a.res_stride != a.y_stride)
+        return fail(S2_ERR_INVALID, "in place needs one row stride");
+    return S2_OK;
+}
+
+int s2_linear_workspace_bytes(int m, int n, int k, s2_dtype x_dtype, size_t* bytes) {
+    if (!bytes) return fail(S2_ERR_INVALID, "null bytes");
+    if (m < 0 || n <= 0 || k <= 0 || !dtype_ok(x_dtype))
+        return fail(S2_ERR_INVALID, "invalid linear shape");
+    *bytes = s2::matmul_workspace(m, n, k, (int)x_dtype);
+    return S2_OK;
+}
+
+int s2_linear(const void* x, s2_dtype x_dtype, long x_stride, int m, const void* weight,
+              s2_dtype w_dtype, const float* bias, int n, int k, int activation,
+              const void* residual, long residual_stride, void* y, s2_dtype y_dtype,
+              long y_stride, void* workspace, size_t workspace_bytes, s2_stream_t stream) {
+    const s2::MatmulArgs a{x, (int)x_dtype, x_stride, m, nullptr, 1, weight, (int)w_dtype, bias, n, k,
+                           activation, residual, residual_stride, y, (int)y_dtype, y_stride};
+    const int ret = matmul_args_ok(a, m > 0);
+    if (ret != S2_OK) return ret;
+    if (workspace && !aligned(workspace, 16))
+        return fail(S2_ERR_INVALID, "workspace must be 16-byte aligned");
+    S2_HIP(s2::launch_matmul(a, workspace, workspace ? workspace_bytes : 0, (hipStream_t)stream));
+    return S2_OK;
+}
+
+int s2_grouped_linear(const void* x, s2_dtype x_dtype, long x_stride, int m, const int* offsets,
+                      int groups, const void* weight, s2_dtype w_dtype, const float* bias, int n,
+                      int k, int activation, const void* residual, long residual_stride, void* y,
+                      s2_dtype y_dtype, long y_stride, s2_stream_t stream) {
+    const s2::MatmulArgs a{x, (int)x_dtype, x_stride, m, offsets, groups, weight, (int)w_dtype, bias,
+                           n, k, activation, residual, residual_stride, y, (int)y_dtype, y_stride};
+    if (groups < 0) return fail(S2_ERR_INVALID, "groups must be >= 0");
+    const int ret = matmul_args_ok(a, m > 0 && groups > 0);
+    if (ret != S2_OK) return ret;
+    if (m == 0 || groups == 0) return S2_OK;
+    if (!offsets) return fail(S2_ERR_INVALID, "null offsets");
+    S2_HIP(s2::launch_matmul(a, nullptr, 0, (hipStream_t)stream));
     return S2_OK;
 }
 

@@ -13,6 +13,7 @@
 #include <mutex>
 #include <type_traits>
 
+#include "activations.h"
 #include "awa_index.h"
 #include "awa_kernels.h"
 #include "s2_device.h"
@@ -57,28 +58,6 @@ __device__ __forceinline__ uint4 load_chunk(const float* p) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) h[i] = f32_to_bf16(v[i]);
     return pack8_bf16(h);
-}
-
-// erf-GELU, 0.5 x (1 + erf(x / sqrt 2)) = max(x, 0) - |x| Q(|x|) with
-// Q(a) = 0.5 erfc(a / sqrt 2): both signs reduce to one fma, and for x < 0
-// the result is the product -|x| Q directly, without cancellation.  erfc is
-// Abramowitz & Stegun 7.1.26, erfc(z) = (a1 t + ... + a5 t^5) e^(-z^2),
-// t = 1 / (1 + p z), |error| <= 1.5e-7; the factor 0.5 is folded into a1..a5
-// and e^(-z^2) = 2^(-w^2) with w = z sqrt(log2 e).  (Q as 2^p(a), p a degree-8
-// fit of log2 Q, has one transcendental less and took 1854 us for the 720p
-// MLP against 1882, but its rms error over |x| <= 0.1 is 3.5 times this one's,
-// 1.8e-8 against 5.3e-9, and its relative error over [-8, -6] 5% against 1%.)
-__device__ __forceinline__ float gelu(float x) {
-    constexpr float kSqrtLog2e = 1.2011224087864498f;
-    const float ax = fabsf(x);
-    const float w = ax * (0.70710678118654752f * kSqrtLog2e);
-    const float t = __builtin_amdgcn_rcpf(fmaf(w, 0.3275911f / kSqrtLog2e, 1.f));
-    const float poly =
-        t * (0.5f * 0.254829592f +
-             t * (0.5f * -0.284496736f +
-                  t * (0.5f * 1.421413741f + t * (0.5f * -1.453152027f + t * (0.5f * 1.061405429f)))));
-    const float q = poly * __builtin_amdgcn_exp2f(-w * w);   // Q(|x|)
-    return fmaf(-ax, q, fmaxf(x, 0.f));
 }
 
 }  // namespace

@@ -1,0 +1,98 @@
+"""float64 forms of group norm, linear and grouped linear, and how far an fp32
+computation of them may be off."""
+import torch
+
+from seedvr2_ncnn_amd import capi
+
+U = 2.0 ** -24   # half a step of fp32, relative
+ACTS = {"none": capi.ACT_NONE, "gelu": capi.ACT_GELU, "silu": capi.ACT_SILU,
+        "gelu_tanh": capi.ACT_GELU_TANH}
+
+
+def activation(v, act):
+    if act == "silu":
+        return v * torch.sigmoid(v)
+    if act == "gelu":
+        return v * torch.special.ndtr(v)
+    if act == "gelu_tanh":
+        return v * torch.sigmoid(1.5957691216057308 * (v + 0.044715 * v ** 3))
+    return v
+
+
+def activation_error(v, act):
+    """Of the fp32 activation at v (its argument exact).  The exponentials'
+    arguments z are off by 4 U |z| at most, which moves the result by as much
+    relative to itself; their exponential, sum, reciprocal and product by 12 U.
+    erfc's formula is off by 1.5e-7, times |v| / 2, and by 16 U."""
+    y = activation(v, act).abs()
+    if act == "silu":
+        return (12 + 4 * v.abs()) * U * y
+    if act == "gelu_tanh":
+        return (12 + 4 * 1.6 * (v.abs() + 0.045 * v.abs() ** 3)) * U * y
+    if act == "gelu":
+        return (0.75e-7 + 16 * U) * v.abs()
+    return torch.zeros_like(v)
+
+
+def rounding(y, dtype):
+    """Half a step of dtype at y; subnormals' step is the smallest number's."""
+    info = torch.finfo(dtype)
+    return y.abs() * (info.eps / 2) + info.smallest_normal * info.eps / 2
+
+
+def finish(v, v_err, act, residual, dtype):
+    """(result, bound) of residual + act(v) rounded to dtype, v off by v_err;
+    the activations' slopes stay under 1.13 in magnitude."""
+    y = activation(v, act)
+    err = (1.13 if act != "none" else 1.0) * v_err + activation_error(v, act)
+    if residual is not None:
+        y = y + residual.double()
+        err = err + U * y.abs()
+    return y, err + rounding(y.abs() + err, dtype)
+
+
+def linear(x, w, bias, act, residual, dtype):
+    """k products summed in any order in fp32: (k + 2) U of the sum of their
+    magnitudes, the bias one sum more; an fp32 x as two terms (16-bit results)
+    is off by 2^-15 of itself."""
+    xd, wt = x.double(), w.double().t().contiguous()
+    v = xd @ wt
+    size = xd.abs() @ wt.abs()
+    if bias is not None:
+        v, size = v + bias.double(), size + bias.double().abs()
+    err = (x.shape[1] + 3) * U * size
+    if x.dtype == torch.float32 and dtype != torch.float32:
+        err = err + 2.0 ** -15 * size
+    return finish(v, err, act, residual, dtype)
+
+
+def group_norm(x, groups, gamma, beta, eps, act, dtype):
+    """A thread sums L values x - K and their squares, K one of them: the sum of
+    squares is off by (L + 3) U of itself, the mean by (L + 3) U of the mean
+    distance from K and, stored in fp32 three times, by 3 U of itself."""
+    f, p, c = x.shape
+    xd = x.double().reshape(f, p, groups, c // groups)
+    mean = xd.mean(dim=(1, 3), keepdim=True)
+    d = xd - mean
+    var = (d * d).mean(dim=(1, 3), keepdim=True)
+    far = (xd.amax(dim=1, keepdim=True) - xd.amin(dim=1, keepdim=True)).amax(dim=3, keepdim=True)
+    length = max(16384 // c, -(-p // max(1, 1024 // f)), 1)
+    length = min(length, p)
+    mean_err = (length + 3) * U * far + 3 * U * mean.abs()
+    # the deviations' sum of squares, from sums about K (at most `far` away) and
+    # from means of parts that are off by mean_err each
+    var_err = 2 * (length + 3) * U * far ** 2 + 2 * mean_err * far + mean_err ** 2
+    std = (var + eps).sqrt()
+    hat = d / std
+    hat_err = (mean_err + 2 * U * d.abs()) / std + hat.abs() * (0.5 * var_err / (var + eps) + 4 * U)
+    g = 1.0 if gamma is None else gamma.double()
+    b = 0.0 if beta is None else beta.double()
+    v = hat.reshape(f, p, c) * g + b
+    v_err = hat_err.expand_as(hat).reshape(f, p, c) * abs(g) + 2 * U * v.abs()
+    return finish(v, v_err, act, None, dtype)
+
+
+def check(got, want, bound):
+    off = (got.double() - want).abs()
+    worst = (off / bound).max().item() if off.numel() else 0.0
+    assert worst <= 1.0, f"{worst:.3g} times the bound"

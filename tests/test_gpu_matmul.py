@@ -1,0 +1,315 @@
+"""s2_linear and s2_grouped_linear against a float64 form: types, sizes from one
+row, column and product to many tiles, strides, alignment, residuals in place,
+ragged and empty groups, rows outside them, and non-finite values."""
+import pytest
+
+from seedvr2_ncnn_amd import capi
+
+pytestmark = pytest.mark.gpu
+
+# x, weight
+PAIRS = [("float32", "bfloat16"), ("bfloat16", "bfloat16"), ("float16", "float16")]
+Y_TYPES = ["float32", "bfloat16", "float16"]
+# (m, k, n): single ones; k below, at and past a k-step and of no even alignment;
+# n that ends inside a 16-column piece, a wave's and a tile's columns; row counts
+# around 16, 64, 128 and 256
+SIZES = [(1, 1, 1), (1, 2560, 130), (2, 7, 16), (3, 132, 300), (15, 33, 17), (16, 64, 64),
+         (17, 72, 48), (33, 129, 257), (64, 1000, 129), (65, 192, 512), (127, 8, 8), (129, 320, 100),
+         (255, 640, 264), (257, 65, 128), (300, 2048, 256), (520, 96, 1030)]
+
+
+def _gen(seed):
+    import torch
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    return lambda *s: torch.randn(*s, generator=gen, device="cuda")
+
+
+def _operands(m, k, n, pair, y_type, groups=0, seed=0):
+    import torch
+    draw = _gen(seed + m + 7 * k + n)
+    x = draw(m, k).to(getattr(torch, pair[0]))
+    lead = (groups,) if groups else ()
+    w = (draw(*lead, n, k) * k ** -0.5).to(getattr(torch, pair[1]))
+    bias = draw(*lead, n)
+    res = draw(m, n).to(getattr(torch, y_type))
+    return x, w, bias, res
+
+
+def _check(got, x, w, bias, act, res):
+    import row_operators as ro
+    want, bound = ro.linear(x, w, bias, act, res, got.dtype)
+    ro.check(got, want, bound)
+
+
+@pytest.mark.parametrize("size", SIZES, ids=str)
+@pytest.mark.parametrize("pair", PAIRS, ids="-".join)
+def test_sizes(size, pair):
+    import torch
+    m, k, n = size
+    x, w, bias, res = _operands(m, k, n, pair, "float32")
+    got = capi.linear(x, w, bias, residual=res, out_dtype=torch.float32)
+    _check(got, x, w, bias, "none", res)
+
+
+@pytest.mark.parametrize("size", [(1, 512, 160), (40, 256, 96), (200, 384, 272), (130, 100, 77)], ids=str)
+@pytest.mark.parametrize("pair", PAIRS, ids="-".join)
+@pytest.mark.parametrize("y_type", Y_TYPES)
+def test_types_activations_and_residuals(size, pair, y_type):
+    import torch
+    import row_operators as ro
+    m, k, n = size
+    x, w, bias, res = _operands(m, k, n, pair, y_type)
+    for act, code in ro.ACTS.items():
+        for b, r in ((bias, None), (None, res), (bias, res)):
+            got = capi.linear(x, w, b, code, r, out_dtype=getattr(torch, y_type))
+            _check(got, x, w, b, act, r)
+
+
+@pytest.mark.parametrize("m", [1, 48, 96, 300])
+@pytest.mark.parametrize("pair", PAIRS, ids="-".join)
+@pytest.mark.parametrize("pads", [(8, 8, 8), (4, 12, 4), (1, 3, 5)], ids=str)
+def test_strides_and_in_place(m, pair, pads):
+    """Rows inside wider buffers at aligned and odd places; the residual as the
+    output; nothing outside the output's rows and columns changes."""
+    import torch
+    k, n = 320, 136
+    y_type = pair[0]
+    x, w, bias, res = _operands(m, k, n, pair, y_type)
+    px, pr, py = pads
+    xw = torch.full((m, k + px), float("nan"), dtype=x.dtype, device="cuda")
+    xw[:, px:] = x
+    rw = torch.full((m, n + pr), float("nan"), dtype=res.dtype, device="cuda")
+    rw[:, pr:] = res
+    yw = torch.full((m + 2, n + 2 * py), 5.0, dtype=res.dtype, device="cuda")
+    got = capi.linear(xw[:, px:], w, bias, capi.ACT_SILU, rw[:, pr:], out=yw[1:m + 1, py:py + n])
+    _check(got, x, w, bias, "silu", res)
+    inside = torch.zeros_like(yw, dtype=torch.bool)
+    inside[1:m + 1, py:py + n] = True
+    assert (yw[~inside] == 5).all()
+    capi.linear(xw[:, px:], w, bias, capi.ACT_SILU, rw[:, pr:], out=rw[:, pr:])
+    assert torch.equal(rw[:, pr:], got) and rw[:, :pr].isnan().all()
+
+
+@pytest.mark.parametrize("pair", PAIRS, ids="-".join)
+def test_weights_at_odd_places(pair):
+    """Weight and bias that start at no 16-byte boundary."""
+    import torch
+    for m in (2, 90, 300):
+        x, w, bias, res = _operands(m, 256, 128, pair, "float32")
+        wide = torch.empty(w.numel() + 3, dtype=w.dtype, device="cuda")
+        odd = wide[3:].view_as(w)
+        odd.copy_(w)
+        wb = torch.empty(129, device="cuda")
+        wb[1:] = bias
+        got = capi.linear(x, odd, wb[1:], residual=res, out_dtype=torch.float32)
+        _check(got, x, w, bias, "none", res)
+
+
+@pytest.mark.parametrize("m,k,n", [(1, 512, 100), (60, 520, 64), (200, 4096, 130), (300, 132, 257)])
+@pytest.mark.parametrize("pair", PAIRS, ids="-".join)
+def test_non_finite_values_stay_in_their_row(m, k, n, pair):
+    """An infinity and a NaN in a row of x, a NaN in a residual: the row (the
+    element) becomes non-finite, the others keep their bits; so do a column's
+    neighbours of an infinite weight."""
+    import torch
+    x, w, bias, res = _operands(m, k, n, pair, "float32")
+    clean = capi.linear(x, w, bias, residual=res, out_dtype=torch.float32)
+    x[0, k // 2] = float("inf")
+    x[m - 1, k - 1] = float("nan")
+    res[m // 2, n - 1] = float("nan")
+    got = capi.linear(x, w, bias, residual=res, out_dtype=torch.float32)
+    assert not got[0].isfinite().any() and got[m - 1].isnan().all() and got[m // 2, n - 1].isnan()
+    keep = torch.ones_like(got, dtype=torch.bool)
+    keep[0] = keep[m - 1] = False
+    keep[m // 2, n - 1] = False
+    assert torch.equal(got[keep], clean[keep])
+    x, w, bias, res = _operands(m, k, n, pair, "float32")
+    w[n // 2, 3] = float("-inf")
+    got = capi.linear(x, w, bias, residual=res, out_dtype=torch.float32)
+    keep = torch.ones_like(got, dtype=torch.bool)
+    keep[:, n // 2] = False
+    assert not got[:, n // 2].isfinite().any() and torch.equal(got[keep], clean[keep])
+
+
+def test_large_fp32_values():
+    """fp32 rows at the type's largest values and with 24-bit significands: taken
+    exactly where y is fp32."""
+    import torch
+    x = torch.full((5, 64), torch.finfo(torch.float32).max, device="cuda")
+    w = torch.zeros(32, 64, dtype=torch.bfloat16, device="cuda")
+    w[torch.arange(32), torch.arange(32)] = 1.0
+    got = capi.linear(x, w)
+    assert torch.equal(got, x[:, :32])
+    x = torch.randn(300, 64, device="cuda")
+    assert torch.equal(capi.linear(x, w), x[:, :32])
+    assert torch.equal(capi.linear(x[:3], w), x[:3, :32])
+
+
+@pytest.mark.parametrize("m,k,n", [(77, 5120, 256), (130, 2560, 300), (257, 1024, 520)])
+def test_with_and_without_workspace(m, k, n):
+    """Split along k or not: both within the bound, each the same again."""
+    import torch
+    x, w, bias, res = _operands(m, k, n, PAIRS[1], "float32")
+    none = torch.empty(0, dtype=torch.uint8, device="cuda")
+    for ws in (None, none):
+        got = capi.linear(x, w, bias, capi.ACT_GELU, res, out_dtype=torch.float32, workspace=ws)
+        _check(got, x, w, bias, "gelu", res)
+        again = capi.linear(x, w, bias, capi.ACT_GELU, res, out_dtype=torch.float32, workspace=ws)
+        assert torch.equal(got, again)
+
+
+GROUPS = [[5], [0, 3, 0], [1] * 9, [130, 0, 1, 64, 0, 0, 257], [0] * 70 + [20, 0, 33], [16] * 40,
+          [700, 2]]
+
+
+@pytest.mark.parametrize("rows", GROUPS, ids=lambda r: "-".join(map(str, r[-5:])))
+@pytest.mark.parametrize("pair", PAIRS, ids="-".join)
+@pytest.mark.parametrize("kn", [(256, 136), (72, 33), (1000, 260)], ids=str)
+def test_groups(rows, pair, kn):
+    """Rows before the first group and behind the last one keep what they held."""
+    import torch
+    import row_operators as ro
+    k, n = kn
+    before, behind = 3, 5
+    m = before + sum(rows) + behind
+    x, w, bias, res = _operands(m, k, n, pair, "float32", len(rows))
+    x[:before] = float("nan")
+    x[m - behind:] = float("inf")
+    ends = [before]
+    for r in rows:
+        ends.append(ends[-1] + r)
+    offsets = torch.tensor(ends, dtype=torch.int32, device="cuda")
+    out = torch.full((m, n), 9.0, device="cuda")
+    capi.grouped_linear(x, offsets, w, bias, capi.ACT_GELU_TANH, res, out=out)
+    for g, (a, b) in enumerate(zip(ends[:-1], ends[1:])):
+        if a < b:
+            _check(out[a:b], x[a:b], w[g], bias[g], "gelu_tanh", res[a:b])
+    assert (out[:before] == 9).all() and (out[m - behind:] == 9).all()
+    got = capi.grouped_linear(x, offsets, w, out_dtype=torch.bfloat16)
+    a = next(g for g, r in enumerate(rows) if r)
+    _check(got[ends[a]:ends[a + 1]], x[ends[a]:ends[a + 1]], w[a], None, "none", None)
+
+
+def test_offsets_out_of_range_are_clamped():
+    """Offsets below 0 and past m stand for 0 and m; descending ones leave every
+    byte outside y alone."""
+    import torch
+    x, w, bias, res = _operands(90, 128, 64, PAIRS[1], "float32", 3)
+    whole = torch.full((94, 64), 2.0, device="cuda")
+    out = whole[2:92]
+    offs = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")
+    capi.grouped_linear(x, offs(-7, 30, 60, 2 ** 31 - 1), w, bias, out=out)
+    for g in range(3):
+        _check(out[30 * g:30 * g + 30], x[30 * g:30 * g + 30], w[g], bias[g], "none", None)
+    capi.grouped_linear(x, offs(80, 10, 200, -5), w, bias, out=out)
+    torch.cuda.synchronize()
+    assert (whole[:2] == 2).all() and (whole[92:] == 2).all()
+
+
+def test_no_rows_and_no_groups():
+    import torch
+    w = torch.zeros(24, 16, dtype=torch.bfloat16, device="cuda")
+    x = torch.empty(0, 16, dtype=torch.bfloat16, device="cuda")
+    assert capi.linear(x, w).shape == (0, 24)
+    offs = torch.zeros(3, dtype=torch.int32, device="cuda")
+    assert capi.grouped_linear(x, offs, w.expand(2, 24, 16).contiguous()).shape == (0, 24)
+    out = torch.ones(4, 24, dtype=torch.bfloat16, device="cuda")
+    rows = torch.zeros(4, 16, dtype=torch.bfloat16, device="cuda")
+    capi.grouped_linear(rows, offs[:1], w[None][:0], out=out)
+    capi.grouped_linear(rows, offs, w.expand(2, 24, 16).contiguous(), out=out)
+    torch.cuda.synchronize()
+    assert (out == 1).all()
+
+
+def test_repeats_streams_and_capture():
+    import torch
+    x, w, bias, res = _operands(300, 1280, 256, PAIRS[1], "bfloat16")
+    _, wg, bg, _ = _operands(300, 1280, 256, PAIRS[1], "bfloat16", 3)
+    offsets = torch.tensor([0, 100, 100, 290], dtype=torch.int32, device="cuda")
+
+    def both():
+        y = capi.linear(x, w, bias, capi.ACT_SILU, res)
+        z = torch.zeros_like(y)
+        return y, capi.grouped_linear(x, offsets, wg, bg, capi.ACT_GELU, res, out=z)
+
+    want = both()
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        again = both()
+    side.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(again, want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = both()
+    for i in range(3):
+        x.copy_(_gen(40 + i)(300, 1280))
+        offsets.copy_(torch.tensor([i, 90 + i, 120, 300], dtype=torch.int32))
+        for t in out:
+            t.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(out, both()):
+            assert torch.equal(a, b)
+
+
+def test_timestep_embedding_chain():
+    """Two timesteps to a block's modulation rows as the DiT's frontend does:
+    embedding, product + SiLU, product + SiLU, product; fp32 rows, bf16 weights."""
+    import torch
+    import row_operators as ro
+    draw = _gen(2)
+    ws = [(draw(n, k) * k ** -0.5).bfloat16() for n, k in ((640, 256), (640, 640), (3840, 640))]
+    bs = [0.1 * draw(w.shape[0]) for w in ws]
+    h = capi.timestep_embedding([999.0, 0.5])
+    for w, b, act in zip(ws, bs, ("silu", "silu", "none")):
+        got = capi.linear(h, w, b, ro.ACTS[act])
+        _check(got, h, w, b, act, None)
+        h = got
+    assert h.shape == (2, 3840)
+
+
+def test_vae_attention_block():
+    """The VAE's mid block on channels-last rows: group norm into VAEChunkedMHA, then
+    x's 1x1x1 shortcut with the attention's output as its residual, in place; each
+    step of this library against float64 on what went into it."""
+    import torch
+    import row_operators as ro
+    draw = _gen(4)
+    seq, c = 330, 128
+    x = draw(1, seq, c).bfloat16()
+    gamma, beta = 1 + 0.1 * draw(c), 0.1 * draw(c)
+    h = capi.group_norm(x, 32, gamma, beta)
+    ro.check(h, *ro.group_norm(x, 32, gamma, beta, 1e-6, "none", h.dtype))
+    mats = [draw(c, c) * c ** -0.5 for _ in range(4)]
+    zero = torch.zeros(c, device="cuda")
+    mha = capi.Mha(1, *(t for w in mats for t in (w, zero)), scale=c ** -0.5)
+    a = mha.forward(h[0])
+    q, k, v = (h[0].float() @ w.t() for w in mats[:3])
+    ref = torch.softmax(q @ k.t() * c ** -0.5, dim=-1) @ v @ mats[3].t()
+    # bf16 projections, weights and sums: a few of their half steps
+    assert ((a.float() - ref).norm() / ref.norm()).item() < 6 * 2.0 ** -8
+    w, b = (draw(c, c) * c ** -0.5).bfloat16(), 0.1 * draw(c)
+    before = a.clone()
+    y = capi.linear(x[0], w, b, residual=a, out=a)
+    _check(y, x[0], w, b, "none", before)
+
+
+def test_two_stream_mlp():
+    """A DiT block's MLP whose video and text rows have weights of their own, onto
+    the fp32 residual stream in place."""
+    import torch
+    draw = _gen(6)
+    rows, hidden, inner = [450, 64], 256, 1024
+    m = sum(rows)
+    offs = torch.tensor([0, rows[0], m], dtype=torch.int32, device="cuda")
+    up = (draw(2, inner, hidden) * hidden ** -0.5).bfloat16()
+    down = (draw(2, hidden, inner) * inner ** -0.5).bfloat16()
+    bu, bd = 0.1 * draw(2, inner), 0.1 * draw(2, hidden)
+    x, res = draw(m, hidden).bfloat16(), draw(m, hidden)
+    start = res.clone()
+    h = capi.grouped_linear(x, offs, up, bu, capi.ACT_GELU_TANH)
+    capi.grouped_linear(h, offs, down, bd, residual=res, out=res)
+    for g, (a, b) in enumerate(((0, rows[0]), (rows[0], m))):
+        _check(h[a:b], x[a:b], up[g], bu[g], "gelu_tanh", None)
+        _check(res[a:b], h[a:b], down[g], bd[g], "none", start[a:b])

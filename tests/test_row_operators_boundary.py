@@ -1,0 +1,126 @@
+"""Refusals of s2_group_norm, s2_linear and s2_grouped_linear and of their
+bindings, all before a device is touched."""
+import ctypes
+
+import pytest
+
+from seedvr2_ncnn_amd import capi
+
+F32, BF16, F16 = capi.DTYPE_F32, capi.DTYPE_BF16, capi.DTYPE_F16
+P = 0x10000   # stands for a device address; none of these calls gets to use it
+
+NORM = dict(x=P, x_dtype=F32, x_frame=4096, x_pixel=64, frames=2, pixels=64, channels=64, groups=8,
+            gamma=P, beta=P, epsilon=1e-6, activation=capi.ACT_NONE, y=2 * P, y_dtype=F32,
+            y_frame=4096, y_pixel=64, workspace=P, workspace_bytes=1 << 20, stream=None)
+LINEAR = dict(x=P, x_dtype=BF16, x_stride=64, m=4, weight=P, w_dtype=BF16, bias=P, n=32, k=64,
+              activation=capi.ACT_NONE, residual=P, residual_stride=32, y=2 * P, y_dtype=F32,
+              y_stride=32, workspace=None, workspace_bytes=0, stream=None)
+GROUPED = dict(x=P, x_dtype=BF16, x_stride=64, m=4, offsets=P, groups=2, weight=P, w_dtype=BF16,
+               bias=P, n=32, k=64, activation=capi.ACT_NONE, residual=P, residual_stride=32, y=2 * P,
+               y_dtype=F32, y_stride=32, stream=None)
+
+
+def _call(name, base, **changes):
+    assert set(changes) <= set(base)
+    return getattr(capi.lib(), name)(*dict(base, **changes).values())
+
+
+@pytest.mark.parametrize("changes", [
+    dict(frames=-1), dict(frames=65536), dict(pixels=-1), dict(groups=0), dict(groups=-8),
+    dict(groups=7), dict(channels=0), dict(channels=4104, groups=8), dict(x_dtype=3), dict(y_dtype=-1),
+    dict(activation=capi.ACT_SWIGLU), dict(activation=5), dict(epsilon=-1e-6),
+    dict(epsilon=float("nan")), dict(x=None), dict(y=None), dict(x_frame=-1), dict(x_pixel=-64),
+    dict(y_pixel=63), dict(y_frame=63), dict(y_frame=4095), dict(x=P + 2), dict(y=P + 2),
+    dict(gamma=P + 2), dict(beta=P + 1), dict(workspace=None), dict(workspace_bytes=8),
+    dict(workspace=P + 4), dict(y=P, y_dtype=BF16), dict(y=P, y_frame=8192)], ids=str)
+def test_group_norm_refuses(changes):
+    assert _call("s2_group_norm", NORM, **changes) == capi.S2_ERR_INVALID
+    assert capi.last_error()
+
+
+def test_group_norm_takes_interleaved_frames_as_far_as_the_device():
+    """Frames interleaved by pixel pass the checks of the strides."""
+    if capi.device_count():
+        pytest.skip("the call would run")
+    assert _call("s2_group_norm", NORM, y_frame=64, y_pixel=128) == capi.S2_ERR_DEVICE
+
+
+def test_group_norm_of_nothing():
+    assert _call("s2_group_norm", NORM, frames=0, x=None, y=None) == capi.S2_OK
+    assert _call("s2_group_norm", NORM, pixels=0, workspace=None) == capi.S2_OK
+    assert capi.group_norm_workspace(0, 5, 8, 2) == 0
+    assert capi.group_norm_workspace(3, 50000, 8, 2) > 0
+    for bad in ((1, 1, 9, 2), (1, 1, 8192, 2), (-1, 1, 8, 2), (1, -1, 8, 2)):
+        with pytest.raises(capi.S2Error):
+            capi.group_norm_workspace(*bad)
+
+
+MATMUL = [
+    dict(m=-1), dict(n=0), dict(k=0), dict(n=-4), dict(x_dtype=3), dict(y_dtype=7),
+    dict(w_dtype=F32), dict(w_dtype=F16), dict(x_dtype=F16), dict(x_dtype=F32, w_dtype=F16),
+    dict(activation=capi.ACT_SWIGLU), dict(activation=-1), dict(x=None), dict(weight=None),
+    dict(y=None), dict(x_stride=63), dict(y_stride=31), dict(residual_stride=31), dict(x=P + 1),
+    dict(weight=P + 1), dict(y=P + 2), dict(residual=P + 2), dict(bias=P + 2),
+    dict(residual=2 * P, residual_stride=40)]
+
+
+@pytest.mark.parametrize("changes", MATMUL + [dict(workspace=P + 8, workspace_bytes=64)], ids=str)
+def test_linear_refuses(changes):
+    assert _call("s2_linear", LINEAR, **changes) == capi.S2_ERR_INVALID
+    assert capi.last_error()
+
+
+@pytest.mark.parametrize("changes", MATMUL + [dict(groups=-1), dict(offsets=None), dict(offsets=P + 2)],
+                         ids=str)
+def test_grouped_linear_refuses(changes):
+    assert _call("s2_grouped_linear", GROUPED, **changes) == capi.S2_ERR_INVALID
+    assert capi.last_error()
+
+
+def test_linear_of_nothing():
+    assert _call("s2_linear", LINEAR, m=0, x=None, y=None) == capi.S2_OK
+    assert _call("s2_grouped_linear", GROUPED, m=0) == capi.S2_OK
+    assert _call("s2_grouped_linear", GROUPED, groups=0, offsets=None) == capi.S2_OK
+    assert capi.linear_workspace(0, 8, 8) == 0
+    for bad in ((-1, 8, 8), (1, 0, 8), (1, 8, 0)):
+        with pytest.raises(capi.S2Error):
+            capi.linear_workspace(*bad)
+    assert capi.lib().s2_linear_workspace_bytes(1, 1, 1, 0, None) == capi.S2_ERR_INVALID
+    assert capi.lib().s2_group_norm_workspace_bytes(1, 1, 1, 1, None) == capi.S2_ERR_INVALID
+
+
+def test_other_entry_points_do_not_take_the_new_activations():
+    n = ctypes.c_void_p(P)
+    for act in (capi.ACT_SILU, capi.ACT_GELU_TANH):
+        assert capi.lib().s2_shared_linear_forward(n, 8, None, 0, BF16, n, None, 64, 64, act, n, None,
+                                                   BF16, None) == capi.S2_ERR_INVALID
+
+
+def test_bindings_check_shapes_and_types():
+    import torch
+    x, w = torch.zeros(4, 64), torch.zeros(32, 64, dtype=torch.bfloat16)
+    offs = torch.zeros(3, dtype=torch.int32)
+    wg = torch.zeros(2, 32, 64, dtype=torch.bfloat16)
+    frames = torch.zeros(2, 8, 64)
+    for call in (lambda: capi.linear(x[:, :32], w), lambda: capi.linear(x.t().contiguous().t(), w),
+                 lambda: capi.linear(x, w.t().contiguous().t()),
+                 lambda: capi.linear(x, w, torch.zeros(31)),
+                 lambda: capi.linear(x, w, torch.zeros(32, dtype=torch.float64)),
+                 lambda: capi.linear(x, w, residual=torch.zeros(4, 31)),
+                 lambda: capi.linear(x, w, residual=torch.zeros(4, 32).half()),
+                 lambda: capi.linear(x, w, out=torch.zeros(5, 32)),
+                 lambda: capi.grouped_linear(x, offs.long(), wg),
+                 lambda: capi.grouped_linear(x, offs[:2], wg),
+                 lambda: capi.grouped_linear(x, offs, wg, torch.zeros(32)),
+                 lambda: capi.group_norm(frames[0], 8), lambda: capi.group_norm(frames.transpose(1, 2), 8),
+                 lambda: capi.group_norm(frames, 8, torch.zeros(8)),
+                 lambda: capi.group_norm(frames, 8, out=torch.zeros(2, 8, 65)),
+                 # host memory
+                 lambda: capi.group_norm(frames, 8), lambda: capi.linear(x, w),
+                 lambda: capi.grouped_linear(x, offs, wg)):
+        with pytest.raises(ValueError):
+            call()
+    with pytest.raises(TypeError):
+        capi.linear(x.double(), w)
+    with pytest.raises(TypeError):
+        capi.group_norm(frames.double(), 8)
