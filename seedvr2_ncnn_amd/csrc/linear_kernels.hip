@@ -230,8 +230,6 @@ __global__ __launch_bounds__(256, 2) void shared_linear_kernel(
 // counter.  No workgroup waits on another.
 namespace {
 
-__device__ __forceinline__ int lds_swizzle(int r) { return ((r >> 1) ^ ((r & 1) << 2)) & 7; }
-
 // Sum over aligned groups of N lanes (N = 8 or 16) by DPP lane moves: quad
 // permutations [1,0,3,2] and [2,3,0,1], then the half-row and row mirrors.
 // Each step adds the value of a lane of the other half of the group, which

@@ -161,6 +161,10 @@ __device__ __forceinline__ void lds_dma16(i32x4 rsrc, uint32_t lds_addr, uint32_
                  : "memory", "m0");
 }
 
+// 16-byte chunk c of a 128-byte LDS row r is kept at position c ^ lds_swizzle(r):
+// the rows that one ds_read_b128 phase touches land on distinct banks
+__device__ __forceinline__ int lds_swizzle(int r) { return ((r >> 1) ^ ((r & 1) << 2)) & 7; }
+
 // Physical workgroup id -> logical id such that consecutive logical ids run
 // on the same XCD (the hardware deals workgroups to XCDs round-robin).
 __device__ __forceinline__ int xcd_remap(int bid, int nblocks) {

@@ -18,6 +18,11 @@ SIZES = [(1, 1, 1), (1, 2560, 130), (2, 7, 16), (3, 132, 300), (15, 33, 17), (16
          (255, 640, 264), (257, 65, 128), (300, 2048, 256), (520, 96, 1030)]
 
 
+# enough tiles of 256 x 256 for every compute unit; one to six k steps, the last one
+# ragged or not
+MANY_TILES = [(4900, 64, 2560), (5001, 200, 2564), (3100, 328, 4104)]
+
+
 def _gen(seed):
     import torch
     gen = torch.Generator(device="cuda").manual_seed(seed)
@@ -49,6 +54,19 @@ def test_sizes(size, pair):
     x, w, bias, res = _operands(m, k, n, pair, "float32")
     got = capi.linear(x, w, bias, residual=res, out_dtype=torch.float32)
     _check(got, x, w, bias, "none", res)
+
+
+@pytest.mark.parametrize("size", MANY_TILES, ids=str)
+@pytest.mark.parametrize("y_type", Y_TYPES)
+def test_many_tiles(size, y_type):
+    import torch
+    import row_operators as ro
+    m, k, n = size
+    for pair in PAIRS[1:]:
+        x, w, bias, res = _operands(m, k, n, pair, y_type)
+        for act, r in (("gelu", None), ("none", res), ("gelu_tanh", res)):
+            got = capi.linear(x, w, bias, ro.ACTS[act], r, out_dtype=getattr(torch, y_type))
+            _check(got, x, w, bias, act, r)
 
 
 @pytest.mark.parametrize("size", [(1, 512, 160), (40, 256, 96), (200, 384, 272), (130, 100, 77)], ids=str)
@@ -160,12 +178,23 @@ def test_with_and_without_workspace(m, k, n):
 
 GROUPS = [[5], [0, 3, 0], [1] * 9, [130, 0, 1, 64, 0, 0, 257], [0] * 70 + [20, 0, 33], [16] * 40,
           [700, 2]]
+# the same with enough 256 x 256 tiles for every compute unit
+MANY_ROWS = [4000, 0, 255, 1, 0, 600]
 
 
 @pytest.mark.parametrize("rows", GROUPS, ids=lambda r: "-".join(map(str, r[-5:])))
 @pytest.mark.parametrize("pair", PAIRS, ids="-".join)
 @pytest.mark.parametrize("kn", [(256, 136), (72, 33), (1000, 260)], ids=str)
 def test_groups(rows, pair, kn):
+    _groups(rows, pair, kn)
+
+
+@pytest.mark.parametrize("pair", PAIRS[1:], ids="-".join)
+def test_groups_of_many_tiles(pair):
+    _groups(MANY_ROWS, pair, (136, 2560))
+
+
+def _groups(rows, pair, kn):
     """Rows before the first group and behind the last one keep what they held."""
     import torch
     import row_operators as ro
