@@ -201,6 +201,139 @@ __device__ __forceinline__ void split_bf16(float x, uint16_t (&h)[XP]) {
     }
 }
 
+// Eight consecutive k of a row as an MFMA operand piece.  GRAN elements lie together
+// (8: 16 bytes of 16-bit elements, 4, or 1); FULL: all eight are before k.
+template <int GRAN, bool FULL>
+__device__ __forceinline__ uint4 piece16(const uint16_t* p, int left) {
+    if constexpr (GRAN == 8) {
+        if (FULL || left > 0) return *reinterpret_cast<const uint4*>(p);
+        return make_uint4(0, 0, 0, 0);
+    } else {
+        alignas(16) uint16_t h[8];
+#pragma unroll
+        for (int e = 0; e < 8; e += GRAN) {
+            if constexpr (GRAN == 4) {
+                uint2 q = make_uint2(0, 0);
+                if (FULL || left > e) q = *reinterpret_cast<const uint2*>(p + e);
+                *reinterpret_cast<uint2*>(h + e) = q;
+            } else {
+                h[e] = FULL || left > e ? p[e] : (uint16_t)0;
+            }
+        }
+        return pack8_bf16(h);
+    }
+}
+
+template <int GRAN, bool FULL>
+__device__ __forceinline__ void piece32(const float* p, int left, float (&v)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; e += 4) {
+        if constexpr (GRAN >= 4) {
+            f32x4 q = {0.f, 0.f, 0.f, 0.f};
+            if (FULL || left > e) q = *reinterpret_cast<const f32x4*>(p + e);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[e + i] = q[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[e + i] = FULL || left > e + i ? p[e + i] : 0.f;
+        }
+    }
+}
+
+// Few rows: up to 16 * MT of them by 16 columns a workgroup.  What costs is reading
+// the weight, once, straight into the MFMAs' operand registers; the waves take every
+// other 64 k (128 bytes of each weight row), x comes from the caches, and the waves'
+// sums meet in LDS.  Rows and columns past the end repeat the last one, and are
+// dropped.
+template <int T, int XP, int MT, int GRAN>
+__global__ __launch_bounds__(512) void matmul_rows_kernel(MatmulArgs a, int ntiles) {
+    constexpr int U = MT * (XP ? 2 : 1) >= 4 ? 2 : 4;   // 64-k chunks in flight
+    constexpr int PL = XP ? XP : 1;
+    __shared__ float sums[8][MT * 256];
+    const RowTile rt = row_tile(a, blockIdx.x / ntiles, 16 * MT);
+    const int col0 = blockIdx.x % ntiles * 16;
+    const int rows = min(rt.end - rt.row0, 16 * MT);
+    if (rows <= 0) return;   // the whole workgroup
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int waves = blockDim.x >> 6;
+    const int l16 = lane & 15, g = lane >> 4;
+    const uint16_t* w = (const uint16_t*)a.w +
+                        ((long)rt.group * a.n + min(col0 + l16, a.n - 1)) * a.k + 8 * g;
+    long xo[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) xo[i] = (long)(rt.row0 + min(16 * i + l16, rows - 1)) * a.x_stride + 8 * g;
+    f32x4 acc[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+    // C chunks from k0, waves * 64 apart
+    auto chunks = [&](int k0, auto count, auto full) {
+        constexpr int C = decltype(count)::value;
+        constexpr bool FULL = decltype(full)::value;
+        uint4 fw[2 * C], fx[XP ? 1 : 2 * C][XP ? 1 : MT];
+        float ff[XP ? 2 * C : 1][XP ? MT : 1][8];
+#pragma unroll
+        for (int c = 0; c < 2 * C; ++c) {
+            const int kc = k0 + (c >> 1) * waves * 64 + (c & 1) * 32;
+            fw[c] = piece16<GRAN, FULL>(w + kc, a.k - kc - 8 * g);
+        }
+#pragma unroll
+        for (int c = 0; c < 2 * C; ++c) {
+            const int kc = k0 + (c >> 1) * waves * 64 + (c & 1) * 32;
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                if constexpr (XP)
+                    piece32<GRAN, FULL>((const float*)a.x + xo[i] + kc, a.k - kc - 8 * g, ff[c][i]);
+                else
+                    fx[c][i] = piece16<GRAN, FULL>((const uint16_t*)a.x + xo[i] + kc, a.k - kc - 8 * g);
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < 2 * C; ++c)
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                if constexpr (XP) {
+                    alignas(16) uint16_t h[PL][8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        uint16_t one[PL];
+                        split_bf16<PL>(ff[c][i][e], one);
+#pragma unroll
+                        for (int q = 0; q < PL; ++q) h[q][e] = one[q];
+                    }
+#pragma unroll
+                    for (int q = 0; q < PL; ++q) acc[i] = mfma<T>(fw[c], pack8_bf16(h[q]), acc[i]);
+                } else {
+                    acc[i] = mfma<T>(fw[c], fx[c][i], acc[i]);
+                }
+            }
+    };
+    int k0 = wave * 64;
+    const int step = waves * 64;
+    for (; k0 + (U - 1) * step + 64 <= a.k; k0 += U * step)
+        chunks(k0, std::integral_constant<int, U>{}, std::true_type{});
+    for (; k0 + 64 <= a.k; k0 += step) chunks(k0, std::integral_constant<int, 1>{}, std::true_type{});
+    if (k0 < a.k) chunks(k0, std::integral_constant<int, 1>{}, std::false_type{});
+
+    // accumulator register r: column 4 g + r of row l16
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+        *reinterpret_cast<f32x4*>(&sums[wave][(i * 16 + l16) * 16 + 4 * g]) = acc[i];
+    __syncthreads();
+    for (int o = threadIdx.x; o < rows * 16; o += blockDim.x) {
+        const int col = col0 + (o & 15);
+        if (col >= a.n) continue;
+        const long row = rt.row0 + (o >> 4);
+        float v = sums[0][o];
+        for (int s = 1; s < waves; ++s) v += sums[s][o];
+        if (a.bias) v += a.bias[(long)rt.group * a.n + col];
+        v = activate(v, a.act);
+        if (a.res) v += load1(a.res, row * a.res_stride + col, a.y_kind);
+        store1(a.y, row * a.y_stride + col, v, a.y_kind);
+    }
+}
+
 // Any strides, alignment, n and k; fp32 activations.  Block tile 128x128,
 // k-step 32, four waves in a 2x2 grid of 64x64, both operands through registers
 // into double-buffered LDS.  XP: bf16 planes that stand for an fp32 x (0: x is of
@@ -689,8 +822,48 @@ hipError_t launch_tiles(const MatmulArgs& a, void* workspace, size_t workspace_b
     return hipGetLastError();
 }
 
+// Elements that lie together in every row of x and of the weight.
+int row_gran(const MatmulArgs& a) {
+    for (int e : {8, 4})
+        if (a.k % e == 0 && a.x_stride % e == 0 && (uintptr_t)a.w % (2 * e) == 0 &&
+            (uintptr_t)a.x % (a.x_kind ? 2 * e : 16) == 0)
+            return e;
+    return 1;
+}
+
+template <int T, int XP, int MT>
+hipError_t launch_rows_mt(const MatmulArgs& a, hipStream_t stream) {
+    const int ntiles = (a.n + 15) / 16;
+    const long blocks = row_tiles(a, 16 * MT) * ntiles;
+    if (blocks > 0x7fffffffL) return hipErrorInvalidValue;
+    const int chunks = (a.k + 63) / 64;
+    const int waves = std::min(8, std::max(1, chunks));
+    const unsigned nb = (unsigned)blocks, nt = 64 * waves;
+    const int gran = row_gran(a);
+    if (gran == 8)
+        matmul_rows_kernel<T, XP, MT, 8><<<nb, nt, 0, stream>>>(a, ntiles);
+    else if (gran == 4)
+        matmul_rows_kernel<T, XP, MT, 4><<<nb, nt, 0, stream>>>(a, ntiles);
+    else
+        matmul_rows_kernel<T, XP, MT, 1><<<nb, nt, 0, stream>>>(a, ntiles);
+    return hipGetLastError();
+}
+
+template <int T, int XP>
+hipError_t launch_rows(const MatmulArgs& a, int rows, hipStream_t stream) {
+    if (rows <= 16) return launch_rows_mt<T, XP, 1>(a, stream);
+    if (rows <= 32) return launch_rows_mt<T, XP, 2>(a, stream);
+    return launch_rows_mt<T, XP, 4>(a, stream);
+}
+
 template <int YK>
 hipError_t launch_y(const MatmulArgs& a, void* workspace, size_t workspace_bytes, hipStream_t stream) {
+    const int rows = a.offsets ? (a.m + a.groups - 1) / a.groups : a.m;   // of a group
+    if (rows <= 64) {
+        if (a.w_kind == 2) return launch_rows<2, 0>(a, rows, stream);
+        if (a.x_kind == 1) return launch_rows<1, 0>(a, rows, stream);
+        return launch_rows<1, YK == 0 ? 3 : 2>(a, rows, stream);
+    }
     if (tiles_take(a))
         return a.w_kind == 2 ? launch_tiles<2, YK>(a, workspace, workspace_bytes, stream)
                              : launch_tiles<1, YK>(a, workspace, workspace_bytes, stream);
@@ -708,6 +881,7 @@ size_t matmul_workspace(int m, int n, int k, int x_kind) {
     a.n = n;
     a.k = k;
     a.groups = 1;
+    if (m <= 64) return 0;
     const int parts = plan_tiles(a, ~(size_t)0).parts;
     return parts > 1 ? (size_t)parts * m * n * sizeof(float) : 0;
 }
