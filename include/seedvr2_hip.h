@@ -534,11 +534,14 @@ S2_API int s2_group_norm(const void* x, s2_dtype x_dtype, long x_frame_stride,
  *   >= n.  y is the residual itself (same stride) or does not overlap it; y
  *   overlaps nothing else.
  * Any m >= 0 (0 does nothing), n and k; pointers aligned to their elements.
- *   Rows whose starts are 16-byte aligned are fastest.
+ *   Fastest are k a multiple of 8 and n of 4, with x and weight rows that start
+ *   at 16 bytes and y and residual rows at four elements.
  * workspace: s2_linear_workspace_bytes, 16-byte aligned (calls that may overlap
- *   in time need one each), or NULL: then nothing is split along k, which is
- *   slower where there are few output tiles. */
-S2_API int s2_linear_workspace_bytes(int m, int n, int k, s2_dtype x_dtype, size_t* bytes);
+ *   in time need one each): rows repacked for the matrix cores, sums of ranges of
+ *   k.  A smaller one, or NULL, is accepted: the call then does without, slower
+ *   for fp32 x, for k that is no multiple of 8 and for few output tiles. */
+S2_API int s2_linear_workspace_bytes(int m, int n, int k, s2_dtype x_dtype, s2_dtype y_dtype,
+                                     size_t* bytes);
 S2_API int s2_linear(const void* x, s2_dtype x_dtype, long x_stride, int m, const void* weight,
                      s2_dtype w_dtype, const float* bias, int n, int k, int activation,
                      const void* residual, long residual_stride, void* y, s2_dtype y_dtype,
@@ -554,12 +557,15 @@ S2_API int s2_linear(const void* x, s2_dtype x_dtype, long x_stride, int m, cons
  *   taken as the nearest of the two; rows that descending offsets put into two
  *   groups, or into none, have unspecified values.
  * weight: device [groups][n][k]; bias: device fp32 [groups][n] or NULL; the
- *   rest as for s2_linear. */
+ *   rest as for s2_linear, workspace: s2_grouped_linear_workspace_bytes. */
+S2_API int s2_grouped_linear_workspace_bytes(int m, int groups, int n, int k, s2_dtype x_dtype,
+                                             s2_dtype y_dtype, size_t* bytes);
 S2_API int s2_grouped_linear(const void* x, s2_dtype x_dtype, long x_stride, int m,
                              const int* offsets, int groups, const void* weight, s2_dtype w_dtype,
                              const float* bias, int n, int k, int activation,
                              const void* residual, long residual_stride, void* y,
-                             s2_dtype y_dtype, long y_stride, s2_stream_t stream);
+                             s2_dtype y_dtype, long y_stride, void* workspace,
+                             size_t workspace_bytes, s2_stream_t stream);
 
 /* ---- DecomposedConv3D (VAE) ---------------------------------------------- */
 /* The causal 3-D convolution of the VAE (src/seedvr2/decomposed_conv3d.h:33-88,

@@ -46,7 +46,8 @@ EXPORTS = (
     "s2_stream_wait", "s2_stream_scratch_acquire", "s2_stream_scratch_release",
     "s2_binary_op", "s2_unary_op", "s2_reduce", "s2_rms_norm", "s2_copy_2d",
     "s2_shared_linear_residual", "s2_group_norm_workspace_bytes", "s2_group_norm",
-    "s2_linear_workspace_bytes", "s2_linear", "s2_grouped_linear",
+    "s2_linear_workspace_bytes", "s2_linear", "s2_grouped_linear_workspace_bytes",
+    "s2_grouped_linear",
 )
 
 
@@ -181,11 +182,12 @@ def lib() -> ctypes.CDLL:
         L.s2_group_norm_workspace_bytes.argtypes = [ci, ci, ci, ci, P(sz)]
         L.s2_group_norm.argtypes = [vp, ci, cl, cl, ci, ci, ci, ci, vp, vp, cf, ci, vp, ci, cl, cl,
                                     vp, sz, vp]
-        L.s2_linear_workspace_bytes.argtypes = [ci, ci, ci, ci, P(sz)]
+        L.s2_linear_workspace_bytes.argtypes = [ci, ci, ci, ci, ci, P(sz)]
+        L.s2_grouped_linear_workspace_bytes.argtypes = [ci, ci, ci, ci, ci, ci, P(sz)]
         L.s2_linear.argtypes = [vp, ci, cl, ci, vp, ci, vp, ci, ci, ci, vp, cl, vp, ci, cl, vp, sz,
                                 vp]
         L.s2_grouped_linear.argtypes = [vp, ci, cl, ci, vp, ci, vp, ci, vp, ci, ci, ci, vp, cl, vp,
-                                        ci, cl, vp]
+                                        ci, cl, vp, sz, vp]
         _LIB = L
     return _LIB
 
@@ -759,12 +761,30 @@ def _matmul_views(x, n, k, weight, residual, out, out_dtype):
     return out
 
 
-def linear_workspace(m, n, k, x_dtype=DTYPE_BF16) -> int:
+def linear_workspace(m, n, k, x_dtype=DTYPE_BF16, y_dtype=DTYPE_BF16) -> int:
     """s2_linear_workspace_bytes."""
     b = ctypes.c_size_t()
-    check(lib().s2_linear_workspace_bytes(m, n, k, x_dtype, ctypes.byref(b)),
+    check(lib().s2_linear_workspace_bytes(m, n, k, x_dtype, y_dtype, ctypes.byref(b)),
           "s2_linear_workspace_bytes")
     return b.value
+
+
+def grouped_linear_workspace(m, groups, n, k, x_dtype=DTYPE_BF16, y_dtype=DTYPE_BF16) -> int:
+    """s2_grouped_linear_workspace_bytes."""
+    b = ctypes.c_size_t()
+    check(lib().s2_grouped_linear_workspace_bytes(m, groups, n, k, x_dtype, y_dtype,
+                                                  ctypes.byref(b)),
+          "s2_grouped_linear_workspace_bytes")
+    return b.value
+
+
+def _workspace(workspace, size, device):
+    """(workspace or None, bytes): the caller's, or `size()` bytes made here."""
+    import torch
+    if workspace is not None:
+        return workspace, workspace.numel() * workspace.element_size()
+    size = size()
+    return (torch.empty(size, dtype=torch.uint8, device=device) if size else None), size
 
 
 def linear(x, weight, bias=None, activation=ACT_NONE, residual=None, out=None, out_dtype=None,
@@ -777,41 +797,38 @@ def linear(x, weight, bias=None, activation=ACT_NONE, residual=None, out=None, o
     n, k = weight.shape
     out = _matmul_views(x, n, k, weight, residual, out, out_dtype)
     _vector(bias, n, "bias")
-    m, xd = x.shape[0], _dtype_code(x)
+    m, xd, yd = x.shape[0], _dtype_code(x), _dtype_code(out)
     _on_current_device(x, weight, bias, residual, out, workspace)
-    size = 0
-    if workspace is None:
-        size = linear_workspace(m, n, k, xd)
-        if size:
-            workspace = torch.empty(size, dtype=torch.uint8, device=x.device)
-    else:
-        size = workspace.numel() * workspace.element_size()
+    workspace, size = _workspace(workspace, lambda: linear_workspace(m, n, k, xd, yd), x.device)
     check(lib().s2_linear(_ptr(x), xd, x.stride(0), m, _ptr(weight), _dtype_code(weight),
                           _ptr(bias), n, k, activation, _ptr(residual),
-                          residual.stride(0) if residual is not None else 0, _ptr(out),
-                          _dtype_code(out), out.stride(0), _ptr(workspace), size,
-                          _stream(stream)), "s2_linear")
+                          residual.stride(0) if residual is not None else 0, _ptr(out), yd,
+                          out.stride(0), _ptr(workspace), size, _stream(stream)), "s2_linear")
     return out
 
 
 def grouped_linear(x, offsets, weight, bias=None, activation=ACT_NONE, residual=None, out=None,
-                   out_dtype=None, stream=None):
+                   out_dtype=None, workspace=None, stream=None):
     """s2_grouped_linear: linear over the row groups offsets[g] ..
     offsets[g + 1] - 1 (int32 on the device) with weight [groups, n, k] and
     bias [groups, n].  Rows in no group are left as they are in out (undefined
-    in one that this call makes).  Returns out [m, n]."""
+    in one that this call makes).  workspace: grouped_linear_workspace(...)
+    bytes, allocated on the current stream if None.  Returns out [m, n]."""
     import torch
     groups, n, k = weight.shape
     out = _matmul_views(x, n, k, weight, residual, out, out_dtype)
     if offsets.dtype != torch.int32 or offsets.numel() != groups + 1 or not offsets.is_contiguous():
         raise ValueError(f"offsets must be {groups + 1} contiguous int32 values")
     _vector(bias, groups * n, "bias")
-    _on_current_device(x, offsets, weight, bias, residual, out)
-    check(lib().s2_grouped_linear(_ptr(x), _dtype_code(x), x.stride(0), x.shape[0], _ptr(offsets),
-                                  groups, _ptr(weight), _dtype_code(weight), _ptr(bias), n, k,
-                                  activation, _ptr(residual),
-                                  residual.stride(0) if residual is not None else 0, _ptr(out),
-                                  _dtype_code(out), out.stride(0), _stream(stream)),
+    m, xd, yd = x.shape[0], _dtype_code(x), _dtype_code(out)
+    _on_current_device(x, offsets, weight, bias, residual, out, workspace)
+    workspace, size = _workspace(
+        workspace, lambda: grouped_linear_workspace(m, groups, n, k, xd, yd), x.device)
+    check(lib().s2_grouped_linear(_ptr(x), xd, x.stride(0), m, _ptr(offsets), groups, _ptr(weight),
+                                  _dtype_code(weight), _ptr(bias), n, k, activation,
+                                  _ptr(residual),
+                                  residual.stride(0) if residual is not None else 0, _ptr(out), yd,
+                                  out.stride(0), _ptr(workspace), size, _stream(stream)),
           "s2_grouped_linear")
     return out
 

@@ -1337,12 +1337,37 @@ static int matmul_args_ok(const s2::MatmulArgs& a, bool any_rows) {
     return S2_OK;
 }
 
-int s2_linear_workspace_bytes(int m, int n, int k, s2_dtype x_dtype, size_t* bytes) {
+static int matmul_workspace(int m, const int* offsets, int groups, int n, int k, s2_dtype x_dtype,
+                            s2_dtype y_dtype, size_t* bytes) {
     if (!bytes) return fail(S2_ERR_INVALID, "null bytes");
-    if (m < 0 || n <= 0 || k <= 0 || !dtype_ok(x_dtype))
-        return fail(S2_ERR_INVALID, "invalid linear shape");
-    *bytes = s2::matmul_workspace(m, n, k, (int)x_dtype);
+    if (m < 0 || groups < 0 || n <= 0 || k <= 0) return fail(S2_ERR_INVALID, "invalid linear shape");
+    if (!dtype_ok(x_dtype) || !dtype_ok(y_dtype)) return fail(S2_ERR_INVALID, "unsupported dtype");
+    *bytes = 0;
+    if (m == 0 || groups == 0) return S2_OK;
+    s2::MatmulArgs a{};
+    a.x_kind = (int)x_dtype;
+    a.x_stride = k;
+    a.m = m;
+    a.offsets = offsets;
+    a.groups = groups;
+    a.w_kind = x_dtype == S2_DTYPE_F16 ? S2_DTYPE_F16 : S2_DTYPE_BF16;
+    a.n = n;
+    a.k = k;
+    a.y_kind = (int)y_dtype;
+    a.y_stride = n;
+    *bytes = s2::plan_matmul(a, (size_t)1 << 62).bytes();
     return S2_OK;
+}
+
+int s2_linear_workspace_bytes(int m, int n, int k, s2_dtype x_dtype, s2_dtype y_dtype,
+                              size_t* bytes) {
+    return matmul_workspace(m, nullptr, 1, n, k, x_dtype, y_dtype, bytes);
+}
+
+int s2_grouped_linear_workspace_bytes(int m, int groups, int n, int k, s2_dtype x_dtype,
+                                      s2_dtype y_dtype, size_t* bytes) {
+    static const int some = 0;   // offsets that only say that there are some
+    return matmul_workspace(m, &some, groups, n, k, x_dtype, y_dtype, bytes);
 }
 
 int s2_linear(const void* x, s2_dtype x_dtype, long x_stride, int m, const void* weight,
@@ -1350,7 +1375,7 @@ int s2_linear(const void* x, s2_dtype x_dtype, long x_stride, int m, const void*
               const void* residual, long residual_stride, void* y, s2_dtype y_dtype,
               long y_stride, void* workspace, size_t workspace_bytes, s2_stream_t stream) {
     const s2::MatmulArgs a{x, (int)x_dtype, x_stride, m, nullptr, 1, weight, (int)w_dtype, bias, n, k,
-                           activation, residual, residual_stride, y, (int)y_dtype, y_stride};
+                           activation, residual, residual_stride, y, (int)y_dtype, y_stride, 1, 0};
     const int ret = matmul_args_ok(a, m > 0);
     if (ret != S2_OK) return ret;
     if (workspace && !aligned(workspace, 16))
@@ -1362,15 +1387,18 @@ int s2_linear(const void* x, s2_dtype x_dtype, long x_stride, int m, const void*
 int s2_grouped_linear(const void* x, s2_dtype x_dtype, long x_stride, int m, const int* offsets,
                       int groups, const void* weight, s2_dtype w_dtype, const float* bias, int n,
                       int k, int activation, const void* residual, long residual_stride, void* y,
-                      s2_dtype y_dtype, long y_stride, s2_stream_t stream) {
+                      s2_dtype y_dtype, long y_stride, void* workspace, size_t workspace_bytes,
+                      s2_stream_t stream) {
     const s2::MatmulArgs a{x, (int)x_dtype, x_stride, m, offsets, groups, weight, (int)w_dtype, bias,
-                           n, k, activation, residual, residual_stride, y, (int)y_dtype, y_stride};
+                           n, k, activation, residual, residual_stride, y, (int)y_dtype, y_stride, 1, 0};
     if (groups < 0) return fail(S2_ERR_INVALID, "groups must be >= 0");
     const int ret = matmul_args_ok(a, m > 0 && groups > 0);
     if (ret != S2_OK) return ret;
     if (m == 0 || groups == 0) return S2_OK;
     if (!offsets) return fail(S2_ERR_INVALID, "null offsets");
-    S2_HIP(s2::launch_matmul(a, nullptr, 0, (hipStream_t)stream));
+    if (workspace && !aligned(workspace, 16))
+        return fail(S2_ERR_INVALID, "workspace must be 16-byte aligned");
+    S2_HIP(s2::launch_matmul(a, workspace, workspace ? workspace_bytes : 0, (hipStream_t)stream));
     return S2_OK;
 }
 

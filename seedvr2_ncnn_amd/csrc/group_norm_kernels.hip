@@ -4,13 +4,14 @@
 // the channels of a group.
 //
 // Bound by memory: x is read for the statistics and again for the result, which
-// only caches can make cheaper than two passes.
+// only caches can make cheaper than two passes; groups of few values are held in
+// registers between the two.
 //
 // Statistics.  A thread sums x - K and (x - K)^2 of its channels over its pixels,
 // K being its own first value of each channel: no cancellation where a mean is
 // many deviations large, and one outlying K spoils a single thread's part at
 // most.  Parts meet as (mean, sum of squared deviations) by the parallel variance
-// formula (Chan, Golub, LeVeque), in double.  Every order of summation is fixed.
+// formula (Chan, Golub, LeVeque).  Every order of summation is fixed.
 #include "group_norm_kernels.h"
 
 #include <algorithm>
@@ -22,12 +23,7 @@ namespace s2 {
 
 namespace {
 
-constexpr int kThreads = 256;
 constexpr int kMaxChannels = 4096;
-
-// Frames whose groups hold at most this many values take one launch, a
-// workgroup per frame and group.
-constexpr long kSmallGroup = 16384;
 
 template <int KIND>
 struct Elem;
@@ -77,129 +73,157 @@ __device__ __forceinline__ void store_v(void* base, long idx, const float (&v)[V
     }
 }
 
-__device__ __forceinline__ double wave_sum(double v) {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
+// Sum over aligned runs of `lanes` lanes, a power of two.
+__device__ __forceinline__ float lanes_sum(float v, int lanes) {
+    for (int o = 1; o < lanes; o <<= 1) v += __shfl_xor(v, o);
     return v;
 }
 
-// A chunk's (mean, sum of squared deviations) of every group:
-// parts[frame][chunk][group].
+// Lanes that share a group's sums: a power of two, at most a wave, that lets all the
+// groups have theirs at once where there are enough.
+__device__ __forceinline__ int lanes_per_group(int groups, int threads) {
+    int l = 64;
+    while (l > 1 && l * groups > threads) l >>= 1;
+    return l;
+}
+
+// The division of a chunk's pixels and channels among the threads: `seg` vectors of V
+// channels side by side, `rows` pixels at once.  More vectors than threads: sweeps of
+// one pixel row each.
+struct Split {
+    int cv, seg, rows;
+    __device__ Split(int channels, int v, int threads) {
+        cv = channels / v;
+        seg = min(cv, threads);
+        rows = cv > threads ? 1 : threads / seg;
+    }
+};
+
+constexpr int kThreads = 512;
+
+// A chunk's (mean, sum of squared deviations) of every group: parts[frame][group][chunk].
 template <int XK, int V>
 __global__ __launch_bounds__(kThreads) void group_norm_stats_kernel(GroupNormArgs p, int chunk,
                                                                    float2* __restrict__ parts) {
     typedef typename Elem<XK>::T T;
-    __shared__ float2 rows_lds[kThreads * V];
-    __shared__ float2 chan_lds[kMaxChannels];
+    constexpr int ENTRIES = kThreads * V > kMaxChannels ? kThreads * V : kMaxChannels;
+    __shared__ float2 entry[ENTRIES];   // [row][channel]
     const int tid = threadIdx.x;
     const int f = blockIdx.y;
     const long p0 = (long)blockIdx.x * chunk;
     const int np = (int)min((long)chunk, p.pixels - p0);
-    const int cv = p.channels / V;
-    const T* x = (const T*)p.x + f * p.x_frame + p0 * p.x_pixel;
-    for (int c0 = 0; c0 < cv; c0 += kThreads) {
-        const int seg = min(cv - c0, kThreads);   // vectors of channels in this sweep
-        const int rows = kThreads / seg;
-        const int row = tid / seg;
-        const int col = tid - row * seg;
-        if (row < rows && row < np) {
-            const T* q = x + (long)row * p.x_pixel + (long)(c0 + col) * V;
-            const long step = (long)rows * p.x_pixel;
-            const int count = (np - row + rows - 1) / rows;
-            float first[V], s1[V], s2[V], v[V];
-            load_v<V>(q, first);
+    const Split sp(p.channels, V, kThreads);
+    const int row = tid / sp.seg;
+    const int col = tid - row * sp.seg;
+    const int base = np / sp.rows, extra = np - base * sp.rows;   // pixels of a row
+    const T* x = (const T*)p.x + f * p.x_frame + p0 * p.x_pixel + (long)row * p.x_pixel;
+    const int count = row < sp.rows ? base + (row < extra) : 0;
+    const long step = (long)sp.rows * p.x_pixel;
+    for (int c = col; c < sp.cv && count > 0; c += sp.seg) {
+        const T* q = x + (long)c * V;
+        float first[V], s1[V], s2[V];
+        load_v<V>(q, first);
 #pragma unroll
-            for (int i = 0; i < V; ++i) s1[i] = s2[i] = 0.f;
-#pragma unroll 4
-            for (int j = 1; j < count; ++j) {
-                load_v<V>(q + j * step, v);
+        for (int i = 0; i < V; ++i) s1[i] = s2[i] = 0.f;
+#pragma unroll 8
+        for (int j = 1; j < count; ++j) {
+            float v[V];
+            load_v<V>(q + j * step, v);
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    const float d = v[i] - first[i];
-                    s1[i] += d;
-                    s2[i] = fmaf(d, d, s2[i]);
+            for (int i = 0; i < V; ++i) {
+                const float d = v[i] - first[i];
+                s1[i] += d;
+                s2[i] = fmaf(d, d, s2[i]);
+            }
+        }
+        const float inv = 1.f / (float)count;
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            entry[row * p.channels + c * V + i] =
+                make_float2(fmaf(s1[i], inv, first[i]), fmaxf(fmaf(-s1[i] * inv, s1[i], s2[i]), 0.f));
+    }
+    __syncthreads();
+    const int each = p.channels / p.groups;
+    const int used = min(sp.rows, np);
+    const int lanes = lanes_per_group(p.groups, kThreads);
+    const int lane = tid & (lanes - 1);
+    const float per_value = 1.f / ((float)np * (float)each);
+    for (int g0 = 0; g0 < p.groups; g0 += kThreads / lanes) {   // the same count in every thread
+        const int g = g0 + tid / lanes;
+        const float2* e = entry + g * each;
+        const float ref = g < p.groups ? e[0].x : 0.f;
+        float sum = 0.f;
+        if (g < p.groups)
+            for (int r = 0; r < used; ++r) {
+                const float n = (float)(base + (r < extra));
+                for (int c = lane; c < each; c += lanes) sum = fmaf(n, e[r * p.channels + c].x - ref, sum);
+            }
+        const float mean = fmaf(lanes_sum(sum, lanes), per_value, ref);
+        float m2 = 0.f;
+        if (g < p.groups)
+            for (int r = 0; r < used; ++r) {
+                const float n = (float)(base + (r < extra));
+                for (int c = lane; c < each; c += lanes) {
+                    const float2 v = e[r * p.channels + c];
+                    const float d = v.x - mean;
+                    m2 += fmaf(n * d, d, v.y);
                 }
             }
-            const float inv = 1.f / (float)count;
-#pragma unroll
-            for (int i = 0; i < V; ++i)
-                rows_lds[(row * seg + col) * V + i] =
-                    make_float2(first[i] + s1[i] * inv, fmaxf(s2[i] - s1[i] * s1[i] * inv, 0.f));
-        }
-        __syncthreads();
-        // the rows of each channel
-        const int used = min(rows, np);
-        for (int c = tid; c < seg * V; c += kThreads) {
-            double sum = 0., m2 = 0.;
-            for (int r = 0; r < used; ++r)
-                sum += (double)((np - r + rows - 1) / rows) * rows_lds[r * seg * V + c].x;
-            const double mean = sum / np;
-            for (int r = 0; r < used; ++r) {
-                const float2 e = rows_lds[r * seg * V + c];
-                const double d = e.x - mean;
-                m2 += e.y + (double)((np - r + rows - 1) / rows) * d * d;
-            }
-            chan_lds[c0 * V + c] = make_float2((float)mean, (float)m2);
-        }
-        __syncthreads();
-    }
-    // the channels of each group
-    const int each = p.channels / p.groups;
-    const int lane = tid & 63;
-    for (int g = tid >> 6; g < p.groups; g += kThreads / 64) {
-        double sum = 0.;
-        for (int c = lane; c < each; c += 64) sum += chan_lds[g * each + c].x;
-        const double mean = wave_sum(sum) / each;
-        double m2 = 0.;
-        for (int c = lane; c < each; c += 64) {
-            const float2 e = chan_lds[g * each + c];
-            const double d = e.x - mean;
-            m2 += e.y + np * d * d;
-        }
-        m2 = wave_sum(m2);
-        if (lane == 0)
-            parts[((long)f * gridDim.x + blockIdx.x) * p.groups + g] = make_float2((float)mean, (float)m2);
+        m2 = lanes_sum(m2, lanes);
+        if (g < p.groups && lane == 0)
+            parts[((long)f * p.groups + g) * gridDim.x + blockIdx.x] = make_float2(mean, m2);
     }
 }
 
 template <int XK, int YK, int V>
-__global__ __launch_bounds__(kThreads) void group_norm_apply_kernel(GroupNormArgs p, int chunk,
+__global__ __launch_bounds__(kThreads) void group_norm_apply_kernel(GroupNormArgs p, int part_chunk,
+                                                                   int chunks, int chunk,
                                                                    const float2* __restrict__ parts) {
     typedef typename Elem<XK>::T T;
     __shared__ float2 stat[kMaxChannels];   // (mean, rstd) of each group
     const int tid = threadIdx.x;
     const int f = blockIdx.y;
-    const int chunks = gridDim.x;
     const int each = p.channels / p.groups;
-    const int lane = tid & 63;
-    const float2* fp = parts + (long)f * chunks * p.groups;
-    for (int g = tid >> 6; g < p.groups; g += kThreads / 64) {
-        double sum = 0.;
-        for (int c = lane; c < chunks; c += 64)
-            sum += (double)min((long)chunk, p.pixels - (long)c * chunk) * fp[(long)c * p.groups + g].x;
-        const double mean = wave_sum(sum) / p.pixels;
-        double m2 = 0.;
-        for (int c = lane; c < chunks; c += 64) {
-            const float2 e = fp[(long)c * p.groups + g];
-            const double d = e.x - mean;
-            m2 += e.y + (double)min((long)chunk, p.pixels - (long)c * chunk) * each * d * d;
+    const int lanes = lanes_per_group(p.groups, kThreads);
+    const int lane = tid & (lanes - 1);
+    for (int g0 = 0; g0 < p.groups; g0 += kThreads / lanes) {
+        const int g = g0 + tid / lanes;
+        const float2* e = parts + ((long)f * p.groups + min(g, p.groups - 1)) * chunks;
+        // deviations from the first part's mean: as far from it as the parts are from
+        // one another
+        const float ref = e[0].x;
+        float sum = 0.f, sq = 0.f, m2 = 0.f;
+#pragma unroll 4
+        for (int c = lane; c < chunks; c += lanes) {
+            const float2 v = e[c];
+            const float n = (float)min((long)part_chunk, p.pixels - (long)c * part_chunk);
+            const float d = v.x - ref;
+            sum = fmaf(n, d, sum);
+            sq = fmaf(n * d, d, sq);
+            m2 += v.y;
         }
-        m2 = wave_sum(m2);
-        if (lane == 0)
-            stat[g] = make_float2((float)mean,
-                                  (float)(1. / sqrt(m2 / ((double)p.pixels * each) + (double)p.eps)));
+        sum = lanes_sum(sum, lanes);
+        sq = lanes_sum(sq, lanes);
+        m2 = lanes_sum(m2, lanes);
+        if (g < p.groups && lane == 0) {
+            const float mean = sum / (float)p.pixels;
+            const float var = (fmaxf(fmaf(-mean, sum, sq), 0.f) * (float)each + m2) /
+                              ((float)p.pixels * (float)each);
+            // an infinity or NaN in any part makes m2 NaN
+            stat[g] = make_float2(ref + mean, 1.f / sqrtf(var + p.eps));
+        }
     }
     __syncthreads();
     const long p0 = (long)blockIdx.x * chunk;
     const int np = (int)min((long)chunk, p.pixels - p0);
-    const int cv = p.channels / V;
+    const Split sp(p.channels, V, kThreads);
+    const int row = tid / sp.seg;
+    const int col = tid - row * sp.seg;
+    if (row >= sp.rows) return;
     const T* x = (const T*)p.x + f * p.x_frame + p0 * p.x_pixel;
-    for (int c0 = 0; c0 < cv; c0 += kThreads) {
-        const int seg = min(cv - c0, kThreads);
-        const int rows = kThreads / seg;
-        const int row = tid / seg;
-        const int c = (c0 + tid - row * seg) * V;
-        if (row >= rows) continue;
+    const long y0 = f * p.y_frame + p0 * p.y_pixel;
+    for (int cc = col; cc < sp.cv; cc += sp.seg) {
+        const int c = cc * V;
         float mean[V], scale[V], shift[V];
 #pragma unroll
         for (int i = 0; i < V; ++i) {
@@ -208,47 +232,141 @@ __global__ __launch_bounds__(kThreads) void group_norm_apply_kernel(GroupNormArg
             scale[i] = s.y * (p.gamma ? p.gamma[c + i] : 1.f);
             shift[i] = p.beta ? p.beta[c + i] : 0.f;
         }
-#pragma unroll 4
-        for (int j = row; j < np; j += rows) {
-            float v[V];
-            load_v<V>(x + (long)j * p.x_pixel + c, v);
+        constexpr int U = 4;   // pixels in flight
+        for (int j = row; j < np; j += U * sp.rows) {
+            float v[U][V];
 #pragma unroll
-            for (int i = 0; i < V; ++i) v[i] = activate(fmaf(v[i] - mean[i], scale[i], shift[i]), p.act);
-            store_v<V, YK>(p.y, f * p.y_frame + (p0 + j) * p.y_pixel + c, v);
+            for (int u = 0; u < U; ++u)
+                if (j + u * sp.rows < np) load_v<V>(x + (long)(j + u * sp.rows) * p.x_pixel + c, v[u]);
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (j + u * sp.rows < np) {
+#pragma unroll
+                    for (int i = 0; i < V; ++i)
+                        v[u][i] = activate(fmaf(v[u][i] - mean[i], scale[i], shift[i]), p.act);
+                    store_v<V, YK>(p.y, y0 + (long)(j + u * sp.rows) * p.y_pixel + c, v[u]);
+                }
         }
     }
 }
 
-// How a frame's pixels are cut: enough workgroups to fill the chip, each with
-// enough pixels to be worth its reductions.
-int chunk_pixels(int frames, int pixels, int channels) {
-    const long want = std::max<long>(1, 1024 / frames);                  // chunks of a frame
-    const long least = std::max<long>(1, 16384 / channels);              // pixels of a chunk
-    return (int)std::min<long>(pixels, std::max(least, (pixels + want - 1) / want));
+// Few values: a workgroup holds a frame's group in registers, one launch in all.  The
+// mean first, then the deviations from it.
+constexpr int kSmallThreads = 256;
+constexpr int kSmallVectors = 8;   // of a thread
+
+__device__ __forceinline__ float block_sum(float v, float* lds) {
+    v = lanes_sum(v, 64);
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = 0.f;
+#pragma unroll
+    for (int i = 0; i < kSmallThreads / 64; ++i) v += lds[i];
+    return v;
 }
 
 template <int XK, int YK, int V>
-hipError_t run(const GroupNormArgs& p, float2* parts, hipStream_t stream) {
-    const int chunk = chunk_pixels(p.frames, p.pixels, p.channels);
-    const dim3 grid((unsigned)((p.pixels + (long)chunk - 1) / chunk), (unsigned)p.frames);
-    group_norm_stats_kernel<XK, V><<<grid, kThreads, 0, stream>>>(p, chunk, parts);
-    group_norm_apply_kernel<XK, YK, V><<<grid, kThreads, 0, stream>>>(p, chunk, parts);
-    return hipGetLastError();
+__global__ __launch_bounds__(kSmallThreads) void group_norm_small_kernel(GroupNormArgs p) {
+    typedef typename Elem<XK>::T T;
+    __shared__ float lds[2][kSmallThreads / 64];
+    const int f = blockIdx.y, g = blockIdx.x;
+    const int each = p.channels / p.groups;
+    const int ev = each / V;   // vectors of a pixel
+    const int all = p.pixels * ev;
+    const T* x = (const T*)p.x + f * p.x_frame + (long)g * each;
+    float v[kSmallVectors][V];
+    int pix[kSmallVectors], ch[kSmallVectors];
+#pragma unroll
+    for (int u = 0; u < kSmallVectors; ++u) {
+        const int i = threadIdx.x + u * kSmallThreads;
+        pix[u] = i / ev;
+        ch[u] = (i - pix[u] * ev) * V;
+        if (i < all) load_v<V>(x + pix[u] * p.x_pixel + ch[u], v[u]);
+    }
+    // deviations from the first value: no digits are lost to a large mean
+    const float ref = to_f32(*x);
+    float sum = 0.f;
+#pragma unroll
+    for (int u = 0; u < kSmallVectors; ++u)
+        if (threadIdx.x + u * kSmallThreads < all)
+#pragma unroll
+            for (int i = 0; i < V; ++i) sum += v[u][i] - ref;
+    const float count = (float)all * V;
+    const float mean = ref + block_sum(sum, lds[0]) / count;
+    float m2 = 0.f;
+#pragma unroll
+    for (int u = 0; u < kSmallVectors; ++u)
+        if (threadIdx.x + u * kSmallThreads < all)
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const float d = v[u][i] - mean;
+                m2 = fmaf(d, d, m2);
+            }
+    const float rstd = 1.f / sqrtf(block_sum(m2, lds[1]) / count + p.eps);
+#pragma unroll
+    for (int u = 0; u < kSmallVectors; ++u)
+        if (threadIdx.x + u * kSmallThreads < all) {
+            const int c = g * each + ch[u];
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                v[u][i] = activate(fmaf(v[u][i] - mean, rstd * (p.gamma ? p.gamma[c + i] : 1.f),
+                                        p.beta ? p.beta[c + i] : 0.f),
+                                   p.act);
+            store_v<V, YK>(p.y, f * p.y_frame + pix[u] * p.y_pixel + c, v[u]);
+        }
 }
 
-// V consecutive channels are whole 16-byte pieces (8 bytes: four 16-bit ones)
-// of every row of a view
+// V channels are whole 16-byte pieces (8 bytes: four 16-bit ones) of every row of a view
 bool fits(const void* base, int kind, long frame, long pixel, int v) {
     const int bytes = std::min(16, v * (kind ? 2 : 4));
     return (uintptr_t)base % bytes == 0 && frame % v == 0 && pixel % v == 0;
 }
 
+bool fits(const GroupNormArgs& p, int width, int v) {
+    return width % v == 0 && fits(p.x, p.x_kind, p.x_frame, p.x_pixel, v) &&
+           fits(p.y, p.y_kind, p.y_frame, p.y_pixel, v);
+}
+
+// How a frame's pixels are cut: into at most 256 chunks, whose parts every workgroup of
+// the second kernel reads, and about 512 workgroups in all.
+int chunk_pixels(int frames, int pixels, int channels) {
+    const long want = std::min<long>(256, std::max<long>(1, 512 / frames));   // chunks of a frame
+    const long least = std::max<long>(1, 8192 / channels);                    // pixels of a chunk
+    return (int)std::min<long>(pixels, std::max(least, (pixels + want - 1) / want));
+}
+
+long chunks_of(int pixels, int chunk) { return ((long)pixels + chunk - 1) / chunk; }
+
+template <int XK, int YK, int V>
+hipError_t run(const GroupNormArgs& p, float2* parts, hipStream_t stream) {
+    const int part = chunk_pixels(p.frames, p.pixels, p.channels);
+    const int chunks = (int)chunks_of(p.pixels, part);
+    group_norm_stats_kernel<XK, V>
+        <<<dim3((unsigned)chunks, (unsigned)p.frames), kThreads, 0, stream>>>(p, part, parts);
+    const int chunk = part;
+    group_norm_apply_kernel<XK, YK, V>
+        <<<dim3((unsigned)chunks_of(p.pixels, chunk), (unsigned)p.frames), kThreads, 0, stream>>>(
+            p, part, chunks, chunk, parts);
+    return hipGetLastError();
+}
+
 template <int XK, int YK>
 hipError_t pick(const GroupNormArgs& p, float2* parts, hipStream_t stream) {
-    for (int v : {8, 4})
-        if (p.channels % v == 0 && fits(p.x, XK, p.x_frame, p.x_pixel, v) &&
-            fits(p.y, YK, p.y_frame, p.y_pixel, v))
-            return v == 8 ? run<XK, YK, 8>(p, parts, stream) : run<XK, YK, 4>(p, parts, stream);
+    const int each = p.channels / p.groups;
+    for (int v : {8, 4, 1}) {
+        if (v > 1 && !fits(p, each, v)) continue;
+        if ((long)p.pixels * (each / v) > kSmallThreads * kSmallVectors) break;
+        const dim3 grid((unsigned)p.groups, (unsigned)p.frames);
+        if (v == 8)
+            group_norm_small_kernel<XK, YK, 8><<<grid, kSmallThreads, 0, stream>>>(p);
+        else if (v == 4)
+            group_norm_small_kernel<XK, YK, 4><<<grid, kSmallThreads, 0, stream>>>(p);
+        else
+            group_norm_small_kernel<XK, YK, 1><<<grid, kSmallThreads, 0, stream>>>(p);
+        return hipGetLastError();
+    }
+    if (fits(p, p.channels, 8)) return run<XK, YK, 8>(p, parts, stream);
+    if (fits(p, p.channels, 4)) return run<XK, YK, 4>(p, parts, stream);
     return run<XK, YK, 1>(p, parts, stream);
 }
 
@@ -264,11 +382,14 @@ hipError_t pick_y(const GroupNormArgs& p, float2* parts, hipStream_t stream) {
 size_t group_norm_workspace(int frames, int pixels, int channels, int groups) {
     if (frames <= 0 || pixels <= 0) return 0;
     const int chunk = chunk_pixels(frames, pixels, channels);
-    return (size_t)frames * (size_t)((pixels + (long)chunk - 1) / chunk) * groups * sizeof(float2);
+    return (size_t)frames * (size_t)chunks_of(pixels, chunk) * groups * sizeof(float2);
 }
 
-hipError_t launch_group_norm(const GroupNormArgs& p, void* workspace, hipStream_t stream) {
-    if (p.frames <= 0 || p.pixels <= 0) return hipSuccess;
+hipError_t launch_group_norm(const GroupNormArgs& args, void* workspace, hipStream_t stream) {
+    if (args.frames <= 0 || args.pixels <= 0) return hipSuccess;
+    GroupNormArgs p = args;
+    if (p.frames == 1) p.x_frame = p.y_frame = 0;   // strides of single ones say nothing
+    if (p.pixels == 1) p.x_pixel = p.y_pixel = 0;
     return p.x_kind == 1   ? pick_y<1>(p, (float2*)workspace, stream)
            : p.x_kind == 2 ? pick_y<2>(p, (float2*)workspace, stream)
                            : pick_y<0>(p, (float2*)workspace, stream);

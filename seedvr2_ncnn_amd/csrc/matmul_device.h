@@ -1,0 +1,226 @@
+// Device side of the linear and grouped linear kernels: row tiles of ragged groups,
+// the MFMA step, fp32 rows as bf16 terms, and the epilogue.
+#pragma once
+
+#include <type_traits>
+
+#include "activations.h"
+#include "matmul_kernels.h"
+#include "s2_device.h"
+
+namespace s2 {
+
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+// T: 1 bf16, 2 fp16
+template <int T>
+__device__ __forceinline__ f32x4 mfma(uint4 a, uint4 b, f32x4 c) {
+    if constexpr (T == 1)
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(a), as_bf16x8(b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
+                                                      __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+// Rows [row0, end) of group `group` that tile t of tm rows starts at; end == row0
+// when there is no such tile.
+struct RowTile {
+    int row0, end, group;
+};
+
+__device__ __forceinline__ RowTile row_tile(const MatmulArgs& a, int t, int tm) {
+    if (!a.offsets) return RowTile{t * tm, a.m, 0};
+    // every wave counts the groups' tiles, 64 groups at a time; offsets are kept
+    // to [0, m], whatever they hold
+    const int lane = threadIdx.x & 63;
+    for (int g0 = 0; g0 < a.groups; g0 += 64) {
+        const int g = g0 + lane;
+        int start = 0, end = 0;
+        if (g < a.groups) {
+            start = max(a.offsets[g], 0);
+            end = min(a.offsets[g + 1], a.m);
+        }
+        const int tiles = end > start ? (end - start + tm - 1) / tm : 0;
+        int upto = tiles;   // tiles of the groups up to this one
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int other = __shfl_up(upto, o);
+            if (lane >= o) upto += other;
+        }
+        const uint64_t past = __ballot(upto > t);
+        if (past) {
+            const int l = __ffsll((unsigned long long)past) - 1;
+            const int first = __shfl(start, l) + (t - __shfl(upto - tiles, l)) * tm;
+            return RowTile{__builtin_amdgcn_readfirstlane(first),
+                           __builtin_amdgcn_readfirstlane(__shfl(end, l)),
+                           __builtin_amdgcn_readfirstlane(g0 + l)};
+        }
+        t -= __builtin_amdgcn_readfirstlane(__shfl(upto, 63));
+    }
+    return RowTile{0, 0, 0};
+}
+
+__device__ __forceinline__ float load1(const void* p, long idx, int kind) {
+    if (kind == 1) return bf16_to_f32(((const uint16_t*)p)[idx]);
+    if (kind == 2) return (float)((const _Float16*)p)[idx];
+    return ((const float*)p)[idx];
+}
+
+__device__ __forceinline__ void store1(void* p, long idx, float v, int kind) {
+    if (kind == 1)
+        ((uint16_t*)p)[idx] = f32_to_bf16(v);
+    else if (kind == 2)
+        ((_Float16*)p)[idx] = f32_to_f16(v);
+    else
+        ((float*)p)[idx] = v;
+}
+
+template <int ACT>
+__device__ __forceinline__ float act_of(float v) {
+    return activate(v, ACT);
+}
+
+// Epilogue of a wave's tile of NI x 16 rows and 64 columns: accumulator [i][j][r] is
+// row row_w + 16 i + 4 g + r of the block tile's `rows`, column col + j.  WHOLE: pieces
+// of four; else single elements.
+template <int YK, int NI, bool WHOLE>
+__device__ __forceinline__ void epilogue(const MatmulArgs& a, const RowTile& rt, int rows, int row_w,
+                                         int col, const f32x4 (&acc)[NI][4]) {
+    const int g = (threadIdx.x & 63) >> 4;
+    if (col >= a.n) return;
+    f32x4 b = {0.f, 0.f, 0.f, 0.f};
+    if (a.bias) {
+        const float* bias = a.bias + (long)rt.group * a.n + col;
+        if (WHOLE) {
+            b = *reinterpret_cast<const f32x4*>(bias);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (col + j < a.n) b[j] = bias[j];
+        }
+    }
+    auto emit = [&](auto act_tag) {
+        constexpr int ACT = decltype(act_tag)::value;
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+            const int r0 = row_w + 16 * i + 4 * g;
+            const long row = rt.row0 + r0;
+            f32x4 res[4];
+            if (a.res) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    if (r0 + r >= rows) continue;
+                    const long at = (row + r) * a.res_stride + col;
+                    if (!WHOLE) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            if (col + j < a.n) res[r][j] = load1(a.res, at + j, YK);
+                    } else if (YK == 0) {
+                        res[r] = *reinterpret_cast<const f32x4*>((const float*)a.res + at);
+                    } else {
+                        const uint2 q = *reinterpret_cast<const uint2*>((const uint16_t*)a.res + at);
+                        const uint32_t w[2] = {q.x, q.y};
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const uint16_t h = (uint16_t)(w[j >> 1] >> (16 * (j & 1)));
+                            res[r][j] = YK == 1 ? bf16_to_f32(h) : (float)__builtin_bit_cast(_Float16, h);
+                        }
+                    }
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                if (r0 + r >= rows) continue;
+                float v[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    v[j] = act_of<ACT>(acc[i][j][r] + b[j]);
+                    if (a.res) v[j] += res[r][j];
+                }
+                const long at = (row + r) * a.y_stride + col;
+                if (WHOLE) {
+                    store4(a.y, at, v[0], v[1], v[2], v[3], YK);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (col + j < a.n) store1(a.y, at + j, v[j], YK);
+                }
+            }
+        }
+    };
+    if (a.act == S2_ACT_NONE)
+        emit(std::integral_constant<int, S2_ACT_NONE>{});
+    else if (a.act == S2_ACT_GELU)
+        emit(std::integral_constant<int, S2_ACT_GELU>{});
+    else if (a.act == S2_ACT_SILU)
+        emit(std::integral_constant<int, S2_ACT_SILU>{});
+    else
+        emit(std::integral_constant<int, S2_ACT_GELU_TANH>{});
+}
+
+// fp32 as a sum of PL bf16 values: all but the last take the top 8 bits of what the
+// ones before leave, by truncation, which cannot overflow and leaves an exact rest; the
+// last rounds (two terms: to 2^-15 of x) or, of three, holds the rest exactly.  An
+// infinity stays in the first term, a NaN reaches the later ones.  v: pairs of
+// values, h[q]: their terms q packed.
+template <int PL>
+__device__ __forceinline__ void split2(float v0, float v1, uint32_t (&h)[PL]) {
+#pragma unroll
+    for (int q = 0; q + 1 < PL; ++q) {
+        const uint32_t b0 = __float_as_uint(v0) & 0xffff0000u, b1 = __float_as_uint(v1) & 0xffff0000u;
+        h[q] = (b0 >> 16) | b1;
+        v0 = fabsf(v0) == __builtin_inff() ? 0.f : v0 - __uint_as_float(b0);
+        v1 = fabsf(v1) == __builtin_inff() ? 0.f : v1 - __uint_as_float(b1);
+    }
+    h[PL - 1] = pack2_bf16_rne(v0, v1);
+}
+
+template <int PL>
+__device__ __forceinline__ void split8(const float (&v)[8], uint4 (&out)[PL]) {
+    uint32_t w[4][PL];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) split2<PL>(v[2 * e], v[2 * e + 1], w[e]);
+#pragma unroll
+    for (int q = 0; q < PL; ++q) out[q] = make_uint4(w[0][q], w[1][q], w[2][q], w[3][q]);
+}
+
+// Eight consecutive k of a row as an MFMA operand piece.  GRAN elements lie together
+// (8: 16 bytes of 16-bit elements, 4, or 1); FULL: all eight are before k.
+template <int GRAN, bool FULL>
+__device__ __forceinline__ uint4 piece16(const uint16_t* p, int left) {
+    if constexpr (GRAN == 8) {
+        if (FULL || left > 0) return *reinterpret_cast<const uint4*>(p);
+        return make_uint4(0, 0, 0, 0);
+    } else {
+        alignas(16) uint16_t h[8];
+#pragma unroll
+        for (int e = 0; e < 8; e += GRAN) {
+            if constexpr (GRAN == 4) {
+                uint2 q = make_uint2(0, 0);
+                if (FULL || left > e) q = *reinterpret_cast<const uint2*>(p + e);
+                *reinterpret_cast<uint2*>(h + e) = q;
+            } else {
+                h[e] = FULL || left > e ? p[e] : (uint16_t)0;
+            }
+        }
+        return pack8_bf16(h);
+    }
+}
+
+template <int GRAN, bool FULL>
+__device__ __forceinline__ void piece32(const float* p, int left, float (&v)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; e += 4) {
+        if constexpr (GRAN >= 4) {
+            f32x4 q = {0.f, 0.f, 0.f, 0.f};
+            if (FULL || left > e) q = *reinterpret_cast<const f32x4*>(p + e);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[e + i] = q[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[e + i] = FULL || left > e + i ? p[e + i] : 0.f;
+        }
+    }
+}
+
+}  // namespace s2

@@ -67,21 +67,23 @@ def linear(x, w, bias, act, residual, dtype):
 
 
 def group_norm(x, groups, gamma, beta, eps, act, dtype):
-    """A thread sums L values x - K and their squares, K one of them: the sum of
-    squares is off by (L + 3) U of itself, the mean by (L + 3) U of the mean
-    distance from K and, stored in fp32 three times, by 3 U of itself."""
+    """Means and sums of squares are of deviations from a value of the group, at most
+    `far`, the group's range, each.  A value passes through at most `steps` additions
+    in a row: those of its thread (`length`, or 64 where a thread holds them all), of
+    the parts of its workgroup that a lane adds (64 at most), of lanes (8) and of
+    chunks (32 of a lane in these shapes).  So the mean is off by steps U far and,
+    stored in fp32 three times, by 3 U of itself; the mean square by 2 steps U far^2
+    and by what the parts' means are off, 2 mean_err far + mean_err^2."""
     f, p, c = x.shape
     xd = x.double().reshape(f, p, groups, c // groups)
     mean = xd.mean(dim=(1, 3), keepdim=True)
     d = xd - mean
     var = (d * d).mean(dim=(1, 3), keepdim=True)
-    far = (xd.amax(dim=1, keepdim=True) - xd.amin(dim=1, keepdim=True)).amax(dim=3, keepdim=True)
-    length = max(16384 // c, -(-p // max(1, 1024 // f)), 1)
-    length = min(length, p)
-    mean_err = (length + 3) * U * far + 3 * U * mean.abs()
-    # the deviations' sum of squares, from sums about K (at most `far` away) and
-    # from means of parts that are off by mean_err each
-    var_err = 2 * (length + 3) * U * far ** 2 + 2 * mean_err * far + mean_err ** 2
+    far = xd.amax(dim=(1, 3), keepdim=True) - xd.amin(dim=(1, 3), keepdim=True)
+    length = min(max(16384 // c, -(-p // max(1, 1024 // f)), 1), p)
+    steps = length + 64 + 64 + 8 + 32
+    mean_err = steps * U * far + 3 * U * mean.abs()
+    var_err = 2 * steps * U * far ** 2 + 2 * mean_err * far + mean_err ** 2
     std = (var + eps).sqrt()
     hat = d / std
     hat_err = (mean_err + 2 * U * d.abs()) / std + hat.abs() * (0.5 * var_err / (var + eps) + 4 * U)

@@ -17,7 +17,7 @@ LINEAR = dict(x=P, x_dtype=BF16, x_stride=64, m=4, weight=P, w_dtype=BF16, bias=
               y_stride=32, workspace=None, workspace_bytes=0, stream=None)
 GROUPED = dict(x=P, x_dtype=BF16, x_stride=64, m=4, offsets=P, groups=2, weight=P, w_dtype=BF16,
                bias=P, n=32, k=64, activation=capi.ACT_NONE, residual=P, residual_stride=32, y=2 * P,
-               y_dtype=F32, y_stride=32, stream=None)
+               y_dtype=F32, y_stride=32, workspace=None, workspace_bytes=0, stream=None)
 
 
 def _call(name, base, **changes):
@@ -70,7 +70,8 @@ def test_linear_refuses(changes):
     assert capi.last_error()
 
 
-@pytest.mark.parametrize("changes", MATMUL + [dict(groups=-1), dict(offsets=None), dict(offsets=P + 2)],
+@pytest.mark.parametrize("changes", MATMUL + [dict(groups=-1), dict(offsets=None), dict(offsets=P + 2),
+                                              dict(workspace=P + 8, workspace_bytes=64)],
                          ids=str)
 def test_grouped_linear_refuses(changes):
     assert _call("s2_grouped_linear", GROUPED, **changes) == capi.S2_ERR_INVALID
@@ -85,7 +86,13 @@ def test_linear_of_nothing():
     for bad in ((-1, 8, 8), (1, 0, 8), (1, 8, 0)):
         with pytest.raises(capi.S2Error):
             capi.linear_workspace(*bad)
-    assert capi.lib().s2_linear_workspace_bytes(1, 1, 1, 0, None) == capi.S2_ERR_INVALID
+    assert capi.grouped_linear_workspace(0, 2, 8, 8) == capi.grouped_linear_workspace(9, 0, 8, 8) == 0
+    assert capi.grouped_linear_workspace(900, 2, 8, 8, F32) > 0   # fp32 rows are repacked
+    for bad in ((-1, 1, 8, 8), (1, -1, 8, 8), (1, 1, 0, 8), (1, 1, 8, 0), (1, 1, 8, 8, 3), (1, 1, 8, 8, 0, 3)):
+        with pytest.raises(capi.S2Error):
+            capi.grouped_linear_workspace(*bad)
+    assert capi.lib().s2_linear_workspace_bytes(1, 1, 1, 0, 0, None) == capi.S2_ERR_INVALID
+    assert capi.lib().s2_grouped_linear_workspace_bytes(1, 1, 1, 1, 0, 0, None) == capi.S2_ERR_INVALID
     assert capi.lib().s2_group_norm_workspace_bytes(1, 1, 1, 1, None) == capi.S2_ERR_INVALID
 
 
