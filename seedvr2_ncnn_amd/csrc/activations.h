@@ -3,6 +3,8 @@
 
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+
 #include "seedvr2_hip.h"
 
 namespace s2 {
@@ -47,6 +49,20 @@ __device__ __forceinline__ float activate(float x, int act) {
     if (act == S2_ACT_GELU) return gelu(x);
     if (act == S2_ACT_GELU_TANH) return gelu_tanh_f32(x);
     return x;
+}
+
+// f(std::integral_constant<int, act>): one branch around a loop, instead of branches
+// at each of its values, whose code a short kernel would spend its time fetching
+template <typename F>
+__device__ __forceinline__ void with_activation(int act, F&& f) {
+    if (act == S2_ACT_NONE)
+        f(std::integral_constant<int, S2_ACT_NONE>{});
+    else if (act == S2_ACT_GELU)
+        f(std::integral_constant<int, S2_ACT_GELU>{});
+    else if (act == S2_ACT_SILU)
+        f(std::integral_constant<int, S2_ACT_SILU>{});
+    else
+        f(std::integral_constant<int, S2_ACT_GELU_TANH>{});
 }
 
 }  // namespace s2

@@ -38,27 +38,39 @@ __device__ __forceinline__ float to_f32(float v) { return v; }
 __device__ __forceinline__ float to_f32(uint16_t v) { return bf16_to_f32(v); }
 __device__ __forceinline__ float to_f32(_Float16 v) { return (float)v; }
 
-// V consecutive elements as floats; V elements are aligned to min(16, their size) bytes
-template <int V, typename T>
-__device__ __forceinline__ void load_v(const T* p, float (&v)[V]) {
-    constexpr int B = V * (int)sizeof(T);
-    if constexpr (V == 1) {
-        v[0] = to_f32(*p);
-    } else {
-        alignas(16) T e[V];
-        if constexpr (B == 8) {
+// V consecutive elements as they lie in memory, aligned to min(16, their size) bytes
+template <typename T, int V>
+struct Raw {
+    alignas(V * sizeof(T) > 16 ? 16 : V * sizeof(T)) T e[V];
+    __device__ __forceinline__ void load(const T* p) {
+        constexpr int B = V * (int)sizeof(T);
+        if constexpr (V == 1) {
+            e[0] = *p;
+        } else if constexpr (B == 8) {
             *reinterpret_cast<uint2*>(e) = *reinterpret_cast<const uint2*>(p);
         } else {
 #pragma unroll
             for (int i = 0; i < B / 16; ++i)
                 reinterpret_cast<uint4*>(e)[i] = reinterpret_cast<const uint4*>(p)[i];
         }
+    }
+    __device__ __forceinline__ void get(float (&v)[V]) const {
 #pragma unroll
         for (int i = 0; i < V; ++i) v[i] = to_f32(e[i]);
     }
+};
+
+template <int V, typename T>
+__device__ __forceinline__ void load_v(const T* p, float (&v)[V]) {
+    Raw<T, V> r;
+    r.load(p);
+    r.get(v);
 }
 
-template <int V, int KIND>
+typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+
+template <int V, int KIND, bool NT = false>
 __device__ __forceinline__ void store_v(void* base, long idx, const float (&v)[V]) {
     if constexpr (V == 1) {
         if (KIND == 1)
@@ -67,53 +79,86 @@ __device__ __forceinline__ void store_v(void* base, long idx, const float (&v)[V
             ((_Float16*)base)[idx] = f32_to_f16(v[0]);
         else
             ((float*)base)[idx] = v[0];
+    } else if constexpr (KIND != 0) {
+        uint32_t w[V / 2];
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i)
+            w[i] = KIND == 1 ? pack2_bf16_rne(v[2 * i], v[2 * i + 1]) : pack2_f16_rne(v[2 * i], v[2 * i + 1]);
+        typedef typename std::conditional<V == 8, u32x4, u32x2>::type Q;
+        Q q;
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) q[i] = w[i];
+        Q* at = reinterpret_cast<Q*>((uint16_t*)base + idx);
+        if (NT)
+            __builtin_nontemporal_store(q, at);
+        else
+            *at = q;
     } else {
 #pragma unroll
-        for (int i = 0; i < V; i += 4) store4(base, idx + i, v[i], v[i + 1], v[i + 2], v[i + 3], KIND);
+        for (int i = 0; i < V; i += 4) {
+            const f32x4 q = {v[i], v[i + 1], v[i + 2], v[i + 3]};
+            f32x4* at = reinterpret_cast<f32x4*>((float*)base + idx + i);
+            if (NT)
+                __builtin_nontemporal_store(q, at);
+            else
+                *at = q;
+        }
     }
 }
 
-// Sum over aligned runs of `lanes` lanes, a power of two.
-__device__ __forceinline__ float lanes_sum(float v, int lanes) {
-    for (int o = 1; o < lanes; o <<= 1) v += __shfl_xor(v, o);
+// Sum over aligned runs of 2^bits lanes, the same bits in every lane.  Within a row of
+// 16 by DPP moves (quad permutations, then the half-row and row mirrors, whose lanes
+// hold the same partial sums as lane ^ 4 and lane ^ 8): no LDS round trips.
+template <int CTRL>
+__device__ __forceinline__ float dpp_move(float v) {
+    return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), CTRL, 0xF, 0xF, false));
+}
+
+__device__ __forceinline__ float lanes_sum(float v, int bits) {
+    if (bits > 0) v += dpp_move<0xB1>(v);
+    if (bits > 1) v += dpp_move<0x4E>(v);
+    if (bits > 2) v += dpp_move<0x141>(v);
+    if (bits > 3) v += dpp_move<0x140>(v);
+    if (bits > 4) v += __shfl_xor(v, 16);
+    if (bits > 5) v += __shfl_xor(v, 32);
     return v;
 }
 
-// Lanes that share a group's sums: a power of two, at most a wave, that lets all the
-// groups have theirs at once where there are enough.
-__device__ __forceinline__ int lanes_per_group(int groups, int threads) {
-    int l = 64;
-    while (l > 1 && l * groups > threads) l >>= 1;
-    return l;
-}
+constexpr int kThreads = 512;
 
-// The division of a chunk's pixels and channels among the threads: `seg` vectors of V
-// channels side by side, `rows` pixels at once.  More vectors than threads: sweeps of
-// one pixel row each.
+// How a workgroup's threads divide a chunk, made on the host: `seg` vectors of V
+// channels side by side and `rows` pixels at once (more vectors than threads: one
+// pixel, in sweeps), and 2^lane_bits lanes that share a group's sums, at most a wave,
+// as many as let all the groups have theirs at once where that can be.
 struct Split {
     int cv, seg, rows;
-    __device__ Split(int channels, int v, int threads) {
+    int inv_seg;     // thread / seg = thread * inv_seg >> 20
+    int lane_bits;
+    Split(int channels, int groups, int v) {
         cv = channels / v;
-        seg = min(cv, threads);
-        rows = cv > threads ? 1 : threads / seg;
+        seg = std::min(cv, kThreads);
+        rows = cv > kThreads ? 1 : kThreads / seg;
+        inv_seg = (1 << 20) / seg + 1;   // exact below 2^20 / seg threads
+        lane_bits = 6;
+        while (lane_bits > 0 && (groups << lane_bits) > kThreads) --lane_bits;
     }
 };
 
-constexpr int kThreads = 512;
-
 // A chunk's (mean, sum of squared deviations) of every group: parts[frame][group][chunk].
-template <int XK, int V>
-__global__ __launch_bounds__(kThreads) void group_norm_stats_kernel(GroupNormArgs p, int chunk,
+// A thread joins runs of SUB of its channels, which divides a group's.
+template <int XK, int V, int SUB>
+__global__ __launch_bounds__(kThreads) void group_norm_stats_kernel(GroupNormArgs p, Split sp,
+                                                                   int chunk,
                                                                    float2* __restrict__ parts) {
     typedef typename Elem<XK>::T T;
-    constexpr int ENTRIES = kThreads * V > kMaxChannels ? kThreads * V : kMaxChannels;
-    __shared__ float2 entry[ENTRIES];   // [row][channel]
+    constexpr int ENTRIES = (kThreads * V > kMaxChannels ? kThreads * V : kMaxChannels) / SUB;
+    __shared__ float2 entry[ENTRIES];   // [row][run of channels]
+    const int runs = p.channels / SUB;
     const int tid = threadIdx.x;
     const int f = blockIdx.y;
     const long p0 = (long)blockIdx.x * chunk;
     const int np = (int)min((long)chunk, p.pixels - p0);
-    const Split sp(p.channels, V, kThreads);
-    const int row = tid / sp.seg;
+    const int row = tid * sp.inv_seg >> 20;
     const int col = tid - row * sp.seg;
     const int base = np / sp.rows, extra = np - base * sp.rows;   // pixels of a row
     const T* x = (const T*)p.x + f * p.x_frame + p0 * p.x_pixel + (long)row * p.x_pixel;
@@ -125,128 +170,221 @@ __global__ __launch_bounds__(kThreads) void group_norm_stats_kernel(GroupNormArg
         load_v<V>(q, first);
 #pragma unroll
         for (int i = 0; i < V; ++i) s1[i] = s2[i] = 0.f;
-#pragma unroll 8
-        for (int j = 1; j < count; ++j) {
-            float v[V];
-            load_v<V>(q + j * step, v);
+        auto add = [&](const float (&v)[V]) {
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 const float d = v[i] - first[i];
                 s1[i] += d;
                 s2[i] = fmaf(d, d, s2[i]);
             }
-        }
-        const float inv = 1.f / (float)count;
+        };
+        constexpr int U = 8;   // pixels in flight
+        int j = 1;
+        for (; j + U <= count; j += U) {
+            Raw<T, V> raw[U];
 #pragma unroll
-        for (int i = 0; i < V; ++i)
-            entry[row * p.channels + c * V + i] =
-                make_float2(fmaf(s1[i], inv, first[i]), fmaxf(fmaf(-s1[i] * inv, s1[i], s2[i]), 0.f));
+            for (int u = 0; u < U; ++u) raw[u].load(q + (j + u) * step);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                float v[V];
+                raw[u].get(v);
+                add(v);
+            }
+        }
+        Raw<T, V> raw[U];
+#pragma unroll
+        for (int u = 0; u < U - 1; ++u)
+            if (j + u < count) raw[u].load(q + (j + u) * step);
+#pragma unroll
+        for (int u = 0; u < U - 1; ++u)
+            if (j + u < count) {
+                float v[V];
+                raw[u].get(v);
+                add(v);
+            }
+        const float n = (float)count, inv = 1.f / n;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {   // to mean and sum of squared deviations
+            first[i] = fmaf(s1[i], inv, first[i]);
+            s2[i] = fmaxf(fmaf(-s1[i] * inv, s1[i], s2[i]), 0.f);
+        }
+#pragma unroll
+        for (int i = 0; i < V; i += SUB) {
+            float off = 0.f, m2 = 0.f;
+#pragma unroll
+            for (int e = 1; e < SUB; ++e) off += first[i + e] - first[i];
+            const float mean = fmaf(off, 1.f / SUB, first[i]);
+#pragma unroll
+            for (int e = 0; e < SUB; ++e) {
+                const float d = SUB > 1 ? first[i + e] - mean : 0.f;
+                m2 += fmaf(n * d, d, s2[i + e]);
+            }
+            entry[row * runs + (c * V + i) / SUB] = make_float2(mean, m2);
+        }
     }
     __syncthreads();
-    const int each = p.channels / p.groups;
+    const int each = runs / p.groups;   // runs of a group
     const int used = min(sp.rows, np);
-    const int lanes = lanes_per_group(p.groups, kThreads);
+    const int lanes = 1 << sp.lane_bits;
+    // of a group's lanes, `across` take neighbouring runs, the others rows
+    const int across_bits = min(sp.lane_bits, 32 - __clz(each - 1));
+    const int across = 1 << across_bits;
     const int lane = tid & (lanes - 1);
-    const float per_value = 1.f / ((float)np * (float)each);
-    for (int g0 = 0; g0 < p.groups; g0 += kThreads / lanes) {   // the same count in every thread
-        const int g = g0 + tid / lanes;
-        const float2* e = entry + g * each;
-        const float ref = g < p.groups ? e[0].x : 0.f;
+    const int c0 = lane & (across - 1), r0 = lane >> across_bits, dr = lanes >> across_bits;
+    const float per_run = 1.f / ((float)np * (float)each);
+    for (int g0 = 0; g0 < p.groups; g0 += kThreads >> sp.lane_bits) {   // as often in every thread
+        const int g = g0 + (tid >> sp.lane_bits);
+        const float2* e = entry + min(g, p.groups - 1) * each;
+        const float ref = e[0].x;
         float sum = 0.f;
-        if (g < p.groups)
-            for (int r = 0; r < used; ++r) {
-                const float n = (float)(base + (r < extra));
-                for (int c = lane; c < each; c += lanes) sum = fmaf(n, e[r * p.channels + c].x - ref, sum);
-            }
-        const float mean = fmaf(lanes_sum(sum, lanes), per_value, ref);
+        for (int c = c0; c < each; c += across)
+#pragma unroll 4
+            for (int r = r0; r < used; r += dr)
+                sum = fmaf((float)(base + (r < extra)), e[r * runs + c].x - ref, sum);
+        const float mean = fmaf(lanes_sum(sum, sp.lane_bits), per_run, ref);
         float m2 = 0.f;
-        if (g < p.groups)
-            for (int r = 0; r < used; ++r) {
-                const float n = (float)(base + (r < extra));
-                for (int c = lane; c < each; c += lanes) {
-                    const float2 v = e[r * p.channels + c];
-                    const float d = v.x - mean;
-                    m2 += fmaf(n * d, d, v.y);
-                }
+        for (int c = c0; c < each; c += across)
+#pragma unroll 4
+            for (int r = r0; r < used; r += dr) {
+                const float2 v = e[r * runs + c];
+                const float d = v.x - mean;
+                m2 += fmaf((float)((base + (r < extra)) * SUB) * d, d, v.y);
             }
-        m2 = lanes_sum(m2, lanes);
+        m2 = lanes_sum(m2, sp.lane_bits);
         if (g < p.groups && lane == 0)
             parts[((long)f * p.groups + g) * gridDim.x + blockIdx.x] = make_float2(mean, m2);
     }
 }
 
+// V consecutive values of gamma or beta, or `none` without one
+template <int V>
+__device__ __forceinline__ void load_affine(const float* p, int c, float none, float (&v)[V]) {
+    if (!p) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] = none;
+    } else {
+        __builtin_memcpy(v, p + c, sizeof(v));
+    }
+}
+
+// y.  Frames and chunks in the reverse of the first kernel's order, and stores that pass
+// the caches by: what of x was read last is still there to be read again (118 MB of x:
+// 66 us, 82 with plain stores; 944 MB: 528 against 542).
 template <int XK, int YK, int V>
-__global__ __launch_bounds__(kThreads) void group_norm_apply_kernel(GroupNormArgs p, int part_chunk,
-                                                                   int chunks, int chunk,
+__global__ __launch_bounds__(kThreads) void group_norm_apply_kernel(GroupNormArgs p, Split sp,
+                                                                   int part_chunk, int chunks,
+                                                                   int chunk,
                                                                    const float2* __restrict__ parts) {
     typedef typename Elem<XK>::T T;
     __shared__ float2 stat[kMaxChannels];   // (mean, rstd) of each group
     const int tid = threadIdx.x;
-    const int f = blockIdx.y;
+    const int f = gridDim.y - 1 - blockIdx.y;
     const int each = p.channels / p.groups;
-    const int lanes = lanes_per_group(p.groups, kThreads);
+    const long p0 = (long)(gridDim.x - 1 - blockIdx.x) * chunk;
+    const int np = (int)min((long)chunk, p.pixels - p0);
+    const int row = tid * sp.inv_seg >> 20;
+    const int col = tid - row * sp.seg;
+    const T* x = (const T*)p.x + f * p.x_frame + p0 * p.x_pixel;
+    constexpr int U = 4;   // pixels in flight
+    Raw<T, V> raw[U];
+    // (pixels past the end repeat the last one)
+    auto fetch = [&](int c, int j) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) raw[u].load(x + (long)min(j + u * sp.rows, np - 1) * p.x_pixel + c);
+    };
+    float scale[V], shift[V];
+    auto affine = [&](int c) {
+        load_affine<V>(p.gamma, c, 1.f, scale);
+        load_affine<V>(p.beta, c, 0.f, shift);
+    };
+    const int lanes = 1 << sp.lane_bits;
     const int lane = tid & (lanes - 1);
-    for (int g0 = 0; g0 < p.groups; g0 += kThreads / lanes) {
-        const int g = g0 + tid / lanes;
+    const float whole = (float)part_chunk;
+    const float rest = (float)(p.pixels - (long)(chunks - 1) * part_chunk);   // the last part
+    for (int g0 = 0; g0 < p.groups; g0 += kThreads >> sp.lane_bits) {
+        const int g = g0 + (tid >> sp.lane_bits);
         const float2* e = parts + ((long)f * p.groups + min(g, p.groups - 1)) * chunks;
-        // deviations from the first part's mean: as far from it as the parts are from
-        // one another
         const float ref = e[0].x;
-        float sum = 0.f, sq = 0.f, m2 = 0.f;
-#pragma unroll 4
-        for (int c = lane; c < chunks; c += lanes) {
-            const float2 v = e[c];
-            const float n = (float)min((long)part_chunk, p.pixels - (long)c * part_chunk);
-            const float d = v.x - ref;
-            sum = fmaf(n, d, sum);
-            sq = fmaf(n * d, d, sq);
-            m2 += v.y;
+        constexpr int C = 4;   // parts in flight
+        float2 v[C];
+        auto get = [&](int i0) {
+#pragma unroll
+            for (int c = 0; c < C; ++c) v[c] = e[min(i0 + c * lanes, chunks - 1)];
+        };
+        auto pixels = [&](int at) { return at + 1 < chunks ? whole : at + 1 == chunks ? rest : 0.f; };
+        get(lane);
+        if (g0 == 0) {
+            // once the parts are there, the thread's first pixels: under the arithmetic
+#pragma unroll
+            for (int c = 0; c < C; ++c) asm volatile("" : "+v"(v[c].x), "+v"(v[c].y)::"memory");
+            fetch(col * V, row);
+            affine(col * V);
         }
-        sum = lanes_sum(sum, lanes);
-        sq = lanes_sum(sq, lanes);
-        m2 = lanes_sum(m2, lanes);
+        float sum = 0.f, m2 = 0.f;
+        for (int i0 = lane;;) {
+#pragma unroll
+            for (int c = 0; c < C; ++c) sum = fmaf(pixels(i0 + c * lanes), v[c].x - ref, sum);
+            i0 += C * lanes;
+            if (i0 >= chunks) break;
+            get(i0);
+        }
+        const float off = lanes_sum(sum, sp.lane_bits) / (float)p.pixels;   // of the mean from ref
+        if (chunks > C * lanes) get(lane);
+        for (int i0 = lane;;) {
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                const int at = i0 + c * lanes;
+                const float d = v[c].x - ref - off;
+                m2 += at < chunks ? fmaf(pixels(at) * (float)each * d, d, v[c].y) : 0.f;
+            }
+            i0 += C * lanes;
+            if (i0 >= chunks) break;
+            get(i0);
+        }
+        m2 = lanes_sum(m2, sp.lane_bits);
         if (g < p.groups && lane == 0) {
-            const float mean = sum / (float)p.pixels;
-            const float var = (fmaxf(fmaf(-mean, sum, sq), 0.f) * (float)each + m2) /
-                              ((float)p.pixels * (float)each);
-            // an infinity or NaN in any part makes m2 NaN
-            stat[g] = make_float2(ref + mean, 1.f / sqrtf(var + p.eps));
+            const float var = m2 / ((float)p.pixels * (float)each);
+            stat[g] = make_float2(ref + off, 1.f / sqrtf(var + p.eps));
         }
     }
     __syncthreads();
-    const long p0 = (long)blockIdx.x * chunk;
-    const int np = (int)min((long)chunk, p.pixels - p0);
-    const Split sp(p.channels, V, kThreads);
-    const int row = tid / sp.seg;
-    const int col = tid - row * sp.seg;
     if (row >= sp.rows) return;
-    const T* x = (const T*)p.x + f * p.x_frame + p0 * p.x_pixel;
     const long y0 = f * p.y_frame + p0 * p.y_pixel;
     for (int cc = col; cc < sp.cv; cc += sp.seg) {
         const int c = cc * V;
-        float mean[V], scale[V], shift[V];
+        if (cc != col) {
+            fetch(c, row);
+            affine(c);
+        }
+        float mean[V];
+        int g = c / each, in = c - g * each;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            const float2 s = stat[(c + i) / each];
-            mean[i] = s.x;
-            scale[i] = s.y * (p.gamma ? p.gamma[c + i] : 1.f);
-            shift[i] = p.beta ? p.beta[c + i] : 0.f;
+            const float2 st = stat[g];
+            mean[i] = st.x;
+            scale[i] *= st.y;
+            if (++in == each) {
+                in = 0;
+                ++g;
+            }
         }
-        constexpr int U = 4;   // pixels in flight
-        for (int j = row; j < np; j += U * sp.rows) {
-            float v[U][V];
+        with_activation(p.act, [&](auto act) {
+            for (int j = row; j < np; j += U * sp.rows) {
+                float v[U][V];
 #pragma unroll
-            for (int u = 0; u < U; ++u)
-                if (j + u * sp.rows < np) load_v<V>(x + (long)(j + u * sp.rows) * p.x_pixel + c, v[u]);
+                for (int u = 0; u < U; ++u) raw[u].get(v[u]);
+                if (j + U * sp.rows < np) fetch(c, j + U * sp.rows);
 #pragma unroll
-            for (int u = 0; u < U; ++u)
-                if (j + u * sp.rows < np) {
+                for (int u = 0; u < U; ++u)
+                    if (j + u * sp.rows < np) {
 #pragma unroll
-                    for (int i = 0; i < V; ++i)
-                        v[u][i] = activate(fmaf(v[u][i] - mean[i], scale[i], shift[i]), p.act);
-                    store_v<V, YK>(p.y, y0 + (long)(j + u * sp.rows) * p.y_pixel + c, v[u]);
-                }
-        }
+                        for (int i = 0; i < V; ++i)
+                            v[u][i] = activate(fmaf(v[u][i] - mean[i], scale[i], shift[i]),
+                                               decltype(act)::value);
+                        store_v<V, YK, true>(p.y, y0 + (long)(j + u * sp.rows) * p.y_pixel + c, v[u]);
+                    }
+            }
+        });
     }
 }
 
@@ -256,7 +394,7 @@ constexpr int kSmallThreads = 256;
 constexpr int kSmallVectors = 8;   // of a thread
 
 __device__ __forceinline__ float block_sum(float v, float* lds) {
-    v = lanes_sum(v, 64);
+    v = lanes_sum(v, 6);
     if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
     __syncthreads();
     v = 0.f;
@@ -271,49 +409,57 @@ __global__ __launch_bounds__(kSmallThreads) void group_norm_small_kernel(GroupNo
     __shared__ float lds[2][kSmallThreads / 64];
     const int f = blockIdx.y, g = blockIdx.x;
     const int each = p.channels / p.groups;
-    const int ev = each / V;   // vectors of a pixel
-    const int all = p.pixels * ev;
-    const T* x = (const T*)p.x + f * p.x_frame + (long)g * each;
-    float v[kSmallVectors][V];
-    int pix[kSmallVectors], ch[kSmallVectors];
+    const int ev = each / V;   // vectors of a pixel, at most the threads
+    const int rows = kSmallThreads / ev;
+    const int row = threadIdx.x / ev;
+    const int c = g * each + (threadIdx.x - row * ev) * V;
+    const int count = row < rows ? (p.pixels - row + rows - 1) / rows : 0;   // of this thread
+    const T* x = (const T*)p.x + f * p.x_frame;
+    Raw<T, V> raw[kSmallVectors];
 #pragma unroll
-    for (int u = 0; u < kSmallVectors; ++u) {
-        const int i = threadIdx.x + u * kSmallThreads;
-        pix[u] = i / ev;
-        ch[u] = (i - pix[u] * ev) * V;
-        if (i < all) load_v<V>(x + pix[u] * p.x_pixel + ch[u], v[u]);
+    for (int u = 0; u < kSmallVectors; ++u)
+        if (u < count) raw[u].load(x + (long)(row + u * rows) * p.x_pixel + c);
+    float scale[V], shift[V];
+    if (count > 0) {
+        load_affine<V>(p.gamma, c, 1.f, scale);
+        load_affine<V>(p.beta, c, 0.f, shift);
     }
     // deviations from the first value: no digits are lost to a large mean
-    const float ref = to_f32(*x);
+    const float ref = to_f32(x[g * each]);
+    float v[kSmallVectors][V];
     float sum = 0.f;
 #pragma unroll
     for (int u = 0; u < kSmallVectors; ++u)
-        if (threadIdx.x + u * kSmallThreads < all)
+        if (u < count) {
+            raw[u].get(v[u]);
 #pragma unroll
             for (int i = 0; i < V; ++i) sum += v[u][i] - ref;
-    const float count = (float)all * V;
-    const float mean = ref + block_sum(sum, lds[0]) / count;
+        }
+    const float per_value = 1.f / ((float)p.pixels * (float)each);
+    const float mean = fmaf(block_sum(sum, lds[0]), per_value, ref);
     float m2 = 0.f;
 #pragma unroll
     for (int u = 0; u < kSmallVectors; ++u)
-        if (threadIdx.x + u * kSmallThreads < all)
+        if (u < count)
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 const float d = v[u][i] - mean;
                 m2 = fmaf(d, d, m2);
             }
-    const float rstd = 1.f / sqrtf(block_sum(m2, lds[1]) / count + p.eps);
+    const float rstd = 1.f / sqrtf(fmaf(block_sum(m2, lds[1]), per_value, p.eps));
+    if (count == 0) return;
 #pragma unroll
-    for (int u = 0; u < kSmallVectors; ++u)
-        if (threadIdx.x + u * kSmallThreads < all) {
-            const int c = g * each + ch[u];
+    for (int i = 0; i < V; ++i) scale[i] *= rstd;
+    with_activation(p.act, [&](auto act) {
 #pragma unroll
-            for (int i = 0; i < V; ++i)
-                v[u][i] = activate(fmaf(v[u][i] - mean, rstd * (p.gamma ? p.gamma[c + i] : 1.f),
-                                        p.beta ? p.beta[c + i] : 0.f),
-                                   p.act);
-            store_v<V, YK>(p.y, f * p.y_frame + pix[u] * p.y_pixel + c, v[u]);
-        }
+        for (int u = 0; u < kSmallVectors; ++u)
+            if (u < count) {
+#pragma unroll
+                for (int i = 0; i < V; ++i)
+                    v[u][i] = activate(fmaf(v[u][i] - mean, scale[i], shift[i]), decltype(act)::value);
+                store_v<V, YK>(p.y, f * p.y_frame + (long)(row + u * rows) * p.y_pixel + c, v[u]);
+            }
+    });
 }
 
 // V channels are whole 16-byte pieces (8 bytes: four 16-bit ones) of every row of a view
@@ -327,11 +473,11 @@ bool fits(const GroupNormArgs& p, int width, int v) {
            fits(p.y, p.y_kind, p.y_frame, p.y_pixel, v);
 }
 
-// How a frame's pixels are cut: into at most 256 chunks, whose parts every workgroup of
-// the second kernel reads, and about 512 workgroups in all.
+// How a frame's pixels are cut for the statistics: about one workgroup for each compute
+// unit, and 64 to 256 parts, which every workgroup of the second kernel joins.
 int chunk_pixels(int frames, int pixels, int channels) {
-    const long want = std::min<long>(256, std::max<long>(1, 512 / frames));   // chunks of a frame
-    const long least = std::max<long>(1, 8192 / channels);                    // pixels of a chunk
+    const long want = std::min(256, std::max(64, 256 / frames));   // chunks of a frame
+    const long least = std::max<long>(1, 8192 / channels);         // pixels of a chunk
     return (int)std::min<long>(pixels, std::max(least, (pixels + want - 1) / want));
 }
 
@@ -339,14 +485,30 @@ long chunks_of(int pixels, int chunk) { return ((long)pixels + chunk - 1) / chun
 
 template <int XK, int YK, int V>
 hipError_t run(const GroupNormArgs& p, float2* parts, hipStream_t stream) {
+    const int each = p.channels / p.groups;
+    const Split sp(p.channels, p.groups, V);
     const int part = chunk_pixels(p.frames, p.pixels, p.channels);
     const int chunks = (int)chunks_of(p.pixels, part);
-    group_norm_stats_kernel<XK, V>
-        <<<dim3((unsigned)chunks, (unsigned)p.frames), kThreads, 0, stream>>>(p, part, parts);
-    const int chunk = part;
+    // the second kernel's workgroups have 512 KB of x each where that makes 256 to 2048
+    // of them: a workgroup costs microseconds before its first result, and few have too
+    // little in flight.  14400 x 512 in bf16 (14.7 MB): 17 us with 256, 25 with 1024;
+    // 230400 x 256 (118 MB): 66 with 256, 76 with 2048; four frames of 921600 x 128
+    // (944 MB): 547 with 256, 528 with 2048.
+    const long bytes = (long)p.frames * p.pixels * p.channels * (XK ? 2 : 4);
+    const long blocks = std::min(2048L, std::max(256L, bytes >> 19));
+    const long least = std::max<long>(1, 8192 / p.channels);
+    const int chunk =
+        (int)std::min<long>(p.pixels, std::max(least, ((long)p.pixels * p.frames + blocks - 1) / blocks));
+    const dim3 grid((unsigned)chunks, (unsigned)p.frames);
+    if (each % V == 0)
+        group_norm_stats_kernel<XK, V, V><<<grid, kThreads, 0, stream>>>(p, sp, part, parts);
+    else if (V == 8 && each % 4 == 0)
+        group_norm_stats_kernel<XK, V, V == 8 ? 4 : 1><<<grid, kThreads, 0, stream>>>(p, sp, part, parts);
+    else
+        group_norm_stats_kernel<XK, V, 1><<<grid, kThreads, 0, stream>>>(p, sp, part, parts);
+    const dim3 grid2((unsigned)chunks_of(p.pixels, chunk), (unsigned)p.frames);
     group_norm_apply_kernel<XK, YK, V>
-        <<<dim3((unsigned)chunks_of(p.pixels, chunk), (unsigned)p.frames), kThreads, 0, stream>>>(
-            p, part, chunks, chunk, parts);
+        <<<grid2, kThreads, 0, stream>>>(p, sp, part, chunks, chunk, parts);
     return hipGetLastError();
 }
 
@@ -355,7 +517,7 @@ hipError_t pick(const GroupNormArgs& p, float2* parts, hipStream_t stream) {
     const int each = p.channels / p.groups;
     for (int v : {8, 4, 1}) {
         if (v > 1 && !fits(p, each, v)) continue;
-        if ((long)p.pixels * (each / v) > kSmallThreads * kSmallVectors) break;
+        if (each / v > kSmallThreads || p.pixels > kSmallThreads / (each / v) * kSmallVectors) break;
         const dim3 grid((unsigned)p.groups, (unsigned)p.frames);
         if (v == 8)
             group_norm_small_kernel<XK, YK, 8><<<grid, kSmallThreads, 0, stream>>>(p);

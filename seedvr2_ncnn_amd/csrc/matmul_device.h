@@ -75,11 +75,6 @@ __device__ __forceinline__ void store1(void* p, long idx, float v, int kind) {
         ((float*)p)[idx] = v;
 }
 
-template <int ACT>
-__device__ __forceinline__ float act_of(float v) {
-    return activate(v, ACT);
-}
-
 // Epilogue of a wave's tile of NI x 16 rows and 64 columns: accumulator [i][j][r] is
 // row row_w + 16 i + 4 g + r of the block tile's `rows`, column col + j.  WHOLE: pieces
 // of four; else single elements.
@@ -99,7 +94,7 @@ __device__ __forceinline__ void epilogue(const MatmulArgs& a, const RowTile& rt,
                 if (col + j < a.n) b[j] = bias[j];
         }
     }
-    auto emit = [&](auto act_tag) {
+    with_activation(a.act, [&](auto act_tag) {
         constexpr int ACT = decltype(act_tag)::value;
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
@@ -134,7 +129,7 @@ __device__ __forceinline__ void epilogue(const MatmulArgs& a, const RowTile& rt,
                 float v[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    v[j] = act_of<ACT>(acc[i][j][r] + b[j]);
+                    v[j] = activate(acc[i][j][r] + b[j], ACT);
                     if (a.res) v[j] += res[r][j];
                 }
                 const long at = (row + r) * a.y_stride + col;
@@ -147,15 +142,7 @@ __device__ __forceinline__ void epilogue(const MatmulArgs& a, const RowTile& rt,
                 }
             }
         }
-    };
-    if (a.act == S2_ACT_NONE)
-        emit(std::integral_constant<int, S2_ACT_NONE>{});
-    else if (a.act == S2_ACT_GELU)
-        emit(std::integral_constant<int, S2_ACT_GELU>{});
-    else if (a.act == S2_ACT_SILU)
-        emit(std::integral_constant<int, S2_ACT_SILU>{});
-    else
-        emit(std::integral_constant<int, S2_ACT_GELU_TANH>{});
+    });
 }
 
 // fp32 as a sum of PL bf16 values: all but the last take the top 8 bits of what the
