@@ -512,7 +512,8 @@ S2_API int s2_shared_linear_residual(const void* x_video, int m_video, const voi
  * channels: a multiple of groups, at most 4096; frames at most 65535.
  *   frames == 0 or pixels == 0 does nothing.
  * workspace: s2_group_norm_workspace_bytes, 8-byte aligned (partial
- *   statistics; calls that may overlap in time need one each).
+ *   statistics; calls that may overlap in time need one each; 0 for small
+ *   groups, then it may be NULL).
  * An infinity or NaN makes its frame's group NaN, no other. */
 S2_API int s2_group_norm_workspace_bytes(int frames, int pixels, int channels, int groups,
                                          size_t* bytes);

@@ -7,6 +7,7 @@ library is missing, or no gfx950 device is visible, calls raise.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 
 _PKG = os.path.dirname(os.path.abspath(__file__))
@@ -691,17 +692,18 @@ def denoise_update(positive_patches, negative_patches, frames, height, width, cf
 def _vector(t, size, name):
     """Checks an optional contiguous fp32 device vector (gamma, beta, bias)."""
     import torch
-    if t is not None and (t.dtype != torch.float32 or t.numel() != size or not t.is_contiguous()):
+    if t is not None and (t.dtype is not torch.float32 or t.numel() != size or
+                          not t.is_contiguous()):
         raise ValueError(f"{name} must be {size} contiguous fp32 values")
 
 
-def _on_current_device(*tensors):
+def _on_current_device(x, *others):
     """Refuses tensors that the current device's kernels cannot reach."""
     import torch
-    device = torch.cuda.current_device() if torch.cuda.is_available() else 0
-    for t in tensors:
-        if t is not None and t.get_device() != device:
-            raise ValueError(f"operands must be on the current device, cuda:{device}")
+    device = x.get_device()
+    if device < 0 or device != torch._C._cuda_getDevice() or any(
+            t is not None and t.get_device() != device for t in others):
+        raise ValueError("operands must be on the current device")
 
 
 def group_norm(x, groups, gamma=None, beta=None, epsilon=1e-6, activation=ACT_NONE, out=None,
@@ -718,22 +720,22 @@ def group_norm(x, groups, gamma=None, beta=None, epsilon=1e-6, activation=ACT_NO
     xd = _dtype_code(x)
     if out is None:
         out = torch.empty((f, p, c), dtype=out_dtype or x.dtype, device=x.device)
-    if out.shape != x.shape or (c > 1 and (x.stride(2) != 1 or out.stride(2) != 1)):
-        raise ValueError("x and out must be of one shape with contiguous channels")
+    elif out.shape != x.shape:
+        raise ValueError("x and out must be of one shape")
+    if c > 1 and (x.stride(2) != 1 or out.stride(2) != 1):
+        raise ValueError("channels must be contiguous")
     _vector(gamma, c, "gamma")
     _vector(beta, c, "beta")
     _on_current_device(x, out, gamma, beta, workspace)
-    if workspace is None:
-        workspace = torch.empty(group_norm_workspace(f, p, c, groups), dtype=torch.uint8,
-                                device=x.device)
-    check(lib().s2_group_norm(_ptr(x), xd, x.stride(0), x.stride(1), f, p, c, groups,
-                              _ptr(gamma), _ptr(beta), float(epsilon), activation, _ptr(out),
+    workspace, size = _workspace(workspace, group_norm_workspace, x, f, p, c, groups)
+    check(lib().s2_group_norm(x.data_ptr(), xd, x.stride(0), x.stride(1), f, p, c, groups,
+                              _ptr(gamma), _ptr(beta), epsilon, activation, out.data_ptr(),
                               _dtype_code(out), out.stride(0), out.stride(1), _ptr(workspace),
-                              workspace.numel() * workspace.element_size(), _stream(stream)),
-          "s2_group_norm")
+                              size, _stream(stream)), "s2_group_norm")
     return out
 
 
+@functools.lru_cache(maxsize=4096)
 def group_norm_workspace(frames, pixels, channels, groups) -> int:
     """s2_group_norm_workspace_bytes."""
     n = ctypes.c_size_t()
@@ -745,22 +747,22 @@ def group_norm_workspace(frames, pixels, channels, groups) -> int:
 def _matmul_views(x, n, k, weight, residual, out, out_dtype):
     """The checked output of linear and grouped_linear."""
     import torch
-    if x.dim() != 2 or x.shape[1] != k:
-        raise ValueError(f"x must be [m, {k}]")
+    if x.dim() != 2 or x.shape[1] != k or (k > 1 and x.stride(1) != 1):
+        raise ValueError(f"x must be [m, {k}] with contiguous rows")
     if not weight.is_contiguous():
         raise ValueError("weight must be contiguous")
     m = x.shape[0]
     if out is None:
         out = torch.empty((m, n), dtype=out_dtype or x.dtype, device=x.device)
-    for t in (x, residual, out):
-        if t is not None and t.shape[1] > 1 and t.stride(1) != 1:
-            raise ValueError("rows must be contiguous")
-    if out.shape != (m, n) or (residual is not None and
-                               (residual.shape != out.shape or residual.dtype != out.dtype)):
-        raise ValueError(f"out and residual must be [{m}, {n}] of one type")
+    elif out.shape != (m, n) or (n > 1 and out.stride(1) != 1):
+        raise ValueError(f"out must be [{m}, {n}] with contiguous rows")
+    if residual is not None and (residual.shape != (m, n) or residual.dtype is not out.dtype or
+                                 (n > 1 and residual.stride(1) != 1)):
+        raise ValueError(f"residual must be [{m}, {n}] of out's type with contiguous rows")
     return out
 
 
+@functools.lru_cache(maxsize=4096)
 def linear_workspace(m, n, k, x_dtype=DTYPE_BF16, y_dtype=DTYPE_BF16) -> int:
     """s2_linear_workspace_bytes."""
     b = ctypes.c_size_t()
@@ -769,6 +771,7 @@ def linear_workspace(m, n, k, x_dtype=DTYPE_BF16, y_dtype=DTYPE_BF16) -> int:
     return b.value
 
 
+@functools.lru_cache(maxsize=4096)
 def grouped_linear_workspace(m, groups, n, k, x_dtype=DTYPE_BF16, y_dtype=DTYPE_BF16) -> int:
     """s2_grouped_linear_workspace_bytes."""
     b = ctypes.c_size_t()
@@ -778,13 +781,13 @@ def grouped_linear_workspace(m, groups, n, k, x_dtype=DTYPE_BF16, y_dtype=DTYPE_
     return b.value
 
 
-def _workspace(workspace, size, device):
-    """(workspace or None, bytes): the caller's, or `size()` bytes made here."""
+def _workspace(workspace, size, x, *sizes):
+    """(workspace or None, bytes): the caller's, or size(*sizes) bytes made here."""
     import torch
     if workspace is not None:
         return workspace, workspace.numel() * workspace.element_size()
-    size = size()
-    return (torch.empty(size, dtype=torch.uint8, device=device) if size else None), size
+    n = size(*sizes)
+    return (torch.empty(n, dtype=torch.uint8, device=x.device) if n else None), n
 
 
 def linear(x, weight, bias=None, activation=ACT_NONE, residual=None, out=None, out_dtype=None,
@@ -799,10 +802,10 @@ def linear(x, weight, bias=None, activation=ACT_NONE, residual=None, out=None, o
     _vector(bias, n, "bias")
     m, xd, yd = x.shape[0], _dtype_code(x), _dtype_code(out)
     _on_current_device(x, weight, bias, residual, out, workspace)
-    workspace, size = _workspace(workspace, lambda: linear_workspace(m, n, k, xd, yd), x.device)
-    check(lib().s2_linear(_ptr(x), xd, x.stride(0), m, _ptr(weight), _dtype_code(weight),
+    workspace, size = _workspace(workspace, linear_workspace, x, m, n, k, xd, yd)
+    check(lib().s2_linear(x.data_ptr(), xd, x.stride(0), m, weight.data_ptr(), _dtype_code(weight),
                           _ptr(bias), n, k, activation, _ptr(residual),
-                          residual.stride(0) if residual is not None else 0, _ptr(out), yd,
+                          residual.stride(0) if residual is not None else 0, out.data_ptr(), yd,
                           out.stride(0), _ptr(workspace), size, _stream(stream)), "s2_linear")
     return out
 
@@ -822,12 +825,12 @@ def grouped_linear(x, offsets, weight, bias=None, activation=ACT_NONE, residual=
     _vector(bias, groups * n, "bias")
     m, xd, yd = x.shape[0], _dtype_code(x), _dtype_code(out)
     _on_current_device(x, offsets, weight, bias, residual, out, workspace)
-    workspace, size = _workspace(
-        workspace, lambda: grouped_linear_workspace(m, groups, n, k, xd, yd), x.device)
-    check(lib().s2_grouped_linear(_ptr(x), xd, x.stride(0), m, _ptr(offsets), groups, _ptr(weight),
+    workspace, size = _workspace(workspace, grouped_linear_workspace, x, m, groups, n, k, xd, yd)
+    check(lib().s2_grouped_linear(x.data_ptr(), xd, x.stride(0), m, offsets.data_ptr(), groups,
+                                  weight.data_ptr(),
                                   _dtype_code(weight), _ptr(bias), n, k, activation,
                                   _ptr(residual),
-                                  residual.stride(0) if residual is not None else 0, _ptr(out), yd,
+                                  residual.stride(0) if residual is not None else 0, out.data_ptr(), yd,
                                   out.stride(0), _ptr(workspace), size, _stream(stream)),
           "s2_grouped_linear")
     return out

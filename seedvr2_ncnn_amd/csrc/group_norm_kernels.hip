@@ -473,6 +473,11 @@ bool fits(const GroupNormArgs& p, int width, int v) {
            fits(p.y, p.y_kind, p.y_frame, p.y_pixel, v);
 }
 
+// Whether a workgroup can hold a frame's group, `vectors` to a pixel.
+bool small_holds(int pixels, int vectors) {
+    return vectors <= kSmallThreads && pixels <= kSmallThreads / vectors * kSmallVectors;
+}
+
 // How a frame's pixels are cut for the statistics: about one workgroup for each compute
 // unit, and 64 to 256 parts, which every workgroup of the second kernel joins.
 int chunk_pixels(int frames, int pixels, int channels) {
@@ -517,7 +522,7 @@ hipError_t pick(const GroupNormArgs& p, float2* parts, hipStream_t stream) {
     const int each = p.channels / p.groups;
     for (int v : {8, 4, 1}) {
         if (v > 1 && !fits(p, each, v)) continue;
-        if (each / v > kSmallThreads || p.pixels > kSmallThreads / (each / v) * kSmallVectors) break;
+        if (!small_holds(p.pixels, each / v)) break;
         const dim3 grid((unsigned)p.groups, (unsigned)p.frames);
         if (v == 8)
             group_norm_small_kernel<XK, YK, 8><<<grid, kSmallThreads, 0, stream>>>(p);
@@ -543,6 +548,8 @@ hipError_t pick_y(const GroupNormArgs& p, float2* parts, hipStream_t stream) {
 
 size_t group_norm_workspace(int frames, int pixels, int channels, int groups) {
     if (frames <= 0 || pixels <= 0) return 0;
+    // groups in registers, by single elements if need be
+    if (small_holds(pixels, channels / groups)) return 0;
     const int chunk = chunk_pixels(frames, pixels, channels);
     return (size_t)frames * (size_t)chunks_of(pixels, chunk) * groups * sizeof(float2);
 }
