@@ -75,76 +75,6 @@ __device__ __forceinline__ void store1(void* p, long idx, float v, int kind) {
         ((float*)p)[idx] = v;
 }
 
-// Epilogue of a wave's tile of NI x 16 rows and 64 columns: accumulator [i][j][r] is
-// row row_w + 16 i + 4 g + r of the block tile's `rows`, column col + j.  WHOLE: pieces
-// of four; else single elements.
-template <int YK, int NI, bool WHOLE>
-__device__ __forceinline__ void epilogue(const MatmulArgs& a, const RowTile& rt, int rows, int row_w,
-                                         int col, const f32x4 (&acc)[NI][4]) {
-    const int g = (threadIdx.x & 63) >> 4;
-    if (col >= a.n) return;
-    f32x4 b = {0.f, 0.f, 0.f, 0.f};
-    if (a.bias) {
-        const float* bias = a.bias + (long)rt.group * a.n + col;
-        if (WHOLE) {
-            b = *reinterpret_cast<const f32x4*>(bias);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (col + j < a.n) b[j] = bias[j];
-        }
-    }
-    with_activation(a.act, [&](auto act_tag) {
-        constexpr int ACT = decltype(act_tag)::value;
-#pragma unroll
-        for (int i = 0; i < NI; ++i) {
-            const int r0 = row_w + 16 * i + 4 * g;
-            const long row = rt.row0 + r0;
-            f32x4 res[4];
-            if (a.res) {
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    if (r0 + r >= rows) continue;
-                    const long at = (row + r) * a.res_stride + col;
-                    if (!WHOLE) {
-#pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            if (col + j < a.n) res[r][j] = load1(a.res, at + j, YK);
-                    } else if (YK == 0) {
-                        res[r] = *reinterpret_cast<const f32x4*>((const float*)a.res + at);
-                    } else {
-                        const uint2 q = *reinterpret_cast<const uint2*>((const uint16_t*)a.res + at);
-                        const uint32_t w[2] = {q.x, q.y};
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const uint16_t h = (uint16_t)(w[j >> 1] >> (16 * (j & 1)));
-                            res[r][j] = YK == 1 ? bf16_to_f32(h) : (float)__builtin_bit_cast(_Float16, h);
-                        }
-                    }
-                }
-            }
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                if (r0 + r >= rows) continue;
-                float v[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    v[j] = activate(acc[i][j][r] + b[j], ACT);
-                    if (a.res) v[j] += res[r][j];
-                }
-                const long at = (row + r) * a.y_stride + col;
-                if (WHOLE) {
-                    store4(a.y, at, v[0], v[1], v[2], v[3], YK);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        if (col + j < a.n) store1(a.y, at + j, v[j], YK);
-                }
-            }
-        }
-    });
-}
-
 // fp32 as a sum of PL bf16 values: all but the last take the top 8 bits of what the
 // ones before leave, by truncation, which cannot overflow and leaves an exact rest; the
 // last rounds (two terms: to 2^-15 of x) or, of three, holds the rest exactly.  An

@@ -50,6 +50,7 @@ struct MatmulPlan {
     int rows;              // kRows: rows of a tile, 16, 32 or 64
     int bm, bn;            // kTiles: the tile
     int parts;             // kTiles: ranges of k
+    bool whole;            // kTiles: y and residual in pieces of four columns
     bool pack_x, pack_w;
     size_t x_bytes, w_bytes, sum_bytes;   // 256-byte multiples, in this order
     size_t bytes() const { return x_bytes + w_bytes + sum_bytes; }

@@ -24,6 +24,76 @@ bool whole_pieces(const MatmulArgs& a) {
            (!a.res || (a.res_stride % 4 == 0 && (uintptr_t)a.res % e == 0));
 }
 
+// Epilogue of the kernel below, any strides: a wave's tile of NI x 16 rows and 64 columns, accumulator [i][j][r] is
+// row row_w + 16 i + 4 g + r of the block tile's `rows`, column col + j.  WHOLE: pieces
+// of four; else single elements.
+template <int YK, int NI, bool WHOLE>
+__device__ __forceinline__ void epilogue(const MatmulArgs& a, const RowTile& rt, int rows, int row_w,
+                                         int col, const f32x4 (&acc)[NI][4]) {
+    const int g = (threadIdx.x & 63) >> 4;
+    if (col >= a.n) return;
+    f32x4 b = {0.f, 0.f, 0.f, 0.f};
+    if (a.bias) {
+        const float* bias = a.bias + (long)rt.group * a.n + col;
+        if (WHOLE) {
+            b = *reinterpret_cast<const f32x4*>(bias);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (col + j < a.n) b[j] = bias[j];
+        }
+    }
+    with_activation(a.act, [&](auto act_tag) {
+        constexpr int ACT = decltype(act_tag)::value;
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+            const int r0 = row_w + 16 * i + 4 * g;
+            const long row = rt.row0 + r0;
+            f32x4 res[4];
+            if (a.res) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    if (r0 + r >= rows) continue;
+                    const long at = (row + r) * a.res_stride + col;
+                    if (!WHOLE) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            if (col + j < a.n) res[r][j] = load1(a.res, at + j, YK);
+                    } else if (YK == 0) {
+                        res[r] = *reinterpret_cast<const f32x4*>((const float*)a.res + at);
+                    } else {
+                        const uint2 q = *reinterpret_cast<const uint2*>((const uint16_t*)a.res + at);
+                        const uint32_t w[2] = {q.x, q.y};
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const uint16_t h = (uint16_t)(w[j >> 1] >> (16 * (j & 1)));
+                            res[r][j] = YK == 1 ? bf16_to_f32(h) : (float)__builtin_bit_cast(_Float16, h);
+                        }
+                    }
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                if (r0 + r >= rows) continue;
+                float v[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    v[j] = activate(acc[i][j][r] + b[j], ACT);
+                    if (a.res) v[j] += res[r][j];
+                }
+                const long at = (row + r) * a.y_stride + col;
+                if (WHOLE) {
+                    store4(a.y, at, v[0], v[1], v[2], v[3], YK);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (col + j < a.n) store1(a.y, at + j, v[j], YK);
+                }
+            }
+        }
+    });
+}
+
 // Any strides, alignment, n and k; fp32 activations.  Block tile 128x128,
 // k-step 32, four waves in a 2x2 grid of 64x64, both operands through registers
 // into double-buffered LDS.  XP: bf16 planes that stand for an fp32 x (0: x is of
@@ -263,15 +333,18 @@ MatmulPlan plan_matmul(const MatmulArgs& a, size_t workspace_bytes) {
         return p;
     }
     const long pitch = p.pack_x ? packed_planes(a) * packed_width(a) : a.x_stride;
-    if (!whole_pieces(a) || !room || 256 * pitch * 2 >= 0x7fffffffL || 256L * a.k * 2 >= 0x7fffffffL) {
+    const long out = std::max(a.y_stride, a.res ? a.res_stride : 0L) * (a.y_kind ? 2 : 4);
+    if (!room || 256 * pitch * 2 >= 0x7fffffffL || 256L * a.k * 2 >= 0x7fffffffL ||
+        256 * out >= 0x7fffffffL || (long)a.n * 4 >= 0x7fffffffL) {
         p.kernel = MatmulPlan::kAny;
         p.pack_x = p.pack_w = false;
         p.x_bytes = p.w_bytes = 0;
         return p;
     }
     p.kernel = MatmulPlan::kTiles;
+    p.whole = whole_pieces(a);
     const long steps = ((long)a.k + 63) / 64 * packed_planes(a);
-    const size_t each = (size_t)a.m * a.n * sizeof(float);
+    const size_t each = (size_t)a.m * round_up(a.n, 4) * sizeof(float);   // a range's sums
     const long most = a.offsets ? 1 : std::min<long>(16, (long)((workspace_bytes - p.bytes()) / each));
     double best = 0.;
     for (const TileCost& t : kTileCosts) {
