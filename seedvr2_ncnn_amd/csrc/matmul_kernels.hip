@@ -24,82 +24,12 @@ bool whole_pieces(const MatmulArgs& a) {
            (!a.res || (a.res_stride % 4 == 0 && (uintptr_t)a.res % e == 0));
 }
 
-// Epilogue of the kernel below, any strides: a wave's tile of NI x 16 rows and 64 columns, accumulator [i][j][r] is
-// row row_w + 16 i + 4 g + r of the block tile's `rows`, column col + j.  WHOLE: pieces
-// of four; else single elements.
-template <int YK, int NI, bool WHOLE>
-__device__ __forceinline__ void epilogue(const MatmulArgs& a, const RowTile& rt, int rows, int row_w,
-                                         int col, const f32x4 (&acc)[NI][4]) {
-    const int g = (threadIdx.x & 63) >> 4;
-    if (col >= a.n) return;
-    f32x4 b = {0.f, 0.f, 0.f, 0.f};
-    if (a.bias) {
-        const float* bias = a.bias + (long)rt.group * a.n + col;
-        if (WHOLE) {
-            b = *reinterpret_cast<const f32x4*>(bias);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (col + j < a.n) b[j] = bias[j];
-        }
-    }
-    with_activation(a.act, [&](auto act_tag) {
-        constexpr int ACT = decltype(act_tag)::value;
-#pragma unroll
-        for (int i = 0; i < NI; ++i) {
-            const int r0 = row_w + 16 * i + 4 * g;
-            const long row = rt.row0 + r0;
-            f32x4 res[4];
-            if (a.res) {
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    if (r0 + r >= rows) continue;
-                    const long at = (row + r) * a.res_stride + col;
-                    if (!WHOLE) {
-#pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            if (col + j < a.n) res[r][j] = load1(a.res, at + j, YK);
-                    } else if (YK == 0) {
-                        res[r] = *reinterpret_cast<const f32x4*>((const float*)a.res + at);
-                    } else {
-                        const uint2 q = *reinterpret_cast<const uint2*>((const uint16_t*)a.res + at);
-                        const uint32_t w[2] = {q.x, q.y};
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const uint16_t h = (uint16_t)(w[j >> 1] >> (16 * (j & 1)));
-                            res[r][j] = YK == 1 ? bf16_to_f32(h) : (float)__builtin_bit_cast(_Float16, h);
-                        }
-                    }
-                }
-            }
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                if (r0 + r >= rows) continue;
-                float v[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    v[j] = activate(acc[i][j][r] + b[j], ACT);
-                    if (a.res) v[j] += res[r][j];
-                }
-                const long at = (row + r) * a.y_stride + col;
-                if (WHOLE) {
-                    store4(a.y, at, v[0], v[1], v[2], v[3], YK);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        if (col + j < a.n) store1(a.y, at + j, v[j], YK);
-                }
-            }
-        }
-    });
-}
-
 // Any strides, alignment, n and k; fp32 activations.  Block tile 128x128,
 // k-step 32, four waves in a 2x2 grid of 64x64, both operands through registers
 // into double-buffered LDS.  XP: bf16 planes that stand for an fp32 x (0: x is of
 // the weight's type).  GRAN: elements loaded at once, 4 where rows allow it, or 1.
-template <int T, int XP, int GRAN, int YK, bool WHOLE>
-__global__ __launch_bounds__(256, 2) void matmul_any_kernel(MatmulArgs a, int ntiles) {
+template <int T, int XP, int GRAN, int YK>
+__global__ __launch_bounds__(256, 2) void matmul_any_kernel(MatmulArgs a, int ntiles, bool whole) {
     constexpr int BM = 128, BN = 128, BK = 32, P = BK + 8, PL = XP ? XP : 1;
     __shared__ __attribute__((aligned(16))) uint16_t x_lds[2][PL][BM * P];
     __shared__ __attribute__((aligned(16))) uint16_t w_lds[2][BN * P];
@@ -172,6 +102,7 @@ __global__ __launch_bounds__(256, 2) void matmul_any_kernel(MatmulArgs a, int nt
         }
     };
 
+    TileEnd<YK, 4> end(a, rt, rows, wm * 64, col0 + wn * 64 + 4 * l16, whole);
     f32x4 acc[4][4];   // [row tile][column tile]
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -201,7 +132,7 @@ __global__ __launch_bounds__(256, 2) void matmul_any_kernel(MatmulArgs a, int nt
         if (kt + 1 < nk) put(buf ^ 1);
         __syncthreads();
     }
-    epilogue<YK, 4, WHOLE>(a, rt, rows, wm * 64, col0 + wn * 64 + 4 * l16, acc);
+    end.finish(a, acc);
 }
 
 template <int T, int XP, int YK>
@@ -212,66 +143,75 @@ hipError_t launch_any(const MatmulArgs& a, hipStream_t stream) {
     const bool four = a.k % 4 == 0 && a.x_stride % 4 == 0 && (uintptr_t)a.x % (XP ? 16 : 8) == 0 &&
                       (uintptr_t)a.w % 8 == 0;
     const bool whole = whole_pieces(a);
-    const unsigned nb = (unsigned)blocks;
-    if (four && whole)
-        matmul_any_kernel<T, XP, 4, YK, true><<<nb, 256, 0, stream>>>(a, ntiles);
-    else if (four)
-        matmul_any_kernel<T, XP, 4, YK, false><<<nb, 256, 0, stream>>>(a, ntiles);
-    else if (whole)
-        matmul_any_kernel<T, XP, 1, YK, true><<<nb, 256, 0, stream>>>(a, ntiles);
+    if (four)
+        matmul_any_kernel<T, XP, 4, YK><<<(unsigned)blocks, 256, 0, stream>>>(a, ntiles, whole);
     else
-        matmul_any_kernel<T, XP, 1, YK, false><<<nb, 256, 0, stream>>>(a, ntiles);
+        matmul_any_kernel<T, XP, 1, YK><<<(unsigned)blocks, 256, 0, stream>>>(a, ntiles, whole);
     return hipGetLastError();
 }
 
-// Rows for the tile kernels, eight elements a thread: [rows][PL][width] from
-// [rows][k], zeros from k to width.  KIND 0: fp32 as PL bf16 terms; else 16-bit
-// elements as they are.  VEC: rows in 16-byte pieces.
-template <int KIND, int PL, bool VEC>
-__global__ __launch_bounds__(256) void matmul_pack_kernel(const void* __restrict__ src, long stride,
-                                                          long rows, int k, int width,
-                                                          uint16_t* __restrict__ dst) {
-    const int pieces = width / 8;
-    const long all = rows * pieces;
-    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < all; i += (long)gridDim.x * 256) {
-        const long row = i / pieces;
-        const int kc = (int)(i - row * pieces) * 8;
-        uint16_t* out = dst + row * PL * width + kc;
-        if constexpr (KIND == 0) {
-            float v[8];
-            piece32<VEC ? 4 : 1, false>((const float*)src + row * stride + kc, k - kc, v);
-            uint4 h[PL];
-            split8<PL>(v, h);
+// Rows for the tile kernels: [rows][planes][width] from [rows][k], zeros from k to
+// width, in pieces of eight elements.  An fp32 row is packed as `planes` bf16 terms, a
+// 16-bit one as it is, `planes` times.
+struct PackJob {
+    const void* src;
+    int kind;           // 0 fp32, else 16 bits
+    bool vec;           // source rows in pieces of four elements
+    long stride, rows;
+    int planes, width;
+    uint16_t* dst;
+};
+
+template <int PL, bool VEC>
+__device__ __forceinline__ void pack_piece(const PackJob& job, int k, long i) {
+    const int pieces = job.width / 8;
+    const long row = i / pieces;
+    const int kc = (int)(i - row * pieces) * 8;
+    uint16_t* out = job.dst + row * job.planes * job.width + kc;
+    if (job.kind == 0) {
+        float v[8];
+        uint4 h[PL];
+        piece32<VEC ? 4 : 1, false>((const float*)job.src + row * job.stride + kc, k - kc, v);
+        split8<PL>(v, h);
 #pragma unroll
-            for (int q = 0; q < PL; ++q) *reinterpret_cast<uint4*>(out + (long)q * width) = h[q];
+        for (int q = 0; q < PL; ++q) *reinterpret_cast<uint4*>(out + (long)q * job.width) = h[q];
+    } else {
+        const uint4 h = piece16<VEC ? 4 : 1, false>((const uint16_t*)job.src + row * job.stride + kc, k - kc);
+        for (int q = 0; q < job.planes; ++q) *reinterpret_cast<uint4*>(out + (long)q * job.width) = h;
+    }
+}
+
+// x, then the weight, either of which may have no rows.
+template <int PL>
+__global__ __launch_bounds__(256) void matmul_pack_kernel(PackJob x, PackJob w, int k) {
+    const long nx = x.rows * (x.width / 8), all = nx + w.rows * (w.width / 8);
+    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < all; i += (long)gridDim.x * 256) {
+        if (i < nx) {
+            if (x.vec)
+                pack_piece<PL, true>(x, k, i);
+            else
+                pack_piece<PL, false>(x, k, i);
+        } else if (w.vec) {
+            pack_piece<PL, true>(w, k, i - nx);
         } else {
-            *reinterpret_cast<uint4*>(out) =
-                piece16<VEC ? 4 : 1, false>((const uint16_t*)src + row * stride + kc, k - kc);
+            pack_piece<PL, false>(w, k, i - nx);
         }
     }
 }
 
-hipError_t launch_pack(const void* src, int kind, long stride, long rows, int k, int planes, int width,
-                       uint16_t* dst, hipStream_t stream) {
-    const long pieces = rows * (width / 8);
-    const unsigned nb = (unsigned)std::min<long>((pieces + 255) / 256, 65536);
-    const bool vec = k % 4 == 0 && stride % 4 == 0 && (uintptr_t)src % (kind ? 8 : 16) == 0;
-    if (kind) {
-        if (vec)
-            matmul_pack_kernel<1, 1, true><<<nb, 256, 0, stream>>>(src, stride, rows, k, width, dst);
-        else
-            matmul_pack_kernel<1, 1, false><<<nb, 256, 0, stream>>>(src, stride, rows, k, width, dst);
-    } else if (planes == 3) {
-        if (vec)
-            matmul_pack_kernel<0, 3, true><<<nb, 256, 0, stream>>>(src, stride, rows, k, width, dst);
-        else
-            matmul_pack_kernel<0, 3, false><<<nb, 256, 0, stream>>>(src, stride, rows, k, width, dst);
-    } else {
-        if (vec)
-            matmul_pack_kernel<0, 2, true><<<nb, 256, 0, stream>>>(src, stride, rows, k, width, dst);
-        else
-            matmul_pack_kernel<0, 2, false><<<nb, 256, 0, stream>>>(src, stride, rows, k, width, dst);
-    }
+PackJob pack_job(const void* src, int kind, long stride, long rows, int k, int planes, int width,
+                 uint16_t* dst) {
+    return PackJob{src, kind, k % 4 == 0 && stride % 4 == 0 && (uintptr_t)src % (kind ? 8 : 16) == 0,
+                   stride, rows, planes, width, dst};
+}
+
+hipError_t launch_pack(const PackJob& x, const PackJob& w, int k, hipStream_t stream) {
+    const long all = x.rows * (x.width / 8) + w.rows * (w.width / 8);
+    const unsigned nb = (unsigned)std::min<long>((all + 255) / 256, 65536);
+    if (x.planes == 3)
+        matmul_pack_kernel<3><<<nb, 256, 0, stream>>>(x, w, k);
+    else
+        matmul_pack_kernel<2><<<nb, 256, 0, stream>>>(x, w, k);
     return hipGetLastError();
 }
 
@@ -303,9 +243,13 @@ constexpr double kSumBytesUs = 9e6;
 
 long round_up(long v, long to) { return (v + to - 1) / to * to; }
 
-// Packed rows: bf16 terms of an fp32 x, and their pitch.
+// bf16 terms of an fp32 x
 int packed_planes(const MatmulArgs& a) { return a.x_kind ? 1 : a.y_kind ? 2 : 3; }
-long packed_width(const MatmulArgs& a) { return round_up(a.k, 64); }
+
+// Elements of a packed plane.  Where the weight is packed too it is repeated for each
+// plane of x, so that the planes are one longer row; else its rows are read once for
+// each plane, in steps of 64 k that x has to fill.
+long packed_width(const MatmulArgs& a, bool pack_w) { return round_up(a.k, pack_w ? 8 : 64); }
 
 // 16-byte rows of 16-bit elements
 bool rows16(const void* p, long stride) { return stride % 8 == 0 && (uintptr_t)p % 16 == 0; }
@@ -319,8 +263,10 @@ MatmulPlan plan_matmul(const MatmulArgs& a, size_t workspace_bytes) {
     // what the tile kernels need: 16-byte rows, packed here where a call's are not
     p.pack_x = a.x_kind == 0 || a.k % 8 != 0 || !rows16(a.x, a.x_stride);
     p.pack_w = a.k % 8 != 0 || (uintptr_t)a.w % 16 != 0;
-    if (p.pack_x) p.x_bytes = round_up((size_t)a.m * packed_planes(a) * packed_width(a) * 2, 256);
-    if (p.pack_w) p.w_bytes = round_up((size_t)a.groups * a.n * round_up(a.k, 8) * 2, 256);
+    const long row = packed_planes(a) * packed_width(a, p.pack_w);
+    if (p.pack_w) p.pack_x = true;   // a weight of padded rows needs padded x
+    if (p.pack_x) p.x_bytes = round_up((size_t)a.m * row * 2, 256);
+    if (p.pack_w) p.w_bytes = round_up((size_t)a.groups * a.n * row * 2, 256);
     const bool room = p.bytes() <= workspace_bytes;
     if (rows <= 32) {
         p.kernel = MatmulPlan::kRows;
@@ -332,18 +278,20 @@ MatmulPlan plan_matmul(const MatmulArgs& a, size_t workspace_bytes) {
         p.w_bytes = 0;
         return p;
     }
-    const long pitch = p.pack_x ? packed_planes(a) * packed_width(a) : a.x_stride;
+    const long pitch = p.pack_x ? row : a.x_stride;
     const long out = std::max(a.y_stride, a.res ? a.res_stride : 0L) * (a.y_kind ? 2 : 4);
-    if (!room || 256 * pitch * 2 >= 0x7fffffffL || 256L * a.k * 2 >= 0x7fffffffL ||
-        256 * out >= 0x7fffffffL || (long)a.n * 4 >= 0x7fffffffL) {
-        p.kernel = MatmulPlan::kAny;
+    const bool near = 256 * out < 0x7fffffffL && (long)a.n * 4 < 0x7fffffffL;   // 32-bit offsets
+    if (!near || !room || 256 * pitch * 2 >= 0x7fffffffL ||
+        256 * std::max<long>(a.k, p.pack_w ? row : 0) * 2 >= 0x7fffffffL) {
+        p.kernel = near ? MatmulPlan::kAny : MatmulPlan::kRows;
+        p.rows = 64;
         p.pack_x = p.pack_w = false;
         p.x_bytes = p.w_bytes = 0;
         return p;
     }
     p.kernel = MatmulPlan::kTiles;
     p.whole = whole_pieces(a);
-    const long steps = ((long)a.k + 63) / 64 * packed_planes(a);
+    const long steps = p.pack_w ? (row + 63) / 64 : ((long)a.k + 63) / 64 * packed_planes(a);
     const size_t each = (size_t)a.m * round_up(a.n, 4) * sizeof(float);   // a range's sums
     const long most = a.offsets ? 1 : std::min<long>(16, (long)((workspace_bytes - p.bytes()) / each));
     double best = 0.;
@@ -381,26 +329,23 @@ hipError_t launch_matmul(const MatmulArgs& args, void* workspace, size_t workspa
     const MatmulPlan p = plan_matmul(a, workspace_bytes);
     char* at = (char*)workspace;
     if (p.pack_x) {
-        const int planes = packed_planes(a);
-        const long width = packed_width(a);
-        const hipError_t e = launch_pack(a.x, a.x_kind, a.x_stride, a.m, a.k, planes, (int)width,
-                                         (uint16_t*)at, stream);
+        const int planes = packed_planes(a), width = (int)packed_width(a, p.pack_w);
+        const PackJob x = pack_job(a.x, a.x_kind, a.x_stride, a.m, a.k, planes, width, (uint16_t*)at);
+        const PackJob w = pack_job(a.w, a.w_kind, a.k, p.pack_w ? (long)a.groups * a.n : 0, a.k, planes,
+                                   width, (uint16_t*)(at + p.x_bytes));
+        const hipError_t e = launch_pack(x, w, a.k, stream);
         if (e != hipSuccess) return e;
-        a.x = at;
+        a.x = x.dst;
         a.x_kind = a.w_kind;
-        a.x_stride = planes * width;
-        a.planes = planes;
-        a.plane = width;
-        at += p.x_bytes;
-    }
-    if (p.pack_w) {
-        const int width = (int)round_up(a.k, 8);
-        const hipError_t e = launch_pack(a.w, a.w_kind, a.k, (long)a.groups * a.n, a.k, 1, width,
-                                         (uint16_t*)at, stream);
-        if (e != hipSuccess) return e;
-        a.w = at;
-        a.k = width;
-        at += p.w_bytes;
+        a.x_stride = (long)planes * width;
+        if (p.pack_w) {   // one long row
+            a.w = w.dst;
+            a.k = planes * width;
+        } else {
+            a.planes = planes;
+            a.plane = width;
+        }
+        at += p.x_bytes + p.w_bytes;
     }
     switch (p.kernel) {
         case MatmulPlan::kRows: return launch_matmul_rows(a, p.rows, stream);
