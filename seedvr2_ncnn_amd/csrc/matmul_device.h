@@ -28,19 +28,34 @@ struct RowTile {
     int row0, end, group;
 };
 
+// Group g's rows, kept to [0, m] whatever the offsets hold, and its tiles of tm rows.
+__device__ __forceinline__ int group_tiles(const MatmulArgs& a, int g, int tm, int& start, int& end) {
+    start = end = 0;
+    if (g < a.groups) {
+        start = max(a.offsets[g], 0);
+        end = min(a.offsets[g + 1], a.m);
+    }
+    return end > start ? (end - start + tm - 1) / tm : 0;
+}
+
+// Tiles of tm rows that there are; mtiles is what there can be.  Every wave counts for
+// itself, 64 groups at a time.
+__device__ __forceinline__ int count_row_tiles(const MatmulArgs& a, int tm, int mtiles) {
+    if (!a.offsets) return mtiles;
+    int sum = 0, start, end;
+    for (int g = threadIdx.x & 63; g < a.groups; g += 64) sum += group_tiles(a, g, tm, start, end);
+#pragma unroll
+    for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
+    // (offsets that descend can make more of them than the grid has workgroups for)
+    return min(__builtin_amdgcn_readfirstlane(sum), mtiles);
+}
+
 __device__ __forceinline__ RowTile row_tile(const MatmulArgs& a, int t, int tm) {
     if (!a.offsets) return RowTile{t * tm, a.m, 0};
-    // every wave counts the groups' tiles, 64 groups at a time; offsets are kept
-    // to [0, m], whatever they hold
     const int lane = threadIdx.x & 63;
     for (int g0 = 0; g0 < a.groups; g0 += 64) {
-        const int g = g0 + lane;
-        int start = 0, end = 0;
-        if (g < a.groups) {
-            start = max(a.offsets[g], 0);
-            end = min(a.offsets[g + 1], a.m);
-        }
-        const int tiles = end > start ? (end - start + tm - 1) / tm : 0;
+        int start, end;
+        const int tiles = group_tiles(a, g0 + lane, tm, start, end);
         int upto = tiles;   // tiles of the groups up to this one
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {

@@ -10,6 +10,8 @@
 //
 // This file: which kernel takes a call, the packing of rows that the tile kernels
 // cannot read, and the kernel for any shape and alignment.
+#include <cmath>
+
 #include "matmul_device.h"
 
 namespace s2 {
@@ -33,7 +35,9 @@ __global__ __launch_bounds__(256, 2) void matmul_any_kernel(MatmulArgs a, int nt
     constexpr int BM = 128, BN = 128, BK = 32, P = BK + 8, PL = XP ? XP : 1;
     __shared__ __attribute__((aligned(16))) uint16_t x_lds[2][PL][BM * P];
     __shared__ __attribute__((aligned(16))) uint16_t w_lds[2][BN * P];
-    const int lid = xcd_remap(blockIdx.x, gridDim.x);
+    const int blocks = count_row_tiles(a, BM, gridDim.x / ntiles) * ntiles;
+    if ((int)blockIdx.x >= blocks) return;   // the whole workgroup
+    const int lid = xcd_remap(blockIdx.x, blocks);
     const RowTile rt = row_tile(a, lid / ntiles, BM);
     const int col0 = lid % ntiles * BN;
     const int rows = min(rt.end - rt.row0, BM);
@@ -224,22 +228,33 @@ hipError_t launch_any_y(const MatmulArgs& a, hipStream_t stream) {
 
 constexpr int kUnits = 256;   // compute units of an MI355X
 
-// What a tile takes, in microseconds, from which the tile and the ranges of k are
-// chosen: `start` with its launch, first loads and epilogue, `step` for 64 k, of a
-// compute unit that holds one such tile or more.  Measured with bf16 rows, 72 to 2048
-// of them, k of 256 to 10240 and n of 512 to 15360.  The choice against the best of
-// these tiles and 1 to 12 ranges: 77 x 5120 by 2560 x 5120 15 us either way (one range
-// of 128 x 128: 48); 512 x 512 by 512 x 512 6.5 (128 x 128: 11); 1024 x 2560 by
-// 2560 x 2560 28 (256 x 256: 51); 2048 x 2560 by 15360 x 2560 136 (128 x 128: 186).
+// What tiles take, in microseconds, from which the tile and the ranges of k are
+// chosen: a compute unit holds `each` workgroups of a kind at once; such a round costs
+// `round` for first loads and epilogues and, for 64 k, `one` step of a single workgroup
+// or `full` of all of them.  Measured with bf16 rows, 72 to 2048 of them, k of 256 to
+// 10240 and n of 512 to 15360.  Against the best of the four tiles and 1 to 12 ranges:
+// 77 x 5120 by 2560 x 5120 15 us either way (one range of 128 x 128: 48); 512 x 512 by
+// 512 x 512 6.5 (128 x 128: 11); 14400 x 512 by 512 x 512 15 (256 x 256: 19); 1024 x
+// 2560 by 2560 x 2560 28 (256 x 256: 47); 2048 x 2560 by 15360 x 2560 136 (128 x 128:
+// 186).
 struct TileCost {
-    int bm, bn;
-    double start, step;
+    int bm, bn, each;
+    double round, one, full;
 };
-constexpr TileCost kTileCosts[] = {
-    {256, 256, 9.5, 1.3}, {128, 128, 7., 0.57}, {128, 64, 5.3, 0.38}, {64, 64, 4., 0.3}};
+constexpr TileCost kTileCosts[] = {{256, 256, 1, 6.5, 1.3, 1.3},
+                                   {128, 128, 2, 4.5, 0.57, 0.88},
+                                   {128, 64, 2, 3.5, 0.38, 0.57},
+                                   {64, 64, 2, 2.5, 0.3, 0.45}};
 
-// Bytes a microsecond at which the sums of k ranges are written and read again.
-constexpr double kSumBytesUs = 9e6;
+double tiles_us(const TileCost& t, double blocks, double steps) {
+    const double slots = (double)kUnits * t.each;
+    const double rounds = std::floor(blocks / slots), rest = blocks - rounds * slots;
+    return rounds * (t.round + steps * t.full) +
+           (rest > 0 ? t.round + steps * (rest <= kUnits ? t.one : t.full) : 0.);
+}
+
+// The sums of k ranges: a launch, and bytes a microsecond written and read again.
+constexpr double kSumUs = 3., kSumBytesUs = 9e6;
 
 long round_up(long v, long to) { return (v + to - 1) / to * to; }
 
@@ -301,9 +316,8 @@ MatmulPlan plan_matmul(const MatmulArgs& a, size_t workspace_bytes) {
                                         : (double)row_tiles(a, t.bm)) *
                              (double)((a.n + t.bn - 1) / t.bn);
         for (long parts = 1; parts <= std::max<long>(1, std::min(most, steps / 4)); ++parts) {
-            const double each_unit = std::max(1., tiles * parts / kUnits);
-            const double us = t.start + each_unit * t.step * ((double)steps / parts) +
-                              (parts > 1 ? 3. + 2. * parts * each / kSumBytesUs : 0.);
+            const double us = tiles_us(t, tiles * parts, (double)steps / parts) +
+                              (parts > 1 ? kSumUs + 2. * parts * each / kSumBytesUs : 0.);
             if (best == 0. || us < best) {
                 best = us;
                 p.bm = t.bm;
