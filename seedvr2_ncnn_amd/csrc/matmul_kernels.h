@@ -47,7 +47,7 @@ inline long row_tiles(const MatmulArgs& a, int tm) {
 // A call's kernel and what it keeps in the workspace.
 struct MatmulPlan {
     enum Kernel { kRows, kTiles, kAny } kernel;
-    int rows;              // kRows: rows of a tile, 16, 32 or 64
+    int rows, cols;        // kRows: of a tile, 16, 32 or 64 each
     int bm, bn;            // kTiles: the tile
     int parts;             // kTiles: ranges of k
     bool whole;            // kTiles: y and residual in pieces of four columns
@@ -64,6 +64,6 @@ hipError_t launch_matmul(const MatmulArgs& a, void* workspace, size_t workspace_
 // The kernels' own launchers, for calls that plan_matmul gives them.
 hipError_t launch_matmul_tiles(const MatmulArgs& a, const MatmulPlan& plan, float* sums,
                                hipStream_t stream);
-hipError_t launch_matmul_rows(const MatmulArgs& a, int rows, hipStream_t stream);
+hipError_t launch_matmul_rows(const MatmulArgs& a, const MatmulPlan& plan, hipStream_t stream);
 
 }  // namespace s2

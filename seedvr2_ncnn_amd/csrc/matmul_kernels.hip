@@ -256,6 +256,18 @@ double tiles_us(const TileCost& t, double blocks, double steps) {
 // The sums of k ranges: a launch, and bytes a microsecond written and read again.
 constexpr double kSumUs = 3., kSumBytesUs = 9e6;
 
+// Reading the weight once, at 5 TB/s.
+double weight_us(const MatmulArgs& a) {
+    return (double)std::min(a.groups, a.m) * a.n * a.k * 2 / 5e6;
+}
+
+// A call on the rows kernel: a workgroup gets its weight rows and its rows of x through
+// the caches at about 30 KB a microsecond.
+double rows_us(const MatmulArgs& a, const MatmulPlan& r, long rows) {
+    const double blocks = (double)row_tiles(a, r.rows) * ((a.n + r.cols - 1) / r.cols);
+    return std::max(1., blocks / kUnits) * (r.cols + rows) * (double)a.k * 2 / 30e3;
+}
+
 long round_up(long v, long to) { return (v + to - 1) / to * to; }
 
 // bf16 terms of an fp32 x
@@ -278,56 +290,71 @@ MatmulPlan plan_matmul(const MatmulArgs& a, size_t workspace_bytes) {
     // what the tile kernels need: 16-byte rows, packed here where a call's are not
     p.pack_x = a.x_kind == 0 || a.k % 8 != 0 || !rows16(a.x, a.x_stride);
     p.pack_w = a.k % 8 != 0 || (uintptr_t)a.w % 16 != 0;
+    const bool direct = !p.pack_x && !p.pack_w;
     const long row = packed_planes(a) * packed_width(a, p.pack_w);
     if (p.pack_w) p.pack_x = true;   // a weight of padded rows needs padded x
     if (p.pack_x) p.x_bytes = round_up((size_t)a.m * row * 2, 256);
     if (p.pack_w) p.w_bytes = round_up((size_t)a.groups * a.n * row * 2, 256);
     const bool room = p.bytes() <= workspace_bytes;
-    if (rows <= 32) {
-        p.kernel = MatmulPlan::kRows;
-        p.rows = rows <= 16 ? 16 : 32;
-        // fp32 rows are split here, once, where there are more than a few of them
-        if (!(a.x_kind == 0 && rows > 16 && !p.pack_w && room)) p.pack_x = false;
-        p.pack_w = false;
-        if (!p.pack_x) p.x_bytes = 0;
-        p.w_bytes = 0;
-        return p;
-    }
     const long pitch = p.pack_x ? row : a.x_stride;
     const long out = std::max(a.y_stride, a.res ? a.res_stride : 0L) * (a.y_kind ? 2 : 4);
     const bool near = 256 * out < 0x7fffffffL && (long)a.n * 4 < 0x7fffffffL;   // 32-bit offsets
-    if (!near || !room || 256 * pitch * 2 >= 0x7fffffffL ||
-        256 * std::max<long>(a.k, p.pack_w ? row : 0) * 2 >= 0x7fffffffL) {
-        p.kernel = near ? MatmulPlan::kAny : MatmulPlan::kRows;
-        p.rows = 64;
-        p.pack_x = p.pack_w = false;
-        p.x_bytes = p.w_bytes = 0;
-        return p;
-    }
-    p.kernel = MatmulPlan::kTiles;
-    p.whole = whole_pieces(a);
-    const long steps = p.pack_w ? (row + 63) / 64 : ((long)a.k + 63) / 64 * packed_planes(a);
-    const size_t each = (size_t)a.m * round_up(a.n, 4) * sizeof(float);   // a range's sums
-    const long most = a.offsets ? 1 : std::min<long>(16, (long)((workspace_bytes - p.bytes()) / each));
-    double best = 0.;
-    for (const TileCost& t : kTileCosts) {
-        // a group's last tile is half empty, on average
-        const double tiles = (a.offsets ? (double)a.m / t.bm + 0.5 * std::min(a.groups, a.m)
-                                        : (double)row_tiles(a, t.bm)) *
-                             (double)((a.n + t.bn - 1) / t.bn);
-        for (long parts = 1; parts <= std::max<long>(1, std::min(most, steps / 4)); ++parts) {
-            const double us = tiles_us(t, tiles * parts, (double)steps / parts) +
-                              (parts > 1 ? kSumUs + 2. * parts * each / kSumBytesUs : 0.);
-            if (best == 0. || us < best) {
-                best = us;
-                p.bm = t.bm;
-                p.bn = t.bn;
-                p.parts = (int)parts;
+    const bool tiles = near && room && 256 * pitch * 2 < 0x7fffffffL &&
+                       256 * std::max<long>(a.k, p.pack_w ? row : 0) * 2 < 0x7fffffffL;
+
+    double tile_us = 0.;
+    if (tiles) {
+        p.kernel = MatmulPlan::kTiles;
+        p.whole = whole_pieces(a);
+        const long steps = p.pack_w ? (row + 63) / 64 : ((long)a.k + 63) / 64 * packed_planes(a);
+        const size_t each = (size_t)a.m * round_up(a.n, 4) * sizeof(float);   // a range's sums
+        const long most =
+            a.offsets ? 1 : std::min<long>(16, (long)((workspace_bytes - p.bytes()) / each));
+        for (const TileCost& t : kTileCosts) {
+            // a group's last tile is half empty, on average
+            const double count = (a.offsets ? (double)a.m / t.bm + 0.5 * std::min(a.groups, a.m)
+                                            : (double)row_tiles(a, t.bm)) *
+                                 (double)((a.n + t.bn - 1) / t.bn);
+            for (long parts = 1; parts <= std::max<long>(1, std::min(most, steps / 4)); ++parts) {
+                const double us =
+                    std::max(tiles_us(t, count * parts, (double)steps / parts), weight_us(a)) +
+                    (parts > 1 ? kSumUs + 2. * parts * each / kSumBytesUs : 0.);
+                if (tile_us == 0. || us < tile_us) {
+                    tile_us = us;
+                    p.bm = t.bm;
+                    p.bn = t.bn;
+                    p.parts = (int)parts;
+                }
             }
         }
+        if (p.parts > 1) p.sum_bytes = p.parts * each;
+        if (rows > 32) return p;
     }
-    if (p.parts > 1) p.sum_bytes = p.parts * each;
-    return p;
+
+    // few rows
+    MatmulPlan r{};
+    r.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+    // the more columns a workgroup has, the fewer times x is read from the L2; as long as
+    // three quarters of the compute units have one (1 x 2560 by 15360 x 2560: 19.0 us by
+    // 16 columns, 15.9 by 32, 14.9 by 64; by 2560 x 2560: 6.8, 9.2, 13.2)
+    const long row_blocks = row_tiles(a, r.rows);
+    r.cols = 16;
+    for (int c : {32, 64})
+        if (row_blocks * ((a.n + c - 1) / c) >= kUnits * 3 / 4) r.cols = c;
+    if (rows <= 32) {
+        r.kernel = MatmulPlan::kRows;
+        r.parts = 1;
+        // against the tiles where those need no packing (16 x 10240 by 2560 x 10240 15 us
+        // on tiles, 22 on rows; 1 x 10240 18 and 15); more than a few fp32 rows are packed
+        // rather than split by every workgroup (32 x 2560 by 2560 x 2560 20 and 22)
+        const bool use_tiles = direct ? tile_us < rows_us(a, r, std::min(rows, (long)a.m))
+                                      : a.x_kind == 0 && rows > 16 && !p.pack_w;
+        return tiles && use_tiles ? p : r;
+    }
+    // any shape, without a workspace; rows that 32-bit offsets do not reach
+    r.kernel = near ? MatmulPlan::kAny : MatmulPlan::kRows;
+    r.parts = 1;
+    return r;
 }
 
 hipError_t launch_matmul(const MatmulArgs& args, void* workspace, size_t workspace_bytes,
@@ -362,7 +389,7 @@ hipError_t launch_matmul(const MatmulArgs& args, void* workspace, size_t workspa
         at += p.x_bytes + p.w_bytes;
     }
     switch (p.kernel) {
-        case MatmulPlan::kRows: return launch_matmul_rows(a, p.rows, stream);
+        case MatmulPlan::kRows: return launch_matmul_rows(a, p, stream);
         case MatmulPlan::kTiles: return launch_matmul_tiles(a, p, (float*)at, stream);
         default:
             return a.y_kind == 0   ? launch_any_y<0>(a, stream)

@@ -11,12 +11,12 @@ namespace {
 // x comes from the caches.  The waves' sums meet in LDS.  Rows and columns past the end
 // repeat the last one, and are dropped.
 //
-// PL terms stand for a value of x: SPLIT, made here from fp32 (few rows), or read from
-// the planes of packed rows.
-template <int T, int PL, bool SPLIT, int MT, int NT, int GRAN>
+// PL bf16 terms stand for a value of an fp32 x, split here by every workgroup; 1: x is of
+// the weight's type.
+template <int T, int PL, int MT, int NT, int GRAN>
 __global__ __launch_bounds__(512) void matmul_rows_kernel(MatmulArgs a, int ntiles) {
-    constexpr int XL = SPLIT ? 1 : PL;                      // loaded pieces of a row
-    constexpr int REGS = 2 * 4 * (NT + MT * (SPLIT ? 2 : PL));   // of a 64-k chunk
+    constexpr bool SPLIT = PL > 1;
+    constexpr int REGS = 2 * 4 * (NT + MT * (SPLIT ? 2 : 1));   // of a 64-k chunk
     constexpr int U = REGS >= 40 ? 1 : REGS >= 24 ? 2 : 4;  // chunks of a batch
     constexpr bool TWO = U * REGS <= 80;                    // the next batch in flight
     __shared__ float sums[8][MT * NT * 256];
@@ -45,7 +45,7 @@ __global__ __launch_bounds__(512) void matmul_rows_kernel(MatmulArgs a, int ntil
     // C chunks of 64 k, waves * 64 apart
     struct Batch {
         uint4 w[2 * U][NT];
-        uint4 x[SPLIT ? 1 : 2 * U][SPLIT ? 1 : MT][XL];
+        uint4 x[SPLIT ? 1 : 2 * U][SPLIT ? 1 : MT];
         float f[SPLIT ? 2 * U : 1][SPLIT ? MT : 1][8];
     };
     auto load = [&](Batch& b, int k0, auto count, auto full) {
@@ -59,14 +59,10 @@ __global__ __launch_bounds__(512) void matmul_rows_kernel(MatmulArgs a, int ntil
             for (int j = 0; j < NT; ++j) b.w[c][j] = piece16<GRAN, FULL>(w[j] + kc, left);
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
-                if constexpr (SPLIT) {
+                if constexpr (SPLIT)
                     piece32<GRAN, FULL>((const float*)a.x + xo[i] + kc, left, b.f[c][i]);
-                } else {
-#pragma unroll
-                    for (int q = 0; q < PL; ++q)
-                        b.x[c][i][q] =
-                            piece16<GRAN, FULL>((const uint16_t*)a.x + xo[i] + q * a.plane + kc, left);
-                }
+                else
+                    b.x[c][i] = piece16<GRAN, FULL>((const uint16_t*)a.x + xo[i] + kc, left);
             }
         }
     };
@@ -77,12 +73,10 @@ __global__ __launch_bounds__(512) void matmul_rows_kernel(MatmulArgs a, int ntil
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
                 uint4 t[PL];
-                if constexpr (SPLIT) {
+                if constexpr (SPLIT)
                     split8<PL>(b.f[c][i], t);
-                } else {
-#pragma unroll
-                    for (int q = 0; q < PL; ++q) t[q] = b.x[c][i][q];
-                }
+                else
+                    t[0] = b.x[c][i];
 #pragma unroll
                 for (int q = 0; q < PL; ++q)
 #pragma unroll
@@ -154,52 +148,41 @@ int row_gran(const MatmulArgs& a) {
     return 1;
 }
 
-template <int T, int PL, bool SPLIT, int MT, int NT, int GRAN>
+template <int T, int PL, int MT, int NT, int GRAN>
 hipError_t run(const MatmulArgs& a, hipStream_t stream) {
     const int ntiles = (a.n + 16 * NT - 1) / (16 * NT);
     const long blocks = row_tiles(a, 16 * MT) * ntiles;
     if (blocks > 0x7fffffffL) return hipErrorInvalidValue;
     const int waves = std::min(8, (a.k + 63) / 64);
-    matmul_rows_kernel<T, PL, SPLIT, MT, NT, GRAN><<<(unsigned)blocks, 64 * waves, 0, stream>>>(a, ntiles);
+    matmul_rows_kernel<T, PL, MT, NT, GRAN><<<(unsigned)blocks, 64 * waves, 0, stream>>>(a, ntiles);
     return hipGetLastError();
 }
 
-template <int T, int PL, bool SPLIT, int MT>
-hipError_t pick(const MatmulArgs& a, hipStream_t stream) {
+template <int T, int PL, int MT>
+hipError_t pick(const MatmulArgs& a, int cols, hipStream_t stream) {
     const int gran = row_gran(a);
     if (gran == 8) {
         constexpr int MOST = MT * PL <= 4 ? 4 : 2;   // by registers
-        const long tiles = row_tiles(a, 16 * MT);
-        // the more columns a workgroup has, the fewer times x is read from the L2; as
-        // long as three quarters of the compute units have one (1 x 2560 by 15360 x 2560:
-        // 19.0 us by 16 columns, 15.9 by 32, 14.9 by 64; by 2560 x 2560: 6.8, 9.2, 13.2)
-        if (tiles * ((a.n + 63) / 64) >= 192) return run<T, PL, SPLIT, MT, MOST, 8>(a, stream);
-        if (tiles * ((a.n + 31) / 32) >= 192) return run<T, PL, SPLIT, MT, 2, 8>(a, stream);
-        return run<T, PL, SPLIT, MT, 1, 8>(a, stream);
+        if (cols == 64) return run<T, PL, MT, MOST, 8>(a, stream);
+        if (cols == 32) return run<T, PL, MT, 2, 8>(a, stream);
+        return run<T, PL, MT, 1, 8>(a, stream);
     }
-    if constexpr (PL > 1 && !SPLIT) {
-        return hipErrorInvalidValue;   // packed rows are 16-byte rows
-    } else {
-        return gran == 4 ? run<T, PL, SPLIT, MT, 1, 4>(a, stream) : run<T, PL, SPLIT, MT, 1, 1>(a, stream);
-    }
+    return gran == 4 ? run<T, PL, MT, 1, 4>(a, stream) : run<T, PL, MT, 1, 1>(a, stream);
 }
 
-template <int T, int PL, bool SPLIT>
-hipError_t pick_rows(const MatmulArgs& a, int rows, hipStream_t stream) {
-    return rows == 16   ? pick<T, PL, SPLIT, 1>(a, stream)
-           : rows == 32 ? pick<T, PL, SPLIT, 2>(a, stream)
-                        : pick<T, PL, SPLIT, 4>(a, stream);
+template <int T, int PL>
+hipError_t pick_rows(const MatmulArgs& a, const MatmulPlan& plan, hipStream_t stream) {
+    return plan.rows == 16   ? pick<T, PL, 1>(a, plan.cols, stream)
+           : plan.rows == 32 ? pick<T, PL, 2>(a, plan.cols, stream)
+                             : pick<T, PL, 4>(a, plan.cols, stream);
 }
 
 }  // namespace
 
-hipError_t launch_matmul_rows(const MatmulArgs& a, int rows, hipStream_t stream) {
-    if (a.w_kind == 2) return pick_rows<2, 1, false>(a, rows, stream);
-    if (a.x_kind == 0)
-        return a.y_kind == 0 ? pick_rows<1, 3, true>(a, rows, stream) : pick_rows<1, 2, true>(a, rows, stream);
-    if (a.planes == 2) return pick_rows<1, 2, false>(a, rows, stream);
-    if (a.planes == 3) return pick_rows<1, 3, false>(a, rows, stream);
-    return pick_rows<1, 1, false>(a, rows, stream);
+hipError_t launch_matmul_rows(const MatmulArgs& a, const MatmulPlan& plan, hipStream_t stream) {
+    if (a.w_kind == 2) return pick_rows<2, 1>(a, plan, stream);
+    if (a.x_kind) return pick_rows<1, 1>(a, plan, stream);
+    return a.y_kind == 0 ? pick_rows<1, 3>(a, plan, stream) : pick_rows<1, 2>(a, plan, stream);
 }
 
 }  // namespace s2
