@@ -706,20 +706,38 @@ def _on_current_device(x, *others):
         raise ValueError("operands must be on the current device")
 
 
+def _empty(shape, dtype, x, stream):
+    """An uninitialised tensor beside x, whose memory belongs to the stream that the
+    call runs on."""
+    import torch
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=x.device)
+    with torch.cuda.stream(stream):
+        return torch.empty(shape, dtype=dtype, device=x.device)
+
+
+def _workspace(workspace, stream, x, size, *sizes):
+    """(workspace or None, bytes): the caller's, or size(*sizes) bytes made here."""
+    if workspace is not None:
+        return workspace, workspace.numel() * workspace.element_size()
+    import torch
+    n = size(*sizes)
+    return (_empty(n, torch.uint8, x, stream) if n else None), n
+
+
 def group_norm(x, groups, gamma=None, beta=None, epsilon=1e-6, activation=ACT_NONE, out=None,
                out_dtype=None, workspace=None, stream=None):
     """s2_group_norm: act(normalised x * gamma + beta) of frames [frames, pixels,
     channels] (any frame and pixel strides, contiguous channels), statistics per
     frame and group of channels.  out may be x.  workspace: at least
-    group_norm_workspace(...) bytes, allocated on the current stream if None.
+    group_norm_workspace(...) bytes, made here if None.
     Returns out."""
-    import torch
     if x.dim() != 3:
         raise ValueError("x must be [frames, pixels, channels]")
     f, p, c = x.shape
     xd = _dtype_code(x)
     if out is None:
-        out = torch.empty((f, p, c), dtype=out_dtype or x.dtype, device=x.device)
+        out = _empty((f, p, c), out_dtype or x.dtype, x, stream)
     elif out.shape != x.shape:
         raise ValueError("x and out must be of one shape")
     if c > 1 and (x.stride(2) != 1 or out.stride(2) != 1):
@@ -727,7 +745,7 @@ def group_norm(x, groups, gamma=None, beta=None, epsilon=1e-6, activation=ACT_NO
     _vector(gamma, c, "gamma")
     _vector(beta, c, "beta")
     _on_current_device(x, out, gamma, beta, workspace)
-    workspace, size = _workspace(workspace, group_norm_workspace, x, f, p, c, groups)
+    workspace, size = _workspace(workspace, stream, x, group_norm_workspace, f, p, c, groups)
     check(lib().s2_group_norm(x.data_ptr(), xd, x.stride(0), x.stride(1), f, p, c, groups,
                               _ptr(gamma), _ptr(beta), epsilon, activation, out.data_ptr(),
                               _dtype_code(out), out.stride(0), out.stride(1), _ptr(workspace),
@@ -744,16 +762,15 @@ def group_norm_workspace(frames, pixels, channels, groups) -> int:
     return n.value
 
 
-def _matmul_views(x, n, k, weight, residual, out, out_dtype):
+def _matmul_views(x, n, k, weight, residual, out, out_dtype, stream):
     """The checked output of linear and grouped_linear."""
-    import torch
     if x.dim() != 2 or x.shape[1] != k or (k > 1 and x.stride(1) != 1):
         raise ValueError(f"x must be [m, {k}] with contiguous rows")
     if not weight.is_contiguous():
         raise ValueError("weight must be contiguous")
     m = x.shape[0]
     if out is None:
-        out = torch.empty((m, n), dtype=out_dtype or x.dtype, device=x.device)
+        out = _empty((m, n), out_dtype or x.dtype, x, stream)
     elif out.shape != (m, n) or (n > 1 and out.stride(1) != 1):
         raise ValueError(f"out must be [{m}, {n}] with contiguous rows")
     if residual is not None and (residual.shape != (m, n) or residual.dtype is not out.dtype or
@@ -781,28 +798,18 @@ def grouped_linear_workspace(m, groups, n, k, x_dtype=DTYPE_BF16, y_dtype=DTYPE_
     return b.value
 
 
-def _workspace(workspace, size, x, *sizes):
-    """(workspace or None, bytes): the caller's, or size(*sizes) bytes made here."""
-    import torch
-    if workspace is not None:
-        return workspace, workspace.numel() * workspace.element_size()
-    n = size(*sizes)
-    return (torch.empty(n, dtype=torch.uint8, device=x.device) if n else None), n
-
-
 def linear(x, weight, bias=None, activation=ACT_NONE, residual=None, out=None, out_dtype=None,
            workspace=None, stream=None):
     """s2_linear: residual + act(x W^T + bias) of rows x [m, k] with weight
     [n, k] (bf16 for fp32 and bf16 rows, fp16 for fp16 rows).  Rows may be
     strided.  out may be the residual.  workspace: linear_workspace(...) bytes,
-    allocated on the current stream if None.  Returns out [m, n]."""
-    import torch
+    made here if None.  Returns out [m, n]."""
     n, k = weight.shape
-    out = _matmul_views(x, n, k, weight, residual, out, out_dtype)
+    out = _matmul_views(x, n, k, weight, residual, out, out_dtype, stream)
     _vector(bias, n, "bias")
     m, xd, yd = x.shape[0], _dtype_code(x), _dtype_code(out)
     _on_current_device(x, weight, bias, residual, out, workspace)
-    workspace, size = _workspace(workspace, linear_workspace, x, m, n, k, xd, yd)
+    workspace, size = _workspace(workspace, stream, x, linear_workspace, m, n, k, xd, yd)
     check(lib().s2_linear(x.data_ptr(), xd, x.stride(0), m, weight.data_ptr(), _dtype_code(weight),
                           _ptr(bias), n, k, activation, _ptr(residual),
                           residual.stride(0) if residual is not None else 0, out.data_ptr(), yd,
@@ -816,16 +823,17 @@ def grouped_linear(x, offsets, weight, bias=None, activation=ACT_NONE, residual=
     offsets[g + 1] - 1 (int32 on the device) with weight [groups, n, k] and
     bias [groups, n].  Rows in no group are left as they are in out (undefined
     in one that this call makes).  workspace: grouped_linear_workspace(...)
-    bytes, allocated on the current stream if None.  Returns out [m, n]."""
+    bytes, made here if None.  Returns out [m, n]."""
     import torch
     groups, n, k = weight.shape
-    out = _matmul_views(x, n, k, weight, residual, out, out_dtype)
+    out = _matmul_views(x, n, k, weight, residual, out, out_dtype, stream)
     if offsets.dtype != torch.int32 or offsets.numel() != groups + 1 or not offsets.is_contiguous():
         raise ValueError(f"offsets must be {groups + 1} contiguous int32 values")
     _vector(bias, groups * n, "bias")
     m, xd, yd = x.shape[0], _dtype_code(x), _dtype_code(out)
     _on_current_device(x, offsets, weight, bias, residual, out, workspace)
-    workspace, size = _workspace(workspace, grouped_linear_workspace, x, m, groups, n, k, xd, yd)
+    workspace, size = _workspace(workspace, stream, x, grouped_linear_workspace, m, groups, n, k, xd,
+                                 yd)
     check(lib().s2_grouped_linear(x.data_ptr(), xd, x.stride(0), m, offsets.data_ptr(), groups,
                                   weight.data_ptr(),
                                   _dtype_code(weight), _ptr(bias), n, k, activation,

@@ -1334,6 +1334,7 @@ static int matmul_args_ok(const s2::MatmulArgs& a, bool any_rows) {
         return fail(S2_ERR_INVALID, "operands must be aligned to their elements");
     if (a.res == a.y && a.m > 1 && a.res_stride != a.y_stride)
         return fail(S2_ERR_INVALID, "in place needs one row stride");
+    if (a.y == a.x || a.y == a.w) return fail(S2_ERR_INVALID, "y overlaps x or the weight");
     return S2_OK;
 }
 

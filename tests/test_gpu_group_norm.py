@@ -144,3 +144,25 @@ def test_repeats_streams_and_capture():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, capi.group_norm(x, 32, gamma, beta, activation=capi.ACT_SILU))
+
+
+def test_frames_far_apart():
+    """Frame strides past 2^31 elements, pixel strides past 2^24."""
+    import torch
+    x, gamma, beta = _draw((3, 90, 64), "bfloat16", 11)
+    for shape, strides in (((3, 90, 64), (2 ** 31 + 64, 64, 1)), ((3, 90, 64), (64, 2 ** 25, 1))):
+        size = sum((n - 1) * s for n, s in zip(shape, strides)) + 1
+        big = [torch.empty(size, dtype=x.dtype, device="cuda").as_strided(shape, strides) for _ in range(2)]
+        big[0].copy_(x)
+        capi.group_norm(big[0], 8, gamma, beta, out=big[1])
+        _check(x, 8, gamma, beta, 1e-6, "none", big[1])
+        del big
+    torch.cuda.empty_cache()
+
+
+def test_more_pixels_than_24_bits():
+    """One frame of 17 million pixels: counts that fp32 rounds, many chunks."""
+    import torch
+    x, gamma, beta = _draw((1, 17_000_003, 4), "float16", 12)
+    got = capi.group_norm(x, 2, gamma, beta)
+    _check(x, 2, gamma, beta, 1e-6, "none", got)

@@ -342,3 +342,78 @@ def test_two_stream_mlp():
     for g, (a, b) in enumerate(((0, rows[0]), (rows[0], m))):
         _check(h[a:b], x[a:b], up[g], bu[g], "gelu_tanh", None)
         _check(res[a:b], h[a:b], down[g], bd[g], "none", start[a:b])
+
+
+def test_rows_far_apart():
+    """Row strides whose offsets pass 32 bits within a tile and over the call: x, the
+    residual and y each spread over 4.7 GB."""
+    import torch
+    m, k, n, far = 70, 72, 40, 2 ** 25 + 8
+    for pair in PAIRS[1:]:
+        x, w, bias, res = _operands(m, k, n, pair, pair[0])
+        spread = [torch.empty(m * far, dtype=x.dtype, device="cuda") for _ in range(3)]
+        xw, rw, yw = (t.as_strided((m, c), (far, 1)) for t, c in zip(spread, (k, n, n)))
+        xw.copy_(x)
+        rw.copy_(res)
+        for args in ((xw, res, None), (x, res, yw), (x, rw, None), (xw, rw, rw)):
+            got = capi.linear(args[0], w, bias, capi.ACT_SILU, args[1], out=args[2])
+            _check(got, x, w, bias, "silu", res)
+        del spread, xw, rw, yw
+    torch.cuda.empty_cache()
+
+
+def test_groups_whose_weights_pass_32_bits():
+    """Three weights of 2^30 elements: the last one starts 4.3 GB in."""
+    import torch
+    n = k = 2 ** 15
+    draw = _gen(7)
+    w = torch.empty(3, n, k, dtype=torch.bfloat16, device="cuda")
+    for part in w.view(-1, 2 ** 12, k):
+        part.copy_(draw(2 ** 12, k) * k ** -0.5)
+    for rows in ([1, 0, 2], [100, 3, 70]):
+        ends = [0, rows[0], rows[0] + rows[1], sum(rows)]
+        x = draw(ends[-1], k).bfloat16()
+        got = capi.grouped_linear(x, torch.tensor(ends, dtype=torch.int32, device="cuda"), w,
+                                  out_dtype=torch.float32)
+        for g in (0, 2):
+            for cols in (slice(0, 64), slice(n - 64, n)):
+                _check(got[ends[g]:ends[g + 1], cols], x[ends[g]:ends[g + 1]], w[g, cols], None, "none", None)
+    del w
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("m", [5, 90, 400])
+def test_a_stream_that_is_not_the_current_one(m):
+    """stream= with outputs and workspaces made by the call, while the current stream
+    keeps taking and giving back memory of the same sizes."""
+    import torch
+    x, w, bias, res = _operands(m, 2560, 640, PAIRS[0], "float32")
+    frames = x.view(1, m, 2560)
+    want = capi.linear(x, w, bias, capi.ACT_SILU, res), capi.group_norm(frames, 32)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(8):
+        got.append((capi.linear(x, w, bias, capi.ACT_SILU, res, stream=side),
+                    capi.group_norm(frames, 32, stream=side)))
+        size = capi.linear_workspace(m, 640, 2560, capi.DTYPE_F32, capi.DTYPE_F32)
+        torch.empty(max(size, 512), dtype=torch.uint8, device="cuda").fill_(255)
+        torch.empty_like(want[0]).fill_(float("nan"))
+    torch.cuda.synchronize()
+    for y, z in got:
+        assert torch.equal(y, want[0]) and torch.equal(z, want[1])
+
+
+def test_two_streams_at_once():
+    """Calls of one shape on two streams, each with a workspace of its own."""
+    import torch
+    cases = [_operands(77, 5120, 512, PAIRS[1], "bfloat16", seed=s) for s in range(2)]
+    want = [capi.linear(x, w, b, residual=r) for x, w, b, r in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i, (x, w, b, r) in enumerate(cases):
+            got[i].append(capi.linear(x, w, b, residual=r, stream=streams[i]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want[i]) for i in range(2) for y in got[i])

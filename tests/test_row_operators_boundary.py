@@ -61,7 +61,7 @@ MATMUL = [
     dict(activation=capi.ACT_SWIGLU), dict(activation=-1), dict(x=None), dict(weight=None),
     dict(y=None), dict(x_stride=63), dict(y_stride=31), dict(residual_stride=31), dict(x=P + 1),
     dict(weight=P + 1), dict(y=P + 2), dict(residual=P + 2), dict(bias=P + 2),
-    dict(residual=2 * P, residual_stride=40)]
+    dict(residual=2 * P, residual_stride=40), dict(y=P), dict(x=3 * P, y=P)]
 
 
 @pytest.mark.parametrize("changes", MATMUL + [dict(workspace=P + 8, workspace_bytes=64)], ids=str)
