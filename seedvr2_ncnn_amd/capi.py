@@ -690,20 +690,25 @@ def denoise_update(positive_patches, negative_patches, frames, height, width, cf
 # ---- group norm, linear, grouped linear --------------------------------------
 
 def _vector(t, size, name):
-    """Checks an optional contiguous fp32 device vector (gamma, beta, bias)."""
+    """Checks a contiguous fp32 vector (gamma, beta, bias); returns its address."""
     import torch
-    if t is not None and (t.dtype is not torch.float32 or t.numel() != size or
-                          not t.is_contiguous()):
+    if t.dtype is not torch.float32 or t.numel() != size or not t.is_contiguous():
         raise ValueError(f"{name} must be {size} contiguous fp32 values")
+    return t.data_ptr()
 
 
-def _on_current_device(x, *others):
-    """Refuses tensors that the current device's kernels cannot reach."""
+def _raw_stream(x, stream, *others):
+    """The stream's handle; refuses tensors that the current device's kernels
+    cannot reach."""
     import torch
     device = x.get_device()
-    if device < 0 or device != torch._C._cuda_getDevice() or any(
-            t is not None and t.get_device() != device for t in others):
+    near = device >= 0 and device == torch._C._cuda_getDevice()
+    for t in others:
+        if t is not None and t.get_device() != device:
+            near = False
+    if not near:
         raise ValueError("operands must be on the current device")
+    return torch._C._cuda_getCurrentRawStream(device) if stream is None else stream.cuda_stream
 
 
 def _empty(shape, dtype, x, stream):
@@ -716,13 +721,16 @@ def _empty(shape, dtype, x, stream):
         return torch.empty(shape, dtype=dtype, device=x.device)
 
 
-def _workspace(workspace, stream, x, size, *sizes):
-    """(workspace or None, bytes): the caller's, or size(*sizes) bytes made here."""
-    if workspace is not None:
-        return workspace, workspace.numel() * workspace.element_size()
-    import torch
-    n = size(*sizes)
-    return (_empty(n, torch.uint8, x, stream) if n else None), n
+def _workspace(workspace, stream, x, n):
+    """(workspace or None, its address, bytes): the caller's, or n bytes made here."""
+    if workspace is None:
+        if n == 0:
+            return None, None, 0
+        import torch
+        workspace = _empty(n, torch.uint8, x, stream)
+    else:
+        n = workspace.numel() * workspace.element_size()
+    return workspace, workspace.data_ptr(), n
 
 
 def group_norm(x, groups, gamma=None, beta=None, epsilon=1e-6, activation=ACT_NONE, out=None,
@@ -730,8 +738,7 @@ def group_norm(x, groups, gamma=None, beta=None, epsilon=1e-6, activation=ACT_NO
     """s2_group_norm: act(normalised x * gamma + beta) of frames [frames, pixels,
     channels] (any frame and pixel strides, contiguous channels), statistics per
     frame and group of channels.  out may be x.  workspace: at least
-    group_norm_workspace(...) bytes, made here if None.
-    Returns out."""
+    group_norm_workspace(...) bytes, made here if None.  Returns out."""
     if x.dim() != 3:
         raise ValueError("x must be [frames, pixels, channels]")
     f, p, c = x.shape
@@ -740,16 +747,17 @@ def group_norm(x, groups, gamma=None, beta=None, epsilon=1e-6, activation=ACT_NO
         out = _empty((f, p, c), out_dtype or x.dtype, x, stream)
     elif out.shape != x.shape:
         raise ValueError("x and out must be of one shape")
-    if c > 1 and (x.stride(2) != 1 or out.stride(2) != 1):
+    xf, xp, xc = x.stride()
+    of, op, oc = out.stride()
+    if c > 1 and (xc != 1 or oc != 1):
         raise ValueError("channels must be contiguous")
-    _vector(gamma, c, "gamma")
-    _vector(beta, c, "beta")
-    _on_current_device(x, out, gamma, beta, workspace)
-    workspace, size = _workspace(workspace, stream, x, group_norm_workspace, f, p, c, groups)
-    check(lib().s2_group_norm(x.data_ptr(), xd, x.stride(0), x.stride(1), f, p, c, groups,
-                              _ptr(gamma), _ptr(beta), epsilon, activation, out.data_ptr(),
-                              _dtype_code(out), out.stride(0), out.stride(1), _ptr(workspace),
-                              size, _stream(stream)), "s2_group_norm")
+    ga = None if gamma is None else _vector(gamma, c, "gamma")
+    be = None if beta is None else _vector(beta, c, "beta")
+    handle = _raw_stream(x, stream, out, gamma, beta, workspace)
+    workspace, ws, size = _workspace(workspace, stream, x, group_norm_workspace(f, p, c, groups))
+    check(lib().s2_group_norm(x.data_ptr(), xd, xf, xp, f, p, c, groups, ga, be, epsilon, activation,
+                              out.data_ptr(), _dtype_code(out), of, op, ws, size, handle),
+          "s2_group_norm")
     return out
 
 
@@ -763,7 +771,8 @@ def group_norm_workspace(frames, pixels, channels, groups) -> int:
 
 
 def _matmul_views(x, n, k, weight, residual, out, out_dtype, stream):
-    """The checked output of linear and grouped_linear."""
+    """(out, m, x's, residual's and out's row strides) of linear and grouped_linear,
+    checked."""
     if x.dim() != 2 or x.shape[1] != k or (k > 1 and x.stride(1) != 1):
         raise ValueError(f"x must be [m, {k}] with contiguous rows")
     if not weight.is_contiguous():
@@ -771,12 +780,18 @@ def _matmul_views(x, n, k, weight, residual, out, out_dtype, stream):
     m = x.shape[0]
     if out is None:
         out = _empty((m, n), out_dtype or x.dtype, x, stream)
-    elif out.shape != (m, n) or (n > 1 and out.stride(1) != 1):
-        raise ValueError(f"out must be [{m}, {n}] with contiguous rows")
-    if residual is not None and (residual.shape != (m, n) or residual.dtype is not out.dtype or
-                                 (n > 1 and residual.stride(1) != 1)):
-        raise ValueError(f"residual must be [{m}, {n}] of out's type with contiguous rows")
-    return out
+        os_ = n
+    else:
+        if out.shape != (m, n) or (n > 1 and out.stride(1) != 1):
+            raise ValueError(f"out must be [{m}, {n}] with contiguous rows")
+        os_ = out.stride(0)
+    rs = 0
+    if residual is not None:
+        if residual.shape != (m, n) or residual.dtype is not out.dtype or (
+                n > 1 and residual.stride(1) != 1):
+            raise ValueError(f"residual must be [{m}, {n}] of out's type with contiguous rows")
+        rs = residual.stride(0)
+    return out, m, x.stride(0), rs, os_
 
 
 @functools.lru_cache(maxsize=4096)
@@ -805,15 +820,14 @@ def linear(x, weight, bias=None, activation=ACT_NONE, residual=None, out=None, o
     strided.  out may be the residual.  workspace: linear_workspace(...) bytes,
     made here if None.  Returns out [m, n]."""
     n, k = weight.shape
-    out = _matmul_views(x, n, k, weight, residual, out, out_dtype, stream)
-    _vector(bias, n, "bias")
-    m, xd, yd = x.shape[0], _dtype_code(x), _dtype_code(out)
-    _on_current_device(x, weight, bias, residual, out, workspace)
-    workspace, size = _workspace(workspace, stream, x, linear_workspace, m, n, k, xd, yd)
-    check(lib().s2_linear(x.data_ptr(), xd, x.stride(0), m, weight.data_ptr(), _dtype_code(weight),
-                          _ptr(bias), n, k, activation, _ptr(residual),
-                          residual.stride(0) if residual is not None else 0, out.data_ptr(), yd,
-                          out.stride(0), _ptr(workspace), size, _stream(stream)), "s2_linear")
+    out, m, xs, rs, os_ = _matmul_views(x, n, k, weight, residual, out, out_dtype, stream)
+    xd, yd = _dtype_code(x), _dtype_code(out)
+    bi = None if bias is None else _vector(bias, n, "bias")
+    handle = _raw_stream(x, stream, weight, bias, residual, out, workspace)
+    workspace, ws, size = _workspace(workspace, stream, x, linear_workspace(m, n, k, xd, yd))
+    check(lib().s2_linear(x.data_ptr(), xd, xs, m, weight.data_ptr(), _dtype_code(weight), bi, n, k,
+                          activation, _ptr(residual), rs, out.data_ptr(), yd, os_, ws, size, handle),
+          "s2_linear")
     return out
 
 
@@ -826,20 +840,17 @@ def grouped_linear(x, offsets, weight, bias=None, activation=ACT_NONE, residual=
     bytes, made here if None.  Returns out [m, n]."""
     import torch
     groups, n, k = weight.shape
-    out = _matmul_views(x, n, k, weight, residual, out, out_dtype, stream)
-    if offsets.dtype != torch.int32 or offsets.numel() != groups + 1 or not offsets.is_contiguous():
+    out, m, xs, rs, os_ = _matmul_views(x, n, k, weight, residual, out, out_dtype, stream)
+    if offsets.dtype is not torch.int32 or offsets.numel() != groups + 1 or not offsets.is_contiguous():
         raise ValueError(f"offsets must be {groups + 1} contiguous int32 values")
-    _vector(bias, groups * n, "bias")
-    m, xd, yd = x.shape[0], _dtype_code(x), _dtype_code(out)
-    _on_current_device(x, offsets, weight, bias, residual, out, workspace)
-    workspace, size = _workspace(workspace, stream, x, grouped_linear_workspace, m, groups, n, k, xd,
-                                 yd)
-    check(lib().s2_grouped_linear(x.data_ptr(), xd, x.stride(0), m, offsets.data_ptr(), groups,
-                                  weight.data_ptr(),
-                                  _dtype_code(weight), _ptr(bias), n, k, activation,
-                                  _ptr(residual),
-                                  residual.stride(0) if residual is not None else 0, out.data_ptr(), yd,
-                                  out.stride(0), _ptr(workspace), size, _stream(stream)),
+    xd, yd = _dtype_code(x), _dtype_code(out)
+    bi = None if bias is None else _vector(bias, groups * n, "bias")
+    handle = _raw_stream(x, stream, offsets, weight, bias, residual, out, workspace)
+    workspace, ws, size = _workspace(workspace, stream, x,
+                                     grouped_linear_workspace(m, groups, n, k, xd, yd))
+    check(lib().s2_grouped_linear(x.data_ptr(), xd, xs, m, offsets.data_ptr(), groups,
+                                  weight.data_ptr(), _dtype_code(weight), bi, n, k, activation,
+                                  _ptr(residual), rs, out.data_ptr(), yd, os_, ws, size, handle),
           "s2_grouped_linear")
     return out
 

@@ -390,34 +390,39 @@ __global__ __launch_bounds__(kThreads) void group_norm_apply_kernel(GroupNormArg
 
 // Few values: a workgroup holds a frame's group in registers, one launch in all.  The
 // mean first, then the deviations from it.
-constexpr int kSmallThreads = 256;
-constexpr int kSmallVectors = 8;   // of a thread
+// A thread holds up to 4 vectors of 8, or 8 of 4 or 1; 256 threads, or 1024 (2000 x 512
+// in bf16 in 32 groups 7.3 us, 12 by two launches; 4000 x 512 with 8 vectors of 8 a
+// thread 16.6 and 13: the group's pieces of 32 bytes come to one compute unit).
+constexpr int kSmallMost = 1024;   // threads
+constexpr int small_vectors(int v) { return v == 8 ? 4 : 8; }
 
+template <int THREADS>
 __device__ __forceinline__ float block_sum(float v, float* lds) {
     v = lanes_sum(v, 6);
     if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
     __syncthreads();
     v = 0.f;
 #pragma unroll
-    for (int i = 0; i < kSmallThreads / 64; ++i) v += lds[i];
+    for (int i = 0; i < THREADS / 64; ++i) v += lds[i];
     return v;
 }
 
-template <int XK, int YK, int V>
-__global__ __launch_bounds__(kSmallThreads) void group_norm_small_kernel(GroupNormArgs p) {
+template <int XK, int YK, int V, int THREADS>
+__global__ __launch_bounds__(THREADS) void group_norm_small_kernel(GroupNormArgs p) {
     typedef typename Elem<XK>::T T;
-    __shared__ float lds[2][kSmallThreads / 64];
+    constexpr int VECS = small_vectors(V);
+    __shared__ float lds[2][THREADS / 64];
     const int f = blockIdx.y, g = blockIdx.x;
     const int each = p.channels / p.groups;
     const int ev = each / V;   // vectors of a pixel, at most the threads
-    const int rows = kSmallThreads / ev;
+    const int rows = THREADS / ev;
     const int row = threadIdx.x / ev;
     const int c = g * each + (threadIdx.x - row * ev) * V;
     const int count = row < rows ? (p.pixels - row + rows - 1) / rows : 0;   // of this thread
     const T* x = (const T*)p.x + f * p.x_frame;
-    Raw<T, V> raw[kSmallVectors];
+    Raw<T, V> raw[VECS];
 #pragma unroll
-    for (int u = 0; u < kSmallVectors; ++u)
+    for (int u = 0; u < VECS; ++u)
         if (u < count) raw[u].load(x + (long)(row + u * rows) * p.x_pixel + c);
     float scale[V], shift[V];
     if (count > 0) {
@@ -426,33 +431,33 @@ __global__ __launch_bounds__(kSmallThreads) void group_norm_small_kernel(GroupNo
     }
     // deviations from the first value: no digits are lost to a large mean
     const float ref = to_f32(x[g * each]);
-    float v[kSmallVectors][V];
+    float v[VECS][V];
     float sum = 0.f;
 #pragma unroll
-    for (int u = 0; u < kSmallVectors; ++u)
+    for (int u = 0; u < VECS; ++u)
         if (u < count) {
             raw[u].get(v[u]);
 #pragma unroll
             for (int i = 0; i < V; ++i) sum += v[u][i] - ref;
         }
     const float per_value = 1.f / ((float)p.pixels * (float)each);
-    const float mean = fmaf(block_sum(sum, lds[0]), per_value, ref);
+    const float mean = fmaf(block_sum<THREADS>(sum, lds[0]), per_value, ref);
     float m2 = 0.f;
 #pragma unroll
-    for (int u = 0; u < kSmallVectors; ++u)
+    for (int u = 0; u < VECS; ++u)
         if (u < count)
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 const float d = v[u][i] - mean;
                 m2 = fmaf(d, d, m2);
             }
-    const float rstd = 1.f / sqrtf(fmaf(block_sum(m2, lds[1]), per_value, p.eps));
+    const float rstd = 1.f / sqrtf(fmaf(block_sum<THREADS>(m2, lds[1]), per_value, p.eps));
     if (count == 0) return;
 #pragma unroll
     for (int i = 0; i < V; ++i) scale[i] *= rstd;
     with_activation(p.act, [&](auto act) {
 #pragma unroll
-        for (int u = 0; u < kSmallVectors; ++u)
+        for (int u = 0; u < VECS; ++u)
             if (u < count) {
 #pragma unroll
                 for (int i = 0; i < V; ++i)
@@ -473,9 +478,11 @@ bool fits(const GroupNormArgs& p, int width, int v) {
            fits(p.y, p.y_kind, p.y_frame, p.y_pixel, v);
 }
 
-// Whether a workgroup can hold a frame's group, `vectors` to a pixel.
-bool small_holds(int pixels, int vectors) {
-    return vectors <= kSmallThreads && pixels <= kSmallThreads / vectors * kSmallVectors;
+// Whether a workgroup of so many threads can hold a frame's group of `each` channels in
+// vectors of v.
+bool small_holds(int pixels, int each, int v, int threads) {
+    const int vectors = each / v;   // of a pixel
+    return vectors <= threads && pixels <= threads / vectors * small_vectors(v);
 }
 
 // How a frame's pixels are cut for the statistics: about one workgroup for each compute
@@ -517,20 +524,25 @@ hipError_t run(const GroupNormArgs& p, float2* parts, hipStream_t stream) {
     return hipGetLastError();
 }
 
+template <int XK, int YK, int V>
+hipError_t run_small(const GroupNormArgs& p, hipStream_t stream) {
+    const dim3 grid((unsigned)p.groups, (unsigned)p.frames);
+    if (small_holds(p.pixels, p.channels / p.groups, V, 256))
+        group_norm_small_kernel<XK, YK, V, 256><<<grid, 256, 0, stream>>>(p);
+    else
+        group_norm_small_kernel<XK, YK, V, kSmallMost><<<grid, kSmallMost, 0, stream>>>(p);
+    return hipGetLastError();
+}
+
 template <int XK, int YK>
 hipError_t pick(const GroupNormArgs& p, float2* parts, hipStream_t stream) {
     const int each = p.channels / p.groups;
     for (int v : {8, 4, 1}) {
         if (v > 1 && !fits(p, each, v)) continue;
-        if (!small_holds(p.pixels, each / v)) break;
-        const dim3 grid((unsigned)p.groups, (unsigned)p.frames);
-        if (v == 8)
-            group_norm_small_kernel<XK, YK, 8><<<grid, kSmallThreads, 0, stream>>>(p);
-        else if (v == 4)
-            group_norm_small_kernel<XK, YK, 4><<<grid, kSmallThreads, 0, stream>>>(p);
-        else
-            group_norm_small_kernel<XK, YK, 1><<<grid, kSmallThreads, 0, stream>>>(p);
-        return hipGetLastError();
+        if (!small_holds(p.pixels, each, v, kSmallMost)) break;
+        return v == 8   ? run_small<XK, YK, 8>(p, stream)
+               : v == 4 ? run_small<XK, YK, 4>(p, stream)
+                        : run_small<XK, YK, 1>(p, stream);
     }
     if (fits(p, p.channels, 8)) return run<XK, YK, 8>(p, parts, stream);
     if (fits(p, p.channels, 4)) return run<XK, YK, 4>(p, parts, stream);
@@ -549,7 +561,7 @@ hipError_t pick_y(const GroupNormArgs& p, float2* parts, hipStream_t stream) {
 size_t group_norm_workspace(int frames, int pixels, int channels, int groups) {
     if (frames <= 0 || pixels <= 0) return 0;
     // groups in registers, by single elements if need be
-    if (small_holds(pixels, channels / groups)) return 0;
+    if (small_holds(pixels, channels / groups, 1, kSmallMost)) return 0;
     const int chunk = chunk_pixels(frames, pixels, channels);
     return (size_t)frames * (size_t)chunks_of(pixels, chunk) * groups * sizeof(float2);
 }

@@ -9,9 +9,9 @@ from seedvr2_ncnn_amd import capi
 F32, BF16, F16 = capi.DTYPE_F32, capi.DTYPE_BF16, capi.DTYPE_F16
 P = 0x10000   # stands for a device address; none of these calls gets to use it
 
-NORM = dict(x=P, x_dtype=F32, x_frame=40960, x_pixel=64, frames=2, pixels=640, channels=64, groups=8,
+NORM = dict(x=P, x_dtype=F32, x_frame=163840, x_pixel=64, frames=2, pixels=2560, channels=64, groups=8,
             gamma=P, beta=P, epsilon=1e-6, activation=capi.ACT_NONE, y=2 * P, y_dtype=F32,
-            y_frame=40960, y_pixel=64, workspace=P, workspace_bytes=1 << 20, stream=None)
+            y_frame=163840, y_pixel=64, workspace=P, workspace_bytes=1 << 20, stream=None)
 LINEAR = dict(x=P, x_dtype=BF16, x_stride=64, m=4, weight=P, w_dtype=BF16, bias=P, n=32, k=64,
               activation=capi.ACT_NONE, residual=P, residual_stride=32, y=2 * P, y_dtype=F32,
               y_stride=32, workspace=None, workspace_bytes=0, stream=None)
@@ -30,9 +30,9 @@ def _call(name, base, **changes):
     dict(groups=7), dict(channels=0), dict(channels=4104, groups=8), dict(x_dtype=3), dict(y_dtype=-1),
     dict(activation=capi.ACT_SWIGLU), dict(activation=5), dict(epsilon=-1e-6),
     dict(epsilon=float("nan")), dict(x=None), dict(y=None), dict(x_frame=-1), dict(x_pixel=-64),
-    dict(y_pixel=63), dict(y_frame=63), dict(y_frame=40959), dict(x=P + 2), dict(y=P + 2),
+    dict(y_pixel=63), dict(y_frame=63), dict(y_frame=163839), dict(x=P + 2), dict(y=P + 2),
     dict(gamma=P + 2), dict(beta=P + 1), dict(workspace=None), dict(workspace_bytes=8),
-    dict(workspace=P + 4), dict(y=P, y_dtype=BF16), dict(y=P, y_frame=81920)], ids=str)
+    dict(workspace=P + 4), dict(y=P, y_dtype=BF16), dict(y=P, y_frame=327680)], ids=str)
 def test_group_norm_refuses(changes):
     assert _call("s2_group_norm", NORM, **changes) == capi.S2_ERR_INVALID
     assert capi.last_error()
