@@ -38,42 +38,50 @@ __device__ __forceinline__ int group_tiles(const MatmulArgs& a, int g, int tm, i
     return end > start ? (end - start + tm - 1) / tm : 0;
 }
 
-// Tiles of tm rows that there are; mtiles is what there can be.  Every wave counts for
-// itself, 64 groups at a time.
-__device__ __forceinline__ int count_row_tiles(const MatmulArgs& a, int tm, int mtiles) {
-    if (!a.offsets) return mtiles;
-    int sum = 0, start, end;
-    for (int g = threadIdx.x & 63; g < a.groups; g += 64) sum += group_tiles(a, g, tm, start, end);
-#pragma unroll
-    for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
-    // (offsets that descend can make more of them than the grid has workgroups for)
-    return min(__builtin_amdgcn_readfirstlane(sum), mtiles);
-}
+// The row tiles of a call: `count` of them, of at most mtiles.  Every wave counts for
+// itself, 64 groups at a time, and keeps the count of up to 64 groups.
+struct RowTiles {
+    const MatmulArgs& a;
+    int tm, count;
+    int start, end, upto;   // of group `lane`; tiles of the groups up to it
 
-__device__ __forceinline__ RowTile row_tile(const MatmulArgs& a, int t, int tm) {
-    if (!a.offsets) return RowTile{t * tm, a.m, 0};
-    const int lane = threadIdx.x & 63;
-    for (int g0 = 0; g0 < a.groups; g0 += 64) {
-        int start, end;
-        const int tiles = group_tiles(a, g0 + lane, tm, start, end);
-        int upto = tiles;   // tiles of the groups up to this one
+    // groups g0 .. g0 + 63; returns the tiles in them
+    __device__ __forceinline__ int scan(int g0) {
+        const int lane = threadIdx.x & 63;
+        upto = group_tiles(a, g0 + lane, tm, start, end);
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
             const int other = __shfl_up(upto, o);
             if (lane >= o) upto += other;
         }
-        const uint64_t past = __ballot(upto > t);
-        if (past) {
-            const int l = __ffsll((unsigned long long)past) - 1;
-            const int first = __shfl(start, l) + (t - __shfl(upto - tiles, l)) * tm;
-            return RowTile{__builtin_amdgcn_readfirstlane(first),
-                           __builtin_amdgcn_readfirstlane(__shfl(end, l)),
-                           __builtin_amdgcn_readfirstlane(g0 + l)};
-        }
-        t -= __builtin_amdgcn_readfirstlane(__shfl(upto, 63));
+        return __builtin_amdgcn_readfirstlane(__shfl(upto, 63));
     }
-    return RowTile{0, 0, 0};
-}
+
+    __device__ __forceinline__ RowTiles(const MatmulArgs& args, int rows, int mtiles) : a(args), tm(rows) {
+        count = mtiles;
+        if (!a.offsets) return;
+        int sum = 0;
+        for (int g0 = 0; g0 < a.groups; g0 += 64) sum += scan(g0);
+        count = min(sum, mtiles);   // (descending offsets can make more than the grid has)
+    }
+
+    __device__ __forceinline__ RowTile at(int t) {
+        if (!a.offsets) return RowTile{t * tm, a.m, 0};
+        for (int g0 = 0; g0 < a.groups; g0 += 64) {
+            const int sum = a.groups > 64 ? scan(g0) : count;
+            const uint64_t past = __ballot(upto > t);
+            if (past) {
+                const int l = __ffsll((unsigned long long)past) - 1;
+                const int before = l ? __shfl(upto, l - 1) : 0;   // (l is the wave's)
+                return RowTile{__builtin_amdgcn_readfirstlane(__shfl(start, l) + (t - before) * tm),
+                               __builtin_amdgcn_readfirstlane(__shfl(end, l)),
+                               __builtin_amdgcn_readfirstlane(g0 + l)};
+            }
+            t -= sum;
+        }
+        return RowTile{0, 0, 0};
+    }
+};
 
 __device__ __forceinline__ float load1(const void* p, long idx, int kind) {
     if (kind == 1) return bf16_to_f32(((const uint16_t*)p)[idx]);

@@ -35,10 +35,11 @@ __global__ __launch_bounds__(256, 2) void matmul_any_kernel(MatmulArgs a, int nt
     constexpr int BM = 128, BN = 128, BK = 32, P = BK + 8, PL = XP ? XP : 1;
     __shared__ __attribute__((aligned(16))) uint16_t x_lds[2][PL][BM * P];
     __shared__ __attribute__((aligned(16))) uint16_t w_lds[2][BN * P];
-    const int blocks = count_row_tiles(a, BM, gridDim.x / ntiles) * ntiles;
+    RowTiles rts(a, BM, gridDim.x / ntiles);
+    const int blocks = rts.count * ntiles;
     if ((int)blockIdx.x >= blocks) return;   // the whole workgroup
     const int lid = xcd_remap(blockIdx.x, blocks);
-    const RowTile rt = row_tile(a, lid / ntiles, BM);
+    const RowTile rt = rts.at(lid / ntiles);
     const int col0 = lid % ntiles * BN;
     const int rows = min(rt.end - rt.row0, BM);
     if (rows <= 0) return;   // the whole workgroup

@@ -20,7 +20,7 @@ __global__ __launch_bounds__(512) void matmul_rows_kernel(MatmulArgs a, int ntil
     constexpr int U = REGS >= 40 ? 1 : REGS >= 24 ? 2 : 4;  // chunks of a batch
     constexpr bool TWO = U * REGS <= 80;                    // the next batch in flight
     __shared__ float sums[8][MT * NT * 256];
-    const RowTile rt = row_tile(a, blockIdx.x / ntiles, 16 * MT);
+    const RowTile rt = RowTiles(a, 16 * MT, gridDim.x / ntiles).at(blockIdx.x / ntiles);
     const int col0 = blockIdx.x % ntiles * 16 * NT;
     const int rows = min(rt.end - rt.row0, 16 * MT);
     if (rows <= 0) return;   // the whole workgroup

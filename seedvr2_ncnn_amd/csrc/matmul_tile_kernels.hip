@@ -87,7 +87,8 @@ __device__ __forceinline__ TilePlace tile_place(const MatmulArgs& a, const TileS
     // make it, and workgroups without a tile come last (dealt out over the grid, 238 of
     // 301 tiles were two rounds on six of the eight XCDs, 72 us; 34 so).
     constexpr int GROUP = 4;
-    const int mtiles = count_row_tiles(a, bm, sp.mtiles);
+    RowTiles rts(a, bm, sp.mtiles);
+    const int mtiles = rts.count;
     const int blocks = mtiles * sp.ntiles * sp.parts;
     TilePlace p;
     if ((int)blockIdx.x >= blocks) {
@@ -100,7 +101,7 @@ __device__ __forceinline__ TilePlace tile_place(const MatmulArgs& a, const TileS
     const int first = t / (GROUP * sp.ntiles) * GROUP;
     const int gm = min(mtiles - first, GROUP);
     const int in = t % (GROUP * sp.ntiles);
-    p.rt = row_tile(a, first + in % gm, bm);
+    p.rt = rts.at(first + in % gm);
     p.rows = min(p.rt.end - p.rt.row0, bm);
     p.col0 = in / gm * bn;
     p.nk = (a.k + kBK - 1) / kBK;
