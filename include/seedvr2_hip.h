@@ -535,7 +535,7 @@ S2_API int s2_group_norm(const void* x, s2_dtype x_dtype, long x_frame_stride,
  *   stride residual_stride >= n, or NULL; y: device [m][n], row stride y_stride
  *   >= n.  y is the residual itself (same stride) or does not overlap it; y
  *   overlaps nothing else.
- * Any m >= 0 (0 does nothing), n and k; pointers aligned to their elements.
+ * Any m (0 does nothing), n and k up to 2^30; pointers aligned to their elements.
  *   Fastest are k a multiple of 8 and n of 4, with x and weight rows that start
  *   at 16 bytes and y and residual rows at four elements.
  * workspace: s2_linear_workspace_bytes, 16-byte aligned (calls that may overlap
@@ -554,10 +554,11 @@ S2_API int s2_linear(const void* x, s2_dtype x_dtype, long x_stride, int m, cons
  * block that do not share weights, a weight per sample or per expert.
  *
  * offsets: device int32 [groups + 1], ascending, 0 <= offsets[g] <= m, read by
- *   the kernels.  Groups may be empty.  Rows before offsets[0] and from
- *   offsets[groups] on are neither read nor written.  Offsets outside [0, m] are
- *   taken as the nearest of the two; rows that descending offsets put into two
- *   groups, or into none, have unspecified values.
+ *   the kernels; at most 2^30 groups, which may be empty, and 2^28 rows.  Rows
+ *   before offsets[0] and from offsets[groups] on are not written, and what they
+ *   hold is not used.  Offsets outside [0, m] are taken as the nearest of the two;
+ *   rows that descending offsets put into two groups, or into none, have
+ *   unspecified values.
  * weight: device [groups][n][k]; bias: device fp32 [groups][n] or NULL; the
  *   rest as for s2_linear, workspace: s2_grouped_linear_workspace_bytes. */
 S2_API int s2_grouped_linear_workspace_bytes(int m, int groups, int n, int k, s2_dtype x_dtype,

@@ -1315,16 +1315,23 @@ int s2_group_norm(const void* x, s2_dtype x_dtype, long x_frame_stride, long x_p
     return S2_OK;
 }
 
+// Sizes that leave room in 32 bits for what lies past the last group, tile and k step,
+// and for the tiles of 64 groups that, by wrong offsets, have all the rows each.
+static bool matmul_shape_ok(int m, bool grouped, int groups, int n, int k) {
+    return m >= 0 && groups >= 0 && n > 0 && k > 0 && m <= (grouped ? 1 << 28 : 1 << 30) &&
+           std::max({groups, n, k}) <= 1 << 30;
+}
+
 // Argument checks of s2_linear and s2_grouped_linear.
-static int matmul_args_ok(const s2::MatmulArgs& a, bool any_rows) {
-    if (a.m < 0 || a.n <= 0 || a.k <= 0) return fail(S2_ERR_INVALID, "invalid linear shape");
+static int matmul_args_ok(const s2::MatmulArgs& a, bool grouped) {
+    if (!matmul_shape_ok(a.m, grouped, a.groups, a.n, a.k)) return fail(S2_ERR_INVALID, "invalid linear shape");
     if (!dtype_ok((s2_dtype)a.x_kind) || !dtype_ok((s2_dtype)a.w_kind) || !dtype_ok((s2_dtype)a.y_kind))
         return fail(S2_ERR_INVALID, "unsupported dtype");
     if (!((a.w_kind == S2_DTYPE_BF16 && a.x_kind != S2_DTYPE_F16) ||
           (a.w_kind == S2_DTYPE_F16 && a.x_kind == S2_DTYPE_F16)))
         return fail(S2_ERR_INVALID, "the weight is bf16 for fp32 and bf16 rows, fp16 for fp16 rows");
     if (!row_activation(a.act)) return fail(S2_ERR_INVALID, "unknown activation");
-    if (!any_rows) return S2_OK;
+    if (a.m == 0 || a.groups == 0) return S2_OK;
     if (!a.x || !a.w || !a.y) return fail(S2_ERR_INVALID, "null operand");
     if (a.m > 1 && (a.x_stride < a.k || a.y_stride < a.n || (a.res && a.res_stride < a.n)))
         return fail(S2_ERR_INVALID, "row strides shorter than rows");
@@ -1341,7 +1348,7 @@ static int matmul_args_ok(const s2::MatmulArgs& a, bool any_rows) {
 static int matmul_workspace(int m, const int* offsets, int groups, int n, int k, s2_dtype x_dtype,
                             s2_dtype y_dtype, size_t* bytes) {
     if (!bytes) return fail(S2_ERR_INVALID, "null bytes");
-    if (m < 0 || groups < 0 || n <= 0 || k <= 0) return fail(S2_ERR_INVALID, "invalid linear shape");
+    if (!matmul_shape_ok(m, offsets, groups, n, k)) return fail(S2_ERR_INVALID, "invalid linear shape");
     if (!dtype_ok(x_dtype) || !dtype_ok(y_dtype)) return fail(S2_ERR_INVALID, "unsupported dtype");
     *bytes = 0;
     if (m == 0 || groups == 0) return S2_OK;
@@ -1377,7 +1384,7 @@ int s2_linear(const void* x, s2_dtype x_dtype, long x_stride, int m, const void*
               long y_stride, void* workspace, size_t workspace_bytes, s2_stream_t stream) {
     const s2::MatmulArgs a{x, (int)x_dtype, x_stride, m, nullptr, 1, weight, (int)w_dtype, bias, n, k,
                            activation, residual, residual_stride, y, (int)y_dtype, y_stride, 1, 0};
-    const int ret = matmul_args_ok(a, m > 0);
+    const int ret = matmul_args_ok(a, false);
     if (ret != S2_OK) return ret;
     if (workspace && !aligned(workspace, 16))
         return fail(S2_ERR_INVALID, "workspace must be 16-byte aligned");
@@ -1392,8 +1399,7 @@ int s2_grouped_linear(const void* x, s2_dtype x_dtype, long x_stride, int m, con
                       s2_stream_t stream) {
     const s2::MatmulArgs a{x, (int)x_dtype, x_stride, m, offsets, groups, weight, (int)w_dtype, bias,
                            n, k, activation, residual, residual_stride, y, (int)y_dtype, y_stride, 1, 0};
-    if (groups < 0) return fail(S2_ERR_INVALID, "groups must be >= 0");
-    const int ret = matmul_args_ok(a, m > 0 && groups > 0);
+    const int ret = matmul_args_ok(a, true);
     if (ret != S2_OK) return ret;
     if (m == 0 || groups == 0) return S2_OK;
     if (!offsets) return fail(S2_ERR_INVALID, "null offsets");

@@ -60,9 +60,9 @@ struct RowTiles {
     __device__ __forceinline__ RowTiles(const MatmulArgs& args, int rows, int mtiles) : a(args), tm(rows) {
         count = mtiles;
         if (!a.offsets) return;
-        int sum = 0;
-        for (int g0 = 0; g0 < a.groups; g0 += 64) sum += scan(g0);
-        count = min(sum, mtiles);   // (descending offsets can make more than the grid has)
+        // (descending offsets can make more than the grid has)
+        count = 0;
+        for (int g0 = 0; g0 < a.groups; g0 += 64) count = min(count + scan(g0), mtiles);
     }
 
     __device__ __forceinline__ RowTile at(int t) {

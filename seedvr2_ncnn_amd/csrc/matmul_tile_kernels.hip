@@ -85,7 +85,7 @@ __device__ __forceinline__ TilePlace tile_place(const MatmulArgs& a, const TileS
     // consecutive tiles share an XCD's L2; four row tiles sweep the columns together.
     // Dealt out over the tiles that there are: a grid is as large as the groups' sizes can
     // make it, and workgroups without a tile come last (dealt out over the grid, 238 of
-    // 301 tiles were two rounds on six of the eight XCDs, 72 us; 34 so).
+    // 301 tiles were two rounds on six of the eight XCDs, 72 us; 41 so).
     constexpr int GROUP = 4;
     RowTiles rts(a, bm, sp.mtiles);
     const int mtiles = rts.count;

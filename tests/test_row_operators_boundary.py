@@ -78,6 +78,29 @@ def test_grouped_linear_refuses(changes):
     assert capi.last_error()
 
 
+@pytest.mark.parametrize("size", ["m", "n", "k"])
+def test_sizes_past_the_kernels_indexes_are_refused(size):
+    """2^30 at most: steps past the last k or tile stay in 32 bits."""
+    changes = {"m": 1, "x_stride": 1 << 31, "y_stride": 1 << 31, "residual_stride": 1 << 31,
+               size: (1 << 30) + 1}
+    assert _call("s2_linear", LINEAR, **changes) == capi.S2_ERR_INVALID
+    assert _call("s2_grouped_linear", GROUPED, **changes) == capi.S2_ERR_INVALID
+    sizes = {"m": 8, "n": 8, "k": 8, size: (1 << 30) + 1}
+    with pytest.raises(capi.S2Error):
+        capi.linear_workspace(**sizes)
+    with pytest.raises(capi.S2Error):
+        capi.grouped_linear_workspace(groups=2, **sizes)
+
+
+def test_groups_past_the_kernels_indexes_are_refused():
+    assert _call("s2_grouped_linear", GROUPED, groups=(1 << 30) + 1) == capi.S2_ERR_INVALID
+    with pytest.raises(capi.S2Error):
+        capi.grouped_linear_workspace(8, (1 << 30) + 1, 8, 8)
+    assert _call("s2_grouped_linear", GROUPED, m=(1 << 28) + 1) == capi.S2_ERR_INVALID
+    with pytest.raises(capi.S2Error):
+        capi.grouped_linear_workspace((1 << 28) + 1, 2, 8, 8)
+
+
 def test_linear_of_nothing():
     assert _call("s2_linear", LINEAR, m=0, x=None, y=None) == capi.S2_OK
     assert _call("s2_grouped_linear", GROUPED, m=0) == capi.S2_OK
