@@ -514,7 +514,8 @@ S2_API int s2_shared_linear_residual(const void* x_video, int m_video, const voi
  * workspace: s2_group_norm_workspace_bytes, 8-byte aligned (partial
  *   statistics; calls that may overlap in time need one each; 0 for small
  *   groups, then it may be NULL).
- * An infinity or NaN makes its frame's group NaN, no other. */
+ * An infinity or NaN makes its frame's group NaN, no other; deviations whose
+ * squares pass fp32's range leave a group NaN or act(beta). */
 S2_API int s2_group_norm_workspace_bytes(int frames, int pixels, int channels, int groups,
                                          size_t* bytes);
 S2_API int s2_group_norm(const void* x, s2_dtype x_dtype, long x_frame_stride,

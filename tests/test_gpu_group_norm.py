@@ -116,6 +116,31 @@ def test_non_finite_values_stay_in_their_group(bad, pixels):
     assert torch.equal(got[keep], clean[keep])
 
 
+@pytest.mark.parametrize("pixels", [40, 9000, 200000])
+def test_deviations_whose_squares_overflow_show(pixels):
+    """Squares past fp32's range leave no plausible values: NaN, or zeros of an
+    infinite variance; other groups stay as they are."""
+    import torch
+    x, _, _ = _draw((1, pixels, 32), "float32", 5)
+    want = capi.group_norm(x, 4)
+    x[:, :, 8:16] *= 1e25
+    got = capi.group_norm(x, 4)
+    bad = got[:, :, 8:16]
+    assert (bad.isnan() | (bad == 0)).all()
+    keep = [c for c in range(32) if not 8 <= c < 16]
+    assert torch.equal(got[:, :, keep], want[:, :, keep])
+
+
+def test_equal_parts_with_overflowing_squares_show():
+    """The same when every part of the sums has one mean, so that none of the
+    variance lies between parts: blocks of 64 pixels, zero and 1e25 in turn."""
+    import torch
+    p = 256 * 768
+    x = torch.where((torch.arange(p, device="cuda") // 64) % 2 == 0, 0.0, 1e25)
+    got = capi.group_norm(x[None, :, None].expand(1, p, 32).contiguous(), 4)
+    assert (got.isnan() | (got == 0)).all()
+
+
 def test_no_rows():
     import torch
     for shape in ((0, 5, 16), (2, 0, 16)):

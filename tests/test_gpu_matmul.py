@@ -176,6 +176,38 @@ def test_with_and_without_workspace(m, k, n):
         assert torch.equal(got, again)
 
 
+# above 32 rows; k and n even and odd; tiles beside and below each other
+@pytest.mark.parametrize("size", [(33, 72, 48), (130, 100, 77), (129, 1000, 260), (300, 33, 513)], ids=str)
+@pytest.mark.parametrize("pair", PAIRS, ids="-".join)
+@pytest.mark.parametrize("y_type", Y_TYPES)
+def test_sizes_without_workspace(size, pair, y_type):
+    import torch
+    m, k, n = size
+    none = torch.empty(0, dtype=torch.uint8, device="cuda")
+    x, w, bias, res = _operands(m, k, n, pair, y_type)
+    got = capi.linear(x, w, bias, capi.ACT_SILU, res, out_dtype=res.dtype, workspace=none)
+    _check(got, x, w, bias, "silu", res)
+
+
+@pytest.mark.parametrize("pair", PAIRS, ids="-".join)
+@pytest.mark.parametrize("kn", [(72, 33), (130, 260)], ids=str)
+def test_groups_without_workspace(pair, kn):
+    """Ragged and empty groups; rows in none keep what the output holds."""
+    import torch
+    k, n = kn
+    starts = [3, 3, 150, 151, 400]
+    x, w, bias, res = _operands(410, k, n, pair, pair[0], groups=4)
+    none = torch.empty(0, dtype=torch.uint8, device="cuda")
+    out = torch.full((410, n), 5.0, dtype=res.dtype, device="cuda")
+    capi.grouped_linear(x, torch.tensor(starts, dtype=torch.int32, device="cuda"), w, bias,
+                        capi.ACT_GELU, res, out=out, workspace=none)
+    for g in range(4):
+        at = slice(starts[g], starts[g + 1])
+        if starts[g] < starts[g + 1]:
+            _check(out[at], x[at], w[g], bias[g], "gelu", res[at])
+    assert (out[:3] == 5).all() and (out[400:] == 5).all()
+
+
 GROUPS = [[5], [0, 3, 0], [1] * 9, [130, 0, 1, 64, 0, 0, 257], [0] * 70 + [20, 0, 33], [16] * 40,
           [700, 2]]
 # the same with enough 256 x 256 tiles for every compute unit
