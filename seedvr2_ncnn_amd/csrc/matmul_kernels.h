@@ -44,13 +44,22 @@ inline long row_tiles(const MatmulArgs& a, int tm) {
     return ((long)a.m + (long)std::min(a.groups, a.m) * (tm - 1)) / tm;
 }
 
+// Elements that lie together in every row of x and of the weight.
+inline int row_gran(const MatmulArgs& a) {
+    for (int e : {8, 4})
+        if (a.k % e == 0 && a.x_stride % e == 0 && (uintptr_t)a.w % (2 * e) == 0 &&
+            (uintptr_t)a.x % (a.x_kind ? 2 * e : 16) == 0)
+            return e;
+    return 1;
+}
+
 // A call's kernel and what it keeps in the workspace.
 struct MatmulPlan {
-    enum Kernel { kRows, kTiles, kAny } kernel;
+    enum Kernel { kRows, kTiles, kShort, kAny } kernel;
     int rows, cols;        // kRows: of a tile, 16, 32 or 64 each
     int bm, bn;            // kTiles: the tile
-    int parts;             // kTiles: ranges of k
-    bool whole;            // kTiles: y and residual in pieces of four columns
+    int parts;             // kTiles: ranges of k; kShort: of rows
+    bool whole;            // kTiles, kShort: y and residual in pieces of four columns
     bool pack_x, pack_w;
     size_t x_bytes, w_bytes, sum_bytes;   // 256-byte multiples, in this order
     size_t bytes() const { return x_bytes + w_bytes + sum_bytes; }
@@ -64,6 +73,9 @@ hipError_t launch_matmul(const MatmulArgs& a, void* workspace, size_t workspace_
 // The kernels' own launchers, for calls that plan_matmul gives them.
 hipError_t launch_matmul_tiles(const MatmulArgs& a, const MatmulPlan& plan, float* sums,
                                hipStream_t stream);
+// The most k steps of 32 of the kernel for short k, of rows of that many bf16 terms.
+int matmul_short_steps(int planes);
+hipError_t launch_matmul_short(const MatmulArgs& a, const MatmulPlan& plan, hipStream_t stream);
 hipError_t launch_matmul_rows(const MatmulArgs& a, const MatmulPlan& plan, hipStream_t stream);
 
 }  // namespace s2

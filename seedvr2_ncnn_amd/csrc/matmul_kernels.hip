@@ -303,6 +303,20 @@ MatmulPlan plan_matmul(const MatmulArgs& a, size_t workspace_bytes) {
     const bool tiles = near && room && 256 * pitch * 2 < 0x7fffffffL &&
                        256 * std::max<long>(a.k, p.pack_w ? row : 0) * 2 < 0x7fffffffL;
 
+    // many fp32 rows of a short k.  By 2560 x 132 rows of 2700 17 -> 13 us, 21600 64 -> 41
+    // (packed and on tiles -> here); by 2560 x 160 17 -> 17, 65 -> 52; by 1024 x 64 of 5000
+    // and 21600 10.6 -> 11.1, 26 -> 18; fewer outputs gain only where the weight would be
+    // packed too
+    if (a.x_kind == 0 && !a.offsets && rows > 32 && (long)a.m * a.n >= 6L << 20 && near &&
+        (a.k + 31) / 32 <= matmul_short_steps(packed_planes(a)) && row_gran(a) >= 4 &&
+        a.x_stride < 1L << 24) {
+        MatmulPlan s{};
+        s.kernel = MatmulPlan::kShort;
+        s.parts = std::max(1, kUnits / ((a.n + 255) / 256));
+        s.whole = whole_pieces(a);
+        return s;
+    }
+
     double tile_us = 0.;
     if (tiles) {
         p.kernel = MatmulPlan::kTiles;
@@ -391,6 +405,7 @@ hipError_t launch_matmul(const MatmulArgs& args, void* workspace, size_t workspa
     }
     switch (p.kernel) {
         case MatmulPlan::kRows: return launch_matmul_rows(a, p, stream);
+        case MatmulPlan::kShort: return launch_matmul_short(a, p, stream);
         case MatmulPlan::kTiles: return launch_matmul_tiles(a, p, (float*)at, stream);
         default:
             return a.y_kind == 0   ? launch_any_y<0>(a, stream)

@@ -139,15 +139,6 @@ __global__ __launch_bounds__(512) void matmul_rows_kernel(MatmulArgs a, int ntil
     }
 }
 
-// Elements that lie together in every row of x and of the weight.
-int row_gran(const MatmulArgs& a) {
-    for (int e : {8, 4})
-        if (a.k % e == 0 && a.x_stride % e == 0 && (uintptr_t)a.w % (2 * e) == 0 &&
-            (uintptr_t)a.x % (a.x_kind ? 2 * e : 16) == 0)
-            return e;
-    return 1;
-}
-
 template <int T, int PL, int MT, int NT, int GRAN>
 hipError_t run(const MatmulArgs& a, hipStream_t stream) {
     const int ntiles = (a.n + 16 * NT - 1) / (16 * NT);

@@ -176,6 +176,46 @@ def test_with_and_without_workspace(m, k, n):
         assert torch.equal(got, again)
 
 
+# many fp32 rows of short k: k in one to five steps of 32, all but one element of
+# columns and rows in whole tiles, and columns that end in every part of 256
+SHORT_K = [(2500, 132, 2564, "bfloat16"), (2601, 4, 2561, "bfloat16"), (20001, 96, 330, "float16"),
+           (6300, 160, 1088, "float16"), (3333, 100, 2000, "bfloat16"), (2500, 96, 2564, "float32"),
+           (25000, 36, 257, "float32"), (110000, 64, 60, "float32")]
+
+
+@pytest.mark.parametrize("size", SHORT_K, ids=str)
+def test_short_k(size):
+    """Rows inside wider ones, a residual in place, every activation; an infinity and a
+    NaN stay in their rows; one set of bits whatever the workspace."""
+    import torch
+    import row_operators as ro
+    m, k, n, y_type = size
+    x, w, bias, res = _operands(m, k, n, PAIRS[0], y_type)
+    wide = torch.full((m, k + 8), float("nan"), device="cuda")
+    wide[:, 4:4 + k] = x
+    view = wide[:, 4:4 + k]
+    for act, b, r in (("none", bias, None), ("gelu", None, res), ("silu", bias, res),
+                      ("gelu_tanh", bias, None)):
+        got = capi.linear(view, w, b, ro.ACTS[act], r, out_dtype=res.dtype)
+        _check(got, x, w, b, act, r)
+    none = torch.empty(0, dtype=torch.uint8, device="cuda")
+    assert torch.equal(got, capi.linear(x, w, bias, ro.ACTS["gelu_tanh"], out_dtype=res.dtype,
+                                        workspace=none))
+    out = torch.full((m + 2, n + 4), 5.0, dtype=res.dtype, device="cuda")
+    out[1:m + 1, 4:] = res
+    inner = out[1:m + 1, 4:]
+    want = capi.linear(x, w, bias, capi.ACT_SILU, res, out_dtype=res.dtype)
+    capi.linear(x, w, bias, capi.ACT_SILU, inner, out=inner)
+    assert torch.equal(inner, want)
+    assert (out[0] == 5).all() and (out[-1] == 5).all() and (out[:, :4] == 5).all()
+    plain = capi.linear(x, w, out_dtype=res.dtype)
+    view[7, 0], view[m - 1, k - 1] = float("inf"), float("nan")
+    bad = capi.linear(view, w, out_dtype=res.dtype)
+    good = [i for i in range(m) if i not in (7, m - 1)]
+    assert torch.equal(bad[good], plain[good])
+    assert not bad[7].isfinite().any() and bad[m - 1].isnan().all()
+
+
 # above 32 rows; k and n even and odd; tiles beside and below each other
 @pytest.mark.parametrize("size", [(33, 72, 48), (130, 100, 77), (129, 1000, 260), (300, 33, 513)], ids=str)
 @pytest.mark.parametrize("pair", PAIRS, ids="-".join)
