@@ -38,21 +38,20 @@ __device__ __forceinline__ float to_f32(float v) { return v; }
 __device__ __forceinline__ float to_f32(uint16_t v) { return bf16_to_f32(v); }
 __device__ __forceinline__ float to_f32(_Float16 v) { return (float)v; }
 
-// V consecutive elements as they lie in memory, aligned to min(16, their size) bytes
+typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+// in memory
+typedef u32x2 u32x2_at4 __attribute__((aligned(4)));
+typedef u32x4 u32x4_at4 __attribute__((aligned(4)));
+typedef f32x4 f32x4_at4 __attribute__((aligned(4)));
+
+// V consecutive elements as they lie in memory
 template <typename T, int V>
 struct Raw {
     alignas(V * sizeof(T) > 16 ? 16 : V * sizeof(T)) T e[V];
     __device__ __forceinline__ void load(const T* p) {
-        constexpr int B = V * (int)sizeof(T);
-        if constexpr (V == 1) {
-            e[0] = *p;
-        } else if constexpr (B == 8) {
-            *reinterpret_cast<uint2*>(e) = *reinterpret_cast<const uint2*>(p);
-        } else {
-#pragma unroll
-            for (int i = 0; i < B / 16; ++i)
-                reinterpret_cast<uint4*>(e)[i] = reinterpret_cast<const uint4*>(p)[i];
-        }
+        // vectors lie on four bytes (on two they take several times as long)
+        __builtin_memcpy(e, V > 1 ? __builtin_assume_aligned(p, 4) : p, sizeof(e));
     }
     __device__ __forceinline__ void get(float (&v)[V]) const {
 #pragma unroll
@@ -67,8 +66,13 @@ __device__ __forceinline__ void load_v(const T* p, float (&v)[V]) {
     r.get(v);
 }
 
-typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
-typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+template <bool NT, typename P, typename Q>
+__device__ __forceinline__ void put(P* at, Q q) {
+    if constexpr (NT)
+        __builtin_nontemporal_store(q, at);
+    else
+        *at = q;
+}
 
 template <int V, int KIND, bool NT = false>
 __device__ __forceinline__ void store_v(void* base, long idx, const float (&v)[V]) {
@@ -84,25 +88,19 @@ __device__ __forceinline__ void store_v(void* base, long idx, const float (&v)[V
 #pragma unroll
         for (int i = 0; i < V / 2; ++i)
             w[i] = KIND == 1 ? pack2_bf16_rne(v[2 * i], v[2 * i + 1]) : pack2_f16_rne(v[2 * i], v[2 * i + 1]);
-        typedef typename std::conditional<V == 8, u32x4, u32x2>::type Q;
-        Q q;
-#pragma unroll
-        for (int i = 0; i < V / 2; ++i) q[i] = w[i];
-        Q* at = reinterpret_cast<Q*>((uint16_t*)base + idx);
-        if (NT)
-            __builtin_nontemporal_store(q, at);
-        else
-            *at = q;
+        if constexpr (V == 2) {
+            put<NT>((u32_any*)((uint16_t*)base + idx), w[0]);
+        } else if constexpr (V == 4) {
+            put<NT>((u32x2_at4*)((uint16_t*)base + idx), u32x2{w[0], w[1]});
+        } else {
+            put<NT>((u32x4_at4*)((uint16_t*)base + idx), u32x4{w[0], w[1], w[2], w[3]});
+        }
+    } else if constexpr (V == 2) {
+        put<NT>((u32x2_at4*)((float*)base + idx), u32x2{__float_as_uint(v[0]), __float_as_uint(v[1])});
     } else {
 #pragma unroll
-        for (int i = 0; i < V; i += 4) {
-            const f32x4 q = {v[i], v[i + 1], v[i + 2], v[i + 3]};
-            f32x4* at = reinterpret_cast<f32x4*>((float*)base + idx + i);
-            if (NT)
-                __builtin_nontemporal_store(q, at);
-            else
-                *at = q;
-        }
+        for (int i = 0; i < V; i += 4)
+            put<NT>((f32x4_at4*)((float*)base + idx + i), f32x4{v[i], v[i + 1], v[i + 2], v[i + 3]});
     }
 }
 
@@ -390,7 +388,7 @@ __global__ __launch_bounds__(kThreads) void group_norm_apply_kernel(GroupNormArg
 
 // Few values: a workgroup holds a frame's group in registers, one launch in all.  The
 // mean first, then the deviations from it.
-// A thread holds up to 4 vectors of 8, or 8 of 4 or 1; 256 threads, or 1024 (2000 x 512
+// A thread holds up to 4 vectors of 8, or 8 of 4, 2 or 1; 256 threads, or 1024 (2000 x 512
 // in bf16 in 32 groups 7.3 us, 12 by two launches; 4000 x 512 with 8 vectors of 8 a
 // thread 16.6 and 13: the group's pieces of 32 bytes come to one compute unit).
 constexpr int kSmallMost = 1024;   // threads
@@ -467,15 +465,15 @@ __global__ __launch_bounds__(THREADS) void group_norm_small_kernel(GroupNormArgs
     });
 }
 
-// V channels are whole 16-byte pieces (8 bytes: four 16-bit ones) of every row of a view
-bool fits(const void* base, int kind, long frame, long pixel, int v) {
-    const int bytes = std::min(16, v * (kind ? 2 : 4));
-    return (uintptr_t)base % bytes == 0 && frame % v == 0 && pixel % v == 0;
+// Rows of a view, every one of them, start on four bytes.
+bool fits(const void* base, int kind, long frame, long pixel) {
+    return (uintptr_t)base % 4 == 0 && (!kind || (frame % 2 == 0 && pixel % 2 == 0));
 }
 
+// Channels can be taken v at a time.
 bool fits(const GroupNormArgs& p, int width, int v) {
-    return width % v == 0 && fits(p.x, p.x_kind, p.x_frame, p.x_pixel, v) &&
-           fits(p.y, p.y_kind, p.y_frame, p.y_pixel, v);
+    return width % v == 0 && fits(p.x, p.x_kind, p.x_frame, p.x_pixel) &&
+           fits(p.y, p.y_kind, p.y_frame, p.y_pixel);
 }
 
 // Whether a workgroup of so many threads can hold a frame's group of `each` channels in
@@ -537,15 +535,17 @@ hipError_t run_small(const GroupNormArgs& p, hipStream_t stream) {
 template <int XK, int YK>
 hipError_t pick(const GroupNormArgs& p, float2* parts, hipStream_t stream) {
     const int each = p.channels / p.groups;
-    for (int v : {8, 4, 1}) {
+    for (int v : {8, 4, 2, 1}) {
         if (v > 1 && !fits(p, each, v)) continue;
         if (!small_holds(p.pixels, each, v, kSmallMost)) break;
         return v == 8   ? run_small<XK, YK, 8>(p, stream)
                : v == 4 ? run_small<XK, YK, 4>(p, stream)
+               : v == 2 ? run_small<XK, YK, 2>(p, stream)
                         : run_small<XK, YK, 1>(p, stream);
     }
     if (fits(p, p.channels, 8)) return run<XK, YK, 8>(p, parts, stream);
     if (fits(p, p.channels, 4)) return run<XK, YK, 4>(p, parts, stream);
+    if (fits(p, p.channels, 2)) return run<XK, YK, 2>(p, parts, stream);
     return run<XK, YK, 1>(p, parts, stream);
 }
 

@@ -126,6 +126,7 @@ __device__ __forceinline__ bf16x8 as_bf16x8(uint4 v) {
 // Raw buffer descriptor over [base, base + bytes): loads past the end return
 // zero.  Word 3 is the gfx950 descriptor format for untyped dword access.
 typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32_any __attribute__((may_alias));   // two 16-bit elements as one
 
 __device__ __forceinline__ i32x4 buffer_rsrc(const void* base, uint32_t bytes) {
     const uint64_t a = (uint64_t)base;

@@ -116,6 +116,26 @@ def test_non_finite_values_stay_in_their_group(bad, pixels):
     assert torch.equal(got[keep], clean[keep])
 
 
+@pytest.mark.parametrize("x_type", TYPES)
+@pytest.mark.parametrize("y_type", TYPES)
+@pytest.mark.parametrize("c,g", [(2, 1), (6, 2), (18, 9), (134, 2), (40, 5), (1030, 103)])
+def test_rows_on_four_bytes_and_on_two(x_type, y_type, c, g):
+    """Channels in pieces of two and more, rows that start anywhere."""
+    import torch
+    for p in (33, 2500):
+        x, gamma, beta = _draw((2, p, c), x_type, c + p)
+        plain = capi.group_norm(x, g, gamma, beta, 1e-6, capi.ACT_SILU, out_dtype=getattr(torch, y_type))
+        _check(x, g, gamma, beta, 1e-6, "silu", plain)
+        for pad, first in ((2, 2), (4, 2), (3, 1), (1, 0)):
+            wide = torch.full((2, p, c + pad), float("nan"), dtype=x.dtype, device="cuda")
+            wide[:, :, first:first + c] = x
+            out = torch.full((2, p, c + pad), 5.0, dtype=plain.dtype, device="cuda")
+            capi.group_norm(wide[:, :, first:first + c], g, gamma, beta, 1e-6, capi.ACT_SILU,
+                            out=out[:, :, first:first + c])
+            _check(x, g, gamma, beta, 1e-6, "silu", out[:, :, first:first + c])
+            assert (out[:, :, :first] == 5).all() and (out[:, :, first + c:] == 5).all()
+
+
 @pytest.mark.parametrize("pixels", [40, 9000, 200000])
 def test_deviations_whose_squares_overflow_show(pixels):
     """Squares past fp32's range leave no plausible values: NaN, or zeros of an
