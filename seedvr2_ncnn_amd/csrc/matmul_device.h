@@ -101,6 +101,25 @@ __device__ __forceinline__ void store1(void* p, long idx, float v, int kind) {
 typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 
+// Vectors at any element: loads and stores need no more alignment than that.
+typedef u32x2 u32x2_at2 __attribute__((aligned(2)));
+typedef u32x4 u32x4_at2 __attribute__((aligned(2)));
+typedef u32x4 u32x4_at4 __attribute__((aligned(4)));
+typedef f32x4 f32x4_at4 __attribute__((aligned(4)));
+
+// Four values at any element.
+template <int YK>
+__device__ __forceinline__ void store4_any(void* p, long idx, f32x4 v) {
+    if constexpr (YK == 0)
+        *reinterpret_cast<f32x4_at4*>((float*)p + idx) = v;
+    else if constexpr (YK == 1)
+        *reinterpret_cast<u32x2_at2*>((uint16_t*)p + idx) =
+            u32x2{pack2_bf16_rne(v[0], v[1]), pack2_bf16_rne(v[2], v[3])};
+    else
+        *reinterpret_cast<u32x2_at2*>((uint16_t*)p + idx) =
+            u32x2{pack2_f16_rne(v[0], v[1]), pack2_f16_rne(v[2], v[3])};
+}
+
 constexpr int kRawBufferFormat = 0x00020000;   // word 3 of an untyped buffer descriptor
 constexpr uint32_t kOutside = 0x80000000u;     // an offset past every descriptor's end
 
@@ -117,11 +136,13 @@ struct TileEnd {
     static constexpr int D = NI < 4 ? NI : YK == 0 && NI == 8 ? 2 : 4;   // by registers
     typedef typename std::conditional<YK == 0, u32x4, u32x2>::type Piece;   // four columns
 
-    const char *y, *res;
+    char* y;
+    const char* res;
     int y_bytes, res_bytes;
     uint32_t y_at, res_at, y_row, res_row;   // of the lane's first piece; bytes between rows
     uint32_t drop[4];                        // of column col + j
-    bool whole;                              // pieces of four, else single elements
+    bool whole;                              // pieces of four through the descriptors
+    bool four;                               // else: this lane's four columns are all in the row
     f32x4 bias;
     Piece held[D][4];
 
@@ -129,7 +150,7 @@ struct TileEnd {
                                        int col, bool whole_pieces) {
         const int g = (threadIdx.x & 63) >> 4;
         whole = whole_pieces;
-        y = (const char*)a.y + (long)rt.row0 * a.y_stride * ES;
+        y = (char*)a.y + (long)rt.row0 * a.y_stride * ES;
         y_bytes = (int)(((long)(rows - 1) * a.y_stride + a.n) * ES);
         y_row = (uint32_t)(a.y_stride * ES);
         y_at = (row_w + 4 * g) * y_row + col * ES;
@@ -139,6 +160,7 @@ struct TileEnd {
         res_at = (row_w + 4 * g) * res_row + col * ES;
 #pragma unroll
         for (int j = 0; j < 4; ++j) drop[j] = col + j < a.n ? 0u : kOutside;
+        four = !(YK == 0 && NI == 8) && col + 3 < a.n;   // (there it spills, and gains 4%)
         bias = f32x4{0.f, 0.f, 0.f, 0.f};
         if (a.bias) {
             const __amdgpu_buffer_rsrc_t rb = __builtin_amdgcn_make_buffer_rsrc(
@@ -161,6 +183,14 @@ struct TileEnd {
             const uint32_t at = res_at + (16 * i + r) * res_row;
             Piece& q = held[i % D][r];
             if (!whole) {
+                if (four) {
+                    if constexpr (YK == 0) {   // 16 bytes through a descriptor at any fourth
+                        q = __builtin_amdgcn_raw_buffer_load_b128(rs, at, 0, 0);
+                    } else {
+                        q = Piece{};
+                        if (at < (uint32_t)res_bytes) q = *reinterpret_cast<const u32x2_at2*>(res + at);
+                    }
+                } else
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const uint32_t o = (at + j * ES) | drop[j];
@@ -218,6 +248,12 @@ struct TileEnd {
                                        : pack2_f16_rne(v[r][2 * j], v[r][2 * j + 1]);
                 }
                 if constexpr (!WHOLE) {
+                    if (four) {
+                        if constexpr (YK == 0)
+                            __builtin_amdgcn_raw_buffer_store_b128(q, rs, at, 0, 0);
+                        else if (at < (uint32_t)y_bytes)
+                            *reinterpret_cast<u32x2_at2*>(y + at) = q;
+                    } else
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         const uint32_t o = (at + j * ES) | drop[j];
@@ -272,42 +308,43 @@ __device__ __forceinline__ void split8(const float (&v)[8], uint4 (&out)[PL]) {
     for (int q = 0; q < PL; ++q) out[q] = make_uint4(w[0][q], w[1][q], w[2][q], w[3][q]);
 }
 
-// Eight consecutive k of a row as an MFMA operand piece.  GRAN elements lie together
-// (8: 16 bytes of 16-bit elements, 4, or 1); FULL: all eight are before k.
-template <int GRAN, bool FULL>
+// Eight consecutive k of a row as an MFMA operand piece, zeros from `left` of them on.
+// FULL: all eight are there.  ODD: rows may begin in the middle of four bytes, where a
+// 16-byte load takes several times as long (1 x 5001 by 5000 x 5001: 31 us): the four or
+// five words that hold the eight are loaded and shifted.
+template <bool FULL, bool ODD = false>
 __device__ __forceinline__ uint4 piece16(const uint16_t* p, int left) {
-    if constexpr (GRAN == 8) {
-        if (FULL || left > 0) return *reinterpret_cast<const uint4*>(p);
-        return make_uint4(0, 0, 0, 0);
-    } else {
-        alignas(16) uint16_t h[8];
-#pragma unroll
-        for (int e = 0; e < 8; e += GRAN) {
-            if constexpr (GRAN == 4) {
-                uint2 q = make_uint2(0, 0);
-                if (FULL || left > e) q = *reinterpret_cast<const uint2*>(p + e);
-                *reinterpret_cast<uint2*>(h + e) = q;
-            } else {
-                h[e] = FULL || left > e ? p[e] : (uint16_t)0;
-            }
+    if constexpr (ODD) {
+        if (FULL || left >= 8) {
+            const uint32_t odd = (uintptr_t)p >> 1 & 1;
+            const u32_any* a = (const u32_any*)(p - odd);
+            const u32x4 q = *reinterpret_cast<const u32x4_at4*>(a);
+            const uint32_t top = a[3 + odd], s = 16 * odd;
+            return make_uint4(__builtin_amdgcn_alignbit(q[1], q[0], s), __builtin_amdgcn_alignbit(q[2], q[1], s),
+                              __builtin_amdgcn_alignbit(q[3], q[2], s), __builtin_amdgcn_alignbit(top, q[3], s));
         }
-        return pack8_bf16(h);
+    } else if (FULL || left >= 8) {
+        const u32x4 q = *reinterpret_cast<const u32x4_at2*>(p);
+        return make_uint4(q[0], q[1], q[2], q[3]);
     }
+    alignas(16) uint16_t h[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) h[e] = left > e ? p[e] : (uint16_t)0;
+    return pack8_bf16(h);
 }
 
-template <int GRAN, bool FULL>
+template <bool FULL>
 __device__ __forceinline__ void piece32(const float* p, int left, float (&v)[8]) {
+    if (FULL || left >= 8) {
 #pragma unroll
-    for (int e = 0; e < 8; e += 4) {
-        if constexpr (GRAN >= 4) {
-            f32x4 q = {0.f, 0.f, 0.f, 0.f};
-            if (FULL || left > e) q = *reinterpret_cast<const f32x4*>(p + e);
+        for (int e = 0; e < 8; e += 4) {
+            const f32x4 q = *reinterpret_cast<const f32x4_at4*>(p + e);
 #pragma unroll
             for (int i = 0; i < 4; ++i) v[e + i] = q[i];
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[e + i] = FULL || left > e + i ? p[e + i] : 0.f;
         }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = left > e ? p[e] : 0.f;
     }
 }
 

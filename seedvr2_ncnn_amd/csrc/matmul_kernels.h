@@ -44,15 +44,6 @@ inline long row_tiles(const MatmulArgs& a, int tm) {
     return ((long)a.m + (long)std::min(a.groups, a.m) * (tm - 1)) / tm;
 }
 
-// Elements that lie together in every row of x and of the weight.
-inline int row_gran(const MatmulArgs& a) {
-    for (int e : {8, 4})
-        if (a.k % e == 0 && a.x_stride % e == 0 && (uintptr_t)a.w % (2 * e) == 0 &&
-            (uintptr_t)a.x % (a.x_kind ? 2 * e : 16) == 0)
-            return e;
-    return 1;
-}
-
 // A call's kernel and what it keeps in the workspace.
 struct MatmulPlan {
     enum Kernel { kRows, kTiles, kShort, kAny } kernel;

@@ -29,8 +29,8 @@ bool whole_pieces(const MatmulArgs& a) {
 // Any strides, alignment, n and k; fp32 activations.  Block tile 128x128,
 // k-step 32, four waves in a 2x2 grid of 64x64, both operands through registers
 // into double-buffered LDS.  XP: bf16 planes that stand for an fp32 x (0: x is of
-// the weight's type).  GRAN: elements loaded at once, 4 where rows allow it, or 1.
-template <int T, int XP, int GRAN, int YK>
+// the weight's type).
+template <int T, int XP, int YK>
 __global__ __launch_bounds__(256, 2) void matmul_any_kernel(MatmulArgs a, int ntiles, bool whole) {
     constexpr int BM = 128, BN = 128, BK = 32, P = BK + 8, PL = XP ? XP : 1;
     __shared__ __attribute__((aligned(16))) uint16_t x_lds[2][PL][BM * P];
@@ -53,41 +53,20 @@ __global__ __launch_bounds__(256, 2) void matmul_any_kernel(MatmulArgs a, int nt
 
     // thread -> (LDS row, quarter of 8 k) twice per operand
     float xf[XP ? 2 : 1][8];
-    alignas(16) uint16_t xr[2][8], wr[2][8];
+    uint4 xr[2], wr[2];
     auto load = [&](int k0) {
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
             const int r = (tid >> 2) + 64 * c;
             const int kc = k0 + (tid & 3) * 8;
             const int col = col0 + (r & ~63) + 4 * (r & 15) + ((r >> 4) & 3);
-            const bool xin = r < rows, win = col < a.n;
             const long xo = (long)(rt.row0 + r) * a.x_stride + kc;
-            const long wo = (long)col * a.k + kc;
-#pragma unroll
-            for (int e = 0; e < 8; e += GRAN) {
-                const bool kin = kc + e < a.k;
-                if constexpr (GRAN == 4) {
-                    uint2 q = make_uint2(0, 0);
-                    if (win && kin) q = *reinterpret_cast<const uint2*>(w + wo + e);
-                    *reinterpret_cast<uint2*>(&wr[c][e]) = q;
-                    if constexpr (XP) {
-                        f32x4 q4 = {0.f, 0.f, 0.f, 0.f};
-                        if (xin && kin) q4 = *reinterpret_cast<const f32x4*>((const float*)a.x + xo + e);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) xf[c][e + i] = q4[i];
-                    } else {
-                        q = make_uint2(0, 0);
-                        if (xin && kin) q = *reinterpret_cast<const uint2*>((const uint16_t*)a.x + xo + e);
-                        *reinterpret_cast<uint2*>(&xr[c][e]) = q;
-                    }
-                } else {
-                    wr[c][e] = win && kin ? w[wo + e] : (uint16_t)0;
-                    if constexpr (XP)
-                        xf[c][e] = xin && kin ? ((const float*)a.x)[xo + e] : 0.f;
-                    else
-                        xr[c][e] = xin && kin ? ((const uint16_t*)a.x)[xo + e] : (uint16_t)0;
-                }
-            }
+            wr[c] = piece16<false>(w + (long)col * a.k + kc, col < a.n ? a.k - kc : 0);
+            const int left = r < rows ? a.k - kc : 0;
+            if constexpr (XP)
+                piece32<false>((const float*)a.x + xo, left, xf[c]);
+            else
+                xr[c] = piece16<false>((const uint16_t*)a.x + xo, left);
         }
     };
     auto put = [&](int buf) {
@@ -95,14 +74,14 @@ __global__ __launch_bounds__(256, 2) void matmul_any_kernel(MatmulArgs a, int nt
         for (int c = 0; c < 2; ++c) {
             const int r = (tid >> 2) + 64 * c;
             const int at = r * P + (tid & 3) * 8;
-            *reinterpret_cast<uint4*>(&w_lds[buf][at]) = pack8_bf16(wr[c]);
+            *reinterpret_cast<uint4*>(&w_lds[buf][at]) = wr[c];
             if constexpr (XP) {
                 uint4 h[PL];
                 split8<PL>(xf[c], h);
 #pragma unroll
                 for (int i = 0; i < PL; ++i) *reinterpret_cast<uint4*>(&x_lds[buf][i][at]) = h[i];
             } else {
-                *reinterpret_cast<uint4*>(&x_lds[buf][0][at]) = pack8_bf16(xr[c]);
+                *reinterpret_cast<uint4*>(&x_lds[buf][0][at]) = xr[c];
             }
         }
     };
@@ -145,13 +124,7 @@ hipError_t launch_any(const MatmulArgs& a, hipStream_t stream) {
     const int ntiles = (a.n + 127) / 128;
     const long blocks = row_tiles(a, 128) * ntiles;
     if (blocks > 0x7fffffffL) return hipErrorInvalidValue;
-    const bool four = a.k % 4 == 0 && a.x_stride % 4 == 0 && (uintptr_t)a.x % (XP ? 16 : 8) == 0 &&
-                      (uintptr_t)a.w % 8 == 0;
-    const bool whole = whole_pieces(a);
-    if (four)
-        matmul_any_kernel<T, XP, 4, YK><<<(unsigned)blocks, 256, 0, stream>>>(a, ntiles, whole);
-    else
-        matmul_any_kernel<T, XP, 1, YK><<<(unsigned)blocks, 256, 0, stream>>>(a, ntiles, whole);
+    matmul_any_kernel<T, XP, YK><<<(unsigned)blocks, 256, 0, stream>>>(a, ntiles, whole_pieces(a));
     return hipGetLastError();
 }
 
@@ -161,13 +134,12 @@ hipError_t launch_any(const MatmulArgs& a, hipStream_t stream) {
 struct PackJob {
     const void* src;
     int kind;           // 0 fp32, else 16 bits
-    bool vec;           // source rows in pieces of four elements
     long stride, rows;
     int planes, width;
     uint16_t* dst;
 };
 
-template <int PL, bool VEC>
+template <int PL>
 __device__ __forceinline__ void pack_piece(const PackJob& job, int k, long i) {
     const int pieces = job.width / 8;
     const long row = i / pieces;
@@ -176,12 +148,12 @@ __device__ __forceinline__ void pack_piece(const PackJob& job, int k, long i) {
     if (job.kind == 0) {
         float v[8];
         uint4 h[PL];
-        piece32<VEC ? 4 : 1, false>((const float*)job.src + row * job.stride + kc, k - kc, v);
+        piece32<false>((const float*)job.src + row * job.stride + kc, k - kc, v);
         split8<PL>(v, h);
 #pragma unroll
         for (int q = 0; q < PL; ++q) *reinterpret_cast<uint4*>(out + (long)q * job.width) = h[q];
     } else {
-        const uint4 h = piece16<VEC ? 4 : 1, false>((const uint16_t*)job.src + row * job.stride + kc, k - kc);
+        const uint4 h = piece16<false>((const uint16_t*)job.src + row * job.stride + kc, k - kc);
         for (int q = 0; q < job.planes; ++q) *reinterpret_cast<uint4*>(out + (long)q * job.width) = h;
     }
 }
@@ -191,23 +163,11 @@ template <int PL>
 __global__ __launch_bounds__(256) void matmul_pack_kernel(PackJob x, PackJob w, int k) {
     const long nx = x.rows * (x.width / 8), all = nx + w.rows * (w.width / 8);
     for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < all; i += (long)gridDim.x * 256) {
-        if (i < nx) {
-            if (x.vec)
-                pack_piece<PL, true>(x, k, i);
-            else
-                pack_piece<PL, false>(x, k, i);
-        } else if (w.vec) {
-            pack_piece<PL, true>(w, k, i - nx);
-        } else {
-            pack_piece<PL, false>(w, k, i - nx);
-        }
+        if (i < nx)
+            pack_piece<PL>(x, k, i);
+        else
+            pack_piece<PL>(w, k, i - nx);
     }
-}
-
-PackJob pack_job(const void* src, int kind, long stride, long rows, int k, int planes, int width,
-                 uint16_t* dst) {
-    return PackJob{src, kind, k % 4 == 0 && stride % 4 == 0 && (uintptr_t)src % (kind ? 8 : 16) == 0,
-                   stride, rows, planes, width, dst};
 }
 
 hipError_t launch_pack(const PackJob& x, const PackJob& w, int k, hipStream_t stream) {
@@ -308,7 +268,7 @@ MatmulPlan plan_matmul(const MatmulArgs& a, size_t workspace_bytes) {
     // and 21600 10.6 -> 11.1, 26 -> 18; fewer outputs gain only where the weight would be
     // packed too
     if (a.x_kind == 0 && !a.offsets && rows > 32 && (long)a.m * a.n >= 6L << 20 && near &&
-        (a.k + 31) / 32 <= matmul_short_steps(packed_planes(a)) && row_gran(a) >= 4 &&
+        (a.k + 31) / 32 <= matmul_short_steps(packed_planes(a)) &&
         a.x_stride < 1L << 24) {
         MatmulPlan s{};
         s.kernel = MatmulPlan::kShort;
@@ -386,9 +346,9 @@ hipError_t launch_matmul(const MatmulArgs& args, void* workspace, size_t workspa
     char* at = (char*)workspace;
     if (p.pack_x) {
         const int planes = packed_planes(a), width = (int)packed_width(a, p.pack_w);
-        const PackJob x = pack_job(a.x, a.x_kind, a.x_stride, a.m, a.k, planes, width, (uint16_t*)at);
-        const PackJob w = pack_job(a.w, a.w_kind, a.k, p.pack_w ? (long)a.groups * a.n : 0, a.k, planes,
-                                   width, (uint16_t*)(at + p.x_bytes));
+        const PackJob x{a.x, a.x_kind, a.x_stride, a.m, planes, width, (uint16_t*)at};
+        const PackJob w{a.w, a.w_kind, a.k, p.pack_w ? (long)a.groups * a.n : 0, planes, width,
+                        (uint16_t*)(at + p.x_bytes)};
         const hipError_t e = launch_pack(x, w, a.k, stream);
         if (e != hipSuccess) return e;
         a.x = x.dst;

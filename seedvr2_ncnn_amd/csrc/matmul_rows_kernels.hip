@@ -13,7 +13,7 @@ namespace {
 //
 // PL bf16 terms stand for a value of an fp32 x, split here by every workgroup; 1: x is of
 // the weight's type.
-template <int T, int PL, int MT, int NT, int GRAN>
+template <int T, int PL, int MT, int NT, bool ODD>
 __global__ __launch_bounds__(512) void matmul_rows_kernel(MatmulArgs a, int ntiles) {
     constexpr bool SPLIT = PL > 1;
     constexpr int REGS = 2 * 4 * (NT + MT * (SPLIT ? 2 : 1));   // of a 64-k chunk
@@ -56,13 +56,13 @@ __global__ __launch_bounds__(512) void matmul_rows_kernel(MatmulArgs a, int ntil
             const int kc = k0 + (c >> 1) * waves * 64 + (c & 1) * 32;
             const int left = a.k - kc - 8 * g;
 #pragma unroll
-            for (int j = 0; j < NT; ++j) b.w[c][j] = piece16<GRAN, FULL>(w[j] + kc, left);
+            for (int j = 0; j < NT; ++j) b.w[c][j] = piece16<FULL, ODD>(w[j] + kc, left);
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
                 if constexpr (SPLIT)
-                    piece32<GRAN, FULL>((const float*)a.x + xo[i] + kc, left, b.f[c][i]);
+                    piece32<FULL>((const float*)a.x + xo[i] + kc, left, b.f[c][i]);
                 else
-                    b.x[c][i] = piece16<GRAN, FULL>((const uint16_t*)a.x + xo[i] + kc, left);
+                    b.x[c][i] = piece16<FULL, ODD>((const uint16_t*)a.x + xo[i] + kc, left);
             }
         }
     };
@@ -139,26 +139,23 @@ __global__ __launch_bounds__(512) void matmul_rows_kernel(MatmulArgs a, int ntil
     }
 }
 
-template <int T, int PL, int MT, int NT, int GRAN>
+template <int T, int PL, int MT, int NT, bool ODD>
 hipError_t run(const MatmulArgs& a, hipStream_t stream) {
     const int ntiles = (a.n + 16 * NT - 1) / (16 * NT);
     const long blocks = row_tiles(a, 16 * MT) * ntiles;
     if (blocks > 0x7fffffffL) return hipErrorInvalidValue;
     const int waves = std::min(8, (a.k + 63) / 64);
-    matmul_rows_kernel<T, PL, MT, NT, GRAN><<<(unsigned)blocks, 64 * waves, 0, stream>>>(a, ntiles);
+    matmul_rows_kernel<T, PL, MT, NT, ODD><<<(unsigned)blocks, 64 * waves, 0, stream>>>(a, ntiles);
     return hipGetLastError();
 }
 
 template <int T, int PL, int MT>
 hipError_t pick(const MatmulArgs& a, int cols, hipStream_t stream) {
-    const int gran = row_gran(a);
-    if (gran == 8) {
-        constexpr int MOST = MT * PL <= 4 ? 4 : 2;   // by registers
-        if (cols == 64) return run<T, PL, MT, MOST, 8>(a, stream);
-        if (cols == 32) return run<T, PL, MT, 2, 8>(a, stream);
-        return run<T, PL, MT, 1, 8>(a, stream);
-    }
-    return gran == 4 ? run<T, PL, MT, 1, 4>(a, stream) : run<T, PL, MT, 1, 1>(a, stream);
+    constexpr int MOST = MT * PL <= 4 ? 4 : 2;   // by registers
+    const bool odd = (a.k & 1) || (uintptr_t)a.w % 4 || (a.x_kind && ((a.x_stride & 1) || (uintptr_t)a.x % 4));
+    if (odd) return run<T, PL, MT, 1, true>(a, stream);
+    if (cols == 64) return run<T, PL, MT, MOST, false>(a, stream);
+    return cols == 32 ? run<T, PL, MT, 2, false>(a, stream) : run<T, PL, MT, 1, false>(a, stream);
 }
 
 template <int T, int PL>

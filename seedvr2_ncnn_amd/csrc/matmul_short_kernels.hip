@@ -2,9 +2,9 @@
 //
 // On block tiles a workgroup's first loads and its epilogue are as long as a few k
 // steps, and fp32 rows are packed before.  Here a workgroup keeps the weight rows of
-// 256 columns in LDS for its whole life, and each of its waves takes 32 rows at a time
+// 256 columns in LDS for its whole life, and each of its waves takes 16 rows at a time
 // on its own: their k straight from memory into registers, split there into bf16 terms
-// once for the 256 columns, then 128 columns after 128.  No wave waits for another once
+// once for the 256 columns, then 64 columns after 64.  No wave waits for another once
 // the weight is there, so that one stores or loads while another multiplies.
 #include "matmul_device.h"
 
@@ -17,8 +17,16 @@ constexpr int kCols = 256, kRows = 16;
 // Waves of a workgroup, by registers.
 constexpr int waves_of(int pl) { return pl == 2 ? 16 : 12; }
 
-// PL: bf16 terms of a value; STEPS: k steps of 32, zeros past k.  Rows of x lie on 16
-// bytes, of the weight on eight.
+// Four of a row's k, zeros from `left` of them on.
+__device__ __forceinline__ u32x2 four16(const uint16_t* p, int left) {
+    if (left >= 4) return *reinterpret_cast<const u32x2_at2*>(p);
+    uint32_t h[3];
+#pragma unroll
+    for (int e = 0; e < 3; ++e) h[e] = left > e ? p[e] : 0;
+    return u32x2{h[0] | h[1] << 16, h[2]};
+}
+
+// PL: bf16 terms of a value; STEPS: k steps of 32, zeros past k.
 template <int PL, int YK, int STEPS>
 __global__ __launch_bounds__(64 * waves_of(PL)) void matmul_short_kernel(MatmulArgs a, int blocks_n, int splits,
                                                            bool whole) {
@@ -62,26 +70,23 @@ __global__ __launch_bounds__(64 * waves_of(PL)) void matmul_short_kernel(MatmulA
             }
     };
     load(t0);
-    const __amdgpu_buffer_rsrc_t ws = __builtin_amdgcn_make_buffer_rsrc(
-        (void*)((const uint16_t*)a.w + (long)col0 * a.k), (short)0, cols * a.k * 2, kRawBufferFormat);
+    const uint16_t* w = (const uint16_t*)a.w + (long)col0 * a.k;
     constexpr int ALL = kCols * PIECES, EACH = (ALL + kThreads - 1) / kThreads;   // pieces of a thread
     u32x2 h[EACH][2];
 #pragma unroll
     for (int b = 0; b < EACH; ++b) {
         const int i = tid + kThreads * b, r = i / PIECES, u = i % PIECES;
-        const int k = 32 * (u >> 2) + 4 * (u & 3);
-        const uint32_t row = ((r & ~63) + 4 * (r & 15) + ((r >> 4) & 3)) * a.k;
+        const int k = 32 * (u >> 2) + 4 * (u & 3), col = (r & ~63) + 4 * (r & 15) + ((r >> 4) & 3);
 #pragma unroll
         for (int e = 0; e < 2; ++e)
-            h[b][e] = __builtin_amdgcn_raw_buffer_load_b64(
-                ws, (row + k + 16 * e) * 2 | (k + 16 * e < a.k && i < ALL ? 0u : kOutside), 0, 0);
+            h[b][e] = four16(w + (long)col * a.k + k + 16 * e, col < cols && i < ALL ? a.k - k - 16 * e : 0);
     }
 #pragma unroll
     for (int b = 0; b < EACH; ++b) {
         const int i = tid + kThreads * b;
         if (ALL % kThreads == 0 || i < ALL)
             *reinterpret_cast<uint4*>(&w_lds[i / PIECES * P + i % PIECES * 8]) =
-            make_uint4(h[b][0][0], h[b][0][1], h[b][1][0], h[b][1][1]);
+                make_uint4(h[b][0][0], h[b][0][1], h[b][1][0], h[b][1][1]);
     }
     if (tid < kCols) bias[tid] = a.bias && tid < cols ? a.bias[col0 + tid] : 0.f;
     __syncthreads();
@@ -92,6 +97,14 @@ __global__ __launch_bounds__(64 * waves_of(PL)) void matmul_short_kernel(MatmulA
     for (int t = t0; t < t1; t += kWaves) {
         const RowTile rt{t * kRows, a.m, 0};
         const int rows = min(a.m - rt.row0, kRows);
+        if (a.k % 4 != 0)   // four values may end in the next row
+#pragma unroll
+            for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+                for (int e = 0; e < 8; e += 4)
+#pragma unroll
+                    for (int v = 1; v < 4; ++v)
+                        if (32 * s + 4 * g + 4 * e + v >= a.k) f[s][e + v] = 0.f;
         uint4 fx[STEPS][PL];
 #pragma unroll
         for (int s = 0; s < STEPS; ++s) split8<PL>(f[s], fx[s]);

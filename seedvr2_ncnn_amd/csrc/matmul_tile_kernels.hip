@@ -377,6 +377,8 @@ __global__ __launch_bounds__(256) void matmul_sum_kernel(MatmulArgs a, TileSplit
         const long at = row * a.y_stride + col;
         if (sp.whole) {
             store4(a.y, at, v[0], v[1], v[2], v[3], YK);
+        } else if (cols == 4) {
+            store4_any<YK>(a.y, at, v);
         } else {
 #pragma unroll
             for (int j = 0; j < 4; ++j)
