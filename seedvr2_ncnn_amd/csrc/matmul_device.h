@@ -126,7 +126,10 @@ constexpr uint32_t kOutside = 0x80000000u;     // an offset past every descripto
 // Epilogue of a wave's tile of 16 NI rows and 64 columns: accumulator [i][j][r] is row
 // 16 i + 4 g + r from row_w on, column col + j.  y and the residual go through buffer
 // descriptors that end with the block tile's rows, so the range check drops what lies
-// outside, without a branch.  The residual of up to D row tiles is in flight.
+// outside, without a branch.  The residual of up to D row tiles is in flight.  Rows that
+// four columns do not divide, or that begin anywhere: a lane whose four columns are in
+// the row stores them by one unaligned store, the last ones one at a time (8000 x 2560 by
+// 2001 x 2560 in bf16 66 us, 74 with single ones; 64 with 2000 columns).
 //
 // With 64-bit addresses, a branch a row and the residual of one row tile at a time this
 // took 8.7 of 19.5 us of 14400 x 512 by 512 x 512 with a residual.
@@ -141,8 +144,8 @@ struct TileEnd {
     int y_bytes, res_bytes;
     uint32_t y_at, res_at, y_row, res_row;   // of the lane's first piece; bytes between rows
     uint32_t drop[4];                        // of column col + j
-    bool whole;                              // pieces of four through the descriptors
-    bool four;                               // else: this lane's four columns are all in the row
+    bool whole;   // aligned pieces of four in every row
+    bool four;    // else: this lane's four columns are all in the row
     f32x4 bias;
     Piece held[D][4];
 
@@ -160,7 +163,7 @@ struct TileEnd {
         res_at = (row_w + 4 * g) * res_row + col * ES;
 #pragma unroll
         for (int j = 0; j < 4; ++j) drop[j] = col + j < a.n ? 0u : kOutside;
-        four = !(YK == 0 && NI == 8) && col + 3 < a.n;   // (there it spills, and gains 4%)
+        four = col + 3 < a.n;
         bias = f32x4{0.f, 0.f, 0.f, 0.f};
         if (a.bias) {
             const __amdgpu_buffer_rsrc_t rb = __builtin_amdgcn_make_buffer_rsrc(
@@ -169,12 +172,13 @@ struct TileEnd {
             for (int j = 0; j < 4; ++j)
                 bias[j] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rb, (col + j) * 4, 0, 0));
         }
-        if (res)
+        if (res && whole)
 #pragma unroll
-            for (int i = 0; i < D; ++i) load(i);
+            for (int i = 0; i < D; ++i) load<true>(i);
     }
 
     // the residual of row tile i
+    template <bool WHOLE>
     __device__ __forceinline__ void load(int i) {
         const __amdgpu_buffer_rsrc_t rs =
             __builtin_amdgcn_make_buffer_rsrc((void*)res, (short)0, res_bytes, kRawBufferFormat);
@@ -182,15 +186,19 @@ struct TileEnd {
         for (int r = 0; r < 4; ++r) {
             const uint32_t at = res_at + (16 * i + r) * res_row;
             Piece& q = held[i % D][r];
-            if (!whole) {
-                if (four) {
-                    if constexpr (YK == 0) {   // 16 bytes through a descriptor at any fourth
-                        q = __builtin_amdgcn_raw_buffer_load_b128(rs, at, 0, 0);
-                    } else {
-                        q = Piece{};
-                        if (at < (uint32_t)res_bytes) q = *reinterpret_cast<const u32x2_at2*>(res + at);
-                    }
-                } else
+            if constexpr (WHOLE) {
+                if constexpr (YK == 0)
+                    q = __builtin_amdgcn_raw_buffer_load_b128(rs, at | drop[0], 0, 0);
+                else
+                    q = __builtin_amdgcn_raw_buffer_load_b64(rs, at | drop[0], 0, 0);
+            } else if (four) {
+                if constexpr (YK == 0) {   // 16 bytes through a descriptor at any fourth
+                    q = __builtin_amdgcn_raw_buffer_load_b128(rs, at, 0, 0);
+                } else {
+                    q = Piece{};
+                    if (at < (uint32_t)res_bytes) q = *reinterpret_cast<const u32x2_at2*>(res + at);
+                }
+            } else {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const uint32_t o = (at + j * ES) | drop[j];
@@ -201,10 +209,6 @@ struct TileEnd {
                         q[j >> 1] = j & 1 ? q[j >> 1] | (h << 16) : h;
                     }
                 }
-            } else if constexpr (YK == 0) {
-                q = __builtin_amdgcn_raw_buffer_load_b128(rs, at | drop[0], 0, 0);
-            } else {
-                q = __builtin_amdgcn_raw_buffer_load_b64(rs, at | drop[0], 0, 0);
             }
         }
     }
@@ -213,6 +217,9 @@ struct TileEnd {
     __device__ __forceinline__ void emit(const f32x4 (&acc)[NI][4]) {
         const __amdgpu_buffer_rsrc_t rs =
             __builtin_amdgcn_make_buffer_rsrc((void*)y, (short)0, y_bytes, kRawBufferFormat);
+        if (!WHOLE && res)
+#pragma unroll
+            for (int i = 0; i < D; ++i) load<false>(i);
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
             float v[4][4];
@@ -232,7 +239,7 @@ struct TileEnd {
                             v[r][j] += YK == 1 ? bf16_to_f32(h) : (float)__builtin_bit_cast(_Float16, h);
                         }
                     }
-                if (i + D < NI) load(i + D);
+                if (i + D < NI) load<WHOLE>(i + D);
             }
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
