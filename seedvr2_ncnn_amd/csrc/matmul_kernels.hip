@@ -263,10 +263,10 @@ MatmulPlan plan_matmul(const MatmulArgs& a, size_t workspace_bytes) {
     const bool tiles = near && room && 256 * pitch * 2 < 0x7fffffffL &&
                        256 * std::max<long>(a.k, p.pack_w ? row : 0) * 2 < 0x7fffffffL;
 
-    // many fp32 rows of a short k.  By 2560 x 132 rows of 2700 17 -> 13 us, 21600 64 -> 41
-    // (packed and on tiles -> here); by 2560 x 160 17 -> 17, 65 -> 52; by 1024 x 64 of 5000
-    // and 21600 10.6 -> 11.1, 26 -> 18; fewer outputs gain only where the weight would be
-    // packed too
+    // many fp32 rows of a short k, packed and on tiles -> here: by 2560 x 132 2700 rows 17
+    // -> 13 us, 21600 66 -> 43; by 2560 x 160 17 -> 17 and 65 -> 52; by 1024 x 64 5000 rows
+    // 10.6 -> 11.1, 21600 26 -> 18.  Fewer outputs gain only where the weight would be
+    // packed too.
     if (a.x_kind == 0 && !a.offsets && rows > 32 && (long)a.m * a.n >= 6L << 20 && near &&
         (a.k + 31) / 32 <= matmul_short_steps(packed_planes(a)) &&
         a.x_stride < 1L << 24) {

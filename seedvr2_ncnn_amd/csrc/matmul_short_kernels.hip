@@ -6,6 +6,12 @@
 // on its own: their k straight from memory into registers, split there into bf16 terms
 // once for the 256 columns, then 64 columns after 64.  No wave waits for another once
 // the weight is there, so that one stores or loads while another multiplies.
+//
+// 21600 x 132 by 2560 x 132, bf16 results: 43 us.  The 110 MB of y take 21, and each of
+// a compute unit's matrix, vector (the terms and the epilogue) and LDS pipes is busy for
+// 15 to 18; without its stores the kernel took two thirds of the time, without its
+// matrix instructions half.  32 rows a wave halve the LDS reads, but leave registers for
+// eight waves only, and took 9% longer.
 #include "matmul_device.h"
 
 namespace s2 {
