@@ -176,11 +176,12 @@ def test_with_and_without_workspace(m, k, n):
         assert torch.equal(got, again)
 
 
-# many fp32 rows of short k: k in one to five steps of 32, all but one element of
-# columns and rows in whole tiles, and columns that end in every part of 256
+# many fp32 rows of short k: k in one to five steps of 32, whole quads of it or not;
+# rows and columns in and out of whole tiles
 SHORT_K = [(2500, 132, 2564, "bfloat16"), (2601, 4, 2561, "bfloat16"), (20001, 96, 330, "float16"),
            (6300, 160, 1088, "float16"), (3333, 100, 2000, "bfloat16"), (2500, 96, 2564, "float32"),
-           (25000, 36, 257, "float32"), (110000, 64, 60, "float32")]
+           (25000, 36, 257, "float32"), (110000, 64, 60, "float32"), (2500, 133, 2564, "bfloat16"),
+           (7001, 1, 1000, "float16"), (6300, 158, 1088, "bfloat16"), (2500, 95, 2563, "float32")]
 
 
 @pytest.mark.parametrize("size", SHORT_K, ids=str)
@@ -214,6 +215,28 @@ def test_short_k(size):
     good = [i for i in range(m) if i not in (7, m - 1)]
     assert torch.equal(bad[good], plain[good])
     assert not bad[7].isfinite().any() and bad[m - 1].isnan().all()
+
+
+# k, n and strides of every parity, so that rows begin anywhere; few rows and tiles
+@pytest.mark.parametrize("m", [1, 17, 32, 70, 300])
+@pytest.mark.parametrize("pair", PAIRS, ids="-".join)
+@pytest.mark.parametrize("kn", [(5001, 67), (515, 130), (262, 129), (1023, 258)], ids=str)
+def test_rows_that_begin_anywhere(m, pair, kn):
+    import torch
+    k, n = kn
+    x, w, bias, res = _operands(m, k, n, pair, "float16" if pair[0] == "float16" else "bfloat16")
+    for first, pad in ((0, 0), (1, 2), (2, 3), (3, 6)):
+        wide = torch.full((m, first + k + pad), float("nan"), dtype=x.dtype, device="cuda")
+        wide[:, first:first + k] = x
+        flat = torch.full((first + n * k + 9,), float("nan"), dtype=w.dtype, device="cuda")
+        odd = flat[first:first + n * k].view(n, k)
+        odd.copy_(w)
+        out = torch.full((m + 1, first + n + pad), 5.0, dtype=res.dtype, device="cuda")
+        inner = out[:m, first:first + n]
+        inner.copy_(res)
+        capi.linear(wide[:, first:first + k], odd, bias, capi.ACT_NONE, inner, out=inner)
+        _check(inner, x, w, bias, "none", res)
+        assert (out[m] == 5).all() and (out[:, :first] == 5).all() and (out[:, first + n:] == 5).all()
 
 
 # above 32 rows; k and n even and odd; tiles beside and below each other
