@@ -528,9 +528,8 @@ S2_API int s2_group_norm(const void* x, s2_dtype x_dtype, long x_frame_stride,
  *
  * x: device [m][k] in x_dtype, row stride x_stride >= k; weight: device [n][k]
  *   in w_dtype, contiguous; BF16 with F32 or BF16 x, or F16 with F16 x.  The
- *   products are those of the operands as given: an fp32 x is taken as two
- *   (y 16 bits wide: to 2^-15) or three (exactly) bf16 terms on the matrix
- *   cores.  An infinity or NaN of x reaches its row of y alone, one of the weight
+ *   products are those of the operands as given: an fp32 x is taken as three bf16
+ *   terms, which hold it exactly, on the matrix cores.  An infinity or NaN of x reaches its row of y alone, one of the weight
  *   its column (an infinite weight there makes NaN of fp32 rows' finite values).
  * bias: device fp32 [n] or NULL.  residual: device [m][n] in y_dtype, row
  *   stride residual_stride >= n, or NULL; y: device [m][n], row stride y_stride

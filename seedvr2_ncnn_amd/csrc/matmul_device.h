@@ -289,30 +289,31 @@ struct TileEnd {
     }
 };
 
-// fp32 as a sum of PL bf16 values: all but the last take the top 8 bits of what the
-// ones before leave, by truncation, which cannot overflow and leaves an exact rest; the
-// last rounds (two terms: to 2^-15 of x) or, of three, holds the rest exactly.  An
-// infinity stays in the first term, a NaN reaches the later ones.  v: pairs of
-// values, h[q]: their terms q packed.
-template <int PL>
-__device__ __forceinline__ void split2(float v0, float v1, uint32_t (&h)[PL]) {
+// fp32 as a sum of three bf16 values, exactly, whatever y's type: with two (off by 2^-17)
+// a product whose leading bits cancel would be off by more than y's rounding.  The first
+// two take the top 8 bits of what the ones before leave, by truncation, which cannot
+// overflow and leaves an exact rest; the last holds the rest.  An infinity stays in the
+// first term, a NaN reaches the later ones.  v: pairs of values, h[q]: their terms q
+// packed.
+constexpr int kTerms = 3;
+
+__device__ __forceinline__ void split2(float v0, float v1, uint32_t (&h)[kTerms]) {
 #pragma unroll
-    for (int q = 0; q + 1 < PL; ++q) {
+    for (int q = 0; q + 1 < kTerms; ++q) {
         const uint32_t b0 = __float_as_uint(v0) & 0xffff0000u, b1 = __float_as_uint(v1) & 0xffff0000u;
         h[q] = (b0 >> 16) | b1;
         v0 = fabsf(v0) == __builtin_inff() ? 0.f : v0 - __uint_as_float(b0);
         v1 = fabsf(v1) == __builtin_inff() ? 0.f : v1 - __uint_as_float(b1);
     }
-    h[PL - 1] = pack2_bf16_rne(v0, v1);
+    h[kTerms - 1] = pack2_bf16_rne(v0, v1);
 }
 
-template <int PL>
-__device__ __forceinline__ void split8(const float (&v)[8], uint4 (&out)[PL]) {
-    uint32_t w[4][PL];
+__device__ __forceinline__ void split8(const float (&v)[8], uint4 (&out)[kTerms]) {
+    uint32_t w[4][kTerms];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) split2<PL>(v[2 * e], v[2 * e + 1], w[e]);
+    for (int e = 0; e < 4; ++e) split2(v[2 * e], v[2 * e + 1], w[e]);
 #pragma unroll
-    for (int q = 0; q < PL; ++q) out[q] = make_uint4(w[0][q], w[1][q], w[2][q], w[3][q]);
+    for (int q = 0; q < kTerms; ++q) out[q] = make_uint4(w[0][q], w[1][q], w[2][q], w[3][q]);
 }
 
 // Eight consecutive k of a row as an MFMA operand piece, zeros from `left` of them on.

@@ -4,6 +4,7 @@
 //   matmul_kernels.hip       which kernel takes a call; packing; any shape and alignment
 //   matmul_tile_kernels.hip  block tiles fed by DMA, and the sum of split k ranges
 //   matmul_rows_kernels.hip  few rows
+//   matmul_short_kernels.hip many fp32 rows of a short k
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -64,8 +65,7 @@ hipError_t launch_matmul(const MatmulArgs& a, void* workspace, size_t workspace_
 // The kernels' own launchers, for calls that plan_matmul gives them.
 hipError_t launch_matmul_tiles(const MatmulArgs& a, const MatmulPlan& plan, float* sums,
                                hipStream_t stream);
-// The most k steps of 32 of the kernel for short k, of rows of that many bf16 terms.
-int matmul_short_steps(int planes);
+constexpr int kShortMost = 160;   // k of the kernel for short k
 hipError_t launch_matmul_short(const MatmulArgs& a, const MatmulPlan& plan, hipStream_t stream);
 hipError_t launch_matmul_rows(const MatmulArgs& a, const MatmulPlan& plan, hipStream_t stream);
 

@@ -28,11 +28,11 @@ bool whole_pieces(const MatmulArgs& a) {
 
 // Any strides, alignment, n and k; fp32 activations.  Block tile 128x128,
 // k-step 32, four waves in a 2x2 grid of 64x64, both operands through registers
-// into double-buffered LDS.  XP: bf16 planes that stand for an fp32 x (0: x is of
-// the weight's type).
-template <int T, int XP, int YK>
+// into double-buffered LDS.  SPLIT: an fp32 x as bf16 terms (else x is of the weight's
+// type).
+template <int T, bool SPLIT, int YK>
 __global__ __launch_bounds__(256, 2) void matmul_any_kernel(MatmulArgs a, int ntiles, bool whole) {
-    constexpr int BM = 128, BN = 128, BK = 32, P = BK + 8, PL = XP ? XP : 1;
+    constexpr int BM = 128, BN = 128, BK = 32, P = BK + 8, PL = SPLIT ? kTerms : 1;
     __shared__ __attribute__((aligned(16))) uint16_t x_lds[2][PL][BM * P];
     __shared__ __attribute__((aligned(16))) uint16_t w_lds[2][BN * P];
     RowTiles rts(a, BM, gridDim.x / ntiles);
@@ -52,7 +52,7 @@ __global__ __launch_bounds__(256, 2) void matmul_any_kernel(MatmulArgs a, int nt
     const uint16_t* w = (const uint16_t*)a.w + (long)rt.group * a.n * a.k;
 
     // thread -> (LDS row, quarter of 8 k) twice per operand
-    float xf[XP ? 2 : 1][8];
+    float xf[SPLIT ? 2 : 1][8];
     uint4 xr[2], wr[2];
     auto load = [&](int k0) {
 #pragma unroll
@@ -63,7 +63,7 @@ __global__ __launch_bounds__(256, 2) void matmul_any_kernel(MatmulArgs a, int nt
             const long xo = (long)(rt.row0 + r) * a.x_stride + kc;
             wr[c] = piece16<false>(w + (long)col * a.k + kc, col < a.n ? a.k - kc : 0);
             const int left = r < rows ? a.k - kc : 0;
-            if constexpr (XP)
+            if constexpr (SPLIT)
                 piece32<false>((const float*)a.x + xo, left, xf[c]);
             else
                 xr[c] = piece16<false>((const uint16_t*)a.x + xo, left);
@@ -75,9 +75,9 @@ __global__ __launch_bounds__(256, 2) void matmul_any_kernel(MatmulArgs a, int nt
             const int r = (tid >> 2) + 64 * c;
             const int at = r * P + (tid & 3) * 8;
             *reinterpret_cast<uint4*>(&w_lds[buf][at]) = wr[c];
-            if constexpr (XP) {
+            if constexpr (SPLIT) {
                 uint4 h[PL];
-                split8<PL>(xf[c], h);
+                split8(xf[c], h);
 #pragma unroll
                 for (int i = 0; i < PL; ++i) *reinterpret_cast<uint4*>(&x_lds[buf][i][at]) = h[i];
             } else {
@@ -119,12 +119,12 @@ __global__ __launch_bounds__(256, 2) void matmul_any_kernel(MatmulArgs a, int nt
     end.finish(a, acc);
 }
 
-template <int T, int XP, int YK>
+template <int T, bool SPLIT, int YK>
 hipError_t launch_any(const MatmulArgs& a, hipStream_t stream) {
     const int ntiles = (a.n + 127) / 128;
     const long blocks = row_tiles(a, 128) * ntiles;
     if (blocks > 0x7fffffffL) return hipErrorInvalidValue;
-    matmul_any_kernel<T, XP, YK><<<(unsigned)blocks, 256, 0, stream>>>(a, ntiles, whole_pieces(a));
+    matmul_any_kernel<T, SPLIT, YK><<<(unsigned)blocks, 256, 0, stream>>>(a, ntiles, whole_pieces(a));
     return hipGetLastError();
 }
 
@@ -139,7 +139,6 @@ struct PackJob {
     uint16_t* dst;
 };
 
-template <int PL>
 __device__ __forceinline__ void pack_piece(const PackJob& job, int k, long i) {
     const int pieces = job.width / 8;
     const long row = i / pieces;
@@ -147,11 +146,11 @@ __device__ __forceinline__ void pack_piece(const PackJob& job, int k, long i) {
     uint16_t* out = job.dst + row * job.planes * job.width + kc;
     if (job.kind == 0) {
         float v[8];
-        uint4 h[PL];
+        uint4 h[kTerms];
         piece32<false>((const float*)job.src + row * job.stride + kc, k - kc, v);
-        split8<PL>(v, h);
+        split8(v, h);
 #pragma unroll
-        for (int q = 0; q < PL; ++q) *reinterpret_cast<uint4*>(out + (long)q * job.width) = h[q];
+        for (int q = 0; q < kTerms; ++q) *reinterpret_cast<uint4*>(out + (long)q * job.width) = h[q];
     } else {
         const uint4 h = piece16<false>((const uint16_t*)job.src + row * job.stride + kc, k - kc);
         for (int q = 0; q < job.planes; ++q) *reinterpret_cast<uint4*>(out + (long)q * job.width) = h;
@@ -159,32 +158,28 @@ __device__ __forceinline__ void pack_piece(const PackJob& job, int k, long i) {
 }
 
 // x, then the weight, either of which may have no rows.
-template <int PL>
 __global__ __launch_bounds__(256) void matmul_pack_kernel(PackJob x, PackJob w, int k) {
     const long nx = x.rows * (x.width / 8), all = nx + w.rows * (w.width / 8);
     for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < all; i += (long)gridDim.x * 256) {
         if (i < nx)
-            pack_piece<PL>(x, k, i);
+            pack_piece(x, k, i);
         else
-            pack_piece<PL>(w, k, i - nx);
+            pack_piece(w, k, i - nx);
     }
 }
 
 hipError_t launch_pack(const PackJob& x, const PackJob& w, int k, hipStream_t stream) {
     const long all = x.rows * (x.width / 8) + w.rows * (w.width / 8);
     const unsigned nb = (unsigned)std::min<long>((all + 255) / 256, 65536);
-    if (x.planes == 3)
-        matmul_pack_kernel<3><<<nb, 256, 0, stream>>>(x, w, k);
-    else
-        matmul_pack_kernel<2><<<nb, 256, 0, stream>>>(x, w, k);
+    matmul_pack_kernel<<<nb, 256, 0, stream>>>(x, w, k);
     return hipGetLastError();
 }
 
 template <int YK>
 hipError_t launch_any_y(const MatmulArgs& a, hipStream_t stream) {
-    if (a.w_kind == 2) return launch_any<2, 0, YK>(a, stream);
-    if (a.x_kind == 0) return launch_any<1, YK == 0 ? 3 : 2, YK>(a, stream);
-    return launch_any<1, 0, YK>(a, stream);
+    if (a.w_kind == 2) return launch_any<2, false, YK>(a, stream);
+    if (a.x_kind == 0) return launch_any<1, true, YK>(a, stream);
+    return launch_any<1, false, YK>(a, stream);
 }
 
 constexpr int kUnits = 256;   // compute units of an MI355X
@@ -231,8 +226,8 @@ double rows_us(const MatmulArgs& a, const MatmulPlan& r, long rows) {
 
 long round_up(long v, long to) { return (v + to - 1) / to * to; }
 
-// bf16 terms of an fp32 x
-int packed_planes(const MatmulArgs& a) { return a.x_kind ? 1 : a.y_kind ? 2 : 3; }
+// bf16 terms of a value of x
+int packed_planes(const MatmulArgs& a) { return a.x_kind ? 1 : kTerms; }
 
 // Elements of a packed plane.  Where the weight is packed too it is repeated for each
 // plane of x, so that the planes are one longer row; else its rows are read once for
@@ -263,12 +258,12 @@ MatmulPlan plan_matmul(const MatmulArgs& a, size_t workspace_bytes) {
     const bool tiles = near && room && 256 * pitch * 2 < 0x7fffffffL &&
                        256 * std::max<long>(a.k, p.pack_w ? row : 0) * 2 < 0x7fffffffL;
 
-    // many fp32 rows of a short k, packed and on tiles -> here: by 2560 x 132 2700 rows 17
-    // -> 13 us, 21600 66 -> 43; by 2560 x 160 17 -> 17 and 65 -> 52; by 1024 x 64 5000 rows
-    // 10.6 -> 11.1, 21600 26 -> 18.  Fewer outputs gain only where the weight would be
-    // packed too.
+    // many fp32 rows of a short k, packed and on tiles -> here: by 2560 x 132 2700 rows 20
+    // -> 15 us, 21600 80 -> 60; by 2560 x 160 19 -> 17 and 83 -> 60; with fp32 results 91 ->
+    // 56 and 95 -> 62; by 1024 x 64 5000 rows 14.4 -> 13.7, 7000 14.1 -> 12.3, 21600 29 ->
+    // 21.  Fewer outputs gain only where the weight would be packed too.
     if (a.x_kind == 0 && !a.offsets && rows > 32 && (long)a.m * a.n >= 6L << 20 && near &&
-        (a.k + 31) / 32 <= matmul_short_steps(packed_planes(a)) &&
+        a.k <= kShortMost &&
         a.x_stride < 1L << 24) {
         MatmulPlan s{};
         s.kernel = MatmulPlan::kShort;

@@ -11,11 +11,10 @@ namespace {
 // x comes from the caches.  The waves' sums meet in LDS.  Rows and columns past the end
 // repeat the last one, and are dropped.
 //
-// PL bf16 terms stand for a value of an fp32 x, split here by every workgroup; 1: x is of
-// the weight's type.
-template <int T, int PL, int MT, int NT, bool ODD>
+// SPLIT: an fp32 x as bf16 terms, by every workgroup; else x is of the weight's type.
+template <int T, bool SPLIT, int MT, int NT, bool ODD>
 __global__ __launch_bounds__(512) void matmul_rows_kernel(MatmulArgs a, int ntiles) {
-    constexpr bool SPLIT = PL > 1;
+    constexpr int PL = SPLIT ? kTerms : 1;
     constexpr int REGS = 2 * 4 * (NT + MT * (SPLIT ? 2 : 1));   // of a 64-k chunk
     constexpr int U = REGS >= 40 ? 1 : REGS >= 24 ? 2 : 4;  // chunks of a batch
     constexpr bool TWO = U * REGS <= 80;                    // the next batch in flight
@@ -74,7 +73,7 @@ __global__ __launch_bounds__(512) void matmul_rows_kernel(MatmulArgs a, int ntil
             for (int i = 0; i < MT; ++i) {
                 uint4 t[PL];
                 if constexpr (SPLIT)
-                    split8<PL>(b.f[c][i], t);
+                    split8(b.f[c][i], t);
                 else
                     t[0] = b.x[c][i];
 #pragma unroll
@@ -139,38 +138,37 @@ __global__ __launch_bounds__(512) void matmul_rows_kernel(MatmulArgs a, int ntil
     }
 }
 
-template <int T, int PL, int MT, int NT, bool ODD>
+template <int T, bool SPLIT, int MT, int NT, bool ODD>
 hipError_t run(const MatmulArgs& a, hipStream_t stream) {
     const int ntiles = (a.n + 16 * NT - 1) / (16 * NT);
     const long blocks = row_tiles(a, 16 * MT) * ntiles;
     if (blocks > 0x7fffffffL) return hipErrorInvalidValue;
     const int waves = std::min(8, (a.k + 63) / 64);
-    matmul_rows_kernel<T, PL, MT, NT, ODD><<<(unsigned)blocks, 64 * waves, 0, stream>>>(a, ntiles);
+    matmul_rows_kernel<T, SPLIT, MT, NT, ODD><<<(unsigned)blocks, 64 * waves, 0, stream>>>(a, ntiles);
     return hipGetLastError();
 }
 
-template <int T, int PL, int MT>
+template <int T, bool SPLIT, int MT>
 hipError_t pick(const MatmulArgs& a, int cols, hipStream_t stream) {
-    constexpr int MOST = MT * PL <= 4 ? 4 : 2;   // by registers
+    constexpr int MOST = MT * (SPLIT ? kTerms : 1) <= 4 ? 4 : 2;   // by registers
     const bool odd = (a.k & 1) || (uintptr_t)a.w % 4 || (a.x_kind && ((a.x_stride & 1) || (uintptr_t)a.x % 4));
-    if (odd) return run<T, PL, MT, 1, true>(a, stream);
-    if (cols == 64) return run<T, PL, MT, MOST, false>(a, stream);
-    return cols == 32 ? run<T, PL, MT, 2, false>(a, stream) : run<T, PL, MT, 1, false>(a, stream);
+    if (odd) return run<T, SPLIT, MT, 1, true>(a, stream);
+    if (cols == 64) return run<T, SPLIT, MT, MOST, false>(a, stream);
+    return cols == 32 ? run<T, SPLIT, MT, 2, false>(a, stream) : run<T, SPLIT, MT, 1, false>(a, stream);
 }
 
-template <int T, int PL>
+template <int T, bool SPLIT>
 hipError_t pick_rows(const MatmulArgs& a, const MatmulPlan& plan, hipStream_t stream) {
-    return plan.rows == 16   ? pick<T, PL, 1>(a, plan.cols, stream)
-           : plan.rows == 32 ? pick<T, PL, 2>(a, plan.cols, stream)
-                             : pick<T, PL, 4>(a, plan.cols, stream);
+    return plan.rows == 16   ? pick<T, SPLIT, 1>(a, plan.cols, stream)
+           : plan.rows == 32 ? pick<T, SPLIT, 2>(a, plan.cols, stream)
+                             : pick<T, SPLIT, 4>(a, plan.cols, stream);
 }
 
 }  // namespace
 
 hipError_t launch_matmul_rows(const MatmulArgs& a, const MatmulPlan& plan, hipStream_t stream) {
-    if (a.w_kind == 2) return pick_rows<2, 1>(a, plan, stream);
-    if (a.x_kind) return pick_rows<1, 1>(a, plan, stream);
-    return a.y_kind == 0 ? pick_rows<1, 3>(a, plan, stream) : pick_rows<1, 2>(a, plan, stream);
+    if (a.w_kind == 2) return pick_rows<2, false>(a, plan, stream);
+    return a.x_kind ? pick_rows<1, false>(a, plan, stream) : pick_rows<1, true>(a, plan, stream);
 }
 
 }  // namespace s2

@@ -7,11 +7,11 @@
 // once for the 256 columns, then 64 columns after 64.  No wave waits for another once
 // the weight is there, so that one stores or loads while another multiplies.
 //
-// 21600 x 132 by 2560 x 132, bf16 results: 43 us.  The 110 MB of y take 21, and each of
-// a compute unit's matrix, vector (the terms and the epilogue) and LDS pipes is busy for
-// 15 to 18; without its stores the kernel took two thirds of the time, without its
-// matrix instructions half.  32 rows a wave halve the LDS reads, but leave registers for
-// eight waves only, and took 9% longer.
+// 21600 x 132 by 2560 x 132, bf16 results: 58 us.  The 110 MB of y take 21, the matrix
+// instructions (three terms, k as 160) 23 at their peak rate; the vector (terms, epilogue)
+// and LDS pipes are busy for 15 to 20 each.  With two terms, which hold 16 bits of x, the
+// kernel took 47; then 32 rows a wave, which halve the LDS reads but leave registers for
+// eight waves only, took 9% longer.
 #include "matmul_device.h"
 
 namespace s2 {
@@ -21,7 +21,7 @@ namespace {
 constexpr int kCols = 256, kRows = 16;
 
 // Waves of a workgroup, by registers.
-constexpr int waves_of(int pl) { return pl == 2 ? 16 : 12; }
+constexpr int waves_of(int steps) { return steps == 3 ? 16 : 12; }
 
 // Four of a row's k, zeros from `left` of them on.
 __device__ __forceinline__ u32x2 four16(const uint16_t* p, int left) {
@@ -32,13 +32,13 @@ __device__ __forceinline__ u32x2 four16(const uint16_t* p, int left) {
     return u32x2{h[0] | h[1] << 16, h[2]};
 }
 
-// PL: bf16 terms of a value; STEPS: k steps of 32, zeros past k.
-template <int PL, int YK, int STEPS>
-__global__ __launch_bounds__(64 * waves_of(PL)) void matmul_short_kernel(MatmulArgs a, int blocks_n, int splits,
-                                                           bool whole) {
+// STEPS: k steps of 32, zeros past k.
+template <int YK, int STEPS>
+__global__ __launch_bounds__(64 * waves_of(STEPS)) void matmul_short_kernel(MatmulArgs a, int blocks_n,
+                                                                            int splits, bool whole) {
     // an odd number of 16-byte pieces a row: 16 rows' reads spread over all banks
     constexpr int P = STEPS * 32 + 8, PIECES = STEPS * 4;
-    constexpr int kWaves = waves_of(PL), kThreads = 64 * kWaves;
+    constexpr int kWaves = waves_of(STEPS), kThreads = 64 * kWaves;
     __shared__ __attribute__((aligned(16))) uint16_t w_lds[kCols * P];
     __shared__ __attribute__((aligned(16))) float bias[kCols];
     const int tid = threadIdx.x;
@@ -111,9 +111,9 @@ __global__ __launch_bounds__(64 * waves_of(PL)) void matmul_short_kernel(MatmulA
 #pragma unroll
                     for (int v = 1; v < 4; ++v)
                         if (32 * s + 4 * g + 4 * e + v >= a.k) f[s][e + v] = 0.f;
-        uint4 fx[STEPS][PL];
+        uint4 fx[STEPS][kTerms];
 #pragma unroll
-        for (int s = 0; s < STEPS; ++s) split8<PL>(f[s], fx[s]);
+        for (int s = 0; s < STEPS; ++s) split8(f[s], fx[s]);
         f32x4 acc[1][4];
         auto multiply = [&](int c) {
 #pragma unroll
@@ -131,7 +131,7 @@ __global__ __launch_bounds__(64 * waves_of(PL)) void matmul_short_kernel(MatmulA
                 if (u + 1 < 2 * STEPS) read(u + 1);
                 __builtin_amdgcn_sched_barrier(0);   // else all reads come first, and spill
 #pragma unroll
-                for (int q = 0; q < PL; ++q)
+                for (int q = 0; q < kTerms; ++q)
 #pragma unroll
                     for (int j = 0; j < 2; ++j)
                         acc[0][2 * (u & 1) + j] =
@@ -160,22 +160,25 @@ __global__ __launch_bounds__(64 * waves_of(PL)) void matmul_short_kernel(MatmulA
     }
 }
 
-template <int PL, int YK, int STEPS>
+template <int YK, int STEPS>
 hipError_t run(const MatmulArgs& a, const MatmulPlan& p, hipStream_t stream) {
     const int blocks_n = (a.n + kCols - 1) / kCols;
-    matmul_short_kernel<PL, YK, STEPS><<<(unsigned)(blocks_n * p.parts), 64 * waves_of(PL), 0, stream>>>(
-        a, blocks_n, p.parts, p.whole);
+    matmul_short_kernel<YK, STEPS>
+        <<<(unsigned)(blocks_n * p.parts), 64 * waves_of(STEPS), 0, stream>>>(a, blocks_n, p.parts,
+                                                                              p.whole);
     return hipGetLastError();
 }
 
 }  // namespace
 
-int matmul_short_steps(int planes) { return planes == 2 ? 5 : 3; }
-
 hipError_t launch_matmul_short(const MatmulArgs& a, const MatmulPlan& plan, hipStream_t stream) {
-    if (a.y_kind == 0) return run<3, 0, 3>(a, plan, stream);
-    if (a.k <= 96) return a.y_kind == 1 ? run<2, 1, 3>(a, plan, stream) : run<2, 2, 3>(a, plan, stream);
-    return a.y_kind == 1 ? run<2, 1, 5>(a, plan, stream) : run<2, 2, 5>(a, plan, stream);
+    if (a.k <= 96)
+        return a.y_kind == 0   ? run<0, 3>(a, plan, stream)
+               : a.y_kind == 1 ? run<1, 3>(a, plan, stream)
+                               : run<2, 3>(a, plan, stream);
+    return a.y_kind == 0   ? run<0, 5>(a, plan, stream)
+           : a.y_kind == 1 ? run<1, 5>(a, plan, stream)
+                           : run<2, 5>(a, plan, stream);
 }
 
 }  // namespace s2

@@ -512,3 +512,33 @@ def test_two_streams_at_once():
             got[i].append(capi.linear(x, w, b, residual=r, stream=streams[i]))
     torch.cuda.synchronize()
     assert all(torch.equal(y, want[i]) for i in range(2) for y in got[i])
+
+
+# few rows, tiles, the short k's kernel, no workspace
+@pytest.mark.parametrize("m,k,n,workspace", [(1, 640, 96, True), (20, 133, 200, True), (300, 512, 264, True),
+                                             (2500, 132, 2564, True), (2500, 64, 2564, True),
+                                             (300, 512, 264, False)])
+@pytest.mark.parametrize("y_type", Y_TYPES)
+def test_fp32_rows_keep_their_bits(m, k, n, workspace, y_type):
+    """Differences of two of a row's values, both near a thousand: exact products whose
+    leading bits cancel.  A value is a sum of three bf16 terms at most, so a result is one
+    of six products, added in five steps that are off by a step of fp32 (2 U) of the
+    largest partial sum each, |a| + |b|; then it is rounded to y."""
+    import torch
+    import row_operators as ro
+    draw = _gen(m + k + n)
+    x = 1000.0 + draw(m, k)
+    w = torch.zeros(n, k, dtype=torch.bfloat16, device="cuda")
+    a = torch.arange(n, device="cuda") % k
+    b = (a + 1 + torch.arange(n, device="cuda") // k) % k
+    rows = torch.arange(n, device="cuda")
+    w[rows, a], w[rows, b] = 1.0, -1.0
+    room = None if workspace else torch.empty(0, dtype=torch.uint8, device="cuda")
+    got = capi.linear(x, w, out_dtype=getattr(torch, y_type), workspace=room)
+    offs = torch.tensor([0, m // 2, m], dtype=torch.int32, device="cuda")
+    parts = capi.grouped_linear(x, offs, torch.stack([w, w]), out_dtype=got.dtype, workspace=room)
+    xd = x.double()
+    want = xd[:, a] - xd[:, b]
+    err = 5 * 2 * ro.U * (xd[:, a].abs() + xd[:, b].abs())
+    for y in (got, parts):
+        ro.check(y, want, err + ro.rounding(want.abs() + err, y.dtype))
