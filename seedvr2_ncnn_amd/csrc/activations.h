@@ -41,7 +41,9 @@ __device__ __forceinline__ float gelu(float x) {
              t * (0.5f * -0.284496736f +
                   t * (0.5f * 1.421413741f + t * (0.5f * -1.453152027f + t * (0.5f * 1.061405429f)))));
     const float q = poly * __builtin_amdgcn_exp2f(-w * w);   // Q(|x|)
-    return fmaf(-ax, q, fmaxf(x, 0.f));
+    // +inf meets q = 0 as the largest finite value, and stays; -inf gives -inf * 0, NaN,
+    // as the product 0.5 x (1 + erf) does
+    return fmaf(-fabsf(fminf(x, __FLT_MAX__)), q, fmaxf(x, 0.f));
 }
 
 __device__ __forceinline__ float activate(float x, int act) {

@@ -58,3 +58,15 @@ def test_gelu_limits():
     assert torch.equal(y[:4], x[:4])
     assert torch.equal(y[4:7], torch.zeros(3, device="cuda"))
     assert torch.isnan(y[7])
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
+def test_gelu_of_infinities(dtype):
+    """+inf stays; -inf is -inf times 0, NaN as the formula has it; the largest finite
+    values are themselves and -0."""
+    import torch
+    big = torch.finfo(getattr(torch, dtype)).max
+    x = torch.tensor([math.inf, -math.inf, math.nan, big, -big], dtype=getattr(torch, dtype), device="cuda")
+    y = capi.gelu(x).tolist()
+    assert y[0] == math.inf and math.isnan(y[1]) and math.isnan(y[2])
+    assert y[3] == big and y[4] == 0.0

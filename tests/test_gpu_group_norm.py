@@ -211,3 +211,19 @@ def test_more_pixels_than_24_bits():
     x, gamma, beta = _draw((1, 17_000_003, 4), "float16", 12)
     got = capi.group_norm(x, 2, gamma, beta)
     _check(x, 2, gamma, beta, 1e-6, "none", got)
+
+
+@pytest.mark.parametrize("act", ["gelu", "silu", "gelu_tanh"])
+@pytest.mark.parametrize("y_type", TYPES)
+@pytest.mark.parametrize("pixels", [40, 30000])
+def test_activations_of_infinities(act, y_type, pixels):
+    """By a beta: +inf stays, a NaN too, -inf is -inf times 0, NaN."""
+    import torch
+    import row_operators as ro
+    x, gamma, beta = _draw((2, pixels, 24), "float32", 8)
+    beta[:8] = float("inf")
+    beta[8:12] = float("-inf")
+    beta[12:16] = float("nan")
+    y = capi.group_norm(x, 3, gamma, beta, 1e-6, ro.ACTS[act], out_dtype=getattr(torch, y_type))
+    assert (y[:, :, :8] == float("inf")).all()
+    assert y[:, :, 8:16].isnan().all() and y[:, :, 16:].isfinite().all()

@@ -542,3 +542,27 @@ def test_fp32_rows_keep_their_bits(m, k, n, workspace, y_type):
     err = 5 * 2 * ro.U * (xd[:, a].abs() + xd[:, b].abs())
     for y in (got, parts):
         ro.check(y, want, err + ro.rounding(want.abs() + err, y.dtype))
+
+
+@pytest.mark.parametrize("act", ["gelu", "silu", "gelu_tanh"])
+@pytest.mark.parametrize("y_type", Y_TYPES)
+@pytest.mark.parametrize("m,k,n", [(1, 64, 96), (300, 64, 96), (77, 5120, 96), (2500, 32, 2564)], ids=str)
+@pytest.mark.parametrize("pair", PAIRS, ids="-".join)
+def test_activations_of_infinities(act, y_type, m, k, n, pair):
+    """By a bias: +inf stays, a NaN too, -inf is -inf times 0, NaN as the formulas have
+    it; on few rows, tiles, ranges of k and the short k's kernel, ragged rows among them."""
+    import torch
+    import row_operators as ro
+    x, w, _, _ = _operands(m, k, n, pair, y_type)
+    bias = torch.zeros(n, device="cuda")
+    bias[::3] = float("inf")
+    bias[1::6] = float("-inf")
+    bias[4::6] = float("nan")
+    for width in (n, n - 3):
+        for y in (capi.linear(x, w[:width], bias[:width], ro.ACTS[act], out_dtype=getattr(torch, y_type)),
+                  capi.grouped_linear(x, torch.tensor([0, m], dtype=torch.int32, device="cuda"),
+                                      w[None, :width], bias[None, :width], ro.ACTS[act],
+                                      out_dtype=getattr(torch, y_type))):
+            assert (y[:, ::3] == float("inf")).all()
+            assert y[:, 1::3].isnan().all()
+            assert y[:, 2::3].isfinite().all()
