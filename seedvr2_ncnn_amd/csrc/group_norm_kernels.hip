@@ -7,11 +7,13 @@
 // only caches can make cheaper than two passes; groups of few values are held in
 // registers between the two.
 //
-// Statistics.  A thread sums x - K and (x - K)^2 of its channels over its pixels,
-// K being its own first value of each channel: no cancellation where a mean is
-// many deviations large, and one outlying K spoils a single thread's part at
-// most.  Parts meet as (mean, sum of squared deviations) by the parallel variance
-// formula (Chan, Golub, LeVeque).  Every order of summation is fixed.
+// Statistics.  A thread sums x - K and (x - K)^2 of its channels over eight of its
+// pixels, K being the first of them: no cancellation where a mean is many deviations
+// large, and a K far from all others, whose square the difference of the two sums would
+// lose digits of, stands against seven values only (against all of a thread's 450 it
+// left a frame's variance off by 3e-3, now 2e-6).  Those sums and all parts after them
+// meet as (mean, sum of squared deviations) by the parallel variance formula (Chan,
+// Golub, LeVeque).  Every order of summation is fixed.
 #include "group_norm_kernels.h"
 
 #include <algorithm>
@@ -142,6 +144,54 @@ struct Split {
     }
 };
 
+// A thread's (mean, sum of squared deviations) of V channels, in two floats each: as
+// many joinings as a thread has pixels would round them otherwise.
+template <int V>
+struct Part {
+    float mean[V], mean_rest[V], m2[V], m2_rest[V];
+
+    // `count` pixels of raw, at most U, to the `before` that are in
+    template <int U, typename T>
+    __device__ __forceinline__ void add(const Raw<T, V> (&raw)[U], int count, int before) {
+        float first[V], s1[V], s2[V];
+        raw[0].get(first);
+        if (before == 0)
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                mean[i] = first[i];
+                mean_rest[i] = m2[i] = m2_rest[i] = 0.f;
+            }
+#pragma unroll
+        for (int i = 0; i < V; ++i) s1[i] = s2[i] = 0.f;
+#pragma unroll
+        for (int u = 1; u < U; ++u)
+            if (u < count) {
+                float v[V];
+                raw[u].get(v);
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    const float d = v[i] - first[i];
+                    s1[i] += d;
+                    s2[i] = fmaf(d, d, s2[i]);
+                }
+            }
+        const float share = (float)count / (float)(before + count), each = 1.f / (float)count;
+        const float weight = share * (float)before;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const float off = s1[i] * each;   // of these pixels' mean from the first
+            const float own = fmaxf(fmaf(-off, s1[i], s2[i]), 0.f);
+            const float d = (first[i] - mean[i]) + (off - mean_rest[i]);
+            const float step = d * share, sum = mean[i] + step;
+            mean_rest[i] += (mean[i] - sum) + step;
+            mean[i] = sum;
+            const float more = fmaf(d * weight, d, own), total = m2[i] + more;
+            m2_rest[i] += (m2[i] - total) + more;
+            m2[i] = total;
+        }
+    }
+};
+
 // A chunk's (mean, sum of squared deviations) of every group: parts[frame][group][chunk].
 // A thread joins runs of SUB of its channels, which divides a group's.
 template <int XK, int V, int SUB>
@@ -164,47 +214,27 @@ __global__ __launch_bounds__(kThreads) void group_norm_stats_kernel(GroupNormArg
     const long step = (long)sp.rows * p.x_pixel;
     for (int c = col; c < sp.cv && count > 0; c += sp.seg) {
         const T* q = x + (long)c * V;
-        float first[V], s1[V], s2[V];
-        load_v<V>(q, first);
-#pragma unroll
-        for (int i = 0; i < V; ++i) s1[i] = s2[i] = 0.f;
-        auto add = [&](const float (&v)[V]) {
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const float d = v[i] - first[i];
-                s1[i] += d;
-                s2[i] = fmaf(d, d, s2[i]);
-            }
-        };
+        Part<V> part;
         constexpr int U = 8;   // pixels in flight
-        int j = 1;
+        Raw<T, V> raw[U];
+        int j = 0;
         for (; j + U <= count; j += U) {
-            Raw<T, V> raw[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) raw[u].load(q + (j + u) * step);
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                float v[V];
-                raw[u].get(v);
-                add(v);
-            }
+            part.template add<U>(raw, U, j);
         }
-        Raw<T, V> raw[U];
+        if (j < count) {
 #pragma unroll
-        for (int u = 0; u < U - 1; ++u)
-            if (j + u < count) raw[u].load(q + (j + u) * step);
+            for (int u = 0; u < U - 1; ++u)
+                if (j + u < count) raw[u].load(q + (j + u) * step);
+            part.template add<U>(raw, count - j, j);
+        }
+        const float n = (float)count;
+        float first[V], s2[V];   // mean and sum of squared deviations
 #pragma unroll
-        for (int u = 0; u < U - 1; ++u)
-            if (j + u < count) {
-                float v[V];
-                raw[u].get(v);
-                add(v);
-            }
-        const float n = (float)count, inv = 1.f / n;
-#pragma unroll
-        for (int i = 0; i < V; ++i) {   // to mean and sum of squared deviations
-            first[i] = fmaf(s1[i], inv, first[i]);
-            s2[i] = fmaxf(fmaf(-s1[i] * inv, s1[i], s2[i]), 0.f);
+        for (int i = 0; i < V; ++i) {
+            first[i] = part.mean[i] + part.mean_rest[i];
+            s2[i] = part.m2[i] + part.m2_rest[i];
         }
 #pragma unroll
         for (int i = 0; i < V; i += SUB) {
@@ -241,16 +271,20 @@ __global__ __launch_bounds__(kThreads) void group_norm_stats_kernel(GroupNormArg
                 sum = fmaf((float)(base + (r < extra)), e[r * runs + c].x - ref, sum);
         const float mean = fmaf(lanes_sum(sum, sp.lane_bits), per_run, ref);
         float m2 = 0.f;
+        sum = 0.f;   // what the mean is off by, where ref is far from it
         for (int c = c0; c < each; c += across)
 #pragma unroll 4
             for (int r = r0; r < used; r += dr) {
                 const float2 v = e[r * runs + c];
-                const float d = v.x - mean;
-                m2 += fmaf((float)((base + (r < extra)) * SUB) * d, d, v.y);
+                const float n = (float)(base + (r < extra)), d = v.x - mean;
+                sum = fmaf(n, d, sum);
+                m2 += fmaf(n * (float)SUB * d, d, v.y);
             }
         m2 = lanes_sum(m2, sp.lane_bits);
+        sum = lanes_sum(sum, sp.lane_bits);
         if (g < p.groups && lane == 0)
-            parts[((long)f * p.groups + g) * gridDim.x + blockIdx.x] = make_float2(mean, m2);
+            parts[((long)f * p.groups + g) * gridDim.x + blockIdx.x] =
+                make_float2(fmaf(sum, per_run, mean), m2);
     }
 }
 
@@ -387,29 +421,35 @@ __global__ __launch_bounds__(kThreads) void group_norm_apply_kernel(GroupNormArg
 }
 
 // Few values: a workgroup holds a frame's group in registers, one launch in all.  The
-// mean first, then the deviations from it.
+// mean first, from deviations from the first value; then the deviations from it, whose
+// own mean corrects it where the first value is far from it.
 // A thread holds up to 4 vectors of 8, or 8 of 4, 2 or 1; 256 threads, or 1024 (2000 x 512
 // in bf16 in 32 groups 7.3 us, 12 by two launches; 4000 x 512 with 8 vectors of 8 a
 // thread 16.6 and 13: the group's pieces of 32 bytes come to one compute unit).
 constexpr int kSmallMost = 1024;   // threads
 constexpr int small_vectors(int v) { return v == 8 ? 4 : 8; }
 
-template <int THREADS>
-__device__ __forceinline__ float block_sum(float v, float* lds) {
-    v = lanes_sum(v, 6);
-    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = 0.f;
+template <int THREADS, int N>
+__device__ __forceinline__ void block_sum(float (&v)[N], float (*lds)[THREADS / 64]) {
 #pragma unroll
-    for (int i = 0; i < THREADS / 64; ++i) v += lds[i];
-    return v;
+    for (int j = 0; j < N; ++j) {
+        v[j] = lanes_sum(v[j], 6);
+        if ((threadIdx.x & 63) == 0) lds[j][threadIdx.x >> 6] = v[j];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        v[j] = 0.f;
+#pragma unroll
+        for (int i = 0; i < THREADS / 64; ++i) v[j] += lds[j][i];
+    }
 }
 
 template <int XK, int YK, int V, int THREADS>
 __global__ __launch_bounds__(THREADS) void group_norm_small_kernel(GroupNormArgs p) {
     typedef typename Elem<XK>::T T;
     constexpr int VECS = small_vectors(V);
-    __shared__ float lds[2][THREADS / 64];
+    __shared__ float lds[3][THREADS / 64];
     const int f = blockIdx.y, g = blockIdx.x;
     const int each = p.channels / p.groups;
     const int ev = each / V;   // vectors of a pixel, at most the threads
@@ -430,26 +470,30 @@ __global__ __launch_bounds__(THREADS) void group_norm_small_kernel(GroupNormArgs
     // deviations from the first value: no digits are lost to a large mean
     const float ref = to_f32(x[g * each]);
     float v[VECS][V];
-    float sum = 0.f;
+    float sum[1] = {0.f};
 #pragma unroll
     for (int u = 0; u < VECS; ++u)
         if (u < count) {
             raw[u].get(v[u]);
 #pragma unroll
-            for (int i = 0; i < V; ++i) sum += v[u][i] - ref;
+            for (int i = 0; i < V; ++i) sum[0] += v[u][i] - ref;
         }
     const float per_value = 1.f / ((float)p.pixels * (float)each);
-    const float mean = fmaf(block_sum<THREADS>(sum, lds[0]), per_value, ref);
-    float m2 = 0.f;
+    block_sum<THREADS>(sum, lds);
+    const float near = fmaf(sum[0], per_value, ref);
+    float dev[2] = {0.f, 0.f};   // deviations' squares, deviations
 #pragma unroll
     for (int u = 0; u < VECS; ++u)
         if (u < count)
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                const float d = v[u][i] - mean;
-                m2 = fmaf(d, d, m2);
+                const float d = v[u][i] - near;
+                dev[0] = fmaf(d, d, dev[0]);
+                dev[1] += d;
             }
-    const float rstd = 1.f / sqrtf(fmaf(block_sum<THREADS>(m2, lds[1]), per_value, p.eps));
+    block_sum<THREADS>(dev, lds + 1);
+    const float off = dev[1] * per_value, mean = near + off;
+    const float rstd = 1.f / sqrtf(fmaf(-off, off, dev[0] * per_value) + p.eps);
     if (count == 0) return;
 #pragma unroll
     for (int i = 0; i < V; ++i) scale[i] *= rstd;

@@ -94,6 +94,36 @@ def group_norm(x, groups, gamma, beta, eps, act, dtype):
     return finish(v, v_err, act, None, dtype)
 
 
+def group_norm_by_variance(x, groups, gamma, beta, eps, act, dtype):
+    """As group_norm, for any distribution: what the statistics may be off by goes by a
+    group's deviation alone, however far single values lie.
+
+    A thread sums eight pixels about the first of them, K, then joins their mean b and
+    sum of squared deviations M to those of the pixels before.  About K the squares sum
+    to at most 9 M, (K - b)^2 being at most M: with eleven roundings of each and eight of
+    their sum's, b's part off by 16 and 2, M is off by at most 29 * 9 U M = 261 U M.  The
+    joining's difference of means is off by U times itself and 10.5 U sqrt(M), which moves
+    its square, weighed by at most 8, by 14 U of itself and 84 U M.  Those sums are kept in
+    two floats.  After that every sum is of squares or of deviations from a mean that
+    is already near: 64 + 8 + 32 additions in a row at most, 54 where a thread holds its
+    values, and 16 among channels; of means stored in fp32, 4 U of themselves.  So the
+    variance is off by less than 600 U of itself, the mean by 200 U deviations."""
+    f, p, c = x.shape
+    xd = x.double().reshape(f, p, groups, c // groups)
+    mean = xd.mean(dim=(1, 3), keepdim=True)
+    d = xd - mean
+    var = (d * d).mean(dim=(1, 3), keepdim=True)
+    std = (var + eps).sqrt()
+    mean_err = 200 * U * var.sqrt() + 4 * U * mean.abs()
+    var_err = 600 * U * var + 2 * mean_err * var.sqrt() + mean_err ** 2
+    hat = d / std
+    hat_err = (mean_err + 2 * U * d.abs()) / std + hat.abs() * (0.5 * var_err / (var + eps) + 4 * U)
+    g = 1.0 if gamma is None else gamma.double()
+    b = 0.0 if beta is None else beta.double()
+    v = hat.reshape(f, p, c) * g + b
+    v_err = hat_err.reshape(f, p, c) * abs(g) + 2 * U * v.abs()
+    return finish(v, v_err, act, None, dtype)
+
 def check(got, want, bound):
     off = (got.double() - want).abs()
     worst = (off / bound).max().item() if off.numel() else 0.0

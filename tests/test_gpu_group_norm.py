@@ -227,3 +227,29 @@ def test_activations_of_infinities(act, y_type, pixels):
     y = capi.group_norm(x, 3, gamma, beta, 1e-6, ro.ACTS[act], out_dtype=getattr(torch, y_type))
     assert (y[:, :, :8] == float("inf")).all()
     assert y[:, :, 8:16].isnan().all() and y[:, :, 16:].isfinite().all()
+
+
+# one launch; single channels, 450 pixels a thread; vectors of four, 200; frames of
+# 16-bit rows, vectors of eight, 112
+@pytest.mark.parametrize("size", [(1, 64, 512, 32, "float32"), (2, 2000, 512, 32, "float32"),
+                                  (1, 7000, 4, 1, "float32"), (1, 59_000_000, 1, 1, "float32"),
+                                  (1, 26_214_400, 4, 1, "float32"), (4, 230400, 128, 32, "bfloat16")], ids=str)
+@pytest.mark.parametrize("far", [1e2, 1e4, 1e6])
+@pytest.mark.parametrize("count", [1, 700])
+def test_values_far_from_the_others(size, far, count):
+    """The first value, or the first pixels (a border), far from all others, which are
+    where the statistics begin."""
+    import torch
+    import row_operators as ro
+    f, p, c, g, dtype = size
+    gen = torch.Generator(device="cuda").manual_seed(c)
+    x = torch.randn(f, p, c, generator=gen, device="cuda")
+    if count == 1:
+        x[:, 0, ::c // g] += far
+    else:
+        x[:, :min(count, p // 3)] += far
+    x = x.to(getattr(torch, dtype))
+    y = capi.group_norm(x, g, out_dtype=torch.float32)
+    for i in range(f):
+        want, bound = ro.group_norm_by_variance(x[i:i + 1], g, None, None, 1e-6, "none", y.dtype)
+        ro.check(y[i:i + 1], want, bound)
