@@ -411,8 +411,8 @@ __global__ __launch_bounds__(kThreads) void group_norm_apply_kernel(GroupNormArg
                     if (j + u * sp.rows < np) {
 #pragma unroll
                         for (int i = 0; i < V; ++i)
-                            v[u][i] = activate(fmaf(v[u][i] - mean[i], scale[i], shift[i]),
-                                               decltype(act)::value);
+                            v[u][i] = activate<YK == 0>(fmaf(v[u][i] - mean[i], scale[i], shift[i]),
+                                                        decltype(act)::value);
                         store_v<V, YK, true>(p.y, y0 + (long)(j + u * sp.rows) * p.y_pixel + c, v[u]);
                     }
             }
@@ -503,7 +503,8 @@ __global__ __launch_bounds__(THREADS) void group_norm_small_kernel(GroupNormArgs
             if (u < count) {
 #pragma unroll
                 for (int i = 0; i < V; ++i)
-                    v[u][i] = activate(fmaf(v[u][i] - mean, scale[i], shift[i]), decltype(act)::value);
+                    v[u][i] = activate<YK == 0>(fmaf(v[u][i] - mean, scale[i], shift[i]),
+                                                decltype(act)::value);
                 store_v<V, YK>(p.y, f * p.y_frame + (long)(row + u * rows) * p.y_pixel + c, v[u]);
             }
     });

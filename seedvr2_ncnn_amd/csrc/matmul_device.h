@@ -226,7 +226,7 @@ struct TileEnd {
 #pragma unroll
             for (int r = 0; r < 4; ++r)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) v[r][j] = activate(acc[i][j][r] + bias[j], ACT);
+                for (int j = 0; j < 4; ++j) v[r][j] = activate<YK == 0>(acc[i][j][r] + bias[j], ACT);
             if (res) {
 #pragma unroll
                 for (int r = 0; r < 4; ++r)

@@ -132,7 +132,7 @@ __global__ __launch_bounds__(512) void matmul_rows_kernel(MatmulArgs a, int ntil
         float v = sums[0][o];
         for (int s = 1; s < waves; ++s) v += sums[s][o];
         if (a.bias) v += a.bias[(long)rt.group * a.n + col];
-        v = activate(v, a.act);
+        v = a.y_kind ? activate<false>(v, a.act) : activate<true>(v, a.act);
         if (a.res) v += load1(a.res, row * a.res_stride + col, a.y_kind);
         store1(a.y, row * a.y_stride + col, v, a.y_kind);
     }

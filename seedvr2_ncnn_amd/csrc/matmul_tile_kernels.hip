@@ -368,7 +368,7 @@ __global__ __launch_bounds__(256) void matmul_sum_kernel(MatmulArgs a, TileSplit
                 if (j < cols) v[j] += a.bias[col + j];
         with_activation(a.act, [&](auto act) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] = activate(v[j], decltype(act)::value);
+            for (int j = 0; j < 4; ++j) v[j] = activate<YK == 0>(v[j], decltype(act)::value);
         });
         if (a.res)
 #pragma unroll

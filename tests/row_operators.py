@@ -34,6 +34,18 @@ def activation_error(v, act):
     return torch.zeros_like(v)
 
 
+def exact_gelu(v):
+    return 0.5 * v * torch.erfc(-v / 2.0 ** 0.5)
+
+
+def exact_gelu_error(v):
+    """Of an erf-GELU as the product of v / 2 and erfc(-v / sqrt 2) in fp32: erfc's
+    argument z is off by 2 U |z|, which moves it by no more than 2 z^2 + 1 times as much
+    relative to itself (its slope is under 2 z + 1 times it); it is off by 4 steps (8 U),
+    the products by 3 U, all relative to the value."""
+    return (12 + 2 * (v * v + 1)) * U * exact_gelu(v).abs() + torch.finfo(torch.float32).tiny
+
+
 def rounding(y, dtype):
     """Half a step of dtype at y; subnormals' step is the smallest number's."""
     info = torch.finfo(dtype)

@@ -253,3 +253,17 @@ def test_values_far_from_the_others(size, far, count):
     for i in range(f):
         want, bound = ro.group_norm_by_variance(x[i:i + 1], g, None, None, 1e-6, "none", y.dtype)
         ro.check(y[i:i + 1], want, bound)
+
+
+@pytest.mark.parametrize("c", [4000, 4001])
+@pytest.mark.parametrize("pixels", [3, 300])
+def test_erf_gelu_of_fp32_results(c, pixels):
+    """To fp32's precision relative to the value, out into the negative tail."""
+    import torch
+    import row_operators as ro
+    beta = torch.linspace(-12, 12, c, device="cuda")
+    for dtype in TYPES:
+        x = torch.full((1, pixels, c), 3.0, dtype=getattr(torch, dtype), device="cuda")
+        y = capi.group_norm(x, 1, None, beta, 1e-6, capi.ACT_GELU, out_dtype=torch.float32)
+        v = beta.double().expand(1, pixels, c)
+        ro.check(y, ro.exact_gelu(v), ro.exact_gelu_error(v))

@@ -566,3 +566,28 @@ def test_activations_of_infinities(act, y_type, m, k, n, pair):
             assert (y[:, ::3] == float("inf")).all()
             assert y[:, 1::3].isnan().all()
             assert y[:, 2::3].isfinite().all()
+
+
+@pytest.mark.parametrize("m,k,width", [(1, 64, 4001), (40, 64, 4000), (300, 64, 4001), (77, 5120, 4000),
+                                       (2500, 32, 4001)], ids=str)
+@pytest.mark.parametrize("pair", PAIRS, ids="-".join)
+@pytest.mark.parametrize("workspace", [True, False])
+def test_erf_gelu_of_fp32_results(m, k, width, pair, workspace):
+    """To fp32's precision relative to the value, out into the negative tail; the
+    values come by the bias, and with a residual."""
+    import torch
+    import row_operators as ro
+    x, w, _, res = _operands(m, k, width, pair, "float32")
+    x.zero_()
+    bias = torch.linspace(-12, 12, width, device="cuda")
+    v = bias.double().expand(m, width)
+    room = None if workspace else torch.empty(0, dtype=torch.uint8, device="cuda")
+    offs = torch.tensor([0, m], dtype=torch.int32, device="cuda")
+    for r in (None, res * 1e-6):
+        want, err = ro.exact_gelu(v), ro.exact_gelu_error(v)
+        if r is not None:
+            want = want + r.double()
+            err = err + ro.U * (want.abs() + err)
+        ro.check(capi.linear(x, w, bias, capi.ACT_GELU, r, out_dtype=torch.float32, workspace=room), want, err)
+        ro.check(capi.grouped_linear(x, offs, w[None], bias[None], capi.ACT_GELU, r, out_dtype=torch.float32,
+                                     workspace=room), want, err)
