@@ -540,12 +540,19 @@ S2_API int s2_group_norm(const void* x, s2_dtype x_dtype, long x_frame_stride,
  * Any m (0 does nothing), n and k up to 2^30; pointers aligned to their elements.
  *   Fastest are k a multiple of 8 and n of 4, with x and weight rows that start
  *   at 16 bytes and y and residual rows at four elements.
- * workspace: s2_linear_workspace_bytes, 16-byte aligned (calls that may overlap
- *   in time need one each): rows repacked for the matrix cores, sums of ranges of
- *   k.  A smaller one, or NULL, is accepted: the call then does without, slower
- *   for fp32 x, for k that is no multiple of 8 and for few output tiles. */
+ * workspace: 16-byte aligned (calls that may overlap in time need one each): rows
+ *   repacked for the matrix cores, sums of ranges of k.  s2_linear_workspace_bytes
+ *   is what a call with contiguous x takes, x and weight starting at 16 bytes;
+ *   s2_linear_view_workspace_bytes what one takes with x's row stride and where x
+ *   and weight lie (addresses of the same alignment do; none is read, NULL is an
+ *   aligned one).  A smaller workspace, or NULL, is accepted: the call then does
+ *   without, slower for fp32 x, for k or an x_stride that is no multiple of 8, for x
+ *   or weight that start at no 16 bytes and for few output tiles. */
 S2_API int s2_linear_workspace_bytes(int m, int n, int k, s2_dtype x_dtype, s2_dtype y_dtype,
                                      size_t* bytes);
+S2_API int s2_linear_view_workspace_bytes(const void* x, s2_dtype x_dtype, long x_stride, int m,
+                                          const void* weight, int n, int k, s2_dtype y_dtype,
+                                          size_t* bytes);
 S2_API int s2_linear(const void* x, s2_dtype x_dtype, long x_stride, int m, const void* weight,
                      s2_dtype w_dtype, const float* bias, int n, int k, int activation,
                      const void* residual, long residual_stride, void* y, s2_dtype y_dtype,
@@ -562,9 +569,13 @@ S2_API int s2_linear(const void* x, s2_dtype x_dtype, long x_stride, int m, cons
  *   rows that descending offsets put into two groups, or into none, have
  *   unspecified values.
  * weight: device [groups][n][k]; bias: device fp32 [groups][n] or NULL; the
- *   rest as for s2_linear, workspace: s2_grouped_linear_workspace_bytes. */
+ *   rest as for s2_linear, workspace: s2_grouped_linear_workspace_bytes and
+ *   s2_grouped_linear_view_workspace_bytes. */
 S2_API int s2_grouped_linear_workspace_bytes(int m, int groups, int n, int k, s2_dtype x_dtype,
                                              s2_dtype y_dtype, size_t* bytes);
+S2_API int s2_grouped_linear_view_workspace_bytes(const void* x, s2_dtype x_dtype, long x_stride,
+                                                  int m, int groups, const void* weight, int n,
+                                                  int k, s2_dtype y_dtype, size_t* bytes);
 S2_API int s2_grouped_linear(const void* x, s2_dtype x_dtype, long x_stride, int m,
                              const int* offsets, int groups, const void* weight, s2_dtype w_dtype,
                              const float* bias, int n, int k, int activation,

@@ -48,7 +48,8 @@ EXPORTS = (
     "s2_binary_op", "s2_unary_op", "s2_reduce", "s2_rms_norm", "s2_copy_2d",
     "s2_shared_linear_residual", "s2_group_norm_workspace_bytes", "s2_group_norm",
     "s2_linear_workspace_bytes", "s2_linear", "s2_grouped_linear_workspace_bytes",
-    "s2_grouped_linear",
+    "s2_grouped_linear", "s2_linear_view_workspace_bytes",
+    "s2_grouped_linear_view_workspace_bytes",
 )
 
 
@@ -185,6 +186,8 @@ def lib() -> ctypes.CDLL:
                                     vp, sz, vp]
         L.s2_linear_workspace_bytes.argtypes = [ci, ci, ci, ci, ci, P(sz)]
         L.s2_grouped_linear_workspace_bytes.argtypes = [ci, ci, ci, ci, ci, ci, P(sz)]
+        L.s2_linear_view_workspace_bytes.argtypes = [vp, ci, cl, ci, vp, ci, ci, ci, P(sz)]
+        L.s2_grouped_linear_view_workspace_bytes.argtypes = [vp, ci, cl, ci, ci, vp, ci, ci, ci, P(sz)]
         L.s2_linear.argtypes = [vp, ci, cl, ci, vp, ci, vp, ci, ci, ci, vp, cl, vp, ci, cl, vp, sz,
                                 vp]
         L.s2_grouped_linear.argtypes = [vp, ci, cl, ci, vp, ci, vp, ci, vp, ci, ci, ci, vp, cl, vp,
@@ -795,21 +798,26 @@ def _matmul_views(x, n, k, weight, residual, out, out_dtype, stream):
 
 
 @functools.lru_cache(maxsize=4096)
-def linear_workspace(m, n, k, x_dtype=DTYPE_BF16, y_dtype=DTYPE_BF16) -> int:
-    """s2_linear_workspace_bytes."""
+def linear_workspace(m, n, k, x_dtype=DTYPE_BF16, y_dtype=DTYPE_BF16, x_stride=None, x_start=0,
+                     weight_start=0) -> int:
+    """s2_linear_view_workspace_bytes of rows x_stride elements apart (None: k) in x and
+    weight that start so many bytes after a 16-byte boundary."""
     b = ctypes.c_size_t()
-    check(lib().s2_linear_workspace_bytes(m, n, k, x_dtype, y_dtype, ctypes.byref(b)),
-          "s2_linear_workspace_bytes")
+    check(lib().s2_linear_view_workspace_bytes(x_start, x_dtype, k if x_stride is None else x_stride, m,
+                                               weight_start, n, k, y_dtype, ctypes.byref(b)),
+          "s2_linear_view_workspace_bytes")
     return b.value
 
 
 @functools.lru_cache(maxsize=4096)
-def grouped_linear_workspace(m, groups, n, k, x_dtype=DTYPE_BF16, y_dtype=DTYPE_BF16) -> int:
-    """s2_grouped_linear_workspace_bytes."""
+def grouped_linear_workspace(m, groups, n, k, x_dtype=DTYPE_BF16, y_dtype=DTYPE_BF16, x_stride=None,
+                             x_start=0, weight_start=0) -> int:
+    """s2_grouped_linear_view_workspace_bytes; x_stride, x_start and weight_start as for
+    linear_workspace."""
     b = ctypes.c_size_t()
-    check(lib().s2_grouped_linear_workspace_bytes(m, groups, n, k, x_dtype, y_dtype,
-                                                  ctypes.byref(b)),
-          "s2_grouped_linear_workspace_bytes")
+    check(lib().s2_grouped_linear_view_workspace_bytes(
+        x_start, x_dtype, k if x_stride is None else x_stride, m, groups, weight_start, n, k, y_dtype,
+        ctypes.byref(b)), "s2_grouped_linear_view_workspace_bytes")
     return b.value
 
 
@@ -817,15 +825,17 @@ def linear(x, weight, bias=None, activation=ACT_NONE, residual=None, out=None, o
            workspace=None, stream=None):
     """s2_linear: residual + act(x W^T + bias) of rows x [m, k] with weight
     [n, k] (bf16 for fp32 and bf16 rows, fp16 for fp16 rows).  Rows may be
-    strided.  out may be the residual.  workspace: linear_workspace(...) bytes,
-    made here if None.  Returns out [m, n]."""
+    strided.  out may be the residual.  workspace: linear_workspace(...) bytes for
+    these strides and addresses, made here if None.  Returns out [m, n]."""
     n, k = weight.shape
     out, m, xs, rs, os_ = _matmul_views(x, n, k, weight, residual, out, out_dtype, stream)
     xd, yd = _dtype_code(x), _dtype_code(out)
     bi = None if bias is None else _vector(bias, n, "bias")
     handle = _raw_stream(x, stream, weight, bias, residual, out, workspace)
-    workspace, ws, size = _workspace(workspace, stream, x, linear_workspace(m, n, k, xd, yd))
-    check(lib().s2_linear(x.data_ptr(), xd, xs, m, weight.data_ptr(), _dtype_code(weight), bi, n, k,
+    xp, wp = x.data_ptr(), weight.data_ptr()
+    workspace, ws, size = _workspace(workspace, stream, x,
+                                     linear_workspace(m, n, k, xd, yd, xs, xp & 15, wp & 15))
+    check(lib().s2_linear(xp, xd, xs, m, wp, _dtype_code(weight), bi, n, k,
                           activation, _ptr(residual), rs, out.data_ptr(), yd, os_, ws, size, handle),
           "s2_linear")
     return out
@@ -846,10 +856,11 @@ def grouped_linear(x, offsets, weight, bias=None, activation=ACT_NONE, residual=
     xd, yd = _dtype_code(x), _dtype_code(out)
     bi = None if bias is None else _vector(bias, groups * n, "bias")
     handle = _raw_stream(x, stream, offsets, weight, bias, residual, out, workspace)
-    workspace, ws, size = _workspace(workspace, stream, x,
-                                     grouped_linear_workspace(m, groups, n, k, xd, yd))
-    check(lib().s2_grouped_linear(x.data_ptr(), xd, xs, m, offsets.data_ptr(), groups,
-                                  weight.data_ptr(), _dtype_code(weight), bi, n, k, activation,
+    xp, wp = x.data_ptr(), weight.data_ptr()
+    workspace, ws, size = _workspace(workspace, stream, x, grouped_linear_workspace(
+        m, groups, n, k, xd, yd, xs, xp & 15, wp & 15))
+    check(lib().s2_grouped_linear(xp, xd, xs, m, offsets.data_ptr(), groups,
+                                  wp, _dtype_code(weight), bi, n, k, activation,
                                   _ptr(residual), rs, out.data_ptr(), yd, os_, ws, size, handle),
           "s2_grouped_linear")
     return out

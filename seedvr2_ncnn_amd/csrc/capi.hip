@@ -1345,19 +1345,26 @@ static int matmul_args_ok(const s2::MatmulArgs& a, bool grouped) {
     return S2_OK;
 }
 
-static int matmul_workspace(int m, const int* offsets, int groups, int n, int k, s2_dtype x_dtype,
-                            s2_dtype y_dtype, size_t* bytes) {
+// x and weight: addresses of the operands' alignment, not read.
+static int matmul_workspace(const void* x, s2_dtype x_dtype, long x_stride, int m, const int* offsets,
+                            int groups, const void* weight, int n, int k, s2_dtype y_dtype,
+                            size_t* bytes) {
     if (!bytes) return fail(S2_ERR_INVALID, "null bytes");
     if (!matmul_shape_ok(m, offsets, groups, n, k)) return fail(S2_ERR_INVALID, "invalid linear shape");
     if (!dtype_ok(x_dtype) || !dtype_ok(y_dtype)) return fail(S2_ERR_INVALID, "unsupported dtype");
     *bytes = 0;
     if (m == 0 || groups == 0) return S2_OK;
+    if (m > 1 && x_stride < k) return fail(S2_ERR_INVALID, "row strides shorter than rows");
+    if (!aligned(x, dtype_bytes(x_dtype)) || !aligned(weight, 2))
+        return fail(S2_ERR_INVALID, "operands must be aligned to their elements");
     s2::MatmulArgs a{};
+    a.x = x;
     a.x_kind = (int)x_dtype;
-    a.x_stride = k;
+    a.x_stride = m > 1 ? x_stride : k;
     a.m = m;
     a.offsets = offsets;
     a.groups = groups;
+    a.w = weight;
     a.w_kind = x_dtype == S2_DTYPE_F16 ? S2_DTYPE_F16 : S2_DTYPE_BF16;
     a.n = n;
     a.k = k;
@@ -1369,13 +1376,25 @@ static int matmul_workspace(int m, const int* offsets, int groups, int n, int k,
 
 int s2_linear_workspace_bytes(int m, int n, int k, s2_dtype x_dtype, s2_dtype y_dtype,
                               size_t* bytes) {
-    return matmul_workspace(m, nullptr, 1, n, k, x_dtype, y_dtype, bytes);
+    return matmul_workspace(nullptr, x_dtype, k, m, nullptr, 1, nullptr, n, k, y_dtype, bytes);
 }
+
+int s2_linear_view_workspace_bytes(const void* x, s2_dtype x_dtype, long x_stride, int m,
+                                   const void* weight, int n, int k, s2_dtype y_dtype, size_t* bytes) {
+    return matmul_workspace(x, x_dtype, x_stride, m, nullptr, 1, weight, n, k, y_dtype, bytes);
+}
+
+static const int some_offsets = 0;   // stand for a call's own, which the plan does not read
 
 int s2_grouped_linear_workspace_bytes(int m, int groups, int n, int k, s2_dtype x_dtype,
                                       s2_dtype y_dtype, size_t* bytes) {
-    static const int some = 0;   // offsets that only say that there are some
-    return matmul_workspace(m, &some, groups, n, k, x_dtype, y_dtype, bytes);
+    return matmul_workspace(nullptr, x_dtype, k, m, &some_offsets, groups, nullptr, n, k, y_dtype, bytes);
+}
+
+int s2_grouped_linear_view_workspace_bytes(const void* x, s2_dtype x_dtype, long x_stride, int m,
+                                           int groups, const void* weight, int n, int k,
+                                           s2_dtype y_dtype, size_t* bytes) {
+    return matmul_workspace(x, x_dtype, x_stride, m, &some_offsets, groups, weight, n, k, y_dtype, bytes);
 }
 
 int s2_linear(const void* x, s2_dtype x_dtype, long x_stride, int m, const void* weight,

@@ -209,6 +209,14 @@ double tiles_us(const TileCost& t, double blocks, double steps) {
            (rest > 0 ? t.round + steps * (rest <= kUnits ? t.one : t.full) : 0.);
 }
 
+// The kernel for any shape with 16-bit rows, by the same measure, against packing those
+// rows (and the weight) first: a launch, and bytes a microsecond read and written.  Rows
+// apart by four elements too many: 8000 x 2560 by 2560 x 2560 177 us here and 118 packed,
+// 300 x 2560 by 512 x 2560 66 and 14, 14400 x 1024 by 512 x 1024 37 and 34, but x 512 19
+// and 25, 100000 x 512 by 64 x 512 39 and 52, 2000 x 128 by 512 x 128 8 and 11.
+constexpr TileCost kAnyCost = {128, 128, 2, 2.5, 1.5, 2.1};
+constexpr double kPackUs = 5., kPackBytesUs = 5e6;
+
 // The sums of k ranges: a launch, and bytes a microsecond written and read again.
 constexpr double kSumUs = 3., kSumBytesUs = 9e6;
 
@@ -280,11 +288,14 @@ MatmulPlan plan_matmul(const MatmulArgs& a, size_t workspace_bytes) {
         const size_t each = (size_t)a.m * round_up(a.n, 4) * sizeof(float);   // a range's sums
         const long most =
             a.offsets ? 1 : std::min<long>(16, (long)((workspace_bytes - p.bytes()) / each));
+        // a group's last tile is half empty, on average
+        auto count_of = [&](const TileCost& t) {
+            return (a.offsets ? (double)a.m / t.bm + 0.5 * std::min(a.groups, a.m)
+                              : (double)row_tiles(a, t.bm)) *
+                   (double)((a.n + t.bn - 1) / t.bn);
+        };
         for (const TileCost& t : kTileCosts) {
-            // a group's last tile is half empty, on average
-            const double count = (a.offsets ? (double)a.m / t.bm + 0.5 * std::min(a.groups, a.m)
-                                            : (double)row_tiles(a, t.bm)) *
-                                 (double)((a.n + t.bn - 1) / t.bn);
+            const double count = count_of(t);
             for (long parts = 1; parts <= std::max<long>(1, std::min(most, steps / 4)); ++parts) {
                 const double us =
                     std::max(tiles_us(t, count * parts, (double)steps / parts), weight_us(a)) +
@@ -298,7 +309,10 @@ MatmulPlan plan_matmul(const MatmulArgs& a, size_t workspace_bytes) {
             }
         }
         if (p.parts > 1) p.sum_bytes = p.parts * each;
-        if (rows > 32) return p;
+        const bool any = a.x_kind != 0 && p.pack_x &&
+                         tiles_us(kAnyCost, count_of(kAnyCost), (a.k + 63) / 64) <
+                             tile_us + kPackUs + 2. * (double)(p.x_bytes + p.w_bytes) / kPackBytesUs;
+        if (rows > 32 && !any) return p;
     }
 
     // few rows
@@ -321,7 +335,7 @@ MatmulPlan plan_matmul(const MatmulArgs& a, size_t workspace_bytes) {
                                       : a.x_kind == 0 && rows > 16 && !p.pack_w;
         return tiles && use_tiles ? p : r;
     }
-    // any shape, without a workspace; rows that 32-bit offsets do not reach
+    // any shape, unpacked; rows that 32-bit offsets do not reach
     r.kernel = near ? MatmulPlan::kAny : MatmulPlan::kRows;
     r.parts = 1;
     return r;

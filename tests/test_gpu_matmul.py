@@ -591,3 +591,37 @@ def test_erf_gelu_of_fp32_results(m, k, width, pair, workspace):
         ro.check(capi.linear(x, w, bias, capi.ACT_GELU, r, out_dtype=torch.float32, workspace=room), want, err)
         ro.check(capi.grouped_linear(x, offs, w[None], bias[None], capi.ACT_GELU, r, out_dtype=torch.float32,
                                      workspace=room), want, err)
+
+
+@pytest.mark.parametrize("pair", PAIRS[1:], ids="-".join)
+@pytest.mark.parametrize("m,k,n", [(40, 512, 96), (300, 320, 136), (1000, 2560, 2001)], ids=str)
+def test_room_for_rows_that_the_tiles_cannot_read(m, k, n, pair, monkeypatch):
+    """Rows of x apart by no multiple of eight elements, rows and weights that start at no
+    16-byte boundary: the bindings' workspace has room to repack them, and the call takes
+    the same kernels as with any amount."""
+    import torch
+    taken = []
+    made = capi._workspace
+    monkeypatch.setattr(capi, "_workspace", lambda w, s, x, size: (taken.append(size), made(w, s, x, size))[1])
+    x, w, bias, res = _operands(m, k, n, pair, pair[0])
+    offs = torch.tensor([0, m // 3, m], dtype=torch.int32, device="cuda")
+    wg, bg = torch.stack([w, w]), torch.stack([bias, bias])
+    for first, pad, odd in ((0, 4, 0), (3, 5, 0), (0, 0, 1), (4, 4, 4)):
+        xw = torch.full((m, k + pad), float("nan"), dtype=x.dtype, device="cuda")
+        xw = torch.cat([xw.flatten(), xw.new_zeros(first)])[first:first + m * (k + pad)].view(m, k + pad)[:, :k]
+        xw.copy_(x)
+
+        def moved(t):
+            flat = torch.empty(t.numel() + odd, dtype=t.dtype, device="cuda")
+            return flat[odd:].view_as(t).copy_(t)
+
+        need = 2 * m * k + (2 * n * k if odd else 0)
+        got = capi.linear(xw, moved(w), bias, capi.ACT_SILU, res)
+        assert taken[-1] >= need
+        _check(got, x, w, bias, "silu", res)
+        plenty = torch.empty(8 * (need + 64 * m * n), dtype=torch.uint8, device="cuda")
+        assert torch.equal(got, capi.linear(xw, moved(w), bias, capi.ACT_SILU, res, workspace=plenty))
+        got = capi.grouped_linear(xw, offs, moved(wg), bg, capi.ACT_SILU, res)
+        if m // 2 > 32:
+            assert taken[-2] >= need
+        _check(got, x, w, bias, "silu", res)

@@ -154,3 +154,30 @@ def test_bindings_check_shapes_and_types():
         capi.linear(x.double(), w)
     with pytest.raises(TypeError):
         capi.group_norm(frames.double(), 8)
+
+
+def test_workspaces_of_strided_and_unaligned_operands():
+    """Room to repack 16-bit rows that are apart by no multiple of eight elements or start
+    at no 16-byte boundary, and weights that do; the strides of a single row say nothing."""
+    for dtype in (BF16, F16):
+        base = capi.linear_workspace(8000, 2001, 2560, dtype, dtype)
+        assert capi.linear_workspace(8000, 2001, 2560, dtype, dtype, x_stride=2560) == base
+        assert capi.linear_workspace(8000, 2001, 2560, dtype, dtype, x_stride=2568, x_start=32) == base
+        rows = 8000 * 2560 * 2
+        for change in (dict(x_stride=2564), dict(x_start=8), dict(x_stride=2561, x_start=2)):
+            assert capi.linear_workspace(8000, 2001, 2560, dtype, dtype, **change) >= base + rows
+            assert capi.grouped_linear_workspace(8000, 2, 2001, 2560, dtype, dtype, **change) >= rows
+        assert capi.linear_workspace(8000, 2001, 2560, dtype, dtype, weight_start=2) >= rows + 2001 * 2560 * 2
+        assert capi.grouped_linear_workspace(8000, 3, 2001, 2560, dtype, dtype,
+                                             weight_start=6) >= rows + 3 * 2001 * 2560 * 2
+        one = capi.linear_workspace(1, 2001, 2560, dtype, dtype)
+        assert capi.linear_workspace(1, 2001, 2560, dtype, dtype, x_stride=3) == one
+    for bad in (dict(x_stride=63), dict(x_start=1), dict(weight_start=3)):
+        with pytest.raises(capi.S2Error):
+            capi.linear_workspace(9, 32, 64, BF16, BF16, **bad)
+        with pytest.raises(capi.S2Error):
+            capi.grouped_linear_workspace(9, 2, 32, 64, BF16, BF16, **bad)
+    assert capi.lib().s2_linear_view_workspace_bytes(None, BF16, 64, 9, None, 32, 64, BF16,
+                                                     None) == capi.S2_ERR_INVALID
+    assert capi.lib().s2_grouped_linear_view_workspace_bytes(None, BF16, 64, 9, 2, None, 32, 64, BF16,
+                                                             None) == capi.S2_ERR_INVALID
