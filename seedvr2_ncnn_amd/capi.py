@@ -54,8 +54,8 @@ EXPORTS = (
 
 
 class S2Error(RuntimeError):
-    def __init__(self, code, what=""):
-        super().__init__(f"{what} returned {code}: {last_error()}")
+    def __init__(self, code, what="", why=None):
+        super().__init__(f"{what} returned {code}: {last_error() if why is None else why}")
         self.code = code
 
 
@@ -692,6 +692,21 @@ def denoise_update(positive_patches, negative_patches, frames, height, width, cf
 
 # ---- group norm, linear, grouped linear --------------------------------------
 
+_INT_MAX = 2 ** 31 - 1
+_ROW_ACTIVATIONS = frozenset((ACT_NONE, ACT_GELU, ACT_SILU, ACT_GELU_TANH))
+
+
+def _refuse(what, why):
+    raise S2Error(S2_ERR_INVALID, what, why)
+
+
+def _c_ints(what, *values):
+    """Refuses what a C int does not hold: ctypes would pass it modulo 2^32."""
+    for v in values:
+        if not -_INT_MAX <= v <= _INT_MAX:
+            _refuse(what, f"{v} is out of range")
+
+
 def _vector(t, size, name):
     """Checks a contiguous fp32 vector (gamma, beta, bias); returns its address."""
     import torch
@@ -742,13 +757,17 @@ def group_norm(x, groups, gamma=None, beta=None, epsilon=1e-6, activation=ACT_NO
     channels] (any frame and pixel strides, contiguous channels), statistics per
     frame and group of channels.  out may be x.  workspace: at least
     group_norm_workspace(...) bytes, made here if None.  Returns out."""
-    if x.dim() != 3:
+    shape = x.shape
+    if len(shape) != 3:
         raise ValueError("x must be [frames, pixels, channels]")
-    f, p, c = x.shape
+    f, p, c = shape
+    need = group_norm_workspace(f, p, c, groups)
+    if activation not in _ROW_ACTIVATIONS:
+        _refuse("group_norm", "unknown activation")
     xd = _dtype_code(x)
     if out is None:
         out = _empty((f, p, c), out_dtype or x.dtype, x, stream)
-    elif out.shape != x.shape:
+    elif out.shape != shape:
         raise ValueError("x and out must be of one shape")
     xf, xp, xc = x.stride()
     of, op, oc = out.stride()
@@ -757,7 +776,7 @@ def group_norm(x, groups, gamma=None, beta=None, epsilon=1e-6, activation=ACT_NO
     ga = None if gamma is None else _vector(gamma, c, "gamma")
     be = None if beta is None else _vector(beta, c, "beta")
     handle = _raw_stream(x, stream, out, gamma, beta, workspace)
-    workspace, ws, size = _workspace(workspace, stream, x, group_norm_workspace(f, p, c, groups))
+    workspace, ws, size = _workspace(workspace, stream, x, need)
     check(lib().s2_group_norm(x.data_ptr(), xd, xf, xp, f, p, c, groups, ga, be, epsilon, activation,
                               out.data_ptr(), _dtype_code(out), of, op, ws, size, handle),
           "s2_group_norm")
@@ -767,20 +786,29 @@ def group_norm(x, groups, gamma=None, beta=None, epsilon=1e-6, activation=ACT_NO
 @functools.lru_cache(maxsize=4096)
 def group_norm_workspace(frames, pixels, channels, groups) -> int:
     """s2_group_norm_workspace_bytes."""
+    _c_ints("group_norm_workspace", frames, pixels, channels, groups)
     n = ctypes.c_size_t()
     check(lib().s2_group_norm_workspace_bytes(frames, pixels, channels, groups, ctypes.byref(n)),
           "s2_group_norm_workspace_bytes")
     return n.value
 
 
-def _matmul_views(x, n, k, weight, residual, out, out_dtype, stream):
+def _matmul_views(x, groups, n, k, weight, activation, residual, out, out_dtype, stream):
     """(out, m, x's, residual's and out's row strides) of linear and grouped_linear,
     checked."""
-    if x.dim() != 2 or x.shape[1] != k or (k > 1 and x.stride(1) != 1):
+    shape = x.shape
+    if len(shape) != 2 or shape[1] != k:
+        raise ValueError(f"x must be [m, {k}] with contiguous rows")
+    m = shape[0]
+    if m > _INT_MAX or n > _INT_MAX or k > _INT_MAX or groups > _INT_MAX:
+        _refuse("linear", "a size is out of range")   # ctypes would pass it modulo 2^32
+    if activation not in _ROW_ACTIVATIONS:
+        _refuse("linear", "unknown activation")
+    xs, step = x.stride()
+    if k > 1 and step != 1:
         raise ValueError(f"x must be [m, {k}] with contiguous rows")
     if not weight.is_contiguous():
         raise ValueError("weight must be contiguous")
-    m = x.shape[0]
     if out is None:
         out = _empty((m, n), out_dtype or x.dtype, x, stream)
         os_ = n
@@ -794,7 +822,7 @@ def _matmul_views(x, n, k, weight, residual, out, out_dtype, stream):
                 n > 1 and residual.stride(1) != 1):
             raise ValueError(f"residual must be [{m}, {n}] of out's type with contiguous rows")
         rs = residual.stride(0)
-    return out, m, x.stride(0), rs, os_
+    return out, m, xs, rs, os_
 
 
 @functools.lru_cache(maxsize=4096)
@@ -802,6 +830,7 @@ def linear_workspace(m, n, k, x_dtype=DTYPE_BF16, y_dtype=DTYPE_BF16, x_stride=N
                      weight_start=0) -> int:
     """s2_linear_view_workspace_bytes of rows x_stride elements apart (None: k) in x and
     weight that start so many bytes after a 16-byte boundary."""
+    _c_ints("linear_workspace", m, n, k, x_dtype, y_dtype)
     b = ctypes.c_size_t()
     check(lib().s2_linear_view_workspace_bytes(x_start, x_dtype, k if x_stride is None else x_stride, m,
                                                weight_start, n, k, y_dtype, ctypes.byref(b)),
@@ -814,6 +843,7 @@ def grouped_linear_workspace(m, groups, n, k, x_dtype=DTYPE_BF16, y_dtype=DTYPE_
                              x_start=0, weight_start=0) -> int:
     """s2_grouped_linear_view_workspace_bytes; x_stride, x_start and weight_start as for
     linear_workspace."""
+    _c_ints("grouped_linear_workspace", m, groups, n, k, x_dtype, y_dtype)
     b = ctypes.c_size_t()
     check(lib().s2_grouped_linear_view_workspace_bytes(
         x_start, x_dtype, k if x_stride is None else x_stride, m, groups, weight_start, n, k, y_dtype,
@@ -828,7 +858,8 @@ def linear(x, weight, bias=None, activation=ACT_NONE, residual=None, out=None, o
     strided.  out may be the residual.  workspace: linear_workspace(...) bytes for
     these strides and addresses, made here if None.  Returns out [m, n]."""
     n, k = weight.shape
-    out, m, xs, rs, os_ = _matmul_views(x, n, k, weight, residual, out, out_dtype, stream)
+    out, m, xs, rs, os_ = _matmul_views(x, 1, n, k, weight, activation, residual, out, out_dtype,
+                                        stream)
     xd, yd = _dtype_code(x), _dtype_code(out)
     bi = None if bias is None else _vector(bias, n, "bias")
     handle = _raw_stream(x, stream, weight, bias, residual, out, workspace)
@@ -850,7 +881,8 @@ def grouped_linear(x, offsets, weight, bias=None, activation=ACT_NONE, residual=
     bytes, made here if None.  Returns out [m, n]."""
     import torch
     groups, n, k = weight.shape
-    out, m, xs, rs, os_ = _matmul_views(x, n, k, weight, residual, out, out_dtype, stream)
+    out, m, xs, rs, os_ = _matmul_views(x, groups, n, k, weight, activation, residual, out, out_dtype,
+                                        stream)
     if offsets.dtype is not torch.int32 or offsets.numel() != groups + 1 or not offsets.is_contiguous():
         raise ValueError(f"offsets must be {groups + 1} contiguous int32 values")
     xd, yd = _dtype_code(x), _dtype_code(out)

@@ -181,3 +181,41 @@ def test_workspaces_of_strided_and_unaligned_operands():
                                                      None) == capi.S2_ERR_INVALID
     assert capi.lib().s2_grouped_linear_view_workspace_bytes(None, BF16, 64, 9, 2, None, 32, 64, BF16,
                                                              None) == capi.S2_ERR_INVALID
+
+
+@pytest.mark.parametrize("wrap", [1 << 31, (1 << 32) + 3, -(1 << 32) + 3], ids=str)
+def test_sizes_that_32_bits_would_wrap_are_refused(wrap):
+    """A C int would take 2^32 + 3 for 3."""
+    for at in range(4):
+        sizes = [2, 8, 8, 2]
+        sizes[at] = wrap
+        with pytest.raises(capi.S2Error):
+            capi.group_norm_workspace(*sizes)
+        with pytest.raises(capi.S2Error):
+            capi.grouped_linear_workspace(*sizes)
+    for at in range(3):
+        sizes = [8, 8, 8]
+        sizes[at] = wrap
+        with pytest.raises(capi.S2Error):
+            capi.linear_workspace(*sizes)
+    with pytest.raises(capi.S2Error):
+        capi.linear_workspace(8, 8, 8, wrap, BF16)
+    with pytest.raises(capi.S2Error):
+        capi.grouped_linear_workspace(8, 2, 8, 8, BF16, wrap)
+
+
+def test_bindings_refuse_sizes_that_32_bits_would_wrap():
+    """Before anything of that size is made."""
+    import torch
+    many = (1 << 32) + 3
+    w, wide = torch.zeros(1, 1, dtype=torch.bfloat16), torch.zeros(1, 1, dtype=torch.bfloat16).expand(many, 1)
+    offs = torch.zeros(2, dtype=torch.int32)
+    for call in (lambda: capi.linear(wide, w), lambda: capi.linear(w, wide),
+                 lambda: capi.grouped_linear(wide, offs, w[None]),
+                 lambda: capi.group_norm(wide[None], 1), lambda: capi.group_norm(wide[:, None], 1),
+                 lambda: capi.group_norm(wide.t()[None], 1),
+                 lambda: capi.group_norm(w[None], many),
+                 lambda: capi.linear(w, w, activation=many), lambda: capi.group_norm(w[None], 1, activation=many),
+                 lambda: capi.grouped_linear(w, offs, w[None], activation=1 << 32)):
+        with pytest.raises(capi.S2Error):
+            call()
