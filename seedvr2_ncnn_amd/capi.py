@@ -717,7 +717,7 @@ def _vector(t, size, name):
 
 def _raw_stream(x, stream, *others):
     """The stream's handle; refuses tensors that the current device's kernels
-    cannot reach."""
+    cannot reach, and another device's stream, on which they would run there."""
     import torch
     device = x.get_device()
     near = device >= 0 and device == torch._C._cuda_getDevice()
@@ -726,7 +726,11 @@ def _raw_stream(x, stream, *others):
             near = False
     if not near:
         raise ValueError("operands must be on the current device")
-    return torch._C._cuda_getCurrentRawStream(device) if stream is None else stream.cuda_stream
+    if stream is None:
+        return torch._C._cuda_getCurrentRawStream(device)
+    if stream.device_index != device:
+        raise ValueError("the stream must be the current device's")
+    return stream.cuda_stream
 
 
 def _empty(shape, dtype, x, stream):

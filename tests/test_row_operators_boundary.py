@@ -219,3 +219,20 @@ def test_bindings_refuse_sizes_that_32_bits_would_wrap():
                  lambda: capi.grouped_linear(w, offs, w[None], activation=1 << 32)):
         with pytest.raises(capi.S2Error):
             call()
+
+
+def test_streams_of_another_device_are_refused(monkeypatch):
+    import torch
+
+    class On:
+        def __init__(self, index):
+            self.device_index, self.cuda_stream = index, 64 + index
+
+        def get_device(self):
+            return self.device_index
+
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0, raising=False)
+    assert capi._raw_stream(On(0), On(0), On(0), None) == 64
+    for stream, tensors in ((On(1), [On(0)]), (On(1), [On(1)]), (On(0), [On(0), On(1)])):
+        with pytest.raises(ValueError):
+            capi._raw_stream(tensors[0], stream, *tensors[1:])
