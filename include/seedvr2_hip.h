@@ -499,9 +499,10 @@ S2_API int s2_shared_linear_residual(const void* x_video, int m_video, const voi
  * src/seedvr2/seedvr2_vae.cpp:508-549 and seedvr2_dit.cpp:603-633, whose .param
  * files it does not hold), on rows with channels last.  Activations:
  * S2_ACT_NONE, _GELU, _SILU, _GELU_TANH.  All arithmetic is fp32 or wider; each
- * output is rounded once.  Activations are off by some steps of fp32 relative to
- * themselves (12 + 4 |argument of the exponential| halves at most), erf-GELU of 16-bit
- * outputs by 0.75e-7 of its argument.  Of -inf they are -inf * 0, NaN. */
+ * output is rounded once.  SiLU and tanh-GELU are off by at most (12 + 4 |z|) 2^-24
+ * of themselves, z being their exponential's argument, erf-GELU at x by (14 + 2 x^2)
+ * 2^-24 of itself for fp32 outputs and 0.75e-7 |x| for 16-bit ones; results under 2^-119
+ * may be zero.  Of -inf all three are -inf * 0, NaN. */
 
 /* y[f][p][c] = act((x[f][p][c] - mean) / sqrt(var + epsilon) * gamma[c] +
  * beta[c]), mean and (biased) variance over the pixels of frame f and the

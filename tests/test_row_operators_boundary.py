@@ -236,3 +236,15 @@ def test_streams_of_another_device_are_refused(monkeypatch):
     for stream, tensors in ((On(1), [On(0)]), (On(1), [On(1)]), (On(0), [On(0), On(1)])):
         with pytest.raises(ValueError):
             capi._raw_stream(tensors[0], stream, *tensors[1:])
+
+
+@pytest.mark.parametrize("types", [(F32, BF16), (F32, F32), (BF16, BF16), (F16, F32)], ids=str)
+@pytest.mark.parametrize("mnk", [(1, 640, 2560), (77, 2560, 5120), (300, 257, 133), (21600, 2560, 132)], ids=str)
+def test_workspaces_of_contiguous_operands(mnk, types):
+    """The queries without a view are those of contiguous, aligned operands."""
+    m, n, k = mnk
+    size = ctypes.c_size_t()
+    assert capi.lib().s2_linear_workspace_bytes(m, n, k, *types, ctypes.byref(size)) == capi.S2_OK
+    assert size.value == capi.linear_workspace(m, n, k, *types, x_stride=k)
+    assert capi.lib().s2_grouped_linear_workspace_bytes(m, 2, n, k, *types, ctypes.byref(size)) == capi.S2_OK
+    assert size.value == capi.grouped_linear_workspace(m, 2, n, k, *types, x_stride=k)
