@@ -330,7 +330,8 @@ MatmulPlan plan_matmul(const MatmulArgs& a, size_t workspace_bytes) {
         r.parts = 1;
         // against the tiles where those need no packing (16 x 10240 by 2560 x 10240 15 us
         // on tiles, 22 on rows; 1 x 10240 18 and 15); more than a few fp32 rows are packed
-        // rather than split by every workgroup (32 x 2560 by 2560 x 2560 20 and 22)
+        // rather than split by every workgroup (32 rows by 2560 x 10240 26 us and 49, by
+        // 2560 x 5120 18 and 26, by 2560 x 2560 15 both, but by 1024 x 1024 13 and 8)
         const bool use_tiles = direct ? tile_us < rows_us(a, r, std::min(rows, (long)a.m))
                                       : a.x_kind == 0 && rows > 16 && !p.pack_w;
         return tiles && use_tiles ? p : r;
