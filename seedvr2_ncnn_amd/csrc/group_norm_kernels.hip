@@ -61,13 +61,6 @@ struct Raw {
     }
 };
 
-template <int V, typename T>
-__device__ __forceinline__ void load_v(const T* p, float (&v)[V]) {
-    Raw<T, V> r;
-    r.load(p);
-    r.get(v);
-}
-
 template <bool NT, typename P, typename Q>
 __device__ __forceinline__ void put(P* at, Q q) {
     if constexpr (NT)

@@ -625,3 +625,28 @@ def test_room_for_rows_that_the_tiles_cannot_read(m, k, n, pair, monkeypatch):
         if m // 2 > 32:
             assert taken[-2] >= need
         _check(got, x, w, bias, "silu", res)
+
+
+def test_fp32_rows_far_apart():
+    """As test_rows_far_apart for fp32 rows: 70 of x, the residual and y over 9.4 GB each,
+    and rows enough for the short k's kernel whose x is apart by less and by more than
+    its offsets reach."""
+    import torch
+    m, k, n, far = 70, 72, 40, 2 ** 25 + 8
+    x, w, bias, res = _operands(m, k, n, PAIRS[0], "float32")
+    spread = [torch.empty(m * far, device="cuda") for _ in range(3)]
+    xw, rw, yw = (t.as_strided((m, c), (far, 1)) for t, c in zip(spread, (k, n, n)))
+    xw.copy_(x)
+    rw.copy_(res)
+    for args in ((xw, res, None), (x, res, yw), (x, rw, None), (xw, rw, rw)):
+        got = capi.linear(args[0], w, bias, capi.ACT_SILU, args[1], out=args[2])
+        _check(got, x, w, bias, "silu", res)
+    del spread, xw, rw, yw
+    m, k, n = 600, 60, 11000
+    x, w, bias, _ = _operands(m, k, n, PAIRS[0], "bfloat16")
+    for far in (2 ** 24 - 4, 2 ** 24 + 4):
+        xw = torch.empty(m * far, device="cuda").as_strided((m, k), (far, 1))
+        xw.copy_(x)
+        _check(capi.linear(xw, w, bias, out_dtype=torch.bfloat16), x, w, bias, "none", None)
+        del xw
+    torch.cuda.empty_cache()
