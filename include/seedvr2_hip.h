@@ -584,6 +584,99 @@ S2_API int s2_grouped_linear(const void* x, s2_dtype x_dtype, long x_stride, int
                              s2_dtype y_dtype, long y_stride, void* workspace,
                              size_t workspace_bytes, s2_stream_t stream);
 
+/* ---- MXFP4: rows and weights in four bits ------------------------------------ */
+/* A row of k values in MXFP4 is ceil(k / 32) blocks of 32, values past k being zeros:
+ * e2m1 codes (a sign and 0, 0.5, 1, 1.5, 2, 3, 4 or 6), two a byte, the first in the low
+ * half, 16 bytes a block; and an e8m0 scale a block, 2^(byte - 127), 255 for NaN, the
+ * microscaling formats' layout.  A value is its code's number times its block's scale.
+ *
+ * codes: device [rows][code_stride bytes], 16-byte aligned, code_stride a multiple of 16
+ *   and at least 16 ceil(k / 32).
+ * scales: device [rows][scale_stride bytes], scale_stride at least ceil(k / 32).  Products
+ *   are fastest with scales that start at 16 bytes, rows a multiple of 16 bytes apart. */
+
+/* Rows x [m][k] (x_dtype, row stride in elements) to MXFP4.  A block's scale is
+ * 2^(floor(log2 of its largest magnitude) - 2), at least 2^-127; a code is that of the
+ * number nearest to value / scale, ties to the even code, 6 for what is larger (up to
+ * 8).  Blocks with a NaN or an infinity become NaN.  Whole blocks are written, in
+ * codes and scales, nothing behind them.  m == 0 does nothing; k is 1 to 2^30. */
+S2_API int s2_mx_quantize(const void* x, s2_dtype x_dtype, long x_stride, int m, int k,
+                          void* codes, long code_stride, void* scales, long scale_stride,
+                          s2_stream_t stream);
+/* The values of MXFP4 rows, rounded to y_dtype (fp32 and bf16 hold them all up to their
+ * largest numbers, fp16 those of rows quantised from fp16). */
+S2_API int s2_mx_dequantize(const void* codes, long code_stride, const void* scales,
+                            long scale_stride, int m, int k, void* y, s2_dtype y_dtype,
+                            long y_stride, s2_stream_t stream);
+
+/* y = residual + act(x W^T + bias) of rows x [m][k] and a weight [n][k] in MXFP4, the
+ * products those of the values, exact, the sums in fp32; x in MXFP4 too (s2_mx_linear), or
+ * in x_dtype with a row stride in elements (s2_mx_weight_linear: fp32, bf16 or fp16, as
+ * one to three bf16 terms that hold it exactly).
+ *
+ * w_codes: contiguous rows of 16 ceil(k / 32) bytes.  Where k is no multiple of 32 the
+ *   codes past it are zeros in x or in the weight, as s2_mx_quantize writes them.
+ * bias, activation, residual, y: as for s2_linear; m, n and k up to 2^30.
+ * workspace: 16-byte aligned (calls that may overlap in time need one each); the queries
+ *   give what the fastest form takes, whatever the operands' strides and addresses.  A smaller one, or NULL, is
+ *   accepted: the call then does without, slower for many rows of x in x_dtype, for few
+ *   output tiles and for scales that start at no 16 bytes. */
+S2_API int s2_mx_linear_workspace_bytes(int m, int n, int k, s2_dtype y_dtype, size_t* bytes);
+S2_API int s2_mx_linear(const void* x_codes, long x_code_stride, const void* x_scales,
+                        long x_scale_stride, int m, const void* w_codes, const void* w_scales,
+                        long w_scale_stride, const float* bias, int n, int k, int activation,
+                        const void* residual, long residual_stride, void* y, s2_dtype y_dtype,
+                        long y_stride, void* workspace, size_t workspace_bytes,
+                        s2_stream_t stream);
+S2_API int s2_mx_weight_linear_workspace_bytes(int m, int n, int k, s2_dtype x_dtype,
+                                               s2_dtype y_dtype, size_t* bytes);
+S2_API int s2_mx_weight_linear(const void* x, s2_dtype x_dtype, long x_stride, int m,
+                               const void* w_codes, const void* w_scales, long w_scale_stride,
+                               const float* bias, int n, int k, int activation,
+                               const void* residual, long residual_stride, void* y,
+                               s2_dtype y_dtype, long y_stride, void* workspace,
+                               size_t workspace_bytes, s2_stream_t stream);
+
+/* ---- cross attention ------------------------------------------------------------ */
+/* out = softmax(scale q k^T) v per sample and head: tokens against an encoder's states,
+ * whose number is their own.  Head h of q reads head h / (heads / kv_heads) of k and v.
+ *
+ * Samples: `batch` of them, either padded to one length (q_offsets and k_offsets NULL):
+ *   q and out [batch][lq][heads][head_dim], k and v [batch][lk][kv_heads][head_dim],
+ *   key_lengths (device int32 [batch], or NULL) the keys of each, 0 to lk; or one after the
+ *   other: q and out [lq][heads][head_dim], k and v [lk][kv_heads][head_dim], sample b's
+ *   rows being q_offsets[b] .. q_offsets[b + 1] - 1 and k_offsets[b] .. k_offsets[b + 1]
+ *   - 1 (device int32 [batch + 1], ascending, read by the kernels, taken as the nearest
+ *   value in [0, lq] or [0, lk] where they are outside; key_lengths is NULL then).  Rows
+ *   of out in no sample are not written.
+ * Strides in elements, batch (unused with offsets), row, head, elements contiguous: for
+ *   q, k, v and out in turn, strides[0..11].  q, k and v are of one dtype; their rows
+ *   start at 16 bytes (strides a multiple of 16 bytes too); out's at its elements, its
+ *   rows do not overlap, and it overlaps nothing else, but may be q itself
+ *   (same dtype and strides).
+ * key_mask: device bytes [batch][mask_stride], or [lk] with offsets, 0 for keys to leave
+ *   out, or NULL.  What k and v hold where a key is left out, infinities and NaN among it,
+ *   is not used.  A query with no key left, or with scores of -inf
+ *   alone, gives zeros.
+ * head_dim: a multiple of 8 up to 256; heads a multiple of kv_heads.
+ * Scores, exponentials, their sums and out's sums are fp32; fp32 operands are multiplied in
+ *   fp32, 16-bit ones on the matrix cores, where the weights of v are rounded to their type.
+ * workspace: s2_cross_attention_workspace_bytes, 16-byte aligned (calls that may overlap
+ *   in time need one each): the sums of ranges of keys where there are few queries.  A
+ *   smaller one, or NULL, is accepted, and the ranges are fewer. */
+typedef struct s2_cross_attention_shape {
+    int batch, lq, lk, heads, kv_heads, head_dim;
+    s2_dtype dtype, out_dtype;
+    float scale;
+} s2_cross_attention_shape;
+S2_API int s2_cross_attention_workspace_bytes(const s2_cross_attention_shape* shape, int ragged,
+                                              size_t* bytes);
+S2_API int s2_cross_attention(const s2_cross_attention_shape* shape, const void* q, const void* k,
+                              const void* v, void* out, const long* strides,
+                              const int* q_offsets, const int* k_offsets, const int* key_lengths,
+                              const void* key_mask, long mask_stride, void* workspace,
+                              size_t workspace_bytes, s2_stream_t stream);
+
 /* ---- DecomposedConv3D (VAE) ---------------------------------------------- */
 /* The causal 3-D convolution of the VAE (src/seedvr2/decomposed_conv3d.h:33-88,
  * decomposed_conv3d.cpp:605-755) as one implicit GEMM on the matrix cores:

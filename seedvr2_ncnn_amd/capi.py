@@ -9,6 +9,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import os
+from typing import NamedTuple
 
 _PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_PKG, "lib", "libseedvr2_hip.so")
@@ -49,7 +50,9 @@ EXPORTS = (
     "s2_shared_linear_residual", "s2_group_norm_workspace_bytes", "s2_group_norm",
     "s2_linear_workspace_bytes", "s2_linear", "s2_grouped_linear_workspace_bytes",
     "s2_grouped_linear", "s2_linear_view_workspace_bytes",
-    "s2_grouped_linear_view_workspace_bytes",
+    "s2_grouped_linear_view_workspace_bytes", "s2_mx_quantize", "s2_mx_dequantize",
+    "s2_mx_linear_workspace_bytes", "s2_mx_linear", "s2_mx_weight_linear_workspace_bytes",
+    "s2_mx_weight_linear", "s2_cross_attention_workspace_bytes", "s2_cross_attention",
 )
 
 
@@ -99,6 +102,12 @@ class MhaConfig(ctypes.Structure):
     """s2_mha_config: VAEChunkedMHA's embed_dim, num_heads, qdim and scale."""
     _fields_ = [("embed_dim", ctypes.c_int), ("num_heads", ctypes.c_int), ("qdim", ctypes.c_int),
                 ("scale", ctypes.c_float)]
+
+
+class CrossAttentionShape(ctypes.Structure):
+    """s2_cross_attention_shape."""
+    _fields_ = [(n, ctypes.c_int) for n in ("batch", "lq", "lk", "heads", "kv_heads", "head_dim",
+                                            "dtype", "out_dtype")] + [("scale", ctypes.c_float)]
 
 
 class PlanInfo(ctypes.Structure):
@@ -155,6 +164,17 @@ def lib() -> ctypes.CDLL:
         L.s2_apply_cfg.argtypes = [vp, vp, cl, cf, cf, vp, vp]
         L.s2_euler_step.argtypes = [vp, cl, vp, cl, cf, vp]
         L.s2_denoise_update.argtypes = [vp, vp, ci, ci, ci, cf, cf, cf, vp, cl, vp]
+        L.s2_mx_quantize.argtypes = [vp, ci, cl, ci, ci, vp, cl, vp, cl, vp]
+        L.s2_mx_dequantize.argtypes = [vp, cl, vp, cl, ci, ci, vp, ci, cl, vp]
+        L.s2_mx_linear_workspace_bytes.argtypes = [ci, ci, ci, ci, P(sz)]
+        L.s2_mx_linear.argtypes = [vp, cl, vp, cl, ci, vp, vp, cl, vp, ci, ci, ci, vp, cl, vp, ci, cl,
+                                   vp, sz, vp]
+        L.s2_mx_weight_linear_workspace_bytes.argtypes = [ci, ci, ci, ci, ci, P(sz)]
+        L.s2_mx_weight_linear.argtypes = [vp, ci, cl, ci, vp, vp, cl, vp, ci, ci, ci, vp, cl, vp, ci,
+                                          cl, vp, sz, vp]
+        A3 = P(CrossAttentionShape)
+        L.s2_cross_attention_workspace_bytes.argtypes = [A3, ci, P(sz)]
+        L.s2_cross_attention.argtypes = [A3, vp, vp, vp, vp, vp, vp, vp, vp, vp, cl, vp, sz, vp]
         C3 = P(Conv3dConfig)
         L.s2_conv3d_output_shape.argtypes = [C3, ci, ci, ci, ci, P(ci)]
         L.s2_conv3d_packed_weight_bytes.argtypes = [C3, P(sz)]
@@ -899,6 +919,235 @@ def grouped_linear(x, offsets, weight, bias=None, activation=ACT_NONE, residual=
                                   wp, _dtype_code(weight), bi, n, k, activation,
                                   _ptr(residual), rs, out.data_ptr(), yd, os_, ws, size, handle),
           "s2_grouped_linear")
+    return out
+
+
+# ---- MXFP4 ---------------------------------------------------------------------
+
+class MxRows(NamedTuple):
+    """Rows of k values in MXFP4 (include/seedvr2_hip.h): codes uint8 [rows, 16 blocks]
+    and scales uint8 [rows, blocks] with blocks = ceil(k / 32), elements contiguous."""
+    codes: "torch.Tensor"
+    scales: "torch.Tensor"
+    k: int
+
+
+def _mx_rows(rows, name):
+    """Checks MxRows; returns (row count, codes' and scales' row strides)."""
+    import torch
+    codes, scales, k = rows
+    blocks = (k + 31) // 32
+    if k < 1 or k > _INT_MAX:
+        _refuse(name, "k is out of range")
+    if (codes.dtype is not torch.uint8 or scales.dtype is not torch.uint8 or codes.dim() != 2 or
+            scales.dim() != 2 or codes.shape[1] != 16 * blocks or scales.shape[1] != blocks or
+            codes.shape[0] != scales.shape[0]):
+        raise ValueError(f"{name}: codes must be uint8 [rows, {16 * blocks}], scales [rows, {blocks}]")
+    cs, step = codes.stride()
+    ss, sstep = scales.stride()
+    if step != 1 or (blocks > 1 and sstep != 1):
+        raise ValueError(f"{name}: codes and scales must have contiguous rows")
+    if codes.shape[0] > _INT_MAX:
+        _refuse(name, "a size is out of range")
+    return codes.shape[0], cs, ss
+
+
+def _mx_empty(m, k, x, stream):
+    """Uninitialised MxRows whose scale rows are a multiple of 16 bytes apart."""
+    import torch
+    blocks = (k + 31) // 32
+    scales = _empty((m, (blocks + 15) // 16 * 16), torch.uint8, x, stream)
+    return MxRows(_empty((m, 16 * blocks), torch.uint8, x, stream), scales[:, :blocks], k)
+
+
+def mx_quantize(x, out=None, stream=None):
+    """s2_mx_quantize: rows x [m, k] (strided, elements contiguous) as MxRows, into out if
+    given."""
+    if x.dim() != 2 or (x.shape[1] > 1 and x.stride(1) != 1):
+        raise ValueError("x must be [m, k] with contiguous rows")
+    m, k = x.shape
+    if m > _INT_MAX or k > _INT_MAX:
+        _refuse("mx_quantize", "a size is out of range")
+    xd = _dtype_code(x)
+    if out is None:
+        out = _mx_empty(m, k, x, stream)
+    elif out.k != k or out.codes.shape[0] != m:
+        raise ValueError("x and out must be of one shape")
+    _, cs, ss = _mx_rows(out, "mx_quantize")
+    handle = _raw_stream(x, stream, out.codes, out.scales)
+    check(lib().s2_mx_quantize(x.data_ptr(), xd, x.stride(0), m, k, out.codes.data_ptr(), cs,
+                               out.scales.data_ptr(), ss, handle), "s2_mx_quantize")
+    return out
+
+
+def mx_dequantize(rows, dtype=None, out=None, stream=None):
+    """s2_mx_dequantize: the values [m, k] of MxRows in dtype (bf16 if None), into out if
+    given."""
+    import torch
+    m, cs, ss = _mx_rows(rows, "mx_dequantize")
+    k = rows.k
+    if out is None:
+        out = _empty((m, k), dtype or torch.bfloat16, rows.codes, stream)
+    elif out.shape != (m, k) or (k > 1 and out.stride(1) != 1):
+        raise ValueError(f"out must be [{m}, {k}] with contiguous rows")
+    handle = _raw_stream(rows.codes, stream, rows.scales, out)
+    check(lib().s2_mx_dequantize(rows.codes.data_ptr(), cs, rows.scales.data_ptr(), ss, m, k,
+                                 out.data_ptr(), _dtype_code(out), out.stride(0), handle),
+          "s2_mx_dequantize")
+    return out
+
+
+@functools.lru_cache(maxsize=4096)
+def mx_linear_workspace(m, n, k, x_dtype=None, y_dtype=DTYPE_BF16) -> int:
+    """s2_mx_linear_workspace_bytes (x_dtype None: x in MXFP4) or
+    s2_mx_weight_linear_workspace_bytes."""
+    _c_ints("mx_linear_workspace", m, n, k, x_dtype or 0, y_dtype)
+    b = ctypes.c_size_t()
+    if x_dtype is None:
+        check(lib().s2_mx_linear_workspace_bytes(m, n, k, y_dtype, ctypes.byref(b)),
+              "s2_mx_linear_workspace_bytes")
+    else:
+        check(lib().s2_mx_weight_linear_workspace_bytes(m, n, k, x_dtype, y_dtype, ctypes.byref(b)),
+              "s2_mx_weight_linear_workspace_bytes")
+    return b.value
+
+
+def mx_linear(x, weight, bias=None, activation=ACT_NONE, residual=None, out=None, out_dtype=None,
+              workspace=None, stream=None):
+    """s2_mx_linear, or s2_mx_weight_linear where x is a tensor [m, k]: residual + act(x W^T +
+    bias) with weight MxRows of n rows (contiguous codes) and x MxRows or strided rows in
+    fp32, bf16 or fp16.  out_dtype: x's, or bf16 for MxRows, if None.  out may be the
+    residual.  workspace: mx_linear_workspace(...) bytes, made here if None.  Returns
+    out [m, n]."""
+    import torch
+    n, wcs, wss = _mx_rows(weight, "weight")
+    k = weight.k
+    if wcs != weight.codes.shape[1] and n > 1:
+        raise ValueError("the weight's codes must be contiguous")
+    mx = isinstance(x, MxRows)
+    near = x.codes if mx else x
+    if mx:
+        m, xcs, xss = _mx_rows(x, "x")
+        if x.k != k:
+            raise ValueError(f"x must have rows of {k}")
+    else:
+        if x.dim() != 2 or x.shape[1] != k or (k > 1 and x.stride(1) != 1):
+            raise ValueError(f"x must be [m, {k}] with contiguous rows")
+        m = x.shape[0]
+        if m > _INT_MAX:
+            _refuse("mx_linear", "a size is out of range")
+        xd = _dtype_code(x)
+    if activation not in _ROW_ACTIVATIONS:
+        _refuse("mx_linear", "unknown activation")
+    if out is None:
+        out = _empty((m, n), out_dtype or (torch.bfloat16 if mx else x.dtype), near, stream)
+    elif out.shape != (m, n) or (n > 1 and out.stride(1) != 1):
+        raise ValueError(f"out must be [{m}, {n}] with contiguous rows")
+    rs = 0
+    if residual is not None:
+        if residual.shape != (m, n) or residual.dtype is not out.dtype or (
+                n > 1 and residual.stride(1) != 1):
+            raise ValueError(f"residual must be [{m}, {n}] of out's type with contiguous rows")
+        rs = residual.stride(0)
+    yd = _dtype_code(out)
+    bi = None if bias is None else _vector(bias, n, "bias")
+    handle = _raw_stream(near, stream, x.scales if mx else None, weight.codes, weight.scales, bias, residual,
+                         out, workspace)
+    workspace, ws, size = _workspace(workspace, stream, near,
+                                     mx_linear_workspace(m, n, k, None if mx else xd, yd))
+    tail = (weight.codes.data_ptr(), weight.scales.data_ptr(), wss, bi, n, k, activation, _ptr(residual),
+            rs, out.data_ptr(), yd, out.stride(0), ws, size, handle)
+    if mx:
+        check(lib().s2_mx_linear(x.codes.data_ptr(), xcs, x.scales.data_ptr(), xss, m, *tail), "s2_mx_linear")
+    else:
+        check(lib().s2_mx_weight_linear(x.data_ptr(), xd, x.stride(0), m, *tail), "s2_mx_weight_linear")
+    return out
+
+
+# ---- cross attention -------------------------------------------------------------
+
+@functools.lru_cache(maxsize=4096)
+def cross_attention_workspace(batch, lq, lk, heads, kv_heads, head_dim, dtype=DTYPE_BF16,
+                              ragged=False) -> int:
+    """s2_cross_attention_workspace_bytes; lq and lk are those of all samples if ragged."""
+    _c_ints("cross_attention_workspace", batch, lq, lk, heads, kv_heads, head_dim, dtype)
+    shape = CrossAttentionShape(batch, lq, lk, heads, kv_heads, head_dim, dtype, dtype, 1.0)
+    b = ctypes.c_size_t()
+    check(lib().s2_cross_attention_workspace_bytes(ctypes.byref(shape), int(ragged), ctypes.byref(b)),
+          "s2_cross_attention_workspace_bytes")
+    return b.value
+
+
+_Strides = ctypes.c_long * 12
+
+
+def cross_attention(q, k, v, scale=None, q_offsets=None, k_offsets=None, key_lengths=None, key_mask=None,
+                    out=None, out_dtype=None, workspace=None, stream=None):
+    """s2_cross_attention: softmax(scale q k^T) v per sample and head.
+
+    q [batch, lq, heads, d], k and v [batch, lk, kv_heads, d], with key_lengths (int32
+    [batch]) where samples have fewer keys; or, with q_offsets and k_offsets (int32
+    [batch + 1] on the device), q [rows, heads, d], k and v [key rows, kv_heads, d].
+    Any strides of multiples of 16 bytes but contiguous d.  key_mask: bool or uint8
+    [batch, lk], or [key rows] with offsets, false for keys to leave out.  scale: d^-0.5
+    if None.  out may be q; rows in no sample are left as they are in out (undefined
+    in one that this call makes).  workspace: cross_attention_workspace(...) bytes, made
+    here if None.  Returns out, of q's shape."""
+    import torch
+    ragged = q_offsets is not None
+    dims = 3 if ragged else 4
+    if q.dim() != dims or k.dim() != dims or k.shape != v.shape or q.shape[-1] != k.shape[-1]:
+        raise ValueError("q must be [batch, lq, heads, d], k and v [batch, lk, kv_heads, d], or without "
+                         "batch and with offsets")
+    if q.dtype is not k.dtype or q.dtype is not v.dtype:
+        raise ValueError("q, k and v must be of one type")
+    lq, heads, d = q.shape[-3:]
+    lk, kv_heads = k.shape[-3:-1]
+    lead = () if ragged else (q.shape[0],)
+    if ragged:
+        batch = q_offsets.numel() - 1
+        for t in (q_offsets, k_offsets):
+            if t is None or t.dtype is not torch.int32 or t.numel() != batch + 1 or t.dim() != 1 or (
+                    not t.is_contiguous()) or batch < 0:
+                raise ValueError("q_offsets and k_offsets must be batch + 1 contiguous int32 values each")
+    else:
+        batch = q.shape[0]
+        if k_offsets is not None:
+            raise ValueError("k_offsets need q_offsets")
+        if k.shape[0] != batch:
+            raise ValueError("q, k and v must have one batch")
+    if key_lengths is not None and (ragged or key_lengths.dtype is not torch.int32 or
+                                    key_lengths.numel() != batch or not key_lengths.is_contiguous()):
+        raise ValueError(f"key_lengths must be {batch} contiguous int32 values, without offsets")
+    ms = 0
+    if key_mask is not None:
+        if key_mask.dtype not in (torch.bool, torch.uint8) or key_mask.shape != lead + (lk,) or (
+                lk > 1 and key_mask.stride(-1) != 1):
+            raise ValueError(f"key_mask must be bool or uint8 {list(lead + (lk,))} with contiguous rows")
+        ms = 0 if ragged else key_mask.stride(0)
+    if out is None:
+        out = _empty(q.shape, out_dtype or q.dtype, q, stream)
+    elif out.shape != q.shape:
+        raise ValueError("out must be of q's shape")
+    strides = []
+    for t in (q, k, v, out):
+        s = t.stride()
+        if d > 1 and s[-1] != 1:
+            raise ValueError("head elements must be contiguous")
+        strides += s[:3] if not ragged else (0,) + s[:2]
+    for n in (batch, lq, lk, heads, kv_heads, d):
+        if n > _INT_MAX:
+            _refuse("cross_attention", "a size is out of range")
+    dt = _dtype_code(q)
+    shape = CrossAttentionShape(batch, lq, lk, heads, kv_heads, d, dt, _dtype_code(out),
+                                d ** -0.5 if scale is None else scale)
+    handle = _raw_stream(q, stream, k, v, out, q_offsets, k_offsets, key_lengths, key_mask, workspace)
+    workspace, ws, size = _workspace(workspace, stream, q, cross_attention_workspace(
+        batch, lq, lk, heads, kv_heads, d, dt, ragged))
+    check(lib().s2_cross_attention(ctypes.byref(shape), q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                                   out.data_ptr(), _Strides(*strides), _ptr(q_offsets), _ptr(k_offsets),
+                                   _ptr(key_lengths), _ptr(key_mask), ms, ws, size, handle),
+          "s2_cross_attention")
     return out
 
 

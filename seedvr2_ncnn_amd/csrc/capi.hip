@@ -11,10 +11,12 @@
 #include "awa_plan.h"
 #include "block_kernels.h"
 #include "conv3d_kernels.h"
+#include "cross_attention_kernels.h"
 #include "graph_ops_kernels.h"
 #include "group_norm_kernels.h"
 #include "matmul_kernels.h"
 #include "mha_kernels.h"
+#include "mx_kernels.h"
 #include "pipeline_kernels.h"
 #include "seedvr2_hip.h"
 #include "stream_scratch.h"
@@ -1425,6 +1427,254 @@ int s2_grouped_linear(const void* x, s2_dtype x_dtype, long x_stride, int m, con
     if (workspace && !aligned(workspace, 16))
         return fail(S2_ERR_INVALID, "workspace must be 16-byte aligned");
     S2_HIP(s2::launch_matmul(a, workspace, workspace ? workspace_bytes : 0, (hipStream_t)stream));
+    return S2_OK;
+}
+
+/* ---- MXFP4 ---------------------------------------------------------------- */
+
+static const int kMxMost = 1 << 30;
+
+// Checks codes and scales of a [rows][k] operand.
+static int mx_rows_ok(const void* codes, long code_stride, const void* scales, long scale_stride,
+                      int rows, int k) {
+    if (!codes || !scales) return fail(S2_ERR_INVALID, "null operand");
+    if (!aligned(codes, 16) || code_stride % 16 != 0)
+        return fail(S2_ERR_INVALID, "codes must start at multiples of 16 bytes");
+    if (rows > 1 && (code_stride < 16L * s2::mx_blocks(k) || scale_stride < s2::mx_blocks(k)))
+        return fail(S2_ERR_INVALID, "row strides shorter than rows");
+    return S2_OK;
+}
+
+static bool mx_shape_ok(int m, int k) { return m >= 0 && k > 0 && m <= kMxMost && k <= kMxMost; }
+
+int s2_mx_quantize(const void* x, s2_dtype x_dtype, long x_stride, int m, int k, void* codes,
+                   long code_stride, void* scales, long scale_stride, s2_stream_t stream) {
+    if (!mx_shape_ok(m, k)) return fail(S2_ERR_INVALID, "invalid mx shape");
+    if (!dtype_ok(x_dtype)) return fail(S2_ERR_INVALID, "unsupported dtype");
+    if (m == 0) return S2_OK;
+    if (!x || !aligned(x, dtype_bytes(x_dtype)))
+        return fail(S2_ERR_INVALID, "null operand, or one not aligned to its elements");
+    if (m > 1 && x_stride < 0) return fail(S2_ERR_INVALID, "negative stride");
+    const int ret = mx_rows_ok(codes, code_stride, scales, scale_stride, m, k);
+    if (ret != S2_OK) return ret;
+    if (codes == x || scales == x || codes == scales) return fail(S2_ERR_INVALID, "operands overlap");
+    S2_HIP(s2::launch_mx_quantize(x, (int)x_dtype, x_stride, m, k, (uint8_t*)codes, code_stride,
+                                  (uint8_t*)scales, scale_stride, (hipStream_t)stream));
+    return S2_OK;
+}
+
+int s2_mx_dequantize(const void* codes, long code_stride, const void* scales, long scale_stride,
+                     int m, int k, void* y, s2_dtype y_dtype, long y_stride, s2_stream_t stream) {
+    if (!mx_shape_ok(m, k)) return fail(S2_ERR_INVALID, "invalid mx shape");
+    if (!dtype_ok(y_dtype)) return fail(S2_ERR_INVALID, "unsupported dtype");
+    if (m == 0) return S2_OK;
+    const int ret = mx_rows_ok(codes, code_stride, scales, scale_stride, m, k);
+    if (ret != S2_OK) return ret;
+    if (!y || !aligned(y, dtype_bytes(y_dtype)))
+        return fail(S2_ERR_INVALID, "null operand, or one not aligned to its elements");
+    if (m > 1 && y_stride < k) return fail(S2_ERR_INVALID, "row strides shorter than rows");
+    if (codes == y || scales == y) return fail(S2_ERR_INVALID, "operands overlap");
+    S2_HIP(s2::launch_mx_dequantize(
+        s2::MxRows{(const uint8_t*)codes, code_stride, (const uint8_t*)scales, scale_stride}, m, k, y,
+        (int)y_dtype, y_stride, (hipStream_t)stream));
+    return S2_OK;
+}
+
+static int mx_linear_workspace_bytes(bool mx, int m, int n, int k, s2_dtype x_dtype, s2_dtype y_dtype,
+                                     size_t* bytes) {
+    if (!bytes) return fail(S2_ERR_INVALID, "null bytes");
+    if (!mx_shape_ok(m, k) || n <= 0 || n > kMxMost) return fail(S2_ERR_INVALID, "invalid linear shape");
+    if (!dtype_ok(x_dtype) || !dtype_ok(y_dtype)) return fail(S2_ERR_INVALID, "unsupported dtype");
+    s2::MxLinearArgs a{};
+    a.mx = mx;
+    a.x_kind = (int)x_dtype;
+    a.m = m;
+    a.n = n;
+    a.k = k;
+    a.y_kind = (int)y_dtype;
+    *bytes = m ? s2::mx_linear_workspace(a) : 0;
+    return S2_OK;
+}
+
+int s2_mx_linear_workspace_bytes(int m, int n, int k, s2_dtype y_dtype, size_t* bytes) {
+    return mx_linear_workspace_bytes(true, m, n, k, S2_DTYPE_BF16, y_dtype, bytes);
+}
+
+int s2_mx_weight_linear_workspace_bytes(int m, int n, int k, s2_dtype x_dtype, s2_dtype y_dtype,
+                                        size_t* bytes) {
+    return mx_linear_workspace_bytes(false, m, n, k, x_dtype, y_dtype, bytes);
+}
+
+// The checks that both forms share, and the call.
+static int mx_linear_call(const s2::MxLinearArgs& a, void* workspace, size_t workspace_bytes,
+                          s2_stream_t stream) {
+    if (!dtype_ok((s2_dtype)a.y_kind)) return fail(S2_ERR_INVALID, "unsupported dtype");
+    if (!row_activation(a.act)) return fail(S2_ERR_INVALID, "unknown activation");
+    if (a.m == 0) return S2_OK;
+    const int ret = mx_rows_ok(a.w.codes, a.w.code_stride, a.w.scales, a.w.scale_stride, a.n, a.k);
+    if (ret != S2_OK) return ret;
+    if (!a.y) return fail(S2_ERR_INVALID, "null operand");
+    if (a.m > 1 && (a.y_stride < a.n || (a.res && a.res_stride < a.n)))
+        return fail(S2_ERR_INVALID, "row strides shorter than rows");
+    const size_t ye = dtype_bytes((s2_dtype)a.y_kind);
+    if (!aligned(a.y, ye) || !aligned(a.res, ye) || !aligned(a.bias, 4))
+        return fail(S2_ERR_INVALID, "operands must be aligned to their elements");
+    if (a.res == a.y && a.m > 1 && a.res_stride != a.y_stride)
+        return fail(S2_ERR_INVALID, "in place needs one row stride");
+    if (a.y == a.x || a.y == a.xq.codes || a.y == a.xq.scales || a.y == a.w.codes || a.y == a.w.scales)
+        return fail(S2_ERR_INVALID, "y overlaps x or the weight");
+    if (workspace && !aligned(workspace, 16))
+        return fail(S2_ERR_INVALID, "workspace must be 16-byte aligned");
+    S2_HIP(s2::launch_mx_linear(a, workspace, workspace ? workspace_bytes : 0, (hipStream_t)stream));
+    return S2_OK;
+}
+
+int s2_mx_linear(const void* x_codes, long x_code_stride, const void* x_scales, long x_scale_stride,
+                 int m, const void* w_codes, const void* w_scales, long w_scale_stride,
+                 const float* bias, int n, int k, int activation, const void* residual,
+                 long residual_stride, void* y, s2_dtype y_dtype, long y_stride, void* workspace,
+                 size_t workspace_bytes, s2_stream_t stream) {
+    if (!mx_shape_ok(m, k) || n <= 0 || n > kMxMost) return fail(S2_ERR_INVALID, "invalid linear shape");
+    if (m > 0) {
+        const int ret = mx_rows_ok(x_codes, x_code_stride, x_scales, x_scale_stride, m, k);
+        if (ret != S2_OK) return ret;
+    }
+    const s2::MxLinearArgs a{true,
+                             {(const uint8_t*)x_codes, x_code_stride, (const uint8_t*)x_scales, x_scale_stride},
+                             nullptr, S2_DTYPE_BF16, 0, m,
+                             {(const uint8_t*)w_codes, 16L * s2::mx_blocks(k), (const uint8_t*)w_scales,
+                              w_scale_stride},
+                             bias, n, k, activation, residual, residual_stride, y, (int)y_dtype, y_stride};
+    return mx_linear_call(a, workspace, workspace_bytes, stream);
+}
+
+int s2_mx_weight_linear(const void* x, s2_dtype x_dtype, long x_stride, int m, const void* w_codes,
+                        const void* w_scales, long w_scale_stride, const float* bias, int n, int k,
+                        int activation, const void* residual, long residual_stride, void* y,
+                        s2_dtype y_dtype, long y_stride, void* workspace, size_t workspace_bytes,
+                        s2_stream_t stream) {
+    if (!mx_shape_ok(m, k) || n <= 0 || n > kMxMost) return fail(S2_ERR_INVALID, "invalid linear shape");
+    if (!dtype_ok(x_dtype)) return fail(S2_ERR_INVALID, "unsupported dtype");
+    if (m > 0 && (!x || !aligned(x, dtype_bytes(x_dtype))))
+        return fail(S2_ERR_INVALID, "null operand, or one not aligned to its elements");
+    if (m > 1 && x_stride < k) return fail(S2_ERR_INVALID, "row strides shorter than rows");
+    const s2::MxLinearArgs a{false, {nullptr, 0, nullptr, 0}, x, (int)x_dtype, x_stride, m,
+                             {(const uint8_t*)w_codes, 16L * s2::mx_blocks(k), (const uint8_t*)w_scales,
+                              w_scale_stride},
+                             bias, n, k, activation, residual, residual_stride, y, (int)y_dtype, y_stride};
+    return mx_linear_call(a, workspace, workspace_bytes, stream);
+}
+
+/* ---- cross attention ------------------------------------------------------- */
+
+static int cross_shape_ok(const s2_cross_attention_shape* s) {
+    if (!s) return fail(S2_ERR_INVALID, "null shape");
+    const int most = 1 << 30;
+    if (s->batch < 0 || s->lq < 0 || s->lk < 0 || s->batch > most || s->lq > most || s->lk > most)
+        return fail(S2_ERR_INVALID, "invalid batch or lengths");
+    if (s->heads <= 0 || s->kv_heads <= 0 || s->heads % s->kv_heads != 0 || s->heads > 65535)
+        return fail(S2_ERR_INVALID, "heads must be a multiple of kv_heads, at most 65535");
+    if (s->head_dim <= 0 || s->head_dim % 8 != 0 || s->head_dim > 256)
+        return fail(S2_ERR_INVALID, "head_dim must be a multiple of 8, at most 256");
+    if (!dtype_ok(s->dtype) || !dtype_ok(s->out_dtype)) return fail(S2_ERR_INVALID, "unsupported dtype");
+    if (!(s->scale - s->scale == 0.f)) return fail(S2_ERR_INVALID, "scale must be finite");
+    return S2_OK;
+}
+
+static s2::CrossArgs cross_args(const s2_cross_attention_shape* s) {
+    s2::CrossArgs a{};
+    a.kind = (int)s->dtype;
+    a.out_kind = (int)s->out_dtype;
+    a.batch = s->batch;
+    a.lq = s->lq;
+    a.lk = s->lk;
+    a.heads = s->heads;
+    a.kv_heads = s->kv_heads;
+    a.d = s->head_dim;
+    a.scale = s->scale;
+    return a;
+}
+
+static const int no_offsets = 0;   // stand for a call's own, which the plan does not read
+
+int s2_cross_attention_workspace_bytes(const s2_cross_attention_shape* shape, int ragged, size_t* bytes) {
+    if (!bytes) return fail(S2_ERR_INVALID, "null bytes");
+    const int ret = cross_shape_ok(shape);
+    if (ret != S2_OK) return ret;
+    s2::CrossArgs a = cross_args(shape);
+    if (ragged) a.q_offsets = a.k_offsets = &no_offsets;
+    *bytes = shape->batch && shape->lq ? s2::cross_attention_workspace(a) : 0;
+    return S2_OK;
+}
+
+int s2_cross_attention(const s2_cross_attention_shape* shape, const void* q, const void* k,
+                       const void* v, void* out, const long* strides, const int* q_offsets,
+                       const int* k_offsets, const int* key_lengths, const void* key_mask,
+                       long mask_stride, void* workspace, size_t workspace_bytes,
+                       s2_stream_t stream) {
+    const int ret = cross_shape_ok(shape);
+    if (ret != S2_OK) return ret;
+    if (!q_offsets != !k_offsets || (q_offsets && key_lengths))
+        return fail(S2_ERR_INVALID, "offsets of both queries and keys, without key lengths, or of neither");
+    if (shape->batch == 0 || shape->lq == 0) return S2_OK;
+    if (!q || !out || !strides || (shape->lk > 0 && (!k || !v)))
+        return fail(S2_ERR_INVALID, "null operand");
+    s2::CrossArgs a = cross_args(shape);
+    a.q = q;
+    a.k = k;
+    a.v = v;
+    a.out = out;
+    a.q_offsets = q_offsets;
+    a.k_offsets = k_offsets;
+    a.key_lengths = key_lengths;
+    a.key_mask = (const uint8_t*)key_mask;
+    a.mask_batch = q_offsets ? 0 : mask_stride;
+    s2::CrossRows* rows[4] = {&a.qs, &a.ks, &a.vs, &a.os};
+    const long most = 1L << 40;   // sums of strides times sizes stay in 64 bits
+    for (int i = 0; i < 4; ++i) {
+        *rows[i] = s2::CrossRows{strides[3 * i], strides[3 * i + 1], strides[3 * i + 2]};
+        s2::CrossRows& r = *rows[i];
+        const int len = i == 1 || i == 2 ? shape->lk : shape->lq;
+        const int heads = i == 1 || i == 2 ? shape->kv_heads : shape->heads;
+        if (q_offsets || shape->batch == 1) r.batch = 0;   // what strides of one say is nothing
+        if (len <= 1) r.row = 0;
+        if (heads == 1) r.head = 0;
+        if (r.batch < 0 || r.row < 0 || r.head < 0 || r.batch > most || r.row > most || r.head > most)
+            return fail(S2_ERR_INVALID, "strides negative or too large");
+    }
+    const size_t e = dtype_bytes(shape->dtype), oe = dtype_bytes(shape->out_dtype);
+    for (int i = 0; i < 3; ++i) {
+        const s2::CrossRows& r = *rows[i];
+        if (r.batch * e % 16 || r.row * e % 16 || r.head * e % 16)
+            return fail(S2_ERR_INVALID, "strides of q, k and v must be multiples of 16 bytes");
+    }
+    if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(out, oe) ||
+        !aligned(q_offsets, 4) || !aligned(k_offsets, 4) || !aligned(key_lengths, 4))
+        return fail(S2_ERR_INVALID, "q, k and v must be 16-byte aligned, the rest to its elements");
+    // rows of out are apart: of its three strides each covers what the smaller ones span
+    {
+        typedef __int128 wide;
+        long size[3] = {q_offsets ? 1 : shape->batch, shape->lq, shape->heads};
+        long step[3] = {a.os.batch, a.os.row, a.os.head};
+        for (int i = 0; i < 2; ++i)
+            for (int j = 0; j < 2; ++j)
+                if (step[j] > step[j + 1]) std::swap(step[j], step[j + 1]), std::swap(size[j], size[j + 1]);
+        wide span = shape->head_dim;
+        for (int i = 0; i < 3; ++i) {
+            if (size[i] <= 1) continue;
+            if (step[i] < span) return fail(S2_ERR_INVALID, "rows of out overlap");
+            span += (wide)(size[i] - 1) * step[i];
+        }
+    }
+    if (key_mask && !q_offsets && shape->batch > 1 && mask_stride < shape->lk)
+        return fail(S2_ERR_INVALID, "mask_stride shorter than the keys");
+    if (out == q && (shape->dtype != shape->out_dtype || a.qs.batch != a.os.batch ||
+                     a.qs.row != a.os.row || a.qs.head != a.os.head))
+        return fail(S2_ERR_INVALID, "in place needs one type and one set of strides");
+    if (out == k || out == v) return fail(S2_ERR_INVALID, "out overlaps k or v");
+    if (workspace && !aligned(workspace, 16))
+        return fail(S2_ERR_INVALID, "workspace must be 16-byte aligned");
+    S2_HIP(s2::launch_cross_attention(a, workspace, workspace ? workspace_bytes : 0, (hipStream_t)stream));
     return S2_OK;
 }
 

@@ -1,0 +1,39 @@
+// Cross attention's launchers.  Element kinds are the s2_dtype codes, strides are in
+// elements.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+namespace s2 {
+
+// Rows [.. heads][d] of an operand: sample b's row i of head h begins at b * batch + i *
+// row + h * head.  With offsets, row offsets[b] + i of the whole operand and batch 0.
+struct CrossRows {
+    long batch, row, head;
+};
+
+struct CrossArgs {
+    const void* q;
+    const void* k;
+    const void* v;
+    void* out;
+    int kind, out_kind;
+    CrossRows qs, ks, vs, os;
+    int batch;
+    int lq, lk;               // rows of a sample; with offsets of all samples
+    const int* q_offsets;     // device [batch + 1], both or none
+    const int* k_offsets;
+    const int* key_lengths;   // device [batch] or null
+    const uint8_t* key_mask;  // device [batch][lk] (offsets: [lk]), zero for keys left out, or null
+    long mask_batch;
+    int heads, kv_heads, d;
+    float scale;
+};
+
+size_t cross_attention_workspace(const CrossArgs& a);
+hipError_t launch_cross_attention(const CrossArgs& a, void* workspace, size_t workspace_bytes,
+                                  hipStream_t stream);
+
+}  // namespace s2

@@ -1,0 +1,52 @@
+// The MXFP4 operators' launchers: quantisation of rows and products with weights in
+// MXFP4.  A row of k values is blocks of 32, the last one padded: 16 bytes of e2m1 codes
+// a block (two a byte, the first in the low half) and one e8m0 scale, 2^(byte - 127).
+// Element kinds are the s2_dtype codes; strides are in elements, of codes and scales in
+// bytes.
+//
+//   mx_quantize_kernels.hip  rows to MXFP4 and back
+//   mx_linear_kernels.hip    which kernel takes a product; few rows
+#pragma once
+
+#include "matmul_kernels.h"
+
+namespace s2 {
+
+__host__ __device__ inline int mx_blocks(int k) { return (k + 31) / 32; }
+
+struct MxRows {
+    const uint8_t* codes;    // 16-byte rows
+    long code_stride;
+    const uint8_t* scales;
+    long scale_stride;
+};
+
+// y = residual + act(x W^T + bias): x in MXFP4 (`mx`) or as x_kind says.
+struct MxLinearArgs {
+    bool mx;
+    MxRows xq;
+    const void* x;
+    int x_kind;
+    long x_stride;
+    int m;
+    MxRows w;                // code_stride 16 mx_blocks(k)
+    const float* bias;
+    int n, k;
+    int act;
+    const void* res;
+    long res_stride;
+    void* y;
+    int y_kind;
+    long y_stride;
+};
+
+hipError_t launch_mx_quantize(const void* x, int x_kind, long x_stride, int m, int k, uint8_t* codes,
+                              long code_stride, uint8_t* scales, long scale_stride, hipStream_t stream);
+hipError_t launch_mx_dequantize(const MxRows& rows, int m, int k, void* y, int y_kind, long y_stride,
+                                hipStream_t stream);
+
+size_t mx_linear_workspace(const MxLinearArgs& a);
+hipError_t launch_mx_linear(const MxLinearArgs& a, void* workspace, size_t workspace_bytes,
+                            hipStream_t stream);
+
+}  // namespace s2

@@ -1,0 +1,306 @@
+"""Cross attention against float64."""
+import pytest
+import torch
+
+import mx_cross as mc
+import row_operators as ro
+from seedvr2_ncnn_amd import capi
+
+pytestmark = pytest.mark.gpu
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def _normal(gen, *shape):
+    return torch.randn(*shape, generator=gen, device="cuda")
+
+
+def _sample(q, k, v, scale, kept, out_dtype):
+    """All heads of one sample: (result, bound) [queries, heads, d]."""
+    each = q.shape[1] // k.shape[1]
+    pairs = [mc.attention(q[:, h], k[:, h // each], v[:, h // each], scale, kept, out_dtype)
+             for h in range(q.shape[1])]
+    return torch.stack([p[0] for p in pairs], 1), torch.stack([p[1] for p in pairs], 1)
+
+
+def _padded(batch, lq, lk, heads, kv_heads, d, dtype, lengths=None, mask=None, out_dtype=None, scale=None,
+            seed=0, poison=False, order="bshd", **kwargs):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+
+    def operand(n, h):
+        t = _normal(gen, batch, n, h, d).to(dtype)
+        if order == "bhsd":
+            return t.transpose(1, 2).contiguous().transpose(1, 2)
+        if order == "sbhd":
+            return t.transpose(0, 1).contiguous().transpose(0, 1)
+        return t
+
+    q, k, v = operand(lq, heads), operand(lk, kv_heads), operand(lk, kv_heads)
+    kept = torch.ones(batch, lk, dtype=torch.bool, device="cuda")
+    if lengths is not None:
+        kept &= torch.arange(lk, device="cuda") < torch.tensor(lengths, device="cuda")[:, None]
+        lengths = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    if mask is not None:
+        kept &= mask
+    if poison:
+        k[~kept], v[~kept] = float("nan"), float("inf")
+    got = capi.cross_attention(q, k, v, scale=scale, key_lengths=lengths, key_mask=mask, out_dtype=out_dtype,
+                               **kwargs)
+    assert got.dtype == (out_dtype or dtype)
+    for b in range(batch):
+        want, bound = _sample(q[b], k[b], v[b], d ** -0.5 if scale is None else scale, kept[b], got.dtype)
+        ro.check(got[b], want, bound)
+        if not kept[b].any():
+            assert (got[b] == 0).all()
+    return q, k, v, got
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("batch,lq,lk,heads,kv_heads,d", [
+    (1, 1, 1, 1, 1, 8), (1, 1, 1000, 4, 4, 128), (2, 3, 5, 2, 1, 64), (1, 33, 31, 3, 3, 40),
+    (2, 129, 77, 4, 2, 128), (1, 257, 300, 2, 2, 64), (1, 64, 33, 8, 8, 72), (3, 100, 512, 5, 1, 96),
+    (1, 130, 65, 2, 2, 256), (1, 70, 200, 2, 1, 136), (1, 500, 1, 2, 2, 64), (5, 1, 333, 20, 4, 128),
+    (2, 7, 1500, 8, 1, 64), (1, 1, 5000, 16, 1, 128), (1, 2, 129, 3, 3, 256), (2, 2000, 16, 2, 2, 24),
+    (1, 17, 2049, 1, 1, 120)])
+def test_lengths(dtype, batch, lq, lk, heads, kv_heads, d):
+    _padded(batch, lq, lk, heads, kv_heads, d, dtype, seed=lq + lk)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("lq", [1, 5, 40, 300])
+@pytest.mark.parametrize("d", [64, 128])
+def test_key_lengths_and_masks_with_nan_behind_them(dtype, lq, d):
+    lengths = [0, 1, 31, 32, 33, 64, 100, 199]
+    _padded(8, lq, 199, 4, 2, d, dtype, lengths=lengths, poison=True)
+    gen = torch.Generator(device="cuda").manual_seed(7)
+    mask = torch.rand(8, 199, generator=gen, device="cuda") < 0.5
+    mask[2] = False
+    mask[3] = False
+    mask[3, 198] = True
+    mask[4, :150] = False
+    mask[5, 64:] = False
+    mask[6] = torch.arange(199, device="cuda") % 64 == 63
+    _padded(8, lq, 199, 4, 2, d, dtype, mask=mask, poison=True)
+    _padded(8, lq, 199, 4, 4, d, dtype, mask=mask, lengths=lengths[::-1], poison=True)
+    _padded(8, lq, 199, 2, 2, d, dtype, mask=mask[:, :199], lengths=[199] * 8, poison=True)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_long_masked_keys_of_few_queries(dtype):
+    """Ranges of keys that the mask leaves empty."""
+    mask = torch.zeros(3, 4000, dtype=torch.bool, device="cuda")
+    mask[0, 3999] = True
+    mask[1, 17] = True
+    _padded(3, 2, 4000, 4, 1, 128, dtype, mask=mask, poison=True)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_strided_operands(dtype):
+    for order in ("bhsd", "sbhd"):
+        _padded(3, 70, 90, 4, 2, 64, dtype, order=order)
+        _padded(3, 1, 900, 4, 2, 64, dtype, order=order)
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    wide = _normal(gen, 2, 100, 12, 64).to(dtype)   # a fused projection's q, k, v
+    q, k, v = wide[:, :, :4], wide[:, :, 4:8], wide[:, :, 8:]
+    out = torch.full((2, 100, 5, 67), 9.0, dtype=dtype, device="cuda")
+    got = capi.cross_attention(q, k, v, out=out[:, :, :4, 1:65])
+    assert (out[:, :, 4] == 9).all() and (out[..., 0] == 9).all() and (out[..., 65:] == 9).all()
+    for b in range(2):
+        ro.check(got[b], *_sample(q[b], k[b], v[b], 64 ** -0.5, None, dtype))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("lq", [1, 90])
+def test_broadcast_keys(dtype, lq):
+    """One prompt for every sample, one head for all: strides of zero."""
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    q = _normal(gen, 3, lq, 4, 64).to(dtype)
+    k, v = (_normal(gen, 1, 50, 1, 64).to(dtype).expand(3, 50, 4, 64) for _ in range(2))
+    got = capi.cross_attention(q, k, v)
+    for b in range(3):
+        ro.check(got[b], *_sample(q[b], k[b], v[b], 64 ** -0.5, None, dtype))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("out_dtype", TYPES, ids=str)
+def test_out_types_and_scales(dtype, out_dtype):
+    for lq in (2, 150):
+        _padded(1, lq, 100, 2, 2, 64, dtype, out_dtype=out_dtype, scale=0.3)
+        _padded(1, lq, 100, 2, 2, 128, dtype, out_dtype=out_dtype, scale=-0.05)
+        _padded(1, lq, 100, 2, 2, 64, dtype, out_dtype=out_dtype, scale=0.0)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("lq", [1, 200])
+@pytest.mark.parametrize("size", [8.0, 60.0])
+def test_large_scores(dtype, lq, size):
+    """Weights that all but vanish, rising and falling maxima along the keys."""
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    q, k, v = _normal(gen, 1, lq, 2, 64), _normal(gen, 1, 700, 2, 64), _normal(gen, 1, 700, 2, 64)
+    q *= size
+    k[:, :350] *= torch.linspace(0.1, 2.0, 350, device="cuda")[:, None, None]
+    k[:, 350:] *= torch.linspace(2.0, 0.1, 350, device="cuda")[:, None, None]
+    q, k, v = q.to(dtype), k.to(dtype), v.to(dtype)
+    got = capi.cross_attention(q, k, v)
+    want, bound = _sample(q[0], k[0], v[0], 64 ** -0.5, None, dtype)
+    ro.check(got[0], want, bound)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("lq", [3, 140])
+def test_infinite_scores(dtype, lq):
+    """-inf among the scores is a weight of nought; NaN makes its row NaN."""
+    q = torch.zeros(1, lq, 1, 64, dtype=dtype, device="cuda")
+    q[0, 0, 0, 0], q[0, 1, 0, 0], q[0, 2, 0, 1] = 1.0, -1.0, 1.0
+    k = torch.zeros(1, 40, 1, 64, dtype=dtype, device="cuda")
+    k[0, ::2, 0, 0] = -float("inf")
+    v = torch.arange(40, device="cuda").to(dtype)[None, :, None, None].expand(1, 40, 1, 64).contiguous()
+    got = capi.cross_attention(q, k, v)[0, :, 0].float()
+    assert got[1:].isnan().all()   # 0 * inf
+    k = torch.full((1, 40, 1, 64), -float("inf"), dtype=dtype, device="cuda")
+    k[0, 1::2] = 0.0
+    got = capi.cross_attention(torch.ones_like(q), k, v)[0, :, 0].float()
+    # the mean of the odd ones; 20 weights of one and their sum are exact
+    assert (got == 20.0).all()
+
+
+def _ragged(queries, keys, heads, kv_heads, d, dtype, spare=3, mask=None, seed=0, **kwargs):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    nq, nk = sum(queries), sum(keys)
+    q = _normal(gen, nq + spare, heads, d).to(dtype)
+    kv = _normal(gen, nk + spare, 2 * kv_heads, d).to(dtype)
+    k, v = kv[:, :kv_heads], kv[:, kv_heads:]
+    k[nk:] = float("nan")
+    ends = [[0], [0]]
+    for e, sizes in zip(ends, (queries, keys)):
+        for s in sizes:
+            e.append(e[-1] + s)
+    qo, ko = (torch.tensor(e, dtype=torch.int32, device="cuda") for e in ends)
+    out = torch.full((nq + spare, heads, d), 5.0, dtype=dtype, device="cuda")
+    if mask is not None:
+        k[~mask], v[~mask] = float("inf"), float("nan")
+    assert capi.cross_attention(q, k, v, q_offsets=qo, k_offsets=ko, key_mask=mask, out=out, **kwargs) is out
+    assert (out[nq:] == 5).all()
+    for b in range(len(queries)):
+        qs, ks = slice(ends[0][b], ends[0][b + 1]), slice(ends[1][b], ends[1][b + 1])
+        if queries[b]:
+            ro.check(out[qs], *_sample(q[qs], k[ks], v[ks], d ** -0.5, None if mask is None else mask[ks], dtype))
+            if keys[b] == 0:
+                assert (out[qs] == 0).all()
+    return q, k, v, qo, ko, out
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("queries,keys,heads,kv_heads,d", [
+    ([1], [1], 1, 1, 64), ([5, 0, 130, 1], [77, 3, 0, 40], 4, 2, 128), ([300, 20, 7], [10, 200, 33], 2, 2, 64),
+    ([1] * 40, list(range(0, 120, 3)), 8, 2, 128), ([3] * 70, [9] * 70, 2, 1, 40), ([0, 0, 2], [0, 5, 900], 4, 4, 64),
+    ([1, 1, 1, 1], [3000, 10, 0, 900], 5, 1, 128)])
+def test_ragged(dtype, queries, keys, heads, kv_heads, d):
+    _ragged(queries, keys, heads, kv_heads, d, dtype)
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    mask = torch.rand(sum(keys) + 3, generator=gen, device="cuda") < 0.6
+    mask[sum(keys):] = False
+    _ragged(queries, keys, heads, kv_heads, d, dtype, mask=mask)
+
+
+def test_offsets_outside_the_rows_are_taken_as_their_ends():
+    q, k = torch.randn(20, 2, 64, device="cuda"), torch.randn(30, 2, 64, device="cuda")
+    v = torch.randn(30, 2, 64, device="cuda")
+    far = torch.tensor([-5, 10, 2 ** 31 - 1], dtype=torch.int32, device="cuda")
+    near_q = torch.tensor([0, 10, 20], dtype=torch.int32, device="cuda")
+    near_k = torch.tensor([0, 10, 30], dtype=torch.int32, device="cuda")
+    for t in (torch.float32, torch.bfloat16):
+        a = capi.cross_attention(q.to(t), k.to(t), v.to(t), q_offsets=far, k_offsets=far)
+        b = capi.cross_attention(q.to(t), k.to(t), v.to(t), q_offsets=near_q, k_offsets=near_k)
+        assert torch.equal(a, b)
+    lengths = torch.tensor([99, -3], dtype=torch.int32, device="cuda")
+    y = capi.cross_attention(q.view(2, 10, 2, 64), k.view(2, 15, 2, 64), v.view(2, 15, 2, 64), key_lengths=lengths)
+    assert torch.equal(y[:1], capi.cross_attention(q.view(2, 10, 2, 64)[:1], k.view(2, 15, 2, 64)[:1],
+                                                   v.view(2, 15, 2, 64)[:1]))
+    assert (y[1] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_nothing_to_do(dtype):
+    q = torch.randn(2, 3, 4, 64, device="cuda").to(dtype)
+    k = torch.randn(2, 0, 2, 64, device="cuda").to(dtype)
+    assert (capi.cross_attention(q, k, k) == 0).all()
+    k = torch.randn(2, 5, 2, 64, device="cuda").to(dtype)
+    assert capi.cross_attention(q[:, :0], k, k).shape == (2, 0, 4, 64)
+    assert capi.cross_attention(q[:0], k[:0], k[:0]).shape == (0, 3, 4, 64)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("lq", [1, 300])
+def test_in_place_and_without_workspace(dtype, lq):
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    q, k, v = (_normal(gen, 2, n, 4, 64).to(dtype) for n in (lq, 3000, 3000))
+    want = capi.cross_attention(q, k, v)
+    none = torch.empty(0, dtype=torch.uint8, device="cuda")
+    got = capi.cross_attention(q, k, v, workspace=none)
+    for b in range(2):
+        ro.check(got[b], *_sample(q[b], k[b], v[b], 64 ** -0.5, None, dtype))
+    assert capi.cross_attention(q, k, v, out=q) is q
+    assert torch.equal(q, want)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("lq,lk", [(1, 3000), (300, 100)])
+def test_graphs_and_streams(dtype, lq, lk):
+    """Two captured calls with workspaces of their own, replayed between eager work, the
+    lengths changed in between; equal every time."""
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    sets = [tuple(_normal(gen, 2, n, 4, 64).to(dtype) for n in (lq, lk, lk)) for _ in range(2)]
+    lengths = torch.tensor([lk, lk // 2], dtype=torch.int32, device="cuda")
+    other = torch.tensor([7, lk], dtype=torch.int32, device="cuda")
+    first = [capi.cross_attention(*s, key_lengths=lengths) for s in sets]
+    second = [capi.cross_attention(*s, key_lengths=other) for s in sets]
+    held = lengths.clone()
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    outs = [torch.zeros_like(s[0]) for s in sets]
+    graphs = []
+    for s, o in zip(sets, outs):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            capi.cross_attention(*s, key_lengths=held, out=o)
+        graphs.append(g)
+    for turn in range(4):
+        held.copy_(other if turn % 2 else lengths)
+        for g, o, w in zip(graphs, outs, second if turn % 2 else first):
+            o.zero_()
+            g.replay()
+            assert torch.equal(capi.cross_attention(*sets[0], key_lengths=lengths), first[0])
+            torch.cuda.synchronize()
+            assert torch.equal(o, w)
+    y = capi.cross_attention(*sets[1], key_lengths=lengths, stream=side)
+    side.synchronize()
+    assert torch.equal(y, first[1])
+
+
+def test_text_sublayer():
+    """A text-conditioned sublayer as it would be used: projections with weights in four bits,
+    cross attention to the prompts' states, the out projection onto the residual stream; each
+    step against float64 on its own inputs."""
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    tokens, text, width, heads, d = [400, 130], [77, 12], 256, 4, 64
+    x, states = _normal(gen, sum(tokens), width), _normal(gen, sum(text), 192).bfloat16()
+
+    def weight(n, k):
+        w = _normal(gen, n, k) * k ** -0.5
+        return capi.mx_quantize(w), mc.values(*mc.quantize(w), k).cuda()
+
+    (wq, wqv), (wkv, wkvv), (wo, wov) = weight(width, width), weight(2 * width, 192), weight(width, width)
+    xq = capi.mx_quantize(x)
+    q = capi.mx_linear(xq, wq)
+    kv = capi.mx_linear(states, wkv)
+    ro.check(q, *mc.linear(capi.mx_dequantize(xq, torch.float32).double(), wqv, None, "none", None, torch.bfloat16))
+    ro.check(kv, *mc.linear(states.double(), wkvv, None, "none", None, torch.bfloat16))
+    qo = torch.tensor([0, 400, 530], dtype=torch.int32, device="cuda")
+    ko = torch.tensor([0, 77, 89], dtype=torch.int32, device="cuda")
+    q3, k3, v3 = q.view(-1, heads, d), kv[:, :width].view(-1, heads, d), kv[:, width:].view(-1, heads, d)
+    o = capi.cross_attention(q3, k3, v3, q_offsets=qo, k_offsets=ko)
+    for qs, ks in ((slice(0, 400), slice(0, 77)), (slice(400, 530), slice(77, 89))):
+        ro.check(o[qs], *_sample(q3[qs], k3[ks], v3[ks], d ** -0.5, None, torch.bfloat16))
+    oq = capi.mx_quantize(o.view(-1, width))
+    y = capi.mx_linear(oq, wo, residual=x, out=x.clone())
+    ro.check(y, *mc.linear(capi.mx_dequantize(oq, torch.float32).double(), wov, None, "none", x, torch.float32))
