@@ -57,6 +57,16 @@ struct MatmulPlan {
     size_t bytes() const { return x_bytes + w_bytes + sum_bytes; }
 };
 
+// The tile and the ranges of k that take the least time over `steps` steps of 128 bytes of
+// a row, of tiles of `largest` rows at most and with room for `most` ranges' sums.
+struct TileChoice {
+    double us;
+    int bm, bn, parts;
+};
+TileChoice choose_tiles(const MatmulArgs& a, long steps, long most, int largest = 256);
+// Four neighbours of a row of y, the residual or the bias move as one piece.
+bool whole_pieces(const MatmulArgs& a);
+
 // The plan for a call with that much workspace.
 MatmulPlan plan_matmul(const MatmulArgs& a, size_t workspace_bytes);
 hipError_t launch_matmul(const MatmulArgs& a, void* workspace, size_t workspace_bytes,
@@ -65,6 +75,17 @@ hipError_t launch_matmul(const MatmulArgs& a, void* workspace, size_t workspace_
 // The kernels' own launchers, for calls that plan_matmul gives them.
 hipError_t launch_matmul_tiles(const MatmulArgs& a, const MatmulPlan& plan, float* sums,
                                hipStream_t stream);
+// parts > 1: a tile's k steps are dealt to `parts` workgroups, whose fp32 accumulators
+// go to partial[part][m][n]; matmul_sum_kernel adds them and does the epilogue.  For
+// few tiles and long k.
+struct TileSplit {
+    int ntiles, mtiles;
+    int parts;
+    bool whole;       // y, residual and n in pieces of four columns
+    int pitch;        // of partial's rows: n rounded up to four
+    float* partial;
+};
+hipError_t launch_matmul_sum(const MatmulArgs& a, const TileSplit& split, hipStream_t stream);
 constexpr int kShortMost = 160;   // k of the kernel for short k
 hipError_t launch_matmul_short(const MatmulArgs& a, const MatmulPlan& plan, hipStream_t stream);
 hipError_t launch_matmul_rows(const MatmulArgs& a, const MatmulPlan& plan, hipStream_t stream);

@@ -16,15 +16,14 @@
 
 namespace s2 {
 
-namespace {
-
-// Four neighbours of a row of y, the residual or the bias move as one piece.
 bool whole_pieces(const MatmulArgs& a) {
     const size_t e = a.y_kind ? 8 : 16;
     return a.n % 4 == 0 && a.y_stride % 4 == 0 && (uintptr_t)a.y % e == 0 &&
            (uintptr_t)a.bias % 16 == 0 &&
            (!a.res || (a.res_stride % 4 == 0 && (uintptr_t)a.res % e == 0));
 }
+
+namespace {
 
 // Any strides, alignment, n and k; fp32 activations.  Block tile 128x128,
 // k-step 32, four waves in a 2x2 grid of 64x64, both operands through registers
@@ -209,6 +208,12 @@ double tiles_us(const TileCost& t, double blocks, double steps) {
            (rest > 0 ? t.round + steps * (rest <= kUnits ? t.one : t.full) : 0.);
 }
 
+// a group's last tile is half empty, on average
+double tile_count(const MatmulArgs& a, const TileCost& t) {
+    return (a.offsets ? (double)a.m / t.bm + 0.5 * std::min(a.groups, a.m) : (double)row_tiles(a, t.bm)) *
+           (double)((a.n + t.bn - 1) / t.bn);
+}
+
 // The kernel for any shape with 16-bit rows, by the same measure, against packing those
 // rows (and the weight) first: a launch, and bytes a microsecond read and written.  Rows
 // apart by four elements too many: 8000 x 2560 by 2560 x 2560 177 us here and 118 packed,
@@ -246,6 +251,21 @@ long packed_width(const MatmulArgs& a, bool pack_w) { return round_up(a.k, pack_
 bool rows16(const void* p, long stride) { return stride % 8 == 0 && (uintptr_t)p % 16 == 0; }
 
 }  // namespace
+
+TileChoice choose_tiles(const MatmulArgs& a, long steps, long most, int largest) {
+    TileChoice best{0., 0, 0, 1};
+    const double each = (double)a.m * round_up(a.n, 4) * sizeof(float);   // a range's sums
+    for (const TileCost& t : kTileCosts) {
+        if (t.bm > largest) continue;
+        const double count = tile_count(a, t);
+        for (long parts = 1; parts <= std::max<long>(1, std::min(most, steps / 4)); ++parts) {
+            const double us = std::max(tiles_us(t, count * parts, (double)steps / parts), weight_us(a)) +
+                              (parts > 1 ? kSumUs + 2. * parts * each / kSumBytesUs : 0.);
+            if (best.us == 0. || us < best.us) best = TileChoice{us, t.bm, t.bn, (int)parts};
+        }
+    }
+    return best;
+}
 
 MatmulPlan plan_matmul(const MatmulArgs& a, size_t workspace_bytes) {
     MatmulPlan p{};
@@ -288,29 +308,14 @@ MatmulPlan plan_matmul(const MatmulArgs& a, size_t workspace_bytes) {
         const size_t each = (size_t)a.m * round_up(a.n, 4) * sizeof(float);   // a range's sums
         const long most =
             a.offsets ? 1 : std::min<long>(16, (long)((workspace_bytes - p.bytes()) / each));
-        // a group's last tile is half empty, on average
-        auto count_of = [&](const TileCost& t) {
-            return (a.offsets ? (double)a.m / t.bm + 0.5 * std::min(a.groups, a.m)
-                              : (double)row_tiles(a, t.bm)) *
-                   (double)((a.n + t.bn - 1) / t.bn);
-        };
-        for (const TileCost& t : kTileCosts) {
-            const double count = count_of(t);
-            for (long parts = 1; parts <= std::max<long>(1, std::min(most, steps / 4)); ++parts) {
-                const double us =
-                    std::max(tiles_us(t, count * parts, (double)steps / parts), weight_us(a)) +
-                    (parts > 1 ? kSumUs + 2. * parts * each / kSumBytesUs : 0.);
-                if (tile_us == 0. || us < tile_us) {
-                    tile_us = us;
-                    p.bm = t.bm;
-                    p.bn = t.bn;
-                    p.parts = (int)parts;
-                }
-            }
-        }
+        const TileChoice t = choose_tiles(a, steps, most);
+        tile_us = t.us;
+        p.bm = t.bm;
+        p.bn = t.bn;
+        p.parts = t.parts;
         if (p.parts > 1) p.sum_bytes = p.parts * each;
         const bool any = a.x_kind != 0 && p.pack_x &&
-                         tiles_us(kAnyCost, count_of(kAnyCost), (a.k + 63) / 64) <
+                         tiles_us(kAnyCost, tile_count(a, kAnyCost), (a.k + 63) / 64) <
                              tile_us + kPackUs + 2. * (double)(p.x_bytes + p.w_bytes) / kPackBytesUs;
         if (rows > 32 && !any) return p;
     }

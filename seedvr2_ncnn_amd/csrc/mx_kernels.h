@@ -6,6 +6,7 @@
 //
 //   mx_quantize_kernels.hip  rows to MXFP4 and back
 //   mx_linear_kernels.hip    which kernel takes a product; few rows
+//   mx_tile_kernels.hip      block tiles
 #pragma once
 
 #include "matmul_kernels.h"
@@ -44,6 +45,29 @@ hipError_t launch_mx_quantize(const void* x, int x_kind, long x_stride, int m, i
                               long code_stride, uint8_t* scales, long scale_stride, hipStream_t stream);
 hipError_t launch_mx_dequantize(const MxRows& rows, int m, int k, void* y, int y_kind, long y_stride,
                                 hipStream_t stream);
+
+// What a 256 x 256 tile's workspace holds: scales as its kernel reads them.
+struct DealtBytes {
+    size_t x, w;
+};
+inline DealtBytes mx_dealt_bytes(int m, int n, int blocks) {
+    const size_t steps = (blocks + 7) / 8;
+    return {((size_t)m + 255) / 256 * 2 * steps * 1024, ((size_t)n + 255) / 256 * 4 * steps * 512};
+}
+
+// Scales of a product on tiles: rows that begin at 16 bytes, but for 256 x 256.
+struct MxTileScales {
+    const uint8_t* x;
+    long x_stride;
+    const uint8_t* w;
+    long w_stride;
+    int blocks;
+};
+
+// a: the product with rows of codes as 16-bit elements, k of them eight a block.
+// workspace: mx_dealt_bytes for a 256 x 256 tile.
+hipError_t launch_mx_tiles(const MatmulArgs& a, const MxTileScales& scales, const TileChoice& tile,
+                           float* sums, void* workspace, hipStream_t stream);
 
 size_t mx_linear_workspace(const MxLinearArgs& a);
 hipError_t launch_mx_linear(const MxLinearArgs& a, void* workspace, size_t workspace_bytes,

@@ -151,23 +151,143 @@ hipError_t launch_rows(const MxLinearArgs& a, hipStream_t stream) {
     return a.m <= 16 ? run_rows<XT, 1, 2>(a, stream) : run_rows<XT, 2, 2>(a, stream);
 }
 
+// Scales of x's and of the weight's rows to rows of `width` bytes, either of which may have
+// none.
+struct ScaleJob {
+    const uint8_t* src;
+    long stride, rows;
+    uint8_t* dst;
+};
+
+__global__ __launch_bounds__(256) void mx_scales_kernel(ScaleJob x, ScaleJob w, int blocks, int width) {
+    const long nx = x.rows * blocks, all = nx + w.rows * blocks;
+    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < all; i += (long)gridDim.x * 256) {
+        const ScaleJob& job = i < nx ? x : w;
+        const long at = i < nx ? i : i - nx;
+        const long row = at / blocks;
+        const int b = (int)(at - row * blocks);
+        job.dst[row * width + b] = job.src[row * job.stride + b];
+    }
+}
+
+long round_up(long v, long to) { return (v + to - 1) / to * to; }
+
+// The weight's values as bf16 rows of k, for rows of x of other types.
+size_t weight_bytes(const MxLinearArgs& a) { return round_up((size_t)a.n * a.k * 2, 256); }
+
+MatmulArgs values_args(const MxLinearArgs& a, const void* w) {
+    MatmulArgs m{};
+    m.x = a.x;
+    m.x_kind = a.x_kind;
+    m.x_stride = a.x_stride;
+    m.m = a.m;
+    m.groups = 1;
+    m.w = w;
+    m.w_kind = S2_DTYPE_BF16;
+    m.bias = a.bias;
+    m.n = a.n;
+    m.k = a.k;
+    m.act = a.act;
+    m.res = a.res;
+    m.res_stride = a.res_stride;
+    m.y = a.y;
+    m.y_kind = a.y_kind;
+    m.y_stride = a.y_stride;
+    m.planes = 1;
+    return m;
+}
+
+// The product with rows of codes as 16-bit elements.
+MatmulArgs codes_args(const MxLinearArgs& a) {
+    MatmulArgs m = values_args(a, a.w.codes);
+    m.x = a.xq.codes;
+    m.x_kind = S2_DTYPE_BF16;
+    m.x_stride = a.xq.code_stride / 2;
+    m.k = 8 * mx_blocks(a.k);
+    return m;
+}
+
+constexpr int kRowsMost = 32;   // of x that the kernel for few rows takes
+
+// Ranges of k, at most, whose sums fit `bytes`.
+long ranges(const MxLinearArgs& a, size_t bytes) {
+    return std::min<long>(16, (long)(bytes / ((size_t)a.m * round_up(a.n, 4) * sizeof(float))));
+}
+
+bool scales16(const uint8_t* s, long stride) { return (uintptr_t)s % 16 == 0 && stride % 16 == 0; }
+
+// A product on tiles: what the scales take in the workspace (for 256 x 256 as they are
+// dealt out, else rows that begin at no 16 bytes copied), then the sums.
+struct MxPlan {
+    TileChoice tile;
+    size_t scales, sums;
+    size_t bytes() const { return scales + sums; }
+};
+
+MxPlan mx_plan(const MxLinearArgs& a, bool pack_x, bool pack_w, size_t workspace_bytes) {
+    const MatmulArgs m = codes_args(a);
+    const int blocks = mx_blocks(a.k);
+    const DealtBytes dealt = mx_dealt_bytes(a.m, a.n, blocks);
+    const size_t copied = ((pack_x ? (size_t)a.m : 0) + (pack_w ? (size_t)a.n : 0)) * round_up(blocks, 16);
+    MxPlan p{};
+    for (int largest : {256, 128}) {
+        const size_t least = round_up(largest == 256 ? dealt.x + dealt.w : copied, 256);
+        if (least > workspace_bytes) continue;
+        p.tile = choose_tiles(m, (m.k + 63) / 64, ranges(a, workspace_bytes - least), largest);
+        p.scales = round_up(p.tile.bm == 256 ? dealt.x + dealt.w : copied, 256);
+        p.sums = p.tile.parts > 1 ? (size_t)p.tile.parts * a.m * round_up(a.n, 4) * sizeof(float) : 0;
+        if (p.bytes() <= workspace_bytes) return p;
+    }
+    p.tile.bm = 0;   // not on tiles
+    return p;
+}
+
 }  // namespace
 
-size_t mx_linear_workspace(const MxLinearArgs&) { return 0; }
+size_t mx_linear_workspace(const MxLinearArgs& a) {
+    if (a.m <= kRowsMost) return 0;
+    return mx_plan(a, true, true, (size_t)1 << 62).bytes();
+}
 
-hipError_t launch_mx_linear(const MxLinearArgs& args, void*, size_t, hipStream_t stream) {
+hipError_t launch_mx_linear(const MxLinearArgs& args, void* workspace, size_t workspace_bytes,
+                            hipStream_t stream) {
     if (args.m <= 0) return hipSuccess;
     MxLinearArgs a = args;
+    const int blocks = mx_blocks(a.k);
     if (a.m == 1) {   // the strides of a single row say nothing
         a.x_stride = a.k;
         a.res_stride = a.y_stride = a.n;
-        a.xq.code_stride = 16L * mx_blocks(a.k);
-        a.xq.scale_stride = mx_blocks(a.k);
+        a.xq.code_stride = 16L * blocks;
+        a.xq.scale_stride = round_up(blocks, 16);
     }
-    if (a.mx) return launch_rows<0>(a, stream);
-    return a.x_kind == 0   ? launch_rows<1>(a, stream)
-           : a.x_kind == 1 ? launch_rows<2>(a, stream)
-                           : launch_rows<3>(a, stream);
+    if (a.n == 1) a.w.scale_stride = round_up(blocks, 16);
+    if (!a.mx)
+        return a.x_kind == 0   ? launch_rows<1>(a, stream)
+               : a.x_kind == 1 ? launch_rows<2>(a, stream)
+                               : launch_rows<3>(a, stream);
+    const long out = std::max(a.y_stride, a.res ? a.res_stride : 0L) * (a.y_kind ? 2 : 4);
+    const long far = 0x7fffffffL;   // 32-bit offsets
+    const bool pack_x = !scales16(a.xq.scales, a.xq.scale_stride);
+    const bool pack_w = !scales16(a.w.scales, a.w.scale_stride);
+    MxPlan p{};
+    if (a.m > kRowsMost && 256 * out < far && (long)a.n * 4 < far && 256 * a.xq.code_stride < far &&
+        256 * 16L * blocks < far && 256 * std::max(a.xq.scale_stride, a.w.scale_stride) < far)
+        p = mx_plan(a, pack_x, pack_w, workspace_bytes);
+    if (p.tile.bm == 0) return launch_rows<0>(a, stream);
+    MxTileScales sc{a.xq.scales, a.xq.scale_stride, a.w.scales, a.w.scale_stride, blocks};
+    if (p.tile.bm < 256 && (pack_x || pack_w)) {
+        const int width = (int)round_up(blocks, 16);
+        uint8_t* at = (uint8_t*)workspace;
+        const ScaleJob x{a.xq.scales, a.xq.scale_stride, pack_x ? a.m : 0, at};
+        const ScaleJob w{a.w.scales, a.w.scale_stride, pack_w ? a.n : 0, at + (pack_x ? (size_t)a.m * width : 0)};
+        const long all = (x.rows + w.rows) * blocks;
+        mx_scales_kernel<<<(unsigned)std::min<long>((all + 255) / 256, 4096), 256, 0, stream>>>(x, w, blocks, width);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+        if (pack_x) sc.x = x.dst, sc.x_stride = width;
+        if (pack_w) sc.w = w.dst, sc.w_stride = width;
+    }
+    return launch_mx_tiles(codes_args(a), sc, p.tile, (float*)((char*)workspace + p.scales), workspace, stream);
 }
 
 }  // namespace s2
