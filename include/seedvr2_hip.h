@@ -651,8 +651,8 @@ S2_API int s2_mx_weight_linear(const void* x, s2_dtype x_dtype, long x_stride, i
  *   of out in no sample are not written.
  * Strides in elements, batch (unused with offsets), row, head, elements contiguous: for
  *   q, k, v and out in turn, strides[0..11].  q, k and v are of one dtype; their rows
- *   start at 16 bytes (strides a multiple of 16 bytes too); out's at its elements, its
- *   rows do not overlap, and it overlaps nothing else, but may be q itself
+ *   start at 16 bytes (strides a multiple of 16 bytes too, row strides of k and v up to 2^23
+ *   elements); out's at its elements, its rows do not overlap, and it overlaps nothing else, but may be q itself
  *   (same dtype and strides).
  * key_mask: device bytes [batch][mask_stride], or [lk] with offsets, 0 for keys to leave
  *   out, or NULL.  What k and v hold where a key is left out, infinities and NaN among it,

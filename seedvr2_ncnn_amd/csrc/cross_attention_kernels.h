@@ -1,5 +1,8 @@
 // Cross attention's launchers.  Element kinds are the s2_dtype codes, strides are in
 // elements.
+//
+//   cross_attention_kernels.hip  which kernel takes a call; the joining of ranges of keys
+//   cross_tile_kernels.hip       16-bit operands, tiles of rows
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -31,6 +34,24 @@ struct CrossArgs {
     int heads, kv_heads, d;
     float scale;
 };
+
+// A call's kernel.  Rows: queries times the heads that share a kv head.
+struct CrossPlan {
+    int rows;     // of a tile
+    int tiles;    // of a kv head, at most
+    int parts;    // ranges of keys
+};
+
+// Sums of a range of keys: [row of q][head][part], d floats each, then the maximum and the
+// sum of the weights of each.
+struct CrossParts {
+    int parts;
+    float* sums;
+    float2* weights;
+};
+
+CrossParts cross_parts(const CrossArgs& a, const CrossPlan& plan, void* workspace);
+hipError_t launch_cross_tiles(const CrossArgs& a, const CrossPlan& plan, void* workspace, hipStream_t stream);
 
 size_t cross_attention_workspace(const CrossArgs& a);
 hipError_t launch_cross_attention(const CrossArgs& a, void* workspace, size_t workspace_bytes,

@@ -1,7 +1,6 @@
 // Cross attention: softmax(scale q k^T) v per sample and head, keys of another length
 // than the queries.
-#include "cross_attention_kernels.h"
-#include "matmul_device.h"
+#include "cross_attention_device.h"
 
 namespace s2 {
 
@@ -56,14 +55,85 @@ __global__ __launch_bounds__(256) void cross_any_kernel(CrossArgs a) {
         if (lane + 64 * e < a.d) store1(a.out, oa + lane + 64 * e, l == 0.f ? 0.f : o[e] / l, a.out_kind);
 }
 
+// Four columns of a row a thread: its parts' sums, by how far their maxima lie below the
+// largest.
+__global__ __launch_bounds__(256) void cross_join_kernel(CrossArgs a, CrossParts p, long rows) {
+    const int quads = a.d / 4;
+    const long first = a.q_offsets ? clamped(a.q_offsets[0], a.lq) : 0;
+    const long end = a.q_offsets ? clamped(a.q_offsets[a.batch], a.lq) : rows;
+    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < rows * a.heads * quads; i += (long)gridDim.x * 256) {
+        const long rh = i / quads;
+        const int col = (int)(i - rh * quads) * 4;
+        const long row = rh / a.heads;
+        const int h = (int)(rh - row * a.heads);
+        if (row < first || row >= end) continue;   // in no sample
+        const float2* w = p.weights + rh * p.parts;
+        float m = kLowest;
+        for (int q = 0; q < p.parts; ++q) m = fmaxf(m, w[q].x);
+        float l = 0.f;
+        f32x4 o = {0.f, 0.f, 0.f, 0.f};
+        for (int q = 0; q < p.parts; ++q) {
+            const float f = __builtin_amdgcn_exp2f(w[q].x - m);
+            l += f * w[q].y;
+            o += f * *reinterpret_cast<const f32x4*>(p.sums + (rh * p.parts + q) * a.d + col);
+        }
+        const long b = a.q_offsets ? 0 : row / a.lq;
+        const long at = b * a.os.batch + (row - b * a.lq) * a.os.row + h * a.os.head + col;
+        store4_out(a, at, o * (l == 0.f ? 0.f : 1.f / l));
+    }
+}
+
+long all_rows(const CrossArgs& a) { return a.q_offsets ? (long)a.lq : (long)a.batch * a.lq; }
+
+size_t part_bytes(const CrossArgs& a) { return (size_t)all_rows(a) * a.heads * (a.d * sizeof(float) + sizeof(float2)); }
+
+constexpr int kUnits = 256;   // compute units of an MI355X
+
+CrossPlan cross_plan(const CrossArgs& a, size_t workspace_bytes) {
+    const long group = a.heads / a.kv_heads;
+    auto tiles_of = [&](long each) {
+        return a.q_offsets ? (long)a.lq * group / each + std::min(a.batch, a.lq)
+                           : (long)a.batch * (((long)a.lq * group + each - 1) / each);
+    };
+    CrossPlan p;
+    const long keys = a.q_offsets ? ((long)a.lk + a.batch - 1) / std::max(a.batch, 1) : a.lk;   // of a sample
+    p.rows = a.d <= 128 && keys >= 1024 && tiles_of(256) * a.kv_heads >= 2 * kUnits ? 256 : 128;
+    p.tiles = (int)std::min<long>(tiles_of(p.rows), 0x7fffffffL);
+    const long blocks = (long)p.tiles * a.kv_heads;
+    const long most = std::min<long>(64, (long)(workspace_bytes / part_bytes(a)));
+    p.parts = (int)std::max<long>(1, std::min({3 * kUnits / blocks, keys / 256, most}));
+    return p;
+}
+
 }  // namespace
 
-size_t cross_attention_workspace(const CrossArgs&) { return 0; }
+CrossParts cross_parts(const CrossArgs& a, const CrossPlan& plan, void* workspace) {
+    float* sums = (float*)workspace;
+    return CrossParts{plan.parts, sums,
+                      (float2*)(sums + (size_t)all_rows(a) * a.heads * plan.parts * (plan.parts > 1 ? a.d : 0))};
+}
 
-hipError_t launch_cross_attention(const CrossArgs& a, void*, size_t, hipStream_t stream) {
-    const long rows = a.q_offsets ? (long)a.lq : (long)a.batch * a.lq;
+size_t cross_attention_workspace(const CrossArgs& a) {
+    if (a.kind == 0) return 0;
+    const CrossPlan p = cross_plan(a, (size_t)1 << 62);
+    return p.parts > 1 ? p.parts * part_bytes(a) : 0;
+}
+
+hipError_t launch_cross_attention(const CrossArgs& a, void* workspace, size_t workspace_bytes,
+                                  hipStream_t stream) {
+    const long rows = all_rows(a);
+    if (rows <= 0) return hipSuccess;
+    if (a.kind) {
+        const CrossPlan p = cross_plan(a, workspace_bytes);
+        if ((long)p.tiles * a.kv_heads * p.parts > 0x7fffffffL) return hipErrorInvalidValue;
+        const hipError_t e = launch_cross_tiles(a, p, workspace, stream);
+        if (e != hipSuccess || p.parts == 1) return e;
+        const long all = rows * a.heads * (a.d / 4);
+        cross_join_kernel<<<(unsigned)std::min<long>((all + 255) / 256, 8192), 256, 0, stream>>>(
+            a, cross_parts(a, p, workspace), rows);
+        return hipGetLastError();
+    }
     const long blocks = (rows * a.heads + 3) / 4;
-    if (blocks <= 0) return hipSuccess;
     if (blocks > 0x7fffffffL) return hipErrorInvalidValue;
     cross_any_kernel<<<(unsigned)blocks, 256, 0, stream>>>(a);
     return hipGetLastError();

@@ -1,0 +1,323 @@
+// Cross attention of 16-bit operands on tiles of rows.
+//
+// A wave has 16 NQ rows, whose q stays in registers; k and v go through LDS by DMA in tiles
+// of KT keys that the workgroup's four waves share.  S^T = K Q^T and O^T = V^T P^T on
+// 16x16x32 products: a score accumulator's four registers are four neighbouring keys of one
+// row, and two of them, of 16 keys each, are the second product's operand as they stand.
+// Its other operand, four keys by 16 columns of v, is what a transposing LDS read gives of
+// v's rows.  So weights never leave registers and v is not transposed before.
+//
+// Softmax in powers of two: weights are 2^(c s - m), c = |scale| log2 e (a negative scale turns q's
+// signs), m a maximum that follows the scores' only when a row's passes it by 8: the few
+// rescales cost nothing, and a tile's maxima need not be exchanged between lanes to find
+// that none is due.  Weights are rounded to the operands' type for the second product,
+// at most half a step each, as independent errors of its terms; their sum stays in fp32.
+#include "cross_attention_device.h"
+
+namespace s2 {
+
+namespace {
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+template <int T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    if constexpr (T == 1) {
+        typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2{lo, hi}), b2));
+    } else {
+        typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2{lo, hi}), h2));
+    }
+}
+
+// Four keys' values of one column: lane i of each 16 supplies 8 bytes of row i / 4, and gets
+// column i of the four rows.
+__device__ __forceinline__ uint2 read_columns(const uint8_t* p) {
+    typedef __attribute__((address_space(3))) s16x4* Lds;
+    return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)p));
+}
+
+// fp16 weights reach 2^14 so that its subnormal numbers begin 2^-28 below the largest;
+// 2^8 where a row's maximum is 8 past m.
+template <int T>
+constexpr float kShift = T == 2 ? 6.f : 0.f;
+constexpr float kLazy = 8.f;
+
+// 16-byte chunk c of row r of a k tile stands at c ^ key_swizzle(r): the rows of one read
+// phase lie on distinct banks.  For v, the pairs of chunks that one transposing read takes
+// of eight rows.
+template <int DP>
+__device__ __forceinline__ int key_swizzle(int r) {
+    return DP == 64 ? lds_swizzle(r) : r & 7;
+}
+template <int DP>
+__device__ __forceinline__ int value_swizzle(int r) {
+    return DP == 64 ? ((r >> 1) & 3) * 2 : (r & 7) * 2;
+}
+
+template <int T, int DP, int NQ, int KT, int STAGES, int WGS, bool MASK>
+__global__ __launch_bounds__(256, WGS) void cross_tile_kernel(CrossArgs a, int tiles, CrossParts parts) {
+    constexpr int BM = 64 * NQ;                  // rows of the workgroup
+    constexpr int RB = DP * 2;                   // bytes of a row in LDS
+    constexpr int KB = KT * RB, SB = 2 * KB;     // a tile of k; a stage
+    constexpr int CH = RB / 16;                  // chunks of a row
+    constexpr int KI = KB / 4096;                // DMA instructions of a wave and operand
+    constexpr int NK = DP / 32, ND = DP / 16;    // product steps over d; column tiles
+    constexpr int MB = 128;                      // tiles of a block of mask bits
+    typedef typename std::conditional<KT == 64, uint64_t, uint32_t>::type Bits;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[STAGES * SB];
+    __shared__ uint64_t bits[MASK ? 2 * MB : 1];
+    const CrossTile t = cross_tile(a, BM, tiles, parts.parts);
+    if (t.rows <= 0) return;   // the whole workgroup
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int l16 = lane & 15, g = lane >> 4;
+    const uint32_t base = (uint32_t)(uintptr_t)lds;
+    const int row_w = wave * 16 * NQ;   // of the wave's first row in the tile
+
+    const int nk = __builtin_amdgcn_readfirstlane(t.s.nk);
+    const int all = (nk + KT - 1) / KT;
+    const int kb = (int)((long)all * t.part / parts.parts), ke = (int)((long)all * (t.part + 1) / parts.parts);
+
+    // k and v: one descriptor a tile, from its first row on
+    const long kr = a.ks.row * 2, vr = a.vs.row * 2;
+    const char* kp = (const char*)a.k + (t.s.b * a.ks.batch + t.s.k0 * a.ks.row + t.head * a.ks.head) * 2;
+    const char* vp = (const char*)a.v + (t.s.b * a.vs.batch + t.s.k0 * a.vs.row + t.head * a.vs.head) * 2;
+    uint32_t ko[KI], vo[KI];
+#pragma unroll
+    for (int j = 0; j < KI; ++j) {
+        const int at = (wave * KI + j) * 64 + lane;
+        const int r = at / CH, c = at % CH;
+        const int ck = c ^ key_swizzle<DP>(r), cv = c ^ value_swizzle<DP>(r);
+        ko[j] = ck * 8 < a.d ? (uint32_t)(r * kr) + ck * 16 : kOutside;
+        vo[j] = cv * 8 < a.d ? (uint32_t)(r * vr) + cv * 16 : kOutside;
+    }
+    // keys of tile kt that count
+    auto valid_of = [&](int kt) -> Bits {
+        const int left = nk - kt * KT;
+        Bits v = left >= KT ? ~(Bits)0 : ((Bits)1 << left) - 1;
+        if constexpr (MASK) {
+            const uint32_t* m = (const uint32_t*)&bits[kt / (64 / KT) % (2 * MB)];
+            if constexpr (KT == 64)
+                v &= (uint64_t)__builtin_amdgcn_readfirstlane(m[0]) |
+                     (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane(m[1]) << 32;
+            else
+                v &= (uint32_t)__builtin_amdgcn_readfirstlane(m[kt & 1]);
+        }
+        return v;
+    };
+    // the mask of the next MB * 64 keys as bits, when the first tile of them is loaded
+    auto read_mask = [&](int kt, bool first) {
+        if constexpr (MASK) {
+            const int word = kt / (64 / KT);
+            if (!first && (word % MB != 0 || kt % (64 / KT) != 0)) return;
+            const uint8_t* mask = a.key_mask + t.s.b * a.mask_batch + t.s.k0;
+            for (int w = word / MB * MB + wave; w < (word / MB + 1) * MB; w += 4) {
+                const int key = w * 64 + lane;
+                const uint64_t m = __ballot(key < nk && mask[min(key, nk - 1)] != 0);
+                if (lane == 0) bits[w % (2 * MB)] = m;
+            }
+            __syncthreads();
+        }
+    };
+    auto issue = [&](int kt, bool first) {
+        read_mask(kt, first);
+        const uint32_t st = base + (kt - kb) % STAGES * SB;
+        const i32x4 rk = wave_uniform(buffer_rsrc(kp + (long)kt * KT * kr, (uint32_t)((KT - 1) * kr + RB)));
+        const i32x4 rv = wave_uniform(buffer_rsrc(vp + (long)kt * KT * vr, (uint32_t)((KT - 1) * vr + RB)));
+        const Bits valid = valid_of(kt);
+        if (valid == ~(Bits)0) {
+#pragma unroll
+            for (int j = 0; j < KI; ++j)
+                lds_dma16(rk, __builtin_amdgcn_readfirstlane(st + (wave * KI + j) * 1024), ko[j], 0);
+#pragma unroll
+            for (int j = 0; j < KI; ++j)
+                lds_dma16(rv, __builtin_amdgcn_readfirstlane(st + KB + (wave * KI + j) * 1024), vo[j], 0);
+        } else {   // zeros for keys that do not count, whatever is there
+#pragma unroll
+            for (int j = 0; j < KI; ++j) {
+                const uint32_t out = valid >> (((wave * KI + j) * 64 + lane) / CH) & 1 ? 0u : kOutside;
+                lds_dma16(rk, __builtin_amdgcn_readfirstlane(st + (wave * KI + j) * 1024), ko[j] | out, 0);
+                lds_dma16(rv, __builtin_amdgcn_readfirstlane(st + KB + (wave * KI + j) * 1024), vo[j] | out, 0);
+            }
+        }
+    };
+
+#pragma unroll
+    for (int s = 0; s < STAGES - 1; ++s)
+        if (kb + s < ke) issue(kb + s, s == 0);
+
+    // q: row l16 of each 16, elements 32 kk + 8 g on; zeros past d and past the rows
+    const uint32_t sign = a.scale < 0.f ? 0x80008000u : 0u;
+    // (not nought, by which a masked score of -inf would be NaN)
+    const float c = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 0x1p-126f);
+    uint4 qf[NQ][NK];
+#pragma unroll
+    for (int i = 0; i < NQ; ++i) {
+        const int r = row_w + 16 * i + l16;
+        const uint16_t* p = (const uint16_t*)a.q + cross_row(a, a.qs, t, t.row0 + min(r, t.rows - 1));
+#pragma unroll
+        for (int kk = 0; kk < NK; ++kk) {
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (32 * kk + 8 * g < a.d) v = *reinterpret_cast<const uint4*>(p + 32 * kk + 8 * g);
+            qf[i][kk] = make_uint4(v.x ^ sign, v.y ^ sign, v.z ^ sign, v.w ^ sign);
+        }
+    }
+    // q is there before the loop, in a way that the compiler sees: with these loads perhaps in
+    // flight it would wait for all of the DMA in every tile
+    __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0)
+
+    f32x4 o[ND][NQ];
+#pragma unroll
+    for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+        for (int i = 0; i < NQ; ++i) o[dt][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float m[NQ], l[NQ];   // l: of this lane's keys
+#pragma unroll
+    for (int i = 0; i < NQ; ++i) m[i] = kLowest, l[i] = 0.f;
+    const int ksw = key_swizzle<DP>(l16);
+    const int vrow = 4 * g + (l16 >> 2);          // of the lane's piece of v, of 16 rows
+    const int vsw = value_swizzle<DP>(vrow);
+
+#pragma unroll 1
+    for (int kt = kb; kt < ke; ++kt) {
+        if (kt + 1 < ke) {
+            // tiles after this one may be in flight; STAGES is 3
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * KI) : "memory");
+        } else {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("s_barrier" ::: "memory");   // tile kt is there, tile kt - 1 no longer read
+        __builtin_amdgcn_sched_barrier(0);
+        if (kt + STAGES - 1 < ke) issue(kt + STAGES - 1, false);
+        const Bits valid = valid_of(kt);
+        const uint8_t* st = lds + (kt - kb) % STAGES * SB;
+#pragma unroll
+        for (int u = 0; u < KT / 32; ++u) {
+            f32x4 s[2][NQ];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const uint8_t* kl = st + (32 * u + 16 * h + l16) * RB;
+                uint4 kf[NK];
+#pragma unroll
+                for (int kk = 0; kk < NK; ++kk) kf[kk] = *(const uint4*)(kl + (((4 * kk + g) ^ ksw) * 16));
+#pragma unroll
+                for (int kk = 0; kk < NK; ++kk)
+#pragma unroll
+                    for (int i = 0; i < NQ; ++i)
+                        s[h][i] = mfma<T>(kf[kk], qf[i][kk], kk ? s[h][i] : f32x4{0.f, 0.f, 0.f, 0.f});
+            }
+            if (valid != ~(Bits)0) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const uint32_t v4 = (uint32_t)(valid >> (32 * u + 16 * h)) >> (4 * g);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+#pragma unroll
+                        for (int i = 0; i < NQ; ++i)
+                            if (!(v4 >> r & 1)) s[h][i][r] = -__builtin_inff();
+                }
+            }
+            float top[NQ];
+            bool due = false;
+#pragma unroll
+            for (int i = 0; i < NQ; ++i) {
+                float x = fmaxf(fmaxf(s[0][i][0], s[0][i][1]), s[0][i][2]);
+                x = fmaxf(fmaxf(x, s[0][i][3]), s[1][i][0]);
+                x = fmaxf(fmaxf(x, s[1][i][1]), s[1][i][2]);
+                top[i] = fmaxf(x, s[1][i][3]) * c;
+                due |= top[i] > m[i] + kLazy;
+            }
+            if (__any(due)) {
+#pragma unroll
+                for (int i = 0; i < NQ; ++i) {
+                    float x = top[i];
+                    x = fmaxf(x, __shfl_xor(x, 16));
+                    x = fmaxf(x, __shfl_xor(x, 32));
+                    x = fmaxf(x, m[i]);
+                    const float fade = __builtin_amdgcn_exp2f(m[i] - x);
+                    m[i] = x;
+                    l[i] *= fade;
+#pragma unroll
+                    for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) o[dt][i][r] *= fade;
+                }
+            }
+            uint4 pb[NQ];
+#pragma unroll
+            for (int i = 0; i < NQ; ++i) {
+                float p[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    p[e] = __builtin_amdgcn_exp2f(fmaf(s[e >> 2][i][e & 3], c, kShift<T> - m[i]));
+                pb[i] = make_uint4(pack2<T>(p[0], p[1]), pack2<T>(p[2], p[3]), pack2<T>(p[4], p[5]),
+                                   pack2<T>(p[6], p[7]));
+                l[i] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+            }
+            const uint8_t* vl = st + KB + (32 * u + vrow) * RB + (l16 & 1) * 8;
+#pragma unroll
+            for (int dt = 0; dt < ND; ++dt) {
+                const int at = ((2 * dt + (l16 >> 1 & 1)) ^ vsw) * 16;
+                const uint2 v0 = read_columns(vl + at), v1 = read_columns(vl + at + 16 * RB);
+                const uint4 vf = make_uint4(v0.x, v0.y, v1.x, v1.y);
+#pragma unroll
+                for (int i = 0; i < NQ; ++i) o[dt][i] = mfma<T>(vf, pb[i], o[dt][i]);
+            }
+        }
+    }
+
+#pragma unroll
+    for (int i = 0; i < NQ; ++i) {
+        l[i] += __shfl_xor(l[i], 16);
+        l[i] += __shfl_xor(l[i], 32);
+        const int r = row_w + 16 * i + l16;
+        if (r >= t.rows) continue;
+        if (parts.parts > 1) {
+            const long at = cross_part(a, parts, t, t.row0 + r);
+            if (g == 0) parts.weights[at] = make_float2(m[i], l[i]);
+#pragma unroll
+            for (int dt = 0; dt < ND; ++dt)
+                if (16 * dt + 4 * g < a.d) *reinterpret_cast<f32x4*>(parts.sums + at * a.d + 16 * dt + 4 * g) = o[dt][i];
+        } else {
+            const float scale = l[i] == 0.f ? 0.f : 1.f / l[i];
+            const long at = cross_row(a, a.os, t, t.row0 + r);
+#pragma unroll
+            for (int dt = 0; dt < ND; ++dt)
+                if (16 * dt + 4 * g < a.d) store4_out(a, at + 16 * dt + 4 * g, o[dt][i] * scale);
+        }
+    }
+}
+
+template <int T, int DP, int NQ, int KT, int STAGES, int WGS>
+hipError_t launch(const CrossArgs& a, int tiles, const CrossParts& parts, unsigned blocks, hipStream_t stream) {
+    static_assert(STAGES == 3, "the loop's waits");
+    if (a.key_mask)
+        cross_tile_kernel<T, DP, NQ, KT, STAGES, WGS, true><<<blocks, 256, 0, stream>>>(a, tiles, parts);
+    else
+        cross_tile_kernel<T, DP, NQ, KT, STAGES, WGS, false><<<blocks, 256, 0, stream>>>(a, tiles, parts);
+    return hipGetLastError();
+}
+
+template <int T>
+hipError_t launch_t(const CrossArgs& a, const CrossPlan& p, const CrossParts& parts, hipStream_t stream) {
+    const unsigned nb = (unsigned)((long)p.tiles * a.kv_heads * p.parts);
+    if (a.d > 128) return launch<T, 256, 2, 32, 3, 1>(a, p.tiles, parts, nb, stream);
+    if (a.d > 64)
+        return p.rows == 256 ? launch<T, 128, 4, 64, 3, 1>(a, p.tiles, parts, nb, stream)
+                             : launch<T, 128, 2, 32, 3, 3>(a, p.tiles, parts, nb, stream);
+    return p.rows == 256 ? launch<T, 64, 4, 64, 3, 2>(a, p.tiles, parts, nb, stream)
+                         : launch<T, 64, 2, 32, 3, 3>(a, p.tiles, parts, nb, stream);
+}
+
+}  // namespace
+
+hipError_t launch_cross_tiles(const CrossArgs& a, const CrossPlan& plan, void* workspace, hipStream_t stream) {
+    const CrossParts parts = cross_parts(a, plan, workspace);
+    return a.kind == 1 ? launch_t<1>(a, plan, parts, stream) : launch_t<2>(a, plan, parts, stream);
+}
+
+}  // namespace s2
