@@ -97,7 +97,7 @@ CrossPlan cross_plan(const CrossArgs& a, size_t workspace_bytes) {
     };
     CrossPlan p;
     const long keys = a.q_offsets ? ((long)a.lk + a.batch - 1) / std::max(a.batch, 1) : a.lk;   // of a sample
-    p.rows = a.d <= 128 && keys >= 1024 && tiles_of(256) * a.kv_heads >= 2 * kUnits ? 256 : 128;
+    p.rows = 128;
     p.tiles = (int)std::min<long>(tiles_of(p.rows), 0x7fffffffL);
     const long blocks = (long)p.tiles * a.kv_heads;
     const long most = std::min<long>(64, (long)(workspace_bytes / part_bytes(a)));

@@ -1,11 +1,12 @@
 // Cross attention of 16-bit operands on tiles of rows.
 //
-// A wave has 16 NQ rows, whose q stays in registers; k and v go through LDS by DMA in tiles
-// of KT keys that the workgroup's four waves share.  S^T = K Q^T and O^T = V^T P^T on
-// 16x16x32 products: a score accumulator's four registers are four neighbouring keys of one
-// row, and two of them, of 16 keys each, are the second product's operand as they stand.
-// Its other operand, four keys by 16 columns of v, is what a transposing LDS read gives of
-// v's rows.  So weights never leave registers and v is not transposed before.
+// A wave has 32 rows, whose q stays in registers; k and v go through LDS by DMA in tiles of
+// 32 keys that the workgroup's four waves share.  S^T = K Q^T and O^T = V^T P^T on 16x16x32
+// products: a score accumulator's four registers are four neighbouring keys of one row, and
+// two of them, of 16 keys each, are the second product's operand as they stand.  Its other
+// operand, four keys by 16 columns of v, is what a transposing LDS read gives of v's rows.
+// So weights never leave registers and v is not transposed before.  (32x32x16 products
+// leave the matrix cores waiting less, but the chip clocks lower: 3 to 5% slower.)
 //
 // Softmax in powers of two: weights are 2^(c s - m), c = |scale| log2 e (a negative scale turns q's
 // signs), m a maximum that follows the scores' only when a row's passes it by 8: the few
@@ -45,28 +46,56 @@ template <int T>
 constexpr float kShift = T == 2 ? 6.f : 0.f;
 constexpr float kLazy = 8.f;
 
-// 16-byte chunk c of row r of a k tile stands at c ^ key_swizzle(r): the rows of one read
-// phase lie on distinct banks.  For v, the pairs of chunks that one transposing read takes
-// of eight rows.
+// A read of 16 bytes a lane is done 16 lanes at a time, one of 8 bytes 32 lanes, each 256
+// bytes on 64 banks.  Chunk c (16 bytes) of row r of a k tile stands at c ^ key_swizzle(r):
+// 16 rows of one chunk lie on distinct banks.  Of v, eight rows of a pair of chunks do.
 template <int DP>
 __device__ __forceinline__ int key_swizzle(int r) {
-    return DP == 64 ? lds_swizzle(r) : r & 7;
+    return DP == 64 ? (r >> 1) & 7 : r & 15;
 }
 template <int DP>
 __device__ __forceinline__ int value_swizzle(int r) {
     return DP == 64 ? ((r >> 1) & 3) * 2 : (r & 7) * 2;
 }
 
-template <int T, int DP, int NQ, int KT, int STAGES, int WGS, bool MASK>
+// Two weights' sum and l.
+template <int T>
+__device__ __forceinline__ float add_pair(uint32_t p, float l) {
+    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    if constexpr (T == 1)
+        return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(b2, p), __builtin_bit_cast(b2, 0x3f803f80u), l,
+                                               false);
+    else
+        return __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, p), __builtin_bit_cast(h2, 0x3c003c00u), l, false);
+}
+
+// Of the wave's four groups of 16 lanes.
+__device__ __forceinline__ float max_groups(float x) {
+    auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float sum_groups(float x) {
+    auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// DP: d rounded up to 64, 128 or 256.  STAGES: of LDS; WGS: workgroups on a compute unit.
+template <int T, int DP, int STAGES, int WGS, bool MASK>
 __global__ __launch_bounds__(256, WGS) void cross_tile_kernel(CrossArgs a, int tiles, CrossParts parts) {
-    constexpr int BM = 64 * NQ;                  // rows of the workgroup
+    constexpr int KT = 32;                       // keys of a tile
+    constexpr int BM = 128;                      // rows of the workgroup
     constexpr int RB = DP * 2;                   // bytes of a row in LDS
     constexpr int KB = KT * RB, SB = 2 * KB;     // a tile of k; a stage
     constexpr int CH = RB / 16;                  // chunks of a row
     constexpr int KI = KB / 4096;                // DMA instructions of a wave and operand
     constexpr int NK = DP / 32, ND = DP / 16;    // product steps over d; column tiles
-    constexpr int MB = 128;                      // tiles of a block of mask bits
-    typedef typename std::conditional<KT == 64, uint64_t, uint32_t>::type Bits;
+    constexpr int NQ = 2;                        // 16-row tiles of a wave
+    constexpr int MB = 128;                      // of 64 keys: a block of mask bits
     __shared__ __attribute__((aligned(1024))) uint8_t lds[STAGES * SB];
     __shared__ uint64_t bits[MASK ? 2 * MB : 1];
     const CrossTile t = cross_tile(a, BM, tiles, parts.parts);
@@ -75,7 +104,7 @@ __global__ __launch_bounds__(256, WGS) void cross_tile_kernel(CrossArgs a, int t
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l16 = lane & 15, g = lane >> 4;
     const uint32_t base = (uint32_t)(uintptr_t)lds;
-    const int row_w = wave * 16 * NQ;   // of the wave's first row in the tile
+    const int row_w = 32 * wave;   // of the wave's first row in the tile
 
     const int nk = __builtin_amdgcn_readfirstlane(t.s.nk);
     const int all = (nk + KT - 1) / KT;
@@ -95,24 +124,18 @@ __global__ __launch_bounds__(256, WGS) void cross_tile_kernel(CrossArgs a, int t
         vo[j] = cv * 8 < a.d ? (uint32_t)(r * vr) + cv * 16 : kOutside;
     }
     // keys of tile kt that count
-    auto valid_of = [&](int kt) -> Bits {
+    auto valid_of = [&](int kt) -> uint32_t {
         const int left = nk - kt * KT;
-        Bits v = left >= KT ? ~(Bits)0 : ((Bits)1 << left) - 1;
-        if constexpr (MASK) {
-            const uint32_t* m = (const uint32_t*)&bits[kt / (64 / KT) % (2 * MB)];
-            if constexpr (KT == 64)
-                v &= (uint64_t)__builtin_amdgcn_readfirstlane(m[0]) |
-                     (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane(m[1]) << 32;
-            else
-                v &= (uint32_t)__builtin_amdgcn_readfirstlane(m[kt & 1]);
-        }
+        uint32_t v = left >= KT ? ~0u : (1u << left) - 1;
+        if constexpr (MASK)
+            v &= (uint32_t)__builtin_amdgcn_readfirstlane(((const uint32_t*)&bits[kt / 2 % (2 * MB)])[kt & 1]);
         return v;
     };
-    // the mask of the next MB * 64 keys as bits, when the first tile of them is loaded
+    // the mask of the next 64 MB keys as bits, when the first tile of them is loaded
     auto read_mask = [&](int kt, bool first) {
         if constexpr (MASK) {
-            const int word = kt / (64 / KT);
-            if (!first && (word % MB != 0 || kt % (64 / KT) != 0)) return;
+            const int word = kt / 2;
+            if (!first && kt % (2 * MB) != 0) return;
             const uint8_t* mask = a.key_mask + t.s.b * a.mask_batch + t.s.k0;
             for (int w = word / MB * MB + wave; w < (word / MB + 1) * MB; w += 4) {
                 const int key = w * 64 + lane;
@@ -122,13 +145,17 @@ __global__ __launch_bounds__(256, WGS) void cross_tile_kernel(CrossArgs a, int t
             __syncthreads();
         }
     };
-    auto issue = [&](int kt, bool first) {
+    const char* next_k = kp + (long)kb * KT * kr;   // of the tile that is loaded next
+    const char* next_v = vp + (long)kb * KT * vr;
+    auto issue = [&](int kt, auto stage, bool first) {
         read_mask(kt, first);
-        const uint32_t st = base + (kt - kb) % STAGES * SB;
-        const i32x4 rk = wave_uniform(buffer_rsrc(kp + (long)kt * KT * kr, (uint32_t)((KT - 1) * kr + RB)));
-        const i32x4 rv = wave_uniform(buffer_rsrc(vp + (long)kt * KT * vr, (uint32_t)((KT - 1) * vr + RB)));
-        const Bits valid = valid_of(kt);
-        if (valid == ~(Bits)0) {
+        const uint32_t st = base + decltype(stage)::value * SB;
+        const i32x4 rk = wave_uniform(buffer_rsrc(next_k, (uint32_t)((KT - 1) * kr + RB)));
+        const i32x4 rv = wave_uniform(buffer_rsrc(next_v, (uint32_t)((KT - 1) * vr + RB)));
+        next_k += KT * kr;
+        next_v += KT * vr;
+        const uint32_t valid = valid_of(kt);
+        if (valid == ~0u) {
 #pragma unroll
             for (int j = 0; j < KI; ++j)
                 lds_dma16(rk, __builtin_amdgcn_readfirstlane(st + (wave * KI + j) * 1024), ko[j], 0);
@@ -145,11 +172,11 @@ __global__ __launch_bounds__(256, WGS) void cross_tile_kernel(CrossArgs a, int t
         }
     };
 
-#pragma unroll
-    for (int s = 0; s < STAGES - 1; ++s)
-        if (kb + s < ke) issue(kb + s, s == 0);
+    if (kb < ke) issue(kb, std::integral_constant<int, 0>{}, true);
+    if (STAGES > 2 && kb + 1 < ke) issue(kb + 1, std::integral_constant<int, 1>{}, false);
 
-    // q: row l16 of each 16, elements 32 kk + 8 g on; zeros past d and past the rows
+    // q: row l16 of each 16, elements 32 kk + 8 g on; zeros past d, the last row again past
+    // the rows
     const uint32_t sign = a.scale < 0.f ? 0x80008000u : 0u;
     // (not nought, by which a masked score of -inf would be NaN)
     const float c = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 0x1p-126f);
@@ -177,103 +204,118 @@ __global__ __launch_bounds__(256, WGS) void cross_tile_kernel(CrossArgs a, int t
     float m[NQ], l[NQ];   // l: of this lane's keys
 #pragma unroll
     for (int i = 0; i < NQ; ++i) m[i] = kLowest, l[i] = 0.f;
-    const int ksw = key_swizzle<DP>(l16);
-    const int vrow = 4 * g + (l16 >> 2);          // of the lane's piece of v, of 16 rows
-    const int vsw = value_swizzle<DP>(vrow);
-
-#pragma unroll 1
-    for (int kt = kb; kt < ke; ++kt) {
-        if (kt + 1 < ke) {
-            // tiles after this one may be in flight; STAGES is 3
-            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * KI) : "memory");
-        } else {
+    // unrolled by the stages, so that LDS addresses are registers and constants; 256 bytes
+    // further in a row the swizzles are the same
+    constexpr int KA = NK < 4 ? NK : 4, VA = ND < 8 ? ND : 8;
+    const uint8_t* kl[KA];
+#pragma unroll
+    for (int kk = 0; kk < KA; ++kk)
+        kl[kk] = lds + l16 * RB + (((4 * kk + g) ^ key_swizzle<DP>(l16)) * 16);
+    const int vrow = 4 * g + (l16 >> 2);   // of the lane's eight bytes of v, of 16 rows
+    const uint8_t* vl[VA];
+#pragma unroll
+    for (int dt = 0; dt < VA; ++dt)
+        vl[dt] = lds + KB + vrow * RB + (l16 & 1) * 8 + ((2 * dt + (l16 >> 1 & 1)) ^ value_swizzle<DP>(vrow)) * 16;
+    auto key = [&](int h, int kk, int st) {
+        return *(const uint4*)(kl[kk % KA] + (kk / KA * 256 + 16 * h * RB + st));
+    };
+    auto tile = [&](int kt, auto stage) {
+        constexpr int ST = decltype(stage)::value * SB;
+        if (kt + STAGES - 1 <= ke)   // the loads of STAGES - 2 later tiles may be in flight
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"((STAGES - 2) * 2 * KI) : "memory");
+        else
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        }
         __builtin_amdgcn_sched_barrier(0);
         asm volatile("s_barrier" ::: "memory");   // tile kt is there, tile kt - 1 no longer read
         __builtin_amdgcn_sched_barrier(0);
-        if (kt + STAGES - 1 < ke) issue(kt + STAGES - 1, false);
-        const Bits valid = valid_of(kt);
-        const uint8_t* st = lds + (kt - kb) % STAGES * SB;
+        // these reads' way is under the loads' issue (where registers are left for them)
+        constexpr int AHEAD = DP == 256 ? 0 : NK;
+        uint4 kf[2][NK];
 #pragma unroll
-        for (int u = 0; u < KT / 32; ++u) {
-            f32x4 s[2][NQ];
+        for (int kk = 0; kk < AHEAD; ++kk) kf[0][kk] = key(0, kk, ST);
+        asm volatile("" ::: "memory");
+        if (kt + STAGES - 1 < ke)
+            issue(kt + STAGES - 1, std::integral_constant<int, (decltype(stage)::value + STAGES - 1) % STAGES>{},
+                  false);
+        const uint32_t valid = valid_of(kt);
+        f32x4 s[2][NQ];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int kk = 0; kk < NK; ++kk) {
+                if (h || kk >= AHEAD) kf[h][kk] = key(h, kk, ST);
+#pragma unroll
+                for (int i = 0; i < NQ; ++i)
+                    s[h][i] = mfma<T>(kf[h][kk], qf[i][kk], kk ? s[h][i] : f32x4{0.f, 0.f, 0.f, 0.f});
+            }
+        // other waves' products run beside this wave's exponentials
+        __builtin_amdgcn_s_setprio(1);
+        if (valid != ~0u) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const uint8_t* kl = st + (32 * u + 16 * h + l16) * RB;
-                uint4 kf[NK];
+                const uint32_t v4 = valid >> (16 * h + 4 * g);
 #pragma unroll
-                for (int kk = 0; kk < NK; ++kk) kf[kk] = *(const uint4*)(kl + (((4 * kk + g) ^ ksw) * 16));
-#pragma unroll
-                for (int kk = 0; kk < NK; ++kk)
+                for (int r = 0; r < 4; ++r)
 #pragma unroll
                     for (int i = 0; i < NQ; ++i)
-                        s[h][i] = mfma<T>(kf[kk], qf[i][kk], kk ? s[h][i] : f32x4{0.f, 0.f, 0.f, 0.f});
-            }
-            if (valid != ~(Bits)0) {
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const uint32_t v4 = (uint32_t)(valid >> (32 * u + 16 * h)) >> (4 * g);
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-#pragma unroll
-                        for (int i = 0; i < NQ; ++i)
-                            if (!(v4 >> r & 1)) s[h][i][r] = -__builtin_inff();
-                }
-            }
-            float top[NQ];
-            bool due = false;
-#pragma unroll
-            for (int i = 0; i < NQ; ++i) {
-                float x = fmaxf(fmaxf(s[0][i][0], s[0][i][1]), s[0][i][2]);
-                x = fmaxf(fmaxf(x, s[0][i][3]), s[1][i][0]);
-                x = fmaxf(fmaxf(x, s[1][i][1]), s[1][i][2]);
-                top[i] = fmaxf(x, s[1][i][3]) * c;
-                due |= top[i] > m[i] + kLazy;
-            }
-            if (__any(due)) {
-#pragma unroll
-                for (int i = 0; i < NQ; ++i) {
-                    float x = top[i];
-                    x = fmaxf(x, __shfl_xor(x, 16));
-                    x = fmaxf(x, __shfl_xor(x, 32));
-                    x = fmaxf(x, m[i]);
-                    const float fade = __builtin_amdgcn_exp2f(m[i] - x);
-                    m[i] = x;
-                    l[i] *= fade;
-#pragma unroll
-                    for (int dt = 0; dt < ND; ++dt)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) o[dt][i][r] *= fade;
-                }
-            }
-            uint4 pb[NQ];
-#pragma unroll
-            for (int i = 0; i < NQ; ++i) {
-                float p[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    p[e] = __builtin_amdgcn_exp2f(fmaf(s[e >> 2][i][e & 3], c, kShift<T> - m[i]));
-                pb[i] = make_uint4(pack2<T>(p[0], p[1]), pack2<T>(p[2], p[3]), pack2<T>(p[4], p[5]),
-                                   pack2<T>(p[6], p[7]));
-                l[i] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
-            }
-            const uint8_t* vl = st + KB + (32 * u + vrow) * RB + (l16 & 1) * 8;
-#pragma unroll
-            for (int dt = 0; dt < ND; ++dt) {
-                const int at = ((2 * dt + (l16 >> 1 & 1)) ^ vsw) * 16;
-                const uint2 v0 = read_columns(vl + at), v1 = read_columns(vl + at + 16 * RB);
-                const uint4 vf = make_uint4(v0.x, v0.y, v1.x, v1.y);
-#pragma unroll
-                for (int i = 0; i < NQ; ++i) o[dt][i] = mfma<T>(vf, pb[i], o[dt][i]);
+                        if (!(v4 >> r & 1)) s[h][i][r] = -__builtin_inff();
             }
         }
+        float top[NQ];
+        bool due = false;
+#pragma unroll
+        for (int i = 0; i < NQ; ++i) {
+            float x = fmaxf(fmaxf(s[0][i][0], s[0][i][1]), s[0][i][2]);
+            x = fmaxf(fmaxf(x, s[0][i][3]), s[1][i][0]);
+            x = fmaxf(fmaxf(x, s[1][i][1]), s[1][i][2]);
+            top[i] = fmaxf(x, s[1][i][3]) * c;
+            due |= top[i] > m[i] + kLazy;
+        }
+        if (__any(due)) {
+#pragma unroll
+            for (int i = 0; i < NQ; ++i) {
+                const float x = fmaxf(max_groups(top[i]), m[i]);
+                const float fade = __builtin_amdgcn_exp2f(m[i] - x);
+                m[i] = x;
+                l[i] *= fade;
+#pragma unroll
+                for (int dt = 0; dt < ND; ++dt) o[dt][i] *= fade;
+            }
+        }
+        uint4 pb[NQ];
+#pragma unroll
+        for (int i = 0; i < NQ; ++i) {
+            const float shift = kShift<T> - m[i];
+            uint32_t w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                w[e] = pack2<T>(__builtin_amdgcn_exp2f(fmaf(s[e >> 1][i][2 * (e & 1)], c, shift)),
+                                __builtin_amdgcn_exp2f(fmaf(s[e >> 1][i][2 * (e & 1) + 1], c, shift)));
+            pb[i] = make_uint4(w[0], w[1], w[2], w[3]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) l[i] = add_pair<T>(w[e], l[i]);
+        }
+        __builtin_amdgcn_s_setprio(0);
+#pragma unroll
+        for (int dt = 0; dt < ND; ++dt) {
+            const uint8_t* p = vl[dt % VA] + (dt / VA * 256 + ST);
+            const uint2 v0 = read_columns(p), v1 = read_columns(p + 16 * RB);
+            const uint4 vf = make_uint4(v0.x, v0.y, v1.x, v1.y);
+#pragma unroll
+            for (int i = 0; i < NQ; ++i) o[dt][i] = mfma<T>(vf, pb[i], o[dt][i]);
+        }
+    };
+#pragma unroll 1
+    for (int kt = kb; kt < ke; kt += STAGES) {
+        tile(kt, std::integral_constant<int, 0>{});
+        if (kt + 1 < ke) tile(kt + 1, std::integral_constant<int, 1>{});
+        if constexpr (STAGES > 2)
+            if (kt + 2 < ke) tile(kt + 2, std::integral_constant<int, 2>{});
     }
 
 #pragma unroll
     for (int i = 0; i < NQ; ++i) {
-        l[i] += __shfl_xor(l[i], 16);
-        l[i] += __shfl_xor(l[i], 32);
+        l[i] = sum_groups(l[i]);
         const int r = row_w + 16 * i + l16;
         if (r >= t.rows) continue;
         if (parts.parts > 1) {
@@ -292,25 +334,21 @@ __global__ __launch_bounds__(256, WGS) void cross_tile_kernel(CrossArgs a, int t
     }
 }
 
-template <int T, int DP, int NQ, int KT, int STAGES, int WGS>
+template <int T, int DP, int STAGES, int WGS>
 hipError_t launch(const CrossArgs& a, int tiles, const CrossParts& parts, unsigned blocks, hipStream_t stream) {
-    static_assert(STAGES == 3, "the loop's waits");
     if (a.key_mask)
-        cross_tile_kernel<T, DP, NQ, KT, STAGES, WGS, true><<<blocks, 256, 0, stream>>>(a, tiles, parts);
+        cross_tile_kernel<T, DP, STAGES, WGS, true><<<blocks, 256, 0, stream>>>(a, tiles, parts);
     else
-        cross_tile_kernel<T, DP, NQ, KT, STAGES, WGS, false><<<blocks, 256, 0, stream>>>(a, tiles, parts);
+        cross_tile_kernel<T, DP, STAGES, WGS, false><<<blocks, 256, 0, stream>>>(a, tiles, parts);
     return hipGetLastError();
 }
 
 template <int T>
 hipError_t launch_t(const CrossArgs& a, const CrossPlan& p, const CrossParts& parts, hipStream_t stream) {
     const unsigned nb = (unsigned)((long)p.tiles * a.kv_heads * p.parts);
-    if (a.d > 128) return launch<T, 256, 2, 32, 3, 1>(a, p.tiles, parts, nb, stream);
-    if (a.d > 64)
-        return p.rows == 256 ? launch<T, 128, 4, 64, 3, 1>(a, p.tiles, parts, nb, stream)
-                             : launch<T, 128, 2, 32, 3, 3>(a, p.tiles, parts, nb, stream);
-    return p.rows == 256 ? launch<T, 64, 4, 64, 3, 2>(a, p.tiles, parts, nb, stream)
-                         : launch<T, 64, 2, 32, 3, 3>(a, p.tiles, parts, nb, stream);
+    if (a.d > 128) return launch<T, 256, 2, 2>(a, p.tiles, parts, nb, stream);
+    if (a.d > 64) return launch<T, 128, 3, 3>(a, p.tiles, parts, nb, stream);
+    return launch<T, 64, 3, 4>(a, p.tiles, parts, nb, stream);
 }
 
 }  // namespace
