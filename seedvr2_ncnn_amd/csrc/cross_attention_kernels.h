@@ -37,8 +37,7 @@ struct CrossArgs {
 
 // A call's kernel.  Rows: queries times the heads that share a kv head.
 struct CrossPlan {
-    int rows;     // of a tile
-    int tiles;    // of a kv head, at most
+    int tiles;    // of 128 rows of a kv head, at most
     int parts;    // ranges of keys
 };
 

@@ -1,5 +1,7 @@
 // Cross attention: softmax(scale q k^T) v per sample and head, keys of another length
 // than the queries.
+#include <cmath>
+
 #include "cross_attention_device.h"
 
 namespace s2 {
@@ -88,20 +90,45 @@ long all_rows(const CrossArgs& a) { return a.q_offsets ? (long)a.lq : (long)a.ba
 size_t part_bytes(const CrossArgs& a) { return (size_t)all_rows(a) * a.heads * (a.d * sizeof(float) + sizeof(float2)); }
 
 constexpr int kUnits = 256;   // compute units of an MI355X
+constexpr int kTileRows = 128, kTileKeys = 32;
+
+// Microseconds that a compute unit takes for a tile of keys with 1, 2, .. workgroups on it,
+// `each` at most, for d up to 64, 128 and 256: 4096 x 21600 with 20 heads of 128 in one
+// range of keys is three workgroups on half of the units and two on the others, 899 us; in
+// two ranges five in turn, 837.  1024 x 4096 96 us in one, 62 in three; 300 x 20000, two
+// heads, 429 and 37 in 32.
+struct CrossCost {
+    int each;
+    double us[4];
+};
+constexpr CrossCost kCrossCosts[] = {{4, {0.54, 0.7, 0.88, 1.1}}, {3, {0.7, 1.03, 1.43, 0.}}, {2, {1.45, 2.2, 0., 0.}}};
+constexpr double kJoinUs = 4., kJoinBytesUs = 6e6;   // the joining launch; bytes written and read
 
 CrossPlan cross_plan(const CrossArgs& a, size_t workspace_bytes) {
     const long group = a.heads / a.kv_heads;
-    auto tiles_of = [&](long each) {
-        return a.q_offsets ? (long)a.lq * group / each + std::min(a.batch, a.lq)
-                           : (long)a.batch * (((long)a.lq * group + each - 1) / each);
-    };
+    const long rows = (long)a.lq * group;
     CrossPlan p;
+    p.tiles = (int)std::min<long>(a.q_offsets ? rows / kTileRows + std::min(a.batch, a.lq)
+                                              : a.batch * ((rows + kTileRows - 1) / kTileRows),
+                                  0x7fffffffL);
+    // a sample's last tile is half empty, on average
+    const double blocks = a.kv_heads * (a.q_offsets ? (double)rows / kTileRows + 0.5 * std::min(a.batch, a.lq)
+                                                    : (double)p.tiles);
     const long keys = a.q_offsets ? ((long)a.lk + a.batch - 1) / std::max(a.batch, 1) : a.lk;   // of a sample
-    p.rows = 128;
-    p.tiles = (int)std::min<long>(tiles_of(p.rows), 0x7fffffffL);
-    const long blocks = (long)p.tiles * a.kv_heads;
+    const double tiles = (double)((keys + kTileKeys - 1) / kTileKeys);
     const long most = std::min<long>(64, (long)(workspace_bytes / part_bytes(a)));
-    p.parts = (int)std::max<long>(1, std::min({3 * kUnits / blocks, keys / 256, most}));
+    const CrossCost& c = kCrossCosts[a.d <= 64 ? 0 : a.d <= 128 ? 1 : 2];
+    double best = 0.;
+    p.parts = 1;
+    for (long parts = 1; parts <= std::max<long>(1, std::min<long>(most, (long)tiles / 2)); ++parts) {
+        const double all = blocks * parts, slots = (double)kUnits * c.each;
+        const double rest = all - std::floor(all / slots) * slots;
+        double us = std::floor(all / slots) * c.us[c.each - 1];
+        if (rest > 0) us += c.us[(int)std::ceil(rest / kUnits) - 1];
+        us *= std::ceil(tiles / parts);
+        if (parts > 1) us += kJoinUs + 2. * parts * part_bytes(a) / kJoinBytesUs;
+        if (parts == 1 || us < best) best = us, p.parts = (int)parts;
+    }
     return p;
 }
 
