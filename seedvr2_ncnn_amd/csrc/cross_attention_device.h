@@ -126,5 +126,121 @@ __device__ __forceinline__ void store4_out(const CrossArgs& a, long at, f32x4 v)
 }
 
 constexpr float kLowest = -3.4028234663852886e38f;   // the maximum of no scores
+constexpr float kLazy = 8.f;   // powers of two by which scores may pass m before it follows
+
+// Of the wave's four groups of 16 lanes.
+__device__ __forceinline__ float max_groups(float x) {
+    auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float sum_groups(float x) {
+    auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+constexpr int kMaskWords = 128;                // of 64 keys: a block of mask bits
+constexpr int kMaskBits = 2 * kMaskWords;      // two blocks in LDS
+
+// The tiles of k and v of a workgroup of four waves: DMA into STAGES stages of LDS, a tile of
+// k and then one of v of kTileKeys rows of DP elements of ES bytes each.  Chunk c (16 bytes)
+// of row r stands at c ^ Swizzle::key(r) or value(r).  Keys that do not count, by the
+// sample's length or the mask, and columns from d on are zeros, whatever is there.
+template <int ES, int DP, int STAGES, bool MASK, typename Swizzle>
+struct KeyTiles {
+    static constexpr int RB = DP * ES, KB = kTileKeys * RB, SB = 2 * KB;   // bytes: a row, a tile, a stage
+    static constexpr int CH = RB / 16;      // chunks of a row
+    static constexpr int KI = KB / 4096;    // DMA instructions of a wave and operand
+    int nk, wave;
+    uint32_t base;
+    uint64_t* bits;
+    const uint8_t* mask;
+    long kr, vr;                            // bytes between rows
+    const char* next_k;                     // of the tile that is loaded next
+    const char* next_v;
+    uint32_t ko[KI], vo[KI];
+
+    __device__ __forceinline__ KeyTiles(const CrossArgs& a, const CrossTile& t, int keys, int kb, uint32_t lds,
+                                        uint64_t* mask_bits)
+        : nk(keys), wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)), base(lds), bits(mask_bits),
+          mask(a.key_mask + t.s.b * a.mask_batch + t.s.k0), kr(a.ks.row * ES), vr(a.vs.row * ES) {
+        const long at = (long)kb * kTileKeys;
+        next_k = (const char*)a.k + (t.s.b * a.ks.batch + (t.s.k0 + at) * a.ks.row + t.head * a.ks.head) * ES;
+        next_v = (const char*)a.v + (t.s.b * a.vs.batch + (t.s.k0 + at) * a.vs.row + t.head * a.vs.head) * ES;
+#pragma unroll
+        for (int j = 0; j < KI; ++j) {
+            const int i = (wave * KI + j) * 64 + (threadIdx.x & 63);
+            const int r = i / CH, c = i % CH;
+            const int ck = c ^ Swizzle::key(r), cv = c ^ Swizzle::value(r);
+            ko[j] = ck * (16 / ES) < a.d ? (uint32_t)(r * kr) + ck * 16 : kOutside;
+            vo[j] = cv * (16 / ES) < a.d ? (uint32_t)(r * vr) + cv * 16 : kOutside;
+        }
+    }
+
+    // keys of tile kt that count
+    __device__ __forceinline__ uint32_t valid(int kt) const {
+        const int left = nk - kt * kTileKeys;
+        uint32_t v = left >= kTileKeys ? ~0u : (1u << left) - 1;
+        if constexpr (MASK)
+            v &= (uint32_t)__builtin_amdgcn_readfirstlane(((const uint32_t*)&bits[kt / 2 % kMaskBits])[kt & 1]);
+        return v;
+    }
+
+    // the next block of the mask as bits, when the first tile of it is loaded
+    __device__ __forceinline__ void read_mask(int kt, bool first) {
+        if constexpr (MASK) {
+            if (!first && kt % (2 * kMaskWords) != 0) return;
+            const int block = kt / 2 / kMaskWords * kMaskWords;
+            for (int w = block + wave; w < block + kMaskWords; w += 4) {
+                const int key = w * 64 + (threadIdx.x & 63);
+                const uint64_t m = __ballot(key < nk && mask[min(key, nk - 1)] != 0);
+                if ((threadIdx.x & 63) == 0) bits[w % kMaskBits] = m;
+            }
+            __syncthreads();
+        }
+    }
+
+    // Loads tile kt, the next one; all waves.
+    __device__ __forceinline__ void issue(int kt, int stage, bool first) {
+        read_mask(kt, first);
+        const uint32_t st = base + stage * SB;
+        const i32x4 rk = wave_uniform(buffer_rsrc(next_k, (uint32_t)((kTileKeys - 1) * kr + RB)));
+        const i32x4 rv = wave_uniform(buffer_rsrc(next_v, (uint32_t)((kTileKeys - 1) * vr + RB)));
+        next_k += kTileKeys * kr;
+        next_v += kTileKeys * vr;
+        const uint32_t keys = valid(kt);
+        if (keys == ~0u) {
+#pragma unroll
+            for (int j = 0; j < KI; ++j)
+                lds_dma16(rk, __builtin_amdgcn_readfirstlane(st + (wave * KI + j) * 1024), ko[j], 0);
+#pragma unroll
+            for (int j = 0; j < KI; ++j)
+                lds_dma16(rv, __builtin_amdgcn_readfirstlane(st + KB + (wave * KI + j) * 1024), vo[j], 0);
+        } else {
+#pragma unroll
+            for (int j = 0; j < KI; ++j) {
+                const int r = ((wave * KI + j) * 64 + (threadIdx.x & 63)) / CH;
+                const uint32_t out = keys >> r & 1 ? 0u : kOutside;
+                lds_dma16(rk, __builtin_amdgcn_readfirstlane(st + (wave * KI + j) * 1024), ko[j] | out, 0);
+                lds_dma16(rv, __builtin_amdgcn_readfirstlane(st + KB + (wave * KI + j) * 1024), vo[j] | out, 0);
+            }
+        }
+    }
+
+    // Until tile kt is there for all waves; those after it, STAGES - 2 of them at most, may be in
+    // flight.
+    __device__ __forceinline__ void await(int kt, int ke) const {
+        if (kt + STAGES - 1 <= ke)
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"((STAGES - 2) * 2 * KI) : "memory");
+        else
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("s_barrier" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+    }
+};
 
 }  // namespace s2

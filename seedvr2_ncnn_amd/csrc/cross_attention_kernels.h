@@ -35,6 +35,8 @@ struct CrossArgs {
     float scale;
 };
 
+constexpr int kTileRows = 128, kTileKeys = 32;   // of the 16-bit kernel; of every kernel
+
 // A call's kernel.  Rows: queries times the heads that share a kv head.
 struct CrossPlan {
     int tiles;    // of 128 rows of a kv head, at most

@@ -90,7 +90,6 @@ long all_rows(const CrossArgs& a) { return a.q_offsets ? (long)a.lq : (long)a.ba
 size_t part_bytes(const CrossArgs& a) { return (size_t)all_rows(a) * a.heads * (a.d * sizeof(float) + sizeof(float2)); }
 
 constexpr int kUnits = 256;   // compute units of an MI355X
-constexpr int kTileRows = 128, kTileKeys = 32;
 
 // Microseconds that a compute unit takes for a tile of keys with 1, 2, .. workgroups on it,
 // `each` at most, for d up to 64, 128 and 256: 4096 x 21600 with 20 heads of 128 in one

@@ -44,19 +44,15 @@ __device__ __forceinline__ uint2 read_columns(const uint8_t* p) {
 // 2^8 where a row's maximum is 8 past m.
 template <int T>
 constexpr float kShift = T == 2 ? 6.f : 0.f;
-constexpr float kLazy = 8.f;
 
 // A read of 16 bytes a lane is done 16 lanes at a time, one of 8 bytes 32 lanes, each 256
-// bytes on 64 banks.  Chunk c (16 bytes) of row r of a k tile stands at c ^ key_swizzle(r):
+// bytes on 64 banks.  Chunk c (16 bytes) of row r of a k tile stands at c ^ key(r):
 // 16 rows of one chunk lie on distinct banks.  Of v, eight rows of a pair of chunks do.
 template <int DP>
-__device__ __forceinline__ int key_swizzle(int r) {
-    return DP == 64 ? (r >> 1) & 7 : r & 15;
-}
-template <int DP>
-__device__ __forceinline__ int value_swizzle(int r) {
-    return DP == 64 ? ((r >> 1) & 3) * 2 : (r & 7) * 2;
-}
+struct Swizzle {
+    static __device__ __forceinline__ int key(int r) { return DP == 64 ? (r >> 1) & 7 : r & 15; }
+    static __device__ __forceinline__ int value(int r) { return DP == 64 ? ((r >> 1) & 3) * 2 : (r & 7) * 2; }
+};
 
 // Two weights' sum and l.
 template <int T>
@@ -70,110 +66,38 @@ __device__ __forceinline__ float add_pair(uint32_t p, float l) {
         return __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, p), __builtin_bit_cast(h2, 0x3c003c00u), l, false);
 }
 
-// Of the wave's four groups of 16 lanes.
-__device__ __forceinline__ float max_groups(float x) {
-    auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    x = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-    r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-__device__ __forceinline__ float sum_groups(float x) {
-    auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
-    r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-}
-
 // DP: d rounded up to 64, 128 or 256.  STAGES: of LDS; WGS: workgroups on a compute unit.
 template <int T, int DP, int STAGES, int WGS, bool MASK>
 __global__ __launch_bounds__(256, WGS) void cross_tile_kernel(CrossArgs a, int tiles, CrossParts parts) {
-    constexpr int KT = 32;                       // keys of a tile
-    constexpr int BM = 128;                      // rows of the workgroup
+    constexpr int KT = kTileKeys, BM = kTileRows;
     constexpr int RB = DP * 2;                   // bytes of a row in LDS
     constexpr int KB = KT * RB, SB = 2 * KB;     // a tile of k; a stage
-    constexpr int CH = RB / 16;                  // chunks of a row
-    constexpr int KI = KB / 4096;                // DMA instructions of a wave and operand
     constexpr int NK = DP / 32, ND = DP / 16;    // product steps over d; column tiles
     constexpr int NQ = 2;                        // 16-row tiles of a wave
-    constexpr int MB = 128;                      // of 64 keys: a block of mask bits
     __shared__ __attribute__((aligned(1024))) uint8_t lds[STAGES * SB];
-    __shared__ uint64_t bits[MASK ? 2 * MB : 1];
+    __shared__ uint64_t bits[MASK ? kMaskBits : 1];
     const CrossTile t = cross_tile(a, BM, tiles, parts.parts);
     if (t.rows <= 0) return;   // the whole workgroup
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l16 = lane & 15, g = lane >> 4;
-    const uint32_t base = (uint32_t)(uintptr_t)lds;
     const int row_w = 32 * wave;   // of the wave's first row in the tile
 
     const int nk = __builtin_amdgcn_readfirstlane(t.s.nk);
     const int all = (nk + KT - 1) / KT;
     const int kb = (int)((long)all * t.part / parts.parts), ke = (int)((long)all * (t.part + 1) / parts.parts);
 
-    // k and v: one descriptor a tile, from its first row on
-    const long kr = a.ks.row * 2, vr = a.vs.row * 2;
-    const char* kp = (const char*)a.k + (t.s.b * a.ks.batch + t.s.k0 * a.ks.row + t.head * a.ks.head) * 2;
-    const char* vp = (const char*)a.v + (t.s.b * a.vs.batch + t.s.k0 * a.vs.row + t.head * a.vs.head) * 2;
-    uint32_t ko[KI], vo[KI];
-#pragma unroll
-    for (int j = 0; j < KI; ++j) {
-        const int at = (wave * KI + j) * 64 + lane;
-        const int r = at / CH, c = at % CH;
-        const int ck = c ^ key_swizzle<DP>(r), cv = c ^ value_swizzle<DP>(r);
-        ko[j] = ck * 8 < a.d ? (uint32_t)(r * kr) + ck * 16 : kOutside;
-        vo[j] = cv * 8 < a.d ? (uint32_t)(r * vr) + cv * 16 : kOutside;
-    }
-    // keys of tile kt that count
-    auto valid_of = [&](int kt) -> uint32_t {
-        const int left = nk - kt * KT;
-        uint32_t v = left >= KT ? ~0u : (1u << left) - 1;
-        if constexpr (MASK)
-            v &= (uint32_t)__builtin_amdgcn_readfirstlane(((const uint32_t*)&bits[kt / 2 % (2 * MB)])[kt & 1]);
-        return v;
-    };
-    // the mask of the next 64 MB keys as bits, when the first tile of them is loaded
-    auto read_mask = [&](int kt, bool first) {
-        if constexpr (MASK) {
-            const int word = kt / 2;
-            if (!first && kt % (2 * MB) != 0) return;
-            const uint8_t* mask = a.key_mask + t.s.b * a.mask_batch + t.s.k0;
-            for (int w = word / MB * MB + wave; w < (word / MB + 1) * MB; w += 4) {
-                const int key = w * 64 + lane;
-                const uint64_t m = __ballot(key < nk && mask[min(key, nk - 1)] != 0);
-                if (lane == 0) bits[w % (2 * MB)] = m;
-            }
-            __syncthreads();
-        }
-    };
-    const char* next_k = kp + (long)kb * KT * kr;   // of the tile that is loaded next
-    const char* next_v = vp + (long)kb * KT * vr;
-    auto issue = [&](int kt, auto stage, bool first) {
-        read_mask(kt, first);
-        const uint32_t st = base + decltype(stage)::value * SB;
-        const i32x4 rk = wave_uniform(buffer_rsrc(next_k, (uint32_t)((KT - 1) * kr + RB)));
-        const i32x4 rv = wave_uniform(buffer_rsrc(next_v, (uint32_t)((KT - 1) * vr + RB)));
-        next_k += KT * kr;
-        next_v += KT * vr;
-        const uint32_t valid = valid_of(kt);
-        if (valid == ~0u) {
-#pragma unroll
-            for (int j = 0; j < KI; ++j)
-                lds_dma16(rk, __builtin_amdgcn_readfirstlane(st + (wave * KI + j) * 1024), ko[j], 0);
-#pragma unroll
-            for (int j = 0; j < KI; ++j)
-                lds_dma16(rv, __builtin_amdgcn_readfirstlane(st + KB + (wave * KI + j) * 1024), vo[j], 0);
-        } else {   // zeros for keys that do not count, whatever is there
-#pragma unroll
-            for (int j = 0; j < KI; ++j) {
-                const uint32_t out = valid >> (((wave * KI + j) * 64 + lane) / CH) & 1 ? 0u : kOutside;
-                lds_dma16(rk, __builtin_amdgcn_readfirstlane(st + (wave * KI + j) * 1024), ko[j] | out, 0);
-                lds_dma16(rv, __builtin_amdgcn_readfirstlane(st + KB + (wave * KI + j) * 1024), vo[j] | out, 0);
-            }
-        }
-    };
+    KeyTiles<2, DP, STAGES, MASK, Swizzle<DP>> kv(a, t, nk, kb, (uint32_t)(uintptr_t)lds, bits);
+    if (kb < ke) kv.issue(kb, 0, true);
+    if (STAGES > 2 && kb + 1 < ke) kv.issue(kb + 1, 1, false);
 
-    if (kb < ke) issue(kb, std::integral_constant<int, 0>{}, true);
-    if (STAGES > 2 && kb + 1 < ke) issue(kb + 1, std::integral_constant<int, 1>{}, false);
+    if (row_w >= t.rows) {   // a wave without rows takes part in loads and barriers alone
+        for (int kt = kb; kt < ke; ++kt) {
+            kv.await(kt, ke);
+            if (kt + STAGES - 1 < ke) kv.issue(kt + STAGES - 1, (kt - kb + STAGES - 1) % STAGES, false);
+        }
+        return;
+    }
 
     // q: row l16 of each 16, elements 32 kk + 8 g on; zeros past d, the last row again past
     // the rows
@@ -210,24 +134,18 @@ __global__ __launch_bounds__(256, WGS) void cross_tile_kernel(CrossArgs a, int t
     const uint8_t* kl[KA];
 #pragma unroll
     for (int kk = 0; kk < KA; ++kk)
-        kl[kk] = lds + l16 * RB + (((4 * kk + g) ^ key_swizzle<DP>(l16)) * 16);
+        kl[kk] = lds + l16 * RB + (((4 * kk + g) ^ Swizzle<DP>::key(l16)) * 16);
     const int vrow = 4 * g + (l16 >> 2);   // of the lane's eight bytes of v, of 16 rows
     const uint8_t* vl[VA];
 #pragma unroll
     for (int dt = 0; dt < VA; ++dt)
-        vl[dt] = lds + KB + vrow * RB + (l16 & 1) * 8 + ((2 * dt + (l16 >> 1 & 1)) ^ value_swizzle<DP>(vrow)) * 16;
+        vl[dt] = lds + KB + vrow * RB + (l16 & 1) * 8 + ((2 * dt + (l16 >> 1 & 1)) ^ Swizzle<DP>::value(vrow)) * 16;
     auto key = [&](int h, int kk, int st) {
         return *(const uint4*)(kl[kk % KA] + (kk / KA * 256 + 16 * h * RB + st));
     };
     auto tile = [&](int kt, auto stage) {
         constexpr int ST = decltype(stage)::value * SB;
-        if (kt + STAGES - 1 <= ke)   // the loads of STAGES - 2 later tiles may be in flight
-            asm volatile("s_waitcnt vmcnt(%0)" ::"n"((STAGES - 2) * 2 * KI) : "memory");
-        else
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __builtin_amdgcn_sched_barrier(0);
-        asm volatile("s_barrier" ::: "memory");   // tile kt is there, tile kt - 1 no longer read
-        __builtin_amdgcn_sched_barrier(0);
+        kv.await(kt, ke);   // and tile kt - 1 is no longer read
         // these reads' way is under the loads' issue (where registers are left for them)
         constexpr int AHEAD = DP == 256 ? 0 : NK;
         uint4 kf[2][NK];
@@ -235,9 +153,8 @@ __global__ __launch_bounds__(256, WGS) void cross_tile_kernel(CrossArgs a, int t
         for (int kk = 0; kk < AHEAD; ++kk) kf[0][kk] = key(0, kk, ST);
         asm volatile("" ::: "memory");
         if (kt + STAGES - 1 < ke)
-            issue(kt + STAGES - 1, std::integral_constant<int, (decltype(stage)::value + STAGES - 1) % STAGES>{},
-                  false);
-        const uint32_t valid = valid_of(kt);
+            kv.issue(kt + STAGES - 1, (decltype(stage)::value + STAGES - 1) % STAGES, false);
+        const uint32_t valid = kv.valid(kt);
         f32x4 s[2][NQ];
 #pragma unroll
         for (int h = 0; h < 2; ++h)
