@@ -66,6 +66,12 @@ __device__ __forceinline__ float add_pair(uint32_t p, float l) {
         return __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, p), __builtin_bit_cast(h2, 0x3c003c00u), l, false);
 }
 
+// Four values as out's 16-bit type.
+__device__ __forceinline__ u32x2 out4(const CrossArgs& a, f32x4 v) {
+    if (a.out_kind == 1) return u32x2{pack2_bf16_rne(v[0], v[1]), pack2_bf16_rne(v[2], v[3])};
+    return u32x2{pack2_f16_rne(v[0], v[1]), pack2_f16_rne(v[2], v[3])};
+}
+
 // DP: d rounded up to 64, 128 or 256.  STAGES: of LDS; WGS: workgroups on a compute unit.
 template <int T, int DP, int STAGES, int WGS, bool MASK>
 __global__ __launch_bounds__(256, WGS) void cross_tile_kernel(CrossArgs a, int tiles, CrossParts parts) {
@@ -234,7 +240,7 @@ __global__ __launch_bounds__(256, WGS) void cross_tile_kernel(CrossArgs a, int t
     for (int i = 0; i < NQ; ++i) {
         l[i] = sum_groups(l[i]);
         const int r = row_w + 16 * i + l16;
-        if (r >= t.rows) continue;
+        if (r >= t.rows) continue;   // (all four lanes of a row)
         if (parts.parts > 1) {
             const long at = cross_part(a, parts, t, t.row0 + r);
             if (g == 0) parts.weights[at] = make_float2(m[i], l[i]);
@@ -244,9 +250,27 @@ __global__ __launch_bounds__(256, WGS) void cross_tile_kernel(CrossArgs a, int t
         } else {
             const float scale = l[i] == 0.f ? 0.f : 1.f / l[i];
             const long at = cross_row(a, a.os, t, t.row0 + r);
+            if (a.out_kind == 0) {
 #pragma unroll
-            for (int dt = 0; dt < ND; ++dt)
-                if (16 * dt + 4 * g < a.d) store4_out(a, at + 16 * dt + 4 * g, o[dt][i] * scale);
+                for (int dt = 0; dt < ND; ++dt)
+                    if (16 * dt + 4 * g < a.d) store4_any<0>(a.out, at + 16 * dt + 4 * g, o[dt][i] * scale);
+            } else {
+                // two column tiles' values change lanes, so that a lane has eight neighbours
+#pragma unroll
+                for (int dt = 0; dt < ND; dt += 2) {
+                    u32x2 x = out4(a, o[dt][i] * scale), y = out4(a, o[dt + 1][i] * scale);
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        auto w = __builtin_amdgcn_permlane32_swap(x[e], y[e], false, false);
+                        w = __builtin_amdgcn_permlane16_swap(w[0], w[1], false, false);
+                        x[e] = w[0];
+                        y[e] = w[1];
+                    }
+                    const int col = 16 * (dt + (g >> 1)) + 8 * (g & 1);
+                    if (col < a.d)
+                        *reinterpret_cast<u32x4_at2*>((uint16_t*)a.out + at + col) = u32x4{x[0], x[1], y[0], y[1]};
+                }
+            }
         }
     }
 }
