@@ -1647,7 +1647,7 @@ int s2_cross_attention(const s2_cross_attention_shape* shape, const void* q, con
         const s2::CrossRows& r = *rows[i];
         if (r.batch * e % 16 || r.row * e % 16 || r.head * e % 16)
             return fail(S2_ERR_INVALID, "strides of q, k and v must be multiples of 16 bytes");
-        if (i > 0 && r.row > 1 << 23)   // 32-bit offsets in a tile of keys
+        if (i > 0 && i < 3 && r.row > 1 << 23)   // 32-bit offsets in a tile of keys
             return fail(S2_ERR_INVALID, "row strides of k and v are at most 2^23");
     }
     if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(out, oe) ||

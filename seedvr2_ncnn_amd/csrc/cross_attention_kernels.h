@@ -2,7 +2,8 @@
 // elements.
 //
 //   cross_attention_kernels.hip  which kernel takes a call; the joining of ranges of keys
-//   cross_tile_kernels.hip       16-bit operands, tiles of rows
+//   cross_tile_kernels.hip       16-bit operands
+//   cross_f32_kernels.hip        fp32 operands
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -35,11 +36,12 @@ struct CrossArgs {
     float scale;
 };
 
-constexpr int kTileRows = 128, kTileKeys = 32;   // of the 16-bit kernel; of every kernel
+constexpr int kTileRows = 128, kTileRows32 = 64;   // of 16-bit operands' tiles, of fp32 ones'
+constexpr int kTileKeys = 32;
 
 // A call's kernel.  Rows: queries times the heads that share a kv head.
 struct CrossPlan {
-    int tiles;    // of 128 rows of a kv head, at most
+    int tiles;    // of rows of a kv head, at most
     int parts;    // ranges of keys
 };
 
@@ -53,6 +55,7 @@ struct CrossParts {
 
 CrossParts cross_parts(const CrossArgs& a, const CrossPlan& plan, void* workspace);
 hipError_t launch_cross_tiles(const CrossArgs& a, const CrossPlan& plan, void* workspace, hipStream_t stream);
+hipError_t launch_cross_f32(const CrossArgs& a, const CrossPlan& plan, void* workspace, hipStream_t stream);
 
 size_t cross_attention_workspace(const CrossArgs& a);
 hipError_t launch_cross_attention(const CrossArgs& a, void* workspace, size_t workspace_bytes,

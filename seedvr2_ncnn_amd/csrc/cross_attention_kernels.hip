@@ -8,81 +8,78 @@ namespace s2 {
 
 namespace {
 
-// A wave a query and head, a lane every 64th element of d, key after key with the running
-// maximum and sum.
-__global__ __launch_bounds__(256) void cross_any_kernel(CrossArgs a) {
-    const long item = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63;
-    const int h = (int)(item % a.heads);
-    long i = item / a.heads;
-    int b;
-    long q0 = 0, k0 = 0, keys = a.lk;
-    if (a.q_offsets) {
-        if (i >= a.lq) return;
-        for (b = 0; b < a.batch; ++b)
-            if (i >= a.q_offsets[b] && i < a.q_offsets[b + 1]) break;
-        if (b == a.batch) return;
-        k0 = min(max(a.k_offsets[b], 0), a.lk);
-        keys = min(max(a.k_offsets[b + 1], 0), a.lk) - k0;
-    } else {
-        if (i >= (long)a.batch * a.lq) return;
-        b = (int)(i / a.lq);
-        i -= (long)b * a.lq;
-        if (a.key_lengths) keys = min(max(a.key_lengths[b], 0), a.lk);
+constexpr int kJoinFew = 4;
+
+// Four columns of a row a thread, for few parts: their sums, by how far their maxima lie
+// below the largest.
+__global__ __launch_bounds__(256) void cross_join_few_kernel(CrossArgs a, CrossParts p, long rows) {
+    const int quads = a.d / 4;
+    const long i = (long)blockIdx.x * 256 + threadIdx.x;
+    if (i >= rows * a.heads * quads) return;
+    const long rh = i / quads;
+    const int col = (int)(i - rh * quads) * 4;
+    const long row = rh / a.heads;
+    const int h = (int)(rh - row * a.heads);
+    // rows in no sample
+    if (a.q_offsets && (row < clamped(a.q_offsets[0], a.lq) || row >= clamped(a.q_offsets[a.batch], a.lq))) return;
+    float2 w[kJoinFew];
+    f32x4 o[kJoinFew];
+#pragma unroll
+    for (int q = 0; q < kJoinFew; ++q) {
+        const long at = rh * p.parts + min(q, p.parts - 1);
+        w[q] = p.weights[at];
+        o[q] = *reinterpret_cast<const f32x4*>(p.sums + at * a.d + col);
     }
-    const int hk = h / (a.heads / a.kv_heads);
-    const long qa = b * a.qs.batch + (q0 + i) * a.qs.row + h * a.qs.head;
-    float q[4], o[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int e = 0; e < 4; ++e) q[e] = lane + 64 * e < a.d ? load1(a.q, qa + lane + 64 * e, a.kind) : 0.f;
-    float m = -__builtin_inff(), l = 0.f;
-    for (long j = 0; j < keys; ++j) {
-        if (a.key_mask && !a.key_mask[b * a.mask_batch + k0 + j]) continue;
-        const long ka = b * a.ks.batch + (k0 + j) * a.ks.row + hk * a.ks.head;
-        const long va = b * a.vs.batch + (k0 + j) * a.vs.row + hk * a.vs.head;
-        float s = 0.f;
-        for (int e = 0; e < 4; ++e)
-            if (lane + 64 * e < a.d) s += q[e] * load1(a.k, ka + lane + 64 * e, a.kind);
-        for (int x = 1; x < 64; x <<= 1) s += __shfl_xor(s, x);
-        s *= a.scale;
-        const float top = fmaxf(m, s);
-        const float fade = m == top ? 1.f : expf(m - top);
-        const float p = expf(s - (top == -__builtin_inff() ? 0.f : top));
-        m = top;
-        l = l * fade + p;
-        for (int e = 0; e < 4; ++e)
-            if (lane + 64 * e < a.d) o[e] = o[e] * fade + p * load1(a.v, va + lane + 64 * e, a.kind);
+    float m = w[0].x, l = 0.f;
+#pragma unroll
+    for (int q = 1; q < kJoinFew; ++q) m = fmaxf(m, w[q].x);
+    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int q = 0; q < kJoinFew; ++q) {
+        if (q >= p.parts) break;
+        const float f = __builtin_amdgcn_exp2f(w[q].x - m);
+        l += f * w[q].y;
+        sum += f * o[q];
     }
-    const long oa = b * a.os.batch + (q0 + i) * a.os.row + h * a.os.head;
-    for (int e = 0; e < 4; ++e)
-        if (lane + 64 * e < a.d) store1(a.out, oa + lane + 64 * e, l == 0.f ? 0.f : o[e] / l, a.out_kind);
+    const long b = a.q_offsets ? 0 : row / a.lq;
+    store4_out(a, b * a.os.batch + (row - b * a.lq) * a.os.row + h * a.os.head + col,
+               sum * (l == 0.f ? 0.f : 1.f / l));
 }
 
-// Four columns of a row a thread: its parts' sums, by how far their maxima lie below the
-// largest.
-__global__ __launch_bounds__(256) void cross_join_kernel(CrossArgs a, CrossParts p, long rows) {
-    const int quads = a.d / 4;
-    const long first = a.q_offsets ? clamped(a.q_offsets[0], a.lq) : 0;
-    const long end = a.q_offsets ? clamped(a.q_offsets[a.batch], a.lq) : rows;
-    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < rows * a.heads * quads; i += (long)gridDim.x * 256) {
-        const long rh = i / quads;
-        const int col = (int)(i - rh * quads) * 4;
-        const long row = rh / a.heads;
-        const int h = (int)(rh - row * a.heads);
-        if (row < first || row >= end) continue;   // in no sample
-        const float2* w = p.weights + rh * p.parts;
-        float m = kLowest;
-        for (int q = 0; q < p.parts; ++q) m = fmaxf(m, w[q].x);
-        float l = 0.f;
-        f32x4 o = {0.f, 0.f, 0.f, 0.f};
-        for (int q = 0; q < p.parts; ++q) {
-            const float f = __builtin_amdgcn_exp2f(w[q].x - m);
-            l += f * w[q].y;
-            o += f * *reinterpret_cast<const f32x4*>(p.sums + (rh * p.parts + q) * a.d + col);
-        }
-        const long b = a.q_offsets ? 0 : row / a.lq;
-        const long at = b * a.os.batch + (row - b * a.lq) * a.os.row + h * a.os.head + col;
-        store4_out(a, at, o * (l == 0.f ? 0.f : 1.f / l));
+// The same for many parts, a wave a row and head.
+// `lanes` lanes (a power of two, at least d / 4) have four columns each, and every 64 /
+// lanes-th part.
+__global__ __launch_bounds__(256) void cross_join_kernel(CrossArgs a, CrossParts p, long rows, int lanes) {
+    const long rh = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (rh >= rows * a.heads) return;
+    const long row = rh / a.heads;
+    const int h = (int)(rh - row * a.heads);
+    // rows in no sample
+    if (a.q_offsets && (row < clamped(a.q_offsets[0], a.lq) || row >= clamped(a.q_offsets[a.batch], a.lq))) return;
+    const int lane = threadIdx.x & 63;
+    const float2 w = lane < p.parts ? p.weights[rh * p.parts + lane] : make_float2(kLowest, 0.f);
+    float m = w.x;
+#pragma unroll
+    for (int x = 32; x; x >>= 1) m = fmaxf(m, __shfl_xor(m, x));
+    const float f = __builtin_amdgcn_exp2f(w.x - m);
+    float l = f * w.y;
+#pragma unroll
+    for (int x = 32; x; x >>= 1) l += __shfl_xor(l, x);
+    const int col = (lane & (lanes - 1)) * 4, step = 64 / lanes;
+    const float* sums = p.sums + rh * p.parts * a.d + min(col, a.d - 4);
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int q0 = 0; q0 < p.parts; q0 += step) {
+        const int q = q0 + lane / lanes;   // (parts past the last one have weight 0)
+        const float fq = __shfl(f, min(q, 63));
+        if (q < p.parts) o += fq * *reinterpret_cast<const f32x4*>(sums + (long)q * a.d);
     }
+    for (int x = lanes; x < 64; x <<= 1)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] += __shfl_xor(o[e], x);
+    if (lane >= lanes || col >= a.d) return;
+    const long b = a.q_offsets ? 0 : row / a.lq;
+    store4_out(a, b * a.os.batch + (row - b * a.lq) * a.os.row + h * a.os.head + col, o * (l == 0.f ? 0.f : 1.f / l));
 }
 
 long all_rows(const CrossArgs& a) { return a.q_offsets ? (long)a.lq : (long)a.batch * a.lq; }
@@ -100,23 +97,26 @@ struct CrossCost {
     int each;
     double us[4];
 };
-constexpr CrossCost kCrossCosts[] = {{4, {0.54, 0.7, 0.88, 1.1}}, {3, {0.7, 1.03, 1.43, 0.}}, {2, {1.45, 2.2, 0., 0.}}};
+constexpr CrossCost kCrossCosts[2][3] = {
+    {{4, {0.54, 0.7, 0.88, 1.1}}, {3, {0.7, 1.03, 1.43, 0.}}, {2, {1.45, 2.2, 0., 0.}}},
+    {{4, {1.3, 2., 2.7, 3.5}}, {2, {2.5, 3.7, 0., 0.}}, {1, {5., 0., 0., 0.}}}};   // fp32
 constexpr double kJoinUs = 4., kJoinBytesUs = 6e6;   // the joining launch; bytes written and read
 
 CrossPlan cross_plan(const CrossArgs& a, size_t workspace_bytes) {
     const long group = a.heads / a.kv_heads;
     const long rows = (long)a.lq * group;
+    const int each = a.kind ? kTileRows : kTileRows32;
     CrossPlan p;
-    p.tiles = (int)std::min<long>(a.q_offsets ? rows / kTileRows + std::min(a.batch, a.lq)
-                                              : a.batch * ((rows + kTileRows - 1) / kTileRows),
+    p.tiles = (int)std::min<long>(a.q_offsets ? rows / each + std::min(a.batch, a.lq)
+                                              : a.batch * ((rows + each - 1) / each),
                                   0x7fffffffL);
     // a sample's last tile is half empty, on average
-    const double blocks = a.kv_heads * (a.q_offsets ? (double)rows / kTileRows + 0.5 * std::min(a.batch, a.lq)
+    const double blocks = a.kv_heads * (a.q_offsets ? (double)rows / each + 0.5 * std::min(a.batch, a.lq)
                                                     : (double)p.tiles);
     const long keys = a.q_offsets ? ((long)a.lk + a.batch - 1) / std::max(a.batch, 1) : a.lk;   // of a sample
     const double tiles = (double)((keys + kTileKeys - 1) / kTileKeys);
     const long most = std::min<long>(64, (long)(workspace_bytes / part_bytes(a)));
-    const CrossCost& c = kCrossCosts[a.d <= 64 ? 0 : a.d <= 128 ? 1 : 2];
+    const CrossCost& c = kCrossCosts[a.kind == 0][a.d <= 64 ? 0 : a.d <= 128 ? 1 : 2];
     double best = 0.;
     p.parts = 1;
     for (long parts = 1; parts <= std::max<long>(1, std::min<long>(most, (long)tiles / 2)); ++parts) {
@@ -140,7 +140,6 @@ CrossParts cross_parts(const CrossArgs& a, const CrossPlan& plan, void* workspac
 }
 
 size_t cross_attention_workspace(const CrossArgs& a) {
-    if (a.kind == 0) return 0;
     const CrossPlan p = cross_plan(a, (size_t)1 << 62);
     return p.parts > 1 ? p.parts * part_bytes(a) : 0;
 }
@@ -149,19 +148,20 @@ hipError_t launch_cross_attention(const CrossArgs& a, void* workspace, size_t wo
                                   hipStream_t stream) {
     const long rows = all_rows(a);
     if (rows <= 0) return hipSuccess;
-    if (a.kind) {
-        const CrossPlan p = cross_plan(a, workspace_bytes);
-        if ((long)p.tiles * a.kv_heads * p.parts > 0x7fffffffL) return hipErrorInvalidValue;
-        const hipError_t e = launch_cross_tiles(a, p, workspace, stream);
-        if (e != hipSuccess || p.parts == 1) return e;
-        const long all = rows * a.heads * (a.d / 4);
-        cross_join_kernel<<<(unsigned)std::min<long>((all + 255) / 256, 8192), 256, 0, stream>>>(
-            a, cross_parts(a, p, workspace), rows);
-        return hipGetLastError();
-    }
-    const long blocks = (rows * a.heads + 3) / 4;
+    const CrossPlan p = cross_plan(a, workspace_bytes);
+    if ((long)p.tiles * a.kv_heads * p.parts > 0x7fffffffL) return hipErrorInvalidValue;
+    const hipError_t e = a.kind ? launch_cross_tiles(a, p, workspace, stream) : launch_cross_f32(a, p, workspace, stream);
+    if (e != hipSuccess || p.parts == 1) return e;
+    int lanes = 2;
+    while (lanes * 4 < a.d) lanes *= 2;
+    const CrossParts parts = cross_parts(a, p, workspace);
+    const bool few = p.parts <= kJoinFew;
+    const long blocks = few ? (rows * a.heads * (a.d / 4) + 255) / 256 : (rows * a.heads + 3) / 4;
     if (blocks > 0x7fffffffL) return hipErrorInvalidValue;
-    cross_any_kernel<<<(unsigned)blocks, 256, 0, stream>>>(a);
+    if (few)
+        cross_join_few_kernel<<<(unsigned)blocks, 256, 0, stream>>>(a, parts, rows);
+    else
+        cross_join_kernel<<<(unsigned)blocks, 256, 0, stream>>>(a, parts, rows, lanes);
     return hipGetLastError();
 }
 
