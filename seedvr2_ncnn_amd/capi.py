@@ -934,49 +934,58 @@ class MxRows(NamedTuple):
 
 def _mx_rows(rows, name):
     """Checks MxRows; returns (row count, codes' and scales' row strides)."""
-    import torch
     codes, scales, k = rows
-    blocks = (k + 31) // 32
-    if k < 1 or k > _INT_MAX:
+    if not 1 <= k <= _INT_MAX:
         _refuse(name, "k is out of range")
-    if (codes.dtype is not torch.uint8 or scales.dtype is not torch.uint8 or codes.dim() != 2 or
-            scales.dim() != 2 or codes.shape[1] != 16 * blocks or scales.shape[1] != blocks or
-            codes.shape[0] != scales.shape[0]):
+    blocks = (k + 31) // 32
+    shape = codes.shape
+    if (len(shape) != 2 or shape[1] != 16 * blocks or scales.shape != (shape[0], blocks) or
+            codes.dtype is not _uint8() or scales.dtype is not _uint8()):
         raise ValueError(f"{name}: codes must be uint8 [rows, {16 * blocks}], scales [rows, {blocks}]")
     cs, step = codes.stride()
     ss, sstep = scales.stride()
     if step != 1 or (blocks > 1 and sstep != 1):
         raise ValueError(f"{name}: codes and scales must have contiguous rows")
-    if codes.shape[0] > _INT_MAX:
+    if shape[0] > _INT_MAX:
         _refuse(name, "a size is out of range")
-    return codes.shape[0], cs, ss
+    return shape[0], cs, ss
 
 
-def _mx_empty(m, k, x, stream):
-    """Uninitialised MxRows whose scale rows are a multiple of 16 bytes apart."""
+@functools.lru_cache(maxsize=1)
+def _uint8():
     import torch
-    blocks = (k + 31) // 32
-    scales = _empty((m, (blocks + 15) // 16 * 16), torch.uint8, x, stream)
-    return MxRows(_empty((m, 16 * blocks), torch.uint8, x, stream), scales[:, :blocks], k)
+    return torch.uint8
 
 
 def mx_quantize(x, out=None, stream=None):
     """s2_mx_quantize: rows x [m, k] (strided, elements contiguous) as MxRows, into out if
-    given."""
-    if x.dim() != 2 or (x.shape[1] > 1 and x.stride(1) != 1):
+    given; else into rows of codes and scales that begin at multiples of 16 bytes."""
+    shape = x.shape
+    if len(shape) != 2:
         raise ValueError("x must be [m, k] with contiguous rows")
-    m, k = x.shape
-    if m > _INT_MAX or k > _INT_MAX:
+    m, k = shape
+    xs, step = x.stride()
+    if k > 1 and step != 1:
+        raise ValueError("x must be [m, k] with contiguous rows")
+    if m > _INT_MAX or not 1 <= k <= _INT_MAX:
         _refuse("mx_quantize", "a size is out of range")
     xd = _dtype_code(x)
     if out is None:
-        out = _mx_empty(m, k, x, stream)
-    elif out.k != k or out.codes.shape[0] != m:
-        raise ValueError("x and out must be of one shape")
-    _, cs, ss = _mx_rows(out, "mx_quantize")
-    handle = _raw_stream(x, stream, out.codes, out.scales)
-    check(lib().s2_mx_quantize(x.data_ptr(), xd, x.stride(0), m, k, out.codes.data_ptr(), cs,
-                               out.scales.data_ptr(), ss, handle), "s2_mx_quantize")
+        # scales behind the codes, in one piece of memory
+        blocks = (k + 31) // 32
+        cs, ss = 16 * blocks, (blocks + 15) // 16 * 16
+        both = _empty(m * (cs + ss), _uint8(), x, stream)
+        out = MxRows(both.as_strided((m, cs), (cs, 1)), both.as_strided((m, blocks), (ss, 1), m * cs), k)
+        codes = both.data_ptr()
+        scales = codes + m * cs
+        handle = _raw_stream(x, stream)
+    else:
+        if out.k != k or out.codes.shape[0] != m:
+            raise ValueError("x and out must be of one shape")
+        _, cs, ss = _mx_rows(out, "mx_quantize")
+        codes, scales = out.codes.data_ptr(), out.scales.data_ptr()
+        handle = _raw_stream(x, stream, out.codes, out.scales)
+    check(lib().s2_mx_quantize(x.data_ptr(), xd, xs, m, k, codes, cs, scales, ss, handle), "s2_mx_quantize")
     return out
 
 

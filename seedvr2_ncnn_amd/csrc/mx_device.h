@@ -37,33 +37,23 @@ __device__ __forceinline__ uint4 mx_bf16(uint32_t codes, float scale) {
         __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 3)));
 }
 
-// Eight consecutive k of a row as bf16 terms whose sum is exact, zeros from `left` on: an
-// fp16 value has 11 bits, two terms of eight.
-template <int XK, int TERMS>
-__device__ __forceinline__ void mx_terms(const void* x, long at, int left, uint4 (&t)[TERMS]) {
-    if constexpr (XK == 1) {
-        t[0] = piece16<false>((const uint16_t*)x + at, left);
-    } else if constexpr (XK == 0) {
-        float v[8];
-        piece32<false>((const float*)x + at, left, v);
-        split8(v, t);
-    } else {
-        const uint4 q = piece16<false>((const uint16_t*)x + at, left);
-        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-        uint32_t hi[4], lo[4];
+// Eight fp16 values as two bf16 terms each, whose sum is exact: 11 bits, by truncation the
+// first eight and the rest.
+__device__ __forceinline__ void mx_terms16(uint4 v, uint4 (&t)[2]) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    uint32_t hi[4], lo[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float v0 = (float)__builtin_bit_cast(_Float16, (uint16_t)w[e]);
-            const float v1 = (float)__builtin_bit_cast(_Float16, (uint16_t)(w[e] >> 16));
-            const uint32_t b0 = __float_as_uint(v0) & 0xffff0000u, b1 = __float_as_uint(v1) & 0xffff0000u;
-            hi[e] = (b0 >> 16) | b1;
-            // an infinity stays in the first term, a NaN's payload lies in its upper bits
-            lo[e] = pack2_bf16_rne(fabsf(v0) == __builtin_inff() ? 0.f : v0 - __uint_as_float(b0),
-                                   fabsf(v1) == __builtin_inff() ? 0.f : v1 - __uint_as_float(b1));
-        }
-        t[0] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        t[1] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    for (int e = 0; e < 4; ++e) {
+        const float v0 = (float)__builtin_bit_cast(_Float16, (uint16_t)w[e]);
+        const float v1 = (float)__builtin_bit_cast(_Float16, (uint16_t)(w[e] >> 16));
+        const uint32_t b0 = __float_as_uint(v0) & 0xffff0000u, b1 = __float_as_uint(v1) & 0xffff0000u;
+        hi[e] = (b0 >> 16) | b1;
+        // an infinity stays in the first term, a NaN's payload lies in its upper bits
+        lo[e] = pack2_bf16_rne(fabsf(v0) == __builtin_inff() ? 0.f : v0 - __uint_as_float(b0),
+                               fabsf(v1) == __builtin_inff() ? 0.f : v1 - __uint_as_float(b1));
     }
+    t[0] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+    t[1] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
 }
 
 }  // namespace s2

@@ -7,46 +7,91 @@ namespace s2 {
 
 namespace {
 
-// x as the matrix cores take it: codes (XT 0), or a sum of bf16 terms that holds it exactly
-// (bf16: one, fp16: two, fp32: three) against weights as bf16, which hold a code times
-// its scale exactly.
+// A block of x as it is loaded, and eight k of it as the matrix cores take them: codes (XT
+// 0), or a sum of bf16 terms that holds it exactly (bf16: one, fp16: two, fp32: three)
+// against weights as bf16, which hold a code times its scale exactly.  XT: 0 MXFP4, else 1
+// + x's kind.
 template <int XT>
-constexpr int kXTerms = XT == 0 ? 1 : XT == S2_DTYPE_BF16 + 1 ? 1 : XT == S2_DTYPE_F16 + 1 ? 2 : 3;
+struct MxX {   // 16-bit rows
+    static constexpr int TERMS = XT - 1;
+    struct Block {
+        uint4 v[4];
+    };
+    static __device__ __forceinline__ void load(const MxLinearArgs& a, long row, int block, bool, Block& x) {
+        const uint16_t* p = (const uint16_t*)a.x + row * a.x_stride + 32L * block;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x.v[e] = piece16<false>(p + 8 * e, a.k - 32 * block - 8 * e);
+    }
+    static __device__ __forceinline__ void terms(uint4 v, uint4 (&t)[TERMS]) {
+        if constexpr (TERMS == 1)
+            t[0] = v;
+        else
+            mx_terms16(v, t);
+    }
+    // eight k from `at` on
+    static __device__ __forceinline__ void terms_of(const MxLinearArgs& a, long row, int at, uint4 (&t)[TERMS]) {
+        terms(piece16<false>((const uint16_t*)a.x + row * a.x_stride + at, a.k - at), t);
+    }
+};
+template <>
+struct MxX<0> {
+    static constexpr int TERMS = 1;
+    struct Block {
+        uint4 codes;
+        uint32_t scale;
+    };
+    static __device__ __forceinline__ void load(const MxLinearArgs& a, long row, int block, bool in, Block& x) {
+        const int at = in ? block : 0;
+        x.codes = *reinterpret_cast<const uint4*>(a.xq.codes + row * a.xq.code_stride + 16 * at);
+        x.scale = a.xq.scales[row * a.xq.scale_stride + at];
+        if (!in) x.codes = make_uint4(0, 0, 0, 0), x.scale = 127;
+    }
+};
+template <>
+struct MxX<1> {   // fp32, split by way of LDS alone
+    static constexpr int TERMS = kTerms;
+    struct Block {};
+    static __device__ __forceinline__ void terms_of(const MxLinearArgs& a, long row, int at, uint4 (&t)[TERMS]) {
+        float v[8];
+        piece32<false>((const float*)a.x + row * a.x_stride + at, a.k - at, v);
+        split8(v, t);
+    }
+};
 
-// Up to 16 MT rows by 16 NT columns a workgroup of up to eight waves.  What costs is
-// reading the weight: every wave takes every other 256 k (128 bytes of each weight row)
-// straight into operand registers, the next ones in flight under the products; x comes
-// from the caches.  The waves' sums meet in LDS.  Lane (row l16, group g) holds blocks 2 g
-// and 2 g + 1 of the 256 k, of both operands; rows and columns past the end repeat the
-// last one, and are dropped.  XT: 0 MXFP4, else 1 + x's kind.
-template <int XT, int MT, int NT>
-__global__ __launch_bounds__(512) void mx_rows_kernel(MxLinearArgs a, int ntiles) {
-    constexpr int TERMS = kXTerms<XT>;
-    __shared__ float sums[8][MT * NT * 256];
-    const int row0 = blockIdx.x / ntiles * 16 * MT;
+// Up to 16 rows by 16 NT columns a workgroup of up to eight waves.  What costs is reading
+// the weight: every wave takes every other 256 k (128 bytes of each weight row) straight
+// into operand registers, the next ones in flight under the products.  Lane (row l16, group
+// g) holds blocks 2 g and 2 g + 1 of the 256 k, of both operands; rows and columns past the
+// end repeat the last one, and are dropped.  The waves' sums meet in LDS.
+//
+// SPLIT: x is split into its terms once a workgroup, `span` k at a time, which LDS holds (1 x
+// 2560 in fp32 by 15360 x 2560 8.5 us, 18 with each wave splitting what it takes); else each
+// wave loads its x with the weight.
+template <int XT, int NT, bool SPLIT>
+__global__ __launch_bounds__(512) void mx_rows_kernel(MxLinearArgs a, int ntiles, int span) {
+    typedef MxX<XT> X;
+    __shared__ float sums[8][NT * 256];
+    extern __shared__ __attribute__((aligned(16))) uint16_t split[];   // [TERMS][rows][span]
+    const int row0 = blockIdx.x / ntiles * 16;
     const int col0 = blockIdx.x % ntiles * 16 * NT;
-    const int rows = min(a.m - row0, 16 * MT);
+    const int rows = min(a.m - row0, 16);
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int waves = blockDim.x >> 6;
     const int l16 = lane & 15, g = lane >> 4;
     const int blocks = mx_blocks(a.k);
-    long wrow[NT], xrow[MT];
+    const int xr = min(l16, rows - 1);
+    long wrow[NT];
 #pragma unroll
     for (int j = 0; j < NT; ++j) wrow[j] = min(col0 + 16 * j + l16, a.n - 1);
+    f32x4 acc[NT];
 #pragma unroll
-    for (int i = 0; i < MT; ++i) xrow[i] = row0 + min(16 * i + l16, rows - 1);
-    f32x4 acc[MT][NT];
-#pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < NT; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
     struct Part {   // of 256 k
         uint4 w[2][NT];
         uint32_t ws[2][NT];
-        uint4 x[XT ? 1 : 2][XT ? 1 : MT];
-        uint32_t xs[XT ? 1 : 2][XT ? 1 : MT];
+        typename X::Block x[2];
     };
     auto load = [&](Part& p, int part) {
 #pragma unroll
@@ -60,43 +105,34 @@ __global__ __launch_bounds__(512) void mx_rows_kernel(MxLinearArgs a, int ntiles
                 p.ws[c][j] = a.w.scales[wrow[j] * a.w.scale_stride + at];
                 if (!in) p.w[c][j] = make_uint4(0, 0, 0, 0), p.ws[c][j] = 127;
             }
-            if constexpr (XT == 0)
-#pragma unroll
-                for (int i = 0; i < MT; ++i) {
-                    p.x[c][i] =
-                        *reinterpret_cast<const uint4*>(a.xq.codes + xrow[i] * a.xq.code_stride + 16 * at);
-                    p.xs[c][i] = a.xq.scales[xrow[i] * a.xq.scale_stride + at];
-                    if (!in) p.x[c][i] = make_uint4(0, 0, 0, 0), p.xs[c][i] = 127;
-                }
+            if constexpr (!SPLIT) X::load(a, row0 + xr, b, in, p.x[c]);
         }
     };
-    auto use = [&](const Part& p, int part) {
+    auto use = [&](const Part& p, int part, int k0) {
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
             if constexpr (XT == 0) {
 #pragma unroll
-                for (int i = 0; i < MT; ++i)
-#pragma unroll
-                    for (int j = 0; j < NT; ++j)
-                        acc[i][j] = mx_mfma<0, 0>(p.w[c][j], p.x[c][i], acc[i][j], p.ws[c][j], p.xs[c][i]);
+                for (int j = 0; j < NT; ++j)
+                    acc[j] = mx_mfma<0, 0>(p.w[c][j], p.x[c].codes, acc[j], p.ws[c][j], p.x[c].scale);
             } else {
-                const int k0 = (part * 8 + 2 * g + c) * 32;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {   // eight k
-                    uint4 w[NT];
+                    uint4 t[X::TERMS];
+                    if constexpr (SPLIT) {
+                        const int at = (part * 8 + 2 * g + c) * 32 + 8 * e - k0;
 #pragma unroll
-                    for (int j = 0; j < NT; ++j) {
-                        const uint32_t q[4] = {p.w[c][j].x, p.w[c][j].y, p.w[c][j].z, p.w[c][j].w};
-                        w[j] = mx_bf16(q[e], mx_scale(p.ws[c][j]));
+                        for (int q = 0; q < X::TERMS; ++q)
+                            t[q] = *reinterpret_cast<const uint4*>(&split[(q * rows + xr) * span + at]);
+                    } else {
+                        X::terms(p.x[c].v[e], t);
                     }
 #pragma unroll
-                    for (int i = 0; i < MT; ++i) {
-                        uint4 t[TERMS];
-                        mx_terms<XT - 1, TERMS>(a.x, xrow[i] * a.x_stride + k0 + 8 * e, a.k - k0 - 8 * e, t);
+                    for (int j = 0; j < NT; ++j) {
+                        const uint32_t q4[4] = {p.w[c][j].x, p.w[c][j].y, p.w[c][j].z, p.w[c][j].w};
+                        const uint4 w = mx_bf16(q4[e], mx_scale(p.ws[c][j]));
 #pragma unroll
-                        for (int q = 0; q < TERMS; ++q)
-#pragma unroll
-                            for (int j = 0; j < NT; ++j) acc[i][j] = mfma<1>(w[j], t[q], acc[i][j]);
+                        for (int q = 0; q < X::TERMS; ++q) acc[j] = mfma<1>(w, t[q], acc[j]);
                     }
                 }
             }
@@ -106,22 +142,40 @@ __global__ __launch_bounds__(512) void mx_rows_kernel(MxLinearArgs a, int ntiles
     Part p0, p1;
     int part = wave;
     if (part < parts) load(p0, part);
-    while (part < parts) {
-        if (part + waves < parts) load(p1, part + waves);
-        use(p0, part);
-        part += waves;
-        if (part >= parts) break;
-        if (part + waves < parts) load(p0, part + waves);
-        use(p1, part);
-        part += waves;
+    for (int k0 = 0; k0 < a.k; k0 += span) {
+        int end = parts;
+        if constexpr (SPLIT) {
+            end = min(end, (k0 + span) / 256);
+            if (k0) __syncthreads();
+            for (int i = threadIdx.x; i < rows * (span / 8); i += blockDim.x) {
+                const int r = i / (span / 8), at = i % (span / 8) * 8;
+                uint4 t[X::TERMS];
+                X::terms_of(a, row0 + r, k0 + at, t);
+#pragma unroll
+                for (int q = 0; q < X::TERMS; ++q)
+                    *reinterpret_cast<uint4*>(&split[(q * rows + r) * span + at]) = t[q];
+            }
+            __syncthreads();
+        }
+        while (part < end) {
+            if (part + waves < parts) load(p1, part + waves);
+            use(p0, part, k0);
+            part += waves;
+            if (part >= end) {
+                p0 = p1;
+                break;
+            }
+            if (part + waves < parts) load(p0, part + waves);
+            use(p1, part, k0);
+            part += waves;
+        }
+        if constexpr (!SPLIT) break;
     }
 
     // accumulator register r: column 4 g + r of row l16
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int j = 0; j < NT; ++j)
-            *reinterpret_cast<f32x4*>(&sums[wave][((i * 16 + l16) * NT + j) * 16 + 4 * g]) = acc[i][j];
+    for (int j = 0; j < NT; ++j)
+        *reinterpret_cast<f32x4*>(&sums[wave][(l16 * NT + j) * 16 + 4 * g]) = acc[j];
     __syncthreads();
     for (int o = threadIdx.x; o < rows * 16 * NT; o += blockDim.x) {
         const int col = col0 + o % (16 * NT);
@@ -136,19 +190,58 @@ __global__ __launch_bounds__(512) void mx_rows_kernel(MxLinearArgs a, int ntiles
     }
 }
 
-template <int XT, int MT, int NT>
+constexpr int kSplitBytes = 48 << 10;   // of LDS for terms of x
+
+template <int XT, int NT>
 hipError_t run_rows(const MxLinearArgs& a, hipStream_t stream) {
     const int ntiles = (a.n + 16 * NT - 1) / (16 * NT);
-    const long blocks = ((long)a.m + 16 * MT - 1) / (16 * MT) * ntiles;
+    const long blocks = ((long)a.m + 15) / 16 * ntiles;
     if (blocks > 0x7fffffffL) return hipErrorInvalidValue;
-    const int waves = std::min(8, (mx_blocks(a.k) + 7) / 8);
-    mx_rows_kernel<XT, MT, NT><<<(unsigned)blocks, 64 * waves, 0, stream>>>(a, ntiles);
+    const int parts = (mx_blocks(a.k) + 7) / 8;
+    const int waves = std::min(8, parts);
+    const unsigned nb = (unsigned)blocks;
+    if constexpr (XT == 1 || XT == 3) {
+        const int part = std::min(a.m, 16) * MxX<XT>::TERMS * 2 * 256;   // bytes of 256 k
+        // fp16 rows that several rounds of splitting would take are split by each wave (16 x
+        // 2560 by 15360 x 2560 11.4 us so, 1 x 2560 9.8, by way of LDS 7.6)
+        if (XT == 1 || part * waves <= kSplitBytes) {
+            const int span = std::min(parts, std::max(1, kSplitBytes / part));
+            mx_rows_kernel<XT, NT, true><<<nb, 64 * waves, (size_t)span * part, stream>>>(a, ntiles, 256 * span);
+            return hipGetLastError();
+        }
+    }
+    if constexpr (XT != 1) mx_rows_kernel<XT, NT, false><<<nb, 64 * waves, 0, stream>>>(a, ntiles, 0);
     return hipGetLastError();
+}
+
+constexpr int kUnits = 256;   // compute units of an MI355X
+
+// Tiles of 16 columns of a workgroup: the more there are, the fewer times x is read from the
+// L2; as long as three quarters of the compute units have a workgroup (1 x 2560 in bf16 by
+// 15360 x 2560 8.8 us with one, 7.3 with four; 1 x 5120 by 2560 x 5120 5.9 and 13).
+int rows_tiles(const MxLinearArgs& a) {
+    const long row_blocks = ((long)a.m + 15) / 16;
+    for (int t : {4, 2})
+        if (row_blocks * ((a.n + 16 * t - 1) / (16 * t)) >= kUnits * 3 / 4) return t;
+    return 1;
+}
+
+// What the kernel for few rows takes with x in other types, in microseconds: a workgroup's
+// rounds of 256 k a wave, which splitting lengthens with the rows.
+double rows_us(const MxLinearArgs& a) {
+    const int t = rows_tiles(a), at = t / 2;
+    constexpr double one[2][3] = {{2.3, 3.0, 4.3}, {3.0, 3.8, 5.3}};   // bf16, fp16
+    const double each = a.x_kind == S2_DTYPE_F32 ? 1.1 + 0.6 * at + 0.4 * std::min(a.m, 16)
+                                                 : one[a.x_kind == S2_DTYPE_F16][at];
+    const long blocks = ((long)a.m + 15) / 16 * ((a.n + 16 * t - 1) / (16 * t));
+    const long units = t == 1 ? 2 * kUnits : kUnits;   // workgroups at once
+    return 2.5 + (double)((blocks + units - 1) / units) * ((mx_blocks(a.k) + 63) / 64) * each;
 }
 
 template <int XT>
 hipError_t launch_rows(const MxLinearArgs& a, hipStream_t stream) {
-    return a.m <= 16 ? run_rows<XT, 1, 2>(a, stream) : run_rows<XT, 2, 2>(a, stream);
+    const int t = rows_tiles(a);
+    return t == 4 ? run_rows<XT, 4>(a, stream) : t == 2 ? run_rows<XT, 2>(a, stream) : run_rows<XT, 1>(a, stream);
 }
 
 // Scales of x's and of the weight's rows to rows of `width` bytes, either of which may have
@@ -171,9 +264,6 @@ __global__ __launch_bounds__(256) void mx_scales_kernel(ScaleJob x, ScaleJob w, 
 }
 
 long round_up(long v, long to) { return (v + to - 1) / to * to; }
-
-// The weight's values as bf16 rows of k, for rows of x of other types.
-size_t weight_bytes(const MxLinearArgs& a) { return round_up((size_t)a.n * a.k * 2, 256); }
 
 MatmulArgs values_args(const MxLinearArgs& a, const void* w) {
     MatmulArgs m{};
@@ -207,7 +297,89 @@ MatmulArgs codes_args(const MxLinearArgs& a) {
     return m;
 }
 
-constexpr int kRowsMost = 32;   // of x that the kernel for few rows takes
+constexpr int kRowsMost = 32;   // rows of codes that the kernel for few rows takes
+
+// Many rows of other types: x as planes of bf16 terms (or as it is, in bf16 with 16-byte
+// rows) and the weight's values in bf16, for the tile kernels of 16-bit operands.
+struct ValuesPlan {
+    TileChoice tile;
+    bool pack_x;
+    int planes, width;       // of packed x; k rounded up to 8 where it is not packed
+    size_t x_bytes, w_bytes, sum_bytes;
+    size_t bytes() const { return x_bytes + w_bytes + sum_bytes; }
+    // a launch, bytes a microsecond read and written
+    double us() const { return tile.us + 7. + (2.3 * x_bytes + 1.3 * w_bytes) / 5.5e6; }
+};
+
+ValuesPlan values_plan(const MxLinearArgs& a, size_t workspace_bytes) {
+    ValuesPlan p{};
+    const long k8 = round_up(a.k, 8);
+    p.planes = a.x_kind == S2_DTYPE_F32 ? kTerms : a.x_kind == S2_DTYPE_F16 ? 2 : 1;
+    p.pack_x = p.planes > 1 || a.k % 8 != 0 || a.x_stride % 8 != 0 || (uintptr_t)a.x % 16 != 0;
+    p.width = (int)round_up(a.k, 64);
+    if (p.pack_x) p.x_bytes = round_up((size_t)a.m * p.planes * p.width * 2, 256);
+    p.w_bytes = round_up((size_t)a.n * k8 * 2, 256);
+    if (p.bytes() > workspace_bytes) return p;
+    MatmulArgs m = values_args(a, nullptr);
+    m.k = (int)k8;
+    const size_t each = (size_t)a.m * round_up(a.n, 4) * sizeof(float);
+    p.tile = choose_tiles(m, (k8 + 63) / 64 * p.planes, std::min<long>(16, (long)((workspace_bytes - p.bytes()) / each)));
+    p.sum_bytes = p.tile.parts > 1 ? p.tile.parts * each : 0;
+    return p;
+}
+
+// Pieces of eight: x's first (`xw` a row and plane), then the weight's.
+template <int XT>
+__global__ __launch_bounds__(256) void mx_values_kernel(MxLinearArgs a, uint16_t* x, int xw, uint16_t* w, int ww) {
+    typedef MxX<XT> X;
+    const long nx = (long)a.m * xw, all = nx + (long)a.n * ww;
+    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < all; i += (long)gridDim.x * 256) {
+        if (i < nx) {
+            const long row = i / xw;
+            const int at = (int)(i - row * xw) * 8;
+            uint4 t[X::TERMS];
+            X::terms_of(a, row, at, t);
+#pragma unroll
+            for (int q = 0; q < X::TERMS; ++q)
+                *reinterpret_cast<uint4*>(x + (row * X::TERMS + q) * xw * 8 + at) = t[q];
+        } else {
+            const long row = (i - nx) / ww;
+            const int at = (int)(i - nx - row * ww);   // of four bytes
+            const uint32_t codes = *reinterpret_cast<const uint32_t*>(a.w.codes + row * a.w.code_stride + 4 * at);
+            *reinterpret_cast<uint4*>(w + (row * ww + at) * 8) =
+                mx_bf16(codes, mx_scale(a.w.scales[row * a.w.scale_stride + (at >> 2)]));
+        }
+    }
+}
+
+template <int XT>
+hipError_t launch_values(const MxLinearArgs& a, const ValuesPlan& p, void* workspace, hipStream_t stream) {
+    uint16_t* x = (uint16_t*)workspace;
+    uint16_t* w = (uint16_t*)((char*)workspace + p.x_bytes);
+    MatmulArgs m = values_args(a, w);
+    m.k = (int)round_up(a.k, 8);
+    const int xw = p.pack_x ? p.width / 8 : 0, ww = m.k / 8;
+    MxLinearArgs job = a;
+    if (!p.pack_x) job.m = 0;
+    const long all = (long)job.m * xw + (long)a.n * ww;
+    mx_values_kernel<XT><<<(unsigned)std::min<long>((all + 255) / 256, 65536), 256, 0, stream>>>(job, x, xw, w, ww);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    m.x_kind = S2_DTYPE_BF16;
+    if (p.pack_x) {
+        m.x = x;
+        m.x_stride = (long)p.planes * p.width;
+        m.planes = p.planes;
+        m.plane = p.width;
+    }
+    MatmulPlan t{};
+    t.kernel = MatmulPlan::kTiles;
+    t.bm = p.tile.bm;
+    t.bn = p.tile.bn;
+    t.parts = p.tile.parts;
+    t.whole = whole_pieces(m);
+    return launch_matmul_tiles(m, t, (float*)((char*)w + p.w_bytes), stream);
+}
 
 // Ranges of k, at most, whose sums fit `bytes`.
 long ranges(const MxLinearArgs& a, size_t bytes) {
@@ -245,6 +417,13 @@ MxPlan mx_plan(const MxLinearArgs& a, bool pack_x, bool pack_w, size_t workspace
 }  // namespace
 
 size_t mx_linear_workspace(const MxLinearArgs& a) {
+    if (!a.mx) {
+        MxLinearArgs far = a;
+        far.x_stride = a.k + 1;   // rows that are packed
+        const ValuesPlan p = values_plan(far, (size_t)1 << 62);
+        far.x_stride = round_up(a.k, 8);
+        return std::min(p.us(), values_plan(far, (size_t)1 << 62).us()) < rows_us(a) ? p.bytes() : 0;
+    }
     if (a.m <= kRowsMost) return 0;
     return mx_plan(a, true, true, (size_t)1 << 62).bytes();
 }
@@ -261,12 +440,23 @@ hipError_t launch_mx_linear(const MxLinearArgs& args, void* workspace, size_t wo
         a.xq.scale_stride = round_up(blocks, 16);
     }
     if (a.n == 1) a.w.scale_stride = round_up(blocks, 16);
-    if (!a.mx)
+    const long out = std::max(a.y_stride, a.res ? a.res_stride : 0L) * (a.y_kind ? 2 : 4);
+    const long far = 0x7fffffffL;   // 32-bit offsets
+    if (!a.mx) {
+        if (256 * out < far && (long)a.n * 4 < far && 256 * 2 * a.x_stride < far &&
+            256 * 2 * kTerms * (a.k + 64L) < far) {
+            const ValuesPlan p = values_plan(a, workspace_bytes);
+            // 500 x 2560 in bf16 by 15360 x 2560 60 us, 235 by the kernel for few rows; 77 x 5120 by
+            // 2560 x 5120 28 and 18
+            if (p.tile.bm && p.us() < rows_us(a))
+                return a.x_kind == 0   ? launch_values<1>(a, p, workspace, stream)
+                       : a.x_kind == 1 ? launch_values<2>(a, p, workspace, stream)
+                                       : launch_values<3>(a, p, workspace, stream);
+        }
         return a.x_kind == 0   ? launch_rows<1>(a, stream)
                : a.x_kind == 1 ? launch_rows<2>(a, stream)
                                : launch_rows<3>(a, stream);
-    const long out = std::max(a.y_stride, a.res ? a.res_stride : 0L) * (a.y_kind ? 2 : 4);
-    const long far = 0x7fffffffL;   // 32-bit offsets
+    }
     const bool pack_x = !scales16(a.xq.scales, a.xq.scale_stride);
     const bool pack_w = !scales16(a.w.scales, a.w.scale_stride);
     MxPlan p{};

@@ -5,8 +5,8 @@
 // of 128 bytes (256 k here), the DMA and its swizzle are those of the 16-bit products
 // (matmul_tiles.h, with a row's codes as 16-bit elements, four values each); every step
 // does four times the k.  What comes with it are the scales: 16 bytes of a row (two
-// steps) are one lane's DMA, and a lane takes blocks 2 g and 2 g + 1 of each step, whose
-// scales are one 16-bit LDS read that serves both products by their byte selectors.
+// steps) are one lane's DMA, and a lane takes those of its blocks g and 4 + g out of the
+// eight of a step.
 #include "matmul_tiles.h"
 #include "mx_device.h"
 
@@ -32,19 +32,18 @@ __device__ __forceinline__ ScaleLoad scale_load(const uint8_t* base, int rows, l
     return ScaleLoad{wave_uniform(buffer_rsrc(base, (uint32_t)bytes)), (uint32_t)(row * ld)};
 }
 
-// The scales of a lane's two blocks of step s, in the low two bytes.
-__device__ __forceinline__ uint32_t scale_pair(const uint8_t* row, int s) {
+// The scales of a lane's blocks g and 4 + g of step s, in the lowest bytes.
+__device__ __forceinline__ uint2 scale_pair(const uint8_t* row, int s) {
     const int g = (threadIdx.x & 63) >> 4;
-    return *(const uint16_t*)(row + 8 * (s & 1) + 2 * g);
+    const uint2 v = *(const uint2*)(row + 8 * (s & 1));
+    return make_uint2(v.x >> (8 * g), v.y >> (8 * g));
 }
 
 // Past the last block the codes are zeros; a scale of 1 there, whatever lies behind the
 // row.  left: blocks of the step.
-__device__ __forceinline__ uint32_t scales_past(uint32_t pair, int left) {
+__device__ __forceinline__ uint2 scales_past(uint2 pair, int left) {
     const int g = (threadIdx.x & 63) >> 4;
-    if (2 * g + 1 >= left) pair = (pair & 0xffu) | (127u << 8);
-    if (2 * g >= left) pair = (pair & 0xff00u) | 127u;
-    return pair;
+    return make_uint2(g >= left ? 127u : pair.x, 4 + g >= left ? 127u : pair.y);
 }
 
 constexpr int kScaleRow = 16;   // bytes of a row's scales in LDS: two steps
@@ -297,7 +296,7 @@ __global__ __launch_bounds__(256, 1) void mx_tile_kernel(MatmulArgs a, TileSplit
         const uint8_t* st = lds + stage * SB;
         stage = stage + 1 == STAGES ? 0 : stage + 1;
         const uint8_t* cs = lds + STAGES * SB + ((p.kb + s) >> 1) % PAIRS * CB;
-        uint32_t sx[NI], sw4[4];
+        uint2 sx[NI], sw4[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) sw4[j] = scale_pair(cs + (BM + wn * 64 + 16 * j + l16) * kScaleRow, p.kb + s);
 #pragma unroll
@@ -305,7 +304,7 @@ __global__ __launch_bounds__(256, 1) void mx_tile_kernel(MatmulArgs a, TileSplit
         uint4 fx[2][NI], fw[2][4];
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk) {
-            const int pc = ((2 * g + kk) ^ sw) * 16;
+            const int pc = ((4 * kk + g) ^ sw) * 16;
 #pragma unroll
             for (int j = 0; j < 4; ++j)
                 fw[kk][j] = *(const uint4*)(st + XB + (wn * 64 + 16 * j + l16) * RB + pc);
@@ -326,11 +325,11 @@ __global__ __launch_bounds__(256, 1) void mx_tile_kernel(MatmulArgs a, TileSplit
 #pragma unroll
         for (int i = 0; i < NI; ++i)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) acc[i][j] = mx_mfma<0, 0>(fx[0][i], fw[0][j], acc[i][j], sx[i], sw4[j]);
+            for (int j = 0; j < 4; ++j) acc[i][j] = mx_mfma<0, 0>(fx[0][i], fw[0][j], acc[i][j], sx[i].x, sw4[j].x);
 #pragma unroll
         for (int i = 0; i < NI; ++i)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) acc[i][j] = mx_mfma<1, 1>(fx[1][i], fw[1][j], acc[i][j], sx[i], sw4[j]);
+            for (int j = 0; j < 4; ++j) acc[i][j] = mx_mfma<0, 0>(fx[1][i], fw[1][j], acc[i][j], sx[i].y, sw4[j].y);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
     if (sp.parts > 1)
