@@ -1028,30 +1028,37 @@ def mx_linear(x, weight, bias=None, activation=ACT_NONE, residual=None, out=None
     fp32, bf16 or fp16.  out_dtype: x's, or bf16 for MxRows, if None.  out may be the
     residual.  workspace: mx_linear_workspace(...) bytes, made here if None.  Returns
     out [m, n]."""
-    import torch
     n, wcs, wss = _mx_rows(weight, "weight")
-    k = weight.k
-    if wcs != weight.codes.shape[1] and n > 1:
+    wcodes, wscales, k = weight
+    if n > 1 and wcs != (k + 31) // 32 * 16:
         raise ValueError("the weight's codes must be contiguous")
     mx = isinstance(x, MxRows)
-    near = x.codes if mx else x
     if mx:
         m, xcs, xss = _mx_rows(x, "x")
-        if x.k != k:
+        near, xscales, xk = x
+        if xk != k:
             raise ValueError(f"x must have rows of {k}")
+        xd = None
     else:
-        if x.dim() != 2 or x.shape[1] != k or (k > 1 and x.stride(1) != 1):
+        near, xscales, shape = x, None, x.shape
+        xs, step = x.stride() if len(shape) == 2 else (0, 0)
+        if len(shape) != 2 or shape[1] != k or (k > 1 and step != 1):
             raise ValueError(f"x must be [m, {k}] with contiguous rows")
-        m = x.shape[0]
+        m = shape[0]
         if m > _INT_MAX:
             _refuse("mx_linear", "a size is out of range")
         xd = _dtype_code(x)
     if activation not in _ROW_ACTIVATIONS:
         _refuse("mx_linear", "unknown activation")
     if out is None:
-        out = _empty((m, n), out_dtype or (torch.bfloat16 if mx else x.dtype), near, stream)
-    elif out.shape != (m, n) or (n > 1 and out.stride(1) != 1):
-        raise ValueError(f"out must be [{m}, {n}] with contiguous rows")
+        if out_dtype is None:
+            out_dtype = _bfloat16() if mx else x.dtype
+        out = _empty((m, n), out_dtype, near, stream)
+        os_ = n
+    else:
+        if out.shape != (m, n) or (n > 1 and out.stride(1) != 1):
+            raise ValueError(f"out must be [{m}, {n}] with contiguous rows")
+        os_ = out.stride(0)
     rs = 0
     if residual is not None:
         if residual.shape != (m, n) or residual.dtype is not out.dtype or (
@@ -1060,17 +1067,23 @@ def mx_linear(x, weight, bias=None, activation=ACT_NONE, residual=None, out=None
         rs = residual.stride(0)
     yd = _dtype_code(out)
     bi = None if bias is None else _vector(bias, n, "bias")
-    handle = _raw_stream(near, stream, x.scales if mx else None, weight.codes, weight.scales, bias, residual,
-                         out, workspace)
-    workspace, ws, size = _workspace(workspace, stream, near,
-                                     mx_linear_workspace(m, n, k, None if mx else xd, yd))
-    tail = (weight.codes.data_ptr(), weight.scales.data_ptr(), wss, bi, n, k, activation, _ptr(residual),
-            rs, out.data_ptr(), yd, out.stride(0), ws, size, handle)
+    handle = _raw_stream(near, stream, xscales, wcodes, wscales, bias, residual, out, workspace)
+    workspace, ws, size = _workspace(workspace, stream, near, mx_linear_workspace(m, n, k, xd, yd))
     if mx:
-        check(lib().s2_mx_linear(x.codes.data_ptr(), xcs, x.scales.data_ptr(), xss, m, *tail), "s2_mx_linear")
+        check(lib().s2_mx_linear(near.data_ptr(), xcs, xscales.data_ptr(), xss, m, wcodes.data_ptr(),
+                                 wscales.data_ptr(), wss, bi, n, k, activation, _ptr(residual), rs,
+                                 out.data_ptr(), yd, os_, ws, size, handle), "s2_mx_linear")
     else:
-        check(lib().s2_mx_weight_linear(x.data_ptr(), xd, x.stride(0), m, *tail), "s2_mx_weight_linear")
+        check(lib().s2_mx_weight_linear(x.data_ptr(), xd, xs, m, wcodes.data_ptr(), wscales.data_ptr(), wss, bi,
+                                        n, k, activation, _ptr(residual), rs, out.data_ptr(), yd, os_, ws, size,
+                                        handle), "s2_mx_weight_linear")
     return out
+
+
+@functools.lru_cache(maxsize=1)
+def _bfloat16():
+    import torch
+    return torch.bfloat16
 
 
 # ---- cross attention -------------------------------------------------------------
@@ -1090,6 +1103,17 @@ def cross_attention_workspace(batch, lq, lk, heads, kv_heads, head_dim, dtype=DT
 _Strides = ctypes.c_long * 12
 
 
+@functools.lru_cache(maxsize=4096)
+def _cross_shape(batch, lq, lk, heads, kv_heads, d, dtype, out_dtype, scale, ragged, strides):
+    """(shape by reference, strides, workspace bytes) of a call; read only."""
+    for n in (batch, lq, lk, heads, kv_heads, d):
+        if n > _INT_MAX:
+            _refuse("cross_attention", "a size is out of range")
+    shape = CrossAttentionShape(batch, lq, lk, heads, kv_heads, d, dtype, out_dtype, scale)
+    return ctypes.byref(shape), _Strides(*strides), cross_attention_workspace(batch, lq, lk, heads, kv_heads, d,
+                                                                              dtype, ragged)
+
+
 def cross_attention(q, k, v, scale=None, q_offsets=None, k_offsets=None, key_lengths=None, key_mask=None,
                     out=None, out_dtype=None, workspace=None, stream=None):
     """s2_cross_attention: softmax(scale q k^T) v per sample and head.
@@ -1102,62 +1126,75 @@ def cross_attention(q, k, v, scale=None, q_offsets=None, k_offsets=None, key_len
     if None.  out may be q; rows in no sample are left as they are in out (undefined
     in one that this call makes).  workspace: cross_attention_workspace(...) bytes, made
     here if None.  Returns out, of q's shape."""
-    import torch
     ragged = q_offsets is not None
-    dims = 3 if ragged else 4
-    if q.dim() != dims or k.dim() != dims or k.shape != v.shape or q.shape[-1] != k.shape[-1]:
-        raise ValueError("q must be [batch, lq, heads, d], k and v [batch, lk, kv_heads, d], or without "
-                         "batch and with offsets")
-    if q.dtype is not k.dtype or q.dtype is not v.dtype:
-        raise ValueError("q, k and v must be of one type")
-    lq, heads, d = q.shape[-3:]
-    lk, kv_heads = k.shape[-3:-1]
-    lead = () if ragged else (q.shape[0],)
+    qshape, kshape = q.shape, k.shape
     if ragged:
-        batch = q_offsets.numel() - 1
-        for t in (q_offsets, k_offsets):
-            if t is None or t.dtype is not torch.int32 or t.numel() != batch + 1 or t.dim() != 1 or (
-                    not t.is_contiguous()) or batch < 0:
-                raise ValueError("q_offsets and k_offsets must be batch + 1 contiguous int32 values each")
+        if len(qshape) != 3 or len(kshape) != 3:
+            raise ValueError("with offsets q must be [rows, heads, d], k and v [key rows, kv_heads, d]")
+        lq, heads, d = qshape
+        lk, kv_heads, dk = kshape
+        batch = _check_offsets(q_offsets, k_offsets, key_lengths)
     else:
-        batch = q.shape[0]
+        if len(qshape) != 4 or len(kshape) != 4 or kshape[0] != qshape[0]:
+            raise ValueError("q must be [batch, lq, heads, d], k and v [batch, lk, kv_heads, d], or without "
+                             "batch and with offsets")
+        batch, lq, heads, d = qshape
+        _, lk, kv_heads, dk = kshape
         if k_offsets is not None:
             raise ValueError("k_offsets need q_offsets")
-        if k.shape[0] != batch:
-            raise ValueError("q, k and v must have one batch")
-    if key_lengths is not None and (ragged or key_lengths.dtype is not torch.int32 or
-                                    key_lengths.numel() != batch or not key_lengths.is_contiguous()):
-        raise ValueError(f"key_lengths must be {batch} contiguous int32 values, without offsets")
-    ms = 0
-    if key_mask is not None:
-        if key_mask.dtype not in (torch.bool, torch.uint8) or key_mask.shape != lead + (lk,) or (
-                lk > 1 and key_mask.stride(-1) != 1):
-            raise ValueError(f"key_mask must be bool or uint8 {list(lead + (lk,))} with contiguous rows")
-        ms = 0 if ragged else key_mask.stride(0)
+        if key_lengths is not None and (key_lengths.dtype is not _int32() or key_lengths.numel() != batch or
+                                        not key_lengths.is_contiguous()):
+            raise ValueError(f"key_lengths must be {batch} contiguous int32 values")
+    dtype = q.dtype
+    if d != dk or v.shape != kshape or k.dtype is not dtype or v.dtype is not dtype:
+        raise ValueError("k and v must be of one shape, q, k and v of one type and head_dim")
+    ms = 0 if key_mask is None else _check_mask(key_mask, ragged, batch, lk)
     if out is None:
-        out = _empty(q.shape, out_dtype or q.dtype, q, stream)
-    elif out.shape != q.shape:
+        out = _empty(qshape, out_dtype or dtype, q, stream)
+    elif out.shape != qshape:
         raise ValueError("out must be of q's shape")
-    strides = []
-    for t in (q, k, v, out):
-        s = t.stride()
-        if d > 1 and s[-1] != 1:
-            raise ValueError("head elements must be contiguous")
-        strides += s[:3] if not ragged else (0,) + s[:2]
-    for n in (batch, lq, lk, heads, kv_heads, d):
-        if n > _INT_MAX:
-            _refuse("cross_attention", "a size is out of range")
-    dt = _dtype_code(q)
-    shape = CrossAttentionShape(batch, lq, lk, heads, kv_heads, d, dt, _dtype_code(out),
-                                d ** -0.5 if scale is None else scale)
+    qs, ks, vs, os_ = q.stride(), k.stride(), v.stride(), out.stride()
+    if d > 1 and not qs[-1] == ks[-1] == vs[-1] == os_[-1] == 1:
+        raise ValueError("head elements must be contiguous")
+    if ragged:
+        strides = (0,) + qs[:2] + (0,) + ks[:2] + (0,) + vs[:2] + (0,) + os_[:2]
+    else:
+        strides = qs[:3] + ks[:3] + vs[:3] + os_[:3]
+    shape, strides, need = _cross_shape(batch, lq, lk, heads, kv_heads, d, _dtype_code(q), _dtype_code(out),
+                                        d ** -0.5 if scale is None else float(scale), ragged, strides)
     handle = _raw_stream(q, stream, k, v, out, q_offsets, k_offsets, key_lengths, key_mask, workspace)
-    workspace, ws, size = _workspace(workspace, stream, q, cross_attention_workspace(
-        batch, lq, lk, heads, kv_heads, d, dt, ragged))
-    check(lib().s2_cross_attention(ctypes.byref(shape), q.data_ptr(), k.data_ptr(), v.data_ptr(),
-                                   out.data_ptr(), _Strides(*strides), _ptr(q_offsets), _ptr(k_offsets),
-                                   _ptr(key_lengths), _ptr(key_mask), ms, ws, size, handle),
-          "s2_cross_attention")
+    workspace, ws, size = _workspace(workspace, stream, q, need)
+    check(lib().s2_cross_attention(shape, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), strides,
+                                   _ptr(q_offsets), _ptr(k_offsets), _ptr(key_lengths), _ptr(key_mask), ms, ws,
+                                   size, handle), "s2_cross_attention")
     return out
+
+
+@functools.lru_cache(maxsize=1)
+def _int32():
+    import torch
+    return torch.int32
+
+
+def _check_offsets(q_offsets, k_offsets, key_lengths):
+    """The number of samples."""
+    batch = q_offsets.numel() - 1
+    for t in (q_offsets, k_offsets):
+        if t is None or t.dtype is not _int32() or t.dim() != 1 or t.numel() != batch + 1 or batch < 0 or (
+                not t.is_contiguous()):
+            raise ValueError("q_offsets and k_offsets must be batch + 1 contiguous int32 values each")
+    if key_lengths is not None:
+        raise ValueError("key_lengths are for samples without offsets")
+    return batch
+
+
+def _check_mask(mask, ragged, batch, lk):
+    """The mask's batch stride."""
+    import torch
+    shape = (lk,) if ragged else (batch, lk)
+    if mask.dtype not in (torch.bool, torch.uint8) or mask.shape != shape or (lk > 1 and mask.stride(-1) != 1):
+        raise ValueError(f"key_mask must be bool or uint8 {list(shape)} with contiguous rows")
+    return 0 if ragged else mask.stride(0)
 
 
 # ---- DecomposedConv3D ------------------------------------------------------------
