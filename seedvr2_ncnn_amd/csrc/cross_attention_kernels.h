@@ -38,9 +38,13 @@ struct CrossArgs {
 
 constexpr int kTileRows = 128, kTileRows32 = 64;   // of 16-bit operands' tiles, of fp32 ones'
 constexpr int kTileKeys = 32;
+// keys of a head that LDS holds in the kernel for many rows on few of them, and its workgroups
+// on a compute unit
+constexpr int kShortKeys = 128, kShortEach = 2;
 
 // A call's kernel.  Rows: queries times the heads that share a kv head.
 struct CrossPlan {
+    int run;      // of 128 rows each that a tile has; 1 but for many rows on few keys
     int tiles;    // of rows of a kv head, at most
     int parts;    // ranges of keys
 };

@@ -106,14 +106,35 @@ CrossPlan cross_plan(const CrossArgs& a, size_t workspace_bytes) {
     const long group = a.heads / a.kv_heads;
     const long rows = (long)a.lq * group;
     const int each = a.kind ? kTileRows : kTileRows32;
+    auto tiles_of = [&](long each) {
+        return std::min<long>(a.q_offsets ? rows / each + std::min(a.batch, a.lq)
+                                          : a.batch * ((rows + each - 1) / each),
+                              0x7fffffffL);
+    };
     CrossPlan p;
-    p.tiles = (int)std::min<long>(a.q_offsets ? rows / each + std::min(a.batch, a.lq)
-                                              : a.batch * ((rows + each - 1) / each),
-                                  0x7fffffffL);
+    p.run = 1;
+    p.tiles = (int)tiles_of(each);
     // a sample's last tile is half empty, on average
     const double blocks = a.kv_heads * (a.q_offsets ? (double)rows / each + 0.5 * std::min(a.batch, a.lq)
                                                     : (double)p.tiles);
     const long keys = a.q_offsets ? ((long)a.lk + a.batch - 1) / std::max(a.batch, 1) : a.lk;   // of a sample
+    if (a.kind && a.d > 64 && a.d <= 128 && keys <= kShortKeys) {
+        // the run by which the compute units' turns, of `run` rounds and one to begin, are
+        // fewest; worth it from about four on (4096 queries on 77 keys, 20 heads: two rounds 17.7
+        // us, 14.6 by the other kernel)
+        const long slots = (long)kUnits * kShortEach;
+        long least = 0;
+        for (int run = 1; run <= 64; ++run) {
+            const long turns = (tiles_of((long)each * run) * a.kv_heads + slots - 1) / slots * (run + 1);
+            if (run == 1 || turns < least) least = turns, p.run = run;
+        }
+        if (p.run >= 4) {
+            p.tiles = (int)tiles_of((long)each * p.run);
+            p.parts = 1;
+            return p;
+        }
+        p.run = 1;
+    }
     const double tiles = (double)((keys + kTileKeys - 1) / kTileKeys);
     const long most = std::min<long>(64, (long)(workspace_bytes / part_bytes(a)));
     const CrossCost& c = kCrossCosts[a.kind == 0][a.d <= 64 ? 0 : a.d <= 128 ? 1 : 2];

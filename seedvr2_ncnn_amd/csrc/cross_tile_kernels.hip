@@ -72,95 +72,82 @@ __device__ __forceinline__ u32x2 out4(const CrossArgs& a, f32x4 v) {
     return u32x2{pack2_f16_rne(v[0], v[1]), pack2_f16_rne(v[2], v[3])};
 }
 
-// DP: d rounded up to 64, 128 or 256.  STAGES: of LDS; WGS: workgroups on a compute unit.
-template <int T, int DP, int STAGES, int WGS, bool MASK>
-__global__ __launch_bounds__(256, WGS) void cross_tile_kernel(CrossArgs a, int tiles, CrossParts parts) {
-    constexpr int KT = kTileKeys, BM = kTileRows;
-    constexpr int RB = DP * 2;                   // bytes of a row in LDS
-    constexpr int KB = KT * RB, SB = 2 * KB;     // a tile of k; a stage
-    constexpr int NK = DP / 32, ND = DP / 16;    // product steps over d; column tiles
-    constexpr int NQ = 2;                        // 16-row tiles of a wave
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[STAGES * SB];
-    __shared__ uint64_t bits[MASK ? kMaskBits : 1];
-    const CrossTile t = cross_tile(a, BM, tiles, parts.parts);
-    if (t.rows <= 0) return;   // the whole workgroup
-    const int lane = threadIdx.x & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int l16 = lane & 15, g = lane >> 4;
-    const int row_w = 32 * wave;   // of the wave's first row in the tile
-
-    const int nk = __builtin_amdgcn_readfirstlane(t.s.nk);
-    const int all = (nk + KT - 1) / KT;
-    const int kb = (int)((long)all * t.part / parts.parts), ke = (int)((long)all * (t.part + 1) / parts.parts);
-
-    KeyTiles<2, DP, STAGES, MASK, Swizzle<DP>> kv(a, t, nk, kb, (uint32_t)(uintptr_t)lds, bits);
-    if (kb < ke) kv.issue(kb, 0, true);
-    if (STAGES > 2 && kb + 1 < ke) kv.issue(kb + 1, 1, false);
-
-    if (row_w >= t.rows) {   // a wave without rows takes part in loads and barriers alone
-        for (int kt = kb; kt < ke; ++kt) {
-            kv.await(kt, ke);
-            if (kt + STAGES - 1 < ke) kv.issue(kt + STAGES - 1, (kt - kb + STAGES - 1) % STAGES, false);
-        }
-        return;
-    }
-
-    // q: row l16 of each 16, elements 32 kk + 8 g on; zeros past d, the last row again past
-    // the rows
-    const uint32_t sign = a.scale < 0.f ? 0x80008000u : 0u;
-    // (not nought, by which a masked score of -inf would be NaN)
-    const float c = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 0x1p-126f);
+// A wave's 32 rows: q, the sums and softmax's state.  DP: d rounded up to 64, 128 or 256; lds:
+// the stages of KeyTiles.
+template <int T, int DP>
+struct WaveRows {
+    static constexpr int RB = DP * 2, KB = kTileKeys * RB;   // bytes of a row in LDS, of a tile of k
+    static constexpr int NK = DP / 32, ND = DP / 16;         // product steps over d; column tiles
+    static constexpr int NQ = 2;                             // 16-row tiles
+    // 256 bytes further in a row the swizzles are the same
+    static constexpr int KA = NK < 4 ? NK : 4, VA = ND < 8 ? ND : 8;
+    int l16, g;
+    uint32_t sign;
+    float c;
     uint4 qf[NQ][NK];
+    f32x4 o[ND][NQ];
+    float m[NQ], l[NQ];   // l: of this lane's keys
+    const uint8_t* kl[KA];
+    const uint8_t* vl[VA];
+
+    __device__ __forceinline__ WaveRows(const CrossArgs& a, const uint8_t* lds) {
+        l16 = threadIdx.x & 15;
+        g = (threadIdx.x & 63) >> 4;
+        sign = a.scale < 0.f ? 0x80008000u : 0u;
+        // (not nought, by which a masked score of -inf would be NaN)
+        c = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 0x1p-126f);
 #pragma unroll
-    for (int i = 0; i < NQ; ++i) {
-        const int r = row_w + 16 * i + l16;
-        const uint16_t* p = (const uint16_t*)a.q + cross_row(a, a.qs, t, t.row0 + min(r, t.rows - 1));
+        for (int kk = 0; kk < KA; ++kk) kl[kk] = lds + l16 * RB + (((4 * kk + g) ^ Swizzle<DP>::key(l16)) * 16);
+        const int vrow = 4 * g + (l16 >> 2);   // of the lane's eight bytes of v, of 16 rows
 #pragma unroll
-        for (int kk = 0; kk < NK; ++kk) {
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (32 * kk + 8 * g < a.d) v = *reinterpret_cast<const uint4*>(p + 32 * kk + 8 * g);
-            qf[i][kk] = make_uint4(v.x ^ sign, v.y ^ sign, v.z ^ sign, v.w ^ sign);
+        for (int dt = 0; dt < VA; ++dt)
+            vl[dt] = lds + KB + vrow * RB + (l16 & 1) * 8 +
+                     ((2 * dt + (l16 >> 1 & 1)) ^ Swizzle<DP>::value(vrow)) * 16;
+    }
+
+    // q of rows `first` on of the tile: row l16 of each 16, elements 32 kk + 8 g on; zeros past
+    // d, the last row again past the rows
+    __device__ __forceinline__ void load(const CrossArgs& a, const CrossTile& t, int first, uint4 (&q)[NQ][NK]) const {
+#pragma unroll
+        for (int i = 0; i < NQ; ++i) {
+            const uint16_t* p =
+                (const uint16_t*)a.q + cross_row(a, a.qs, t, t.row0 + min(first + 16 * i + l16, t.rows - 1));
+#pragma unroll
+            for (int kk = 0; kk < NK; ++kk) {
+                q[i][kk] = make_uint4(0, 0, 0, 0);
+                if (32 * kk + 8 * g < a.d) q[i][kk] = *reinterpret_cast<const uint4*>(p + 32 * kk + 8 * g);
+            }
         }
     }
-    // q is there before the loop, in a way that the compiler sees: with these loads perhaps in
-    // flight it would wait for all of the DMA in every tile
-    __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0)
 
-    f32x4 o[ND][NQ];
+    __device__ __forceinline__ void begin(const uint4 (&q)[NQ][NK]) {
 #pragma unroll
-    for (int dt = 0; dt < ND; ++dt)
+        for (int i = 0; i < NQ; ++i) {
 #pragma unroll
-        for (int i = 0; i < NQ; ++i) o[dt][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    float m[NQ], l[NQ];   // l: of this lane's keys
+            for (int kk = 0; kk < NK; ++kk)
+                qf[i][kk] = make_uint4(q[i][kk].x ^ sign, q[i][kk].y ^ sign, q[i][kk].z ^ sign, q[i][kk].w ^ sign);
+            m[i] = kLowest;
+            l[i] = 0.f;
 #pragma unroll
-    for (int i = 0; i < NQ; ++i) m[i] = kLowest, l[i] = 0.f;
-    // unrolled by the stages, so that LDS addresses are registers and constants; 256 bytes
-    // further in a row the swizzles are the same
-    constexpr int KA = NK < 4 ? NK : 4, VA = ND < 8 ? ND : 8;
-    const uint8_t* kl[KA];
-#pragma unroll
-    for (int kk = 0; kk < KA; ++kk)
-        kl[kk] = lds + l16 * RB + (((4 * kk + g) ^ Swizzle<DP>::key(l16)) * 16);
-    const int vrow = 4 * g + (l16 >> 2);   // of the lane's eight bytes of v, of 16 rows
-    const uint8_t* vl[VA];
-#pragma unroll
-    for (int dt = 0; dt < VA; ++dt)
-        vl[dt] = lds + KB + vrow * RB + (l16 & 1) * 8 + ((2 * dt + (l16 >> 1 & 1)) ^ Swizzle<DP>::value(vrow)) * 16;
-    auto key = [&](int h, int kk, int st) {
+            for (int dt = 0; dt < ND; ++dt) o[dt][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+    }
+
+    __device__ __forceinline__ uint4 key(int h, int kk, int st) const {
         return *(const uint4*)(kl[kk % KA] + (kk / KA * 256 + 16 * h * RB + st));
-    };
-    auto tile = [&](int kt, auto stage) {
-        constexpr int ST = decltype(stage)::value * SB;
-        kv.await(kt, ke);   // and tile kt - 1 is no longer read
-        // these reads' way is under the loads' issue (where registers are left for them)
+    }
+
+    // The tile of keys at LDS offset ST.  between(), after the first reads are on their way,
+    // gives the keys that count.
+    template <int ST, typename F>
+    __device__ __forceinline__ void keys(F&& between) {
+        // (reads ahead where registers are left for them)
         constexpr int AHEAD = DP == 256 ? 0 : NK;
         uint4 kf[2][NK];
 #pragma unroll
         for (int kk = 0; kk < AHEAD; ++kk) kf[0][kk] = key(0, kk, ST);
         asm volatile("" ::: "memory");
-        if (kt + STAGES - 1 < ke)
-            kv.issue(kt + STAGES - 1, (decltype(stage)::value + STAGES - 1) % STAGES, false);
-        const uint32_t valid = kv.valid(kt);
+        const uint32_t valid = between();
         f32x4 s[2][NQ];
 #pragma unroll
         for (int h = 0; h < 2; ++h)
@@ -227,6 +214,96 @@ __global__ __launch_bounds__(256, WGS) void cross_tile_kernel(CrossArgs a, int t
 #pragma unroll
             for (int i = 0; i < NQ; ++i) o[dt][i] = mfma<T>(vf, pb[i], o[dt][i]);
         }
+    }
+
+    // Rows `first` on of the tile to out, or to their part.
+    __device__ __forceinline__ void store(const CrossArgs& a, const CrossTile& t, const CrossParts& parts, int first) {
+#pragma unroll
+        for (int i = 0; i < NQ; ++i) {
+            l[i] = sum_groups(l[i]);
+            const int r = first + 16 * i + l16;
+            if (r >= t.rows) continue;   // (all four lanes of a row)
+            if (parts.parts > 1) {
+                const long at = cross_part(a, parts, t, t.row0 + r);
+                if (g == 0) parts.weights[at] = make_float2(m[i], l[i]);
+#pragma unroll
+                for (int dt = 0; dt < ND; ++dt)
+                    if (16 * dt + 4 * g < a.d)
+                        *reinterpret_cast<f32x4*>(parts.sums + at * a.d + 16 * dt + 4 * g) = o[dt][i];
+                continue;
+            }
+            const float scale = l[i] == 0.f ? 0.f : 1.f / l[i];
+            const long at = cross_row(a, a.os, t, t.row0 + r);
+            if (a.out_kind == 0) {
+#pragma unroll
+                for (int dt = 0; dt < ND; ++dt)
+                    if (16 * dt + 4 * g < a.d) store4_any<0>(a.out, at + 16 * dt + 4 * g, o[dt][i] * scale);
+                continue;
+            }
+            // two column tiles' values change lanes, so that a lane has eight neighbours
+#pragma unroll
+            for (int dt = 0; dt < ND; dt += 2) {
+                u32x2 x = out4(a, o[dt][i] * scale), y = out4(a, o[dt + 1][i] * scale);
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    auto w = __builtin_amdgcn_permlane32_swap(x[e], y[e], false, false);
+                    w = __builtin_amdgcn_permlane16_swap(w[0], w[1], false, false);
+                    x[e] = w[0];
+                    y[e] = w[1];
+                }
+                const int col = 16 * (dt + (g >> 1)) + 8 * (g & 1);
+                if (col < a.d)
+                    *reinterpret_cast<u32x4_at2*>((uint16_t*)a.out + at + col) = u32x4{x[0], x[1], y[0], y[1]};
+            }
+        }
+    }
+};
+
+// STAGES: of LDS; WGS: workgroups on a compute unit.
+template <int T, int DP, int STAGES, int WGS, bool MASK>
+__global__ __launch_bounds__(256, WGS) void cross_tile_kernel(CrossArgs a, int tiles, CrossParts parts) {
+    typedef WaveRows<T, DP> Rows;
+    constexpr int SB = 2 * Rows::KB;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[STAGES * SB];
+    __shared__ uint64_t bits[MASK ? kMaskBits : 1];
+    const CrossTile t = cross_tile(a, kTileRows, tiles, parts.parts);
+    if (t.rows <= 0) return;   // the whole workgroup
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int row_w = 32 * wave;   // of the wave's first row in the tile
+    const int nk = __builtin_amdgcn_readfirstlane(t.s.nk);
+    const int all = (nk + kTileKeys - 1) / kTileKeys;
+    const int kb = (int)((long)all * t.part / parts.parts), ke = (int)((long)all * (t.part + 1) / parts.parts);
+
+    KeyTiles<2, DP, STAGES, MASK, Swizzle<DP>> kv(a, t, nk, kb, (uint32_t)(uintptr_t)lds, bits);
+    if (kb < ke) kv.issue(kb, 0, true);
+    if (STAGES > 2 && kb + 1 < ke) kv.issue(kb + 1, 1, false);
+
+    if (row_w >= t.rows) {   // a wave without rows takes part in loads and barriers alone
+        for (int kt = kb; kt < ke; ++kt) {
+            kv.await(kt, ke);
+            if (kt + STAGES - 1 < ke) kv.issue(kt + STAGES - 1, (kt - kb + STAGES - 1) % STAGES, false);
+        }
+        return;
+    }
+
+    Rows rows(a, lds);
+    {
+        uint4 q[Rows::NQ][Rows::NK];
+        rows.load(a, t, row_w, q);
+        rows.begin(q);
+    }
+    // q is there before the loop, in a way that the compiler sees: with these loads perhaps in
+    // flight it would wait for all of the DMA in every tile
+    __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0)
+
+    // unrolled by the stages, so that LDS addresses are registers and constants
+    auto tile = [&](int kt, auto stage) {
+        constexpr int ST = decltype(stage)::value;
+        kv.await(kt, ke);   // and tile kt - 1 is no longer read
+        rows.template keys<ST * SB>([&] {   // the loads' issue
+            if (kt + STAGES - 1 < ke) kv.issue(kt + STAGES - 1, (ST + STAGES - 1) % STAGES, false);
+            return kv.valid(kt);
+        });
     };
 #pragma unroll 1
     for (int kt = kb; kt < ke; kt += STAGES) {
@@ -235,44 +312,70 @@ __global__ __launch_bounds__(256, WGS) void cross_tile_kernel(CrossArgs a, int t
         if constexpr (STAGES > 2)
             if (kt + 2 < ke) tile(kt + 2, std::integral_constant<int, 2>{});
     }
+    rows.store(a, t, parts, row_w);
+}
 
-#pragma unroll
-    for (int i = 0; i < NQ; ++i) {
-        l[i] = sum_groups(l[i]);
-        const int r = row_w + 16 * i + l16;
-        if (r >= t.rows) continue;   // (all four lanes of a row)
-        if (parts.parts > 1) {
-            const long at = cross_part(a, parts, t, t.row0 + r);
-            if (g == 0) parts.weights[at] = make_float2(m[i], l[i]);
-#pragma unroll
-            for (int dt = 0; dt < ND; ++dt)
-                if (16 * dt + 4 * g < a.d) *reinterpret_cast<f32x4*>(parts.sums + at * a.d + 16 * dt + 4 * g) = o[dt][i];
-        } else {
-            const float scale = l[i] == 0.f ? 0.f : 1.f / l[i];
-            const long at = cross_row(a, a.os, t, t.row0 + r);
-            if (a.out_kind == 0) {
-#pragma unroll
-                for (int dt = 0; dt < ND; ++dt)
-                    if (16 * dt + 4 * g < a.d) store4_any<0>(a.out, at + 16 * dt + 4 * g, o[dt][i] * scale);
-            } else {
-                // two column tiles' values change lanes, so that a lane has eight neighbours
-#pragma unroll
-                for (int dt = 0; dt < ND; dt += 2) {
-                    u32x2 x = out4(a, o[dt][i] * scale), y = out4(a, o[dt + 1][i] * scale);
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        auto w = __builtin_amdgcn_permlane32_swap(x[e], y[e], false, false);
-                        w = __builtin_amdgcn_permlane16_swap(w[0], w[1], false, false);
-                        x[e] = w[0];
-                        y[e] = w[1];
-                    }
-                    const int col = 16 * (dt + (g >> 1)) + 8 * (g & 1);
-                    if (col < a.d)
-                        *reinterpret_cast<u32x4_at2*>((uint16_t*)a.out + at + col) = u32x4{x[0], x[1], y[0], y[1]};
-                }
+// Many rows of d from 65 to 128 on few keys: all of a head's keys stay in LDS, up to 128 of
+// them, for `run` times 128 rows, so that waves meet at no barrier and q, loaded a turn
+// ahead, and out are all that moves (21600 queries on 77 keys, 20 heads of 128: 64 us by the
+// kernel above, 52 so, 4.3 TB/s; with heads of 64 30 either way).  Samples of more keys are
+// read again for every 128 rows.
+template <int T, bool MASK>
+__global__ __launch_bounds__(256, kShortEach) void cross_short_kernel(CrossArgs a, int tiles, int run) {
+    constexpr int DP = 128, TILES = kShortKeys / kTileKeys;
+    static_assert(TILES == 4, "the tiles' unrolling");
+    typedef WaveRows<T, DP> Rows;
+    constexpr int SB = 2 * Rows::KB;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[TILES * SB];
+    __shared__ uint64_t bits[MASK ? kMaskBits : 1];
+    const CrossTile t = cross_tile(a, kTileRows * run, tiles, 1);
+    if (t.rows <= 0) return;   // the whole workgroup
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int nk = __builtin_amdgcn_readfirstlane(t.s.nk);
+    const int all = (nk + kTileKeys - 1) / kTileKeys;
+    typedef KeyTiles<2, DP, TILES, MASK, Swizzle<DP>> Keys;
+    Keys kv(a, t, nk, 0, (uint32_t)(uintptr_t)lds, bits);
+    auto load = [&](int k0) {   // tiles k0 .. k0 + TILES - 1
+        for (int s = 0; s < TILES && k0 + s < all; ++s) kv.issue(k0 + s, s, k0 + s == 0);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+    };
+    Rows rows(a, lds);
+    uint4 q[Rows::NQ][Rows::NK];
+    rows.load(a, t, min(32 * wave, t.rows - 1), q);
+    if (all <= TILES) load(0);
+#pragma unroll 1
+    for (int first = 32 * wave, r = 0; r < t.rows; r += kTileRows, first += kTileRows) {
+        rows.begin(q);
+        if (first + kTileRows < t.rows) rows.load(a, t, first + kTileRows, q);
+        for (int k0 = 0; k0 < all; k0 += TILES) {
+            if (all > TILES) {
+                __syncthreads();   // the tiles before are no longer read
+                if (k0 == 0) kv = Keys(a, t, nk, 0, (uint32_t)(uintptr_t)lds, bits);
+                load(k0);
             }
+            if (first >= t.rows) continue;
+            auto tile = [&](auto stage) {
+                constexpr int ST = decltype(stage)::value;
+                if (k0 + ST < all) rows.template keys<ST * SB>([&] { return kv.valid(k0 + ST); });
+            };
+            tile(std::integral_constant<int, 0>{});
+            tile(std::integral_constant<int, 1>{});
+            tile(std::integral_constant<int, 2>{});
+            tile(std::integral_constant<int, 3>{});
         }
+        if (first < t.rows) rows.store(a, t, CrossParts{1, nullptr, nullptr}, first);
     }
+}
+
+template <int T>
+hipError_t launch_short(const CrossArgs& a, const CrossPlan& p, hipStream_t stream) {
+    const unsigned nb = (unsigned)((long)p.tiles * a.kv_heads);
+    if (a.key_mask)
+        cross_short_kernel<T, true><<<nb, 256, 0, stream>>>(a, p.tiles, p.run);
+    else
+        cross_short_kernel<T, false><<<nb, 256, 0, stream>>>(a, p.tiles, p.run);
+    return hipGetLastError();
 }
 
 template <int T, int DP, int STAGES, int WGS>
@@ -286,6 +389,7 @@ hipError_t launch(const CrossArgs& a, int tiles, const CrossParts& parts, unsign
 
 template <int T>
 hipError_t launch_t(const CrossArgs& a, const CrossPlan& p, const CrossParts& parts, hipStream_t stream) {
+    if (p.run > 1) return launch_short<T>(a, p, stream);
     const unsigned nb = (unsigned)((long)p.tiles * a.kv_heads * p.parts);
     if (a.d > 128) return launch<T, 256, 2, 2>(a, p.tiles, parts, nb, stream);
     if (a.d > 64) return launch<T, 128, 3, 3>(a, p.tiles, parts, nb, stream);

@@ -202,6 +202,26 @@ def test_ragged(dtype, queries, keys, heads, kv_heads, d):
     _ragged(queries, keys, heads, kv_heads, d, dtype, mask=mask)
 
 
+@pytest.mark.parametrize("dtype", TYPES[1:], ids=str)
+def test_many_queries_on_few_keys(dtype):
+    _padded(1, 14000, 77, 20, 20, 128, dtype)
+    _padded(2, 9001, 128, 16, 8, 72, dtype, lengths=[128, 0], poison=True)
+    mask = torch.rand(3, 97, generator=torch.Generator(device="cuda").manual_seed(5), device="cuda") < 0.7
+    mask[1] = False
+    mask[2, :40] = False
+    _padded(3, 6000, 97, 16, 16, 128, dtype, mask=mask, poison=True)
+
+
+@pytest.mark.parametrize("dtype", TYPES[1:], ids=str)
+def test_many_queries_on_few_keys_but_for_some_samples(dtype):
+    """Samples of more keys than others have on average, by far."""
+    queries, keys = [9000, 1, 5000, 130, 0, 700], [20, 300, 129, 0, 9, 128]
+    _ragged(queries, keys, 20, 20, 128, dtype)
+    mask = torch.rand(sum(keys) + 3, generator=torch.Generator(device="cuda").manual_seed(6), device="cuda") < 0.5
+    mask[sum(keys):] = False
+    _ragged(queries, keys, 20, 20, 128, dtype, mask=mask)
+
+
 def test_offsets_outside_the_rows_are_taken_as_their_ends():
     q, k = torch.randn(20, 2, 64, device="cuda"), torch.randn(30, 2, 64, device="cuda")
     v = torch.randn(30, 2, 64, device="cuda")
