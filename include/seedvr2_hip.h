@@ -652,13 +652,14 @@ S2_API int s2_mx_weight_linear(const void* x, s2_dtype x_dtype, long x_stride, i
  * Strides in elements, batch (unused with offsets), row, head, elements contiguous: for
  *   q, k, v and out in turn, strides[0..11].  q, k and v are of one dtype; their rows
  *   start at 16 bytes (strides a multiple of 16 bytes too, row strides of k and v up to 2^23
- *   elements); out's at its elements, its rows do not overlap, and it overlaps nothing else, but may be q itself
- *   (same dtype and strides).
- * key_mask: device bytes [batch][mask_stride], or [lk] with offsets, 0 for keys to leave
- *   out, or NULL.  What k and v hold where a key is left out, infinities and NaN among it,
- *   is not used.  A query with no key left, or with scores of -inf
- *   alone, gives zeros.
- * head_dim: a multiple of 8 up to 256; heads a multiple of kv_heads.
+ *   elements); out's at its elements, its rows do not overlap, and it overlaps nothing else,
+ *   but may be q itself (same dtype and strides).
+ * key_mask: device bytes, of sample b at b * mask_stride (0: one mask for all), or [lk] with
+ *   offsets, 0 for keys to leave out, or NULL.  What k and v hold where a key is left out,
+ *   infinities and NaN among it, is not used.  A query with no key left, or with scores of
+ *   -inf alone, gives zeros.
+ * batch, lq times heads / kv_heads, and lk: up to 2^30.  head_dim: a multiple of 8 up to 256;
+ *   heads a multiple of kv_heads, up to 65535.
  * Scores, exponentials, their sums and out's sums are fp32; fp32 operands are multiplied in
  *   fp32, 16-bit ones on the matrix cores, where the weights of v are rounded to their type.
  * workspace: s2_cross_attention_workspace_bytes, 16-byte aligned (calls that may overlap

@@ -1574,6 +1574,8 @@ static int cross_shape_ok(const s2_cross_attention_shape* s) {
         return fail(S2_ERR_INVALID, "invalid batch or lengths");
     if (s->heads <= 0 || s->kv_heads <= 0 || s->heads % s->kv_heads != 0 || s->heads > 65535)
         return fail(S2_ERR_INVALID, "heads must be a multiple of kv_heads, at most 65535");
+    if ((long)s->lq * (s->heads / s->kv_heads) > most)
+        return fail(S2_ERR_INVALID, "lq times the heads of a group is at most 2^30");
     if (s->head_dim <= 0 || s->head_dim % 8 != 0 || s->head_dim > 256)
         return fail(S2_ERR_INVALID, "head_dim must be a multiple of 8, at most 256");
     if (!dtype_ok(s->dtype) || !dtype_ok(s->out_dtype)) return fail(S2_ERR_INVALID, "unsupported dtype");
@@ -1668,8 +1670,8 @@ int s2_cross_attention(const s2_cross_attention_shape* shape, const void* q, con
             span += (wide)(size[i] - 1) * step[i];
         }
     }
-    if (key_mask && !q_offsets && shape->batch > 1 && mask_stride < shape->lk)
-        return fail(S2_ERR_INVALID, "mask_stride shorter than the keys");
+    if (key_mask && !q_offsets && shape->batch > 1 && (mask_stride < 0 || mask_stride > most))
+        return fail(S2_ERR_INVALID, "mask_stride negative or too large");
     if (out == q && (shape->dtype != shape->out_dtype || a.qs.batch != a.os.batch ||
                      a.qs.row != a.os.row || a.qs.head != a.os.head))
         return fail(S2_ERR_INVALID, "in place needs one type and one set of strides");

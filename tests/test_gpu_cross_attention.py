@@ -121,6 +121,50 @@ def test_broadcast_keys(dtype, lq):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("lq", [1, 90])
+def test_one_mask_for_all_samples(dtype, lq):
+    mask = torch.arange(70, device="cuda") % 3 != 0
+    _padded(4, lq, 70, 4, 2, 64, dtype, mask=mask.expand(4, 70), poison=True)
+    wide = torch.zeros(4, 100, dtype=torch.uint8, device="cuda")
+    wide[:, 5:75] = mask * 7   # any byte but nought
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    q, k, v = (_normal(gen, 4, n, 2, 64).to(dtype) for n in (lq, 70, 70))
+    a = capi.cross_attention(q, k, v, key_mask=wide[:, 5:75])
+    assert torch.equal(a, capi.cross_attention(q, k, v, key_mask=mask.expand(4, 70)))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_calls_side_by_side(dtype):
+    """Two streams at once, each call with a workspace of its own."""
+    gen = torch.Generator(device="cuda").manual_seed(11)
+    sets = [tuple(_normal(gen, 1, n, 4, 128).to(dtype) for n in (lq, 4000, 4000)) for lq in (1, 200)]
+    want = [capi.cross_attention(*s) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = [[], []]
+    for _ in range(5):
+        for i, s in enumerate(sets):
+            got[i].append(capi.cross_attention(*s, stream=streams[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(g, want[i]) for g in got[i])
+
+
+@pytest.mark.parametrize("dtype", TYPES[1:], ids=str)
+def test_far_rows_of_keys(dtype):
+    """Key rows so far apart that a tile's reach passes 32 bits from the first one."""
+    n, step = 70, 1 << 23
+    flat = torch.empty((n - 1) * step + 64, dtype=dtype, device="cuda")
+    k = flat.as_strided((1, n, 1, 64), (0, step, 64, 1))
+    gen = torch.Generator(device="cuda").manual_seed(12)
+    k.copy_(_normal(gen, 1, n, 1, 64))
+    q, v = _normal(gen, 1, 40, 1, 64).to(dtype), _normal(gen, 1, n, 1, 64).to(dtype)
+    for lq in (1, 40):
+        got = capi.cross_attention(q[:, :lq], k, v)
+        ro.check(got[0], *_sample(q[0, :lq], k[0], v[0], 64 ** -0.5, None, dtype))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
 @pytest.mark.parametrize("out_dtype", TYPES, ids=str)
 def test_out_types_and_scales(dtype, out_dtype):
     for lq in (2, 150):

@@ -248,6 +248,47 @@ def test_graphs_and_streams(x_kind, m):
     assert torch.equal(y, want[1]) and torch.equal(z, want[1])
 
 
+@pytest.mark.parametrize("x_kind", KINDS, ids=str)
+def test_calls_side_by_side(x_kind):
+    """Two streams at once, each call with a workspace of its own."""
+    weight, _ = _weight(300, 1500, 7, mc.blocks(1500) + 1)
+    rows = [torch.randn(m, 1500, device="cuda").to(x_kind or torch.float32) for m in (90, 700)]
+    xs = [capi.mx_quantize(r) if x_kind is None else r for r in rows]
+    want = [capi.mx_linear(x, weight, out_dtype=torch.float32) for x in xs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in xs]
+    got = [[], []]
+    for _ in range(5):
+        for i, x in enumerate(xs):
+            got[i].append(capi.mx_linear(x, weight, out_dtype=torch.float32, stream=streams[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(g, want[i]) for g in got[i])
+
+
+@pytest.mark.parametrize("x_kind", KINDS[1:], ids=str)
+def test_rows_that_begin_anywhere(x_kind):
+    """Single elements past 16 bytes, odd strides; few rows and many."""
+    weight, w = _weight(50, 333, 8)
+    for m in (2, 20, 600):
+        flat = torch.randn(1 + m * 335, device="cuda").to(x_kind)
+        x = flat[1:].view(m, 335)[:, :333]
+        got = capi.mx_linear(x, weight, out_dtype=torch.float32)
+        ro.check(got, *mc.linear(x.double(), w.cuda(), None, "none", None, torch.float32))
+
+
+@pytest.mark.parametrize("x_kind", KINDS, ids=str)
+def test_broadcast_row(x_kind):
+    """Many equal rows, and an out whose rows lie far apart."""
+    weight, w = _weight(40, 256, 9)
+    row = torch.randn(1, 256, device="cuda").to(x_kind or torch.float32)
+    x = row.repeat(70, 1)
+    x = capi.mx_quantize(x) if x_kind is None else x
+    far = torch.zeros(70, 1 << 16, device="cuda")
+    got = capi.mx_linear(x, weight, out=far[:, 7:47])
+    assert torch.equal(got, got[:1].expand(70, 40)) and far.count_nonzero() == got.count_nonzero()
+
+
 def test_mlp_in_four_bits():
     """Quantise, product with GELU, quantise, product onto the residual, as an MLP runs them:
     every step against float64 on its own inputs."""

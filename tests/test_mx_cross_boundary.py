@@ -106,14 +106,15 @@ def _strides(**at):
 
 
 @pytest.mark.parametrize("changes", [
-    dict(batch=-1), dict(lq=-1), dict(lk=-1), dict(lq=(1 << 30) + 1), dict(heads=0), dict(kv_heads=0),
+    dict(batch=-1), dict(lq=-1), dict(lk=-1), dict(lq=(1 << 30) + 1), dict(lq=1 << 30), dict(lk=(1 << 30) + 1),
+    dict(heads=0), dict(kv_heads=0),
     dict(kv_heads=3), dict(heads=65536, kv_heads=1), dict(head_dim=0), dict(head_dim=60), dict(head_dim=264),
     dict(dtype=3), dict(out_dtype=-1), dict(scale=float("nan")), dict(scale=float("inf")), dict(q=None),
     dict(k=None), dict(v=None), dict(out=None), dict(strides=None), dict(q=P + 8), dict(k=2 * P + 2),
     dict(v=3 * P + 4), dict(out=4 * P + 1), _strides(s0=2564), _strides(s1=260), _strides(s2=68), _strides(s4=129),
     _strides(s7=-128), _strides(s3=-8), _strides(s10=255), _strides(s11=63), _strides(s9=2559), _strides(s11=0), _strides(s4=(1 << 23) + 8, s3=1 << 30), _strides(s7=1 << 24, s6=1 << 30),
     dict(q_offsets=P), dict(k_offsets=P), dict(q_offsets=P, k_offsets=P, key_lengths=P),
-    dict(q_offsets=P + 2, k_offsets=P), dict(key_lengths=P + 1), dict(key_mask=P, mask_stride=19),
+    dict(q_offsets=P + 2, k_offsets=P), dict(key_lengths=P + 1), dict(key_mask=P, mask_stride=-1), dict(key_mask=P, mask_stride=1 << 41),
     dict(out=P, out_dtype=F32), dict(out=P, **_strides(s10=512, s9=5120)), dict(out=2 * P), dict(out=3 * P),
     dict(workspace=P + 8, workspace_bytes=64)], ids=str)
 def test_cross_attention_refuses(changes):
