@@ -604,7 +604,8 @@ S2_API int s2_mx_quantize(const void* x, s2_dtype x_dtype, long x_stride, int m,
                           void* codes, long code_stride, void* scales, long scale_stride,
                           s2_stream_t stream);
 /* The values of MXFP4 rows, rounded to y_dtype (fp32 and bf16 hold them all up to their
- * largest numbers, fp16 those of rows quantised from fp16). */
+ * largest numbers, which scales from 253 on can pass, fp16 those of rows quantised from
+ * fp16).  s2_mx_weight_linear takes a weight's values as bf16, infinities where they pass it. */
 S2_API int s2_mx_dequantize(const void* codes, long code_stride, const void* scales,
                             long scale_stride, int m, int k, void* y, s2_dtype y_dtype,
                             long y_stride, s2_stream_t stream);
@@ -618,9 +619,9 @@ S2_API int s2_mx_dequantize(const void* codes, long code_stride, const void* sca
  *   codes past it are zeros in x or in the weight, as s2_mx_quantize writes them.
  * bias, activation, residual, y: as for s2_linear; m, n and k up to 2^30.
  * workspace: 16-byte aligned (calls that may overlap in time need one each); the queries
- *   give what the fastest form takes, whatever the operands' strides and addresses.  A smaller one, or NULL, is
- *   accepted: the call then does without, slower for many rows of x in x_dtype, for few
- *   output tiles and for scales that start at no 16 bytes. */
+ *   give what the fastest form takes, whatever the operands' strides and addresses.  A
+ *   smaller one, or NULL, is accepted: the call then does without, slower for many rows,
+ *   for few output tiles and for scales that start at no 16 bytes. */
 S2_API int s2_mx_linear_workspace_bytes(int m, int n, int k, s2_dtype y_dtype, size_t* bytes);
 S2_API int s2_mx_linear(const void* x_codes, long x_code_stride, const void* x_scales,
                         long x_scale_stride, int m, const void* w_codes, const void* w_scales,

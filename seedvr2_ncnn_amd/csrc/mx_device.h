@@ -28,7 +28,7 @@ __device__ __forceinline__ f32x4 mx_mfma(uint4 a, uint4 b, f32x4 c, uint32_t sa,
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, y, c, 4, 4, ABYTE, (int)sa, BBYTE, (int)sb);
 }
 
-// Eight codes as bf16, which holds every code times a scale.
+// Eight codes as bf16, which holds every code times a scale up to its largest number.
 __device__ __forceinline__ uint4 mx_bf16(uint32_t codes, float scale) {
     return make_uint4(
         __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 0)),

@@ -195,11 +195,9 @@ constexpr int kSplitBytes = 48 << 10;   // of LDS for terms of x
 template <int XT, int NT>
 hipError_t run_rows(const MxLinearArgs& a, hipStream_t stream) {
     const int ntiles = (a.n + 16 * NT - 1) / (16 * NT);
-    const long blocks = ((long)a.m + 15) / 16 * ntiles;
-    if (blocks > 0x7fffffffL) return hipErrorInvalidValue;
     const int parts = (mx_blocks(a.k) + 7) / 8;
     const int waves = std::min(8, parts);
-    const unsigned nb = (unsigned)blocks;
+    const unsigned nb = (unsigned)(((long)a.m + 15) / 16 * ntiles);
     if constexpr (XT == 1 || XT == 3) {
         const int part = std::min(a.m, 16) * MxX<XT>::TERMS * 2 * 256;   // bytes of 256 k
         // fp16 rows that several rounds of splitting would take are split by each wave (16 x
@@ -241,6 +239,24 @@ double rows_us(const MxLinearArgs& a) {
 template <int XT>
 hipError_t launch_rows(const MxLinearArgs& a, hipStream_t stream) {
     const int t = rows_tiles(a);
+    const long row_blocks = ((long)a.m + 15) / 16, columns = (a.n + 16L * t - 1) / (16 * t);
+    if (row_blocks * columns * 512 >= 1L << 32) {   // threads of a launch
+        if (row_blocks < 2) return hipErrorInvalidValue;
+        MxLinearArgs first = a, second = a;
+        const long m = row_blocks / 2 * 16, ye = a.y_kind ? 2 : 4;
+        first.m = (int)m;
+        second.m -= (int)m;
+        if (XT == 0) {
+            second.xq.codes += m * a.xq.code_stride;
+            second.xq.scales += m * a.xq.scale_stride;
+        } else {
+            second.x = (const char*)a.x + m * a.x_stride * (XT == 1 ? 4 : 2);
+        }
+        if (a.res) second.res = (const char*)a.res + m * a.res_stride * ye;
+        second.y = (char*)a.y + m * a.y_stride * ye;
+        const hipError_t e = launch_rows<XT>(first, stream);
+        return e != hipSuccess ? e : launch_rows<XT>(second, stream);
+    }
     return t == 4 ? run_rows<XT, 4>(a, stream) : t == 2 ? run_rows<XT, 2>(a, stream) : run_rows<XT, 1>(a, stream);
 }
 
@@ -297,7 +313,10 @@ MatmulArgs codes_args(const MxLinearArgs& a) {
     return m;
 }
 
-constexpr int kRowsMost = 32;   // rows of codes that the kernel for few rows takes
+// Rows of codes that the kernel for few rows takes, one round of 16: 16 x 2560 by 15360 x 2560 8.1
+// us, 17 rows 13.1, 7.6 on tiles; 17 x 10240 by 2560 x 10240 13.4 and 9.4, 17 x 2560 by 2560 x
+// 2560 5.5 and 7.3.
+constexpr int kRowsMost = 16;
 
 // Many rows of other types: x as planes of bf16 terms (or as it is, in bf16 with 16-byte
 // rows) and the weight's values in bf16, for the tile kernels of 16-bit operands.

@@ -164,6 +164,17 @@ def test_far_rows_of_keys(dtype):
         ro.check(got[0], *_sample(q[0, :lq], k[0], v[0], 64 ** -0.5, None, dtype))
 
 
+@pytest.mark.parametrize("batch,heads", [(1 << 20, 20), ((1 << 24) + 2, 1)])
+def test_more_tiles_than_a_launch_has(batch, heads):
+    """A key a sample: out is v, to the bit, and nought where the key is masked."""
+    v = torch.arange(batch * heads * 8, device="cuda").remainder_(253).bfloat16().view(batch, 1, heads, 8)
+    lengths = (torch.arange(batch, device="cuda") % 7 != 0).int()
+    mask = torch.arange(batch, device="cuda").view(batch, 1) % 5 != 0
+    got = capi.cross_attention(v, v, v, key_lengths=lengths, key_mask=mask)
+    v[(lengths == 0) | ~mask[:, 0]] = 0
+    assert torch.equal(got, v)
+
+
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
 @pytest.mark.parametrize("out_dtype", TYPES, ids=str)
 def test_out_types_and_scales(dtype, out_dtype):

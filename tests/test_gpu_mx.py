@@ -289,6 +289,27 @@ def test_broadcast_row(x_kind):
     assert torch.equal(got, got[:1].expand(70, 40)) and far.count_nonzero() == got.count_nonzero()
 
 
+@pytest.mark.parametrize("x_kind", KINDS, ids=str)
+@pytest.mark.parametrize("m", [9, 16, 17])
+def test_wide_weight(x_kind, m):
+    """64 columns a workgroup, and as much of x as they hold at once."""
+    none = torch.empty(0, dtype=torch.uint8, device="cuda")
+    _product(m, 12300, 2600, x_kind, torch.float32, "none", False, False, workspace=none)
+
+
+@pytest.mark.parametrize("x_kind", [None, torch.bfloat16], ids=str)
+def test_more_tiles_than_a_launch_has(x_kind):
+    none = torch.empty(0, dtype=torch.uint8, device="cuda")
+    weight, _ = _weight(8192, 32, 10, stride=17)   # (scales that tiles would copy)
+    m, some = (1 << 20) + 20, 37
+    x = torch.randn(some, 32, device="cuda").bfloat16()
+    rows = x.repeat((m + some - 1) // some, 1)[:m]
+    first = capi.mx_linear(capi.mx_quantize(x) if x_kind is None else x, weight, workspace=none)
+    got = capi.mx_linear(capi.mx_quantize(rows) if x_kind is None else rows, weight, workspace=none)
+    whole = m // some * some
+    assert (got[:whole].view(-1, some, 8192) == first).all() and torch.equal(got[whole:], first[:m - whole])
+
+
 def test_mlp_in_four_bits():
     """Quantise, product with GELU, quantise, product onto the residual, as an MLP runs them:
     every step against float64 on its own inputs."""
