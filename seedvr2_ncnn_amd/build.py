@@ -40,7 +40,7 @@ HIP_SOURCES = ["awa_kernels.hip", "linear_kernels.hip", "pipeline_kernels.hip", 
                "conv3d_kernels.hip", "conv3d_narrow_kernels.hip", "mha_kernels.hip", "graph_ops_kernels.hip",
                "group_norm_kernels.hip", "matmul_kernels.hip", "matmul_tile_kernels.hip",
                "matmul_rows_kernels.hip", "matmul_short_kernels.hip", "mx_quantize_kernels.hip",
-               "mx_linear_kernels.hip", "mx_tile_kernels.hip", "cross_attention_kernels.hip",
+               "mx_linear_kernels.hip", "mx_tile_kernels.hip", "mx_weight_kernels.hip", "cross_attention_kernels.hip",
                "cross_tile_kernels.hip", "cross_f32_kernels.hip", "capi.hip",
                "awa_plan.cpp", "stream_scratch.cpp"]
 LAYER_SOURCES = ["ncnn/mat.cpp", "ncnn/layer.cpp", "ncnn/net.cpp", "ncnn/builtin_layers.cpp",

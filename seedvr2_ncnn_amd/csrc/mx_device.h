@@ -12,6 +12,12 @@ typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
 constexpr uint32_t kMxNan = 255;   // the scale of a block without values
 
+// Byte b of four scales as what the conversions of codes take: they read the exponent field
+// alone, 2^-127 for 0 and a NaN for 255.
+__device__ __forceinline__ float mx_scale_of(uint32_t scales, int b) {
+    return __uint_as_float(b == 3 ? scales >> 1 : scales << (23 - 8 * b));
+}
+
 // 2^(scale - 127); a NaN for 255
 __device__ __forceinline__ float mx_scale(uint32_t scale) {
     return __uint_as_float(scale == 0 ? 0x00400000u : scale == kMxNan ? 0x7fc00000u : scale << 23);

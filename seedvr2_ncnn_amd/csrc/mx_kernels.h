@@ -6,7 +6,8 @@
 //
 //   mx_quantize_kernels.hip  rows to MXFP4 and back
 //   mx_linear_kernels.hip    which kernel takes a product; few rows
-//   mx_tile_kernels.hip      block tiles
+//   mx_tile_kernels.hip      block tiles of codes
+//   mx_weight_kernels.hip    block tiles of 16-bit rows and a weight's codes
 #pragma once
 
 #include "matmul_kernels.h"
@@ -68,6 +69,10 @@ struct MxTileScales {
 // workspace: mx_dealt_bytes for a 256 x 256 tile.
 hipError_t launch_mx_tiles(const MatmulArgs& a, const MxTileScales& scales, const TileChoice& tile,
                            float* sums, void* workspace, hipStream_t stream);
+
+// a: the product with x as bf16 rows, or planes of them; its weight the codes.
+hipError_t launch_mx_weight_tiles(const MatmulArgs& a, const MxTileScales& scales, const TileChoice& tile,
+                                  float* sums, hipStream_t stream);
 
 size_t mx_linear_workspace(const MxLinearArgs& a);
 hipError_t launch_mx_linear(const MxLinearArgs& a, void* workspace, size_t workspace_bytes,

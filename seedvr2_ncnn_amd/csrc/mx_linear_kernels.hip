@@ -130,7 +130,7 @@ __global__ __launch_bounds__(512) void mx_rows_kernel(MxLinearArgs a, int ntiles
 #pragma unroll
                     for (int j = 0; j < NT; ++j) {
                         const uint32_t q4[4] = {p.w[c][j].x, p.w[c][j].y, p.w[c][j].z, p.w[c][j].w};
-                        const uint4 w = mx_bf16(q4[e], mx_scale(p.ws[c][j]));
+                        const uint4 w = mx_bf16(q4[e], mx_scale_of(p.ws[c][j], 0));
 #pragma unroll
                         for (int q = 0; q < X::TERMS; ++q) acc[j] = mfma<1>(w, t[q], acc[j]);
                     }
@@ -232,8 +232,10 @@ double rows_us(const MxLinearArgs& a) {
     const double each = a.x_kind == S2_DTYPE_F32 ? 1.1 + 0.6 * at + 0.4 * std::min(a.m, 16)
                                                  : one[a.x_kind == S2_DTYPE_F16][at];
     const long blocks = ((long)a.m + 15) / 16 * ((a.n + 16 * t - 1) / (16 * t));
-    const long units = t == 1 ? 2 * kUnits : kUnits;   // workgroups at once
-    return 2.5 + (double)((blocks + units - 1) / units) * ((mx_blocks(a.k) + 63) / 64) * each;
+    // workgroups of 16 columns run two on a unit, one and a half times as long
+    const double rounds = t == 1 ? (double)((blocks + 2 * kUnits - 1) / (2 * kUnits)) * (blocks > kUnits ? 1.6 : 1.)
+                                 : (double)((blocks + kUnits - 1) / kUnits);
+    return 2.5 + rounds * ((mx_blocks(a.k) + 63) / 64) * each;
 }
 
 template <int XT>
@@ -318,31 +320,58 @@ MatmulArgs codes_args(const MxLinearArgs& a) {
 // 2560 5.5 and 7.3.
 constexpr int kRowsMost = 16;
 
-// Many rows of other types: x as planes of bf16 terms (or as it is, in bf16 with 16-byte
-// rows) and the weight's values in bf16, for the tile kernels of 16-bit operands.
+// Rows of other types on tiles: x as planes of bf16 terms (or as it is, in bf16 with 16-byte
+// rows), the weight's codes as they are, or its values in bf16 for the tile kernels of
+// 16-bit operands, where the largest tiles pay for that.
 struct ValuesPlan {
     TileChoice tile;
-    bool pack_x;
+    bool pack_x, codes;
     int planes, width;       // of packed x; k rounded up to 8 where it is not packed
     size_t x_bytes, w_bytes, sum_bytes;
     size_t bytes() const { return x_bytes + w_bytes + sum_bytes; }
-    // a launch, bytes a microsecond read and written
-    double us() const { return tile.us + 7. + (2.3 * x_bytes + 1.3 * w_bytes) / 5.5e6; }
+    // launches, bytes a microsecond read and written
+    double us() const { return tile.us + 2. + (codes && pack_x ? 3. : 0.) + (2.3 * x_bytes + 1.3 * w_bytes) / 5.5e6; }
 };
 
-ValuesPlan values_plan(const MxLinearArgs& a, size_t workspace_bytes) {
+// What tiles of the weight's codes take, in microseconds: a workgroup's first loads and
+// epilogue, and 256 k, for which its compute unit gets 50 or 41 KB through the caches.
+struct WeightCost {
+    int bm, bn;
+    double round, step;
+};
+constexpr WeightCost kWeightCosts[] = {{64, 128, 2.8, 1.28}, {64, 64, 3., 0.8}};
+
+TileChoice weight_tiles(const MxLinearArgs& a, long steps, long most) {
+    TileChoice best{0., 0, 0, 1};
+    const double each = (double)a.m * round_up(a.n, 4) * sizeof(float);   // a range's sums
+    for (const WeightCost& t : kWeightCosts) {
+        const long count = ((long)a.m + t.bm - 1) / t.bm * ((a.n + t.bn - 1) / t.bn);
+        for (long parts = 1; parts <= std::max<long>(1, std::min(most, steps / 2)); ++parts) {
+            const double rounds = (double)((count * parts + kUnits - 1) / kUnits);
+            const double us = rounds * (t.round + t.step * (double)((steps + parts - 1) / parts)) +
+                              (parts > 1 ? 3. + 2. * parts * each / 9e6 : 0.);
+            if (best.us == 0. || us < best.us) best = TileChoice{us, t.bm, t.bn, (int)parts};
+        }
+    }
+    return best;
+}
+
+ValuesPlan values_plan(const MxLinearArgs& a, bool codes, size_t workspace_bytes) {
     ValuesPlan p{};
     const long k8 = round_up(a.k, 8);
+    p.codes = codes;
     p.planes = a.x_kind == S2_DTYPE_F32 ? kTerms : a.x_kind == S2_DTYPE_F16 ? 2 : 1;
     p.pack_x = p.planes > 1 || a.k % 8 != 0 || a.x_stride % 8 != 0 || (uintptr_t)a.x % 16 != 0;
     p.width = (int)round_up(a.k, 64);
     if (p.pack_x) p.x_bytes = round_up((size_t)a.m * p.planes * p.width * 2, 256);
-    p.w_bytes = round_up((size_t)a.n * k8 * 2, 256);
+    if (!codes) p.w_bytes = round_up((size_t)a.n * k8 * 2, 256);
     if (p.bytes() > workspace_bytes) return p;
     MatmulArgs m = values_args(a, nullptr);
     m.k = (int)k8;
     const size_t each = (size_t)a.m * round_up(a.n, 4) * sizeof(float);
-    p.tile = choose_tiles(m, (k8 + 63) / 64 * p.planes, std::min<long>(16, (long)((workspace_bytes - p.bytes()) / each)));
+    const long most = std::min<long>(16, (long)((workspace_bytes - p.bytes()) / each));
+    p.tile = codes ? weight_tiles(a, (k8 + 255) / 256 * p.planes, most)
+                   : choose_tiles(m, (k8 + 63) / 64 * p.planes, most);
     p.sum_bytes = p.tile.parts > 1 ? p.tile.parts * each : 0;
     return p;
 }
@@ -366,7 +395,7 @@ __global__ __launch_bounds__(256) void mx_values_kernel(MxLinearArgs a, uint16_t
             const int at = (int)(i - nx - row * ww);   // of four bytes
             const uint32_t codes = *reinterpret_cast<const uint32_t*>(a.w.codes + row * a.w.code_stride + 4 * at);
             *reinterpret_cast<uint4*>(w + (row * ww + at) * 8) =
-                mx_bf16(codes, mx_scale(a.w.scales[row * a.w.scale_stride + (at >> 2)]));
+                mx_bf16(codes, mx_scale_of(a.w.scales[row * a.w.scale_stride + (at >> 2)], 0));
         }
     }
 }
@@ -380,10 +409,12 @@ hipError_t launch_values(const MxLinearArgs& a, const ValuesPlan& p, void* works
     const int xw = p.pack_x ? p.width / 8 : 0, ww = m.k / 8;
     MxLinearArgs job = a;
     if (!p.pack_x) job.m = 0;
-    const long all = (long)job.m * xw + (long)a.n * ww;
-    mx_values_kernel<XT><<<(unsigned)std::min<long>((all + 255) / 256, 65536), 256, 0, stream>>>(job, x, xw, w, ww);
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
+    if (p.codes) job.n = 0;
+    if (const long all = (long)job.m * xw + (long)job.n * ww) {
+        mx_values_kernel<XT><<<(unsigned)std::min<long>((all + 255) / 256, 65536), 256, 0, stream>>>(job, x, xw, w, ww);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
     m.x_kind = S2_DTYPE_BF16;
     if (p.pack_x) {
         m.x = x;
@@ -391,13 +422,18 @@ hipError_t launch_values(const MxLinearArgs& a, const ValuesPlan& p, void* works
         m.planes = p.planes;
         m.plane = p.width;
     }
+    float* sums = (float*)((char*)w + p.w_bytes);
+    if (p.codes) {
+        m.w = a.w.codes;
+        return launch_mx_weight_tiles(m, {nullptr, 0, a.w.scales, a.w.scale_stride, mx_blocks(a.k)}, p.tile, sums, stream);
+    }
     MatmulPlan t{};
     t.kernel = MatmulPlan::kTiles;
     t.bm = p.tile.bm;
     t.bn = p.tile.bn;
     t.parts = p.tile.parts;
     t.whole = whole_pieces(m);
-    return launch_matmul_tiles(m, t, (float*)((char*)w + p.w_bytes), stream);
+    return launch_matmul_tiles(m, t, sums, stream);
 }
 
 // Ranges of k, at most, whose sums fit `bytes`.
@@ -439,9 +475,14 @@ size_t mx_linear_workspace(const MxLinearArgs& a) {
     if (!a.mx) {
         MxLinearArgs far = a;
         far.x_stride = a.k + 1;   // rows that are packed
-        const ValuesPlan p = values_plan(far, (size_t)1 << 62);
-        far.x_stride = round_up(a.k, 8);
-        return std::min(p.us(), values_plan(far, (size_t)1 << 62).us()) < rows_us(a) ? p.bytes() : 0;
+        size_t most = 0;
+        for (bool codes : {false, true}) {
+            const ValuesPlan p = values_plan(far, codes, (size_t)1 << 62);
+            MxLinearArgs near = a;
+            near.x_stride = round_up(a.k, 8);
+            if (std::min(p.us(), values_plan(near, codes, (size_t)1 << 62).us()) < rows_us(a)) most = std::max(most, p.bytes());
+        }
+        return most;
     }
     if (a.m <= kRowsMost) return 0;
     return mx_plan(a, true, true, (size_t)1 << 62).bytes();
@@ -464,9 +505,14 @@ hipError_t launch_mx_linear(const MxLinearArgs& args, void* workspace, size_t wo
     if (!a.mx) {
         if (256 * out < far && (long)a.n * 4 < far && 256 * 2 * a.x_stride < far &&
             256 * 2 * kTerms * (a.k + 64L) < far) {
-            const ValuesPlan p = values_plan(a, workspace_bytes);
-            // 500 x 2560 in bf16 by 15360 x 2560 60 us, 235 by the kernel for few rows; 77 x 5120 by
-            // 2560 x 5120 28 and 18
+            ValuesPlan p = values_plan(a, false, workspace_bytes);
+            if (scales16(a.w.scales, a.w.scale_stride) && 256 * a.w.scale_stride < far) {
+                const ValuesPlan c = values_plan(a, true, workspace_bytes);
+                if (c.tile.bm && (!p.tile.bm || c.us() < p.us())) p = c;
+            }
+            // In bf16 by rows, with the weight's values and with its codes on tiles: 77 x 5120 by
+            // 2560 x 5120 14.6, 26, 12.9 us; 128 x 2560 by 15360 x 2560 66, 41, 17; 500 x 2560 by
+            // the same 242, 60, 64; 1000 x 2560 77 and 127; 48 x 2560 by 2560 x 2560 7.2, 18, 8.8.
             if (p.tile.bm && p.us() < rows_us(a))
                 return a.x_kind == 0   ? launch_values<1>(a, p, workspace, stream)
                        : a.x_kind == 1 ? launch_values<2>(a, p, workspace, stream)

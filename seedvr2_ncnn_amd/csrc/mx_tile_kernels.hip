@@ -7,30 +7,11 @@
 // does four times the k.  What comes with it are the scales: 16 bytes of a row (two
 // steps) are one lane's DMA, and a lane takes those of its blocks g and 4 + g out of the
 // eight of a step.
-#include "matmul_tiles.h"
-#include "mx_device.h"
+#include "mx_tiles.h"
 
 namespace s2 {
 
 namespace {
-
-// DMA of the scales of 64 rows, a row a lane.
-struct ScaleLoad {
-    i32x4 rsrc;
-    uint32_t vo;
-};
-
-// LDS row r of x is row r.  Of each 64 weight rows, LDS row 16 j + c is row 4 c + j.
-// rows: from base on; block: of 64 rows.
-template <bool WEIGHT>
-__device__ __forceinline__ ScaleLoad scale_load(const uint8_t* base, int rows, long ld, int blocks,
-                                                int block) {
-    const int lane = threadIdx.x & 63;
-    const int row = 64 * block + (WEIGHT ? 4 * (lane & 15) + (lane >> 4) : lane);
-    // whole dwords: rows begin at 16 bytes, so the last one's is no one else's
-    const long bytes = rows > 0 ? (long)(rows - 1) * ld + (blocks + 3) / 4 * 4 : 0;
-    return ScaleLoad{wave_uniform(buffer_rsrc(base, (uint32_t)bytes)), (uint32_t)(row * ld)};
-}
 
 // The scales of a lane's blocks g and 4 + g of step s, in the lowest bytes.
 __device__ __forceinline__ uint2 scale_pair(const uint8_t* row, int s) {
@@ -45,8 +26,6 @@ __device__ __forceinline__ uint2 scales_past(uint2 pair, int left) {
     const int g = (threadIdx.x & 63) >> 4;
     return make_uint2(g >= left ? 127u : pair.x, 4 + g >= left ? 127u : pair.y);
 }
-
-constexpr int kScaleRow = 16;   // bytes of a row's scales in LDS: two steps
 
 // The step after which a tile's scales are past the row, and how many blocks it has.
 struct LastStep {
