@@ -43,6 +43,15 @@ __device__ __forceinline__ uint4 mx_bf16(uint32_t codes, float scale) {
         __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 3)));
 }
 
+// Eight codes as fp16.
+__device__ __forceinline__ uint4 mx_f16(uint32_t codes) {
+    return make_uint4(
+        __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, 1.f, 0)),
+        __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, 1.f, 1)),
+        __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, 1.f, 2)),
+        __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, 1.f, 3)));
+}
+
 // Eight fp16 values as two bf16 terms each, whose sum is exact: 11 bits, by truncation the
 // first eight and the rest.
 __device__ __forceinline__ void mx_terms16(uint4 v, uint4 (&t)[2]) {

@@ -232,9 +232,8 @@ double rows_us(const MxLinearArgs& a) {
     const double each = a.x_kind == S2_DTYPE_F32 ? 1.1 + 0.6 * at + 0.4 * std::min(a.m, 16)
                                                  : one[a.x_kind == S2_DTYPE_F16][at];
     const long blocks = ((long)a.m + 15) / 16 * ((a.n + 16 * t - 1) / (16 * t));
-    // workgroups of 16 columns run two on a unit, one and a half times as long
-    const double rounds = t == 1 ? (double)((blocks + 2 * kUnits - 1) / (2 * kUnits)) * (blocks > kUnits ? 1.6 : 1.)
-                                 : (double)((blocks + kUnits - 1) / kUnits);
+    // a unit runs two workgroups at once, 1.6 times as long
+    const double rounds = (double)((blocks + 2 * kUnits - 1) / (2 * kUnits)) * (blocks > kUnits ? 1.6 : 1.);
     return 2.5 + rounds * ((mx_blocks(a.k) + 63) / 64) * each;
 }
 
@@ -334,21 +333,22 @@ struct ValuesPlan {
 };
 
 // What tiles of the weight's codes take, in microseconds: a workgroup's first loads and
-// epilogue, and 256 k, for which its compute unit gets 50 or 41 KB through the caches.
+// epilogue, and 256 k, for which its compute unit gets 50 or 41 KB through the caches; by
+// rows in fp16, whose blocks' sums take their scales one by one.
 struct WeightCost {
     int bm, bn;
-    double round, step;
+    double round, step, step_f16;
 };
-constexpr WeightCost kWeightCosts[] = {{64, 128, 2.8, 1.28}, {64, 64, 3., 0.8}};
+constexpr WeightCost kWeightCosts[] = {{64, 128, 2.8, 1.28, 1.8}, {64, 64, 3., 0.8, 1.27}};
 
-TileChoice weight_tiles(const MxLinearArgs& a, long steps, long most) {
+TileChoice weight_tiles(const MxLinearArgs& a, bool f16, long steps, long most) {
     TileChoice best{0., 0, 0, 1};
     const double each = (double)a.m * round_up(a.n, 4) * sizeof(float);   // a range's sums
     for (const WeightCost& t : kWeightCosts) {
         const long count = ((long)a.m + t.bm - 1) / t.bm * ((a.n + t.bn - 1) / t.bn);
         for (long parts = 1; parts <= std::max<long>(1, std::min(most, steps / 2)); ++parts) {
             const double rounds = (double)((count * parts + kUnits - 1) / kUnits);
-            const double us = rounds * (t.round + t.step * (double)((steps + parts - 1) / parts)) +
+            const double us = rounds * (t.round + (f16 ? t.step_f16 : t.step) * (double)((steps + parts - 1) / parts)) +
                               (parts > 1 ? 3. + 2. * parts * each / 9e6 : 0.);
             if (best.us == 0. || us < best.us) best = TileChoice{us, t.bm, t.bn, (int)parts};
         }
@@ -360,8 +360,9 @@ ValuesPlan values_plan(const MxLinearArgs& a, bool codes, size_t workspace_bytes
     ValuesPlan p{};
     const long k8 = round_up(a.k, 8);
     p.codes = codes;
-    p.planes = a.x_kind == S2_DTYPE_F32 ? kTerms : a.x_kind == S2_DTYPE_F16 ? 2 : 1;
-    p.pack_x = p.planes > 1 || a.k % 8 != 0 || a.x_stride % 8 != 0 || (uintptr_t)a.x % 16 != 0;
+    const bool rows16 = a.k % 8 == 0 && a.x_stride % 8 == 0 && (uintptr_t)a.x % 16 == 0;
+    p.planes = a.x_kind == S2_DTYPE_F32 ? kTerms : a.x_kind == S2_DTYPE_F16 && !(codes && rows16) ? 2 : 1;
+    p.pack_x = p.planes > 1 || !rows16;
     p.width = (int)round_up(a.k, 64);
     if (p.pack_x) p.x_bytes = round_up((size_t)a.m * p.planes * p.width * 2, 256);
     if (!codes) p.w_bytes = round_up((size_t)a.n * k8 * 2, 256);
@@ -370,7 +371,7 @@ ValuesPlan values_plan(const MxLinearArgs& a, bool codes, size_t workspace_bytes
     m.k = (int)k8;
     const size_t each = (size_t)a.m * round_up(a.n, 4) * sizeof(float);
     const long most = std::min<long>(16, (long)((workspace_bytes - p.bytes()) / each));
-    p.tile = codes ? weight_tiles(a, (k8 + 255) / 256 * p.planes, most)
+    p.tile = codes ? weight_tiles(a, a.x_kind == S2_DTYPE_F16 && p.planes == 1, (k8 + 255) / 256 * p.planes, most)
                    : choose_tiles(m, (k8 + 63) / 64 * p.planes, most);
     p.sum_bytes = p.tile.parts > 1 ? p.tile.parts * each : 0;
     return p;
@@ -415,7 +416,7 @@ hipError_t launch_values(const MxLinearArgs& a, const ValuesPlan& p, void* works
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
-    m.x_kind = S2_DTYPE_BF16;
+    if (p.pack_x || !p.codes) m.x_kind = S2_DTYPE_BF16;   // else fp16 stays
     if (p.pack_x) {
         m.x = x;
         m.x_stride = (long)p.planes * p.width;

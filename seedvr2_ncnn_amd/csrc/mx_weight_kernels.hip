@@ -1,15 +1,18 @@
-// Products of bf16 rows with weights in MXFP4 on block tiles.
+// Products of 16-bit rows with weights in MXFP4 on block tiles.
 //
 // y = x W^T as W's values in bf16, which hold a code times its scale exactly, on 16x16x32
-// products.  x goes to LDS in steps of 64 k as in the 16-bit products (matmul_tiles.h; fp16
-// and fp32 rows as planes of bf16 terms); the weight as its codes, a quarter of the bytes,
+// products; by fp16 rows the codes alone in fp16 and the scale on each block's sums, a
+// product's 32 k being one block, for fp16 does not reach as far.  x goes to LDS as in the
+// 16-bit products (matmul_tiles.h; fp32 rows, and fp16 ones that begin at no 16 bytes, as
+// planes of bf16 terms); the weight as its codes, a quarter of the bytes,
 // 256 k (128 bytes of a row) at a time, and becomes bf16 in operand registers: four
 // conversions make an operand of a lane's eight codes, which 16 NI rows share.
 //
 // What bounds it are the bytes that a compute unit gets through the caches, about 40 KB a
 // microsecond: 128 x 2560 by 15360 x 2560 17 us, 0.6 PFLOP/s, its bytes once 6.  (In steps
 // of 64 k 30 us, of 256 k with one wave a SIMD 18.4; 41 with the weight's values written
-// for the 16-bit tiles.)
+// for the 16-bit tiles.  By fp16 rows 23, where the scales' products add up, 48 as two planes
+// and 16-bit tiles.)
 #include "mx_tiles.h"
 
 namespace s2 {
@@ -19,7 +22,7 @@ namespace {
 // BM x BN tile, two groups of four waves of 16 NI x 64 (WN of them side by side), 256 k a
 // step, of which each group takes half; their sums meet in LDS at the end.  Wider tiles do
 // not leave LDS for two steps in flight under the products of a third.  a.w: codes.
-template <int YK, int NI, int WN, int STAGES>
+template <int T, int YK, int NI, int WN, int STAGES>
 __global__ __launch_bounds__(512, 1) void mx_weight_kernel(MatmulArgs a, TileSplit sp, MxTileScales sc) {
     constexpr int BM = 16 * NI * (4 / WN), BN = 64 * WN;
     constexpr int RB = kBK * 2, XB = BM * RB, WB = BN * RB;   // of x a quarter of a step
@@ -108,9 +111,18 @@ __global__ __launch_bounds__(512, 1) void mx_weight_kernel(MatmulArgs a, TileSpl
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const uint32_t codes = *(const uint32_t*)(ws + 16 * j * RB + ((4 * grp + b) ^ sw) * 16);
-                const uint4 w = mx_bf16(codes, mx_scale_of(scales[j], b));
+                const uint4 w = T == 1 ? mx_bf16(codes, mx_scale_of(scales[j], b)) : mx_f16(codes);
+                const float scale = mx_scale(scales[j] >> (8 * b) & 255u);
 #pragma unroll
-                for (int i = 0; i < NI; ++i) acc[i][j] = mfma<1>(fx[i], w, acc[i][j]);
+                for (int i = 0; i < NI; ++i) {
+                    if constexpr (T == 1) {
+                        acc[i][j] = mfma<1>(fx[i], w, acc[i][j]);
+                    } else {
+                        const f32x4 v = mfma<2>(fx[i], w, f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) acc[i][j][r] = fmaf(v[r], scale, acc[i][j][r]);
+                    }
+                }
             }
         }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -131,7 +143,7 @@ __global__ __launch_bounds__(512, 1) void mx_weight_kernel(MatmulArgs a, TileSpl
         end.finish(a, acc);
 }
 
-template <int YK>
+template <int T, int YK>
 hipError_t launch(const MatmulArgs& a, const MxTileScales& sc, const TileChoice& t, float* sums, hipStream_t stream) {
     const long mtiles = row_tiles(a, t.bm), ntiles = (a.n + t.bn - 1) / t.bn;
     const long blocks = mtiles * ntiles * t.parts;
@@ -139,20 +151,25 @@ hipError_t launch(const MatmulArgs& a, const MxTileScales& sc, const TileChoice&
     const TileSplit sp{(int)ntiles, (int)mtiles, t.parts, whole_pieces(a), (a.n + 3) / 4 * 4, sums};
     const unsigned nb = (unsigned)blocks;
     if (t.bn == 128)
-        mx_weight_kernel<YK, 2, 2, 3><<<nb, 512, 0, stream>>>(a, sp, sc);
+        mx_weight_kernel<T, YK, 2, 2, 3><<<nb, 512, 0, stream>>>(a, sp, sc);
     else
-        mx_weight_kernel<YK, 1, 1, 3><<<nb, 512, 0, stream>>>(a, sp, sc);
+        mx_weight_kernel<T, YK, 1, 1, 3><<<nb, 512, 0, stream>>>(a, sp, sc);
     if (t.parts > 1) return launch_matmul_sum(a, sp, stream);
     return hipGetLastError();
+}
+
+template <int T>
+hipError_t launch_y(const MatmulArgs& a, const MxTileScales& sc, const TileChoice& t, float* sums, hipStream_t stream) {
+    return a.y_kind == 0   ? launch<T, 0>(a, sc, t, sums, stream)
+           : a.y_kind == 1 ? launch<T, 1>(a, sc, t, sums, stream)
+                           : launch<T, 2>(a, sc, t, sums, stream);
 }
 
 }  // namespace
 
 hipError_t launch_mx_weight_tiles(const MatmulArgs& a, const MxTileScales& scales, const TileChoice& tile, float* sums,
                                   hipStream_t stream) {
-    return a.y_kind == 0   ? launch<0>(a, scales, tile, sums, stream)
-           : a.y_kind == 1 ? launch<1>(a, scales, tile, sums, stream)
-                           : launch<2>(a, scales, tile, sums, stream);
+    return a.x_kind == 2 ? launch_y<2>(a, scales, tile, sums, stream) : launch_y<1>(a, scales, tile, sums, stream);
 }
 
 }  // namespace s2

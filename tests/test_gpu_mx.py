@@ -191,6 +191,26 @@ def test_products_of_far_scales():
 
 
 @pytest.mark.parametrize("x_kind", KINDS, ids=str)
+@pytest.mark.parametrize("m,n", [(3, 96), (130, 96), (1500, 1000), (90, 2560)])
+@pytest.mark.parametrize("low,high", [(0, 4), (0, 190), (180, 210)])
+def test_weights_of_far_scales(x_kind, m, n, low, high):
+    """Scales from the least one on, whose values are subnormal in bf16; sums that are normal."""
+    gen = torch.Generator().manual_seed(4 + low + high)
+    code, scale = torch.randint(0, 16, (n, 704), generator=gen), torch.randint(low, high, (n, 22), generator=gen)
+    rows = (1 + torch.rand(m, 700, generator=gen)) * 1024
+    w = mc.values(code, scale, 704)[:, :700]
+    weight = capi.MxRows(*mc.pack(code, scale), 704)
+    if x_kind is None:
+        xcode, xscale = mc.quantize(torch.nn.functional.pad(rows, (0, 4)))
+        x, xv = capi.MxRows(*mc.pack(xcode, xscale), 704), mc.values(xcode, xscale, 704)[:, :700]
+    else:
+        x = torch.nn.functional.pad(rows, (0, 4)).to(x_kind).cuda()
+        xv = x[:, :700].double().cpu()
+    got = capi.mx_linear(x, weight, out_dtype=torch.float32)
+    ro.check(got, *mc.linear(xv.cuda(), w.cuda(), None, "none", None, torch.float32))
+
+
+@pytest.mark.parametrize("x_kind", KINDS, ids=str)
 @pytest.mark.parametrize("m", [3, 300])
 def test_nan_reaches_its_row_or_column_alone(x_kind, m):
     weight, _ = _weight(70, 320, 1)
@@ -308,6 +328,14 @@ def test_more_tiles_than_a_launch_has(x_kind):
     got = capi.mx_linear(capi.mx_quantize(rows) if x_kind is None else rows, weight, workspace=none)
     whole = m // some * some
     assert (got[:whole].view(-1, some, 8192) == first).all() and torch.equal(got[whole:], first[:m - whole])
+
+
+@pytest.mark.parametrize("x_kind", TYPES, ids=str)
+@pytest.mark.parametrize("m,n,k", [(40, 200, 3000), (65, 513, 264), (129, 2560, 1000), (300, 130, 72), (200, 1543, 8)])
+def test_codes_on_tiles(x_kind, m, n, k):
+    """Rows of other types on tiles of the weight's codes: steps, planes and ranges that end early."""
+    _product(m, n, k, x_kind, torch.float16, "gelu", True, True, seed=m)
+    _product(m, n, k, x_kind, torch.float32, "none", False, False, seed=k, stride=mc.blocks(k) + 1)
 
 
 def test_mlp_in_four_bits():
