@@ -13,6 +13,12 @@
 // rescales cost nothing, and a tile's maxima need not be exchanged between lanes to find
 // that none is due.  Weights are rounded to the operands' type for the second product,
 // at most half a step each, as independent errors of its terms; their sum stays in fp32.
+//
+// On long keys the matrix cores and the exponentials beside them bound it, at the clocks that
+// their power leaves (1.7 GHz): 4096 on 21600 keys, 20 heads of 128, 0.8 ms, 1.1 PFLOP/s;
+// 21600 on 512 130 us, 0.87.  A wave's rows are 32: with 16 a tile's reads of LDS would bound
+// it, 64 do not fit its registers.  Two waves' keys ahead (a second tile's scores before the
+// first one's weights) were slower than three workgroups' waves in turn.
 #include "cross_attention_device.h"
 
 namespace s2 {

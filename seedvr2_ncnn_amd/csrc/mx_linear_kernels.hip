@@ -225,16 +225,16 @@ int rows_tiles(const MxLinearArgs& a) {
 }
 
 // What the kernel for few rows takes with x in other types, in microseconds: a workgroup's
-// rounds of 256 k a wave, which splitting lengthens with the rows.
+// rounds of 256 k a wave, and the splitting of fp32 rows.
 double rows_us(const MxLinearArgs& a) {
     const int t = rows_tiles(a), at = t / 2;
-    constexpr double one[2][3] = {{2.3, 3.0, 4.3}, {3.0, 3.8, 5.3}};   // bf16, fp16
-    const double each = a.x_kind == S2_DTYPE_F32 ? 1.1 + 0.6 * at + 0.4 * std::min(a.m, 16)
-                                                 : one[a.x_kind == S2_DTYPE_F16][at];
+    constexpr double one[3][3] = {{1.1, 1.7, 2.3}, {2.3, 3.0, 4.3}, {3.0, 3.8, 5.3}};   // by x's type
+    const double split = a.x_kind == S2_DTYPE_F32 ? 1. + 0.066 * std::min(a.m, 16) * ((mx_blocks(a.k) + 7) / 8) : 0.;
+    const double each = one[a.x_kind][at] * ((mx_blocks(a.k) + 63) / 64) + split;
     const long blocks = ((long)a.m + 15) / 16 * ((a.n + 16 * t - 1) / (16 * t));
     // a unit runs two workgroups at once, 1.6 times as long
     const double rounds = (double)((blocks + 2 * kUnits - 1) / (2 * kUnits)) * (blocks > kUnits ? 1.6 : 1.);
-    return 2.5 + rounds * ((mx_blocks(a.k) + 63) / 64) * each;
+    return 2.5 + rounds * each;
 }
 
 template <int XT>
@@ -474,15 +474,15 @@ MxPlan mx_plan(const MxLinearArgs& a, bool pack_x, bool pack_w, size_t workspace
 
 size_t mx_linear_workspace(const MxLinearArgs& a) {
     if (!a.mx) {
-        MxLinearArgs far = a;
+        MxLinearArgs near = a, far = a;
+        near.x_stride = round_up(a.k, 8);
         far.x_stride = a.k + 1;   // rows that are packed
         size_t most = 0;
-        for (bool codes : {false, true}) {
-            const ValuesPlan p = values_plan(far, codes, (size_t)1 << 62);
-            MxLinearArgs near = a;
-            near.x_stride = round_up(a.k, 8);
-            if (std::min(p.us(), values_plan(near, codes, (size_t)1 << 62).us()) < rows_us(a)) most = std::max(most, p.bytes());
-        }
+        for (bool codes : {false, true})
+            for (const MxLinearArgs& b : {near, far}) {
+                const ValuesPlan p = values_plan(b, codes, (size_t)1 << 62);
+                if (p.us() < rows_us(a)) most = std::max(most, p.bytes());
+            }
         return most;
     }
     if (a.m <= kRowsMost) return 0;

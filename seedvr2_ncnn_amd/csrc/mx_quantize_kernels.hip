@@ -4,7 +4,9 @@
 // [4, 8) X and e2m1's largest number is 6.  It is the exponent field of the largest bit
 // pattern less two, so no logarithm is taken; x / X is exact and v_cvt_scalef32_pk_fp4_f32
 // rounds it once, to the nearest code, ties to the even one, saturating at 6.  Both
-// kernels move their rows once: memory bounds them.
+// kernels move their rows once: memory bounds them, 21664 x 10240 in bf16 110 and 106 us,
+// 5.1 and 5.3 TB/s of rows and codes (a copy reaches 4.9).  16 or 32 bytes a thread, so that
+// a block is four neighbours and its maximum two lane moves.
 #include "mx_device.h"
 
 namespace s2 {
