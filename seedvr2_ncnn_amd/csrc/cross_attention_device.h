@@ -18,23 +18,11 @@ struct CrossSample {
 
 __device__ __forceinline__ int clamped(int v, int most) { return min(max(v, 0), most); }
 
-__device__ __forceinline__ int sample_queries(const CrossArgs& a, int b) {
-    if (!a.q_offsets) return a.lq;
-    const int start = clamped(a.q_offsets[b], a.lq);
-    return max(clamped(a.q_offsets[b + 1], a.lq) - start, 0);
-}
-
-__device__ __forceinline__ CrossSample cross_sample(const CrossArgs& a, int b) {
-    CrossSample s{0, 0, b, a.lq, a.lk};
-    if (a.q_offsets) {
-        s.q0 = clamped(a.q_offsets[b], a.lq);
-        s.nq = sample_queries(a, b);
-        s.k0 = clamped(a.k_offsets[b], a.lk);
-        s.nk = max(clamped(a.k_offsets[b + 1], a.lk) - (int)s.k0, 0);
-    } else if (a.key_lengths) {
-        s.nk = clamped(a.key_lengths[b], a.lk);
-    }
-    return s;
+// Sample b, of samples one after the other.
+__device__ __forceinline__ CrossSample ragged_sample(const CrossArgs& a, int b) {
+    const int q0 = clamped(a.q_offsets[b], a.lq), q1 = clamped(a.q_offsets[b + 1], a.lq);
+    const int k0 = clamped(a.k_offsets[b], a.lk), k1 = clamped(a.k_offsets[b + 1], a.lk);
+    return CrossSample{q0, k0, b, max(q1 - q0, 0), max(k1 - k0, 0)};
 }
 
 // Tile `tile` of `rows` rows of kv head `head`; the sample's tiles that there are.
@@ -47,18 +35,24 @@ struct CrossTile {
 // The workgroup's tile, or rows 0.  Ordered by part, tile, head: workgroups of one head's
 // tiles follow each other on an XCD, whose L2 then holds the head's keys.  tiles: at most
 // there are.  Samples of any lengths are dealt out over the tiles that they make, found by a
-// scan of 64 offsets at a time.
+// scan of 64 offsets at a time, which are read once where there are no more.
 __device__ __forceinline__ CrossTile cross_tile(const CrossArgs& a, int each, int tiles, int parts) {
     const int group = a.heads / a.kv_heads;
     const int lane = threadIdx.x & 63;
     CrossTile t;
     t.rows = 0;
     int count = tiles;
+    CrossSample s;   // the lane's
+    auto read_lane = [&](int b0) {
+        s = CrossSample{0, 0, b0 + lane, 0, 0};
+        if (b0 + lane < a.batch) s = ragged_sample(a, b0 + lane);
+    };
+    auto made = [&] { return (int)(((long)s.nq * group + each - 1) / each); };
     if (a.q_offsets) {
         count = 0;
         for (int b0 = 0; b0 < a.batch; b0 += 64) {
-            int n = b0 + lane < a.batch ? sample_queries(a, b0 + lane) : 0;
-            n = (int)(((long)n * group + each - 1) / each);
+            read_lane(b0);
+            int n = made();
 #pragma unroll
             for (int o = 32; o; o >>= 1) n += __shfl_xor(n, o);
             count = min(count + n, tiles);   // (descending offsets can make more)
@@ -73,15 +67,15 @@ __device__ __forceinline__ CrossTile cross_tile(const CrossArgs& a, int each, in
     t.head = lid / parts / count;
     if (!a.q_offsets) {
         const int of_sample = (int)(((long)a.lq * group + each - 1) / each);
-        t.s = cross_sample(a, i / of_sample);
+        const int b = i / of_sample;
+        t.s = CrossSample{0, 0, b, a.lq, a.key_lengths ? clamped(a.key_lengths[b], a.lk) : a.lk};
         t.row0 = i % of_sample * each;
         t.rows = (int)min((long)each, (long)a.lq * group - t.row0);
         return t;
     }
     for (int b0 = 0; b0 < a.batch; b0 += 64) {
-        const int nq = b0 + lane < a.batch ? sample_queries(a, b0 + lane) : 0;
-        const int n = (int)(((long)nq * group + each - 1) / each);
-        int upto = n;
+        if (a.batch > 64) read_lane(b0);
+        int upto = made();
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
             const int other = __shfl_up(upto, o);
@@ -89,14 +83,15 @@ __device__ __forceinline__ CrossTile cross_tile(const CrossArgs& a, int each, in
         }
         const uint64_t past = __ballot(upto > i);
         if (past) {
-            const int l = __ffsll((unsigned long long)past) - 1;
-            const int before = l ? __shfl(upto, l - 1) : 0;
-            t.s = cross_sample(a, __builtin_amdgcn_readfirstlane(b0 + l));
-            t.row0 = __builtin_amdgcn_readfirstlane((i - before) * each);
+            const int l = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)past) - 1);
+            auto of_lane = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
+            const int before = l ? __builtin_amdgcn_readlane(upto, max(l - 1, 0)) : 0;
+            t.s = CrossSample{of_lane((int)s.q0), of_lane((int)s.k0), b0 + l, of_lane(s.nq), of_lane(s.nk)};
+            t.row0 = (i - before) * each;
             t.rows = (int)min((long)each, (long)t.s.nq * group - t.row0);
             return t;
         }
-        i -= __builtin_amdgcn_readfirstlane(__shfl(upto, 63));
+        i -= __builtin_amdgcn_readlane(upto, 63);
     }
     return t;
 }
