@@ -143,12 +143,21 @@ struct WaveRows {
         return *(const uint4*)(kl[kk % KA] + (kk / KA * 256 + 16 * h * RB + st));
     }
 
+    __device__ __forceinline__ uint4 value(int dt, int st) const {
+        const uint8_t* p = vl[dt % VA] + (dt / VA * 256 + st);
+        const uint2 v0 = read_columns(p), v1 = read_columns(p + 16 * RB);
+        return make_uint4(v0.x, v0.y, v1.x, v1.y);
+    }
+
     // The tile of keys at LDS offset ST.  between(), after the first reads are on their way,
     // gives the keys that count.
     template <int ST, typename F>
     __device__ __forceinline__ void keys(F&& between) {
-        // (reads ahead where registers are left for them)
-        constexpr int AHEAD = DP == 256 ? 0 : NK;
+        // Reads ahead where registers are left for them: of v under the scores' products and the
+        // softmax, where the compiler would read two operands at a time and wait (4096 on 21600
+        // keys, 20 heads of 128, 807 us, 780 so; 21600 on 512 139 and 134; with heads of 64, four
+        // waves a SIMD, 3% slower)
+        constexpr int AHEAD = DP == 256 ? 0 : NK, VAHEAD = DP == 128 ? ND / 2 : 0;
         uint4 kf[2][NK];
 #pragma unroll
         for (int kk = 0; kk < AHEAD; ++kk) kf[0][kk] = key(0, kk, ST);
@@ -164,6 +173,22 @@ struct WaveRows {
                 for (int i = 0; i < NQ; ++i)
                     s[h][i] = mfma<T>(kf[h][kk], qf[i][kk], kk ? s[h][i] : f32x4{0.f, 0.f, 0.f, 0.f});
             }
+        uint4 vf[ND];
+#pragma unroll
+        for (int dt = 0; dt < VAHEAD; ++dt) vf[dt] = value(dt, ST);
+        asm volatile("" ::: "memory");
+        if constexpr (VAHEAD != 0) {   // reads between the products
+#pragma unroll
+            for (int kk = 0; kk < NK; ++kk) {
+                __builtin_amdgcn_sched_group_barrier(8, NQ, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            }
+#pragma unroll
+            for (int kk = 0; kk < NK; ++kk) {
+                __builtin_amdgcn_sched_group_barrier(8, NQ, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, 2 * VAHEAD / NK, 0);
+            }
+        }
         // other waves' products run beside this wave's exponentials
         __builtin_amdgcn_s_setprio(1);
         if (valid != ~0u) {
@@ -214,11 +239,16 @@ struct WaveRows {
         __builtin_amdgcn_s_setprio(0);
 #pragma unroll
         for (int dt = 0; dt < ND; ++dt) {
-            const uint8_t* p = vl[dt % VA] + (dt / VA * 256 + ST);
-            const uint2 v0 = read_columns(p), v1 = read_columns(p + 16 * RB);
-            const uint4 vf = make_uint4(v0.x, v0.y, v1.x, v1.y);
+            if (dt >= VAHEAD) vf[dt] = value(dt, ST);
 #pragma unroll
-            for (int i = 0; i < NQ; ++i) o[dt][i] = mfma<T>(vf, pb[i], o[dt][i]);
+            for (int i = 0; i < NQ; ++i) o[dt][i] = mfma<T>(vf[dt], pb[i], o[dt][i]);
+        }
+        if constexpr (VAHEAD != 0) {
+#pragma unroll
+            for (int dt = 0; dt < ND; ++dt) {
+                __builtin_amdgcn_sched_group_barrier(8, NQ, 0);
+                if (dt < ND - VAHEAD) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+            }
         }
     }
 
