@@ -137,6 +137,30 @@ __device__ __forceinline__ float sum_groups(float x) {
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+// Keys of the workgroup's sample up to the last one that the mask keeps: padded prompts end
+// there, and so do the ranges of keys.  A wave reads a kilobyte at a time from the end.
+__device__ __forceinline__ int keys_kept(const CrossArgs& a, const CrossTile& t) {
+    typedef uint32_t words __attribute__((ext_vector_type(4), aligned(1)));
+    const uint8_t* mask = a.key_mask + t.s.b * a.mask_batch + t.s.k0;
+    const int lane = threadIdx.x & 63;
+    for (int end = t.s.nk; end > 0; end -= 1024) {
+        const int at = end - 16 * (lane + 1);   // the lane's 16 bytes, or what is left of them
+        int last = -1;
+        if (at >= 0) {
+            const words v = *reinterpret_cast<const words*>(mask + at);
+#pragma unroll
+            for (int w = 0; w < 4; ++w)
+                if (v[w]) last = at + 4 * w + (31 - __builtin_clz(v[w])) / 8;
+        } else {
+            for (int i = 0; i < at + 16; ++i)
+                if (mask[i]) last = i;
+        }
+        const uint64_t some = __ballot(last >= 0);
+        if (some) return __builtin_amdgcn_readlane(last, __ffsll((unsigned long long)some) - 1) + 1;
+    }
+    return 0;
+}
+
 constexpr int kMaskWords = 128;                // of 64 keys: a block of mask bits
 constexpr int kMaskBits = 2 * kMaskWords;      // two blocks in LDS
 

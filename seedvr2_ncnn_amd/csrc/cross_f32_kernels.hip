@@ -32,7 +32,7 @@ __global__ __launch_bounds__(256, WGS) void cross_f32_kernel(CrossArgs a, int ti
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l16 = lane & 15, g = lane >> 4;
-    const int nk = __builtin_amdgcn_readfirstlane(t.s.nk);
+    const int nk = MASK ? keys_kept(a, t) : __builtin_amdgcn_readfirstlane(t.s.nk);
     const int all = (nk + KT - 1) / KT;
     const int kb = (int)((long)all * t.part / parts.parts), ke = (int)((long)all * (t.part + 1) / parts.parts);
     KeyTiles<4, DP, STAGES, MASK, Swizzle32> kv(a, t, nk, kb, (uint32_t)(uintptr_t)lds, bits);
@@ -78,6 +78,7 @@ __global__ __launch_bounds__(256, WGS) void cross_f32_kernel(CrossArgs a, int ti
         kv.await(kt, ke);   // and tile kt - 1 is no longer read
         if (kt + 1 < ke) kv.issue(kt + 1, 1 - decltype(stage)::value, false);
         const uint32_t valid = kv.valid(kt);
+        if (MASK && valid == 0) return;
         f32x4 s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
         for (int kk = 0; kk < NK; ++kk)

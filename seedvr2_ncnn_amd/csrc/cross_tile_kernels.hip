@@ -150,8 +150,8 @@ struct WaveRows {
     }
 
     // The tile of keys at LDS offset ST.  between(), after the first reads are on their way,
-    // gives the keys that count.
-    template <int ST, typename F>
+    // gives the keys that count; MASK: there may be none.
+    template <int ST, bool MASK, typename F>
     __device__ __forceinline__ void keys(F&& between) {
         // Reads ahead where registers are left for them: of v under the scores' products and the
         // softmax, where the compiler would read two operands at a time and wait (4096 on 21600
@@ -163,6 +163,7 @@ struct WaveRows {
         for (int kk = 0; kk < AHEAD; ++kk) kf[0][kk] = key(0, kk, ST);
         asm volatile("" ::: "memory");
         const uint32_t valid = between();
+        if (MASK && valid == 0) return;
         f32x4 s[2][NQ];
 #pragma unroll
         for (int h = 0; h < 2; ++h)
@@ -306,7 +307,7 @@ __global__ __launch_bounds__(256, WGS) void cross_tile_kernel(CrossArgs a, int t
     if (t.rows <= 0) return;   // the whole workgroup
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int row_w = 32 * wave;   // of the wave's first row in the tile
-    const int nk = __builtin_amdgcn_readfirstlane(t.s.nk);
+    const int nk = MASK ? keys_kept(a, t) : __builtin_amdgcn_readfirstlane(t.s.nk);
     const int all = (nk + kTileKeys - 1) / kTileKeys;
     const int kb = (int)((long)all * t.part / parts.parts), ke = (int)((long)all * (t.part + 1) / parts.parts);
 
@@ -336,7 +337,7 @@ __global__ __launch_bounds__(256, WGS) void cross_tile_kernel(CrossArgs a, int t
     auto tile = [&](int kt, auto stage) {
         constexpr int ST = decltype(stage)::value;
         kv.await(kt, ke);   // and tile kt - 1 is no longer read
-        rows.template keys<ST * SB>([&] {   // the loads' issue
+        rows.template keys<ST * SB, MASK>([&] {   // the loads' issue
             if (kt + STAGES - 1 < ke) kv.issue(kt + STAGES - 1, (ST + STAGES - 1) % STAGES, false);
             return kv.valid(kt);
         });
@@ -367,7 +368,7 @@ __global__ __launch_bounds__(256, kShortEach) void cross_short_kernel(CrossArgs 
     const CrossTile t = cross_tile(a, kTileRows * run, tiles, 1);
     if (t.rows <= 0) return;   // the whole workgroup
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int nk = __builtin_amdgcn_readfirstlane(t.s.nk);
+    const int nk = MASK ? keys_kept(a, t) : __builtin_amdgcn_readfirstlane(t.s.nk);
     const int all = (nk + kTileKeys - 1) / kTileKeys;
     typedef KeyTiles<2, DP, TILES, MASK, Swizzle<DP>> Keys;
     Keys kv(a, t, nk, 0, (uint32_t)(uintptr_t)lds, bits);
@@ -393,7 +394,7 @@ __global__ __launch_bounds__(256, kShortEach) void cross_short_kernel(CrossArgs 
             if (first >= t.rows) continue;
             auto tile = [&](auto stage) {
                 constexpr int ST = decltype(stage)::value;
-                if (k0 + ST < all) rows.template keys<ST * SB>([&] { return kv.valid(k0 + ST); });
+                if (k0 + ST < all) rows.template keys<ST * SB, MASK>([&] { return kv.valid(k0 + ST); });
             };
             tile(std::integral_constant<int, 0>{});
             tile(std::integral_constant<int, 1>{});

@@ -134,6 +134,17 @@ def test_one_mask_for_all_samples(dtype, lq):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("d", [64, 104, 256])
+@pytest.mark.parametrize("lq", [3, 700])
+@pytest.mark.parametrize("kept", [(0, 40), (999, 1000), (96, 128), (200, 900)])
+def test_whole_tiles_left_out(dtype, d, lq, kept):
+    keys = torch.arange(1000, device="cuda")
+    mask = (keys >= kept[0]) & (keys < kept[1])
+    both = torch.stack([mask, keys % 300 == 5])
+    _padded(2, lq, 1000, 2, 1, d, dtype, mask=both, poison=True)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
 def test_calls_side_by_side(dtype):
     """Two streams at once, each call with a workspace of its own."""
     gen = torch.Generator(device="cuda").manual_seed(11)
