@@ -181,6 +181,7 @@ struct KeyTiles {
     const char* next_k;                     // of the tile that is loaded next
     const char* next_v;
     uint32_t ko[KI], vo[KI];
+    uint32_t ahead = 0;                     // the mask's bits of the tile after the one last loaded
 
     __device__ __forceinline__ KeyTiles(const CrossArgs& a, const CrossTile& t, int keys, int kb, uint32_t lds,
                                         uint64_t* mask_bits)
@@ -199,14 +200,17 @@ struct KeyTiles {
         }
     }
 
-    // keys of tile kt that count
-    __device__ __forceinline__ uint32_t valid(int kt) const {
-        const int left = nk - kt * kTileKeys;
-        uint32_t v = left >= kTileKeys ? ~0u : (1u << left) - 1;
-        if constexpr (MASK)
-            v &= (uint32_t)__builtin_amdgcn_readfirstlane(((const uint32_t*)&bits[kt / 2 % kMaskBits])[kt & 1]);
-        return v;
+    __device__ __forceinline__ uint32_t mask_bits(int kt) const {
+        return ((const uint32_t*)&bits[kt / 2 % kMaskBits])[kt & 1];
     }
+
+    // keys of tile kt that count, of a mask's `kept`
+    __device__ __forceinline__ uint32_t valid(int kt, uint32_t kept) const {
+        const int left = nk - kt * kTileKeys;
+        const uint32_t v = left >= kTileKeys ? ~0u : (1u << left) - 1;
+        return MASK ? v & (uint32_t)__builtin_amdgcn_readfirstlane(kept) : v;
+    }
+    __device__ __forceinline__ uint32_t valid(int kt) const { return valid(kt, MASK ? mask_bits(kt) : 0u); }
 
     // the next block of the mask as bits, when the first tile of it is loaded
     __device__ __forceinline__ void read_mask(int kt, bool first) {
@@ -219,18 +223,20 @@ struct KeyTiles {
                 if ((threadIdx.x & 63) == 0) bits[w % kMaskBits] = m;
             }
             __syncthreads();
+            ahead = mask_bits(kt);
         }
     }
 
-    // Loads tile kt, the next one; all waves.
-    __device__ __forceinline__ void issue(int kt, int stage, bool first) {
+    // Loads tile kt, the next one; all waves.  Returns its keys that count.
+    __device__ __forceinline__ uint32_t issue(int kt, int stage, bool first) {
         read_mask(kt, first);
         const uint32_t st = base + stage * SB;
         const i32x4 rk = wave_uniform(buffer_rsrc(next_k, (uint32_t)((kTileKeys - 1) * kr + RB)));
         const i32x4 rv = wave_uniform(buffer_rsrc(next_v, (uint32_t)((kTileKeys - 1) * vr + RB)));
         next_k += kTileKeys * kr;
         next_v += kTileKeys * vr;
-        const uint32_t keys = valid(kt);
+        const uint32_t keys = valid(kt, ahead);
+        if constexpr (MASK) ahead = mask_bits(kt + 1);   // (of another block: read again with it)
         if (keys == ~0u) {
 #pragma unroll
             for (int j = 0; j < KI; ++j)
@@ -247,6 +253,7 @@ struct KeyTiles {
                 lds_dma16(rv, __builtin_amdgcn_readfirstlane(st + KB + (wave * KI + j) * 1024), vo[j] | out, 0);
             }
         }
+        return keys;
     }
 
     // Until tile kt is there for all waves; those after it, STAGES - 2 of them at most, may be in

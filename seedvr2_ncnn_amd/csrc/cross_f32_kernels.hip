@@ -36,7 +36,8 @@ __global__ __launch_bounds__(256, WGS) void cross_f32_kernel(CrossArgs a, int ti
     const int all = (nk + KT - 1) / KT;
     const int kb = (int)((long)all * t.part / parts.parts), ke = (int)((long)all * (t.part + 1) / parts.parts);
     KeyTiles<4, DP, STAGES, MASK, Swizzle32> kv(a, t, nk, kb, (uint32_t)(uintptr_t)lds, bits);
-    if (kb < ke) kv.issue(kb, 0, true);
+    uint32_t counts[STAGES] = {};   // keys of the stages' tiles that count
+    if (kb < ke) counts[0] = kv.issue(kb, 0, true);
     if (16 * wave >= t.rows) {   // a wave without rows takes part in loads and barriers alone
         for (int kt = kb; kt < ke; ++kt) {
             kv.await(kt, ke);
@@ -76,8 +77,9 @@ __global__ __launch_bounds__(256, WGS) void cross_f32_kernel(CrossArgs a, int ti
     auto tile = [&](int kt, auto stage) {
         constexpr int ST = decltype(stage)::value * SB;
         kv.await(kt, ke);   // and tile kt - 1 is no longer read
-        if (kt + 1 < ke) kv.issue(kt + 1, 1 - decltype(stage)::value, false);
-        const uint32_t valid = kv.valid(kt);
+        constexpr int NEXT = 1 - decltype(stage)::value;
+        if (kt + 1 < ke) counts[NEXT] = kv.issue(kt + 1, NEXT, false);
+        const uint32_t valid = counts[decltype(stage)::value];
         if (MASK && valid == 0) return;
         f32x4 s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll

@@ -312,8 +312,9 @@ __global__ __launch_bounds__(256, WGS) void cross_tile_kernel(CrossArgs a, int t
     const int kb = (int)((long)all * t.part / parts.parts), ke = (int)((long)all * (t.part + 1) / parts.parts);
 
     KeyTiles<2, DP, STAGES, MASK, Swizzle<DP>> kv(a, t, nk, kb, (uint32_t)(uintptr_t)lds, bits);
-    if (kb < ke) kv.issue(kb, 0, true);
-    if (STAGES > 2 && kb + 1 < ke) kv.issue(kb + 1, 1, false);
+    uint32_t counts[STAGES] = {};   // keys of the stages' tiles that count
+    if (kb < ke) counts[0] = kv.issue(kb, 0, true);
+    if (STAGES > 2 && kb + 1 < ke) counts[1] = kv.issue(kb + 1, 1, false);
 
     if (row_w >= t.rows) {   // a wave without rows takes part in loads and barriers alone
         for (int kt = kb; kt < ke; ++kt) {
@@ -338,8 +339,10 @@ __global__ __launch_bounds__(256, WGS) void cross_tile_kernel(CrossArgs a, int t
         constexpr int ST = decltype(stage)::value;
         kv.await(kt, ke);   // and tile kt - 1 is no longer read
         rows.template keys<ST * SB, MASK>([&] {   // the loads' issue
-            if (kt + STAGES - 1 < ke) kv.issue(kt + STAGES - 1, (ST + STAGES - 1) % STAGES, false);
-            return kv.valid(kt);
+            constexpr int NEXT = (ST + STAGES - 1) % STAGES;
+            const uint32_t now = counts[ST];
+            if (kt + STAGES - 1 < ke) counts[NEXT] = kv.issue(kt + STAGES - 1, NEXT, false);
+            return now;
         });
     };
 #pragma unroll 1
