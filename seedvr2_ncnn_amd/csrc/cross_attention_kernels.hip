@@ -90,9 +90,9 @@ constexpr int kUnits = 256;   // compute units of an MI355X
 
 // Microseconds that a compute unit takes for a tile of keys with 1, 2, .. workgroups on it,
 // `each` at most, for d up to 64, 128 and 256: 4096 x 21600 with 20 heads of 128 in one
-// range of keys is three workgroups on half of the units and two on the others, 899 us; in
-// two ranges five in turn, 837.  1024 x 4096 96 us in one, 62 in three; 300 x 20000, two
-// heads, 429 and 37 in 32.
+// range of keys is three workgroups on half of the units and two on the others, 832 us; in
+// two ranges five in turn, 764.  1024 x 4096 86 us in one, 56 in three; 300 x 20000, two
+// heads, 379 and 32 in 32; in fp32 506 and 357, 1364 and 80.
 struct CrossCost {
     int each;
     double us[4];
