@@ -613,7 +613,7 @@ S2_API int s2_mx_dequantize(const void* codes, long code_stride, const void* sca
 /* y = residual + act(x W^T + bias) of rows x [m][k] and a weight [n][k] in MXFP4, the
  * products those of the values, exact, the sums in fp32; x in MXFP4 too (s2_mx_linear), or
  * in x_dtype with a row stride in elements (s2_mx_weight_linear: fp32, bf16 or fp16, as
- * one to three bf16 terms that hold it exactly).
+ * they are or as two or three bf16 terms that hold them exactly).
  *
  * w_codes: contiguous rows of 16 ceil(k / 32) bytes.  Where k is no multiple of 32 the
  *   codes past it are zeros in x or in the weight, as s2_mx_quantize writes them.
