@@ -93,17 +93,19 @@ __global__ __launch_bounds__(512, 1) void mx_256_kernel(MatmulArgs a, TileSplit 
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int grp = wave >> 2, wq = wave & 3;
     const uint32_t base = (uint32_t)(uintptr_t)lds;
-    // group 0 loads x, group 1 the weight; the first two waves of each 1 KB of scales a step
+    // Group 0 loads x and all scales, its first two waves x's 1 KB a step each, the others the
+    // weight's; group 1 loads the weight.  Group 1 fills a stage while its waves still read it,
+    // which is right for what a wave reads alone, the 64 weight rows that it loads, and for
+    // nothing else; group 0 fills one that no wave reads any more.
     i32x4 rt;
-    const uint32_t* scales;
-    if (grp == 0) {
+    if (grp == 0)
         rt = x_load(a, p).rsrc;
-        scales = x_scales + ((long)p.rt.row0 / 128 + (wq & 1)) * p.nk * 256;
-    } else {
+    else
         rt = w_load(a, p, 256).rsrc;
-        scales = w_scales + ((long)p.col0 / 64 + 2 * (wq & 1)) * p.nk * 128;
-    }
     rt = wave_uniform(rt);
+    const bool of_x = wq < 2;
+    const uint32_t* scales = of_x ? x_scales + ((long)p.rt.row0 / 128 + wq) * p.nk * 256
+                                  : w_scales + ((long)p.col0 / 64 + 2 * (wq & 1)) * p.nk * 128;
     // 64 rows of the weight are 512 bytes a step: lanes 32 .. 63 take the next 64
     const uint32_t half = (uint32_t)p.nk * 512;
     const i32x4 rc = wave_uniform(buffer_rsrc(scales, 2 * half));
@@ -118,14 +120,13 @@ __global__ __launch_bounds__(512, 1) void mx_256_kernel(MatmulArgs a, TileSplit 
     auto issue = [&](int stage, int s) {
         const StepAt at = step_at(a, p, s);
         const int l = this_lane();
-        if (wq < 2)
-            lds_dma16(rc, __builtin_amdgcn_readfirstlane(base + 2 * SB + stage * CB + (grp * 2 + wq) * 1024),
-                      grp == 0 ? l * 16 : (l & 31) * 16 + (l >> 5) * half,
-                      __builtin_amdgcn_readfirstlane((uint32_t)s * (grp == 0 ? 1024 : 512)));
-        if (grp == 0)
+        if (grp == 0) {
+            lds_dma16(rc, __builtin_amdgcn_readfirstlane(base + 2 * SB + stage * CB + wq * 1024),
+                      of_x ? l * 16 : (l & 31) * 16 + (l >> 5) * half,
+                      __builtin_amdgcn_readfirstlane((uint32_t)s * (of_x ? 1024 : 512)));
             tile_issue<false, 8>(tile_lanes<false>(rt, a.x_stride, a.k, l), base + stage * SB, wq * 8, at.x, at.last,
                                  a.x_stride);
-        else
+        } else
             tile_issue<true, 8>(tile_lanes<true>(rt, a.k, a.k, l), base + stage * SB + TB, wq * 8, at.w, at.last, a.k);
     };
     uint4 fx[2][8], fw[2][4];
@@ -156,7 +157,7 @@ __global__ __launch_bounds__(512, 1) void mx_256_kernel(MatmulArgs a, TileSplit 
     issue(0, p.kb);
     if (steps > 1) {
         issue(1, p.kb + 1);
-        asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+        asm volatile("s_waitcnt vmcnt(8)" ::: "memory");   // a step is nine loads, or group 1's eight
     } else {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     }
@@ -198,7 +199,7 @@ __global__ __launch_bounds__(512, 1) void mx_256_kernel(MatmulArgs a, TileSplit 
         for (int i = 0; i < 8; ++i)
             asm volatile("" : "+v"(acc[i][0]), "+v"(acc[i][1]), "+v"(acc[i][2]), "+v"(acc[i][3]));
         __builtin_amdgcn_s_setprio(0);
-        if (grp == 0) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the x rows of step s + 1
+        if (grp == 0) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // x and scales of step s + 1
         // group 1's last phase has no one to meet; group 0's barrier here meets the one
         // after group 1's last read
         if (!(grp == 1 && s + 1 == steps)) block_barrier();

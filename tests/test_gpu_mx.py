@@ -352,3 +352,39 @@ def test_mlp_in_four_bits():
     ro.check(h, *mc.linear(mc.values(code, scale, 320).cuda(), w0.cuda(), None, "gelu", None, torch.bfloat16))
     code, scale = mc.quantize(h)
     ro.check(y, *mc.linear(mc.values(code, scale, 640).cuda(), w1.cuda(), None, "none", x, torch.float32))
+
+
+def _codes(rows, k, gen, low, high, stride=None):
+    """Random codes under scales low .. high - 1 that differ from block to block: (MxRows, values)."""
+    b = mc.blocks(k)
+    code = torch.randint(0, 16, (rows, 32 * b), generator=gen)
+    code[:, k:] = 0
+    scale = torch.randint(low, high, (rows, b), generator=gen)
+    return capi.MxRows(*mc.pack(code, scale, stride=stride), k), mc.values(code, scale, k)
+
+
+def _dealt_bytes(m, n, k):
+    """What the scales of 256 x 256 tiles take: 1 KB for 128 rows of x and 256 k, 512 bytes
+    for 64 rows of the weight."""
+    steps = (mc.blocks(k) + 7) // 8
+    return ((m + 255) // 256 * 2 * 1024 + (n + 255) // 256 * 4 * 512) * steps
+
+
+@pytest.mark.parametrize("y_dtype,act,epilogue", [
+    (torch.float32, "none", False), (torch.bfloat16, "gelu", True), (torch.float16, "silu", True),
+    (torch.float32, "gelu_tanh", True)], ids=str)
+@pytest.mark.parametrize("m,n,k,stride", [
+    (3841, 4000, 1500, None), (4090, 4090, 1700, 55), (2047, 8191, 1600, 50), (3900, 4001, 520, None)])
+def test_largest_tiles(m, n, k, stride, y_dtype, act, epilogue):
+    """256 x 256 tiles that end in rows, columns and k; two steps of 256 k and more, the stages
+    filled again; equal every time."""
+    assert capi.mx_linear_workspace(m, n, k) == (_dealt_bytes(m, n, k) + 255) // 256 * 256
+    gen = torch.Generator().manual_seed(m + k)
+    x, xv = _codes(m, k, gen, 117, 130, stride)
+    weight, w = _codes(n, k, gen, 113, 125, stride)
+    bias = torch.randn(n, generator=gen).cuda() if epilogue else None
+    residual = torch.randn(m, n, generator=gen).to(y_dtype).cuda() if epilogue else None
+    got = capi.mx_linear(x, weight, bias, ro.ACTS[act], residual, out_dtype=y_dtype)
+    ro.check(got, *mc.linear(xv.cuda(), w.cuda(), bias, act, residual, y_dtype))
+    for _ in range(3):
+        assert torch.equal(capi.mx_linear(x, weight, bias, ro.ACTS[act], residual, out_dtype=y_dtype), got)
