@@ -121,7 +121,16 @@ __device__ __forceinline__ void store4_out(const CrossArgs& a, long at, f32x4 v)
 }
 
 constexpr float kLowest = -3.4028234663852886e38f;   // the maximum of no scores
-constexpr float kLazy = 8.f;   // powers of two by which scores may pass m before it follows
+constexpr float kLazy = 8.f;   // powers of two by which weights may pass 1 before m follows
+
+// A weight is 2^((s - m) c), s a score and m a maximum of scores, c = |scale| log2 e (a negative
+// scale turns q's signs).  The difference comes first: s c and m c, rounded or one of them
+// rounded, would differ by more than weights reach where they pass 2^24.  c is within what a
+// difference of nought or -inf can be multiplied by, and 2^-149 leaves the weights of a scale
+// of nought 1 to 2^-21.
+__device__ __forceinline__ float weight_scale(const CrossArgs& a) {
+    return fminf(fmaxf(fabsf(a.scale) * 1.4426950408889634f, 0x1p-149f), 3.4028234663852886e38f);
+}
 
 // Of the wave's four groups of 16 lanes.
 __device__ __forceinline__ float max_groups(float x) {

@@ -30,6 +30,7 @@ __global__ __launch_bounds__(256) void cross_join_few_kernel(CrossArgs a, CrossP
         w[q] = p.weights[at];
         o[q] = *reinterpret_cast<const f32x4*>(p.sums + at * a.d + col);
     }
+    const float c = weight_scale(a);
     float m = w[0].x, l = 0.f;
 #pragma unroll
     for (int q = 1; q < kJoinFew; ++q) m = fmaxf(m, w[q].x);
@@ -37,7 +38,7 @@ __global__ __launch_bounds__(256) void cross_join_few_kernel(CrossArgs a, CrossP
 #pragma unroll
     for (int q = 0; q < kJoinFew; ++q) {
         if (q >= p.parts) break;
-        const float f = __builtin_amdgcn_exp2f(w[q].x - m);
+        const float f = __builtin_amdgcn_exp2f((w[q].x - m) * c);
         l += f * w[q].y;
         sum += f * o[q];
     }
@@ -61,7 +62,7 @@ __global__ __launch_bounds__(256) void cross_join_kernel(CrossArgs a, CrossParts
     float m = w.x;
 #pragma unroll
     for (int x = 32; x; x >>= 1) m = fmaxf(m, __shfl_xor(m, x));
-    const float f = __builtin_amdgcn_exp2f(w.x - m);
+    const float f = __builtin_amdgcn_exp2f((w.x - m) * weight_scale(a));
     float l = f * w.y;
 #pragma unroll
     for (int x = 32; x; x >>= 1) l += __shfl_xor(l, x);

@@ -48,8 +48,7 @@ __global__ __launch_bounds__(256, WGS) void cross_f32_kernel(CrossArgs a, int ti
 
     // q: row l16, elements 16 kk + 4 g on; zeros past d, the last row again past the rows
     const int row = 16 * wave + l16;
-    // (not nought, by which a masked score of -inf would be NaN)
-    const float c = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 0x1p-126f);
+    const float c = weight_scale(a);
     const float sign = a.scale < 0.f ? -1.f : 1.f;
     f32x4 qf[NK];
     {
@@ -100,10 +99,10 @@ __global__ __launch_bounds__(256, WGS) void cross_f32_kernel(CrossArgs a, int ti
         float top = fmaxf(fmaxf(s[0][0], s[0][1]), s[0][2]);
         top = fmaxf(fmaxf(top, s[0][3]), s[1][0]);
         top = fmaxf(fmaxf(top, s[1][1]), s[1][2]);
-        top = fmaxf(top, s[1][3]) * c;
-        if (__any(top > m + kLazy)) {
+        top = fmaxf(top, s[1][3]);
+        if (__any((top - m) * c > kLazy)) {
             const float x = fmaxf(max_groups(top), m);
-            const float fade = __builtin_amdgcn_exp2f(m - x);
+            const float fade = __builtin_amdgcn_exp2f((m - x) * c);
             m = x;
             l *= fade;
 #pragma unroll
@@ -114,7 +113,7 @@ __global__ __launch_bounds__(256, WGS) void cross_f32_kernel(CrossArgs a, int ti
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) s[h][r] = __builtin_amdgcn_exp2f(fmaf(s[h][r], c, -m));
+            for (int r = 0; r < 4; ++r) s[h][r] = __builtin_amdgcn_exp2f((s[h][r] - m) * c);
             l += (s[h][0] + s[h][1]) + (s[h][2] + s[h][3]);
         }
 #pragma unroll

@@ -8,9 +8,9 @@
 // So weights never leave registers and v is not transposed before.  (32x32x16 products
 // leave the matrix cores waiting less, but the chip clocks lower: 3 to 5% slower.)
 //
-// Softmax in powers of two: weights are 2^(c s - m), c = |scale| log2 e (a negative scale turns q's
-// signs), m a maximum that follows the scores' only when a row's passes it by 8: the few
-// rescales cost nothing, and a tile's maxima need not be exchanged between lanes to find
+// Softmax in powers of two: weights are 2^(c (s - m)), c = |scale| log2 e (a negative scale turns
+// q's signs), m a maximum of scores that follows them only when a row's weight passes 2^8: the
+// few rescales cost nothing, and a tile's maxima need not be exchanged between lanes to find
 // that none is due.  Weights are rounded to the operands' type for the second product,
 // at most half a step each, as independent errors of its terms; their sum stays in fp32.
 //
@@ -100,8 +100,7 @@ struct WaveRows {
         l16 = threadIdx.x & 15;
         g = (threadIdx.x & 63) >> 4;
         sign = a.scale < 0.f ? 0x80008000u : 0u;
-        // (not nought, by which a masked score of -inf would be NaN)
-        c = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 0x1p-126f);
+        c = weight_scale(a);
 #pragma unroll
         for (int kk = 0; kk < KA; ++kk) kl[kk] = lds + l16 * RB + (((4 * kk + g) ^ Swizzle<DP>::key(l16)) * 16);
         const int vrow = 4 * g + (l16 >> 2);   // of the lane's eight bytes of v, of 16 rows
@@ -210,14 +209,14 @@ struct WaveRows {
             float x = fmaxf(fmaxf(s[0][i][0], s[0][i][1]), s[0][i][2]);
             x = fmaxf(fmaxf(x, s[0][i][3]), s[1][i][0]);
             x = fmaxf(fmaxf(x, s[1][i][1]), s[1][i][2]);
-            top[i] = fmaxf(x, s[1][i][3]) * c;
-            due |= top[i] > m[i] + kLazy;
+            top[i] = fmaxf(x, s[1][i][3]);
+            due |= (top[i] - m[i]) * c > kLazy;
         }
         if (__any(due)) {
 #pragma unroll
             for (int i = 0; i < NQ; ++i) {
                 const float x = fmaxf(max_groups(top[i]), m[i]);
-                const float fade = __builtin_amdgcn_exp2f(m[i] - x);
+                const float fade = __builtin_amdgcn_exp2f((m[i] - x) * c);
                 m[i] = x;
                 l[i] *= fade;
 #pragma unroll
@@ -227,12 +226,14 @@ struct WaveRows {
         uint4 pb[NQ];
 #pragma unroll
         for (int i = 0; i < NQ; ++i) {
-            const float shift = kShift<T> - m[i];
+            auto weight = [&](float score) {
+                const float x = score - m[i];
+                return __builtin_amdgcn_exp2f(kShift<T> != 0.f ? fmaf(x, c, kShift<T>) : x * c);
+            };
             uint32_t w[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                w[e] = pack2<T>(__builtin_amdgcn_exp2f(fmaf(s[e >> 1][i][2 * (e & 1)], c, shift)),
-                                __builtin_amdgcn_exp2f(fmaf(s[e >> 1][i][2 * (e & 1) + 1], c, shift)));
+                w[e] = pack2<T>(weight(s[e >> 1][i][2 * (e & 1)]), weight(s[e >> 1][i][2 * (e & 1) + 1]));
             pb[i] = make_uint4(w[0], w[1], w[2], w[3]);
 #pragma unroll
             for (int e = 0; e < 4; ++e) l[i] = add_pair<T>(w[e], l[i]);

@@ -390,3 +390,82 @@ def test_text_sublayer():
     oq = capi.mx_quantize(o.view(-1, width))
     y = capi.mx_linear(oq, wo, residual=x, out=x.clone())
     ro.check(y, *mc.linear(capi.mx_dequantize(oq, torch.float32).double(), wov, None, "none", x, torch.float32))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("lq,lk", [(1, 1), (1, 3000), (200, 1), (200, 97), (14000, 77)])
+@pytest.mark.parametrize("d", [64, 128])
+def test_equal_scores_of_any_size(dtype, lq, lk, d):
+    """Scores times log2 e of 2^20 to 2^36, in fp32 up to 2^120, of either sign: as the
+    weights are equal, small numbers in v sum exactly and out is their mean, rounded in the
+    division (U) and to its type."""
+    gen = torch.Generator(device="cuda").manual_seed(13)
+    v = torch.randint(-8, 9, (1, lk, 1, d), generator=gen, device="cuda").to(dtype)
+    mean = v.double().mean(dim=1, keepdim=True)
+    bound = mean.abs() * 2 * ro.U
+    bound = bound + ro.rounding(mean.abs() + bound, dtype)
+    sizes = [(1 + j / 8) * 2.0 ** e for e in range(10, 16) for j in range(8) if dtype != torch.float16 or e < 15]
+    if dtype == torch.float32:
+        sizes += [1.125 * 2.0 ** e for e in (20, 30, 40, 58)]
+    for i, size in enumerate(sizes):
+        q = torch.full((1, lq, 1, d), size, device="cuda").to(dtype)
+        k = torch.full((1, lk, 1, d), size, device="cuda").to(dtype)
+        got = capi.cross_attention(q, -k if i % 3 == 2 else k, v, scale=-0.0884 if i % 3 == 1 else None)
+        ro.check(got, mean.expand(1, lq, 1, d), bound)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("lq,lk", [(1, 3000), (3, 250), (200, 250), (14000, 77)])
+@pytest.mark.parametrize("exponent", [12, 20, 24, 26, 28])
+@pytest.mark.parametrize("order", ["rising", "falling", "mixed"])
+def test_far_scores_that_differ_by_steps(dtype, lq, lk, exponent, order):
+    """Scores 2^exponent + i steps of fp32, i up to 127, whose products and sums are exact.  An
+    exponential's argument, a difference of scores times a factor, is off by 3 U of itself, at
+    most 32 here, the exponential by 4 U; each rescale of the sums by as much again and U.  Of
+    weights, sums and division the rest, as in mx_cross.attention."""
+    d = 64 if lq == 3 else 128
+    big = 2.0 ** (exponent // 2)
+    step = 2.0 ** (exponent - 23)
+    i = torch.arange(lk, device="cuda") * 127 // max(lk - 1, 1)
+    if order == "falling":
+        i = i.flip(0)
+    elif order == "mixed":
+        i = i[torch.randperm(lk, generator=torch.Generator(device="cuda").manual_seed(15), device="cuda")]
+    q = torch.zeros(1, lq, 1, d, device="cuda")
+    k = torch.zeros(1, lk, 1, d, device="cuda")
+    q[..., 3], k[..., 3] = big, 2.0 ** exponent / big
+    q[..., 41], k[..., 41] = 2.0 ** (exponent // 2 - 12), (i * step / 2.0 ** (exponent // 2 - 12))[None, :, None]
+    gen = torch.Generator(device="cuda").manual_seed(14)
+    v = _normal(gen, 1, lk, 1, d).to(dtype)
+    q, k = q.to(dtype), k.to(dtype)
+    assert torch.equal((q[0, 0, 0].double() * k[0, :, 0].double()).sum(1), 2.0 ** exponent + i.double() * step)
+    scale = 0.25 / step
+    got = capi.cross_attention(q, k, v, scale=scale)
+    w = torch.softmax(0.25 * i.double(), dim=0)
+    want = w @ v[0, :, 0].double()
+    tiles = (lk + 31) // 32
+    rel = 2 * (3 * ro.U * 32 + 4 * ro.U + tiles * 5 * ro.U) + (2 * lk + 8) * ro.U
+    if dtype != torch.float32:
+        rel += torch.finfo(dtype).eps / 2
+    bound = rel * (w @ v[0, :, 0].double().abs())
+    if dtype == torch.float16:
+        bound = bound + v[0, :, 0].double().abs().sum(dim=0) * 2.0 ** -25
+    ro.check(got[0, :, 0], want.expand(lq, d), (bound + ro.rounding(want.abs() + bound, dtype)).expand(lq, d))
+
+
+@pytest.mark.parametrize("lq", [1, 200])
+@pytest.mark.parametrize("scale,size", [(0.0, 1e19), (1e-40, 1e19), (1e-38, 1.0), (-1e-45, 1e19), (3e38, 1e-20), (-3e38, 1e-15)])
+def test_smallest_and_largest_scales(lq, scale, size):
+    """Scores of 10^37 under a scale of nought or next to it weigh alike, within 2^-21 of the
+    argument; so do equal ones under the largest."""
+    gen = torch.Generator(device="cuda").manual_seed(16)
+    v = _normal(gen, 1, 300, 2, 64)
+    q = torch.full((1, lq, 2, 64), size / 8, device="cuda")
+    k = q[:, :1].expand(1, 300, 2, 64).clone()
+    if abs(scale) < 1:
+        k *= torch.where(torch.arange(300, device="cuda") % 2 == 0, 1.0, -1.0)[:, None, None]
+    got = capi.cross_attention(q, k, v, scale=scale)
+    want = v.double().mean(dim=1, keepdim=True).expand(1, lq, 2, 64)
+    s = 64 * (size / 8) ** 2 * abs(scale) if abs(scale) < 1 else 0.0
+    bound = (2 * (s + 2.0 ** -20) + 700 * ro.U) * v.double().abs().mean(dim=1, keepdim=True).expand_as(want)
+    ro.check(got, want, bound)
