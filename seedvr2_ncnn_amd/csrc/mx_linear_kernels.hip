@@ -458,16 +458,17 @@ MxPlan mx_plan(const MxLinearArgs& a, bool pack_x, bool pack_w, size_t workspace
     const DealtBytes dealt = mx_dealt_bytes(a.m, a.n, blocks);
     const size_t copied = ((pack_x ? (size_t)a.m : 0) + (pack_w ? (size_t)a.n : 0)) * round_up(blocks, 16);
     MxPlan p{};
+    // what a tile's own scales leave is for the sums, so that the bytes of a plan give it again
     for (int largest : {256, 128}) {
-        const size_t least = round_up(largest == 256 ? dealt.x + dealt.w : copied, 256);
-        if (least > workspace_bytes) continue;
-        p.tile = choose_tiles(m, (m.k + 63) / 64, ranges(a, workspace_bytes - least), largest);
-        p.scales = round_up(p.tile.bm == 256 ? dealt.x + dealt.w : copied, 256);
-        p.sums = p.tile.parts > 1 ? (size_t)p.tile.parts * a.m * round_up(a.n, 4) * sizeof(float) : 0;
-        if (p.bytes() <= workspace_bytes) return p;
+        const size_t scales = round_up(largest == 256 ? dealt.x + dealt.w : copied, 256);
+        if (scales > workspace_bytes) continue;
+        const TileChoice t = choose_tiles(m, (m.k + 63) / 64, ranges(a, workspace_bytes - scales), largest);
+        if ((largest == 256 && t.bm < 256) || (p.tile.bm && p.tile.us <= t.us)) continue;
+        p.tile = t;
+        p.scales = scales;
+        p.sums = t.parts > 1 ? (size_t)t.parts * a.m * round_up(a.n, 4) * sizeof(float) : 0;
     }
-    p.tile.bm = 0;   // not on tiles
-    return p;
+    return p;   // no tile: not on tiles
 }
 
 }  // namespace

@@ -388,3 +388,24 @@ def test_largest_tiles(m, n, k, stride, y_dtype, act, epilogue):
     ro.check(got, *mc.linear(xv.cuda(), w.cuda(), bias, act, residual, y_dtype))
     for _ in range(3):
         assert torch.equal(capi.mx_linear(x, weight, bias, ro.ACTS[act], residual, out_dtype=y_dtype), got)
+
+
+@pytest.mark.parametrize("stride", [None, 1000], ids=str)
+@pytest.mark.parametrize("x_kind", KINDS, ids=str)
+@pytest.mark.parametrize("m,n,k", [
+    (17, 320, 20000), (64, 64, 10240), (200, 2560, 10240), (77, 2560, 5120), (40, 200, 2560), (300, 5120, 2560),
+    (1000, 1000, 9000), (2000, 2000, 8192), (4096, 4096, 2560)])
+def test_queried_workspace_is_what_a_larger_one_gives(m, n, k, x_kind, stride):
+    """The same tiles and ranges of k, and so the same sums to the bit."""
+    gen = torch.Generator().manual_seed(n)
+    weight, _ = _codes(n, k, gen, 113, 125, stride)
+    if x_kind is None:
+        x, _ = _codes(m, k, gen, 117, 130, stride)
+        kind = None
+    else:
+        x = torch.randn(m, k, generator=gen).to(x_kind).cuda()
+        kind = {torch.float32: capi.DTYPE_F32, torch.bfloat16: capi.DTYPE_BF16, torch.float16: capi.DTYPE_F16}[x_kind]
+    size = capi.mx_linear_workspace(m, n, k, kind, capi.DTYPE_F32)
+    queried, more = (torch.empty(s, dtype=torch.uint8, device="cuda") for s in (size, size + (1 << 30)))
+    a = capi.mx_linear(x, weight, out_dtype=torch.float32, workspace=queried)
+    assert torch.equal(a, capi.mx_linear(x, weight, out_dtype=torch.float32, workspace=more))
