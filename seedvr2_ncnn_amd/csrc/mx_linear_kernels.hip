@@ -214,6 +214,9 @@ hipError_t run_rows(const MxLinearArgs& a, hipStream_t stream) {
 
 constexpr int kUnits = 256;   // compute units of an MI355X
 
+// Workgroups of 512 threads of a launch, whose threads 32 bits count.
+constexpr long kWorkgroupsMost = (1L << 23) - 1;
+
 // Tiles of 16 columns of a workgroup: the more there are, the fewer times x is read from the
 // L2; as long as three quarters of the compute units have a workgroup (1 x 2560 in bf16 by
 // 15360 x 2560 8.8 us with one, 7.3 with four; 1 x 5120 by 2560 x 5120 5.9 and 13).
@@ -241,20 +244,33 @@ template <int XT>
 hipError_t launch_rows(const MxLinearArgs& a, hipStream_t stream) {
     const int t = rows_tiles(a);
     const long row_blocks = ((long)a.m + 15) / 16, columns = (a.n + 16L * t - 1) / (16 * t);
-    if (row_blocks * columns * 512 >= 1L << 32) {   // threads of a launch
-        if (row_blocks < 2) return hipErrorInvalidValue;
+    if (row_blocks * columns > kWorkgroupsMost) {   // halves of the rows, or of the columns
         MxLinearArgs first = a, second = a;
-        const long m = row_blocks / 2 * 16, ye = a.y_kind ? 2 : 4;
-        first.m = (int)m;
-        second.m -= (int)m;
-        if (XT == 0) {
-            second.xq.codes += m * a.xq.code_stride;
-            second.xq.scales += m * a.xq.scale_stride;
+        const long ye = a.y_kind ? 2 : 4;
+        long at, res_at;   // of the second half in y and the residual
+        if (row_blocks > 1) {
+            const long m = row_blocks / 2 * 16;
+            first.m = (int)m;
+            second.m -= (int)m;
+            if (XT == 0) {
+                second.xq.codes += m * a.xq.code_stride;
+                second.xq.scales += m * a.xq.scale_stride;
+            } else {
+                second.x = (const char*)a.x + m * a.x_stride * (XT == 1 ? 4 : 2);
+            }
+            at = m * a.y_stride;
+            res_at = m * a.res_stride;
         } else {
-            second.x = (const char*)a.x + m * a.x_stride * (XT == 1 ? 4 : 2);
+            const long n = columns / 2 * 16 * t;
+            first.n = (int)n;
+            second.n -= (int)n;
+            second.w.codes += n * a.w.code_stride;
+            second.w.scales += n * a.w.scale_stride;
+            if (a.bias) second.bias += n;
+            at = res_at = n;
         }
-        if (a.res) second.res = (const char*)a.res + m * a.res_stride * ye;
-        second.y = (char*)a.y + m * a.y_stride * ye;
+        if (a.res) second.res = (const char*)a.res + res_at * ye;
+        second.y = (char*)a.y + at * ye;
         const hipError_t e = launch_rows<XT>(first, stream);
         return e != hipSuccess ? e : launch_rows<XT>(second, stream);
     }
@@ -319,7 +335,7 @@ MatmulArgs codes_args(const MxLinearArgs& a) {
 // 2560 5.5 and 7.3.
 constexpr int kRowsMost = 16;
 
-// Rows of other types on tiles: x as planes of bf16 terms (or as it is, in bf16 with 16-byte
+// Rows of other types on tiles (none: bm of nought): x as planes of bf16 terms (or as it is, in bf16 with 16-byte
 // rows), the weight's codes as they are, or its values in bf16 for the tile kernels of
 // 16-bit operands, where the largest tiles pay for that.
 struct ValuesPlan {
@@ -331,6 +347,12 @@ struct ValuesPlan {
     // launches, bytes a microsecond read and written
     double us() const { return tile.us + 2. + (codes && pack_x ? 3. : 0.) + (2.3 * x_bytes + 1.3 * w_bytes) / 5.5e6; }
 };
+
+// Threads that 32 bits count: 512 a workgroup of 256 x 256 tiles, else 256.
+bool one_launch(const MxLinearArgs& a, const TileChoice& t) {
+    const long blocks = ((long)a.m + t.bm - 1) / t.bm * ((a.n + t.bn - 1) / t.bn) * t.parts;
+    return blocks * (t.bm == 256 ? 512 : 256) < 1L << 32;
+}
 
 // What tiles of the weight's codes take, in microseconds: a workgroup's first loads and
 // epilogue, and 256 k, for which its compute unit gets 50 or 41 KB through the caches; by
@@ -347,6 +369,7 @@ TileChoice weight_tiles(const MxLinearArgs& a, bool f16, long steps, long most) 
     for (const WeightCost& t : kWeightCosts) {
         const long count = ((long)a.m + t.bm - 1) / t.bm * ((a.n + t.bn - 1) / t.bn);
         for (long parts = 1; parts <= std::max<long>(1, std::min(most, steps / 2)); ++parts) {
+            if (count * parts > kWorkgroupsMost) break;
             const double rounds = (double)((count * parts + kUnits - 1) / kUnits);
             const double us = rounds * (t.round + (f16 ? t.step_f16 : t.step) * (double)((steps + parts - 1) / parts)) +
                               (parts > 1 ? 3. + 2. * parts * each / 9e6 : 0.);
@@ -373,6 +396,7 @@ ValuesPlan values_plan(const MxLinearArgs& a, bool codes, size_t workspace_bytes
     const long most = std::min<long>(16, (long)((workspace_bytes - p.bytes()) / each));
     p.tile = codes ? weight_tiles(a, a.x_kind == S2_DTYPE_F16 && p.planes == 1, (k8 + 255) / 256 * p.planes, most)
                    : choose_tiles(m, (k8 + 63) / 64 * p.planes, most);
+    if (!codes && !one_launch(a, p.tile)) p.tile.bm = 0;
     p.sum_bytes = p.tile.parts > 1 ? p.tile.parts * each : 0;
     return p;
 }
@@ -463,7 +487,7 @@ MxPlan mx_plan(const MxLinearArgs& a, bool pack_x, bool pack_w, size_t workspace
         const size_t scales = round_up(largest == 256 ? dealt.x + dealt.w : copied, 256);
         if (scales > workspace_bytes) continue;
         const TileChoice t = choose_tiles(m, (m.k + 63) / 64, ranges(a, workspace_bytes - scales), largest);
-        if ((largest == 256 && t.bm < 256) || (p.tile.bm && p.tile.us <= t.us)) continue;
+        if ((largest == 256 && t.bm < 256) || (p.tile.bm && p.tile.us <= t.us) || !one_launch(a, t)) continue;
         p.tile = t;
         p.scales = scales;
         p.sums = t.parts > 1 ? (size_t)t.parts * a.m * round_up(a.n, 4) * sizeof(float) : 0;
@@ -482,7 +506,7 @@ size_t mx_linear_workspace(const MxLinearArgs& a) {
         for (bool codes : {false, true})
             for (const MxLinearArgs& b : {near, far}) {
                 const ValuesPlan p = values_plan(b, codes, (size_t)1 << 62);
-                if (p.us() < rows_us(a)) most = std::max(most, p.bytes());
+                if (p.tile.bm && p.us() < rows_us(a)) most = std::max(most, p.bytes());
             }
         return most;
     }

@@ -326,7 +326,6 @@ hipError_t launch(const MatmulArgs& a, const MxTileScales& sc, const TileChoice&
                   void* workspace, hipStream_t stream) {
     const long mtiles = row_tiles(a, t.bm), ntiles = (a.n + t.bn - 1) / t.bn;
     const long blocks = mtiles * ntiles * t.parts;
-    if (blocks > 0x7fffffffL) return hipErrorInvalidValue;
     const TileSplit sp{(int)ntiles, (int)mtiles, t.parts, whole_pieces(a), (a.n + 3) / 4 * 4, sums};
     const unsigned nb = (unsigned)blocks;
     if (t.bm == 256) {

@@ -147,7 +147,6 @@ template <int T, int YK>
 hipError_t launch(const MatmulArgs& a, const MxTileScales& sc, const TileChoice& t, float* sums, hipStream_t stream) {
     const long mtiles = row_tiles(a, t.bm), ntiles = (a.n + t.bn - 1) / t.bn;
     const long blocks = mtiles * ntiles * t.parts;
-    if (blocks > 0x7fffffL) return hipErrorInvalidValue;   // (512 threads each)
     const TileSplit sp{(int)ntiles, (int)mtiles, t.parts, whole_pieces(a), (a.n + 3) / 4 * 4, sums};
     const unsigned nb = (unsigned)blocks;
     if (t.bn == 128)

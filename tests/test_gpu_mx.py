@@ -409,3 +409,37 @@ def test_queried_workspace_is_what_a_larger_one_gives(m, n, k, x_kind, stride):
     queried, more = (torch.empty(s, dtype=torch.uint8, device="cuda") for s in (size, size + (1 << 30)))
     a = capi.mx_linear(x, weight, out_dtype=torch.float32, workspace=queried)
     assert torch.equal(a, capi.mx_linear(x, weight, out_dtype=torch.float32, workspace=more))
+
+
+@pytest.mark.parametrize("m", [1, 3])
+@pytest.mark.parametrize("x_kind", [None, torch.bfloat16], ids=str)
+def test_more_columns_than_a_launch_has(x_kind, m):
+    some, n = 37, (1 << 29) + 100
+    times = (n + some - 1) // some
+    gen = torch.Generator().manual_seed(18)
+    few, _ = _codes(some, 32, gen, 113, 125)
+    weight = capi.MxRows(few.codes.repeat(times, 1)[:n], few.scales.repeat(times, 1)[:n], 32)
+    x = torch.randn(m, 32, generator=gen).bfloat16().cuda()
+    if x_kind is None:
+        x = capi.mx_quantize(x)
+    bias = torch.randn(some, generator=gen).cuda()
+    residual = torch.randn(m, some, generator=gen).bfloat16().cuda()
+    first = capi.mx_linear(x, few, bias, capi.ACT_SILU, residual)
+    out = residual.repeat(1, times)[:, :n]
+    capi.mx_linear(x, weight, bias.repeat(times)[:n], capi.ACT_SILU, out, out=out)
+    whole = n // some * some
+    assert (out[:, :whole].view(m, -1, some) == first[:, None]).all()
+    assert torch.equal(out[:, whole:], first[:, :n - whole])
+
+
+def test_more_tiles_of_codes_than_a_launch_has():
+    """Many rows on the weight's codes, which take no workspace."""
+    some, m, n, k = 37, (1 << 29) + 100, 17, 8
+    gen = torch.Generator().manual_seed(19)
+    weight, _ = _codes(n, k, gen, 113, 125, 16)
+    x = torch.randn(some, k, generator=gen).bfloat16().cuda()
+    none = torch.empty(0, dtype=torch.uint8, device="cuda")
+    first = capi.mx_linear(x, weight, workspace=none)
+    got = capi.mx_linear(x.repeat((m + some - 1) // some, 1)[:m], weight, workspace=none)
+    whole = m // some * some
+    assert (got[:whole].view(-1, some, n) == first).all() and torch.equal(got[whole:], first[:m - whole])
