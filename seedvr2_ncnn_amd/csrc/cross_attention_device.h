@@ -34,65 +34,71 @@ struct CrossTile {
 
 // The workgroup's tile, or rows 0.  Ordered by part, tile, head: workgroups of one head's
 // tiles follow each other on an XCD, whose L2 then holds the head's keys.  tiles: at most
-// there are.  Samples of any lengths are dealt out over the tiles that they make, found by a
-// scan of 64 offsets at a time, which are read once where there are no more.
+// there are.
+//
+// Up to kScanSamples samples of any lengths, an offset a lane, are dealt out over the tiles that
+// they make.  Of more each has places of its own: a sample's begin at that of its first row
+// were all rows one sample's, plus its number, which leaves room for last tiles that are not
+// full.  A workgroup searches for its place's sample, a 64th of those left at a time (32768
+// samples of a row, eight heads of 128, 1.7 ms; 111 with a scan of all by each).
 __device__ __forceinline__ CrossTile cross_tile(const CrossArgs& a, int each, int tiles, int parts) {
     const int group = a.heads / a.kv_heads;
     const int lane = threadIdx.x & 63;
     CrossTile t;
     t.rows = 0;
     int count = tiles;
-    CrossSample s;   // the lane's
-    auto read_lane = [&](int b0) {
-        s = CrossSample{0, 0, b0 + lane, 0, 0};
-        if (b0 + lane < a.batch) s = ragged_sample(a, b0 + lane);
-    };
-    auto made = [&] { return (int)(((long)s.nq * group + each - 1) / each); };
-    if (a.q_offsets) {
-        count = 0;
-        for (int b0 = 0; b0 < a.batch; b0 += 64) {
-            read_lane(b0);
-            int n = made();
-#pragma unroll
-            for (int o = 32; o; o >>= 1) n += __shfl_xor(n, o);
-            count = min(count + n, tiles);   // (descending offsets can make more)
-        }
-        count = __builtin_amdgcn_readfirstlane(count);
-    }
-    const long blocks = (long)count * a.kv_heads * parts;
-    if (blockIdx.x >= blocks) return t;
-    const int lid = xcd_remap(blockIdx.x, (int)blocks);
-    t.part = lid % parts;
-    int i = lid / parts % count;
-    t.head = lid / parts / count;
-    if (!a.q_offsets) {
-        const int of_sample = (int)(((long)a.lq * group + each - 1) / each);
-        const int b = i / of_sample;
-        t.s = CrossSample{0, 0, b, a.lq, a.key_lengths ? clamped(a.key_lengths[b], a.lk) : a.lk};
-        t.row0 = i % of_sample * each;
-        t.rows = (int)min((long)each, (long)a.lq * group - t.row0);
-        return t;
-    }
-    for (int b0 = 0; b0 < a.batch; b0 += 64) {
-        if (a.batch > 64) read_lane(b0);
-        int upto = made();
+    CrossSample s = {0, 0, 0, 0, 0};   // the lane's
+    int upto = 0;                      // tiles of the samples up to it
+    const bool scan = a.q_offsets && a.batch <= kScanSamples;
+    if (scan) {
+        if (lane < a.batch) s = ragged_sample(a, lane);
+        upto = (int)(((long)s.nq * group + each - 1) / each);
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
             const int other = __shfl_up(upto, o);
             if (lane >= o) upto += other;
         }
-        const uint64_t past = __ballot(upto > i);
-        if (past) {
-            const int l = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)past) - 1);
-            auto of_lane = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
-            const int before = l ? __builtin_amdgcn_readlane(upto, max(l - 1, 0)) : 0;
-            t.s = CrossSample{of_lane((int)s.q0), of_lane((int)s.k0), b0 + l, of_lane(s.nq), of_lane(s.nk)};
-            t.row0 = (i - before) * each;
-            t.rows = (int)min((long)each, (long)t.s.nq * group - t.row0);
-            return t;
-        }
-        i -= __builtin_amdgcn_readlane(upto, 63);
+        count = min(__builtin_amdgcn_readlane(upto, 63), tiles);   // (descending offsets can make more)
     }
+    const long blocks = (long)count * a.kv_heads * parts;
+    if (blockIdx.x >= blocks) return t;
+    const int lid = xcd_remap(blockIdx.x, (int)blocks);
+    t.part = lid % parts;
+    const int i = lid / parts % count;
+    t.head = lid / parts / count;
+    int before = 0;   // the sample's first tile
+    if (!a.q_offsets) {
+        const int of_sample = (int)(((long)a.lq * group + each - 1) / each);
+        const int b = i / of_sample;
+        t.s = CrossSample{0, 0, b, a.lq, a.key_lengths ? clamped(a.key_lengths[b], a.lk) : a.lk};
+        before = b * of_sample;
+    } else if (scan) {
+        const uint64_t past = __ballot(upto > i);
+        if (!past) return t;
+        const int l = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)past) - 1);
+        auto of_lane = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
+        before = l ? __builtin_amdgcn_readlane(upto, max(l - 1, 0)) : 0;
+        t.s = CrossSample{of_lane((int)s.q0), of_lane((int)s.k0), l, of_lane(s.nq), of_lane(s.nk)};
+    } else {
+        auto place = [&](int b) { return (int)((unsigned)(clamped(a.q_offsets[b], a.lq) * group) / (unsigned)each) + b; };
+        int b = 0;   // the first of n samples, one of which has place i
+        for (int n = a.batch; n > 1;) {
+            const int step = (n + 63) / 64;
+            const int l = __popcll(__ballot(lane * step < n && place(b + min(lane * step, n - 1)) <= i)) - 1;
+            if (l < 0) return t;   // rows ahead of the first sample
+            b += l * step;
+            n = min(step, n - l * step);
+        }
+        b = __builtin_amdgcn_readfirstlane(b);
+        const CrossSample found = ragged_sample(a, b);
+        auto uniform = [](long v) { return __builtin_amdgcn_readfirstlane((int)v); };
+        before = uniform(place(b));
+        t.s = CrossSample{uniform(found.q0), uniform(found.k0), b, uniform(found.nq), uniform(found.nk)};
+    }
+    const long row0 = ((long)i - before) * each;
+    if (row0 < 0) return t;   // (of descending offsets)
+    t.row0 = (int)row0;
+    t.rows = (int)max(min((long)each, (long)t.s.nq * group - row0), 0L);   // (none of a place without a tile)
     return t;
 }
 

@@ -38,6 +38,8 @@ struct CrossArgs {
 
 constexpr int kTileRows = 128, kTileRows32 = 64;   // of 16-bit operands' tiles, of fp32 ones'
 constexpr int kTileKeys = 32;
+// samples whose offsets a wave holds
+constexpr int kScanSamples = 64;
 // keys of a head that LDS holds in the kernel for many rows on few of them, and its workgroups
 // on a compute unit
 constexpr int kShortKeys = 128, kShortEach = 2;

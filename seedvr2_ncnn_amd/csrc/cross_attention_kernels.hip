@@ -108,9 +108,8 @@ CrossPlan cross_plan(const CrossArgs& a, size_t workspace_bytes) {
     const long rows = (long)a.lq * group;
     const int each = a.kind ? kTileRows : kTileRows32;
     auto tiles_of = [&](long each) {
-        return std::min<long>(a.q_offsets ? rows / each + std::min(a.batch, a.lq)
-                                          : a.batch * ((rows + each - 1) / each),
-                              0x7fffffffL);
+        const long last = a.batch <= kScanSamples ? std::min(a.batch, a.lq) : a.batch;   // tiles that are not full
+        return std::min<long>(a.q_offsets ? rows / each + last : a.batch * ((rows + each - 1) / each), 0x7fffffffL);
     };
     CrossPlan p;
     p.run = 1;

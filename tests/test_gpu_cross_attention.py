@@ -469,3 +469,76 @@ def test_smallest_and_largest_scales(lq, scale, size):
     s = 64 * (size / 8) ** 2 * abs(scale) if abs(scale) < 1 else 0.0
     bound = (2 * (s + 2.0 ** -20) + 700 * ro.U) * v.double().abs().mean(dim=1, keepdim=True).expand_as(want)
     ro.check(got, want, bound)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("batch", [63, 64, 65, 66, 1000, 4097])
+def test_many_ragged_samples(dtype, batch):
+    """Samples of no, one and several tiles, without keys and with, rows ahead of the first one
+    and behind the last: each as a call of its own gives it, but for the order of a row's sums."""
+    gen = torch.Generator().manual_seed(batch)
+    nq = torch.randint(0, 4, (batch,), generator=gen) * torch.randint(0, 90, (batch,), generator=gen)
+    nk = torch.randint(0, 3, (batch,), generator=gen) * torch.randint(0, 40, (batch,), generator=gen)
+    nq[batch // 3:batch // 2] = 0
+    nq[-1] = 300
+    qo, ko = (torch.cat([torch.zeros(1, dtype=torch.long), n.cumsum(0)]) + 7 for n in (nq, nk))
+    q = torch.randn(int(qo[-1]) + 5, 4, 64, generator=gen).to(dtype).cuda()
+    k, v = (torch.randn(int(ko[-1]) + 5, 2, 64, generator=gen).to(dtype).cuda() for _ in range(2))
+    out = torch.full_like(q, 5.0)
+    capi.cross_attention(q, k, v, q_offsets=qo.int().cuda(), k_offsets=ko.int().cuda(), out=out)
+    assert (out[:7] == 5).all() and (out[int(qo[-1]):] == 5).all()
+    longest = int(nk.max())
+    sample = torch.repeat_interleave(torch.arange(batch), nq)   # of each row
+    index = (ko[:-1, None] + torch.arange(longest)).clamp(max=int(ko[-1]))[sample].cuda()
+    kept = (torch.arange(longest) < nk[:, None])[sample].cuda()
+    rows = out[7:int(qo[-1])]
+    for at in range(0, rows.shape[0], 20000):   # in 64 bits, all heads of a row at once
+        qs = q[7 + at:7 + at + 20000][:len(rows) - at].double()[:, :, None]
+        ks, vs = (t[index[at:at + 20000]].double().transpose(1, 2).repeat_interleave(2, 1) for t in (k, v))
+        s = (qs * ks).sum(-1) * 0.125
+        size = (qs.abs() * ks.abs()).sum(-1) * 0.125
+        s = s.masked_fill(~kept[at:at + 20000, None], -float("inf"))
+        some = kept[at:at + 20000].any(1)[:, None, None]
+        w = torch.where(some, torch.softmax(s, -1), torch.zeros((), dtype=torch.float64, device="cuda"))
+        want = (w[..., None] * vs).sum(2)
+        # as in mx_cross.attention
+        arg = 68 * ro.U * size.amax(-1) + 2 * ro.U * 1.45 * torch.where(w > 0, s, 0.0).abs().amax(-1)
+        rel = 2 * (2 * arg + 4 * ro.U) + (2 * longest + 8) * ro.U
+        rel = rel + (torch.finfo(dtype).eps / 2 if dtype != torch.float32 else 0.0)
+        bound = (w[..., None] * vs.abs()).sum(2) * rel[..., None]
+        if dtype == torch.float16:
+            bound = bound + (kept[at:at + 20000, None, :, None] * vs.abs()).sum(2) * 2.0 ** -25
+        ro.check(rows[at:at + 20000], want, bound + ro.rounding(want.abs() + bound, dtype))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("heads", [1, 6])
+def test_a_million_ragged_samples(dtype, heads):
+    """A key a sample: out is its v, to the bit; none: nought."""
+    batch = (1 << 20) + 3
+    number = torch.arange(batch, device="cuda")
+    nq, nk = (number % 3).int(), (number % 5 != 0).int()
+    zero = torch.zeros(1, dtype=torch.int32, device="cuda")
+    qo, ko = (torch.cat([zero, n.cumsum(0).int()]) for n in (nq, nk))
+    rows, keys = int(qo[-1]), int(ko[-1])
+    q = torch.ones(rows, heads, 8, dtype=dtype, device="cuda")
+    v = (number[:keys, None, None] * 7 + torch.arange(8 * heads, device="cuda").view(heads, 8)).remainder(251).to(dtype)
+    sample = torch.repeat_interleave(number, nq)
+    want = v[ko[sample].long().clamp(max=keys - 1)]
+    want[nk[sample] == 0] = 0
+    assert torch.equal(capi.cross_attention(q, v, v, q_offsets=qo, k_offsets=ko), want)
+
+
+def test_offsets_in_disorder_stay_within_the_rows():
+    """What descending offsets give is nobody's business, but rows that no sample can have keep
+    their values, and the calls end."""
+    gen = torch.Generator().manual_seed(21)
+    for batch in (5, 64, 65, 700):
+        qo = torch.randint(-50, 900, (batch + 1,), generator=gen, dtype=torch.int32).cuda()
+        ko = torch.randint(-50, 900, (batch + 1,), generator=gen, dtype=torch.int32).cuda()
+        q = torch.randn(1000, 2, 64, device="cuda")
+        for t in (torch.float32, torch.bfloat16):
+            out = torch.full((1000, 2, 64), 5.0, device="cuda", dtype=t)
+            capi.cross_attention(q.to(t)[:800], q.to(t)[:800], q.to(t)[:800], q_offsets=qo, k_offsets=ko, out=out[:800])
+            torch.cuda.synchronize()
+            assert (out[800:] == 5).all()
