@@ -60,9 +60,9 @@ __device__ __forceinline__ CrossTile cross_tile(const CrossArgs& a, int each, in
         }
         count = min(__builtin_amdgcn_readlane(upto, 63), tiles);   // (descending offsets can make more)
     }
-    const long blocks = (long)count * a.kv_heads * parts;
+    const long blocks = (long)count * a.kv_heads * parts - a.first;
     if (blockIdx.x >= blocks) return t;
-    const int lid = xcd_remap(blockIdx.x, (int)blocks);
+    const int lid = a.first + xcd_remap(blockIdx.x, (int)min(blocks, kLaunchBlocks));
     t.part = lid % parts;
     const int i = lid / parts % count;
     t.head = lid / parts / count;

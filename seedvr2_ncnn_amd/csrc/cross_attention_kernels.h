@@ -10,6 +10,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include <algorithm>
+
 namespace s2 {
 
 // Rows [.. heads][d] of an operand: sample b's row i of head h begins at b * batch + i *
@@ -34,10 +36,12 @@ struct CrossArgs {
     long mask_batch;
     int heads, kv_heads, d;
     float scale;
+    int first;                // workgroups of the launches before
 };
 
 constexpr int kTileRows = 128, kTileRows32 = 64;   // of 16-bit operands' tiles, of fp32 ones'
 constexpr int kTileKeys = 32;
+constexpr long kLaunchBlocks = 1 << 23;   // workgroups of a launch
 // samples whose offsets a wave holds
 constexpr int kScanSamples = 64;
 // keys of a head that LDS holds in the kernel for many rows on few of them, and its workgroups
@@ -58,6 +62,19 @@ struct CrossParts {
     float* sums;
     float2* weights;
 };
+
+// `blocks` workgroups of 256 threads, by launches whose threads 32 bits count.
+template <typename F>
+hipError_t launch_in_turn(const CrossArgs& args, long blocks, F&& launch) {
+    CrossArgs a = args;
+    for (long at = 0; at < blocks; at += kLaunchBlocks) {
+        a.first = (int)at;
+        launch(a, (unsigned)std::min(kLaunchBlocks, blocks - at));
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
+}
 
 CrossParts cross_parts(const CrossArgs& a, const CrossPlan& plan, void* workspace);
 hipError_t launch_cross_tiles(const CrossArgs& a, const CrossPlan& plan, void* workspace, hipStream_t stream);

@@ -136,8 +136,11 @@ CrossPlan cross_plan(const CrossArgs& a, size_t workspace_bytes) {
         p.run = 1;
     }
     const double tiles = (double)((keys + kTileKeys - 1) / kTileKeys);
-    const bool joined = (double)all_rows(a) * a.heads * a.d < 0x1p33;   // threads of a join's launch: 32 bits
-    const long most = joined ? std::min<long>(64, (long)(workspace_bytes / part_bytes(a))) : 1;
+    // 32 bits count the workgroups, and the threads of a join's launch, 64 a row at most
+    const bool joined = (double)all_rows(a) * a.heads * 64. < 0x1p32;
+    const long most = joined ? std::min(std::min(64L, (long)(workspace_bytes / part_bytes(a))),
+                                        0x7fffffffL / ((long)p.tiles * a.kv_heads))
+                             : 1;
     const CrossCost& c = kCrossCosts[a.kind == 0][a.d <= 64 ? 0 : a.d <= 128 ? 1 : 2];
     double best = 0.;
     p.parts = 1;
@@ -171,33 +174,20 @@ hipError_t launch_cross_attention(const CrossArgs& a, void* workspace, size_t wo
     const long rows = all_rows(a);
     if (rows <= 0) return hipSuccess;
     const CrossPlan p = cross_plan(a, workspace_bytes);
-    if ((double)p.tiles * a.kv_heads * p.parts * 256. >= 0x1p32) {   // threads of a launch
+    if ((long)p.tiles * a.kv_heads * p.parts >= 0x7fffffffL) {   // workgroups that 32 bits do not count: halves of the heads
+        if (a.kv_heads == 1) return hipErrorInvalidValue;   // no memory holds so many rows of out
         const size_t e = a.kind ? 2 : 4, oe = a.out_kind ? 2 : 4;
         CrossArgs first = a, second = a;
         auto past = [](const void* at, long n, size_t each) { return (const void*)((const char*)at + n * (long)each); };
-        if (a.kv_heads > 1) {
-            const int h = a.kv_heads / 2, qh = h * (a.heads / a.kv_heads);
-            first.kv_heads = h;
-            first.heads = qh;
-            second.kv_heads -= h;
-            second.heads -= qh;
-            second.q = past(a.q, qh * a.qs.head, e);
-            second.k = past(a.k, h * a.ks.head, e);
-            second.v = past(a.v, h * a.vs.head, e);
-            second.out = (void*)past(a.out, qh * a.os.head, oe);
-        } else if (!a.q_offsets && a.batch > 1) {
-            const int b = a.batch / 2;
-            first.batch = b;
-            second.batch -= b;
-            second.q = past(a.q, b * a.qs.batch, e);
-            second.k = past(a.k, b * a.ks.batch, e);
-            second.v = past(a.v, b * a.vs.batch, e);
-            second.out = (void*)past(a.out, b * a.os.batch, oe);
-            if (a.key_lengths) second.key_lengths += b;
-            if (a.key_mask) second.key_mask += b * a.mask_batch;
-        } else {
-            return hipErrorInvalidValue;
-        }
+        const int h = a.kv_heads / 2, qh = h * (a.heads / a.kv_heads);
+        first.kv_heads = h;
+        first.heads = qh;
+        second.kv_heads -= h;
+        second.heads -= qh;
+        second.q = past(a.q, qh * a.qs.head, e);
+        second.k = past(a.k, h * a.ks.head, e);
+        second.v = past(a.v, h * a.vs.head, e);
+        second.out = (void*)past(a.out, qh * a.os.head, oe);
         const hipError_t e1 = launch_cross_attention(first, workspace, workspace_bytes, stream);
         return e1 != hipSuccess ? e1 : launch_cross_attention(second, workspace, workspace_bytes, stream);
     }

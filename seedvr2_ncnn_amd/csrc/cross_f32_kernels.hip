@@ -155,12 +155,12 @@ __global__ __launch_bounds__(256, WGS) void cross_f32_kernel(CrossArgs a, int ti
 
 template <int DP, int WGS>
 hipError_t launch(const CrossArgs& a, const CrossPlan& p, const CrossParts& parts, hipStream_t stream) {
-    const unsigned nb = (unsigned)((long)p.tiles * a.kv_heads * p.parts);
-    if (a.key_mask)
-        cross_f32_kernel<DP, WGS, true><<<nb, 256, 0, stream>>>(a, p.tiles, parts);
-    else
-        cross_f32_kernel<DP, WGS, false><<<nb, 256, 0, stream>>>(a, p.tiles, parts);
-    return hipGetLastError();
+    return launch_in_turn(a, (long)p.tiles * a.kv_heads * p.parts, [&](const CrossArgs& part, unsigned nb) {
+        if (part.key_mask)
+            cross_f32_kernel<DP, WGS, true><<<nb, 256, 0, stream>>>(part, p.tiles, parts);
+        else
+            cross_f32_kernel<DP, WGS, false><<<nb, 256, 0, stream>>>(part, p.tiles, parts);
+    });
 }
 
 }  // namespace

@@ -411,30 +411,30 @@ __global__ __launch_bounds__(256, kShortEach) void cross_short_kernel(CrossArgs 
 
 template <int T>
 hipError_t launch_short(const CrossArgs& a, const CrossPlan& p, hipStream_t stream) {
-    const unsigned nb = (unsigned)((long)p.tiles * a.kv_heads);
-    if (a.key_mask)
-        cross_short_kernel<T, true><<<nb, 256, 0, stream>>>(a, p.tiles, p.run);
-    else
-        cross_short_kernel<T, false><<<nb, 256, 0, stream>>>(a, p.tiles, p.run);
-    return hipGetLastError();
+    return launch_in_turn(a, (long)p.tiles * a.kv_heads, [&](const CrossArgs& part, unsigned nb) {
+        if (part.key_mask)
+            cross_short_kernel<T, true><<<nb, 256, 0, stream>>>(part, p.tiles, p.run);
+        else
+            cross_short_kernel<T, false><<<nb, 256, 0, stream>>>(part, p.tiles, p.run);
+    });
 }
 
 template <int T, int DP, int STAGES, int WGS>
-hipError_t launch(const CrossArgs& a, int tiles, const CrossParts& parts, unsigned blocks, hipStream_t stream) {
-    if (a.key_mask)
-        cross_tile_kernel<T, DP, STAGES, WGS, true><<<blocks, 256, 0, stream>>>(a, tiles, parts);
-    else
-        cross_tile_kernel<T, DP, STAGES, WGS, false><<<blocks, 256, 0, stream>>>(a, tiles, parts);
-    return hipGetLastError();
+hipError_t launch(const CrossArgs& a, int tiles, const CrossParts& parts, hipStream_t stream) {
+    return launch_in_turn(a, (long)tiles * a.kv_heads * parts.parts, [&](const CrossArgs& part, unsigned nb) {
+        if (part.key_mask)
+            cross_tile_kernel<T, DP, STAGES, WGS, true><<<nb, 256, 0, stream>>>(part, tiles, parts);
+        else
+            cross_tile_kernel<T, DP, STAGES, WGS, false><<<nb, 256, 0, stream>>>(part, tiles, parts);
+    });
 }
 
 template <int T>
 hipError_t launch_t(const CrossArgs& a, const CrossPlan& p, const CrossParts& parts, hipStream_t stream) {
     if (p.run > 1) return launch_short<T>(a, p, stream);
-    const unsigned nb = (unsigned)((long)p.tiles * a.kv_heads * p.parts);
-    if (a.d > 128) return launch<T, 256, 2, 2>(a, p.tiles, parts, nb, stream);
-    if (a.d > 64) return launch<T, 128, 3, 3>(a, p.tiles, parts, nb, stream);
-    return launch<T, 64, 3, 4>(a, p.tiles, parts, nb, stream);
+    if (a.d > 128) return launch<T, 256, 2, 2>(a, p.tiles, parts, stream);
+    if (a.d > 64) return launch<T, 128, 3, 3>(a, p.tiles, parts, stream);
+    return launch<T, 64, 3, 4>(a, p.tiles, parts, stream);
 }
 
 }  // namespace

@@ -542,3 +542,37 @@ def test_offsets_in_disorder_stay_within_the_rows():
             capi.cross_attention(q.to(t)[:800], q.to(t)[:800], q.to(t)[:800], q_offsets=qo, k_offsets=ko, out=out[:800])
             torch.cuda.synchronize()
             assert (out[800:] == 5).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+def test_as_many_rows_as_there_may_be(dtype):
+    """One kv head's 2^30 rows; query i of head j is that of i + 1 and j - 1, and so is its row."""
+    lq, heads = 1 << 25, 32
+    gen = torch.Generator(device="cuda").manual_seed(22)
+    flat = _normal(gen, lq + heads, 8).to(dtype)
+    q = flat.as_strided((1, lq, heads, 8), (0, 8, 8, 1))
+    k, v = (_normal(gen, 1, 5, 1, 8).to(dtype) for _ in range(2))
+    out = torch.full((1, lq, heads, 8), 9.0, dtype=torch.bfloat16, device="cuda")
+    capi.cross_attention(q, k, v, out=out)
+    assert torch.equal(out[0, 1:, :-1], out[0, :-1, 1:])
+    for part in (slice(0, 3000), slice(lq - 3000, lq), slice(lq // 2 - 1500, lq // 2 + 1500)):
+        ro.check(out[0, part], *_sample(q[0, part], k[0], v[0], 8 ** -0.5, None, torch.bfloat16))
+
+
+@pytest.mark.parametrize("batch,heads", [((1 << 24) + 5, 1), ((1 << 22) + 1, 5)])
+def test_more_ragged_tiles_than_a_launch_has(batch, heads):
+    """A query and a key a sample: out is v, to the bit."""
+    v = torch.arange(batch * heads * 8, device="cuda").remainder_(253).bfloat16().view(batch, heads, 8)
+    offsets = torch.arange(batch + 1, dtype=torch.int32, device="cuda")
+    assert torch.equal(capi.cross_attention(v, v, v, q_offsets=offsets, k_offsets=offsets), v)
+
+
+def test_more_tiles_than_32_bits_count():
+    """2^31 samples and heads of one row on one key: out is v, to the bit."""
+    batch, heads = 1 << 30, 2
+    flat = torch.arange(8 * (batch + heads), dtype=torch.int32, device="cuda").remainder_(253).bfloat16()
+    v = flat.as_strided((batch, 1, heads, 8), (8, 8, 8, 1))
+    out = torch.full((batch, 1, heads, 8), 9.0, dtype=torch.bfloat16, device="cuda")
+    capi.cross_attention(v, v, v, out=out)
+    for h in range(heads):
+        assert torch.equal(out[:, 0, h], flat.view(-1, 8)[h:h + batch])
