@@ -532,7 +532,8 @@ S2_API int s2_group_norm(const void* x, s2_dtype x_dtype, long x_frame_stride,
  * x: device [m][k] in x_dtype, row stride x_stride >= k; weight: device [n][k]
  *   in w_dtype, contiguous; BF16 with F32 or BF16 x, or F16 with F16 x.  The
  *   products are those of the operands as given: an fp32 x is taken as three bf16
- *   terms, which hold it exactly, on the matrix cores.  An infinity or NaN of x reaches its row of y alone, one of the weight
+ *   terms on the matrix cores, which hold magnitudes from 2^-110 on exactly, smaller ones
+ *   to within 2^-134.  An infinity or NaN of x reaches its row of y alone, one of the weight
  *   its column (an infinite weight there makes NaN of fp32 rows' finite values).
  * bias: device fp32 [n] or NULL.  residual: device [m][n] in y_dtype, row
  *   stride residual_stride >= n, or NULL; y: device [m][n], row stride y_stride
@@ -605,7 +606,7 @@ S2_API int s2_mx_quantize(const void* x, s2_dtype x_dtype, long x_stride, int m,
                           s2_stream_t stream);
 /* The values of MXFP4 rows, rounded to y_dtype (fp32 and bf16 hold them all up to their
  * largest numbers, which scales from 253 on can pass, fp16 those of rows quantised from
- * fp16).  s2_mx_weight_linear takes a weight's values as bf16, infinities where they pass it. */
+ * fp16). */
 S2_API int s2_mx_dequantize(const void* codes, long code_stride, const void* scales,
                             long scale_stride, int m, int k, void* y, s2_dtype y_dtype,
                             long y_stride, s2_stream_t stream);
@@ -613,7 +614,10 @@ S2_API int s2_mx_dequantize(const void* codes, long code_stride, const void* sca
 /* y = residual + act(x W^T + bias) of rows x [m][k] and a weight [n][k] in MXFP4, the
  * products those of the values, exact, the sums in fp32; x in MXFP4 too (s2_mx_linear), or
  * in x_dtype with a row stride in elements (s2_mx_weight_linear: fp32, bf16 or fp16, as
- * they are or as two or three bf16 terms that hold them exactly).
+ * they are, or as two or three bf16 terms: fp16 values exactly, fp32 ones from 2^-110 on, and
+ * to within 2^-134 below).  What a weight's values past bf16's largest number give (of scales
+ * from 253 on) by rows in x_dtype is not defined: infinities, NaN where a term of x is zero,
+ * or the product itself.  They reach their column of y alone.
  *
  * w_codes: contiguous rows of 16 ceil(k / 32) bytes.  Where k is no multiple of 32 the
  *   codes past it are zeros in x or in the weight, as s2_mx_quantize writes them.

@@ -289,8 +289,10 @@ struct TileEnd {
     }
 };
 
-// fp32 as a sum of three bf16 values, exactly, whatever y's type: with two (off by 2^-17)
-// a product whose leading bits cancel would be off by more than y's rounding.  The first
+// fp32 as a sum of three bf16 values, whatever y's type: with two (off by 2^-17) a product
+// whose leading bits cancel would be off by more than y's rounding.  Exactly from 2^-110 on,
+// whose last bit is bf16's smallest number; below, the last term is rounded to that, by
+// 2^-134 at most.  The first
 // two take the top 8 bits of what the ones before leave, by truncation, which cannot
 // overflow and leaves an exact rest; the last holds the rest.  An infinity stays in the
 // first term, a NaN reaches the later ones.  v: pairs of values, h[q]: their terms q

@@ -8,7 +8,7 @@ namespace s2 {
 namespace {
 
 // A block of x as it is loaded, and eight k of it as the matrix cores take them: codes (XT
-// 0), or a sum of bf16 terms that holds it exactly (bf16: one, fp16: two, fp32: three)
+// 0), or a sum of bf16 terms that holds it exactly (bf16: one, fp16: two, fp32: three, from 2^-110 on)
 // against weights as bf16, which hold a code times its scale exactly.  XT: 0 MXFP4, else 1
 // + x's kind.
 template <int XT>

@@ -443,3 +443,32 @@ def test_more_tiles_of_codes_than_a_launch_has():
     got = capi.mx_linear(x.repeat((m + some - 1) // some, 1)[:m], weight, workspace=none)
     whole = m // some * some
     assert (got[:whole].view(-1, some, n) == first).all() and torch.equal(got[whole:], first[:m - whole])
+
+
+@pytest.mark.parametrize("m,n", [(3, 96), (16, 2560), (130, 96), (700, 2560), (3000, 2560)])
+@pytest.mark.parametrize("exponent", [-100, -112, -120, -126, -140])
+def test_fp32_rows_near_the_smallest_numbers(m, n, exponent):
+    """Three bf16 terms hold a value to within half of bf16's smallest number, 2^-134, which large
+    weights bring to light."""
+    gen = torch.Generator().manual_seed(m - exponent)
+    weight, w = _codes(n, 320, gen, 220, 240)
+    x = torch.ldexp(torch.randn(m, 320, generator=gen, dtype=torch.float64), torch.tensor(exponent)).float()
+    got = capi.mx_linear(x.cuda(), weight)
+    want, bound = mc.linear(x.double().cuda(), w.cuda(), None, "none", None, torch.float32)
+    ro.check(got, want, bound + 2.0 ** -134 * w.abs().sum(dim=1).cuda())
+
+
+@pytest.mark.parametrize("x_kind", KINDS, ids=str)
+@pytest.mark.parametrize("m", [3, 300])
+def test_weights_past_the_largest_number_reach_their_column_alone(x_kind, m):
+    gen = torch.Generator().manual_seed(m)
+    weight, w = _codes(70, 320, gen, 113, 125)
+    x, xv = _codes(m, 320, gen, 117, 130)
+    if x_kind is not None:
+        x = xv.to(x_kind).cuda()   # (six of 2^2 at most, four bits)
+    weight.scales[5, 3] = 254
+    weight.codes[5, 3 * 16:4 * 16] = 0x77
+    got = capi.mx_linear(x, weight, out_dtype=torch.float32)
+    want, bound = mc.linear(xv.cuda(), w.cuda(), None, "none", None, torch.float32)
+    keep = torch.arange(70, device="cuda") != 5
+    ro.check(got[:, keep], want[:, keep], bound[:, keep])
