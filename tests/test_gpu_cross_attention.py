@@ -576,3 +576,45 @@ def test_more_tiles_than_32_bits_count():
     capi.cross_attention(v, v, v, out=out)
     for h in range(heads):
         assert torch.equal(out[:, 0, h], flat.view(-1, 8)[h:h + batch])
+
+
+def _block_mask(batch, lk):
+    """Masks of more than one block of bits: kept keys at the blocks' borders, half of all, one
+    far from the end, whole blocks left out."""
+    keys = torch.arange(lk, device="cuda")
+    gen = torch.Generator(device="cuda").manual_seed(lk)
+    mask = torch.rand(batch, lk, generator=gen, device="cuda") < 0.5
+    near = keys.remainder(8192)
+    mask[1] = (near < 2) | (near > 8189) | (keys >= lk - 2)
+    if batch > 2:
+        mask[2] = keys == 8200
+    if batch > 3:
+        mask[3] = (keys < 40) | ((keys >= 8192) & (keys % 5 == 0) & (keys < 16384))
+    return mask
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("lk", [8191, 8192, 8193, 8225, 16384, 16385, 20000])
+@pytest.mark.parametrize("lq,d", [(1, 128), (40, 64), (70, 136)])
+def test_masks_of_several_blocks(dtype, lk, lq, d):
+    """Ranges of keys that begin and end inside blocks, waves without rows, NaN behind the mask."""
+    _padded(4, lq, lk, 2, 1, d, dtype, mask=_block_mask(4, lk), poison=True)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("lk", [8193, 16385, 25000])
+def test_masks_of_several_blocks_in_one_range(dtype, lk):
+    none = torch.empty(0, dtype=torch.uint8, device="cuda")
+    _padded(2, 300, lk, 2, 2, 64, dtype, mask=_block_mask(2, lk), poison=True, workspace=none)
+    _padded(2, 20, lk, 2, 2, 128, dtype, mask=_block_mask(2, lk), lengths=[lk - 3, lk // 2], poison=True,
+            workspace=none)
+
+
+@pytest.mark.parametrize("dtype", TYPES[1:], ids=str)
+def test_a_sample_of_several_blocks_among_short_ones(dtype):
+    """The kernel that keeps short samples' keys, read again for every 128 rows of a long one."""
+    queries, keys = [9000, 300, 700] + [1500] * 157, [20, 17000, 9] + [20] * 157
+    mask = torch.rand(sum(keys) + 3, generator=torch.Generator(device="cuda").manual_seed(23), device="cuda") < 0.5
+    mask[sum(keys):] = False
+    mask[20 + 8192:20 + 8200] = False
+    _ragged(queries, keys, 4, 4, 128, dtype, mask=mask)
