@@ -1146,7 +1146,7 @@ def cross_attention(q, k, v, scale=None, q_offsets=None, k_offsets=None, key_len
                                         not key_lengths.is_contiguous()):
             raise ValueError(f"key_lengths must be {batch} contiguous int32 values")
     dtype = q.dtype
-    if d != dk or v.shape != kshape or k.dtype is not dtype or v.dtype is not dtype:
+    if d == 0 or d != dk or v.shape != kshape or k.dtype is not dtype or v.dtype is not dtype:
         raise ValueError("k and v must be of one shape, q, k and v of one type and head_dim")
     ms = 0 if key_mask is None else _check_mask(key_mask, ragged, batch, lk)
     if out is None:

@@ -181,3 +181,9 @@ def test_cross_attention_binding_checks_shapes_and_types():
                  lambda: capi.cross_attention(q, k, k)):
         with pytest.raises(ValueError):   # the last one: no operand is on a device
             call()
+
+
+def test_cross_attention_binding_refuses_heads_of_no_elements():
+    for scale in (None, 1.0):
+        with pytest.raises(ValueError):
+            capi.cross_attention(torch.zeros(2, 5, 4, 0), torch.zeros(2, 7, 2, 0), torch.zeros(2, 7, 2, 0), scale)
