@@ -91,9 +91,9 @@ constexpr int kUnits = 256;   // compute units of an MI355X
 
 // Microseconds that a compute unit takes for a tile of keys with 1, 2, .. workgroups on it,
 // `each` at most, for d up to 64, 128 and 256: 4096 x 21600 with 20 heads of 128 in one
-// range of keys is three workgroups on half of the units and two on the others, 832 us; in
-// two ranges five in turn, 764.  1024 x 4096 86 us in one, 56 in three; 300 x 20000, two
-// heads, 379 and 32 in 32; in fp32 506 and 357, 1364 and 80.
+// range of keys is three workgroups on half of the units and two on the others, 875 us; in
+// two ranges five in turn, 792.  1024 x 4096 82 us in one, 57 in three; 300 x 20000, two
+// heads, 377 and 31 in 32; in fp32 508 and 359, 1376 and 75.
 struct CrossCost {
     int each;
     double us[4];
@@ -120,8 +120,8 @@ CrossPlan cross_plan(const CrossArgs& a, size_t workspace_bytes) {
     const long keys = a.q_offsets ? ((long)a.lk + a.batch - 1) / std::max(a.batch, 1) : a.lk;   // of a sample
     if (a.kind && a.d > 64 && a.d <= 128 && keys <= kShortKeys) {
         // the run by which the compute units' turns, of `run` rounds and one to begin, are
-        // fewest; worth it from about four on (4096 queries on 77 keys, 20 heads: two rounds 17.7
-        // us, 14.6 by the other kernel)
+        // fewest; worth it from about four on (4096 queries on 77 keys, 20 heads: two rounds 18.5
+        // us, 15.2 by the other kernel)
         const long slots = (long)kUnits * kShortEach;
         long least = 0;
         for (int run = 1; run <= 64; ++run) {

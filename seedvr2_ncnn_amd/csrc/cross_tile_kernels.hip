@@ -15,8 +15,8 @@
 // at most half a step each, as independent errors of its terms; their sum stays in fp32.
 //
 // On long keys the matrix cores and the exponentials beside them bound it, at the clocks that
-// their power leaves (1.7 GHz): 4096 on 21600 keys, 20 heads of 128, 0.76 ms, 1.2 PFLOP/s;
-// 21600 on 512 129 us, 0.88.  A wave's rows are 32: with 16 a tile's reads of LDS would bound
+// their power leaves (1.7 GHz): 4096 on 21600 keys, 20 heads of 128, 0.79 to 0.85 ms by the card,
+// 1.1 PFLOP/s; 21600 on 512 120 to 125 us, 0.92.  A wave's rows are 32: with 16 a tile's reads of LDS would bound
 // it, 64 do not fit its registers.  Two waves' keys ahead (a second tile's scores before the
 // first one's weights) were slower than three workgroups' waves in turn.
 #include "cross_attention_device.h"
@@ -154,7 +154,7 @@ struct WaveRows {
     __device__ __forceinline__ void keys(F&& between) {
         // Reads ahead where registers are left for them: of v under the scores' products and the
         // softmax, where the compiler would read two operands at a time and wait (4096 on 21600
-        // keys, 20 heads of 128, 807 us, 780 so; 21600 on 512 139 and 134; with heads of 64, four
+        // keys, 20 heads of 128, 824 us, 792 so; 21600 on 512 124 and 120; with heads of 64, four
         // waves a SIMD, 3% slower)
         constexpr int AHEAD = DP == 256 ? 0 : NK, VAHEAD = DP == 128 ? ND / 2 : 0;
         uint4 kf[2][NK];
@@ -358,8 +358,8 @@ __global__ __launch_bounds__(256, WGS) void cross_tile_kernel(CrossArgs a, int t
 
 // Many rows of d from 65 to 128 on few keys: all of a head's keys stay in LDS, up to 128 of
 // them, for `run` times 128 rows, so that waves meet at no barrier and q, loaded a turn
-// ahead, and out are all that moves (21600 queries on 77 keys, 20 heads of 128: 64 us by the
-// kernel above, 51 so, 4.4 TB/s; with heads of 64 30 either way).  Samples of more keys are
+// ahead, and out are all that moves (21600 queries on 77 keys, 20 heads of 128: 59 us by the
+// kernel above, 52 so, 4.3 TB/s; with heads of 64 no gain).  Samples of more keys are
 // read again for every 128 rows.
 template <int T, bool MASK>
 __global__ __launch_bounds__(256, kShortEach) void cross_short_kernel(CrossArgs a, int tiles, int run) {

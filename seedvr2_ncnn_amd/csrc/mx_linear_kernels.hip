@@ -355,7 +355,7 @@ bool one_launch(const MxLinearArgs& a, const TileChoice& t) {
 }
 
 // What tiles of the weight's codes take, in microseconds: a workgroup's first loads and
-// epilogue, and 256 k, for which its compute unit gets 50 or 41 KB through the caches; by
+// epilogue, and 256 k, for which its compute unit takes in 50 or 41 KB; by
 // rows in fp16, whose blocks' sums take their scales one by one.
 struct WeightCost {
     int bm, bn;

@@ -80,7 +80,7 @@ __global__ __launch_bounds__(256) void mx_deal_kernel(DealJob x, DealJob w, int 
 
 // 256x256 tile, eight waves (2 x 4) of 128x64, one workgroup per compute unit; the two
 // groups of waves take turns at the matrix cores as in the 16-bit products.  21664 x 2560 by
-// 10240 x 2560 with tanh-GELU 375 us, 3.0 PFLOP/s: ten steps of 2 us and 7 us of first loads
+// 10240 x 2560 with tanh-GELU 360 to 395 us by the card, 3.0 PFLOP/s: ten steps of 2 us and 7 us of first loads
 // and epilogue a tile; 8192^3 3.9 to 4.3, of 6.5 that products of random codes reach without
 // memory at the clocks that their power leaves.
 template <int YK>

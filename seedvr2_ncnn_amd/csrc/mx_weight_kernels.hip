@@ -8,9 +8,9 @@
 // 256 k (128 bytes of a row) at a time, and becomes bf16 in operand registers: four
 // conversions make an operand of a lane's eight codes, which 16 NI rows share.
 //
-// What bounds it are the bytes that a compute unit gets through the caches, about 40 KB a
-// microsecond: 128 x 2560 by 15360 x 2560 17 us, 0.6 PFLOP/s, its bytes once 6.  (In steps
-// of 64 k 30 us, of 256 k with one wave a SIMD 18.4; 41 with the weight's values written
+// A compute unit takes in about 40 KB a microsecond so, with two steps in flight; its caches
+// deliver several times that, and what it waits for has not been taken apart: 128 x 2560 by
+// 15360 x 2560 17 us, 0.6 PFLOP/s, its bytes once 6.  (In steps of 64 k 30 us, of 256 k with one wave a SIMD 18.4; 41 with the weight's values written
 // for the 16-bit tiles.  By fp16 rows 23, where the scales' products add up, 48 as two planes
 // and 16-bit tiles.)
 #include "mx_tiles.h"
